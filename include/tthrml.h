@@ -536,6 +536,59 @@ int tthrml_moments_accumulate(const void* state_dev, int32_t state_dtype, int64_
                               const int64_t* rows_dev, const uint8_t* spin_rows_dev, int32_t order,
                               int64_t n_moments, int32_t spin_as_bool, double* acc_dev, void* stream);
 
+/*
+ * ---------------------------------------------------------------------------
+ * 8-bit integer products around dense couplings.
+ * ---------------------------------------------------------------------------
+ * Element types of operator inputs and outputs.
+ */
+#define TTHRML_DT_F32 0
+#define TTHRML_DT_BF16 1
+#define TTHRML_DT_F16 2
+#define TTHRML_DT_I8 3
+
+/* Columns an int32 accumulator of 8-bit products holds exactly (2^31 / 128^2, less one). */
+#define TTHRML_INT8_MAX_COLS 131071
+
+/*
+ * Rows to 8-bit integers: scale[r] = max|x_r| * fl(1/127), values[r][c] =
+ * rint(x[r][c] * fl(127 / max|x_r|)) clamped to +-127.  A row whose largest
+ * magnitude is below 2^-120 gets zeros and scale 0; a row with an infinity or
+ * NaN gets scale NaN.  x: element (r, c) at r * row_stride + c * col_stride
+ * (element units; fast for col_stride 1 and for row_stride 1).  values:
+ * [rows][pitch] int8, 16-byte aligned, pitch a multiple of 16 >= cols;
+ * columns cols..pitch-1 are written as zeros.  scale: float32 [rows].
+ */
+int tthrml_quantize_rows(const void* x_dev, int32_t dtype, int64_t rows, int64_t cols,
+                         int64_t row_stride, int64_t col_stride, int8_t* values_dev, int64_t pitch,
+                         float* scale_dev, void* stream);
+
+/*
+ * out[m][n] = (sum_k x[m][k] * weights[n][k]) * (x_scale[m] * w_scale[n]) + bias[n]
+ * on the tensor cores: the sum exact in int32 (cols <= TTHRML_INT8_MAX_COLS),
+ * float32 scaling, one rounding to out_dtype.  x / weights: int8, 16-byte
+ * aligned, pitches multiples of 16.  x_scale may be NULL (ones), bias NULL.
+ * out: [rows][out_ld] elements of out_dtype.  error: device int32, set if an
+ * in-kernel wait expires.
+ */
+int tthrml_int8_product(const int8_t* x_dev, int64_t x_pitch, const float* x_scale_dev,
+                        const int8_t* weights_dev, int64_t w_pitch, const float* w_scale_dev,
+                        int64_t rows, int64_t units, int64_t cols, const float* bias_dev,
+                        void* out_dev, int32_t out_dtype, int64_t out_ld, int32_t* error_dev,
+                        void* stream);
+
+/*
+ * The same for 1 to 8 rows in one launch, reading the weights once.  x:
+ * [rows][x_ld] elements of x_dtype; float32, bfloat16 and float16 rows are
+ * quantised in the launch exactly as tthrml_quantize_rows does, int8 rows are
+ * taken with x_scale (NULL: ones).  The padded rows (1, 2, 4 or 8 of
+ * cols rounded up to 16) must fit 160 KiB.
+ */
+int tthrml_int8_product_few(const void* x_dev, int32_t x_dtype, int64_t x_ld, const float* x_scale_dev,
+                            const int8_t* weights_dev, int64_t w_pitch, const float* w_scale_dev,
+                            int64_t rows, int64_t units, int64_t cols, const float* bias_dev,
+                            void* out_dev, int32_t out_dtype, int64_t out_ld, void* stream);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

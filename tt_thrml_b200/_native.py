@@ -19,6 +19,8 @@ OK = 0
 SPIN, CATEGORICAL, GAUSSIAN = 0, 1, 2
 KIND_LINEAR, KIND_PRECISION = 0, 1
 STATE_F32, STATE_I8, STATE_BITS = 0, 1, 2
+DT_F32, DT_BF16, DT_F16, DT_I8 = 0, 1, 2, 3
+INT8_MAX_COLS = 131071
 MAX_CAT_SOURCES = 4
 MAX_CATEGORIES = 64
 
@@ -170,6 +172,15 @@ _SIGNATURES = {
     "tthrml_decode_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, c_vp]),
     "tthrml_encode_rows": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i32, c_i64, c_i64, c_vp, c_vp]),
     "tthrml_sum_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp]),
+    "tthrml_quantize_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "tthrml_int8_product": (
+        c_i32,
+        [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp, c_vp],
+    ),
+    "tthrml_int8_product_few": (
+        c_i32,
+        [c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp],
+    ),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),
     "tthrml_last_error": (ctypes.c_char_p, []),

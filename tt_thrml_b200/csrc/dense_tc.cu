@@ -23,12 +23,7 @@
 //                   32-column chunks), tcgen05.ld, draw, store bf16 rows.
 // Every wait is bounded by a clock limit; on expiry the kernel records an
 // error code, drains its own copies and MMAs (bounded), frees TMEM and exits.
-#include <cuda.h>
-#include <cuda_bf16.h>
-
-#include <mutex>
-
-#include "common.cuh"
+#include "dense_draw.cuh"
 
 namespace tthrml {
 namespace {
@@ -46,53 +41,6 @@ constexpr int kEpiGroups = kEpiWarps / 4;
 constexpr int kDenseThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kTmemCols = 256;
 constexpr int SMEM_BYTES = 1024 /*alignment slack*/ + STAGES * STAGE_BYTES + 256 /*barriers*/;
-constexpr long long kWaitCycles = 4ll << 30;  // about two seconds at 2 GHz
-
-enum : int { kErrNone = 0, kErrFullWait = 1, kErrEmptyWait = 2, kErrAccWait = 3 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Waits for the phase of `parity` to complete; false when the clock limit expires.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  const long long t0 = clock64();
-  while (!mbar_test(bar, parity)) {
-    if (clock64() - t0 > kWaitCycles) return false;
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
-
-// UMMA shared-memory descriptor of a K-major tile in the 128B-swizzle layout
-// written by TMA (rows of 128 B, 8-row groups 1024 B apart): start address,
-// leading offset 16 B, stride offset 1024 B, descriptor version 1, layout 2.
-__device__ __forceinline__ uint64_t umma_desc_sw128(const void* tile) {
-  const uint64_t addr = (uint64_t)(smem_u32(tile) >> 4) & 0x3FFFull;
-  return addr | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
 
 // Instruction descriptor: D fp32, A and B bf16, both K-major, N = BN, M = BM.
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
@@ -103,329 +51,6 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(kIdesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-struct DenseArgs {
-  const float* bias;       // [N] or NULL
-  __nv_bfloat16* out;      // [M][pieces * N] new target state: bf16 pieces, value = sum over pieces
-  float* out_f32;          // [M][N] same values in float32, or NULL
-  int32_t pieces;          // 1: bf16 value; 2-3: successive bf16 remainders (3 is exact for float32)
-  const float* variates;   // [variates_sweeps][N][M] (unit-major, chains innermost) or NULL
-  int64_t variates_sweeps;
-  int64_t M, N, K;
-  int64_t row0;            // flat state row of target unit 0 (Philox counter)
-  int64_t chain_offset;
-  uint64_t seed;
-  uint32_t sweep;
-  int32_t family;          // TTHRML_SPIN or TTHRML_GAUSSIAN
-  float precision;         // gaussian: sum of precision contributions (1 for unit variance)
-  const tthrml_run_ctl* ctl;
-  int* error;              // device word, set on a wait timeout
-  uint32_t* ties;          // near-threshold spin decisions: [count, blocks done, dropped, 0, (m, n) x ties_cap]
-  int64_t ties_cap;        // or NULL: decisions from the float32 field alone
-  int32_t group;           // CTA-pair kernel: row blocks per raster group
-};
-
-// A spin decision whose float32 margin is this close to the threshold (in units of u * (1 + e^(-2 gamma))
-// around 1, or of 2 gamma - logit in variates mode; |t - 1| ~ (1 - u) |2 gamma - logit u|) is decided
-// again from the exact field.  The tensor cores' float32 accumulation of a K-term field can be off by
-// ~1e-5 at K = 4096 with terms of size 0.01; a decision the float32 field gets wrong at a true margin
-// beyond the 1e-5 band therefore shows a float32 margin below (error - 1e-5), which this bound catches
-// for errors up to 2e-5.  The exact field is bias + sum_k A[m][k] B[n][k] in double (bf16 products are
-// exact there).  The epilogue only records such decisions (a few in 10^5); k_dense_settle, launched
-// next on the same stream, decides them again and overwrites their outputs.
-constexpr float kNearTie = 1e-5f;
-#ifndef TTHRML_DENSE_FAST_TRIG
-#define TTHRML_DENSE_FAST_TRIG 1  // Box-Muller angle through the hardware sine / cosine (0: sincospif)
-#endif
-#ifndef TTHRML_DENSE_F32X2
-#define TTHRML_DENSE_F32X2 1  // spin draws with packed f32x2 arithmetic (0: scalar)
-#endif
-#ifndef TTHRML_DENSE_SETTLE
-#define TTHRML_DENSE_SETTLE 2  // 0: no near-threshold check, 1: check only, 2: check and record
-#endif
-constexpr int kTieHeaderWords = 4;  // count, blocks of k_dense_settle done, entries dropped (cumulative), 0
-
-// Appends the (chain m, unit n_first + j) of every bit j of each lane's `near` to the tie list: one
-// atomic per warp, then each lane's entries at its prefix offset.  Entries past the capacity are
-// dropped (their float32 decisions stand) and counted by k_dense_settle.  All 32 lanes call it.
-__device__ __forceinline__ void record_ties(uint32_t* ties, int64_t cap, uint32_t near, int64_t m,
-                                            int64_t n_first) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t cnt = (uint32_t)__popc(near);
-  uint32_t incl = cnt;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  uint32_t base = 0u;
-  if (lane == 31) base = atomicAdd(ties, incl);
-  base = __shfl_sync(0xffffffffu, base, 31);
-  uint32_t idx = base + incl - cnt;
-  uint2* entries = reinterpret_cast<uint2*>(ties + kTieHeaderWords);
-  while (near) {
-    const int j = __ffs(near) - 1;
-    near &= near - 1u;
-    if ((int64_t)idx < cap) entries[idx] = make_uint2((uint32_t)m, (uint32_t)(n_first + j));
-    ++idx;
-  }
-}
-
-// Tile t of a persistent CTA -> (m block, n block): the row blocks are taken
-// `group` at a time and each group is walked row-fastest, so the tiles in
-// flight at one time share one or two B column panels while the group's A
-// row panels stay in L2 for the sweep over the group's columns.  The
-// single-CTA kernel takes 16 row blocks of 128 rows; the CTA-pair kernel
-// sizes its groups of 256-row blocks to about 32 MiB of A panels
-// (group x 256 x K x 2 bytes), which measured lowest in DRAM bytes for both
-// GEMMs of the 4096 x 8192 RBM (K = 4096: 16 blocks, K = 8192: 8 blocks;
-// 64 MiB groups or a plain row-major walk re-read more).
-constexpr int kGroupM = 16;
-__device__ __forceinline__ void tile_coords(int t, int m_blocks, int n_blocks, int group, int& mb, int& nb) {
-  const int per_group = group * n_blocks;
-  const int g = t / per_group, w = t - g * per_group;
-  const int rows = min(group, m_blocks - g * group);
-  mb = g * group + w % rows;
-  nb = w / rows;
-}
-
-// The 32 biases of a chunk (n_first % 32 == 0, bias 16-byte aligned): eight 16-byte loads, the same
-// addresses in every lane; zeros without a bias.
-__device__ __forceinline__ void load_bias32(const float* bias, int64_t n_first, float (&b)[32]) {
-  if (!bias) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) b[j] = 0.0f;
-    return;
-  }
-  const float4* bq = reinterpret_cast<const float4*>(bias + n_first);
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const float4 v = __ldg(bq + q);
-    b[4 * q] = v.x;
-    b[4 * q + 1] = v.y;
-    b[4 * q + 2] = v.z;
-    b[4 * q + 3] = v.w;
-  }
-}
-
-// Spin epilogue of one 32-column chunk of row m: bit j of the result is set when unit n_first + j samples
-// -1.  +1 with probability sigmoid(2 field): u * (1 + e^(-2 field)) < 1 with u = uniform_open of the
-// unit's Philox word (u is built with ALU operations, bit for bit the same value), or 2 field > logit.
-// `near` receives the decisions within kNearTie of their threshold.
-template <bool VARIATES>
-__device__ __forceinline__ uint32_t spin_chunk(const DenseArgs& a, const float (&acc)[32], int64_t m,
-                                               int64_t n_first, uint32_t sweep, const PhiloxKeys& keys,
-                                               int64_t vs, uint32_t& near) {
-  const int64_t gchain = a.chain_offset + m;
-  const int64_t r0 = a.row0 + n_first;
-  uint32_t down = 0u;
-  near = 0u;
-  if (VARIATES) {
-    float b[32];
-    load_bias32(a.bias, n_first, b);
-    const float* vrow = a.variates + (vs * a.N + n_first) * a.M + m;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const float field = __fadd_rn(acc[j], b[j]);
-      const float d = __fsub_rn(__fmul_rn(2.0f, field), __ldg(vrow + (int64_t)j * a.M));
-      down |= (d > 0.0f ? 0u : 1u) << j;
-      if (TTHRML_DENSE_SETTLE) near |= (fabsf(d) < kNearTie ? 1u : 0u) << j;
-    }
-  } else if ((r0 & 3) == 0) {  // the chunk starts a Philox counter: word j % 4 of counter r0 / 4 + j / 4
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const u32x4 r = philox4x32_10(u32x4{(uint32_t)gchain, (uint32_t)((r0 >> 2) + q), sweep, kSaltDenseSpin}, keys);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-      const float4 bq = a.bias ? __ldg(reinterpret_cast<const float4*>(a.bias + n_first) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float b[4] = {bq.x, bq.y, bq.z, bq.w};
-#if TTHRML_DENSE_F32X2
-      // two units per packed instruction: t = u * (1 + 2^(-2 log2(e) field)), decided against 1
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        const int j = 4 * q + i;
-        const float2 field = __fadd2_rn(make_float2(acc[j], acc[j + 1]), make_float2(b[i], b[i + 1]));
-        const float2 x = __fmul2_rn(field, make_float2(-2.8853900817779268f, -2.8853900817779268f));
-        float e0, e1;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(x.x));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(x.y));
-        const float2 u = __fadd2_rn(make_float2(__uint_as_float(0x3F800000u | (w[i] >> 9)),
-                                                __uint_as_float(0x3F800000u | (w[i + 1] >> 9))),
-                                    make_float2(-0.99999994039535522461f, -0.99999994039535522461f));
-        const float2 t = __fmul2_rn(u, __fadd2_rn(make_float2(e0, e1), make_float2(1.0f, 1.0f)));
-        down |= ((t.x < 1.0f ? 0u : 1u) | (t.y < 1.0f ? 0u : 2u)) << j;
-        if (TTHRML_DENSE_SETTLE) {
-          const float2 d = __fadd2_rn(t, make_float2(-1.0f, -1.0f));
-          near |= ((fabsf(d.x) < kNearTie ? 1u : 0u) | (fabsf(d.y) < kNearTie ? 2u : 0u)) << j;
-        }
-      }
-#else
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * q + i;
-        const float field = __fadd_rn(acc[j], b[i]);
-        const float t = uniform_open_alu(w[i]) * (1.0f + __expf(-2.0f * field));
-        down |= (t < 1.0f ? 0u : 1u) << j;
-        if (TTHRML_DENSE_SETTLE) near |= (fabsf(t - 1.0f) < kNearTie ? 1u : 0u) << j;
-      }
-#endif
-    }
-  } else {
-    float b[32];
-    load_bias32(a.bias, n_first, b);
-    u32x4 r{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int64_t row = r0 + j;
-      if (j == 0 || (row & 3) == 0)
-        r = philox4x32_10(u32x4{(uint32_t)gchain, (uint32_t)(row >> 2), sweep, kSaltDenseSpin}, keys);
-      const float field = __fadd_rn(acc[j], b[j]);
-      const float t = uniform_open_alu(word_of(r, (int)(row & 3))) * (1.0f + __expf(-2.0f * field));
-      down |= (t < 1.0f ? 0u : 1u) << j;
-      if (TTHRML_DENSE_SETTLE) near |= (fabsf(t - 1.0f) < kNearTie ? 1u : 0u) << j;
-    }
-  }
-  return down;
-}
-
-// Box-Muller on words 2p, 2p+1 of a counter: the normals of rows 4j+2p (cosine) and 4j+2p+1 (sine).
-__device__ __forceinline__ void box_muller_pair(uint32_t w0, uint32_t w1, float& xc, float& xs) {
-  const float rad = sqrtf(-2.0f * logf(uniform_open(w0)));
-  float sn, cs;
-#if TTHRML_DENSE_FAST_TRIG
-  // theta = 2 pi u1 = phi + pi with phi = 2 pi (u1 - 1/2) in (-pi, pi), where the hardware sine and cosine
-  // are accurate to ~5e-7 absolute: cos theta = -cos phi, sin theta = -sin phi
-  __sincosf(6.2831853071795865f * (uniform_open_alu(w1) - 0.5f), &sn, &cs);
-  xc = -rad * cs;
-  xs = -rad * sn;
-#else
-  sincospif(2.0f * uniform_open(w1), &sn, &cs);
-  xc = rad * cs;
-  xs = rad * sn;
-#endif
-}
-
-// Gaussian epilogue of one 32-column chunk: field * var + sqrt(var) * xi, xi the unit's normal from the
-// counter (chain, row / 4, sweep, "DGAU") (or the uploaded normal).
-template <bool VARIATES>
-__device__ __forceinline__ void gauss_chunk(const DenseArgs& a, const float (&acc)[32], int64_t m,
-                                            int64_t n_first, uint32_t sweep, const PhiloxKeys& keys, float inv,
-                                            float sd_g, int64_t vs, float (&outf)[32]) {
-  float b[32];
-  load_bias32(a.bias, n_first, b);
-  const int64_t gchain = a.chain_offset + m;
-  const int64_t r0 = a.row0 + n_first;
-  float xi[32];
-  if (VARIATES) {
-    const float* vrow = a.variates + (vs * a.N + n_first) * a.M + m;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) xi[j] = __ldg(vrow + (int64_t)j * a.M);
-  } else if ((r0 & 3) == 0) {  // the chunk starts a counter: rows 4q..4q+3 of the chunk share counter q
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const u32x4 r = philox4x32_10(u32x4{(uint32_t)gchain, (uint32_t)((r0 >> 2) + q), sweep, kSaltDenseGauss}, keys);
-      box_muller_pair(r.x, r.y, xi[4 * q], xi[4 * q + 1]);
-      box_muller_pair(r.z, r.w, xi[4 * q + 2], xi[4 * q + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int64_t row = r0 + j;
-      const u32x4 r = philox4x32_10(u32x4{(uint32_t)gchain, (uint32_t)(row >> 2), sweep, kSaltDenseGauss}, keys);
-      const int w = (int)((row >> 1) & 1) * 2;
-      float xc, xs;
-      box_muller_pair(word_of(r, w), word_of(r, w + 1), xc, xs);
-      xi[j] = (row & 1) ? xs : xc;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float field = a.bias ? __fadd_rn(acc[j], b[j]) : acc[j];
-    outf[j] = __fadd_rn(__fmul_rn(field, inv), __fmul_rn(sd_g, xi[j]));
-  }
-}
-
-// Epilogue of one 32-column chunk of one row (chain m): draw and store.  The new value goes to the
-// float32 copy (if any) and as `pieces` bf16 pieces: piece p = bf16(v - pieces 0..p-1), each remainder
-// exact in float32, so three pieces carry all 24 significand bits.  A spin's +-1 is one bf16 piece
-// (0x3F80 / 0xBF80) and zero remainders.
-template <int FAMILY, bool VARIATES>
-__device__ __forceinline__ void draw_chunk(const DenseArgs& a, const float (&acc)[32], int64_t m, int64_t n_first,
-                                           uint32_t sweep, const PhiloxKeys& keys, float inv, float sd_g,
-                                           int64_t vs) {
-  __nv_bfloat16* row = a.out + m * (a.N * a.pieces) + n_first;
-  if (FAMILY == TTHRML_SPIN) {
-    uint32_t near;
-    const uint32_t down = spin_chunk<VARIATES>(a, acc, m, n_first, sweep, keys, vs, near);
-    if (TTHRML_DENSE_SETTLE == 2 && a.ties != nullptr &&
-        __any_sync(0xffffffffu, near != 0u))  // rare: k_dense_settle decides these again from the exact field
-      record_ties(a.ties, a.ties_cap, near, m, n_first);
-    if (a.out_f32) {
-      float4* df = reinterpret_cast<float4*>(a.out_f32 + m * a.N + n_first);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(0x3F800000u | (((down >> (4 * q + i)) & 1u) << 31));
-        df[q] = make_float4(v[0], v[1], v[2], v[3]);
-      }
-    }
-    uint32_t w[16];  // bf16 pairs (unit 2k in the low half)
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      w[k] = 0x3F803F80u | (((down >> (2 * k)) & 1u) << 15) | (((down >> (2 * k + 1)) & 1u) << 31);
-    uint4* dst = reinterpret_cast<uint4*>(row);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-    for (int p = 1; p < a.pieces; ++p) {
-      uint4* z = reinterpret_cast<uint4*>(row + p * a.N);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) z[q] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    return;
-  }
-  float outf[32];
-  gauss_chunk<VARIATES>(a, acc, m, n_first, sweep, keys, inv, sd_g, vs, outf);
-  if (a.out_f32) {
-    float4* df = reinterpret_cast<float4*>(a.out_f32 + m * a.N + n_first);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) df[q] = make_float4(outf[4 * q], outf[4 * q + 1], outf[4 * q + 2], outf[4 * q + 3]);
-  }
-  for (int p = 0; p < a.pieces; ++p) {
-    __align__(16) __nv_bfloat16 outv[32];
-    const bool last = p + 1 == a.pieces;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      outv[j] = __float2bfloat16_rn(outf[j]);
-      if (!last) outf[j] = __fsub_rn(outf[j], __bfloat162float(outv[j]));
-    }
-    uint4* dst = reinterpret_cast<uint4*>(row + p * a.N);
-    const uint4* srcv = reinterpret_cast<const uint4*>(outv);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) dst[q] = srcv[q];
-  }
 }
 
 // Persistent kernel: one CTA per SM walks output tiles; two TMEM accumulators
@@ -618,36 +243,9 @@ constexpr int A2_BYTES = BM2 * BK * 2;   // 16 KiB
 constexpr int B2_BYTES = BN2H * BK * 2;  // 16 KiB
 constexpr int STAGE2_BYTES = A2_BYTES + B2_BYTES;
 constexpr int SMEM2_BYTES = 1024 + STAGES2 * STAGE2_BYTES + 256;
-constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit of a shared::cluster address
 // Instruction descriptor of the pair MMA: D fp32, A and B bf16, K-major, N = 256, M = 256.
 constexpr uint32_t kIdesc2 = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_id_x() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t n_clusters_x() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_leader, int c0,
-                                                 int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-      "[%2];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(bar_leader), "r"(c0), "r"(c1)
-      : "memory");
-}
 __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -656,18 +254,6 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc,
       "l"(a_desc), "l"(b_desc), "r"(kIdesc2), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u),
       "r"(0u), "r"(0u));
 }
-// arrives (once all earlier MMAs of this thread are done) on the barrier at this offset in both CTAs
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)0x3)
-      : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(smem_u32(bar) & kPeerMask) : "memory");
-}
-
 template <int FAMILY, bool VARIATES>
 __global__ void __launch_bounds__(kDenseThreads, 1)
     k_dense_field_sample_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -824,28 +410,6 @@ __global__ void __launch_bounds__(kDenseThreads, 1)
 }
 
 // --- host side --------------------------------------------------------------
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int encode_fn(EncodeTiledFn* out) {
-  static EncodeTiledFn fn = nullptr;
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !p) {
-      set_error("cuTensorMapEncodeTiled is unavailable (%s)", cudaGetErrorString(e));
-      return TTHRML_ERR_CUDA;
-    }
-    fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  *out = fn;
-  return TTHRML_OK;
-}
 
 // Tensor map of a row-major bf16 matrix [rows][cols] read in (box_rows x 64) tiles, 128B swizzle.
 int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, uint32_t box_rows) {

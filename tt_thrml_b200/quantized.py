@@ -1,0 +1,274 @@
+"""8-bit integer products: fields of a batch of rows through weights held as int8.
+
+    y[m, n] = (sum_k q[m, k] w[n, k]) * (s_x[m] * s_w[n]) + bias[n]
+
+with one float32 scale per row m (token / chain) and per unit n (channel).
+`quantize_rows` makes the integers and scales of a matrix, `QuantizedRows`
+holds them, `int8_product` multiplies; rows given as floats are quantised
+within the call.  The sums are exact in int32, so the result does not depend
+on how the kernels split them.  A dense program runs its sweeps on the same
+arithmetic with `dense_precision="int8"` (make_cuda_config).
+
+The kernels launch on the current stream of the rows' device; nothing
+synchronises.  There is no backward pass: rows that require a gradient are
+refused.
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+from . import _native as nat
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def dtype_code(dtype):
+    """The C ABI's code of a floating element type, or None."""
+    torch = _torch()
+    return {torch.float32: nat.DT_F32, torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16}.get(dtype)
+
+
+_error_words: dict = {}
+
+
+def error_word(device):
+    """The device's int32 word that operator kernels set when an in-kernel wait expires."""
+    word = _error_words.get(device.index)
+    if word is None:
+        torch = _torch()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run the operator once on this device before capturing it into a CUDA graph")
+        word = _error_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()
+    return word
+
+
+def check_operator_errors(device=None) -> None:
+    """Raises if an operator kernel on `device` (default: every device used) reported an expired wait."""
+    torch = _torch()
+    for index, word in list(_error_words.items()):
+        if device is not None and torch.device(device).index not in (None, index):
+            continue
+        torch.cuda.synchronize(index)
+        code = int(word.item())
+        if code:
+            raise RuntimeError(f"a device kernel reported an expired wait (code {code})")
+
+
+@contextlib.contextmanager
+def _other_device(index: int):
+    torch = _torch()
+    with torch.cuda.device(index):
+        nat.check(nat.lib().tthrml_set_device(index), "tthrml_set_device")
+        nat._bound.device = index
+        yield
+    nat._bound.device = None  # the library's current device follows torch's again at the next call
+
+
+def on_device(device):
+    """Context in which `device` is current for torch and for the library; cheap when it already is."""
+    torch = _torch()
+    if torch.cuda.current_device() != device.index:
+        return _other_device(device.index)
+    nat.bind_device(device.index)
+    return contextlib.nullcontext()
+
+
+def require_cuda(name: str, t, device=None):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device (there is no CPU path), got {t.device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _no_grad(name: str, t):
+    torch = _torch()
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError(f"{name} requires a gradient, but 8-bit products have no backward pass (use torch.no_grad())")
+
+
+class QuantizedRows:
+    """A matrix as int8 rows with one float32 scale per row: value[r, c] = values[r, c] * scale[r].
+
+    values: int8 [rows, cols]; rows that are not 16-byte aligned and a
+    multiple of 16 bytes apart are laid out again once, here.  scale: float32
+    [rows], or None for ones (spins as +-1 are their own integers).
+    """
+
+    def __init__(self, values, scale=None):
+        torch = _torch()
+        require_cuda("values", values)
+        if values.dtype != torch.int8 or values.dim() != 2:
+            raise ValueError(f"values must be an int8 matrix, got {values.dtype} of shape {tuple(values.shape)}")
+        rows, cols = values.shape
+        if cols < 1 or cols > nat.INT8_MAX_COLS:
+            raise ValueError(f"1 to {nat.INT8_MAX_COLS} columns are supported, got {cols}")
+        if scale is not None:
+            require_cuda("scale", scale, values.device)
+            if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] != rows:
+                raise ValueError(f"scale must be float32 of shape ({rows},), got {scale.dtype} of {tuple(scale.shape)}")
+            scale = scale.contiguous()
+        pitch = values.stride(0) if rows > 1 else -(-cols // 16) * 16
+        if (cols > 1 and values.stride(1) != 1) or pitch % 16 or pitch < cols or values.data_ptr() % 16:
+            laid = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=values.device)
+            laid[:, :cols].copy_(values)
+            values = laid[:, :cols]
+            pitch = laid.shape[1]
+        self.values = values
+        self.scale = scale
+        self.pitch = int(pitch)
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def device(self):
+        return self.values.device
+
+    def dequantize(self):
+        """The float32 matrix that the integers and scales stand for."""
+        v = self.values.float()
+        return v if self.scale is None else v * self.scale[:, None]
+
+
+def quantize_rows(x) -> QuantizedRows:
+    """Rows of a float32, bfloat16 or float16 matrix as int8 with one scale per row.
+
+    scale[r] = max|x_r| / 127 and q = rint(x 127 / max|x_r|), both in float32.
+    A row of zeros (or of magnitudes below 2^-120) gets scale 0, a row that
+    holds an infinity or NaN gets scale NaN.  Any strides; rows and transposed
+    matrices are read at full width.
+    """
+    torch = _torch()
+    require_cuda("x", x)
+    code = dtype_code(x.dtype)
+    if code is None or x.dim() != 2:
+        raise ValueError(f"x must be a float32, bfloat16 or float16 matrix, got {x.dtype} of shape {tuple(x.shape)}")
+    _no_grad("x", x)
+    rows, cols = x.shape
+    if cols < 1 or cols > nat.INT8_MAX_COLS:
+        raise ValueError(f"1 to {nat.INT8_MAX_COLS} columns are supported, got {cols}")
+    if x.stride(1) == 0 and cols > 1:
+        x = x.contiguous()
+    pitch = -(-cols // 16) * 16
+    values = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows:
+        with on_device(x.device):
+            nat.check(
+                nat.lib().tthrml_quantize_rows(
+                    x.data_ptr(), code, rows, cols, x.stride(0), x.stride(1) if cols > 1 else 1, values.data_ptr(),
+                    pitch, scale.data_ptr(), torch.cuda.current_stream(x.device).cuda_stream,
+                ),
+                "tthrml_quantize_rows",
+            )
+    return QuantizedRows(values[:, :cols], scale)
+
+
+_FEW_ROWS = 8
+_FEW_BYTES = 160 * 1024
+
+
+def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=None):
+    """y = x w^T with 8-bit integers: x [..., K] (float rows, quantised here, or QuantizedRows), weights [N, K].
+
+    bias: float32 [N] added after the scaling.  out_dtype: float32, bfloat16
+    or float16 (default: x's type; float32 for QuantizedRows).  out: a tensor
+    [..., N] to write, its rows dense.  Up to eight rows run as one launch that
+    reads the weights once; more rows are quantised and multiplied on the
+    tensor cores.
+    """
+    torch = _torch()
+    if not isinstance(weights, QuantizedRows):
+        raise TypeError(f"weights must be QuantizedRows (see quantize_rows), got {type(weights).__name__}")
+    if weights.scale is None:
+        raise ValueError("weights need a scale per unit")
+    dev = weights.device
+    quantized = isinstance(x, QuantizedRows)
+    if quantized:
+        lead, K = (x.shape[0],), x.shape[1]
+        if x.device != dev:
+            raise ValueError(f"x is on {x.device}, expected {dev}")
+    else:
+        require_cuda("x", x, dev)
+        code = dtype_code(x.dtype)
+        if code is None or x.dim() < 1:
+            raise ValueError(f"x must hold float32, bfloat16 or float16 rows, got {x.dtype} of shape {tuple(x.shape)}")
+        _no_grad("x", x)
+        lead, K = tuple(x.shape[:-1]), x.shape[-1]
+    N = weights.shape[0]
+    if K != weights.shape[1]:
+        raise ValueError(f"x has rows of {K}, the weights have {weights.shape[1]} columns")
+    if bias is not None:
+        require_cuda("bias", bias, dev)
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (N,):
+            raise ValueError(f"bias must be float32 of shape ({N},), got {bias.dtype} of {tuple(bias.shape)}")
+        _no_grad("bias", bias)
+        bias = bias.contiguous()
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else (torch.float32 if quantized else x.dtype)
+    out_code = dtype_code(out_dtype)
+    if out_code is None:
+        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    if out is None:
+        out = torch.empty((*lead, N), dtype=out_dtype, device=dev)
+        out2 = out.view(-1, N) if N else out
+    else:
+        require_cuda("out", out, dev)
+        if out.dtype != out_dtype or tuple(out.shape) != (*lead, N):
+            raise ValueError(f"out must be {out_dtype} of shape {(*lead, N)}, got {out.dtype} of {tuple(out.shape)}")
+        _no_grad("out", out)
+        out2 = out.view(-1, N) if N else out  # raises if the rows cannot be one matrix
+        if out2.numel() and ((N > 1 and out2.stride(1) != 1) or (out2.shape[0] > 1 and out2.stride(0) < N)):
+            raise ValueError("out needs dense rows that do not overlap")
+    if not out.numel():
+        return out
+    M = out2.shape[0]
+    out_ld = out2.stride(0) if M > 1 else N
+    lib = nat.lib()
+    with on_device(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        bias_ptr = None if bias is None else bias.data_ptr()
+        wide = 1 << max(0, M - 1).bit_length()
+        few = M <= _FEW_ROWS and wide * (-(-K // 16) * 16) <= _FEW_BYTES
+        if few:
+            if quantized:
+                rows, ld, sx, code = x.values, x.pitch, x.scale, nat.DT_I8
+            else:
+                rows, sx = x.reshape(-1, K), None
+                if K > 1 and rows.stride(1) != 1 or M > 1 and rows.stride(0) < K:
+                    rows = rows.contiguous()
+                ld = rows.stride(0) if M > 1 else K
+            nat.check(
+                lib.tthrml_int8_product_few(
+                    rows.data_ptr(), code, ld, None if sx is None else sx.data_ptr(), weights.values.data_ptr(),
+                    weights.pitch, weights.scale.data_ptr(), M, N, K, bias_ptr, out2.data_ptr(), out_code, out_ld,
+                    stream,
+                ),
+                "tthrml_int8_product_few",
+            )
+            return out
+        error = error_word(dev)
+        if not quantized:
+            x = quantize_rows(x.reshape(-1, K))
+        nat.check(
+            lib.tthrml_int8_product(
+                x.values.data_ptr(), x.pitch, None if x.scale is None else x.scale.data_ptr(),
+                weights.values.data_ptr(), weights.pitch, weights.scale.data_ptr(), M, N, K, bias_ptr,
+                out2.data_ptr(), out_code, out_ld, error.data_ptr(), stream,
+            ),
+            "tthrml_int8_product",
+        )
+    return out
+
+
+__all__ = ["QuantizedRows", "quantize_rows", "int8_product", "check_operator_errors"]
