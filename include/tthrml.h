@@ -589,6 +589,54 @@ int tthrml_int8_product_few(const void* x_dev, int32_t x_dtype, int64_t x_ld, co
                             int64_t rows, int64_t units, int64_t cols, const float* bias_dev,
                             void* out_dev, int32_t out_dtype, int64_t out_ld, void* stream);
 
+/*
+ * ---------------------------------------------------------------------------
+ * AdamW over many tensors in one launch (Adam with decoupled weight decay).
+ * ---------------------------------------------------------------------------
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+ *   p = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in float32.  The moments of all tensors lie in one buffer; a tensor's
+ * segment starts at `state` (a multiple of 256) and is padded to a multiple of
+ * 256 elements that start out as zeros.
+ */
+typedef struct tthrml_adamw_tensor {
+  void* param;        /* [n] elements of param_dtype */
+  const void* grad;   /* [n] elements of grad_dtype, in the same order */
+  int64_t n;          /* >= 1 */
+  int64_t state;      /* first element of the segment of the moments */
+  int32_t param_dtype, grad_dtype; /* TTHRML_DT_F32, _BF16 or _F16 */
+} tthrml_adamw_tensor;
+
+/* Device-side run control of an optimizer: steps done, learning rate. */
+typedef struct tthrml_adamw_ctl {
+  int64_t step;
+  double lr;
+  unsigned long long ticket; /* 0 between steps */
+} tthrml_adamw_ctl;
+
+/*
+ * One step of every tensor (700 per launch).  tensors: host array, read before
+ * the call returns.  state_bits 32: exp_avg / exp_avg_sq float32 [elements].
+ * state_bits 8: int8 / uint8 codes with one float32 scale per 256 elements,
+ *   m = q |q| scale / 127^2,  v = q^4 scale / 255^4,
+ * scale the block's largest |m| (v); a value is rounded to one of its two
+ * neighbouring codes so that its mean is kept, by the 16-bit halves of Philox
+ * word element % 4 of counter (element / 4, element / 4 >> 32, t, "ADMW") under
+ * `seed` (low half: m, high half: v); v > 0 gets at least code 1; a block
+ * whose largest v is below 2^-90 is held as zeros, one that takes in an infinity
+ * or NaN becomes NaN.  ctl: device; its step is advanced by one.
+ */
+int tthrml_adamw_step(const tthrml_adamw_tensor* tensors_host, int64_t n_tensors, int32_t state_bits,
+                      void* exp_avg_dev, void* exp_avg_sq_dev, float* exp_avg_scale_dev,
+                      float* exp_avg_sq_scale_dev, tthrml_adamw_ctl* ctl_dev, double beta1,
+                      double beta2, double eps, double weight_decay, uint64_t seed, void* stream);
+
+/* The float32 values of 8-bit moments (elements a multiple of 256). */
+int tthrml_adamw_values(const int8_t* exp_avg_dev, const uint8_t* exp_avg_sq_dev,
+                        const float* exp_avg_scale_dev, const float* exp_avg_sq_scale_dev,
+                        int64_t elements, float* exp_avg_out_dev, float* exp_avg_sq_out_dev,
+                        void* stream);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

@@ -74,6 +74,19 @@ class HaloExport(ctypes.Structure):
     ]
 
 
+class AdamWTensor(ctypes.Structure):
+    """tthrml_adamw_tensor (include/tthrml.h)."""
+
+    _fields_ = [
+        ("param", c_vp),
+        ("grad", c_vp),
+        ("n", c_i64),
+        ("state", c_i64),
+        ("param_dtype", c_i32),
+        ("grad_dtype", c_i32),
+    ]
+
+
 class GroupDesc(ctypes.Structure):
     _fields_ = [
         ("blocks", c_vp),
@@ -181,6 +194,12 @@ _SIGNATURES = {
         c_i32,
         [c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp],
     ),
+    "tthrml_adamw_step": (
+        c_i32,
+        [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+         ctypes.c_double, c_u64, c_vp],
+    ),
+    "tthrml_adamw_values": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),
     "tthrml_last_error": (ctypes.c_char_p, []),

@@ -1,0 +1,240 @@
+"""AdamW over many tensors in one launch, moments in float32 or in 8-bit codes.
+
+    m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
+    p = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+What a sampler's moments are turned into: the couplings and biases of a
+program (see `pair_moments` and `DenseLearner`) are tensors of very different
+sizes, stepped together.  With `state_bits=8` the moments take 2 bytes and a
+32nd instead of 8 per element; the codes are rounded at random with the mean
+kept, from a counter-based generator, so a run can be repeated.
+
+The step counter and the learning rate live on the device: a step captured
+into a CUDA graph counts on at every replay, and setting `lr` reaches replayed
+graphs.  Nothing synchronises.
+"""
+
+from __future__ import annotations
+
+import weakref
+from operator import call, is_
+
+import numpy as np
+
+from . import _native as nat
+from .quantized import dtype_code, on_device, require_cuda
+
+BLOCK = 256  # elements per scale of 8-bit moments; segments of the moments are padded to it
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def _dense_order(t):
+    """The order of a tensor's elements in memory as (sizes, strides) of its dimensions longer than one,
+    outermost first, or None if it has gaps or overlaps."""
+    if not t.numel():
+        return ()
+    dims = sorted(((st, s) for s, st in zip(t.shape, t.stride()) if s != 1), reverse=True)
+    want = 1
+    for st, s in reversed(dims):
+        if st != want:
+            return None
+        want *= s
+    return tuple(st if s != 1 else 0 for s, st in zip(t.shape, t.stride()))
+
+
+class AdamW:
+    """AdamW bound to a list of parameter tensors on one CUDA device.
+
+    params: float32, bfloat16 or float16 tensors without gaps or overlaps
+    (any order of dimensions).  `step(grads)` takes one gradient per parameter:
+    the parameter's type or float32, the parameter's shape and memory order;
+    None reads every parameter's `.grad`.  16-bit parameters are rounded to
+    nearest after the step.  state_bits: 32, or 8 for coded moments
+    (`seed` keys their rounding).
+    """
+
+    def __init__(self, params, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
+        torch = _torch()
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("AdamW needs at least one parameter")
+        dev = getattr(self.params[0], "device", None)
+        for i, p in enumerate(self.params):
+            require_cuda(f"parameter {i}", p, dev)
+            if dtype_code(p.dtype) is None:
+                raise ValueError(f"parameter {i} must be float32, bfloat16 or float16, got {p.dtype}")
+            if _dense_order(p) is None:
+                raise ValueError(f"parameter {i} has gaps or overlaps in memory (strides {tuple(p.stride())})")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i)
+                       for i, p in enumerate(self.params) if p.numel())
+        for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
+            if start < end:
+                raise ValueError(f"parameters {i} and {j} share memory")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must lie in [0, 1), got {betas!r}")
+        if not eps > 0.0 or not weight_decay >= 0.0 or not lr >= 0.0:
+            raise ValueError("eps must be above 0, lr and weight_decay not below 0")
+        self.device, self.betas, self.eps, self.weight_decay = dev, tuple(map(float, betas)), float(eps), float(weight_decay)
+        self.state_bits, self.seed = int(state_bits), int(seed) & 0xFFFFFFFFFFFFFFFF
+        # segment of each parameter in the moments
+        self.offsets, total = [], 0
+        for p in self.params:
+            self.offsets.append(total)
+            total += -(-p.numel() // BLOCK) * BLOCK
+        self.elements = total
+        kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
+        self.exp_avg, self.exp_avg_sq = (torch.zeros(max(total, BLOCK), dtype=k, device=dev) for k in kinds)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if state_bits == 8:
+            self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(max(total, BLOCK) // BLOCK, device=dev) for _ in range(2))
+        self._ctl = torch.zeros(3, dtype=torch.int64, device=dev)  # tthrml_adamw_ctl: step, lr (float64), ticket
+        self._lr = None
+        self.lr = lr
+        self._orders = [_dense_order(p) for p in self.params]
+        self._kinds = [(p.dtype, p.device, p.shape, p.stride()) for p in self.params]
+        self._live = np.array([i for i, p in enumerate(self.params) if p.numel()], dtype=np.int64)
+        # tthrml_adamw_tensor rows of the parameters that have elements
+        self._rows = np.zeros(len(self._live), dtype=np.dtype(nat.AdamWTensor))
+        self._rows["n"] = [self.params[i].numel() for i in self._live]
+        self._rows["state"] = [self.offsets[i] for i in self._live]
+        self._rows["param_dtype"] = [dtype_code(self.params[i].dtype) for i in self._live]
+        self._nothing = [None] * len(self.params)
+        self._param_ptrs = self._grad_ptrs = self._grads = None
+        self._state_ptrs = tuple(None if t is None else t.data_ptr() for t in
+                                 (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self._ctl))
+
+    # ---------------------------------------------------------------- control
+
+    @property
+    def lr(self) -> float:
+        return self._lr
+
+    @lr.setter
+    def lr(self, value) -> None:
+        """Queued on the current stream; steps launched (or replayed) after it use the new rate."""
+        value = float(value)
+        if not value >= 0.0:
+            raise ValueError(f"lr must not be below 0, got {value}")
+        if value != self._lr:
+            torch = _torch()
+            with torch.cuda.device(self.device):
+                self._ctl.view(torch.float64)[1].fill_(value)
+            self._lr = value
+
+    @property
+    def steps(self) -> int:
+        """Steps done (reads the device counter: synchronises)."""
+        return int(self._ctl[0].item())
+
+    # ------------------------------------------------------------------- step
+
+    def _check(self, grads) -> None:
+        """Raises unless every gradient has its parameter's device, shape and memory order and a fitting type."""
+        torch = _torch()
+        for i, (p, g, order) in enumerate(zip(self.params, grads, self._orders)):
+            if type(g) is torch.Tensor and (g.dtype, g.device, g.shape, g.stride()) == self._kinds[i]:
+                continue  # the parameter's own type and layout
+            require_cuda(f"gradient {i}", g, self.device)
+            if g.dtype not in (p.dtype, torch.float32):
+                raise ValueError(f"gradient {i} must be {p.dtype} or float32, got {g.dtype}")
+            if g.shape != p.shape or _dense_order(g) != order:
+                raise ValueError(
+                    f"gradient {i} needs the parameter's shape and memory order: shape {tuple(g.shape)}, strides "
+                    f"{tuple(g.stride())} for {tuple(p.shape)}, {tuple(p.stride())}"
+                )
+
+    def _check_params(self, ptrs) -> None:
+        for i, (p, kind) in enumerate(zip(self.params, self._kinds)):
+            if (p.dtype, p.device, p.shape, p.stride()) != kind:
+                raise ValueError(f"parameter {i} changed its type or layout since the optimizer was made")
+        column = np.array(ptrs, dtype=np.uint64)
+        self._rows["param"] = column[self._live]
+
+    def step(self, grads=None) -> None:
+        """One step of all parameters, queued on the current stream of their device."""
+        torch = _torch()
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(self.params)} parameters, {len(grads)} gradients")
+        if any(map(is_, grads, self._nothing)):
+            raise ValueError(f"parameter {next(i for i, g in enumerate(grads) if g is None)} has no gradient")
+        address = torch.Tensor.data_ptr
+        param_ptrs = list(map(address, self.params))
+        if param_ptrs != self._param_ptrs:
+            self._check_params(param_ptrs)
+            self._param_ptrs = param_ptrs
+        same = self._grads is not None and all(map(is_, grads, map(call, self._grads)))
+        if not same or list(map(address, grads)) != self._grad_ptrs:
+            self._grads = None
+            self._check(grads)
+            self._grad_ptrs = list(map(address, grads))
+            self._rows["grad"] = np.array(self._grad_ptrs, dtype=np.uint64)[self._live]
+            self._rows["grad_dtype"] = np.array([dtype_code(g.dtype) for g in grads], dtype=np.int32)[self._live]
+            self._grads = list(map(weakref.ref, grads))
+        m, v, ms, vs, ctl = self._state_ptrs
+        with on_device(self.device):
+            nat.check(
+                nat.lib().tthrml_adamw_step(
+                    self._rows.ctypes.data, len(self._rows), self.state_bits, m, v, ms, vs, ctl, self.betas[0], self.betas[1],
+                    self.eps, self.weight_decay, self.seed, torch.cuda.current_stream(self.device).cuda_stream,
+                ),
+                "tthrml_adamw_step",
+            )
+        torch.autograd.graph.increment_version(self.params)
+
+    # ------------------------------------------------------------------ state
+
+    def state_values(self, flat: bool = False):
+        """(first, second) moments as float32: one tensor per parameter in its shape and memory order, or the
+        two padded buffers (`flat`).  32-bit moments are returned as the optimizer's own buffers."""
+        torch = _torch()
+        m, v = self.exp_avg, self.exp_avg_sq
+        if self.state_bits == 8:
+            m, v = (torch.empty(t.shape, dtype=torch.float32, device=self.device) for t in (m, v))
+            with on_device(self.device):
+                nat.check(
+                    nat.lib().tthrml_adamw_values(
+                        *self._state_ptrs[:4], m.numel(), m.data_ptr(), v.data_ptr(),
+                        torch.cuda.current_stream(self.device).cuda_stream,
+                    ),
+                    "tthrml_adamw_values",
+                )
+        if flat:
+            return m[: self.elements], v[: self.elements]
+        return tuple([torch.as_strided(t, p.shape, p.stride(), o) if p.numel() else t[:0].view(p.shape)
+                      for p, o in zip(self.params, self.offsets)] for t in (m, v))
+
+    def state_dict(self) -> dict:
+        """The state as it is held: step, and copies of the padded buffers (codes and scales with 8 bits)."""
+        n = self.elements
+        d = {"step": self.steps, "exp_avg": self.exp_avg[:n].clone(), "exp_avg_sq": self.exp_avg_sq[:n].clone()}
+        if self.state_bits == 8:
+            d |= {"exp_avg_scale": self.exp_avg_scale[: n // BLOCK].clone(),
+                  "exp_avg_sq_scale": self.exp_avg_sq_scale[: n // BLOCK].clone()}
+        return d
+
+    def load_state_dict(self, state: dict) -> None:
+        names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if self.state_bits == 8 else [])
+        missing = [k for k in ["step", *names] if k not in state]
+        if missing:
+            raise ValueError(f"state without {', '.join(missing)}")
+        if int(state["step"]) < 0:
+            raise ValueError(f"step must not be below 0, got {state['step']}")
+        for k in names:
+            mine, t = getattr(self, k), state[k]
+            n = self.elements // (BLOCK if k.endswith("scale") else 1)
+            if tuple(t.shape) != (n,) or t.dtype != mine.dtype:
+                raise ValueError(f"{k} must be {mine.dtype} of {n} elements, got {t.dtype} of {tuple(t.shape)}")
+        for k in names:
+            getattr(self, k)[: state[k].numel()].copy_(state[k])
+        self._ctl[0].fill_(int(state["step"]))
+
+
+__all__ = ["AdamW"]

@@ -27,10 +27,15 @@ def _torch():
     return torch
 
 
+_codes: dict = {}
+
+
 def dtype_code(dtype):
     """The C ABI's code of a floating element type, or None."""
-    torch = _torch()
-    return {torch.float32: nat.DT_F32, torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16}.get(dtype)
+    if not _codes:
+        torch = _torch()
+        _codes.update({torch.float32: nat.DT_F32, torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16})
+    return _codes.get(dtype)
 
 
 _error_words: dict = {}
