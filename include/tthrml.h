@@ -637,6 +637,37 @@ int tthrml_adamw_values(const int8_t* exp_avg_dev, const uint8_t* exp_avg_sq_dev
                         int64_t elements, float* exp_avg_out_dev, float* exp_avg_sq_out_dev,
                         void* stream);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Pair moments of two blocks over the chain batch (dense programs).
+ * ---------------------------------------------------------------------------
+ */
+#define TTHRML_MAX_PHASES 6
+
+/* One term of a sum of pair moments: chain-major states of the two blocks. */
+typedef struct tthrml_moment_phase {
+  const void* x;  /* [chains][x_ld], 16-byte aligned, x_ld a multiple of 8 */
+  const void* y;  /* [chains][y_ld], likewise */
+  int64_t x_ld, y_ld, chains; /* chains may be 0 */
+  float scale;    /* of x^T y */
+  float x_scale, y_scale; /* of the unit sums */
+  float reserved;
+} tthrml_moment_phase;
+
+/*
+ * out[i][j] (+)= sum_p scale_p sum_c x_p[c][i] y_p[c][j], and, where x_sum /
+ * y_sum are given, x_sum[i] (+)= sum_p x_scale_p sum_c x_p[c][i] (y likewise).
+ * accumulate 0 overwrites, 1 adds to the values there.  dtype: TTHRML_DT_BF16
+ * or _F16 (of every operand); float32 sums and outputs, the same every time.
+ * phases: host array, read before the call returns.  out: [x_units][out_ld].
+ * The likelihood gradient of a dense program's couplings and biases is this
+ * with the data phase at -1 / chains and the model phase at 1 / chains.
+ */
+int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32_t n_phases, int32_t dtype,
+                        int64_t x_units, int64_t y_units, float* out_dev, int64_t out_ld,
+                        float* x_sum_dev, float* y_sum_dev, int32_t accumulate, int32_t* error_dev,
+                        void* stream);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

@@ -33,6 +33,7 @@ from .core import (
 )
 from .executor import Executor, make_executor
 from .mesh import MeshExecutor, make_mesh_executor, mesh_barrier, mesh_device_ids, mesh_size
+from .moments import pair_moments
 from .optim import AdamW
 from .quantized import QuantizedRows, check_operator_errors, int8_product, quantize_rows
 from .rng import generate_bulk_rng, make_rng_spec, slice_rng_for_sweep
@@ -97,5 +98,6 @@ __all__ = [
     "quantize_rows",
     "int8_product",
     "check_operator_errors",
+    "pair_moments",
     "AdamW",
 ]

@@ -21,6 +21,7 @@ KIND_LINEAR, KIND_PRECISION = 0, 1
 STATE_F32, STATE_I8, STATE_BITS = 0, 1, 2
 DT_F32, DT_BF16, DT_F16, DT_I8 = 0, 1, 2, 3
 INT8_MAX_COLS = 131071
+MAX_PHASES = 6
 MAX_CAT_SOURCES = 4
 MAX_CATEGORIES = 64
 
@@ -84,6 +85,22 @@ class AdamWTensor(ctypes.Structure):
         ("state", c_i64),
         ("param_dtype", c_i32),
         ("grad_dtype", c_i32),
+    ]
+
+
+class MomentPhase(ctypes.Structure):
+    """tthrml_moment_phase (include/tthrml.h)."""
+
+    _fields_ = [
+        ("x", c_vp),
+        ("y", c_vp),
+        ("x_ld", c_i64),
+        ("y_ld", c_i64),
+        ("chains", c_i64),
+        ("scale", ctypes.c_float),
+        ("x_scale", ctypes.c_float),
+        ("y_scale", ctypes.c_float),
+        ("reserved", ctypes.c_float),
     ]
 
 
@@ -200,6 +217,7 @@ _SIGNATURES = {
          ctypes.c_double, c_u64, c_vp],
     ),
     "tthrml_adamw_values": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "tthrml_pair_moments": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),
     "tthrml_last_error": (ctypes.c_char_p, []),

@@ -1,0 +1,123 @@
+"""Pair moments of two blocks over the chain batch: what a dense program's couplings are learned from.
+
+    out[i, j] = sum_p s_p sum_c x_p[c, i] y_p[c, j]
+
+over one or several phases p (data against model), with the unit sums
+sum_p s_p sum_c x_p[c, i].  The observers accumulate listed products of a
+row-major state (`DeviceMomentObserver`); this is the same for every pair of
+two dense blocks at once, on the tensor cores.
+"""
+
+from __future__ import annotations
+
+from . import _native as nat
+from .quantized import dtype_code, error_word, on_device, require_cuda
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def _operand(t, units):
+    """(tensor, pitch) of a chain-major operand laid out for the kernel: rows of 16-byte aligned elements."""
+    torch = _torch()
+    ld = t.stride(0) if t.shape[0] > 1 else -(-units // 8) * 8
+    if (t.stride(1) == 1 or units == 1) and ld % 8 == 0 and ld >= units and t.data_ptr() % 16 == 0:
+        return t, ld
+    ld = -(-units // 8) * 8
+    laid = torch.empty((t.shape[0], ld), dtype=t.dtype, device=t.device)[:, :units]
+    laid.copy_(t)
+    return laid, ld
+
+
+def _sum_target(name, t, n, dev):
+    torch = _torch()
+    require_cuda(name, t, dev)
+    if t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of shape ({n},), got {t.dtype} of {tuple(t.shape)}")
+    return t
+
+
+def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
+    """sum_p scale_p x_p^T y_p in float32 [M, N]; with `units` also sum_p scale_p x_p.sum(0) and the same of y.
+
+    x, y: one tensor each ([chains, M] and [chains, N], bfloat16 or float16,
+    one type) or sequences of them, one per phase (at most 6; chains may differ
+    between phases and may be 0); scale: a number or one per phase.  out: float32
+    [M, N] with dense rows (with `units` a tuple of out, x_sum [M], y_sum [N]) to
+    write, or, with `accumulate`, to add to.  The result is the same every time.
+    """
+    torch = _torch()
+    xs, ys = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (x, y))
+    scales = [float(scale)] * len(xs) if isinstance(scale, (int, float)) else [float(s) for s in scale]
+    if not xs or not len(xs) == len(ys) == len(scales):
+        raise ValueError(f"x, y and scale need one entry per phase, got {len(xs)}, {len(ys)} and {len(scales)}")
+    if len(xs) > nat.MAX_PHASES:
+        raise ValueError(f"at most {nat.MAX_PHASES} phases are supported, got {len(xs)}")
+    require_cuda("x", xs[0])
+    dev, dtype = xs[0].device, xs[0].dtype
+    code = dtype_code(dtype)
+    if code not in (nat.DT_BF16, nat.DT_F16):
+        raise ValueError(f"x and y must be bfloat16 or float16, got {dtype}")
+    shapes = []
+    for p, (a, b) in enumerate(zip(xs, ys)):
+        for name, t in ((f"x[{p}]", a), (f"y[{p}]", b)):
+            require_cuda(name, t, dev)
+            if t.dtype != dtype or t.dim() != 2:
+                raise ValueError(f"{name} must be a {dtype} matrix, got {t.dtype} of shape {tuple(t.shape)}")
+            if torch.is_grad_enabled() and t.requires_grad:
+                raise RuntimeError(f"{name} requires a gradient, but pair moments have no backward pass (use torch.no_grad())")
+        if a.shape[0] != b.shape[0]:
+            raise ValueError(f"phase {p}: x has {a.shape[0]} chains, y has {b.shape[0]}")
+        shapes.append((a.shape[1], b.shape[1]))
+    if any(s != shapes[0] for s in shapes):
+        raise ValueError(f"every phase needs the same units, got {shapes}")
+    M, N = shapes[0]
+    if M < 1 or N < 1:
+        raise ValueError(f"both blocks need units, got {M} and {N}")
+    x_sum = y_sum = None
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty((M, N), dtype=torch.float32, device=dev)
+        if units:
+            x_sum, y_sum = (torch.empty(n, dtype=torch.float32, device=dev) for n in (M, N))
+    else:
+        if units:
+            out, x_sum, y_sum = out
+            _sum_target("x_sum", x_sum, M, dev)
+            _sum_target("y_sum", y_sum, N, dev)
+        require_cuda("out", out, dev)
+        if out.dtype != torch.float32 or tuple(out.shape) != (M, N):
+            raise ValueError(f"out must be float32 of shape {(M, N)}, got {out.dtype} of {tuple(out.shape)}")
+        if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError("out needs dense rows that do not overlap")
+    phases = (nat.MomentPhase * len(xs))()
+    with on_device(dev):
+        held = []
+        for row, a, b, s in zip(phases, xs, ys, scales):
+            (a, x_ld), (b, y_ld) = _operand(a, M), _operand(b, N)
+            held.append((a, b))
+            row.x, row.y, row.x_ld, row.y_ld, row.chains = a.data_ptr(), b.data_ptr(), x_ld, y_ld, a.shape[0]
+            row.scale = row.x_scale = row.y_scale = s
+        launch(phases, code, M, N, out, x_sum, y_sum, accumulate, dev)
+    return (out, x_sum, y_sum) if units else out
+
+
+def launch(phases, code, M, N, out, x_sum, y_sum, accumulate, dev, stream=None) -> None:
+    """tthrml_pair_moments on `stream` (default: the current stream of `dev`)."""
+    torch = _torch()
+    stream = torch.cuda.current_stream(dev) if stream is None else stream
+    nat.check(
+        nat.lib().tthrml_pair_moments(
+            phases, len(phases), code, M, N, out.data_ptr(), out.stride(0) if M > 1 else N,
+            None if x_sum is None else x_sum.data_ptr(), None if y_sum is None else y_sum.data_ptr(),
+            1 if accumulate else 0, error_word(dev).data_ptr(), stream.cuda_stream,
+        ),
+        "tthrml_pair_moments",
+    )
+
+
+__all__ = ["pair_moments"]
