@@ -578,6 +578,24 @@ int tthrml_int8_product(const int8_t* x_dev, int64_t x_pitch, const float* x_sca
                         void* stream);
 
 /*
+ * Field GEMM + draw of one dense block on 8-bit operands
+ * (tthrml_dense_field_sample with the field (sum_k source weights) *
+ * (source_scale[chain] * w_scale[unit]) + bias[unit], the sum exact in int32).
+ * source: int8 [n_chains][source_pitch], source_scale float32 [n_chains] or
+ * NULL (ones: spins as +-1).  out_state: int8 [n_chains][n_units] spins (+-1)
+ * or bfloat16 [n_chains][n_units] gaussian values.  n_units % 32 == 0.  The
+ * draws, counters and variates are those of tthrml_dense_field_sample.
+ */
+int tthrml_int8_field_sample(const int8_t* source_dev, int64_t source_pitch,
+                             const float* source_scale_dev, const int8_t* weights_nk_dev,
+                             int64_t w_pitch, const float* w_scale_dev, int64_t n_chains,
+                             int64_t n_units, int64_t n_sources, const float* bias_dev, int32_t family,
+                             float precision, void* out_state_dev, int64_t row0, int64_t chain_offset,
+                             const float* variates_dev, int64_t variates_sweeps, uint64_t seed,
+                             uint32_t sweep, const tthrml_run_ctl* ctl_dev, int32_t* error_dev,
+                             void* stream);
+
+/*
  * The same for 1 to 8 rows in one launch, reading the weights once.  x:
  * [rows][x_ld] elements of x_dtype; float32, bfloat16 and float16 rows are
  * quantised in the launch exactly as tthrml_quantize_rows does, int8 rows are

@@ -1,0 +1,165 @@
+"""Operators' argument checks on the CPU: rejected calls touch neither the device nor the stand-in pointers."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import tt_thrml_b200 as tt
+from tt_thrml_b200 import _native as nat, compiler, workloads
+
+_A, _M = 4096, 4100  # a 16-byte aligned and a misaligned stand-in address
+
+
+def phases(n=1, **kw):
+    rows = (nat.MomentPhase * n)()
+    for r in rows:
+        r.x, r.y, r.x_ld, r.y_ld, r.chains = _A, _A, 64, 64, 10
+        for k, v in kw.items():
+            setattr(r, k, v)
+    return rows
+
+
+def tensors(**kw):
+    rows = (nat.AdamWTensor * 1)()
+    rows[0].param, rows[0].grad, rows[0].n, rows[0].state = _A, _A, 5, 0
+    for k, v in kw.items():
+        setattr(rows[0], k, v)
+    return rows
+
+
+def quantize(x=_A, dtype=0, rows=2, cols=40, rs=40, cs=1, values=_A, pitch=48, scale=_A):
+    return x, dtype, rows, cols, rs, cs, values, pitch, scale, None
+
+
+def product(x=_A, xp=48, w=_A, wp=48, ws=_A, rows=20, units=8, cols=40, out=_A, dt=0, ld=8, err=_A):
+    return x, xp, None, w, wp, ws, rows, units, cols, None, out, dt, ld, err, None
+
+
+def few(x=_A, xd=1, ld=40, w=_A, wp=48, rows=2, units=8, cols=40, out=_A, od=0, old=8):
+    return x, xd, ld, None, w, wp, _A, rows, units, cols, None, out, od, old, None
+
+
+def field(src=_A, sp=64, w=_A, wp=64, ws=_A, c=128, n=256, k=64, bias=None, family=0, out=_A, offset=0, err=_A):
+    return src, sp, None, w, wp, ws, c, n, k, bias, family, 1.0, out, 0, offset, None, 0, 0, 0, None, err, None
+
+
+def moments(ph, n=1, dt=1, m=8, k=8, out=_A, ld=8, err=_A):
+    return ph, n, dt, m, k, out, ld, None, None, 0, err, None
+
+
+def adamw(t, n=1, bits=32, m=_A, v=_A, ms=None, vs=None, ctl=_A, b1=0.9, b2=0.99, eps=1e-8, wd=0.0):
+    return t, n, bits, m, v, ms, vs, ctl, b1, b2, eps, wd, 0, None
+
+
+BAD = [
+    ("tthrml_quantize_rows", quantize(x=None), b"NULL"),
+    ("tthrml_quantize_rows", quantize(cols=0), b"out of range"),
+    ("tthrml_quantize_rows", quantize(cs=0), b"out of range"),
+    ("tthrml_quantize_rows", quantize(pitch=40), b"multiple of 16"),
+    ("tthrml_quantize_rows", quantize(pitch=32), b"multiple of 16"),
+    ("tthrml_quantize_rows", quantize(values=_M), b"16-byte aligned"),
+    ("tthrml_quantize_rows", quantize(dtype=3), b"input type"),
+    ("tthrml_int8_product", product(err=None), b"NULL"),
+    ("tthrml_int8_product", product(cols=131072, xp=131072, wp=131072), b"out of range"),
+    ("tthrml_int8_product", product(rows=-1), b"out of range"),
+    ("tthrml_int8_product", product(dt=3), b"output type"),
+    ("tthrml_int8_product", product(dt=9), b"output type"),
+    ("tthrml_int8_product", product(x=_M), b"16-byte aligned"),
+    ("tthrml_int8_product", product(wp=40), b"16-byte aligned"),
+    ("tthrml_int8_product", product(xp=32), b"16-byte aligned"),
+    ("tthrml_int8_product", product(ld=7), b"must not overlap"),
+    ("tthrml_int8_product_few", few(w=None), b"NULL"),
+    ("tthrml_int8_product_few", few(rows=9), b"1 to 8 rows"),
+    ("tthrml_int8_product_few", few(rows=8, cols=20500, ld=20500, wp=20512), b"shared memory"),
+    ("tthrml_int8_product_few", few(xd=7), b"unknown element type"),
+    ("tthrml_int8_product_few", few(od=3), b"unknown element type"),
+    ("tthrml_int8_product_few", few(ld=39), b"must not overlap"),
+    ("tthrml_int8_product_few", few(w=_M), b"16-byte aligned"),
+    ("tthrml_int8_field_sample", field(out=None), b"NULL"),
+    ("tthrml_int8_field_sample", field(n=40), b"multiple of 32"),
+    ("tthrml_int8_field_sample", field(k=131072, sp=131072, wp=131072), b"at most"),
+    ("tthrml_int8_field_sample", field(family=1), b"spin or gaussian"),
+    ("tthrml_int8_field_sample", field(offset=2), b"chain_offset"),
+    ("tthrml_int8_field_sample", field(bias=_M), b"16-byte aligned"),
+    ("tthrml_int8_field_sample", field(sp=60), b"pitches"),
+    ("tthrml_pair_moments", moments(None), b"NULL"),
+    ("tthrml_pair_moments", moments(phases(7), n=7), b"1 to 6 phases"),
+    ("tthrml_pair_moments", moments(phases(), dt=0), b"bfloat16 or float16"),
+    ("tthrml_pair_moments", moments(phases(), m=0), b"out of range"),
+    ("tthrml_pair_moments", moments(phases(), ld=7), b"out of range"),
+    ("tthrml_pair_moments", moments(phases(x=_M)), b"16-byte aligned"),
+    ("tthrml_pair_moments", moments(phases(y_ld=60)), b"16-byte aligned"),
+    ("tthrml_pair_moments", moments(phases(x_ld=8), m=9), b"16-byte aligned"),
+    ("tthrml_pair_moments", moments(phases(chains=-1)), b"16-byte aligned"),
+    ("tthrml_adamw_step", adamw(None), b"NULL"),
+    ("tthrml_adamw_step", adamw(tensors(), bits=8), b"NULL"),
+    ("tthrml_adamw_step", adamw(tensors(), bits=16), b"8 or 32"),
+    ("tthrml_adamw_step", adamw(tensors(), b1=1.0), b"betas"),
+    ("tthrml_adamw_step", adamw(tensors(), eps=0.0), b"eps"),
+    ("tthrml_adamw_step", adamw(tensors(), b2=float("nan")), b"betas"),
+    ("tthrml_adamw_step", adamw(tensors(), m=_M), b"16-byte aligned"),
+    ("tthrml_adamw_step", adamw(tensors(n=0)), b"tensor 0"),
+    ("tthrml_adamw_step", adamw(tensors(state=128)), b"tensor 0"),
+    ("tthrml_adamw_step", adamw(tensors(param_dtype=3)), b"tensor 0"),
+    ("tthrml_adamw_step", adamw(tensors(grad=_A + 2)), b"tensor 0"),
+    ("tthrml_adamw_values", (_A, _A, _A, _A, 100, _A, _A, None), b"multiple of 256"),
+    ("tthrml_adamw_values", (None, _A, _A, _A, 256, _A, _A, None), b"NULL"),
+]
+
+
+@pytest.mark.parametrize("name,args,message", BAD, ids=[f"{c[0]}-{i}" for i, c in enumerate(BAD)])
+def test_bad_arguments_are_rejected_before_any_cuda_call(name, args, message):
+    lib = nat.lib()
+    assert getattr(lib, name)(*args) == -1
+    assert message in lib.tthrml_last_error(), lib.tthrml_last_error()
+
+
+@pytest.mark.parametrize("name,args", [
+    ("tthrml_quantize_rows", quantize(rows=0, x=None)),
+    ("tthrml_int8_product", product(rows=0, x=None)),
+    ("tthrml_int8_product", product(units=0, w=None)),
+    ("tthrml_int8_product_few", few(rows=0, x=None)),
+    ("tthrml_adamw_step", adamw(None, n=0)),
+    ("tthrml_adamw_values", (None, None, None, None, 0, None, None, None)),
+])
+def test_empty_calls_do_nothing(name, args):
+    assert getattr(nat.lib(), name)(*args) == 0
+
+
+def test_structures_have_the_header_layout():
+    assert ctypes.sizeof(nat.AdamWTensor) == 40 and ctypes.sizeof(nat.MomentPhase) == 56
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.ones((2, 3))
+    for call in (lambda: tt.quantize_rows(x), lambda: tt.QuantizedRows(x.to(torch.int8)), lambda: tt.AdamW([x]),
+                 lambda: tt.pair_moments(x.bfloat16(), x.bfloat16())):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+    with pytest.raises(TypeError):
+        tt.int8_product(x, x)
+    with pytest.raises(ValueError):
+        tt.AdamW([])
+
+
+def test_host_quantisation_and_the_int8_plan():
+    r = np.random.default_rng(0)
+    w = r.standard_normal((5, 37)).astype(np.float32)
+    w[2] = 0.0
+    q, s = compiler.quantize_rows_host(w)
+    assert q.shape == (5, 48) and not q[:, 37:].any() and not q[2].any() and s[2] == 0.0
+    assert np.abs(q).max(1)[[0, 1, 3, 4]].tolist() == [127] * 4
+    # half a step of the row's scale, and float32 roundings
+    assert (np.abs(q[:, :37] * s[:, None].astype(np.float64) - w) <= s[:, None] * (0.5 + 1e-4)).all()
+    w[1, 1] = np.inf
+    with pytest.raises(ValueError):
+        compiler.quantize_rows_host(w)
+    program = workloads.gaussian_bernoulli_rbm(256, 512, seed=1)
+    plans = compiler._plan_dense(program, torch.device("cpu"), "int8")
+    assert [p.weights_nk.dtype for p in plans] == [torch.int8] * 2 and all(p.w_scale is not None for p in plans)
+    with pytest.raises(ValueError):
+        tt.make_cuda_config(dense_precision="int4")
+    a, b = tt.make_cuda_config(dense_precision="int8"), tt.make_cuda_config(dense_precision="bf16")
+    assert a.resolved_dense_precision == "int8" and a.plan_key() != b.plan_key()

@@ -12,7 +12,7 @@ import tt_thrml_b200 as _impl
 from tt_thrml_b200 import *  # noqa: F401,F403
 from tt_thrml_b200 import __all__  # noqa: F401
 
-for _name in ("compiler", "executor", "core", "rng", "mesh", "conditional_samplers", "observers", "backend", "quantized", "optim", "moments"):
+for _name in ("compiler", "executor", "core", "rng", "mesh", "conditional_samplers", "observers", "backend", "quantized", "optim", "moments", "learning"):
     _mod = __import__(f"tt_thrml_b200.{_name}", fromlist=[_name])
     _sys.modules[f"{__name__}.{_name}"] = _mod
     globals()[_name] = _mod

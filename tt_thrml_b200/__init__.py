@@ -32,6 +32,7 @@ from .core import (
     open_mesh_device,
 )
 from .executor import Executor, make_executor
+from .learning import DenseLearner, dense_moments
 from .mesh import MeshExecutor, make_mesh_executor, mesh_barrier, mesh_device_ids, mesh_size
 from .moments import pair_moments
 from .optim import AdamW
@@ -99,5 +100,7 @@ __all__ = [
     "int8_product",
     "check_operator_errors",
     "pair_moments",
+    "dense_moments",
+    "DenseLearner",
     "AdamW",
 ]

@@ -207,6 +207,11 @@ _SIGNATURES = {
         c_i32,
         [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp, c_vp],
     ),
+    "tthrml_int8_field_sample": (
+        c_i32,
+        [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_i32, ctypes.c_float, c_vp, c_i64, c_i64,
+         c_vp, c_i64, c_u64, c_u32, c_vp, c_vp, c_vp],
+    ),
     "tthrml_int8_product_few": (
         c_i32,
         [c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp],

@@ -688,6 +688,8 @@ class DenseGroupPlan:
     group_rows: int = 0
     device: Any = None
     rng_layout: str = "row4"  # Philox counter (chain, row / 4, sweep), word row % 4
+    w_scale: Any = None  # float32 [n_units]: weights_nk is int8 [n_units][pitch], else None
+    owned: bool = False  # the weights and bias are this executor's own (update_dense_weights), not the plan cache's
 
 
 DENSE_CHAIN_MULTIPLE = 128
@@ -706,6 +708,10 @@ def dense_eligible(program, n_chains: int) -> bool:
         if c["n_units"] % DENSE_UNIT_MULTIPLE or Family(c["family"]) not in (Family.SPIN, Family.GAUSSIAN):
             return False
     return True
+
+
+def _dense_state(precision: str) -> str:
+    return "dense_int8" if precision == "int8" else "dense_bf16"
 
 
 def dense_pieces(program, precision: str) -> dict[int, int]:
@@ -793,8 +799,13 @@ def _plan_dense_couplings(couplings: dict, sampling_order, device, precision: st
         bi = int(group[0])
         c = couplings[bi]
         w = np.ascontiguousarray(c["weights_nk"], dtype=np.float32)
-        wt = torch.from_numpy(w).to(device=device, dtype=torch.bfloat16).contiguous()
-        if not torch.equal(wt.float().cpu(), torch.from_numpy(w)):
+        scale = None
+        if precision == "int8":
+            wt, scale = quantize_rows_host(w)
+            wt, scale = torch.from_numpy(wt).to(device), torch.from_numpy(scale).to(device)
+        else:
+            wt = torch.from_numpy(w).to(device=device, dtype=torch.bfloat16).contiguous()
+        if scale is None and not torch.equal(wt.float().cpu(), torch.from_numpy(w)):
             raise ValueError(
                 f"block {bi}: dense couplings must be bf16-representable (round them with "
                 "workloads.bf16_representable) so the tensor-core operands are the model's weights"
@@ -819,9 +830,24 @@ def _plan_dense_couplings(couplings: dict, sampling_order, device, precision: st
                 family_label=fam.value,
                 group_rows=int(c["n_units"]),
                 device=device,
+                w_scale=scale,
             )
         )
     return plans
+
+
+def quantize_rows_host(w: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """(int8 [rows][pitch], float32 scales) of a float32 matrix, as tthrml_quantize_rows makes them on the device."""
+    rows, cols = w.shape
+    top = np.abs(w).max(1) if cols else np.zeros(rows, np.float32)
+    if not np.isfinite(top).all():
+        raise ValueError("8-bit dense couplings must be finite")
+    live = top >= np.float32(2.0**-120)
+    inv = np.zeros_like(top)
+    inv[live] = np.float32(127.0) / top[live]
+    q = np.zeros((rows, -(-cols // 16) * 16), dtype=np.int8)
+    q[:, :cols] = np.clip(np.rint(w * inv[:, None]), -127, 127).astype(np.int8)
+    return q, np.where(live, top * np.float32(1.0 / 127.0), np.float32(0.0)).astype(np.float32)
 
 
 def _dense_specs(program):
@@ -1371,7 +1397,8 @@ def _build_plans(program, config: CUDAConfig, n_chains: int, tdev, force_generic
         order = tuple(tuple(int(i) for i in g) for g in program.gibbs_spec.sampling_order)
         lowered = LoweredProgram(specs, order, len(program.gibbs_spec.free_blocks), specs[0].total_nodes,
                                  tuple(s.block_global_start for s in specs))
-        state_dtype, plans = "dense_bf16", _plan_dense(program, tdev, config.resolved_dense_precision)
+        precision = config.resolved_dense_precision
+        state_dtype, plans = _dense_state(precision), _plan_dense(program, tdev, precision)
     else:
         lowered = pre_lowered if pre_lowered is not None else lower_program(program)
         if not force_generic and config.stencil:
@@ -1385,7 +1412,7 @@ def _build_plans(program, config: CUDAConfig, n_chains: int, tdev, force_generic
         if not force_generic and config.dense_detect and not callable(getattr(program, "tt_stencil", None)):
             couplings = detect_dense_couplings(lowered, n_chains, round_weights=config.dense_round_weights)
         if couplings is not None:
-            state_dtype = "dense_bf16"
+            state_dtype = _dense_state(config.resolved_dense_precision)
             plans = _plan_dense_couplings(couplings, lowered.sampling_order, tdev, config.resolved_dense_precision)
         else:
             state_dtype, plans = plan_program(

@@ -34,7 +34,7 @@ RNG_MODES = ("philox", "parity")
 # multiple of 256 chains), "int8" one byte per chain; "auto" picks bits when
 # the chain count allows.
 SPIN_LAYOUTS = ("auto", "bits", "int8")
-DENSE_PRECISIONS = ("auto", "bf16", "fp32")
+DENSE_PRECISIONS = ("auto", "bf16", "fp32", "int8")
 
 
 @dataclass(frozen=True)
@@ -50,7 +50,10 @@ class CUDAConfig:
     dense_precision: tensor-core path of dense bipartite programs. "bf16"
       keeps gaussian block states as bf16 GEMM operands; "fp32" keeps them
       float32, fed to the GEMM as three bf16 pieces against the weights
-      repeated along K (the float32 field up to summation order); "auto" is
+      repeated along K (the float32 field up to summation order); "int8" rounds
+      the weights to 8 bits with a scale per unit and the gaussian sources to 8
+      bits with a scale per chain before each product (spins are exact; a
+      different model by those roundings, never chosen by itself); "auto" is
       "fp32" in parity mode and "bf16" in Philox mode.
     stencil: run lattice programs on the stencil kernels (False: their tables).
     dense_detect: look for dense bipartite structure in lowered programs (an RBM

@@ -7,8 +7,13 @@
 // blocks.  Warp 0 loads (TMA, 128-byte swizzle, columns and rows behind the ends read as zeros), warp 1 multiplies,
 // then all eight warps move the accumulator to shared memory, and CTA r of the cluster adds the S partial tiles of
 // rows r, r + S, ... over distributed shared memory, scales and stores them as whole rows.
+//
+// k_int8_pair: persistent clusters of two CTAs walk 256 x 256 tiles (tcgen05 cta_group::2, as the bf16 kernel of the dense
+// sweeps does): each CTA holds 128 rows of either operand per stage, the even CTA issues every MMA, two TMEM accumulators let
+// the epilogue of one tile run under the main loop of the next.  The epilogue stores the scaled sums, or takes them as
+// the fields of a dense block and draws its new state.
+#include "dense_draw.cuh"
 #include "int8_common.cuh"
-#include "tc_common.cuh"
 
 namespace tthrml {
 namespace {
@@ -223,6 +228,286 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (split > 1) cluster_sync_all();  // no CTA leaves while another still reads its shared memory
 }
 
+// ---------------------------------------------------------------------------
+// CTA-pair kernel
+// ---------------------------------------------------------------------------
+constexpr int kPairStages = 6, kPairStage = 2 * 128 * 128, kPairThreads = 320, kPairWarps = 8;
+constexpr int kPairRowPitch = 33;  // floats per row of a warp's 32 x 32 transpose (unaligned outputs)
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kPairWarps * 32 * kPairRowPitch * 4;
+enum : int { kStoreFields = 0, kDrawSpins = 1, kDrawGaussians = 2 };
+
+struct PairArgs {
+  ProductArgs p;
+  DenseArgs d;       // draws: bias, variates, counters; M, N
+  int8_t* spins;     // [M][N] new spins
+  __nv_bfloat16* values;  // [M][N] new gaussian values
+};
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc_i8(256, 256)), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u),
+      "r"(0u), "r"(0u), "r"(0u));
+}
+
+// Sums of 32 consecutive units of one row, scaled: (float)sum * (s_x * s_w).
+__device__ __forceinline__ void scale_chunk(const ProductArgs& a, float sx, int n_first, float (&v)[32]) {
+  if (n_first + 32 <= a.N && (uintptr_t)a.w_scale % 16 == 0) {
+    const float4* sw = reinterpret_cast<const float4*>(a.w_scale + n_first);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 w = __ldg(sw + q);
+      v[4 * q] = __fmul_rn((float)__float_as_int(v[4 * q]), __fmul_rn(sx, w.x));
+      v[4 * q + 1] = __fmul_rn((float)__float_as_int(v[4 * q + 1]), __fmul_rn(sx, w.y));
+      v[4 * q + 2] = __fmul_rn((float)__float_as_int(v[4 * q + 2]), __fmul_rn(sx, w.z));
+      v[4 * q + 3] = __fmul_rn((float)__float_as_int(v[4 * q + 3]), __fmul_rn(sx, w.w));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float w = n_first + j < a.N ? __ldg(a.w_scale + n_first + j) : 0.0f;
+      v[j] = __fmul_rn((float)__float_as_int(v[j]), __fmul_rn(sx, w));
+    }
+  }
+}
+
+// Stores one 32-column chunk of 32 rows (lane = row m0 + lane): each lane its own row where rows are aligned, else by way
+// of shared memory, so that a warp stores consecutive elements.
+__device__ __forceinline__ void store_chunk(const ProductArgs& a, int m, int n_first, const float (&v)[32], float* turn) {
+  float y[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    y[j] = v[j];
+    if (a.bias) y[j] = __fadd_rn(y[j], n_first + j < a.N ? __ldg(a.bias + n_first + j) : 0.0f);
+  }
+  if (a.vector_store && n_first + 32 <= a.N) {
+    if (m >= a.M) return;
+    const int64_t at = (int64_t)m * a.out_ld + n_first;
+    if (a.out_dtype == TTHRML_DT_F32) {
+      float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) dst[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+    } else {
+      uint32_t w[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (a.out_dtype == TTHRML_DT_BF16) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __half2 h = __floats2half2_rn(y[2 * j], y[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) turn[lane * kPairRowPitch + j] = y[j];
+  __syncwarp();
+  const int n = n_first + lane;
+  if (n < a.N) {
+    for (int r = 0; r < 32 && m - lane + r < a.M; ++r) {
+      const int64_t at = (int64_t)(m - lane + r) * a.out_ld + n;
+      const float f = turn[r * kPairRowPitch + lane];
+      if (a.out_dtype == TTHRML_DT_F32)
+        reinterpret_cast<float*>(a.out)[at] = f;
+      else if (a.out_dtype == TTHRML_DT_BF16)
+        reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(f);
+      else
+        reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(f);
+    }
+  }
+  __syncwarp();
+}
+
+template <int EPI, bool VARIATES>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    k_int8_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ PairArgs args) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + kPairStages * kPairStage);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;        // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* turns = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);
+
+  const ProductArgs& a = args.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int m_blocks = (a.M + 255) / 256, n_blocks = (a.N + 255) / 256;
+  const int n_tiles = m_blocks * n_blocks;
+  const int first = (int)cluster_id_x(), step = (int)n_clusters_x();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kPairWarps);  // every epilogue warp of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers exist before either signals the other
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  int last_it[2] = {-1, -1};
+
+  if (warp == 0) {
+    if (lane == 0) {  // producer (both CTAs): this CTA's halves of the A and B slices
+      int64_t issued = 0;
+      bool failed = false;
+      for (int t = first; t < n_tiles && !failed; t += step) {
+        int mb, nb;
+        tile_coords(t, m_blocks, n_blocks, args.d.group, mb, nb);
+        for (int kb = 0; kb < a.num_k; ++kb) {
+          const int s = (int)(issued % kPairStages);
+          if (!mbar_wait(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
+            atomicExch(a.error, kErrEmptyWait);
+            failed = true;
+            break;
+          }
+          if (leader) mbar_expect_tx(&full[s], 2 * kPairStage);  // the stage's bytes of both CTAs
+          unsigned char* st = tiles + s * kPairStage;
+          const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
+          tma_load_2d_pair(st, &map_a, bar, kb * 128, mb * 256 + (int)rank * 128);
+          tma_load_2d_pair(st + kPairStage / 2, &map_b, bar, kb * 128, nb * 256 + (int)rank * 128);
+          ++issued;
+        }
+      }
+      // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
+      for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
+        if (!mbar_wait(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u)) atomicExch(a.error, kErrEmptyWait);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {  // MMA issue: the leader only
+      int64_t used = 0;
+      int it = 0;
+      bool failed = false;
+      for (int t = first; t < n_tiles && !failed; t += step, ++it) {
+        const int b = it & 1;
+        if (!mbar_wait(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
+          atomicExch(a.error, kErrAccWait);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(b * 256);
+        for (int kb = 0; kb < a.num_k; ++kb) {
+          const int s = (int)(used % kPairStages);
+          if (!mbar_wait(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
+            atomicExch(a.error, kErrFullWait);
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          const unsigned char* st = tiles + s * kPairStage;
+          const uint64_t ad = umma_desc_sw128(st), bd = umma_desc_sw128(st + kPairStage / 2);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // K = 32 bytes per MMA
+            umma_i8_pair(d, ad + 2ull * kk, bd + 2ull * kk, (kb > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+          ++used;
+        }
+        umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
+        last_it[b] = it;
+      }
+    }
+  } else {
+    const int quad = warp & 3, grp = (warp - 2) >> 2;
+    float* turn = turns + (warp - 2) * 32 * kPairRowPitch;
+    int it = 0;
+    for (int t = first; t < n_tiles; t += step, ++it) {
+      int mb, nb;
+      tile_coords(t, m_blocks, n_blocks, args.d.group, mb, nb);
+      const int b = it & 1;
+      const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane;
+      const float sx = a.x_scale && m < a.M ? __ldg(a.x_scale + m) : 1.0f;
+      if (!mbar_wait(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
+        if (lane == 0) atomicExch(a.error, kErrAccWait);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sweep = args.d.sweep + (EPI != kStoreFields && args.d.ctl ? args.d.ctl->sweep : 0u);
+      const uint64_t sd = EPI != kStoreFields && args.d.ctl ? args.d.ctl->seed : args.d.seed;
+      const PhiloxKeys keys = philox_keys(seed_lo(sd), seed_hi(sd));
+      const float inv = 1.0f / __fadd_rn(args.d.precision, 1e-6f);
+      const float sd_g = sqrtf(inv);
+      const int64_t vs = VARIATES ? (int64_t)(sweep % (uint32_t)(args.d.variates_sweeps > 0 ? args.d.variates_sweeps : 1)) : 0;
+      for (int c = grp; c < 8 && nb * 256 + c * 32 < a.N; c += 2) {
+        const int n_first = nb * 256 + c * 32;
+        float v[32];
+        tmem_load32(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(c * 32), v);
+        scale_chunk(a, sx, n_first, v);
+        if (EPI == kStoreFields) {
+          store_chunk(a, m, n_first, v, turn);
+        } else if (m < a.M) {  // draws: N is a multiple of 32
+          if (EPI == kDrawSpins) {
+            uint32_t near;
+            const uint32_t down = spin_chunk<VARIATES>(args.d, v, m, n_first, sweep, keys, vs, near);
+            uint32_t w[8];  // four spins a word: bit -> 0x01 / 0xFF
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const uint32_t four = (down >> (4 * q)) & 15u;
+              w[q] = 0x01010101u | (((four * 0x00204081u) & 0x01010101u) * 0xFEu);
+            }
+            uint4* dst = reinterpret_cast<uint4*>(args.spins + (int64_t)m * a.N + n_first);
+            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          } else {
+            float f[32];
+            gauss_chunk<VARIATES>(args.d, v, m, n_first, sweep, keys, inv, sd_g, vs, f);
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+              w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            uint4* dst = reinterpret_cast<uint4*>(args.values + (int64_t)m * a.N + n_first);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+          }
+        }
+        __syncwarp();  // the next TMEM load is a warp's
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(&acc_empty[b]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1 && leader) {
+    // every MMA the pair issued has completed (in both CTAs' TMEM) before TMEM is freed
+    if (lane == 0) {
+      for (int b = 0; b < 2; ++b)
+        if (last_it[b] >= 0) (void)mbar_wait(&acc_full[b], (uint32_t)(last_it[b] >> 1) & 1u);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA frees TMEM or exits while the other may still signal it
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
 // Tensor map of an 8-bit matrix [rows][cols] with rows `pitch` bytes apart, read in (box_rows x 128) tiles, 128-byte swizzle.
 int make_map_i8(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, uint32_t box_rows) {
   EncodeTiledFn fn;
@@ -249,6 +534,20 @@ int launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs&
   void* params[3] = {(void*)&ma, (void*)&mb, (void*)&a};
   return launch_clusters((const void*)k_int8_tile<BN>, (unsigned)(tiles * split), (unsigned)split, kTileThreads,
                          TileShape<BN>::kSmem, params, st, "k_int8_tile launch");
+}
+
+// As many clusters as are resident at once walk the tiles.
+int launch_pair(const void* fn, const CUtensorMap& ma, const CUtensorMap& mb, PairArgs& a, int64_t cols, cudaStream_t st) {
+  ClusterFit fit;
+  const int rc = cluster_fit(fn, 2, kPairThreads, kPairSmem, &fit);
+  if (rc) return rc;
+  const int64_t mblk = (a.p.M + 255) / 256, tiles = mblk * ((a.p.N + 255) / 256);
+  const int64_t g = ((int64_t)32 << 20) / (256 * cols);  // raster groups of about 32 MiB of A panels, as in the bf16 kernel
+  a.d.group = (int32_t)(g < 1 ? 1 : (g > mblk ? mblk : g));
+  const int64_t clusters = tiles < fit.clusters ? tiles : fit.clusters;
+  void* params[3] = {(void*)&ma, (void*)&mb, (void*)&a};
+  return launch_clusters(fn, (unsigned)(2 * clusters), 2, kPairThreads, kPairSmem, params, st,
+                         "k_int8_pair launch");
 }
 
 }  // namespace
@@ -295,11 +594,84 @@ extern "C" int tthrml_int8_product(const int8_t* x, int64_t x_pitch, const float
   a.num_k = (int32_t)((cols + 127) / 128);
   a.box_m = rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128));
   a.error = error;
+  cudaStream_t st = (cudaStream_t)stream;
   CUtensorMap ma, mb;
-  int rc = make_map_i8(&ma, x, rows, cols, x_pitch, (uint32_t)a.box_m);
+  int rc;
+  const bool pair = ((rows + 255) / 256) * ((units + 255) / 256) >= 64;
+  if (pair) {
+    rc = make_map_i8(&ma, x, rows, cols, x_pitch, 128u);
+    if (rc == TTHRML_OK) rc = make_map_i8(&mb, weights, units, cols, w_pitch, 128u);
+    if (rc) return rc;
+    PairArgs pa = {};
+    pa.p = a;
+    pa.p.vector_store = (uintptr_t)out % 16 == 0 && (out_ld * dtype_bytes(out_dtype)) % 16 == 0;
+    return launch_pair((const void*)k_int8_pair<kStoreFields, false>, ma, mb, pa, cols, st);
+  }
+  rc = make_map_i8(&ma, x, rows, cols, x_pitch, (uint32_t)a.box_m);
   if (rc) return rc;
   const int bn = 128;
   rc = make_map_i8(&mb, weights, units, cols, w_pitch, (uint32_t)bn);
   if (rc) return rc;
-  return launch_tile<128>(ma, mb, a, 1, (cudaStream_t)stream);
+  return launch_tile<128>(ma, mb, a, 1, st);
+}
+
+extern "C" int tthrml_int8_field_sample(const int8_t* source, int64_t source_pitch, const float* source_scale,
+                                        const int8_t* weights_nk, int64_t w_pitch, const float* w_scale,
+                                        int64_t n_chains, int64_t n_units, int64_t n_sources, const float* bias,
+                                        int32_t family, float precision, void* out_state, int64_t row0,
+                                        int64_t chain_offset, const float* variates, int64_t variates_sweeps,
+                                        uint64_t seed, uint32_t sweep, const tthrml_run_ctl* ctl, int32_t* error,
+                                        void* stream) {
+  using namespace tthrml;
+  if (!source || !weights_nk || !w_scale || !out_state || !error) {
+    set_error("tthrml_int8_field_sample: NULL argument");
+    return TTHRML_ERR_ARG;
+  }
+  if (n_chains <= 0 || n_units <= 0 || n_units % 32 || n_sources <= 0 || n_sources > TTHRML_INT8_MAX_COLS ||
+      n_chains > 0x7fffff00LL || n_units > 0x7fffff00LL || ((n_chains + 255) / 256) * ((n_units + 255) / 256) > 0x0fffffffLL) {
+    set_error("tthrml_int8_field_sample: units must be a multiple of 32 and sources at most %d (got %lld chains, %lld "
+              "units, %lld sources)", TTHRML_INT8_MAX_COLS, (long long)n_chains, (long long)n_units, (long long)n_sources);
+    return TTHRML_ERR_ARG;
+  }
+  if (family != TTHRML_SPIN && family != TTHRML_GAUSSIAN) {
+    set_error("tthrml_int8_field_sample: family must be spin or gaussian");
+    return TTHRML_ERR_ARG;
+  }
+  if (chain_offset % 4 || (uintptr_t)source % 16 || (uintptr_t)weights_nk % 16 || source_pitch % 16 || w_pitch % 16 ||
+      source_pitch < n_sources || w_pitch < n_sources || (uintptr_t)out_state % 16 || (bias && (uintptr_t)bias % 16)) {
+    set_error("tthrml_int8_field_sample: buffers must be 16-byte aligned, pitches multiples of 16 not below the sources "
+              "and chain_offset a multiple of 4 (got pitches %lld, %lld)", (long long)source_pitch, (long long)w_pitch);
+    return TTHRML_ERR_ARG;
+  }
+  PairArgs pa = {};
+  pa.p.x_scale = source_scale;
+  pa.p.w_scale = w_scale;
+  pa.p.M = (int32_t)n_chains;
+  pa.p.N = (int32_t)n_units;
+  pa.p.num_k = (int32_t)((n_sources + 127) / 128);
+  pa.p.error = error;
+  pa.d.bias = bias;
+  pa.d.variates = variates;
+  pa.d.variates_sweeps = variates_sweeps;
+  pa.d.M = n_chains;
+  pa.d.N = n_units;
+  pa.d.K = n_sources;
+  pa.d.row0 = row0;
+  pa.d.chain_offset = chain_offset;
+  pa.d.seed = seed;
+  pa.d.sweep = sweep;
+  pa.d.family = family;
+  pa.d.precision = precision;
+  pa.d.ctl = ctl;
+  pa.spins = (int8_t*)out_state;
+  pa.values = (__nv_bfloat16*)out_state;
+  CUtensorMap ma, mb;
+  int rc = make_map_i8(&ma, source, n_chains, n_sources, source_pitch, 128u);
+  if (rc == TTHRML_OK) rc = make_map_i8(&mb, weights_nk, n_units, n_sources, w_pitch, 128u);
+  if (rc) return rc;
+  const void* fn = family == TTHRML_SPIN ? (variates ? (const void*)k_int8_pair<kDrawSpins, true>
+                                                     : (const void*)k_int8_pair<kDrawSpins, false>)
+                                         : (variates ? (const void*)k_int8_pair<kDrawGaussians, true>
+                                                     : (const void*)k_int8_pair<kDrawGaussians, false>);
+  return launch_pair(fn, ma, mb, pa, n_sources, (cudaStream_t)stream);
 }

@@ -5,7 +5,9 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <map>
 #include <mutex>
+#include <tuple>
 
 #include "common.cuh"
 
@@ -152,11 +154,56 @@ int encode_fn(EncodeTiledFn* out) {
   return TTHRML_OK;
 }
 
-// Launches fn on a one-dimensional grid of clusters, with its shared-memory limit raised.
-int launch_clusters(const void* fn, unsigned grid, unsigned cluster, unsigned threads, int smem, void** params,
-                    cudaStream_t st, const char* what) {
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return cuda_status(e, what);
+// What a launch of fn in clusters needs to know about the current device, asked once per device and function:
+// the raised shared-memory limit and how many clusters are resident at once.
+struct ClusterFit {
+  int sms, clusters;
+};
+inline int cluster_fit(const void* fn, unsigned cluster, unsigned threads, int smem, ClusterFit* out) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, const void*, unsigned>, ClusterFit> known;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_tuple(dev, fn, cluster);
+  const auto it = known.find(key);
+  if (it != known.end()) {
+    *out = it->second;
+    return TTHRML_OK;
+  }
+  ClusterFit f = {0, 0};
+  e = cudaDeviceGetAttribute(&f.sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e, "kernel attributes");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(cluster, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(&f.clusters, fn, &cfg);
+  if (e != cudaSuccess) return cuda_status(e, "cudaOccupancyMaxActiveClusters");
+  if (f.clusters < 1) {
+    set_error("no cluster of %u blocks fits on this device", cluster);
+    return TTHRML_ERR_UNSUPPORTED;
+  }
+  known.emplace(key, f);
+  *out = f;
+  return TTHRML_OK;
+}
+
+// Launches fn on a one-dimensional grid of clusters.
+inline int launch_clusters(const void* fn, unsigned grid, unsigned cluster, unsigned threads, int smem, void** params,
+                           cudaStream_t st, const char* what) {
+  ClusterFit fit;
+  const int rc = cluster_fit(fn, cluster, threads, smem, &fit);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -169,7 +216,7 @@ int launch_clusters(const void* fn, unsigned grid, unsigned cluster, unsigned th
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelExC(&cfg, fn, params);
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, params);
   if (e != cudaSuccess) return cuda_status(e, what);
   return launch_status(what);
 }

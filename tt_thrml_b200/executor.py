@@ -96,7 +96,9 @@ class Executor:
         # elements per state row: chains, or 32-chain words when bit-packed
         self._row_len = self.n_chains // 32 if self._state_code == nat.STATE_BITS else self.n_chains
         # dense (tensor-core) programs keep one bf16 [n_chains, n_units] tensor per block
-        self._dense = self.compiled.state_dtype == "dense_bf16"
+        # (int8 precision: int8 spins, and gaussians with an 8-bit copy made before each product)
+        self._dense = self.compiled.state_dtype in ("dense_bf16", "dense_int8")
+        self._dense_i8 = self.compiled.state_dtype == "dense_int8"
         self._block_states: list | None = None
         self._error_word = None
         self._ties = None
@@ -134,8 +136,20 @@ class Executor:
                 pieces = {plan.block_indices[0]: plan.out_pieces for plan in self._plans()}
                 self._dense_pieces = [pieces.get(bi, 1) for bi in range(len(self.compiled.blocks))]
                 self._block_states = [
-                    torch.empty((self.n_chains, p * cb.spec.n_nodes), dtype=torch.bfloat16, device=self._tdev)
+                    torch.empty(
+                        (self.n_chains, p * cb.spec.n_nodes),
+                        dtype=torch.int8 if self._dense_i8 and cb.spec.family == Family.SPIN else torch.bfloat16,
+                        device=self._tdev,
+                    )
                     for p, cb in zip(self._dense_pieces, self.compiled.blocks)
+                ]
+                # 8-bit operands of the gaussian blocks: int8 rows and a scale per chain
+                self._block_q = [
+                    (torch.empty(b.shape, dtype=torch.int8, device=self._tdev),
+                     torch.empty(self.n_chains, dtype=torch.float32, device=self._tdev))
+                    if self._dense_i8 and b.dtype != torch.int8
+                    else None
+                    for b in self._block_states
                 ]
                 # float32 copies of the blocks held in several pieces (the readable state)
                 self._block_f32 = [
@@ -148,9 +162,10 @@ class Executor:
                 # near-threshold spin decisions of one dense launch, settled from the exact field
                 # (4 header words, then (chain, unit) pairs; a few in 10^5 decisions are near)
                 sizes = [self.n_chains * plan.n_units for plan in self._plans()
-                         if plan.kind == "dense" and plan.family == Family.SPIN]
+                         if plan.kind == "dense" and plan.family == Family.SPIN and plan.w_scale is None]
                 self._ties_cap = min(2**31 - 1, max([min(n, max(4096, n // 256)) for n in sizes], default=1))
-                self._ties = torch.zeros(4 + 2 * self._ties_cap, dtype=torch.int32, device=self._tdev)
+                if not self._dense_i8:  # 8-bit fields are exact sums
+                    self._ties = torch.zeros(4 + 2 * self._ties_cap, dtype=torch.int32, device=self._tdev)
             return self._block_states
         if self._global_state is None:
             self._global_state = torch.empty(
@@ -185,6 +200,9 @@ class Executor:
         if self._block_f32[block_index] is not None:
             self._block_f32[block_index].copy_(rem)
         dst = self._block_states[block_index]
+        if dst.dtype == torch.int8:  # spins
+            dst.copy_(rem)
+            return
         for p in range(self._dense_pieces[block_index]):
             piece = rem.to(torch.bfloat16)
             dst[:, p * n : (p + 1) * n].copy_(piece)
@@ -510,7 +528,33 @@ class Executor:
             ev0 = torch.cuda.Event(enable_timing=True)
             ev1 = torch.cuda.Event(enable_timing=True)
             ev0.record(self._stream)
-        if plan.kind == "dense":
+        if plan.kind == "dense" and plan.w_scale is not None:
+            bi = plan.block_indices[0]
+            v = self._variates(bi)
+            src, scale = self._block_states[plan.source], None
+            if self._block_q[plan.source] is not None:
+                (q, scale), state = self._block_q[plan.source], src
+                nat.check(
+                    self._lib.tthrml_quantize_rows(
+                        state.data_ptr(), nat.DT_BF16, self.n_chains, plan.n_sources, state.stride(0), 1,
+                        q.data_ptr(), q.stride(0), scale.data_ptr(), stream,
+                    ),
+                    "tthrml_quantize_rows",
+                )
+                src = q
+            nat.check(
+                self._lib.tthrml_int8_field_sample(
+                    src.data_ptr(), src.stride(0), None if scale is None else scale.data_ptr(),
+                    plan.weights_nk.data_ptr(), plan.weights_nk.stride(0), plan.w_scale.data_ptr(), self.n_chains,
+                    plan.n_units, plan.n_sources, plan.bias.data_ptr(),
+                    nat.SPIN if plan.family == Family.SPIN else nat.GAUSSIAN, ctypes.c_float(plan.precision),
+                    self._block_states[bi].data_ptr(), plan.row0, self.chain_offset,
+                    None if v is None else v.data_ptr(), self._rng_n_sweeps if v is not None else 0, seed, sweep_idx,
+                    ctl, self._error_word.data_ptr(), stream,
+                ),
+                "tthrml_int8_field_sample",
+            )
+        elif plan.kind == "dense":
             bi = plan.block_indices[0]
             v = self._variates(bi)
             nat.check(
@@ -979,6 +1023,100 @@ class Executor:
                 ),
                 "tthrml_sum_rows",
             )
+
+    # ----------------------------------------------------- dense programs: learning
+
+    def _dense_plans(self, what: str):
+        plans = sorted(self._plans(), key=lambda p: p.block_indices[0])
+        if not self._dense or [p.block_indices for p in plans] != [(0,), (1,)]:
+            raise NotImplementedError(f"{what} needs a dense program of two blocks (this one runs on {plans[0].kind!r})")
+        return plans
+
+    def update_dense_weights(self, weights, bias_0=None, bias_1=None) -> None:
+        """Replaces the couplings (and biases) of a dense program on the device, without recompiling.
+
+        weights: float32 device tensor [n_0, n_1] coupling unit i of block 0 with
+        unit j of block 1; bias_0, bias_1: float32 [n_0], [n_1] or None (kept).  The
+        sampler's operands are rounded from them: to bfloat16, or to int8 with a
+        scale per unit with dense_precision="int8".  The first call gives this
+        executor operands of its own (the plan cache keeps the program's) and drops
+        captured graphs; later calls write in place, so graphs stay valid.  Ordered
+        after the current stream's work and before what it runs next; the tensors
+        may be changed afterwards."""
+        from .quantized import require_cuda
+
+        torch = _torch()
+        plans = self._dense_plans("update_dense_weights")
+        n0, n1 = plans[0].n_units, plans[1].n_units
+        for name, t, shape in (("weights", weights, (n0, n1)), ("bias_0", bias_0, (n0,)), ("bias_1", bias_1, (n1,))):
+            if t is None and name != "weights":
+                continue
+            require_cuda(name, t, self._tdev)
+            if t.dtype != torch.float32 or tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be float32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
+        current = torch.cuda.current_stream(self._tdev)
+        nat.bind_device(self._tdev.index)
+        self._stream.wait_stream(current)
+        with torch.no_grad(), torch.cuda.stream(self._stream):
+            for plan, w, bias in ((plans[0], weights, bias_0), (plans[1], weights.t(), bias_1)):
+                if not plan.owned:
+                    plan.weights_nk, plan.bias = plan.weights_nk.clone(), plan.bias.clone()
+                    plan.w_scale = None if plan.w_scale is None else plan.w_scale.clone()
+                    plan.owned = True
+                    self._graphs.clear()
+                if plan.w_scale is not None:
+                    nat.check(
+                        self._lib.tthrml_quantize_rows(
+                            w.data_ptr(), nat.DT_F32, w.shape[0], w.shape[1], w.stride(0), w.stride(1),
+                            plan.weights_nk.data_ptr(), plan.weights_nk.stride(0), plan.w_scale.data_ptr(),
+                            nat.stream_handle(self._stream),
+                        ),
+                        "tthrml_quantize_rows",
+                    )
+                else:
+                    n = w.shape[1]
+                    plan.weights_nk[:, :n].copy_(w)
+                    for k in range(1, plan.source_pieces):
+                        plan.weights_nk[:, k * n : (k + 1) * n].copy_(plan.weights_nk[:, :n])
+                if bias is not None:
+                    plan.bias.copy_(bias)
+        current.wait_stream(self._stream)
+
+    def _dense_phases(self, scale: float) -> list:
+        """The current states as terms of pair moments: (x, x pitch, y, y pitch, scale, x scale, y scale), 16-bit
+        tensors.  A value held in several pieces is a sum over them; products of two remainders below the third
+        piece are left out (they are below the float32 rounding)."""
+        torch = _torch()
+        self._dense_plans("dense moments")
+        if not self._state_loaded:
+            raise RuntimeError("State must be loaded before taking moments")
+        parts = []
+        with torch.cuda.stream(self._stream):
+            for bi in (0, 1):
+                state = self._block_states[bi]
+                if state.dtype == torch.int8:
+                    copies = self.__dict__.setdefault("_moment_copies", {})
+                    if bi not in copies:
+                        copies[bi] = torch.empty(state.shape, dtype=torch.bfloat16, device=self._tdev)
+                    state = copies[bi].copy_(state)
+                n, p = self.compiled.blocks[bi].spec.n_nodes, self._dense_pieces[bi]
+                # spins have zero remainders
+                spin = self.compiled.blocks[bi].spec.family == Family.SPIN
+                parts.append([state[:, k * n : (k + 1) * n] for k in range(1 if spin else p)])
+        return [
+            (x, x.stride(0), y, y.stride(0), scale, scale if j == 0 else 0.0, scale if i == 0 else 0.0)
+            for i, x in enumerate(parts[0])
+            for j, y in enumerate(parts[1])
+            if i + j < 3
+        ]
+
+    def dense_moments(self, scale: float = 1.0, *, out=None, accumulate: bool = False):
+        """Moments of a dense program's current states over the chains, in float32: (pair [n_0, n_1], sums of
+        block 0 [n_0], sums of block 1 [n_1]), each times `scale`; spins as +-1.  `out` receives them, or with
+        `accumulate` has them added.  What DeviceMomentObserver gives for listed products, for every pair."""
+        from .learning import dense_moments
+
+        return dense_moments([(self, scale)], out=out, accumulate=accumulate)
 
     # --------------------------------------------------------------- schedule
 
