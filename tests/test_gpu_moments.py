@@ -34,16 +34,16 @@ def exact(xs, ys, scales):
 
 def bound(a, chains):
     """Products of 16-bit values are exact in float32.  One MMA adds 16 of them to the accumulator, each operand aligned
-    to the largest within one float32 step (2^-23) of the sum of magnitudes: 17 steps per MMA, at most 32 MMAs before the
+    to the largest within one float32 step (2^-23) of the sum of magnitudes: 17 steps per MMA, at most 64 MMAs before the
     sum moves to a register; there each of the chunks' additions rounds once, and the splits' ones once more."""
-    mmas = min(32, -(-max(chains) // 16))
-    adds = sum(-(-c // 512) for c in chains) + 16
+    mmas = min(64, -(-max(chains) // 16))
+    adds = sum(-(-c // 1024) for c in chains) + 16
     return a * 2.0**-23 * (17 * mmas + adds)
 
 
 SHAPES = [(1, 1, [1]), (1, 9, [3, 0]), (8, 64, [16, 16]), (65, 63, [17, 64]), (127, 129, [65, 1]), (128, 256, [512]),
           (129, 257, [513, 100]), (200, 1000, [1023, 2050]), (640, 72, [64, 128, 192]), (1000, 513, [4000, 70]),
-          (64, 3, [5, 6, 7, 8, 9, 10]), (2, 300, [9000])]
+          (64, 3, [5, 6, 7, 8, 9, 10]), (2, 300, [9000]), (2100, 2333, [70, 1100]), (2600, 2049, [129])]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -56,9 +56,9 @@ def test_moments_match_the_64_bit_sums(tt, m, n, chains, dtype):
     w, a, wx, wy = exact(xs, ys, scales)
     assert ((out.cpu().double() - w).abs() <= bound(a, chains) + 1e-38).all()
     for got, want, ts in ((sx, wx, xs), (sy, wy, ys)):
-        # 20 lanes of at most ceil(chains / 20) additions, then 20 more, one per phase and its scale
+        # 16 lanes or more, each at most ceil(chains / 16) additions, then 20 at most to join them, one per phase and its scale
         mags = sum(abs(s) * t.double().abs().sum(0) for t, s in zip(ts, scales))
-        adds = sum(-(-c // 20) for c in chains) + 20 + 2 * len(chains)
+        adds = sum(-(-c // 16) for c in chains) + 20 + 2 * len(chains)
         assert ((got.cpu().double() - want).abs() <= mags * adds * 2.0**-24 + 1e-38).all()
     again = tt.pair_moments([x.cuda() for x in xs], [y.cuda() for y in ys], scales)
     assert torch.equal(again, out)  # the same every time
@@ -66,7 +66,7 @@ def test_moments_match_the_64_bit_sums(tt, m, n, chains, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("m,n,chains", [(300, 520, [3000, 700]), (130, 70, [100, 1]), (1, 1, [5000, 5000])])
+@pytest.mark.parametrize("m,n,chains", [(300, 520, [3000, 700]), (130, 70, [100, 1]), (1, 1, [5000, 5000]), (2305, 2049, [300, 1100])])
 def test_whole_numbers_are_exact(tt, m, n, chains, dtype):
     xs = [ints((c, m), 8, i).to(dtype) for i, c in enumerate(chains)]
     ys = [(ints((c, n), 8, 20 + i) * 2 + 1).sign().to(dtype) for i, c in enumerate(chains)]

@@ -5,13 +5,20 @@
 //
 // Both operands lie chain-major (the layout of the sampler's states), so the sum runs over the slow axis of each:
 // the tiles are MN-major in shared memory (64 units x 64 chains per TMA box, 128-byte swizzle) and nothing is
-// transposed.  A cluster of S CTAs computes one 128 x BN tile, each CTA a contiguous share of the 64-chain blocks:
-//   warp 0    TMA loads into a ring of stages (chains and units behind the ends read as zeros);
-//   warp 1    MMAs, kChunk blocks (512 chains) into one of two TMEM accumulators;
-//   warps 2-9 add each finished accumulator, times its phase's scale, to float32 registers (BN / 2 per thread).
-// The tensor core's accumulation drops bits over long sums, so a sum longer than 512 chains is carried in registers with
-// rounded float32 additions.  The S partial tiles are added over distributed shared memory in the order of the ranks, so
-// the result is the same every time.  Blocks behind the tiles sum the units.
+// transposed.  Roles of a CTA's twelve warps:
+//   warp 0      TMA loads into a ring of stages (chains and units behind the ends read as zeros);
+//   warp 1      MMAs, kChunkBlocks blocks of 64 chains into one of two TMEM accumulators;
+//   warps 2-9   add each finished accumulator, times its phase's scale, to float32 registers (half a tile row per thread);
+//   warps 10-11 unit sums, a strip of 32 units at a time, beside the tiles.
+// The tensor core's accumulation drops bits over long sums, so a sum longer than kChunkBlocks blocks is carried in registers
+// with rounded float32 additions.
+//
+// k_pair_moments: for few tiles.  A cluster of S CTAs computes one 128 x BN tile, each CTA a contiguous share of the
+// 64-chain blocks; the S partial tiles are added over distributed shared memory in the order of the ranks, so the result
+// is the same every time.
+// k_pair_moments_2sm: for many.  Persistent clusters of two CTAs walk 256 x 256 tiles (tcgen05 cta_group::2): an SM takes in
+// at most 64 bytes a clock, and a 128 x 256 tile of one CTA needs 96 at the full MMA rate, a CTA of a pair 64.  The
+// accumulating warps store a tile from their registers while the next one's first chunks are multiplied.
 #include <cuda_fp16.h>
 
 #include "tc_common.cuh"
@@ -19,9 +26,9 @@
 namespace tthrml {
 namespace {
 
-constexpr int kMomentThreads = 320;
-constexpr int kChunkBlocks = 8;     // 64-chain blocks per TMEM accumulation
-constexpr int kSumUnits = 32;       // units per block of unit sums
+constexpr int kMomentThreads = 384;
+constexpr int kChunkBlocks = 16;  // 64-chain blocks per TMEM accumulation
+constexpr int kSumUnits = 32;     // units per strip of unit sums
 
 struct MomentMaps {
   CUtensorMap x[TTHRML_MAX_PHASES], y[TTHRML_MAX_PHASES];
@@ -42,7 +49,8 @@ struct MomentArgs {
   float* y_sum;
   int32_t accumulate, vector_store;
   int32_t f16;         // elements are float16 (else bfloat16)
-  int32_t tile_blocks; // CTAs that compute tiles; the others sum units
+  int32_t tile_blocks;  // CTAs that compute tiles; any others sum units
+  int32_t group;        // raster of the pair kernel
   int* error;
 };
 
@@ -52,7 +60,7 @@ struct MomentShape {
   static constexpr int kStage = kABytes + kBBytes;
   static constexpr int kStages = BN == 256 ? 4 : (BN == 128 ? 6 : 8);
   static constexpr int kPitch = BN + 4;
-  static constexpr int kSmem = 1024 + kStages * kStage + 256;
+  static constexpr int kSmem = 1024 + kStages * kStage + 256 /*barriers*/ + 256 /*unit sums*/;
   static_assert(128 * kPitch * 4 <= kStages * kStage, "the staged tile reuses the operand stages");
 };
 
@@ -105,47 +113,87 @@ __device__ __forceinline__ float elem(const void* p, int64_t i, bool f16) {
              : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-// Unit sums of units u0 .. u0 + 31 of x (or y) by one CTA: a thread takes two adjacent units of every 20th chain, then
-// the partial sums are added in the order of the chains' lanes.
-__device__ void unit_sums(const MomentArgs& a, bool of_y, int u0, float* part) {
-  constexpr int kLanes = kMomentThreads / (kSumUnits / 2);  // 20 chain lanes
-  const int u = (threadIdx.x % (kSumUnits / 2)) * 2, lane = threadIdx.x / (kSumUnits / 2);
-  const int units = of_y ? a.N : a.M;
-  float t0 = 0.0f, t1 = 0.0f;
+__device__ __forceinline__ void add8(float (&s)[8], const uint4& w, bool f16) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (f16) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&v[i]);
+      s[2 * i] += __low2float(h);
+      s[2 * i + 1] += __high2float(h);
+    } else {
+      s[2 * i] += __uint_as_float(v[i] << 16);
+      s[2 * i + 1] += __uint_as_float(v[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+// Strip `strip` of the unit sums (32 units of x, then of y) by NT threads (t = 0 .. NT - 1, named barrier `bar`): four
+// threads take the 64 bytes of a chain, NT / 4 chains at a time; the partial sums meet by shuffles and then in the order
+// of the warps.
+template <int NT>
+__device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t, int bar, float* part) {
+  const int xs = a.x_sum ? (a.M + kSumUnits - 1) / kSumUnits : 0;
+  const bool of_y = strip >= xs;
+  const int u0 = (of_y ? strip - xs : strip) * kSumUnits, units = of_y ? a.N : a.M;
+  const int u = u0 + (t & 3) * 8, lane = t >> 2;
+  float total[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total[i] = 0.0f;
   for (int p = 0; p < a.n_phases; ++p) {
-    const void* base = of_y ? a.y[p] : a.x[p];
+    const char* base = reinterpret_cast<const char*>(of_y ? a.y[p] : a.x[p]);
     const int64_t ld = of_y ? a.y_ld[p] : a.x_ld[p];
     const float scale = of_y ? a.y_scale[p] : a.x_scale[p];
     if (scale == 0.0f) continue;
-    float s0 = 0.0f, s1 = 0.0f;
-    if (u0 + u + 2 <= units) {  // rows start on 16 bytes, units on even places: a 4-byte load
-#pragma unroll 8
-      for (int64_t c = lane; c < a.chains[p]; c += kLanes) {
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(base) + (c * ld + u0 + u) / 2);
-        if (a.f16) {
-          const __half2 h = *reinterpret_cast<const __half2*>(&w);
-          s0 += __low2float(h);
-          s1 += __high2float(h);
-        } else {
-          s0 += __uint_as_float(w << 16);
-          s1 += __uint_as_float(w & 0xFFFF0000u);
-        }
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+    if (u + 8 <= units) {  // rows start on 16 bytes and the units on multiples of eight
+      const char* at = base + ((int64_t)lane * ld + u) * 2;
+      const int64_t step = (int64_t)(NT / 4) * ld * 2;
+      int64_t c = lane;
+      for (; c + 7 * (NT / 4) < a.chains[p]; c += 8 * (NT / 4), at += 8 * step) {
+        uint4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(at + i * step));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add8(s, w[i], a.f16 != 0);
       }
-    } else if (u0 + u < units) {
-      for (int64_t c = lane; c < a.chains[p]; c += kLanes) s0 += elem(base, c * ld + u0 + u, a.f16 != 0);
+      for (; c < a.chains[p]; c += NT / 4, at += step) add8(s, __ldg(reinterpret_cast<const uint4*>(at)), a.f16 != 0);
+    } else {
+      for (int64_t c = lane; c < a.chains[p]; c += NT / 4)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (u + i < units) s[i] += elem(base, c * ld + u + i, a.f16 != 0);
     }
-    t0 = fmaf(scale, s0, t0);
-    t1 = fmaf(scale, s1, t1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) total[i] = fmaf(scale, s[i], total[i]);
   }
-  part[lane * kSumUnits + u] = t0;
-  part[lane * kSumUnits + u + 1] = t1;
-  __syncthreads();
-  if (threadIdx.x < kSumUnits && u0 + (int)threadIdx.x < units) {
-    float s = 0.0f;
-    for (int i = 0; i < kLanes; ++i) s += part[i * kSumUnits + threadIdx.x];
-    float* dst = (of_y ? a.y_sum : a.x_sum) + u0 + threadIdx.x;
-    *dst = a.accumulate ? *dst + s : s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) total[i] += __shfl_xor_sync(0xffffffffu, total[i], o);
+  if ((t & 31) < 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[(t >> 5) * kSumUnits + (t & 3) * 8 + i] = total[i];
   }
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(NT) : "memory");
+  if (t < kSumUnits && u0 + t < units) {
+    float v = 0.0f;
+    for (int i = 0; i < NT / 32; ++i) v += part[i * kSumUnits + t];
+    float* dst = (of_y ? a.y_sum : a.x_sum) + u0 + t;
+    *dst = a.accumulate ? *dst + v : v;
+  }
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(NT) : "memory");
+}
+__host__ __device__ inline int sum_strips(const MomentArgs& a) {
+  return (a.x_sum ? (a.M + kSumUnits - 1) / kSumUnits : 0) + (a.y_sum ? (a.N + kSumUnits - 1) / kSumUnits : 0);
+}
+// The unit sums that fall to warps 10 and 11 of a tile's CTA.
+__device__ __forceinline__ void side_sums(const MomentArgs& a, float* part) {
+  if ((int)gridDim.x > a.tile_blocks) return;  // CTAs of their own sum the units
+  const int strips = sum_strips(a);
+  for (int s = blockIdx.x; s < strips; s += gridDim.x) unit_sums<64>(a, s, (int)threadIdx.x - 320, 1, part);
 }
 
 template <int BN>
@@ -155,12 +203,9 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   if ((int)blockIdx.x >= a.tile_blocks) {  // whole clusters: the tile blocks are a multiple of the cluster size
-    const int strip = (int)blockIdx.x - a.tile_blocks, xs = a.x_sum ? (a.M + kSumUnits - 1) / kSumUnits : 0;
-    const int ys = a.y_sum ? (a.N + kSumUnits - 1) / kSumUnits : 0;
-    if (strip < xs)
-      unit_sums(a, false, strip * kSumUnits, reinterpret_cast<float*>(tiles));
-    else if (strip - xs < ys)
-      unit_sums(a, true, (strip - xs) * kSumUnits, reinterpret_cast<float*>(tiles));
+    const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks;
+    for (int s = (int)blockIdx.x - a.tile_blocks; s < strips; s += others)
+      unit_sums<kMomentThreads>(a, s, (int)threadIdx.x, 1, reinterpret_cast<float*>(tiles));
     return;
   }
   uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStage);
@@ -168,6 +213,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   uint64_t* acc_full = empty + S::kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;       // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* side = reinterpret_cast<float*>(tiles + S::kStages * S::kStage + 256);  // [2][32]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
@@ -259,6 +305,8 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
         b += c.length;
       }
     }
+  } else if (warp >= 10) {
+    side_sums(a, side);
   } else {
     // accumulating warps: lane = row within the warp's TMEM quadrant, half of the tile's columns each
     const int quad = warp & 3, half = (warp - 2) >> 2;
@@ -340,6 +388,214 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   if (split > 1) cluster_sync_all();  // no CTA leaves while another still reads its shared memory
 }
 
+// ---------------------------------------------------------------------------
+// CTA-pair kernel
+// ---------------------------------------------------------------------------
+constexpr int kPairStages = 6, kPairHalf = 128 * 64 * 2, kPairStage = 2 * kPairHalf;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 /*barriers*/ + 256 /*unit sums*/;
+
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u),
+      "r"(0u), "r"(0u));
+}
+// Tile t -> (m, n) block: `group` row blocks at a time, row-fastest, so that the tiles in flight form a rectangle and
+// share their operands' panels in L2.
+__device__ __forceinline__ void pair_tile(const MomentArgs& a, int t, int& mb, int& nb) {
+  const int m_blocks = (a.M + 255) / 256, n_blocks = (a.N + 255) / 256;
+  const int per = a.group * n_blocks, g = t / per, w = t - g * per;
+  const int rows = min(a.group, m_blocks - g * a.group);
+  mb = g * a.group + w % rows;
+  nb = w / rows;
+}
+
+__global__ void __launch_bounds__(kMomentThreads, 1)
+    k_pair_moments_2sm(const __grid_constant__ MomentMaps maps, const __grid_constant__ MomentArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + kPairStages * kPairStage);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;        // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* side = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int n_tiles = ((a.M + 255) / 256) * ((a.N + 255) / 256);
+  const int first = (int)cluster_id_x(), step = (int)n_clusters_x();
+  const int total = a.total_blocks;  // > 0
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 16);  // every accumulating warp of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers exist before either signals the other
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  int last_chunk[2] = {-1, -1};
+
+  if (warp == 0) {
+    if (lane == 0) {  // producer (both CTAs): this CTA's halves of the x and y units
+      int64_t issued = 0;
+      bool failed = false;
+      for (int t = first; t < n_tiles && !failed; t += step) {
+        int mb, nb;
+        pair_tile(a, t, mb, nb);
+        const int m0 = mb * 256 + (int)rank * 128, n0 = nb * 256 + (int)rank * 128;
+        for (int b = 0; b < total && !failed;) {
+          const Chunk c = chunk_at(a, b, total);
+          for (int i = 0; i < c.length; ++i, ++issued) {
+            const int s = (int)(issued % kPairStages);
+            if (!mbar_wait(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
+              atomicExch(a.error, kErrEmptyWait);
+              failed = true;
+              break;
+            }
+            if (leader) mbar_expect_tx(&full[s], 2 * kPairStage);  // the stage's bytes of both CTAs
+            unsigned char* st = tiles + s * kPairStage;
+            const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
+            const int chain = (c.block + i) * 64;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              tma_load_2d_pair(st + k * 8192, &maps.x[c.phase], bar, m0 + 64 * k, chain);
+              tma_load_2d_pair(st + kPairHalf + k * 8192, &maps.y[c.phase], bar, n0 + 64 * k, chain);
+            }
+          }
+          b += c.length;
+        }
+      }
+      // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
+      for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
+        if (!mbar_wait(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u)) atomicExch(a.error, kErrEmptyWait);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {  // MMA issue: the leader only
+      const uint32_t idesc = (idesc_moments(256, a.f16 != 0) & 0x00FFFFFFu) | (16u << 24);  // M = 256
+      int64_t used = 0;
+      int chunk = 0;
+      bool failed = false;
+      for (int t = first; t < n_tiles && !failed; t += step) {
+        for (int b = 0; b < total && !failed; ++chunk) {
+          const Chunk c = chunk_at(a, b, total);
+          const int buf = chunk & 1;
+          if (!mbar_wait(&acc_empty[buf], ((uint32_t)(chunk >> 1) & 1u) ^ 1u)) {
+            atomicExch(a.error, kErrAccWait);
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(buf * 256);
+          for (int i = 0; i < c.length; ++i, ++used) {
+            const int s = (int)(used % kPairStages);
+            if (!mbar_wait(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
+              atomicExch(a.error, kErrFullWait);
+              failed = true;
+              break;
+            }
+            tc_fence_after();
+            const unsigned char* st = tiles + s * kPairStage;
+            const uint64_t ad = umma_desc_mn128(st), bd = umma_desc_mn128(st + kPairHalf);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // 16 chains per MMA: two groups of eight, 2048 bytes
+              umma_f16_pair(d, ad + 128ull * kk, bd + 128ull * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+          }
+          umma_commit_pair(&acc_full[buf]);  // both CTAs' accumulator halves complete
+          last_chunk[buf] = chunk;
+          b += c.length;
+        }
+      }
+    }
+  } else if (warp >= 10) {
+    side_sums(a, side);
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    int chunk = 0;
+    bool failed = false;
+    for (int t = first; t < n_tiles && !failed; t += step) {
+      int mb, nb;
+      pair_tile(a, t, mb, nb);
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      for (int b = 0; b < total; ++chunk) {
+        const Chunk c = chunk_at(a, b, total);
+        const int buf = chunk & 1;
+        if (!mbar_wait(&acc_full[buf], (uint32_t)(chunk >> 1) & 1u)) {
+          if (lane == 0) atomicExch(a.error, kErrAccWait);
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        const float scale = a.scale[c.phase];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[32];
+          tmem_load32(tmem + (uint32_t)(buf * 256 + half * 128 + q * 32) + ((uint32_t)(quad * 32) << 16), v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[q * 32 + j] = fmaf(scale, v[j], acc[q * 32 + j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_leader(&acc_empty[buf]);
+        b += c.length;
+      }
+      const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane, n = nb * 256 + half * 128;
+      if (failed || m >= a.M) continue;
+      float* o = a.out + (int64_t)m * a.out_ld + n;
+#pragma unroll
+      for (int j = 0; j < 128; j += 4) {
+        if (a.vector_store && n + j + 4 <= a.N) {
+          float4 s = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+          if (a.accumulate) {
+            const float4 old = *reinterpret_cast<const float4*>(o + j);
+            s = make_float4(old.x + s.x, old.y + s.y, old.z + s.z, old.w + s.w);
+          }
+          *reinterpret_cast<float4*>(o + j) = s;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + j + i < a.N) o[j + i] = a.accumulate ? o[j + i] + acc[j + i] : acc[j + i];
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1 && leader) {
+    // every MMA the pair issued has completed (in both CTAs' TMEM) before TMEM is freed
+    if (lane == 0) {
+      for (int b = 0; b < 2; ++b)
+        if (last_chunk[b] >= 0) (void)mbar_wait(&acc_full[b], (uint32_t)(last_chunk[b] >> 1) & 1u);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA frees TMEM or exits while the other may still signal it
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
 // Tensor map of a chain-major 16-bit matrix [chains][units], read in boxes of 64 chains x 64 units, 128-byte swizzle.
 int make_map_units(CUtensorMap* map, const void* base, int64_t chains, int64_t units, int64_t ld, bool f16) {
   EncodeTiledFn fn;
@@ -361,15 +617,62 @@ int make_map_units(CUtensorMap* map, const void* base, int64_t chains, int64_t u
   return TTHRML_OK;
 }
 
+// Estimated clocks of the tiles on clusters of S CTAs: an SM takes in 64 bytes a clock; a tile costs about 6000 clocks
+// beside its main loop, and S > 1 adds the partial tiles at about 32 bytes a clock.
 template <int BN>
-int launch_moments(const MomentMaps& maps, MomentArgs a, int split, cudaStream_t st) {
+int64_t moment_clocks(int64_t tiles, int64_t blocks, int split, int sms) {
+  const int64_t waves = (tiles * split + sms - 1) / sms;
+  const int64_t loop = (blocks + split - 1) / split * (MomentShape<BN>::kStage / 64);
+  return waves * (loop + 6000 + (split > 1 ? 128 * BN * 4 / 32 : 0));
+}
+template <int BN>
+void consider(const MomentArgs& a, int sms, int64_t& best, int& bn, int& split) {
   const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN);
-  a.tile_blocks = (int32_t)(tiles * split);
-  const int64_t strips = (a.x_sum ? (a.M + kSumUnits - 1) / kSumUnits : 0) + (a.y_sum ? (a.N + kSumUnits - 1) / kSumUnits : 0);
-  const int64_t grid = tiles * split + (strips + split - 1) / split * split;
+  for (int s = 1; s <= 8 && s <= a.total_blocks; s *= 2) {
+    const int64_t c = moment_clocks<BN>(tiles, a.total_blocks, s, sms);
+    if (c < best) best = c, bn = BN, split = s;
+  }
+}
+
+template <int BN>
+int launch_tiles(const MomentMaps& maps, MomentArgs& a, int split, int sms, cudaStream_t st) {
+  const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN) * split;
+  a.tile_blocks = (int32_t)tiles;
+  // CTAs of their own for the unit sums where SMs are left over, else the tiles' CTAs take them along
+  const int64_t strips = sum_strips(a), left = tiles < sms ? (sms - tiles) / split : 0;
+  const int64_t want = (strips + split - 1) / split;
+  const int64_t grid = tiles + (strips > 0 && left > 0 ? (want < left ? want : left) * split : 0);
   void* params[2] = {(void*)&maps, (void*)&a};
   return launch_clusters((const void*)k_pair_moments<BN>, (unsigned)grid, (unsigned)split, kMomentThreads,
                          MomentShape<BN>::kSmem, params, st, "k_pair_moments launch");
+}
+
+int launch_moments(const MomentMaps& maps, MomentArgs& a, cudaStream_t st) {
+  ClusterFit fit;
+  int rc = cluster_fit((const void*)k_pair_moments_2sm, 2, kMomentThreads, kPairSmem, &fit);
+  if (rc) return rc;
+  int64_t best = INT64_MAX;
+  int bn = 128, split = 1;
+  consider<64>(a, fit.sms, best, bn, split);
+  consider<128>(a, fit.sms, best, bn, split);
+  consider<256>(a, fit.sms, best, bn, split);
+  const int64_t mblk = (a.M + 255) / 256, nblk = (a.N + 255) / 256, pairs = mblk * nblk;
+  // the pair kernel overlaps a tile's store with the next tile's loop
+  const int64_t waves = (pairs + fit.clusters - 1) / fit.clusters;
+  const int64_t clocks = waves * a.total_blocks * (kPairStage / 64) + 9000;
+  if (a.total_blocks > 0 && clocks < best) {
+    int64_t g = 1;  // about square rectangles of the tiles in flight
+    while ((g + 1) * (g + 1) <= fit.clusters) ++g;
+    a.group = (int32_t)(g < mblk ? g : mblk);
+    const int64_t clusters = pairs < fit.clusters ? pairs : fit.clusters;
+    a.tile_blocks = (int32_t)(2 * clusters);
+    void* params[2] = {(void*)&maps, (void*)&a};
+    return launch_clusters((const void*)k_pair_moments_2sm, (unsigned)(2 * clusters), 2, kMomentThreads, kPairSmem,
+                           params, st, "k_pair_moments_2sm launch");
+  }
+  if (bn == 64) return launch_tiles<64>(maps, a, split, fit.sms, st);
+  if (bn == 128) return launch_tiles<128>(maps, a, split, fit.sms, st);
+  return launch_tiles<256>(maps, a, split, fit.sms, st);
 }
 
 }  // namespace
@@ -451,7 +754,5 @@ extern "C" int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32
   a.vector_store = (uintptr_t)out % 16 == 0 && out_ld % 4 == 0;
   a.f16 = dtype == TTHRML_DT_F16;
   a.error = error;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (y_units > 128) return launch_moments<256>(maps, a, 1, st);
-  return launch_moments<128>(maps, a, 1, st);
+  return launch_moments(maps, a, (cudaStream_t)stream);
 }
