@@ -549,6 +549,8 @@ int tthrml_moments_accumulate(const void* state_dev, int32_t state_dtype, int64_
 
 /* Columns an int32 accumulator of 8-bit products holds exactly (2^31 / 128^2, less one). */
 #define TTHRML_INT8_MAX_COLS 131071
+/* Padded rows that tthrml_int8_product_few holds in shared memory. */
+#define TTHRML_INT8_FEW_BYTES 163840
 
 /*
  * Rows to 8-bit integers: scale[r] = max|x_r| * fl(1/127), values[r][c] =
@@ -671,6 +673,32 @@ typedef struct tthrml_moment_phase {
   float x_scale, y_scale; /* of the unit sums */
   float reserved;
 } tthrml_moment_phase;
+
+/*
+ * Rows of floats through 8-bit weights: tthrml_int8_product_few for up to 8 rows with dense columns, else
+ * tthrml_quantize_rows into the workspace and tthrml_int8_product.  workspace: 16-byte aligned device memory of at least
+ * tthrml_int8_linear_workspace(rows, cols) bytes (0: none is needed for dense rows; strided rows need the padded rows and
+ * their scales, rows * (cols rounded up to 16) + 4 * rows rounded up to 16), free again once the work on `stream` is done.
+ */
+int tthrml_int8_linear(const void* x_dev, int32_t x_dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                       int64_t col_stride, void* workspace_dev, int64_t workspace_bytes,
+                       const int8_t* weights_dev, int64_t w_pitch, const float* w_scale_dev, int64_t units,
+                       const float* bias_dev, void* out_dev, int32_t out_dtype, int64_t out_ld,
+                       int32_t* error_dev, void* stream);
+int64_t tthrml_int8_linear_workspace(int64_t rows, int64_t cols);
+
+/* A matrix of 16-bit elements to lay out again: element (r, c) at r * row_stride + c * col_stride (elements). */
+#define TTHRML_MAX_PACKED 12
+typedef struct tthrml_pack_matrix {
+  const void* src;
+  void* dst;      /* [rows][pitch], 16-byte aligned */
+  int64_t rows, cols, row_stride, col_stride;
+  int64_t pitch;  /* a multiple of 8 >= cols; columns cols..pitch-1 are written as zeros */
+} tthrml_pack_matrix;
+
+/* Lays out up to TTHRML_MAX_PACKED matrices in one launch (operands of
+ * tthrml_pair_moments whose rows are not 16-byte aligned). */
+int tthrml_pack_rows(const tthrml_pack_matrix* matrices_host, int32_t n, void* stream);
 
 /*
  * out[i][j] (+)= sum_p scale_p sum_c x_p[c][i] y_p[c][j], and, where x_sum /

@@ -21,6 +21,7 @@ KIND_LINEAR, KIND_PRECISION = 0, 1
 STATE_F32, STATE_I8, STATE_BITS = 0, 1, 2
 DT_F32, DT_BF16, DT_F16, DT_I8 = 0, 1, 2, 3
 INT8_MAX_COLS = 131071
+INT8_FEW_BYTES = 163840
 MAX_PHASES = 6
 MAX_CAT_SOURCES = 4
 MAX_CATEGORIES = 64
@@ -85,6 +86,14 @@ class AdamWTensor(ctypes.Structure):
         ("state", c_i64),
         ("param_dtype", c_i32),
         ("grad_dtype", c_i32),
+    ]
+
+
+class PackMatrix(ctypes.Structure):
+    """tthrml_pack_matrix (include/tthrml.h)."""
+
+    _fields_ = [(name, c_vp) for name in ("src", "dst")] + [
+        (name, c_i64) for name in ("rows", "cols", "row_stride", "col_stride", "pitch")
     ]
 
 
@@ -212,6 +221,12 @@ _SIGNATURES = {
         [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_i32, ctypes.c_float, c_vp, c_i64, c_i64,
          c_vp, c_i64, c_u64, c_u32, c_vp, c_vp, c_vp],
     ),
+    "tthrml_int8_linear": (
+        c_i32,
+        [c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp,
+         c_vp],
+    ),
+    "tthrml_int8_linear_workspace": (c_i64, [c_i64, c_i64]),
     "tthrml_int8_product_few": (
         c_i32,
         [c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp],
@@ -222,6 +237,7 @@ _SIGNATURES = {
          ctypes.c_double, c_u64, c_vp],
     ),
     "tthrml_adamw_values": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "tthrml_pack_rows": (c_i32, [c_vp, c_i32, c_vp]),
     "tthrml_pair_moments": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),
@@ -264,6 +280,24 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError(f"{path}: unexpected ABI version {handle.tthrml_abi_version()}")
         _lib = handle
     return _lib
+
+
+_host = None
+
+
+def hostcall():
+    """The host module _hostcall (csrc/hostcall.cpp); raises when it has not been built."""
+    global _host
+    if _host is None:
+        import importlib
+
+        import torch  # noqa: F401  (its libraries must be loaded first)
+
+        try:
+            _host = importlib.import_module("tt_thrml_b200._hostcall")
+        except ImportError as e:
+            raise RuntimeError("tt_thrml_b200/_hostcall.so is missing or stale: run python -m tt_thrml_b200.build") from e
+    return _host
 
 
 def check(rc: int, what: str) -> None:

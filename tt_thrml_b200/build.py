@@ -1,4 +1,4 @@
-"""Builds libtthrml_b200.so in-tree from csrc/*.cu with nvcc for sm_100a.
+"""Builds libtthrml_b200.so in-tree from csrc/*.cu with nvcc for sm_100a, and the host module _hostcall.so.
 
 Run as ``python -m tt_thrml_b200.build``.  Objects go to ``_build/`` at the
 repository root; the shared library lands next to this file so it travels with
@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -18,6 +19,7 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 BUILD_DIR = REPO_DIR / "_build" / "tthrml"
 LIB_PATH = PKG_DIR / "libtthrml_b200.so"
+HOSTCALL_PATH = PKG_DIR / "_hostcall.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -44,6 +46,30 @@ def _headers() -> list[Path]:
     return sorted(CSRC.glob("*.cuh")) + sorted((REPO_DIR / "include").glob("*.h"))
 
 
+def build_hostcall(verbose: bool = False, force: bool = False) -> Path:
+    """The CPython module that reads tensors' addresses (g++ against torch's headers)."""
+    src = CSRC / "hostcall.cpp"
+    newest = max(src.stat().st_mtime, (REPO_DIR / "include" / "tthrml.h").stat().st_mtime)
+    if not force and HOSTCALL_PATH.exists() and HOSTCALL_PATH.stat().st_mtime >= newest:
+        return HOSTCALL_PATH
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = HOSTCALL_PATH.with_suffix(".so.tmp")
+    cmd = [
+        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+        f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp), f"-L{root / 'lib'}",
+        "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+    ]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, HOSTCALL_PATH)
+    return HOSTCALL_PATH
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     nvcc = _nvcc()
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
@@ -60,6 +86,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
     newest_obj = max(o.stat().st_mtime for o in objects)
+    build_hostcall(verbose=verbose, force=force)
     if force or not LIB_PATH.exists() or LIB_PATH.stat().st_mtime < newest_obj:
         tmp = LIB_PATH.with_suffix(".so.tmp")
         cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objects)]

@@ -27,7 +27,7 @@ struct FewArgs {
 };
 
 constexpr int kFewThreads = 256, kFewWarps = 8;
-constexpr int kFewSmemMax = 160 * 1024;
+constexpr int kFewSmemMax = TTHRML_INT8_FEW_BYTES;
 
 __device__ __forceinline__ void store_out(void* out, int32_t dtype, int64_t at, float v) {
   if (dtype == TTHRML_DT_F32)

@@ -40,7 +40,7 @@ struct TileShape {
   static constexpr int kStage = kABytes + kBBytes;
   static constexpr int kStages = BN == 256 ? 4 : (BN == 128 ? 6 : 8);
   static constexpr int kPitch = BN + 4;  // words per row of the staged accumulator: rows start four banks apart
-  static constexpr int kSmem = 1024 + kStages * kStage + 256;
+  static constexpr int kSmem = 1024 + kStages * kStage + 256 /*barriers*/ + 512 /*row scales*/;
   static_assert(128 * kPitch * 4 <= kStages * kStage, "the staged tile reuses the operand stages");
 };
 
@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* empty = full + S::kStages;
   uint64_t* done = empty + S::kStages;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  float* row_scale_of = reinterpret_cast<float*>(tiles + S::kStages * S::kStage + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
@@ -123,6 +124,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // the scales and biases of the four columns that this thread will store, and the rows' scales
+  constexpr int kGroups = BN / 4, kRowStep = kTileThreads / kGroups;
+  const int c0 = ((int)threadIdx.x % kGroups) * 4, n = n0 + c0;
+  float sw[4], bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool live = n + j < a.N;
+    sw[j] = live ? __ldg(a.w_scale + n + j) : 0.0f;
+    bias[j] = live && a.bias ? __ldg(a.bias + n + j) : 0.0f;
+  }
+  if (threadIdx.x < 128) row_scale_of[threadIdx.x] = a.x_scale && m0 + (int)threadIdx.x < a.M ? __ldg(a.x_scale + m0 + threadIdx.x) : 1.0f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -196,34 +208,33 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 
   const int rows = min(128, a.M - m0);
-  const int mine = (rows - rank + split - 1) / split;  // rows rank, rank + split, ...
-  for (int i = threadIdx.x; i < mine * (BN / 4); i += kTileThreads) {
-    const int row = rank + (i / (BN / 4)) * split, c = (i % (BN / 4)) * 4, n = n0 + c;
-    if (n >= a.N) continue;
-    int4 sum;
-    if (split == 1) {
-      sum = *reinterpret_cast<const int4*>(staged + row * S::kPitch + c);
-    } else {
-      const uint32_t at = smem_u32(staged + row * S::kPitch + c);
-      sum = make_int4(0, 0, 0, 0);
-      for (int r = 0; r < split; ++r) {
-        const int4 p = ld_cluster(at, (uint32_t)r);
-        sum.x += p.x;
-        sum.y += p.y;
-        sum.z += p.z;
-        sum.w += p.w;
-      }
-    }
-    const float sx = a.x_scale ? __ldg(a.x_scale + m0 + row) : 1.0f;
-    const int32_t v[4] = {sum.x, sum.y, sum.z, sum.w};
-    float y[4];
+  if (n < a.N) {
+#pragma unroll 4
+    for (int row = rank + (int)threadIdx.x / kGroups * split; row < rows; row += kRowStep * split) {
+      int4 sum;
+      if (split == 1) {
+        sum = *reinterpret_cast<const int4*>(staged + row * S::kPitch + c0);
+      } else {
+        const uint32_t at = smem_u32(staged + row * S::kPitch + c0);
+        int4 p[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int nn = n + j < a.N ? n + j : a.N - 1;
-      y[j] = __fmul_rn((float)v[j], __fmul_rn(sx, __ldg(a.w_scale + nn)));
-      if (a.bias) y[j] = __fadd_rn(y[j], __ldg(a.bias + nn));
+        for (int r = 0; r < 8; ++r)
+          if (r < split) p[r] = ld_cluster(at, (uint32_t)r);
+        sum = p[0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r)
+          if (r < split) sum.x += p[r].x, sum.y += p[r].y, sum.z += p[r].z, sum.w += p[r].w;
+      }
+      const float sx = row_scale_of[row];
+      const int32_t v[4] = {sum.x, sum.y, sum.z, sum.w};
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = __fmul_rn((float)v[j], __fmul_rn(sx, sw[j]));
+        if (a.bias) y[j] = __fadd_rn(y[j], bias[j]);
+      }
+      store4(a, m0 + row, n, y);
     }
-    store4(a, m0 + row, n, y);
   }
   if (split > 1) cluster_sync_all();  // no CTA leaves while another still reads its shared memory
 }
@@ -528,8 +539,52 @@ int make_map_i8(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, 
   return TTHRML_OK;
 }
 
+// Clusters of 1, 2, 4 and 8 CTAs of k_int8_tile<BN> that are resident at once on the current device.
 template <int BN>
-int launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, int split, cudaStream_t st) {
+int resident_tiles(const int** out) {
+  static std::mutex mu;
+  static int known[64][4] = {};
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return cuda_status(e == cudaSuccess ? cudaErrorInvalidDevice : e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < 4 && !known[dev][3]; ++i) {
+    ClusterFit fit;
+    const int rc = cluster_fit((const void*)k_int8_tile<BN>, 1u << i, kTileThreads, TileShape<BN>::kSmem, &fit);
+    if (rc) return rc;
+    known[dev][i] = fit.clusters;
+  }
+  *out = known[dev];
+  return TTHRML_OK;
+}
+
+// Estimated clocks of the tiles on clusters of S CTAs: the main loop by its bytes (loop_clocks), about 6000 clocks beside
+// it, and for S > 1 a barrier and the partial tiles at about 32 bytes a clock.  Measured over (BN, S) at five sizes: the
+// choice is the fastest or within 10 % of it (256 x 8192 x 4096: 15.6 us of 15.6 to 76; 128 x 4096 x 8192: 12.8 of 12.8 to
+// 60; 64 x 5008 x 2048: 8.6 of 8.6 to 24).
+template <int BN>
+int consider(const ProductArgs& a, int64_t& best, int& bn, int& split) {
+  const int* resident;
+  const int rc = resident_tiles<BN>(&resident);
+  if (rc) return rc;
+  const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN);
+  for (int i = 0; i < 4 && (1 << i) <= a.num_k; ++i) {
+    const int s = 1 << i;
+    const int64_t waves = (tiles + resident[i] - 1) / resident[i];
+    const int64_t bytes = (int64_t)((a.num_k + s - 1) / s) * (a.box_m + BN) * 128;
+    const int64_t c = waves * (loop_clocks(bytes, (tiles < resident[i] ? tiles : resident[i]) * s) + 6000 +
+                               (s > 1 ? 1500 + (int64_t)(a.M < 128 ? a.M : 128) * BN / 8 : 0));
+    if (c < best) best = c, bn = BN, split = s;
+  }
+  return TTHRML_OK;
+}
+
+template <int BN>
+int launch_tile(const int8_t* weights, int64_t cols, int64_t w_pitch, const CUtensorMap& ma, const ProductArgs& a,
+                int split, cudaStream_t st) {
+  CUtensorMap mb;
+  const int rc = make_map_i8(&mb, weights, a.N, cols, w_pitch, (uint32_t)BN);
+  if (rc) return rc;
   const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN);
   void* params[3] = {(void*)&ma, (void*)&mb, (void*)&a};
   return launch_clusters((const void*)k_int8_tile<BN>, (unsigned)(tiles * split), (unsigned)split, kTileThreads,
@@ -597,22 +652,31 @@ extern "C" int tthrml_int8_product(const int8_t* x, int64_t x_pitch, const float
   cudaStream_t st = (cudaStream_t)stream;
   CUtensorMap ma, mb;
   int rc;
-  const bool pair = ((rows + 255) / 256) * ((units + 255) / 256) >= 64;
-  if (pair) {
+  const void* pair_fn = (const void*)k_int8_pair<kStoreFields, false>;
+  ClusterFit fit;
+  rc = cluster_fit(pair_fn, 2, kPairThreads, kPairSmem, &fit);
+  if (rc) return rc;
+  int64_t best = INT64_MAX;
+  int bn = 128, split = 1;
+  if ((rc = consider<64>(a, best, bn, split)) || (rc = consider<128>(a, best, bn, split)) ||
+      (rc = consider<256>(a, best, bn, split)))
+    return rc;
+  // the pair kernel overlaps a tile's epilogue with the next tile's loop
+  const int64_t pairs = ((rows + 255) / 256) * ((units + 255) / 256), at_once = pairs < fit.clusters ? pairs : fit.clusters;
+  if ((pairs + fit.clusters - 1) / fit.clusters * loop_clocks((int64_t)a.num_k * kPairStage, 2 * at_once) + 14000 < best) {
     rc = make_map_i8(&ma, x, rows, cols, x_pitch, 128u);
     if (rc == TTHRML_OK) rc = make_map_i8(&mb, weights, units, cols, w_pitch, 128u);
     if (rc) return rc;
     PairArgs pa = {};
     pa.p = a;
     pa.p.vector_store = (uintptr_t)out % 16 == 0 && (out_ld * dtype_bytes(out_dtype)) % 16 == 0;
-    return launch_pair((const void*)k_int8_pair<kStoreFields, false>, ma, mb, pa, cols, st);
+    return launch_pair(pair_fn, ma, mb, pa, cols, st);
   }
   rc = make_map_i8(&ma, x, rows, cols, x_pitch, (uint32_t)a.box_m);
   if (rc) return rc;
-  const int bn = 128;
-  rc = make_map_i8(&mb, weights, units, cols, w_pitch, (uint32_t)bn);
-  if (rc) return rc;
-  return launch_tile<128>(ma, mb, a, 1, st);
+  if (bn == 64) return launch_tile<64>(weights, cols, w_pitch, ma, a, split, st);
+  if (bn == 128) return launch_tile<128>(weights, cols, w_pitch, ma, a, split, st);
+  return launch_tile<256>(weights, cols, w_pitch, ma, a, split, st);
 }
 
 extern "C" int tthrml_int8_field_sample(const int8_t* source, int64_t source_pitch, const float* source_scale,
@@ -674,4 +738,38 @@ extern "C" int tthrml_int8_field_sample(const int8_t* source, int64_t source_pit
                                          : (variates ? (const void*)k_int8_pair<kDrawGaussians, true>
                                                      : (const void*)k_int8_pair<kDrawGaussians, false>);
   return launch_pair(fn, ma, mb, pa, n_sources, (cudaStream_t)stream);
+}
+
+extern "C" int tthrml_int8_linear(const void* x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                                  int64_t col_stride, void* workspace, int64_t workspace_bytes, const int8_t* weights,
+                                  int64_t w_pitch, const float* w_scale, int64_t units, const float* bias, void* out,
+                                  int32_t out_dtype, int64_t out_ld, int32_t* error, void* stream) {
+  using namespace tthrml;
+  if (rows == 0 || units == 0) return TTHRML_OK;
+  if (rows < 0 || cols < 1 || cols > TTHRML_INT8_MAX_COLS) {
+    set_error("tthrml_int8_linear: sizes out of range (rows %lld, columns %lld of at most %d)", (long long)rows,
+              (long long)cols, TTHRML_INT8_MAX_COLS);
+    return TTHRML_ERR_ARG;
+  }
+  if (tthrml_int8_linear_workspace(rows, cols) == 0 && col_stride == 1 && (rows == 1 || row_stride >= cols))
+    return tthrml_int8_product_few(x, x_dtype, row_stride, nullptr, weights, w_pitch, w_scale, rows, units, cols, bias,
+                                   out, out_dtype, out_ld, stream);
+  const int64_t pitch = (cols + 15) / 16 * 16, need = rows * pitch + (rows * 4 + 15) / 16 * 16;
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need) {
+    set_error("tthrml_int8_linear: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+              (long long)workspace_bytes);
+    return TTHRML_ERR_ARG;
+  }
+  int8_t* q = (int8_t*)workspace;
+  float* scale = (float*)(q + rows * pitch);
+  const int rc = tthrml_quantize_rows(x, x_dtype, rows, cols, row_stride, col_stride, q, pitch, scale, stream);
+  if (rc) return rc;
+  return tthrml_int8_product(q, pitch, scale, weights, w_pitch, w_scale, rows, units, cols, bias, out, out_dtype, out_ld,
+                             error, stream);
+}
+
+extern "C" int64_t tthrml_int8_linear_workspace(int64_t rows, int64_t cols) {
+  const int64_t pitch = (cols + 15) / 16 * 16, wide = rows <= 1 ? 1 : (rows == 2 ? 2 : (rows <= 4 ? 4 : 8));
+  if (rows <= 8 && wide * pitch <= TTHRML_INT8_FEW_BYTES) return 0;
+  return rows * pitch + (rows * 4 + 15) / 16 * 16;
 }

@@ -151,15 +151,14 @@ __device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t,
     if (u + 8 <= units) {  // rows start on 16 bytes and the units on multiples of eight
       const char* at = base + ((int64_t)lane * ld + u) * 2;
       const int64_t step = (int64_t)(NT / 4) * ld * 2;
-      int64_t c = lane;
-      for (; c + 7 * (NT / 4) < a.chains[p]; c += 8 * (NT / 4), at += 8 * step) {
-        uint4 w[8];
+      for (int64_t c = lane; c < a.chains[p]; c += 16 * (NT / 4), at += 16 * step) {  // 16 loads on their way at a time
+        uint4 w[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(at + i * step));
+        for (int i = 0; i < 16; ++i)
+          w[i] = c + i * (NT / 4) < a.chains[p] ? __ldg(reinterpret_cast<const uint4*>(at + i * step)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) add8(s, w[i], a.f16 != 0);
+        for (int i = 0; i < 16; ++i) add8(s, w[i], a.f16 != 0);
       }
-      for (; c < a.chains[p]; c += NT / 4, at += step) add8(s, __ldg(reinterpret_cast<const uint4*>(at)), a.f16 != 0);
     } else {
       for (int64_t c = lane; c < a.chains[p]; c += NT / 4)
 #pragma unroll
@@ -392,7 +391,8 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
 // CTA-pair kernel
 // ---------------------------------------------------------------------------
 constexpr int kPairStages = 6, kPairHalf = 128 * 64 * 2, kPairStage = 2 * kPairHalf;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 /*barriers*/ + 256 /*unit sums*/;
+constexpr int kTurnPitch = 33;  // floats per row of a warp's 32 x 32 transpose (outputs whose rows are not aligned)
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 /*barriers*/ + 256 /*unit sums*/ + 8 * 32 * kTurnPitch * 4;
 
 __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -423,12 +423,18 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   uint64_t* acc_empty = acc_full + 2;        // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
   float* side = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);
+  if ((int)blockIdx.x >= a.tile_blocks) {  // whole clusters
+    const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks;
+    for (int s = (int)blockIdx.x - a.tile_blocks; s < strips; s += others)
+      unit_sums<kMomentThreads>(a, s, (int)threadIdx.x, 1, reinterpret_cast<float*>(tiles));
+    return;
+  }
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int n_tiles = ((a.M + 255) / 256) * ((a.N + 255) / 256);
-  const int first = (int)cluster_id_x(), step = (int)n_clusters_x();
+  const int first = (int)cluster_id_x(), step = a.tile_blocks / 2;
   const int total = a.total_blocks;  // > 0
 
   if (threadIdx.x == 0) {
@@ -529,6 +535,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
     side_sums(a, side);
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
+    float* turn = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 512) + (warp - 2) * 32 * kTurnPitch;
     int chunk = 0;
     bool failed = false;
     for (int t = first; t < n_tiles && !failed; t += step) {
@@ -559,22 +566,40 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
         if (lane == 0) mbar_arrive_leader(&acc_empty[buf]);
         b += c.length;
       }
+      if (failed) break;
       const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane, n = nb * 256 + half * 128;
-      if (failed || m >= a.M) continue;
       float* o = a.out + (int64_t)m * a.out_ld + n;
 #pragma unroll
-      for (int j = 0; j < 128; j += 4) {
-        if (a.vector_store && n + j + 4 <= a.N) {
-          float4 s = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-          if (a.accumulate) {
-            const float4 old = *reinterpret_cast<const float4*>(o + j);
-            s = make_float4(old.x + s.x, old.y + s.y, old.z + s.z, old.w + s.w);
-          }
-          *reinterpret_cast<float4*>(o + j) = s;
-        } else {
+      for (int q = 0; q < 4; ++q) {
+        const int nq = n + q * 32;
+        if (a.vector_store && nq + 32 <= a.N) {  // each lane its own row, 128 bytes of it
+          if (m < a.M) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + j + i < a.N) o[j + i] = a.accumulate ? o[j + i] + acc[j + i] : acc[j + i];
+            for (int j = 0; j < 32; j += 4) {
+              float4 s = make_float4(acc[q * 32 + j], acc[q * 32 + j + 1], acc[q * 32 + j + 2], acc[q * 32 + j + 3]);
+              float4* at = reinterpret_cast<float4*>(o + q * 32 + j);
+              if (a.accumulate) {
+                const float4 old = *at;
+                s = make_float4(old.x + s.x, old.y + s.y, old.z + s.z, old.w + s.w);
+              }
+              *at = s;
+            }
+          }
+        } else {  // by way of shared memory, so that a warp stores consecutive columns
+#pragma unroll
+          for (int j = 0; j < 32; ++j) turn[lane * kTurnPitch + j] = acc[q * 32 + j];
+          __syncwarp();
+          if (nq + lane < a.N) {
+            float* row = a.out + (int64_t)(m - lane) * a.out_ld + nq + lane;
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+              if (m - lane + r < a.M) {
+                const float v = turn[r * kTurnPitch + lane];
+                row[r * a.out_ld] = a.accumulate ? row[r * a.out_ld] + v : v;
+              }
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -617,21 +642,44 @@ int make_map_units(CUtensorMap* map, const void* base, int64_t chains, int64_t u
   return TTHRML_OK;
 }
 
-// Estimated clocks of the tiles on clusters of S CTAs: an SM takes in 64 bytes a clock; a tile costs about 6000 clocks
-// beside its main loop, and S > 1 adds the partial tiles at about 32 bytes a clock.
+// Clusters of 1, 2, 4 and 8 CTAs of k_pair_moments<BN> that are resident at once on the current device.
 template <int BN>
-int64_t moment_clocks(int64_t tiles, int64_t blocks, int split, int sms) {
-  const int64_t waves = (tiles * split + sms - 1) / sms;
-  const int64_t loop = (blocks + split - 1) / split * (MomentShape<BN>::kStage / 64);
-  return waves * (loop + 6000 + (split > 1 ? 128 * BN * 4 / 32 : 0));
+int resident_tiles(const int** out) {
+  static std::mutex mu;
+  static int known[64][4] = {};
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return cuda_status(e == cudaSuccess ? cudaErrorInvalidDevice : e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < 4 && !known[dev][3]; ++i) {
+    ClusterFit fit;
+    const int rc = cluster_fit((const void*)k_pair_moments<BN>, 1u << i, kMomentThreads, MomentShape<BN>::kSmem, &fit);
+    if (rc) return rc;
+    known[dev][i] = fit.clusters;
+  }
+  *out = known[dev];
+  return TTHRML_OK;
 }
+
+// Estimated clocks of the tiles on clusters of S CTAs: the main loop by its bytes (loop_clocks), about 6000 clocks beside
+// it, and for S > 1 a barrier and the partial tiles at about 32 bytes a clock.  Measured over (BN, S) at five sizes: the
+// choice is the fastest or within 10 % of it (777 x 1999 x 1523 chains: 15.2 us of 15.2 to 92; 512 x 1024 x 9216: 19.7
+// of 19.7 to 60; 256 x 512 x 192: 5.2 of 5.2 to 10).
 template <int BN>
-void consider(const MomentArgs& a, int sms, int64_t& best, int& bn, int& split) {
+int consider(const MomentArgs& a, int64_t& best, int& bn, int& split) {
+  const int* resident;
+  const int rc = resident_tiles<BN>(&resident);
+  if (rc) return rc;
   const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN);
-  for (int s = 1; s <= 8 && s <= a.total_blocks; s *= 2) {
-    const int64_t c = moment_clocks<BN>(tiles, a.total_blocks, s, sms);
+  for (int i = 0; i < 4 && (i == 0 || (1 << i) <= a.total_blocks); ++i) {
+    const int s = 1 << i;
+    const int64_t waves = (tiles + resident[i] - 1) / resident[i];
+    const int64_t bytes = (int64_t)((a.total_blocks + s - 1) / s) * MomentShape<BN>::kStage;
+    const int64_t c = waves * (loop_clocks(bytes, (tiles < resident[i] ? tiles : resident[i]) * s) + 6000 +
+                               (s > 1 ? 1500 + 128 * BN / 8 : 0));
     if (c < best) best = c, bn = BN, split = s;
   }
+  return TTHRML_OK;
 }
 
 template <int BN>
@@ -653,26 +701,65 @@ int launch_moments(const MomentMaps& maps, MomentArgs& a, cudaStream_t st) {
   if (rc) return rc;
   int64_t best = INT64_MAX;
   int bn = 128, split = 1;
-  consider<64>(a, fit.sms, best, bn, split);
-  consider<128>(a, fit.sms, best, bn, split);
-  consider<256>(a, fit.sms, best, bn, split);
+  if ((rc = consider<64>(a, best, bn, split)) || (rc = consider<128>(a, best, bn, split)) ||
+      (rc = consider<256>(a, best, bn, split)))
+    return rc;
   const int64_t mblk = (a.M + 255) / 256, nblk = (a.N + 255) / 256, pairs = mblk * nblk;
   // the pair kernel overlaps a tile's store with the next tile's loop
   const int64_t waves = (pairs + fit.clusters - 1) / fit.clusters;
-  const int64_t clocks = waves * a.total_blocks * (kPairStage / 64) + 9000;
+  const int64_t clocks = waves * loop_clocks((int64_t)a.total_blocks * kPairStage, 2 * (pairs < fit.clusters ? pairs : fit.clusters)) + 20000;
   if (a.total_blocks > 0 && clocks < best) {
     int64_t g = 1;  // about square rectangles of the tiles in flight
     while ((g + 1) * (g + 1) <= fit.clusters) ++g;
     a.group = (int32_t)(g < mblk ? g : mblk);
     const int64_t clusters = pairs < fit.clusters ? pairs : fit.clusters;
     a.tile_blocks = (int32_t)(2 * clusters);
+    // clusters of their own for the unit sums where SMs are left over, else warps of the tiles' CTAs take them along
+    const int64_t want = (sum_strips(a) + 1) / 2, left = fit.clusters - clusters;
+    const int64_t others = want < left ? want : left;
     void* params[2] = {(void*)&maps, (void*)&a};
-    return launch_clusters((const void*)k_pair_moments_2sm, (unsigned)(2 * clusters), 2, kMomentThreads, kPairSmem,
+    return launch_clusters((const void*)k_pair_moments_2sm, (unsigned)(2 * (clusters + others)), 2, kMomentThreads, kPairSmem,
                            params, st, "k_pair_moments_2sm launch");
   }
   if (bn == 64) return launch_tiles<64>(maps, a, split, fit.sms, st);
   if (bn == 128) return launch_tiles<128>(maps, a, split, fit.sms, st);
   return launch_tiles<256>(maps, a, split, fit.sms, st);
+}
+
+// Rows of 16-bit elements from any strides to rows that start on 16 bytes, several matrices in one launch
+// (blockIdx.y): eight elements per thread, columns behind the end as zeros.  Adjacent elements are read as aligned words.
+struct PackArgs {
+  tthrml_pack_matrix m[TTHRML_MAX_PACKED];
+};
+__global__ void __launch_bounds__(256) k_pack_rows(const __grid_constant__ PackArgs a) {
+  const tthrml_pack_matrix& m = a.m[blockIdx.y];
+  const uint32_t per_row = (uint32_t)(m.pitch / 8);
+  const uint32_t rows_at_once = per_row >= 256u ? 1u : 256u / per_row;  // rows that a block takes side by side
+  const uint32_t t_row = threadIdx.x / per_row, t_vec = threadIdx.x - t_row * per_row;
+  if (per_row < 256u && t_row >= rows_at_once) return;
+  for (int64_t row = (int64_t)blockIdx.x * rows_at_once + (per_row < 256u ? t_row : 0u); row < m.rows;
+       row += (int64_t)gridDim.x * rows_at_once) {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(m.src) + row * m.row_stride;
+    for (uint32_t v = per_row < 256u ? t_vec : threadIdx.x; v < per_row; v += 256u) {
+      const int64_t c = (int64_t)v * 8;
+      uint4 out;
+      if (m.col_stride == 1 && c + 8 <= m.cols) {
+        // the words that hold the eight elements; a fifth one where the first element is the upper half of a word
+        const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)(src + c) & ~(uintptr_t)3);
+        const bool odd = ((uintptr_t)(src + c) & 2) != 0;
+        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = odd ? w[4] : 0u;
+        out = odd ? make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
+                               __funnelshift_r(w3, w4, 16))
+                  : make_uint4(w0, w1, w2, w3);
+      } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = c + j < m.cols ? src[(c + j) * m.col_stride] : 0u;
+        out = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+      }
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(m.dst) + row * m.pitch + c) = out;
+    }
+  }
 }
 
 }  // namespace
@@ -755,4 +842,31 @@ extern "C" int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32
   a.f16 = dtype == TTHRML_DT_F16;
   a.error = error;
   return launch_moments(maps, a, (cudaStream_t)stream);
+}
+
+extern "C" int tthrml_pack_rows(const tthrml_pack_matrix* matrices_host, int32_t n, void* stream) {
+  using namespace tthrml;
+  if (n == 0) return TTHRML_OK;
+  if (!matrices_host || n < 0 || n > TTHRML_MAX_PACKED) {
+    set_error("tthrml_pack_rows: 0 to %d matrices are supported (got %d)", TTHRML_MAX_PACKED, (int)n);
+    return TTHRML_ERR_ARG;
+  }
+  PackArgs a = {};
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    const tthrml_pack_matrix& m = matrices_host[i];
+    if (m.rows < 0 || m.cols < 1 || m.pitch < m.cols || m.pitch % 8 || m.pitch > 0x7fffffffLL || m.row_stride < 0 ||
+        m.col_stride < 0 || (m.rows > 0 && (!m.src || !m.dst || (uintptr_t)m.src % 2 || (uintptr_t)m.dst % 16))) {
+      set_error("tthrml_pack_rows: matrix %d: %lld x %lld, pitch %lld (a multiple of 8), targets 16-byte aligned", i,
+                (long long)m.rows, (long long)m.cols, (long long)m.pitch);
+      return TTHRML_ERR_ARG;
+    }
+    a.m[i] = m;
+    const int64_t at_once = m.pitch / 8 >= 256 ? 1 : 256 / (m.pitch / 8), blocks = (m.rows + at_once - 1) / at_once;
+    most = blocks > most ? blocks : most;
+  }
+  if (most == 0) return TTHRML_OK;
+  const int64_t limit = 148 * 8;
+  k_pack_rows<<<dim3((unsigned)(most < limit ? most : limit), (unsigned)n), 256, 0, (cudaStream_t)stream>>>(a);
+  return launch_status("k_pack_rows launch");
 }

@@ -58,7 +58,7 @@ def dense_moments(terms, *, out=None, accumulate: bool = False):
         for p, (x, x_ld, y, y_ld, s, sx, sy) in zip(phases, part):
             p.x, p.y, p.x_ld, p.y_ld, p.chains = x.data_ptr(), y.data_ptr(), x_ld, y_ld, x.shape[0]
             p.scale, p.x_scale, p.y_scale = s, sx, sy
-        launch(phases, nat.DT_BF16, M, N, out[0], out[1], out[2], accumulate or at > 0, dev, current)
+        launch(phases, nat.DT_BF16, M, N, out[0], out[1], out[2], accumulate or at > 0, dev, current.cuda_stream)
     for ex, _ in terms:
         ex.stream.wait_stream(current)
     return out

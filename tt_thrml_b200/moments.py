@@ -11,7 +11,7 @@ two dense blocks at once, on the tensor cores.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import dtype_code, error_word, on_device, require_cuda
+from .quantized import dtype_code, error_word, on_device, raw_stream, require_cuda
 
 
 def _torch():
@@ -20,16 +20,32 @@ def _torch():
     return torch
 
 
-def _operand(t, units):
-    """(tensor, pitch) of a chain-major operand laid out for the kernel: rows of 16-byte aligned elements."""
+def _lay_out(tensors, dev, stream):
+    """[(address, pitch)] of chain-major operands as the kernel reads them, rows 16-byte aligned; the others are
+    copied into one buffer by one launch, which is returned too (it must live until the kernel is queued)."""
     torch = _torch()
-    ld = t.stride(0) if t.shape[0] > 1 else -(-units // 8) * 8
-    if (t.stride(1) == 1 or units == 1) and ld % 8 == 0 and ld >= units and t.data_ptr() % 16 == 0:
-        return t, ld
-    ld = -(-units // 8) * 8
-    laid = torch.empty((t.shape[0], ld), dtype=t.dtype, device=t.device)[:, :units]
-    laid.copy_(t)
-    return laid, ld
+    found, again, size = [], [], 0
+    for i, t in enumerate(tensors):
+        rows, units = t.shape
+        ld = t.stride(0) if rows > 1 else -(-units // 8) * 8
+        if (units == 1 or t.stride(1) == 1) and ld % 8 == 0 and ld >= units and t.data_ptr() % 16 == 0:
+            found.append((t.data_ptr(), ld))
+            continue
+        pitch = -(-units // 8) * 8
+        again.append((i, t, pitch, size))
+        found.append(None)
+        size += rows * pitch
+    if not again:
+        return found, None
+    buffer = torch.empty(max(size, 8), dtype=tensors[0].dtype, device=dev)
+    rows = (nat.PackMatrix * len(again))()
+    for row, (i, t, pitch, at) in zip(rows, again):
+        row.src, row.dst, row.pitch = t.data_ptr(), buffer.data_ptr() + 2 * at, pitch
+        row.rows, row.cols = t.shape
+        row.row_stride, row.col_stride = t.stride()
+        found[i] = (row.dst, pitch)
+    nat.check(nat.lib().tthrml_pack_rows(rows, len(again), stream), "tthrml_pack_rows")
+    return found, buffer
 
 
 def _sum_target(name, t, n, dev):
@@ -61,18 +77,22 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
     code = dtype_code(dtype)
     if code not in (nat.DT_BF16, nat.DT_F16):
         raise ValueError(f"x and y must be bfloat16 or float16, got {dtype}")
+    grad = torch.is_grad_enabled()
     shapes = []
     for p, (a, b) in enumerate(zip(xs, ys)):
-        for name, t in ((f"x[{p}]", a), (f"y[{p}]", b)):
+        for name, t in (("x", a), ("y", b)):
             require_cuda(name, t, dev)
             if t.dtype != dtype or t.dim() != 2:
-                raise ValueError(f"{name} must be a {dtype} matrix, got {t.dtype} of shape {tuple(t.shape)}")
-            if torch.is_grad_enabled() and t.requires_grad:
-                raise RuntimeError(f"{name} requires a gradient, but pair moments have no backward pass (use torch.no_grad())")
-        if a.shape[0] != b.shape[0]:
-            raise ValueError(f"phase {p}: x has {a.shape[0]} chains, y has {b.shape[0]}")
-        shapes.append((a.shape[1], b.shape[1]))
-    if any(s != shapes[0] for s in shapes):
+                raise ValueError(f"{name}[{p}] must be a {dtype} matrix, got {t.dtype} of shape {tuple(t.shape)}")
+            if grad and t.requires_grad:
+                raise RuntimeError(
+                    f"{name}[{p}] requires a gradient, but pair moments have no backward pass (use torch.no_grad())"
+                )
+        (chains, m), (other, n) = a.shape, b.shape
+        if chains != other:
+            raise ValueError(f"phase {p}: x has {chains} chains, y has {other}")
+        shapes.append((m, n))
+    if shapes.count(shapes[0]) != len(shapes):
         raise ValueError(f"every phase needs the same units, got {shapes}")
     M, N = shapes[0]
     if M < 1 or N < 1:
@@ -96,25 +116,25 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
             raise ValueError("out needs dense rows that do not overlap")
     phases = (nat.MomentPhase * len(xs))()
     with on_device(dev):
-        held = []
-        for row, a, b, s in zip(phases, xs, ys, scales):
-            (a, x_ld), (b, y_ld) = _operand(a, M), _operand(b, N)
-            held.append((a, b))
-            row.x, row.y, row.x_ld, row.y_ld, row.chains = a.data_ptr(), b.data_ptr(), x_ld, y_ld, a.shape[0]
+        stream = raw_stream(dev.index)
+        laid, held = _lay_out(xs + ys, dev, stream)
+        for p, (row, s) in enumerate(zip(phases, scales)):
+            row.x, row.x_ld = laid[p]
+            row.y, row.y_ld = laid[len(xs) + p]
+            row.chains = xs[p].shape[0]
             row.scale = row.x_scale = row.y_scale = s
-        launch(phases, code, M, N, out, x_sum, y_sum, accumulate, dev)
+        launch(phases, code, M, N, out, x_sum, y_sum, accumulate, dev, stream)
+    del held
     return (out, x_sum, y_sum) if units else out
 
 
-def launch(phases, code, M, N, out, x_sum, y_sum, accumulate, dev, stream=None) -> None:
-    """tthrml_pair_moments on `stream` (default: the current stream of `dev`)."""
-    torch = _torch()
-    stream = torch.cuda.current_stream(dev) if stream is None else stream
+def launch(phases, code, M, N, out, x_sum, y_sum, accumulate, dev, stream) -> None:
+    """tthrml_pair_moments on a cudaStream_t of `dev`."""
     nat.check(
         nat.lib().tthrml_pair_moments(
             phases, len(phases), code, M, N, out.data_ptr(), out.stride(0) if M > 1 else N,
             None if x_sum is None else x_sum.data_ptr(), None if y_sum is None else y_sum.data_ptr(),
-            1 if accumulate else 0, error_word(dev).data_ptr(), stream.cuda_stream,
+            1 if accumulate else 0, error_word(dev).data_ptr(), stream,
         ),
         "tthrml_pair_moments",
     )

@@ -16,13 +16,10 @@ graphs.  Nothing synchronises.
 
 from __future__ import annotations
 
-import weakref
-from operator import call, is_
-
 import numpy as np
 
 from . import _native as nat
-from .quantized import dtype_code, on_device, require_cuda
+from .quantized import dtype_code, on_device, raw_stream, require_cuda
 
 BLOCK = 256  # elements per scale of 8-bit moments; segments of the moments are padded to it
 
@@ -97,16 +94,16 @@ class AdamW:
         self._ctl = torch.zeros(3, dtype=torch.int64, device=dev)  # tthrml_adamw_ctl: step, lr (float64), ticket
         self._lr = None
         self.lr = lr
-        self._orders = [_dense_order(p) for p in self.params]
         self._kinds = [(p.dtype, p.device, p.shape, p.stride()) for p in self.params]
-        self._live = np.array([i for i, p in enumerate(self.params) if p.numel()], dtype=np.int64)
         # tthrml_adamw_tensor rows of the parameters that have elements
+        self._live = [i for i, p in enumerate(self.params) if p.numel()]
         self._rows = np.zeros(len(self._live), dtype=np.dtype(nat.AdamWTensor))
-        self._rows["n"] = [self.params[i].numel() for i in self._live]
-        self._rows["state"] = [self.offsets[i] for i in self._live]
-        self._rows["param_dtype"] = [dtype_code(self.params[i].dtype) for i in self._live]
-        self._nothing = [None] * len(self.params)
-        self._param_ptrs = self._grad_ptrs = self._grads = None
+        for name, values in (("n", [p.numel() for p in self.params]), ("state", self.offsets),
+                             ("param", [p.data_ptr() for p in self.params]),
+                             ("param_dtype", [dtype_code(p.dtype) for p in self.params])):
+            self._rows[name] = [values[i] for i in self._live]
+        self._rows_at, self._n_rows = self._rows.ctypes.data, len(self._rows)
+        self._host, self._lib = nat.hostcall(), nat.lib()
         self._state_ptrs = tuple(None if t is None else t.data_ptr() for t in
                                  (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self._ctl))
 
@@ -136,58 +133,44 @@ class AdamW:
     # ------------------------------------------------------------------- step
 
     def _check(self, grads) -> None:
-        """Raises unless every gradient has its parameter's device, shape and memory order and a fitting type."""
+        """Fills the rows tensor by tensor; raises unless every gradient has its parameter's device, shape and memory
+        order and a fitting type."""
         torch = _torch()
-        for i, (p, g, order) in enumerate(zip(self.params, grads, self._orders)):
-            if type(g) is torch.Tensor and (g.dtype, g.device, g.shape, g.stride()) == self._kinds[i]:
-                continue  # the parameter's own type and layout
+        for i, (p, g, kind) in enumerate(zip(self.params, grads, self._kinds)):
+            if g is None:
+                raise ValueError(f"parameter {i} has no gradient")
             require_cuda(f"gradient {i}", g, self.device)
+            if (p.dtype, p.device, p.shape, p.stride()) != kind:
+                raise ValueError(f"parameter {i} changed its type or layout since the optimizer was made")
             if g.dtype not in (p.dtype, torch.float32):
                 raise ValueError(f"gradient {i} must be {p.dtype} or float32, got {g.dtype}")
-            if g.shape != p.shape or _dense_order(g) != order:
+            if g.shape != p.shape or _dense_order(g) != _dense_order(p):
                 raise ValueError(
                     f"gradient {i} needs the parameter's shape and memory order: shape {tuple(g.shape)}, strides "
                     f"{tuple(g.stride())} for {tuple(p.shape)}, {tuple(p.stride())}"
                 )
-
-    def _check_params(self, ptrs) -> None:
-        for i, (p, kind) in enumerate(zip(self.params, self._kinds)):
-            if (p.dtype, p.device, p.shape, p.stride()) != kind:
-                raise ValueError(f"parameter {i} changed its type or layout since the optimizer was made")
-        column = np.array(ptrs, dtype=np.uint64)
-        self._rows["param"] = column[self._live]
+        for row, i in zip(self._rows, self._live):
+            row["param"], row["grad"] = self.params[i].data_ptr(), grads[i].data_ptr()
+            row["grad_dtype"] = dtype_code(grads[i].dtype)
 
     def step(self, grads=None) -> None:
         """One step of all parameters, queued on the current stream of their device."""
-        torch = _torch()
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} parameters, {len(grads)} gradients")
-        if any(map(is_, grads, self._nothing)):
-            raise ValueError(f"parameter {next(i for i, g in enumerate(grads) if g is None)} has no gradient")
-        address = torch.Tensor.data_ptr
-        param_ptrs = list(map(address, self.params))
-        if param_ptrs != self._param_ptrs:
-            self._check_params(param_ptrs)
-            self._param_ptrs = param_ptrs
-        same = self._grads is not None and all(map(is_, grads, map(call, self._grads)))
-        if not same or list(map(address, grads)) != self._grad_ptrs:
-            self._grads = None
+        index = self.device.index
+        if self._host.adamw_rows(self.params, grads, self._rows_at, self._n_rows, index) >= 0:
             self._check(grads)
-            self._grad_ptrs = list(map(address, grads))
-            self._rows["grad"] = np.array(self._grad_ptrs, dtype=np.uint64)[self._live]
-            self._rows["grad_dtype"] = np.array([dtype_code(g.dtype) for g in grads], dtype=np.int32)[self._live]
-            self._grads = list(map(weakref.ref, grads))
         m, v, ms, vs, ctl = self._state_ptrs
         with on_device(self.device):
             nat.check(
-                nat.lib().tthrml_adamw_step(
-                    self._rows.ctypes.data, len(self._rows), self.state_bits, m, v, ms, vs, ctl, self.betas[0], self.betas[1],
-                    self.eps, self.weight_decay, self.seed, torch.cuda.current_stream(self.device).cuda_stream,
+                self._lib.tthrml_adamw_step(
+                    self._rows_at, self._n_rows, self.state_bits, m, v, ms, vs, ctl, self.betas[0], self.betas[1],
+                    self.eps, self.weight_decay, self.seed, raw_stream(index),
                 ),
                 "tthrml_adamw_step",
             )
-        torch.autograd.graph.increment_version(self.params)
+        self._host.bump_versions(self.params)
 
     # ------------------------------------------------------------------ state
 
@@ -202,7 +185,7 @@ class AdamW:
                 nat.check(
                     nat.lib().tthrml_adamw_values(
                         *self._state_ptrs[:4], m.numel(), m.data_ptr(), v.data_ptr(),
-                        torch.cuda.current_stream(self.device).cuda_stream,
+                        raw_stream(self.device.index),
                     ),
                     "tthrml_adamw_values",
                 )

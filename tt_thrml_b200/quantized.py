@@ -38,6 +38,12 @@ def dtype_code(dtype):
     return _codes.get(dtype)
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of a device as a cudaStream_t."""
+    torch = _torch()
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 _error_words: dict = {}
 
 
@@ -86,12 +92,13 @@ def on_device(device):
 
 def require_cuda(name: str, t, device=None):
     torch = _torch()
+    if isinstance(t, torch.Tensor) and t.is_cuda and (device is None or t.device == device):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device (there is no CPU path), got {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def _no_grad(name: str, t):
@@ -172,15 +179,11 @@ def quantize_rows(x) -> QuantizedRows:
             nat.check(
                 nat.lib().tthrml_quantize_rows(
                     x.data_ptr(), code, rows, cols, x.stride(0), x.stride(1) if cols > 1 else 1, values.data_ptr(),
-                    pitch, scale.data_ptr(), torch.cuda.current_stream(x.device).cuda_stream,
+                    pitch, scale.data_ptr(), raw_stream(x.device.index),
                 ),
                 "tthrml_quantize_rows",
             )
     return QuantizedRows(values[:, :cols], scale)
-
-
-_FEW_ROWS = 8
-_FEW_BYTES = 160 * 1024
 
 
 def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=None):
@@ -195,84 +198,88 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
     torch = _torch()
     if not isinstance(weights, QuantizedRows):
         raise TypeError(f"weights must be QuantizedRows (see quantize_rows), got {type(weights).__name__}")
-    if weights.scale is None:
+    w, w_scale = weights.values, weights.scale
+    if w_scale is None:
         raise ValueError("weights need a scale per unit")
-    dev = weights.device
+    dev, N = w.device, w.shape[0]
     quantized = isinstance(x, QuantizedRows)
-    if quantized:
-        lead, K = (x.shape[0],), x.shape[1]
-        if x.device != dev:
-            raise ValueError(f"x is on {x.device}, expected {dev}")
-    else:
-        require_cuda("x", x, dev)
-        code = dtype_code(x.dtype)
-        if code is None or x.dim() < 1:
-            raise ValueError(f"x must hold float32, bfloat16 or float16 rows, got {x.dtype} of shape {tuple(x.shape)}")
-        _no_grad("x", x)
-        lead, K = tuple(x.shape[:-1]), x.shape[-1]
-    N = weights.shape[0]
-    if K != weights.shape[1]:
-        raise ValueError(f"x has rows of {K}, the weights have {weights.shape[1]} columns")
+    rows = x.values if quantized else x
+    require_cuda("x", rows, dev)
+    code = nat.DT_I8 if quantized else dtype_code(x.dtype)
+    if code is None or rows.dim() < 1:
+        raise ValueError(f"x must hold float32, bfloat16 or float16 rows, got {x.dtype} of shape {tuple(x.shape)}")
+    _no_grad("x", rows)
+    lead, K = rows.shape[:-1], rows.shape[-1]
+    if K != w.shape[1]:
+        raise ValueError(f"x has rows of {K}, the weights have {w.shape[1]} columns")
+    bias_at = None
     if bias is not None:
         require_cuda("bias", bias, dev)
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (N,):
+        if bias.dtype != torch.float32 or bias.shape != (N,):
             raise ValueError(f"bias must be float32 of shape ({N},), got {bias.dtype} of {tuple(bias.shape)}")
         _no_grad("bias", bias)
         bias = bias.contiguous()
+        bias_at = bias.data_ptr()
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else (torch.float32 if quantized else x.dtype)
     out_code = dtype_code(out_dtype)
     if out_code is None:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     if out is None:
-        out = torch.empty((*lead, N), dtype=out_dtype, device=dev)
-        out2 = out.view(-1, N) if N else out
+        out, out_ld = torch.empty((*lead, N), dtype=out_dtype, device=dev), N
     else:
         require_cuda("out", out, dev)
-        if out.dtype != out_dtype or tuple(out.shape) != (*lead, N):
+        if out.dtype != out_dtype or out.shape != (*lead, N):
             raise ValueError(f"out must be {out_dtype} of shape {(*lead, N)}, got {out.dtype} of {tuple(out.shape)}")
         _no_grad("out", out)
-        out2 = out.view(-1, N) if N else out  # raises if the rows cannot be one matrix
-        if out2.numel() and ((N > 1 and out2.stride(1) != 1) or (out2.shape[0] > 1 and out2.stride(0) < N)):
+        flat = out.view(-1, N) if N else out  # raises if the rows cannot be one matrix
+        if flat.numel() and ((N > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < N)):
             raise ValueError("out needs dense rows that do not overlap")
+        out_ld = flat.stride(0) if N and flat.shape[0] > 1 else N
     if not out.numel():
         return out
-    M = out2.shape[0]
-    out_ld = out2.stride(0) if M > 1 else N
+    if rows.dim() != 2:
+        rows = rows.reshape(-1, K)
+    M = rows.shape[0]
+    row_stride, col_stride = rows.stride()
+    index = dev.index
     lib = nat.lib()
     with on_device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        bias_ptr = None if bias is None else bias.data_ptr()
-        wide = 1 << max(0, M - 1).bit_length()
-        few = M <= _FEW_ROWS and wide * (-(-K // 16) * 16) <= _FEW_BYTES
-        if few:
-            if quantized:
-                rows, ld, sx, code = x.values, x.pitch, x.scale, nat.DT_I8
-            else:
-                rows, sx = x.reshape(-1, K), None
-                if K > 1 and rows.stride(1) != 1 or M > 1 and rows.stride(0) < K:
-                    rows = rows.contiguous()
-                ld = rows.stride(0) if M > 1 else K
-            nat.check(
-                lib.tthrml_int8_product_few(
-                    rows.data_ptr(), code, ld, None if sx is None else sx.data_ptr(), weights.values.data_ptr(),
-                    weights.pitch, weights.scale.data_ptr(), M, N, K, bias_ptr, out2.data_ptr(), out_code, out_ld,
-                    stream,
-                ),
-                "tthrml_int8_product_few",
-            )
-            return out
-        error = error_word(dev)
+        stream = raw_stream(index)
+        error = error_word(dev).data_ptr()
         if not quantized:
-            x = quantize_rows(x.reshape(-1, K))
-        nat.check(
-            lib.tthrml_int8_product(
-                x.values.data_ptr(), x.pitch, None if x.scale is None else x.scale.data_ptr(),
-                weights.values.data_ptr(), weights.pitch, weights.scale.data_ptr(), M, N, K, bias_ptr,
-                out2.data_ptr(), out_code, out_ld, error.data_ptr(), stream,
-            ),
-            "tthrml_int8_product",
+            if K == 1:
+                col_stride = 1
+            elif col_stride == 0:
+                rows = rows.contiguous()
+                row_stride, col_stride = rows.stride()
+            wide = 1 if M == 1 else 2 if M == 2 else 4 if M <= 4 else 8
+            pitch = -(-K // 16) * 16
+            workspace, size = None, 0
+            if M > 8 or wide * pitch > nat.INT8_FEW_BYTES or col_stride != 1 or (M > 1 and row_stride < K):
+                size = M * pitch + -(-M // 4) * 16
+                workspace = torch.empty(size, dtype=torch.int8, device=dev)
+            rc = lib.tthrml_int8_linear(
+                rows.data_ptr(), code, M, K, row_stride, col_stride, None if workspace is None else workspace.data_ptr(),
+                size, w.data_ptr(), weights.pitch, w_scale.data_ptr(), N, bias_at, out.data_ptr(), out_code, out_ld, error,
+                stream,
+            )
+            nat.check(rc, "tthrml_int8_linear")
+            return out
+        x_scale = None if x.scale is None else x.scale.data_ptr()
+        wide = 1 if M == 1 else 2 if M == 2 else 4 if M <= 4 else 8
+        if M <= 8 and wide * (-(-K // 16) * 16) <= nat.INT8_FEW_BYTES:
+            rc = lib.tthrml_int8_product_few(
+                rows.data_ptr(), code, x.pitch, x_scale, w.data_ptr(), weights.pitch, w_scale.data_ptr(), M, N, K,
+                bias_at, out.data_ptr(), out_code, out_ld, stream,
+            )
+            nat.check(rc, "tthrml_int8_product_few")
+            return out
+        rc = lib.tthrml_int8_product(
+            rows.data_ptr(), x.pitch, x_scale, w.data_ptr(), weights.pitch, w_scale.data_ptr(), M, N, K, bias_at,
+            out.data_ptr(), out_code, out_ld, error, stream,
         )
+        nat.check(rc, "tthrml_int8_product")
     return out
 
 
