@@ -598,11 +598,11 @@ int tthrml_int8_field_sample(const int8_t* source_dev, int64_t source_pitch,
                              void* stream);
 
 /*
- * The same for 1 to 8 rows in one launch, reading the weights once.  x:
+ * The same for 1 or 2 rows in one launch, reading the weights once.  x:
  * [rows][x_ld] elements of x_dtype; float32, bfloat16 and float16 rows are
  * quantised in the launch exactly as tthrml_quantize_rows does, int8 rows are
- * taken with x_scale (NULL: ones).  The padded rows (1, 2, 4 or 8 of
- * cols rounded up to 16) must fit 160 KiB.
+ * taken with x_scale (NULL: ones).  The padded rows (cols rounded up to 16) must
+ * fit 160 KiB together.
  */
 int tthrml_int8_product_few(const void* x_dev, int32_t x_dtype, int64_t x_ld, const float* x_scale_dev,
                             const int8_t* weights_dev, int64_t w_pitch, const float* w_scale_dev,
@@ -675,7 +675,7 @@ typedef struct tthrml_moment_phase {
 } tthrml_moment_phase;
 
 /*
- * Rows of floats through 8-bit weights: tthrml_int8_product_few for up to 8 rows with dense columns, else
+ * Rows of floats through 8-bit weights: tthrml_int8_product_few for 1 or 2 rows with dense columns, else
  * tthrml_quantize_rows into the workspace and tthrml_int8_product.  workspace: 16-byte aligned device memory of at least
  * tthrml_int8_linear_workspace(rows, cols) bytes (0: none is needed for dense rows; strided rows need the padded rows and
  * their scales, rows * (cols rounded up to 16) + 4 * rows rounded up to 16), free again once the work on `stream` is done.

@@ -97,12 +97,13 @@ def test_quantize_rows_special_values(tt, cols):
     w = tt.quantize_rows(rand((20, cols), torch.float32, 6).cuda())
     y = tt.int8_product(x.cuda(), w)
     assert torch.isnan(y[[1, 2, 5]]).all() and torch.isfinite(y[[0, 3, 4, 6, 7]]).all()
-    y16 = tt.int8_product(x.cuda().repeat(3, 1), w)  # the tensor-core form
-    assert torch.equal(torch.isnan(y16[:8]), torch.isnan(y)) and torch.equal(y16[8:16].nan_to_num(), y16[:8].nan_to_num())
+    for r in range(8):  # the form for single rows
+        one = tt.int8_product(x[r : r + 1].cuda(), w)
+        assert torch.equal(torch.isnan(one[0]), torch.isnan(y[r])) and torch.equal(one[0].nan_to_num(), y[r].nan_to_num())
 
 
 SHAPES = [(1, 1, 1), (1, 1, 16), (1, 130, 4096), (2, 17, 31), (3, 64, 2048), (4, 255, 5000), (5, 33, 48), (8, 129, 1023),
-          (8, 40, 20480), (9, 1, 1), (9, 130, 127), (16, 64, 128), (17, 65, 129), (37, 203, 501), (64, 128, 256),
+          (8, 40, 20480), (2, 5000, 600), (1, 3001, 12345), (2, 20, 81920), (2, 21, 81921), (9, 1, 1), (9, 130, 127), (16, 64, 128), (17, 65, 129), (37, 203, 501), (64, 128, 256),
           (100, 300, 1000), (128, 256, 512), (129, 257, 640), (300, 70, 3000), (513, 515, 259), (260, 1030, 130)]
 
 

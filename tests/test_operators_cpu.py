@@ -71,8 +71,8 @@ BAD = [
     ("tthrml_int8_product", product(xp=32), b"16-byte aligned"),
     ("tthrml_int8_product", product(ld=7), b"must not overlap"),
     ("tthrml_int8_product_few", few(w=None), b"NULL"),
-    ("tthrml_int8_product_few", few(rows=9), b"1 to 8 rows"),
-    ("tthrml_int8_product_few", few(rows=8, cols=20500, ld=20500, wp=20512), b"shared memory"),
+    ("tthrml_int8_product_few", few(rows=3), b"1 or 2 rows"),
+    ("tthrml_int8_product_few", few(rows=2, cols=82000, ld=82000, wp=82000), b"shared memory"),
     ("tthrml_int8_product_few", few(xd=7), b"unknown element type"),
     ("tthrml_int8_product_few", few(od=3), b"unknown element type"),
     ("tthrml_int8_product_few", few(ld=39), b"must not overlap"),

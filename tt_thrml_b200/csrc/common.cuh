@@ -130,6 +130,13 @@ inline FastDiv make_fastdiv(uint32_t d) {
 __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.m) + n) >> f.l; }
 #endif
 
+#ifdef __CUDACC__
+// Programmatic dependent launch: the next kernel on the stream may start; this one waits for the one before it (at once
+// where it was launched without the attribute).
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
 __host__ __device__ __forceinline__ uint32_t word_of(const u32x4& v, int i) {
   return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
 }

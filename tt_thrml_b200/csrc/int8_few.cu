@@ -1,11 +1,11 @@
-// 8-bit integer product for one to eight rows (single tokens / chains), the rows quantised in the same launch:
+// 8-bit integer product for one or two rows (single tokens / chains), the rows quantised in the same launch:
 //     y[m][n] = (sum_k q[m][k] w[n][k]) * (s_x[m] * s_w[n]) + bias[n].
 //
 // Bound: the weights are read once (N K bytes); there is nothing to reuse them for, so the tensor cores are left
-// alone.  Every CTA quantises the few rows itself into shared memory (M K elements from L2; a launch of its own
-// would cost more than that), while the first weight vectors are already on their way.  Each warp takes R units:
-// a lane holds 16-byte vectors of R weight rows and multiplies them with the rows' vectors from shared memory by
-// dp4a (exact in int32 for K <= 131071).
+// alone.  Every CTA quantises the rows itself into shared memory (M K elements from L2; a launch of its own would cost
+// more than that), while the first weight vectors are already on their way.  The multiplications are dp4a (exact in int32
+// for K <= 131071), whose rate is what ends this form: 33.5 M weights took 10.5, 13.9, 19.4 and 32.5 us for 1, 2, 4
+// and 8 rows, against about 16 us for any of them on the tensor cores.
 #include "int8_common.cuh"
 
 namespace tthrml {
@@ -48,8 +48,7 @@ __device__ __forceinline__ uint4 weights16(const int8_t* row, int64_t k, int64_t
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// Quantises rows of x into xs (pitch kp, zero-padded): a group of 8 / M' warps per row, M' = M rounded up to a power
-// of two, so M = 1 spreads one row over the CTA and M = 8 gives each warp a row.
+// Quantises rows of x into xs (pitch kp, zero-padded): all eight warps take one row, four each of two.
 template <typename T, int MP>
 __device__ __forceinline__ void quantize_into(const FewArgs& a, int8_t* xs, int kp, float* sxs, uint32_t* part) {
   constexpr int kGroup = kFewWarps / MP;  // warps per row
@@ -92,29 +91,30 @@ __device__ __forceinline__ void quantize_into(const FewArgs& a, int8_t* xs, int 
   }
 }
 
-template <typename T, int MP, int R>
-__global__ void __launch_bounds__(kFewThreads) k_int8_few(FewArgs a) {
+// Each warp walks over units, a unit of the weights at a time, kVecs 16-byte vectors per lane and step (a row of 4096
+// weights); the next step's vectors are on their way while the current ones are multiplied, so two CTAs of eight warps
+// keep 128 KB of weights on their way to an SM.
+constexpr int kVecs = 8;
+
+template <typename T, int MP>
+__global__ void __launch_bounds__(kFewThreads, 2) k_int8_few(FewArgs a) {
   extern __shared__ __align__(16) int8_t xs[];
   __shared__ float sxs[8];
   __shared__ uint32_t part[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kp = (a.K + 15) & ~15;
-  const int64_t n0 = ((int64_t)blockIdx.x * kFewWarps + warp) * R;
-  constexpr int U = 4;  // vectors per unit in flight
-  const int8_t* wr[R];
+  const int64_t stride = (int64_t)gridDim.x * kFewWarps;
+  int64_t n = (int64_t)warp * gridDim.x + blockIdx.x;  // the last, partial round of units is spread over the CTAs
+  uint4 next[kVecs];
+  auto fetch = [&](int64_t unit, int k0) {
+    const int8_t* row = a.w + unit * a.w_pitch;
 #pragma unroll
-  for (int r = 0; r < R; ++r) wr[r] = a.w + (n0 + r < a.N ? n0 + r : 0) * a.w_pitch;
-  uint4 v[R][U];
-  const bool active = n0 < a.N;
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < kVecs; ++u) {
       const int k = k0 + (u * 32 + lane) * 16;
-#pragma unroll
-      for (int r = 0; r < R; ++r) v[r][u] = k < a.K ? weights16(wr[r], k, a.K) : make_uint4(0u, 0u, 0u, 0u);
+      next[u] = k < a.K ? weights16(row, k, a.K) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
-  if (active) fetch(0);
+  if (n < a.N) fetch(n, 0);
   if constexpr (sizeof(T) == 1) {
     const int8_t* x = reinterpret_cast<const int8_t*>(a.x);
     for (int m = 0; m < MP; ++m) {
@@ -125,71 +125,70 @@ __global__ void __launch_bounds__(kFewThreads) k_int8_few(FewArgs a) {
     quantize_into<T, MP>(a, xs, kp, sxs, part);
   }
   __syncthreads();
-  if (!active) return;
-  int32_t acc[R][MP];
+  int32_t acc[MP];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int m = 0; m < MP; ++m) acc[m] = 0;
+  for (int k0 = 0; n < a.N;) {
+    uint4 cur[kVecs];
 #pragma unroll
-    for (int m = 0; m < MP; ++m) acc[r][m] = 0;
-  for (int k0 = 0; k0 < a.K; k0 += U * 512) {
-    uint4 cur[R][U];
+    for (int u = 0; u < kVecs; ++u) cur[u] = next[u];
+    const int64_t unit = n;
+    const int base = k0;
+    k0 += kVecs * 512;
+    if (k0 >= a.K) {
+      k0 = 0;
+      n += stride;
+    }
+    if (n < a.N) fetch(n, k0);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < R; ++r) cur[r][u] = v[r][u];
-    if (k0 + U * 512 < a.K) fetch(k0 + U * 512);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + (u * 32 + lane) * 16;
+    for (int u = 0; u < kVecs; ++u) {
+      const int k = base + (u * 32 + lane) * 16;
       if (k < a.K) {
 #pragma unroll
         for (int m = 0; m < MP; ++m) {
           const int4 q = *reinterpret_cast<const int4*>(xs + m * kp + k);
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            acc[r][m] = __dp4a((int)cur[r][u].x, q.x, acc[r][m]);
-            acc[r][m] = __dp4a((int)cur[r][u].y, q.y, acc[r][m]);
-            acc[r][m] = __dp4a((int)cur[r][u].z, q.z, acc[r][m]);
-            acc[r][m] = __dp4a((int)cur[r][u].w, q.w, acc[r][m]);
-          }
+          acc[m] = __dp4a((int)cur[u].x, q.x, acc[m]);
+          acc[m] = __dp4a((int)cur[u].y, q.y, acc[m]);
+          acc[m] = __dp4a((int)cur[u].z, q.z, acc[m]);
+          acc[m] = __dp4a((int)cur[u].w, q.w, acc[m]);
         }
       }
     }
-  }
+    if (k0 == 0) {  // the unit's last step
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-#pragma unroll
-    for (int m = 0; m < MP; ++m) {
-      const int32_t sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
-      if (lane == r * MP + m && m < a.M && n0 + r < a.N) {
-        const int64_t n = n0 + r;
-        float y = __fmul_rn((float)sum, __fmul_rn(sxs[m], __ldg(a.w_scale + n)));
-        if (a.bias) y = __fadd_rn(y, __ldg(a.bias + n));
-        store_out(a.out, a.out_dtype, m * a.out_ld + n, y);
+      for (int m = 0; m < MP; ++m) {
+        const int32_t sum = __reduce_add_sync(0xffffffffu, acc[m]);
+        acc[m] = 0;
+        if (lane == m && m < a.M) {
+          float y = __fmul_rn((float)sum, __fmul_rn(sxs[m], __ldg(a.w_scale + unit)));
+          if (a.bias) y = __fadd_rn(y, __ldg(a.bias + unit));
+          store_out(a.out, a.out_dtype, m * a.out_ld + unit, y);
+        }
       }
     }
   }
 }
 
-template <typename T, int MP, int R>
+template <typename T, int MP>
 int launch_few(const FewArgs& a, cudaStream_t st) {
   const int smem = MP * ((a.K + 15) & ~15);
-  const int64_t grid = (a.N + kFewWarps * R - 1) / (kFewWarps * R);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return cuda_status(e, "tthrml_int8_product_few: device query");
+  const int64_t want = (a.N + kFewWarps - 1) / kFewWarps, most = (int64_t)sms * (smem <= 100 * 1024 ? 2 : 1);
+  const int64_t grid = want < most ? want : most;
   if (smem > 48 * 1024) {  // a per-device attribute of the function; setting it again is cheap
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_int8_few<T, MP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemMax);
+    e = cudaFuncSetAttribute(k_int8_few<T, MP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemMax);
     if (e != cudaSuccess) return cuda_status(e, "k_int8_few shared memory attribute");
   }
-  k_int8_few<T, MP, R><<<(unsigned)grid, kFewThreads, smem, st>>>(a);
+  k_int8_few<T, MP><<<(unsigned)grid, kFewThreads, smem, st>>>(a);
   return launch_status("k_int8_few launch");
 }
 
 template <typename T>
 int launch_few_rows(const FewArgs& a, cudaStream_t st) {
-  if (a.M == 1) return launch_few<T, 1, 2>(a, st);
-  if (a.M == 2) return launch_few<T, 2, 2>(a, st);
-  if (a.M <= 4) return launch_few<T, 4, 2>(a, st);
-  return launch_few<T, 8, 2>(a, st);
+  return a.M == 1 ? launch_few<T, 1>(a, st) : launch_few<T, 2>(a, st);
 }
 
 }  // namespace
@@ -205,13 +204,12 @@ extern "C" int tthrml_int8_product_few(const void* x, int32_t x_dtype, int64_t x
     set_error("tthrml_int8_product_few: NULL argument");
     return TTHRML_ERR_ARG;
   }
-  if (rows < 1 || rows > 8 || units < 1 || cols < 1 || cols > TTHRML_INT8_MAX_COLS || units > 0x3fffffffLL) {
-    set_error("tthrml_int8_product_few: 1 to 8 rows and 1 to %d columns (got %lld rows, %lld units, %lld columns)",
+  if (rows < 1 || rows > 2 || units < 1 || cols < 1 || cols > TTHRML_INT8_MAX_COLS || units > 0x3fffffffLL) {
+    set_error("tthrml_int8_product_few: 1 or 2 rows and 1 to %d columns (got %lld rows, %lld units, %lld columns)",
               TTHRML_INT8_MAX_COLS, (long long)rows, (long long)units, (long long)cols);
     return TTHRML_ERR_ARG;
   }
-  const int64_t mp = rows == 1 ? 1 : (rows == 2 ? 2 : (rows <= 4 ? 4 : 8));
-  if (mp * ((cols + 15) / 16 * 16) > kFewSmemMax) {
+  if (rows * ((cols + 15) / 16 * 16) > kFewSmemMax) {
     set_error("tthrml_int8_product_few: %lld rows of %lld columns exceed the shared memory that holds them",
               (long long)rows, (long long)cols);
     return TTHRML_ERR_ARG;

@@ -134,7 +134,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     sw[j] = live ? __ldg(a.w_scale + n + j) : 0.0f;
     bias[j] = live && a.bias ? __ldg(a.bias + n + j) : 0.0f;
   }
-  if (threadIdx.x < 128) row_scale_of[threadIdx.x] = a.x_scale && m0 + (int)threadIdx.x < a.M ? __ldg(a.x_scale + m0 + threadIdx.x) : 1.0f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -143,8 +142,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       const uint32_t bytes = (uint32_t)(a.box_m * 128 + S::kBBytes);
-      int issued = 0;
-      for (int kb = k_first; kb < k_last; ++kb, ++issued) {
+      const int ahead = min(S::kStages, k_last - k_first);
+      for (int s = 0; s < ahead; ++s) {  // the weights of the first stages, while the rows are still being quantised
+        mbar_expect_tx(&full[s], bytes);
+        tma_load_2d(tiles + s * S::kStage + S::kABytes, &map_b, &full[s], (k_first + s) * 128, n0);
+      }
+      wait_for_previous_kernel();
+      for (int s = 0; s < ahead; ++s) tma_load_2d(tiles + s * S::kStage, &map_a, &full[s], (k_first + s) * 128, m0);
+      int issued = ahead;
+      for (int kb = k_first + ahead; kb < k_last; ++kb, ++issued) {
         const int s = issued % S::kStages;
         if (!mbar_wait(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
           atomicExch(a.error, kErrEmptyWait);
@@ -178,6 +184,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       umma_commit(done);
     }
+  } else if (warp >= 4) {
+    const int row = (int)threadIdx.x - 128;
+    wait_for_previous_kernel();
+    row_scale_of[row] = a.x_scale && m0 + row < a.M ? a.x_scale[m0 + row] : 1.0f;
   }
   const bool ok = mbar_wait(done, 0u);
   if (!ok && lane == 0) atomicExch(a.error, kErrAccWait);
@@ -581,14 +591,14 @@ int consider(const ProductArgs& a, int64_t& best, int& bn, int& split) {
 
 template <int BN>
 int launch_tile(const int8_t* weights, int64_t cols, int64_t w_pitch, const CUtensorMap& ma, const ProductArgs& a,
-                int split, cudaStream_t st) {
+                int split, bool early, cudaStream_t st) {
   CUtensorMap mb;
   const int rc = make_map_i8(&mb, weights, a.N, cols, w_pitch, (uint32_t)BN);
   if (rc) return rc;
   const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN);
   void* params[3] = {(void*)&ma, (void*)&mb, (void*)&a};
   return launch_clusters((const void*)k_int8_tile<BN>, (unsigned)(tiles * split), (unsigned)split, kTileThreads,
-                         TileShape<BN>::kSmem, params, st, "k_int8_tile launch");
+                         TileShape<BN>::kSmem, params, st, "k_int8_tile launch", early);
 }
 
 // As many clusters as are resident at once walk the tiles.
@@ -608,10 +618,12 @@ int launch_pair(const void* fn, const CUtensorMap& ma, const CUtensorMap& mb, Pa
 }  // namespace
 }  // namespace tthrml
 
-extern "C" int tthrml_int8_product(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* weights,
-                                   int64_t w_pitch, const float* w_scale, int64_t rows, int64_t units, int64_t cols,
-                                   const float* bias, void* out, int32_t out_dtype, int64_t out_ld, int32_t* error,
-                                   void* stream) {
+namespace {
+
+// early: the rows were quantised by the kernel just before on the stream, which this one need not wait for at once
+int int8_product(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* weights, int64_t w_pitch,
+                 const float* w_scale, int64_t rows, int64_t units, int64_t cols, const float* bias, void* out,
+                 int32_t out_dtype, int64_t out_ld, int32_t* error, bool early, void* stream) {
   using namespace tthrml;
   if (rows == 0 || units == 0) return TTHRML_OK;
   if (!x || !weights || !w_scale || !out || !error) {
@@ -674,9 +686,19 @@ extern "C" int tthrml_int8_product(const int8_t* x, int64_t x_pitch, const float
   }
   rc = make_map_i8(&ma, x, rows, cols, x_pitch, (uint32_t)a.box_m);
   if (rc) return rc;
-  if (bn == 64) return launch_tile<64>(weights, cols, w_pitch, ma, a, split, st);
-  if (bn == 128) return launch_tile<128>(weights, cols, w_pitch, ma, a, split, st);
-  return launch_tile<256>(weights, cols, w_pitch, ma, a, split, st);
+  if (bn == 64) return launch_tile<64>(weights, cols, w_pitch, ma, a, split, early, st);
+  if (bn == 128) return launch_tile<128>(weights, cols, w_pitch, ma, a, split, early, st);
+  return launch_tile<256>(weights, cols, w_pitch, ma, a, split, early, st);
+}
+
+}  // namespace
+
+extern "C" int tthrml_int8_product(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* weights,
+                                   int64_t w_pitch, const float* w_scale, int64_t rows, int64_t units, int64_t cols,
+                                   const float* bias, void* out, int32_t out_dtype, int64_t out_ld, int32_t* error,
+                                   void* stream) {
+  return int8_product(x, x_pitch, x_scale, weights, w_pitch, w_scale, rows, units, cols, bias, out, out_dtype, out_ld,
+                      error, false, stream);
 }
 
 extern "C" int tthrml_int8_field_sample(const int8_t* source, int64_t source_pitch, const float* source_scale,
@@ -764,12 +786,12 @@ extern "C" int tthrml_int8_linear(const void* x, int32_t x_dtype, int64_t rows, 
   float* scale = (float*)(q + rows * pitch);
   const int rc = tthrml_quantize_rows(x, x_dtype, rows, cols, row_stride, col_stride, q, pitch, scale, stream);
   if (rc) return rc;
-  return tthrml_int8_product(q, pitch, scale, weights, w_pitch, w_scale, rows, units, cols, bias, out, out_dtype, out_ld,
-                             error, stream);
+  return int8_product(q, pitch, scale, weights, w_pitch, w_scale, rows, units, cols, bias, out, out_dtype, out_ld, error,
+                      true, stream);
 }
 
 extern "C" int64_t tthrml_int8_linear_workspace(int64_t rows, int64_t cols) {
-  const int64_t pitch = (cols + 15) / 16 * 16, wide = rows <= 1 ? 1 : (rows == 2 ? 2 : (rows <= 4 ? 4 : 8));
-  if (rows <= 8 && wide * pitch <= TTHRML_INT8_FEW_BYTES) return 0;
+  const int64_t pitch = (cols + 15) / 16 * 16, wide = rows <= 1 ? 1 : 2;
+  if (rows <= 2 && wide * pitch <= TTHRML_INT8_FEW_BYTES) return 0;
   return rows * pitch + (rows * 4 + 15) / 16 * 16;
 }

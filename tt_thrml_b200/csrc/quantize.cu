@@ -18,6 +18,7 @@ __global__ void __launch_bounds__(256)
     k_quantize_rows(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, int vectors,
                     int8_t* __restrict__ q, int64_t pitch, float* __restrict__ scale) {
   __shared__ uint32_t part[8];
+  let_next_kernel_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = W == 1 ? lane : (int)threadIdx.x;
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;

@@ -205,14 +205,16 @@ inline int cluster_fit(const void* fn, unsigned cluster, unsigned threads, int s
   return TTHRML_OK;
 }
 
-// Launches fn on a one-dimensional grid of clusters.
+// Launches fn on a one-dimensional grid of clusters.  early: the kernel may start while the one before it on the stream
+// still runs (programmatic dependent launch); it waits for it by wait_for_previous_kernel() before it reads what that
+// kernel writes.
 inline int launch_clusters(const void* fn, unsigned grid, unsigned cluster, unsigned threads, int smem, void** params,
-                           cudaStream_t st, const char* what) {
+                           cudaStream_t st, const char* what, bool early = false) {
   ClusterFit fit;
   const int rc = cluster_fit(fn, cluster, threads, smem, &fit);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
@@ -222,7 +224,9 @@ inline int launch_clusters(const void* fn, unsigned grid, unsigned cluster, unsi
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, params);
   if (e != cudaSuccess) return cuda_status(e, what);
   return launch_status(what);

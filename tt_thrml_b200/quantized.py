@@ -191,7 +191,7 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
 
     bias: float32 [N] added after the scaling.  out_dtype: float32, bfloat16
     or float16 (default: x's type; float32 for QuantizedRows).  out: a tensor
-    [..., N] to write, its rows dense.  Up to eight rows run as one launch that
+    [..., N] to write, its rows dense.  One or two rows run as one launch that
     reads the weights once; more rows are quantised and multiplied on the
     tensor cores.
     """
@@ -253,10 +253,9 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
             elif col_stride == 0:
                 rows = rows.contiguous()
                 row_stride, col_stride = rows.stride()
-            wide = 1 if M == 1 else 2 if M == 2 else 4 if M <= 4 else 8
             pitch = -(-K // 16) * 16
             workspace, size = None, 0
-            if M > 8 or wide * pitch > nat.INT8_FEW_BYTES or col_stride != 1 or (M > 1 and row_stride < K):
+            if M > 2 or M * pitch > nat.INT8_FEW_BYTES or col_stride != 1 or (M > 1 and row_stride < K):
                 size = M * pitch + -(-M // 4) * 16
                 workspace = torch.empty(size, dtype=torch.int8, device=dev)
             rc = lib.tthrml_int8_linear(
@@ -267,8 +266,7 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
             nat.check(rc, "tthrml_int8_linear")
             return out
         x_scale = None if x.scale is None else x.scale.data_ptr()
-        wide = 1 if M == 1 else 2 if M == 2 else 4 if M <= 4 else 8
-        if M <= 8 and wide * (-(-K // 16) * 16) <= nat.INT8_FEW_BYTES:
+        if M <= 2 and M * (-(-K // 16) * 16) <= nat.INT8_FEW_BYTES:
             rc = lib.tthrml_int8_product_few(
                 rows.data_ptr(), code, x.pitch, x_scale, w.data_ptr(), weights.pitch, w_scale.data_ptr(), M, N, K,
                 bias_at, out.data_ptr(), out_code, out_ld, stream,
