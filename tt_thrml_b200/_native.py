@@ -300,6 +300,17 @@ def hostcall():
     return _host
 
 
+_addresses: dict = {}
+
+
+def address_of(name: str) -> int:
+    """Address of an entry point, for calls from the host module."""
+    at = _addresses.get(name)
+    if at is None:
+        at = _addresses[name] = ctypes.cast(getattr(lib(), name), c_vp).value
+    return at
+
+
 def check(rc: int, what: str) -> None:
     if rc != OK:
         msg = lib().tthrml_last_error().decode(errors="replace")

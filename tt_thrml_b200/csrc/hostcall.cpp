@@ -1,5 +1,9 @@
-// Host side of calls that take many tensors: reads the tensors' addresses and layouts in one pass (Python needs about
-// 0.4 us per tensor and attribute).  A CPython module; the kernels stay behind the C ABI of libtthrml_b200.so.
+// Host side of the operators' calls: reads tensors' addresses and layouts, allocates outputs and calls the C ABI of
+// libtthrml_b200.so in one pass.  Python needs about 0.4 us per tensor and attribute, 2.3 us per allocation and 2 us per
+// ctypes call, which is more than the smallest kernels take.  Each function handles the plain case and returns None for
+// any other, which the Python caller then checks, refuses or lays out.
+#include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -69,7 +73,150 @@ PyObject* bump_versions(PyObject*, PyObject* list) {
   Py_RETURN_NONE;
 }
 
+template <typename Fn>
+Fn address(PyObject* o) {
+  return reinterpret_cast<Fn>(PyLong_AsVoidPtr(o));
+}
+bool wants_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
+using LinearFn = decltype(&tthrml_int8_linear);
+using MomentsFn = decltype(&tthrml_pair_moments);
+using PackFn = decltype(&tthrml_pack_rows);
+
+// int8_product(x, weights, weight scales, pitch, bias or None, function, error word, stream, device) -> the product in x's
+// type, an error code, or None.
+PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) ||
+      !(args[4] == Py_None || THPVariable_Check(args[4])))
+    Py_RETURN_NONE;
+  const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &ws = THPVariable_Unpack(args[2]);
+  const long device = PyLong_AsLong(args[8]);
+  const int64_t pitch = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  const int32_t code = dtype_code(x);
+  if (!plain_cuda(x, device) || code < 0 || x.dim() < 1 || wants_grad(x) || (x.dim() != 2 && !x.is_contiguous()))
+    Py_RETURN_NONE;
+  const int64_t K = x.size(-1), N = w.size(0);
+  if (K != w.size(1) || K < 1 || N < 1 || x.numel() == 0) Py_RETURN_NONE;
+  const int64_t M = x.numel() / K;
+  const float* bias = nullptr;
+  if (args[4] != Py_None) {
+    const at::Tensor& b = THPVariable_Unpack(args[4]);
+    if (!plain_cuda(b, device) || b.scalar_type() != at::kFloat || b.dim() != 1 || b.size(0) != N || !b.is_contiguous() ||
+        wants_grad(b))
+      Py_RETURN_NONE;
+    bias = b.const_data_ptr<float>();
+  }
+  const int64_t rs = x.dim() == 2 ? x.stride(0) : K, cs = x.dim() == 2 && K > 1 ? x.stride(1) : 1;
+  if (cs == 0 || (cs == 1 && M > 1 && rs < K)) Py_RETURN_NONE;
+  try {
+    at::DimVector sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = N;
+    at::Tensor out = at::empty(sizes, x.options().requires_grad(false)), space;
+    int64_t bytes = 0;
+    const int64_t padded = (K + 15) / 16 * 16;
+    if (M > 2 || M * padded > TTHRML_INT8_FEW_BYTES || cs != 1) {
+      bytes = M * padded + (M * 4 + 15) / 16 * 16;
+      space = at::empty({bytes}, x.options().dtype(at::kChar).requires_grad(false));
+    }
+    const int rc = address<LinearFn>(args[5])(
+        x.const_data_ptr(), code, M, K, rs, cs, bytes ? space.mutable_data_ptr() : nullptr, bytes,
+        w.const_data_ptr<int8_t>(), pitch, ws.const_data_ptr<float>(), N, bias, out.mutable_data_ptr(), code, N,
+        address<int32_t*>(args[6]), PyLong_AsVoidPtr(args[7]));
+    if (rc) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(out);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// pair_moments(xs, ys, scales, units, function, pack function, error word, stream, device) -> the moments (with `units` a
+// triple), an error code, or None.
+PyObject* pair_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !PyList_Check(args[2])) Py_RETURN_NONE;
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  if (n < 1 || n > TTHRML_MAX_PHASES || PyList_GET_SIZE(args[1]) != n || PyList_GET_SIZE(args[2]) != n) Py_RETURN_NONE;
+  const bool units = args[3] == Py_True;
+  const long device = PyLong_AsLong(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  tthrml_moment_phase phases[TTHRML_MAX_PHASES] = {};
+  tthrml_pack_matrix packed[TTHRML_MAX_PACKED];
+  const void** packed_into[TTHRML_MAX_PACKED];
+  int32_t n_packed = 0;
+  int64_t M = 0, N = 0, elements = 0;
+  int32_t code = -1;
+  for (Py_ssize_t p = 0; p < n; ++p) {
+    tthrml_moment_phase& ph = phases[p];
+    for (int side = 0; side < 2; ++side) {
+      PyObject* o = PyList_GET_ITEM(args[side], p);
+      if (!THPVariable_Check(o)) Py_RETURN_NONE;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (!plain_cuda(t, device) || t.dim() != 2 || wants_grad(t)) Py_RETURN_NONE;
+      const int32_t c = dtype_code(t);
+      if ((c != TTHRML_DT_BF16 && c != TTHRML_DT_F16) || (code >= 0 && c != code)) Py_RETURN_NONE;
+      code = c;
+      const int64_t chains = t.size(0), u = t.size(1);
+      int64_t& want = side ? N : M;
+      if (u < 1 || (p > 0 && u != want) || (side && chains != ph.chains)) Py_RETURN_NONE;
+      want = u;
+      ph.chains = chains;
+      const void*& at = side ? ph.y : ph.x;
+      int64_t& ld = side ? ph.y_ld : ph.x_ld;
+      ld = chains > 1 ? t.stride(0) : (u + 7) / 8 * 8;
+      at = t.const_data_ptr();
+      if ((u == 1 || t.stride(1) == 1) && ld % 8 == 0 && ld >= u && reinterpret_cast<uintptr_t>(at) % 16 == 0) continue;
+      ld = (u + 7) / 8 * 8;
+      packed_into[n_packed] = &at;
+      packed[n_packed++] = {at, reinterpret_cast<void*>(elements * 2), chains, u, t.stride(0), t.stride(1), ld};
+      elements += chains * ld;
+    }
+    const double s = PyFloat_AsDouble(PyList_GET_ITEM(args[2], p));
+    if (s == -1.0 && PyErr_Occurred()) return nullptr;
+    ph.scale = ph.x_scale = ph.y_scale = (float)s;
+  }
+  void* stream = PyLong_AsVoidPtr(args[7]);
+  try {
+    const at::Tensor& first = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0));
+    const auto options = first.options().dtype(at::kFloat).requires_grad(false);
+    at::Tensor out = at::empty({M, N}, options), xs, ys, space;
+    if (units) {
+      xs = at::empty({M}, options);
+      ys = at::empty({N}, options);
+    }
+    int rc = 0;
+    if (n_packed) {
+      space = at::empty({elements > 0 ? elements : 8}, first.options().requires_grad(false));
+      char* base = static_cast<char*>(space.mutable_data_ptr());
+      for (int i = 0; i < n_packed; ++i) {
+        packed[i].dst = base + reinterpret_cast<uintptr_t>(packed[i].dst);
+        *packed_into[i] = packed[i].dst;
+      }
+      rc = address<PackFn>(args[5])(packed, n_packed, stream);
+    }
+    if (!rc)
+      rc = address<MomentsFn>(args[4])(phases, (int32_t)n, code, M, N, out.mutable_data_ptr<float>(), N,
+                                       units ? xs.mutable_data_ptr<float>() : nullptr,
+                                       units ? ys.mutable_data_ptr<float>() : nullptr, 0, address<int32_t*>(args[6]), stream);
+    if (rc) return PyLong_FromLong(rc);
+    if (!units) return THPVariable_Wrap(out);
+    PyObject *a = THPVariable_Wrap(out), *b = THPVariable_Wrap(xs), *c = THPVariable_Wrap(ys);
+    PyObject* t = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    Py_XDECREF(c);
+    return t;
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 PyMethodDef methods[] = {
+    {"int8_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(int8_product)), METH_FASTCALL,
+     "Product of float rows and 8-bit weights: the plain case, or None."},
+    {"pair_moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pair_moments)), METH_FASTCALL,
+     "Pair moments of lists of phases: the plain case, or None."},
     {"adamw_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_rows)), METH_FASTCALL,
      "Fills gradient addresses into AdamW rows; -1 or the first pair that needs a closer look."},
     {"bump_versions", bump_versions, METH_O, "Marks tensors as written for autograd."},

@@ -11,7 +11,7 @@ two dense blocks at once, on the tensor cores.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import dtype_code, error_word, on_device, raw_stream, require_cuda
+from .quantized import _error_addresses, current_device, dtype_code, error_word, on_device, raw_stream, require_cuda
 
 
 def _torch():
@@ -72,6 +72,17 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
         raise ValueError(f"x, y and scale need one entry per phase, got {len(xs)}, {len(ys)} and {len(scales)}")
     if len(xs) > nat.MAX_PHASES:
         raise ValueError(f"at most {nat.MAX_PHASES} phases are supported, got {len(xs)}")
+    if out is None and not accumulate and type(xs[0]) is torch.Tensor:
+        index = xs[0].get_device()
+        word = _error_addresses.get(index)
+        if word is not None and current_device() == index:  # the plain case, from the second call on
+            nat.bind_device(index)
+            made = nat.hostcall().pair_moments(xs, ys, scales, bool(units), nat.address_of("tthrml_pair_moments"),
+                                               nat.address_of("tthrml_pack_rows"), word, raw_stream(index), index)
+            if made is not None:
+                if type(made) is int:
+                    nat.check(made, "tthrml_pair_moments")
+                return made
     require_cuda("x", xs[0])
     dev, dtype = xs[0].device, xs[0].dtype
     code = dtype_code(dtype)
