@@ -107,19 +107,27 @@ __device__ __forceinline__ float sqrt_approx(float x) {
 __device__ __forceinline__ float near_floor(float x) {
   return __fsub_rn(__fadd_rn(__fsub_rn(x, 0.5f), 12582912.0f), 12582912.0f);
 }
-// 1 / 65536-th uniform of a half word, never 0 or 1
-__device__ __forceinline__ float half_uniform(uint32_t h) {
-  return __fmul_rn(__fadd_rn(__fsub_rn(__uint_as_float(0x4B000000u | h), 8388608.0f), 0.5f), 1.52587890625e-05f);
+// h + 1/2 of a half word h: 65536 times a uniform that is never 0 or 1
+__device__ __forceinline__ float low_half(uint32_t w) {
+  return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7410u)), 8388607.5f);
+}
+__device__ __forceinline__ float high_half(uint32_t w) {
+  return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7432u)), 8388607.5f);
 }
 
-// Code of y = m 127^2 / max|m| >= 0: the largest k with k^2 <= y, or k + 1 with probability (y - k^2) / (2 k + 1).
-__device__ __forceinline__ float code_m(float y, float u) {
+// Code of y = m 127^2 / max|m| >= 0: the largest k with k^2 <= y, or k + 1 with probability (y - k^2) / (2 k + 1).  The
+// approximate root is off by one only next to a whole number; u65536 is 65536 u, and the powers of two are exact.
+__device__ __forceinline__ float code_m(float y, float u65536) {
   float k = near_floor(sqrt_approx(y));
-  k = __fmul_rn(k, k) > y ? k - 1.0f : k;
-  const float n = k + 1.0f;
-  k = __fmul_rn(n, n) <= y ? n : k;
-  const float k2 = __fmul_rn(k, k), span = __fadd_rn(k, k) + 1.0f;
-  const float q = __fmul_rn(u, span) < __fsub_rn(y, k2) ? k + 1.0f : k;
+  float k2 = __fmul_rn(k, k), span = __fadd_rn(__fadd_rn(k, k), 1.0f);
+  float over = __fsub_rn(y, k2);
+  if (over < 0.0f || over >= span) {
+    k = over < 0.0f ? __fsub_rn(k, 1.0f) : __fadd_rn(k, 1.0f);
+    k2 = __fmul_rn(k, k);
+    span = __fadd_rn(__fadd_rn(k, k), 1.0f);
+    over = __fsub_rn(y, k2);
+  }
+  const float q = __fmul_rn(u65536, span) < __fmul_rn(over, 65536.0f) ? __fadd_rn(k, 1.0f) : k;
   return fminf(q, 127.0f);
 }
 __device__ __forceinline__ float fourth(float k) {
@@ -127,13 +135,17 @@ __device__ __forceinline__ float fourth(float k) {
   return __fmul_rn(k2, k2);
 }
 // Code of y = v 255^4 / max v >= 0, likewise with fourth powers; a y > 0 gets at least 1.
-__device__ __forceinline__ float code_v(float y, float u) {
+__device__ __forceinline__ float code_v(float y, float u65536) {
   float k = near_floor(sqrt_approx(sqrt_approx(y)));
-  k = fourth(k) > y ? k - 1.0f : k;
-  k = fourth(k + 1.0f) <= y ? k + 1.0f : k;
-  const float k4 = fourth(k), span = __fsub_rn(fourth(k + 1.0f), k4);
-  float q = __fmul_rn(u, span) < __fsub_rn(y, k4) ? k + 1.0f : k;
-  q = k == 0.0f ? (y > 0.0f ? 1.0f : 0.0f) : q;
+  float k4 = fourth(k), n4 = fourth(__fadd_rn(k, 1.0f));
+  if (k4 > y || n4 <= y) {
+    k = k4 > y ? __fsub_rn(k, 1.0f) : __fadd_rn(k, 1.0f);
+    k4 = fourth(k);
+    n4 = fourth(__fadd_rn(k, 1.0f));
+  }
+  const float span = __fsub_rn(n4, k4), over = __fsub_rn(y, k4);
+  float q = __fmul_rn(u65536, span) < __fmul_rn(over, 65536.0f) ? __fadd_rn(k, 1.0f) : k;
+  if (k == 0.0f) q = y > 0.0f ? 1.0f : 0.0f;
   return fminf(q, 255.0f);
 }
 // Low byte of the integer held by a float in -2^22 .. 2^22.
@@ -158,6 +170,7 @@ __global__ void __launch_bounds__(kAdamThreads)
   }
   __syncthreads();
   const float step_size = coef[0], r_bias2 = coef[1], keep = coef[2];
+  const PhiloxKeys keys = philox_keys((uint32_t)a.seed, (uint32_t)(a.seed >> 32));
   int ti = 0;
   for (int lo = 0, hi = a.n_tensors; hi - lo > 1;) {  // the tensor of the first chunk
     const int mid = (lo + hi) >> 1;
@@ -200,8 +213,15 @@ __global__ void __launch_bounds__(kAdamThreads)
     for (int k = 0; k < 8; ++k) {
       m[k] = __fadd_rn(__fmul_rn(m[k], a.b1), __fmul_rn(g[k], a.d1));
       v[k] = __fadd_rn(__fmul_rn(v[k], a.b2), __fmul_rn(__fmul_rn(g[k], g[k]), a.d2));
-      const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), r_bias2), a.eps);
-      p[k] = __fsub_rn(__fmul_rn(p[k], keep), __fmul_rn(__fdiv_rn(m[k], denom), step_size));
+      if (BITS == 32) {
+        const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), r_bias2), a.eps);
+        p[k] = __fsub_rn(__fmul_rn(p[k], keep), __fmul_rn(__fdiv_rn(m[k], denom), step_size));
+      } else {
+        // the hardware's root and quotient (2^-21 of the update at most, whose moments are codes to about 1 %): the step on
+        // codes is bound by its instructions
+        const float denom = __fadd_rn(__fmul_rn(sqrt_approx(v[k]), r_bias2), a.eps);
+        p[k] = __fsub_rn(__fmul_rn(p[k], keep), __fmul_rn(__fdividef(m[k], denom), step_size));
+      }
     }
     store_any(t.param_dtype, t.param, i, t.n, pv, p);
     if (BITS == 32) {
@@ -232,15 +252,14 @@ __global__ void __launch_bounds__(kAdamThreads)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t word = (e >> 2) + h;
-        const u32x4 r = philox4x32_10(u32x4{(uint32_t)word, (uint32_t)(word >> 32), (uint32_t)step, kSaltAdam},
-                                      (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
+        const u32x4 r = philox4x32_10(u32x4{(uint32_t)word, (uint32_t)(word >> 32), (uint32_t)step, kSaltAdam}, keys);
         const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int k = 4 * h + j;
-          const float q = code_m(__fmul_rn(fabsf(m[k]), im), half_uniform(rw[j] & 0xFFFFu));
-          qm[k] = int_byte(m[k] < 0.0f ? -q : q);
-          qv[k] = int_byte(code_v(__fmul_rn(v[k], iv), half_uniform(rw[j] >> 16)));
+          const float q = code_m(__fmul_rn(fabsf(m[k]), im), low_half(rw[j]));
+          qm[k] = int_byte(copysignf(q, m[k]));
+          qv[k] = int_byte(code_v(__fmul_rn(v[k], iv), high_half(rw[j])));
         }
       }
       *reinterpret_cast<uint2*>(reinterpret_cast<int8_t*>(a.m) + e) =
