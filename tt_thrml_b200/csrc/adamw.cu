@@ -8,8 +8,9 @@
 //
 // The tensors' addresses travel in the launch's parameters, so a step uploads nothing and a captured graph keeps its
 // own copy.  The moments of all tensors lie in one buffer, each tensor's segment padded to 256 elements.  A CTA takes a
-// contiguous range of 2048-element chunks of the concatenated tensors (a chunk never spans two tensors); a thread
-// holds eight consecutive elements.  The step counter and the learning rate stand in device memory, so a replayed
+// contiguous range of 2048-element chunks of the concatenated tensors (a chunk never spans two tensors); a warp holds
+// 256 of them, a thread two groups of four 128 apart, so that every load and store of a warp is contiguous.  The step
+// counter and the learning rate stand in device memory, so a replayed
 // graph counts on; the last CTA of a step's last launch advances the counter.
 //
 // 8-bit codes, one warp per block of 256 elements with the block's largest |m| and v as scales:
@@ -42,50 +43,76 @@ struct AdamArgs {
   float* v_scale;
   tthrml_adamw_ctl* ctl;
   float b1, d1, b2, d2, eps;  // d = 1 - b
+  float minus_zero;
   double beta1, beta2, weight_decay;
   uint64_t seed;
   int32_t n_tensors;
   int32_t last;     // this launch ends the step
 };
 
-template <typename T>
-__device__ __forceinline__ void load_elems(const void* base, int64_t i, int64_t n, bool vectors, float (&f)[8]) {
-  const T* p = reinterpret_cast<const T*>(base) + i;
-  if (vectors && i + 8 <= n) {
-    Vec8<T> v;
+// The bits of four consecutive elements from place i of a tensor of n (16-bit elements in the first two words);
+// `vectors`: the tensor is aligned to four elements.  Loading and converting are apart, so that a thread's loads are all on
+// their way before the first conversion waits for one.
+struct Raw4 {
+  uint32_t w[4];
+};
+__device__ __forceinline__ Raw4 load_raw(int32_t dtype, const void* base, int64_t i, int64_t n, bool vectors) {
+  Raw4 r = {{0u, 0u, 0u, 0u}};
+  if (dtype == TTHRML_DT_F32) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(base) + i;
+    if (vectors && i + 4 <= n) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    } else {
 #pragma unroll
-    for (int k = 0; k < (int)(sizeof(T) / 2); ++k) v.w[k] = *(reinterpret_cast<const uint4*>(p) + k);
-    unpack8(v, f);
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) r.w[k] = p[k];
+    }
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + i;
+    if (vectors && i + 4 <= n) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      r.w[0] = v.x, r.w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) r.w[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
+    }
+  }
+  return r;
+}
+__device__ __forceinline__ void convert(int32_t dtype, const Raw4& r, float2 (&f)[2]) {
+  if (dtype == TTHRML_DT_F32) {
+    f[0] = make_float2(__uint_as_float(r.w[0]), __uint_as_float(r.w[1]));
+    f[1] = make_float2(__uint_as_float(r.w[2]), __uint_as_float(r.w[3]));
+  } else if (dtype == TTHRML_DT_BF16) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) f[k] = make_float2(__uint_as_float(r.w[k] << 16), __uint_as_float(r.w[k] & 0xFFFF0000u));
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = i + k < n ? to_f32(p[k]) : 0.0f;
+    for (int k = 0; k < 2; ++k) f[k] = __half22float2(*reinterpret_cast<const __half2*>(&r.w[k]));
   }
 }
 template <typename T>
-__device__ __forceinline__ void store_elems(void* base, int64_t i, int64_t n, bool vectors, const float (&f)[8]) {
+__device__ __forceinline__ void store_elems(void* base, int64_t i, int64_t n, bool vectors, const float2 (&f)[2]) {
   T* p = reinterpret_cast<T*>(base) + i;
-  if (vectors && i + 8 <= n) {
-    Vec8<T> v;
-    T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = from_f32<T>(f[k]);
-#pragma unroll
-    for (int k = 0; k < (int)(sizeof(T) / 2); ++k) *(reinterpret_cast<uint4*>(p) + k) = v.w[k];
+  if (vectors && i + 4 <= n) {
+    if (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+    } else {
+      uint2 v;
+      T* e = reinterpret_cast<T*>(&v);
+      e[0] = from_f32<T>(f[0].x), e[1] = from_f32<T>(f[0].y), e[2] = from_f32<T>(f[1].x), e[3] = from_f32<T>(f[1].y);
+      *reinterpret_cast<uint2*>(p) = v;
+    }
   } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + k < n) p[k] = from_f32<T>(f[k]);
+    if (i < n) p[0] = from_f32<T>(f[0].x);
+    if (i + 1 < n) p[1] = from_f32<T>(f[0].y);
+    if (i + 2 < n) p[2] = from_f32<T>(f[1].x);
+    if (i + 3 < n) p[3] = from_f32<T>(f[1].y);
   }
 }
-__device__ __forceinline__ void load_any(int32_t dtype, const void* base, int64_t i, int64_t n, bool vectors, float (&f)[8]) {
-  if (dtype == TTHRML_DT_F32)
-    load_elems<float>(base, i, n, vectors, f);
-  else if (dtype == TTHRML_DT_BF16)
-    load_elems<__nv_bfloat16>(base, i, n, vectors, f);
-  else
-    load_elems<__half>(base, i, n, vectors, f);
-}
-__device__ __forceinline__ void store_any(int32_t dtype, void* base, int64_t i, int64_t n, bool vectors, const float (&f)[8]) {
+__device__ __forceinline__ void store_any(int32_t dtype, void* base, int64_t i, int64_t n, bool vectors, const float2 (&f)[2]) {
   if (dtype == TTHRML_DT_F32)
     store_elems<float>(base, i, n, vectors, f);
   else if (dtype == TTHRML_DT_BF16)
@@ -94,68 +121,102 @@ __device__ __forceinline__ void store_any(int32_t dtype, void* base, int64_t i, 
     store_elems<__half>(base, i, n, vectors, f);
 }
 
-// Byte j of a word as a float, unsigned: the byte under the exponent of 2^23, which is subtracted.
-__device__ __forceinline__ float byte_f32(uint32_t w, int j) {
-  return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540u | (uint32_t)j)), 8388608.0f);
+// Pairs of elements: one packed instruction for two float32 operations, each rounded as the single one.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+// A product that goes into a sum: packed products and sums are contracted to one rounding, even with their rounding named,
+// and codes and scales have to be those of the formula bit for bit.  -0, which leaves the product as it is, comes as a
+// value that the compiler does not know.
+__device__ __forceinline__ float2 product2(float2 a, float2 b, float minus_zero) { return __ffma2_rn(a, b, both(minus_zero)); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+
+// Byte j of a word under the exponent of 2^23: 2^23 + byte.
+__device__ __forceinline__ float byte_high(uint32_t w, int j) {
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540u | (uint32_t)j));
 }
 __device__ __forceinline__ float sqrt_approx(float x) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// floor of 0 <= x < 2^22, one too few at odd integers (x - 1/2 is a tie there, rounded to even)
-__device__ __forceinline__ float near_floor(float x) {
-  return __fsub_rn(__fadd_rn(__fsub_rn(x, 0.5f), 12582912.0f), 12582912.0f);
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
-// h + 1/2 of a half word h: 65536 times a uniform that is never 0 or 1
-__device__ __forceinline__ float low_half(uint32_t w) {
-  return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7410u)), 8388607.5f);
+// floors of 0 <= x < 2^22
+__device__ __forceinline__ float2 floor2(float2 x) { return add2(__fadd2_rd(x, both(8388608.0f)), both(-8388608.0f)); }
+// h + 1/2 of the low (high) half words h: 65536 times a uniform that is never 0 or 1
+__device__ __forceinline__ float2 low_halves(uint32_t a, uint32_t b) {
+  return add2(make_float2(__uint_as_float(__byte_perm(a, 0x4B000000u, 0x7410u)),
+                          __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7410u))),
+              both(-8388607.5f));
 }
-__device__ __forceinline__ float high_half(uint32_t w) {
-  return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7432u)), 8388607.5f);
-}
-
-// Code of y = m 127^2 / max|m| >= 0: the largest k with k^2 <= y, or k + 1 with probability (y - k^2) / (2 k + 1).  The
-// approximate root is off by one only next to a whole number; u65536 is 65536 u, and the powers of two are exact.
-__device__ __forceinline__ float code_m(float y, float u65536) {
-  float k = near_floor(sqrt_approx(y));
-  float k2 = __fmul_rn(k, k), span = __fadd_rn(__fadd_rn(k, k), 1.0f);
-  float over = __fsub_rn(y, k2);
-  if (over < 0.0f || over >= span) {
-    k = over < 0.0f ? __fsub_rn(k, 1.0f) : __fadd_rn(k, 1.0f);
-    k2 = __fmul_rn(k, k);
-    span = __fadd_rn(__fadd_rn(k, k), 1.0f);
-    over = __fsub_rn(y, k2);
-  }
-  const float q = __fmul_rn(u65536, span) < __fmul_rn(over, 65536.0f) ? __fadd_rn(k, 1.0f) : k;
-  return fminf(q, 127.0f);
+__device__ __forceinline__ float2 high_halves(uint32_t a, uint32_t b) {
+  return add2(make_float2(__uint_as_float(__byte_perm(a, 0x4B000000u, 0x7432u)),
+                          __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7432u))),
+              both(-8388607.5f));
 }
 __device__ __forceinline__ float fourth(float k) {
   const float k2 = __fmul_rn(k, k);
   return __fmul_rn(k2, k2);
 }
-// Code of y = v 255^4 / max v >= 0, likewise with fourth powers; a y > 0 gets at least 1.
-__device__ __forceinline__ float code_v(float y, float u65536) {
-  float k = near_floor(sqrt_approx(sqrt_approx(y)));
-  float k4 = fourth(k), n4 = fourth(__fadd_rn(k, 1.0f));
-  if (k4 > y || n4 <= y) {
-    k = k4 > y ? __fsub_rn(k, 1.0f) : __fadd_rn(k, 1.0f);
-    k4 = fourth(k);
-    n4 = fourth(__fadd_rn(k, 1.0f));
-  }
-  const float span = __fsub_rn(n4, k4), over = __fsub_rn(y, k4);
-  float q = __fmul_rn(u65536, span) < __fmul_rn(over, 65536.0f) ? __fadd_rn(k, 1.0f) : k;
-  if (k == 0.0f) q = y > 0.0f ? 1.0f : 0.0f;
-  return fminf(q, 255.0f);
+__device__ __forceinline__ float2 fourth2(float2 k) {
+  const float2 k2 = mul2(k, k);
+  return mul2(k2, k2);
 }
-// Low byte of the integer held by a float in -2^22 .. 2^22.
-__device__ __forceinline__ uint32_t int_byte(float q) { return __float_as_uint(__fadd_rn(q, 12582912.0f)); }
+
+// The approximate roots are off by one only next to a whole number: the place of y among the squares (fourth powers) again.
+__device__ __noinline__ float2 place_m(float y, float k) {  // (k, y - k^2)
+  if (__fmul_rn(k, k) > y) k -= 1.0f;
+  if (__fmul_rn(k + 1.0f, k + 1.0f) <= y) k += 1.0f;
+  return make_float2(k, __fsub_rn(y, __fmul_rn(k, k)));
+}
+__device__ __noinline__ float2 place_v(float y, float k) {  // (k, y - k^4)
+  if (fourth(k) > y) k -= 1.0f;
+  if (fourth(k + 1.0f) <= y) k += 1.0f;
+  return make_float2(k, __fsub_rn(y, fourth(k)));
+}
+
+// Codes of y = |m| 127^2 / max|m|: the largest k with k^2 <= y, or k + 1 with probability (y - k^2) / (2 k + 1).  u65536 is
+// 65536 times the uniform; the scaling by powers of two is exact.
+__device__ __forceinline__ float2 codes_m(float2 y, float2 u65536) {
+  float2 k = floor2(make_float2(sqrt_approx(y.x), sqrt_approx(y.y)));
+  float2 over = __ffma2_rn(neg2(k), k, y), span = __ffma2_rn(k, both(2.0f), both(1.0f));  // k^2 and 2 k + 1 are exact
+  if (over.x < 0.0f || over.x >= span.x || over.y < 0.0f || over.y >= span.y) {
+    const float2 a = place_m(y.x, k.x), b = place_m(y.y, k.y);
+    k = make_float2(a.x, b.x);
+    over = make_float2(a.y, b.y);
+    span = __ffma2_rn(k, both(2.0f), both(1.0f));
+  }
+  const float2 t = mul2(u65536, span), o = mul2(over, both(65536.0f)), n = add2(k, both(1.0f));
+  return make_float2(fminf(t.x < o.x ? n.x : k.x, 127.0f), fminf(t.y < o.y ? n.y : k.y, 127.0f));
+}
+// Codes of y = v 255^4 / max v, likewise with fourth powers; a y > 0 gets at least 1.
+__device__ __forceinline__ float2 codes_v(float2 y, float2 u65536) {
+  float2 k = floor2(make_float2(sqrt_approx(sqrt_approx(y.x)), sqrt_approx(sqrt_approx(y.y))));
+  float2 n = add2(k, both(1.0f)), k4 = fourth2(k), n4 = fourth2(n), over = add2(y, neg2(k4));
+  if (over.x < 0.0f || n4.x <= y.x || over.y < 0.0f || n4.y <= y.y) {
+    const float2 a = place_v(y.x, k.x), b = place_v(y.y, k.y);
+    k = make_float2(a.x, b.x);
+    over = make_float2(a.y, b.y);
+    n = add2(k, both(1.0f));
+    k4 = fourth2(k);
+    n4 = fourth2(n);
+  }
+  const float2 t = mul2(u65536, add2(n4, neg2(k4))), o = mul2(over, both(65536.0f));
+  const float qx = t.x < o.x ? n.x : k.x, qy = t.y < o.y ? n.y : k.y;
+  // k = 0 is below 1 and y > 0: code 1
+  return make_float2(fminf(y.x > 0.0f ? fmaxf(qx, 1.0f) : qx, 255.0f), fminf(y.y > 0.0f ? fmaxf(qy, 1.0f) : qy, 255.0f));
+}
+// The low bytes of four words (the integers held by floats in -2^22 .. 2^22 plus 3 2^22).
 __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040u), __byte_perm(c, d, 0x0040u), 0x5410u);
 }
 
 template <int BITS, int T>
-__global__ void __launch_bounds__(kAdamThreads)
+__global__ void __launch_bounds__(kAdamThreads, 4)
     k_adamw(const __grid_constant__ AdamTable<T> tab, const __grid_constant__ AdamArgs a) {
   __shared__ float coef[4];  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd, step
   const int chunks = tab.first_chunk[a.n_tensors];
@@ -180,65 +241,73 @@ __global__ void __launch_bounds__(kAdamThreads)
   for (int c = c_first; c < c_last; ++c) {
     while (tab.first_chunk[ti + 1] <= c) ++ti;
     const tthrml_adamw_tensor& t = tab.t[ti];
-    const int64_t i = (int64_t)(c - tab.first_chunk[ti]) * kChunk + 8 * threadIdx.x;
-    const int64_t padded = (t.n + 255) & ~(int64_t)255;
-    if (i >= padded) continue;  // whole warps: a warp covers 256 elements
-    const int64_t e = t.state + i;
-    const bool pv = (uintptr_t)t.param % 16 == 0, gv = (uintptr_t)t.grad % 16 == 0;
-    float p[8], g[8], m[8], v[8];
-    load_any(t.grad_dtype, t.grad, i, t.n, gv, g);
-    load_any(t.param_dtype, t.param, i, t.n, pv, p);
-    if (BITS == 32) {
-      const float4* mp = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.m) + e);
-      const float4* vp = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.v) + e);
+    const int64_t i = (int64_t)(c - tab.first_chunk[ti]) * kChunk + 256 * (threadIdx.x >> 5) + 4 * (threadIdx.x & 31);
+    if (i - 4 * (threadIdx.x & 31) >= t.n) continue;  // whole warps
+    const int64_t e = t.state + i;  // this thread's groups: e .. e + 3 and e + 128 .. e + 131
+    const bool pv = (uintptr_t)t.param % (t.param_dtype == TTHRML_DT_F32 ? 16 : 8) == 0;
+    const bool gv = (uintptr_t)t.grad % (t.grad_dtype == TTHRML_DT_F32 ? 16 : 8) == 0;
+    float2 p[2][2], g[2][2], m[2][2], v[2][2];
+    Raw4 pr[2], gr[2];
+    uint32_t mc[2], vc[2];
+    float um = 0.0f, uv = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float4 x = mp[k], y = vp[k];
-        m[4 * k] = x.x, m[4 * k + 1] = x.y, m[4 * k + 2] = x.z, m[4 * k + 3] = x.w;
-        v[4 * k] = y.x, v[4 * k + 1] = y.y, v[4 * k + 2] = y.z, v[4 * k + 3] = y.w;
-      }
-    } else {
-      const uint2 mc = *reinterpret_cast<const uint2*>(reinterpret_cast<const int8_t*>(a.m) + e);
-      const uint2 vc = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.v) + e);
-      const float um = __fmul_rn(a.m_scale[e >> 8], 1.0f / 16129.0f), uv = __fmul_rn(a.v_scale[e >> 8], 1.0f / 4228250625.0f);
-      const uint32_t mw[2] = {mc.x ^ 0x80808080u, mc.y ^ 0x80808080u}, vw[2] = {vc.x, vc.y};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float c8 = __fsub_rn(byte_f32(mw[k >> 2], k & 3), 128.0f);
-        m[k] = __fmul_rn(__fmul_rn(c8, fabsf(c8)), um);
-        v[k] = __fmul_rn(fourth(byte_f32(vw[k >> 2], k & 3)), uv);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      m[k] = __fadd_rn(__fmul_rn(m[k], a.b1), __fmul_rn(g[k], a.d1));
-      v[k] = __fadd_rn(__fmul_rn(v[k], a.b2), __fmul_rn(__fmul_rn(g[k], g[k]), a.d2));
+    for (int h = 0; h < 2; ++h) {
+      gr[h] = load_raw(t.grad_dtype, t.grad, i + 128 * h, t.n, gv);
+      pr[h] = load_raw(t.param_dtype, t.param, i + 128 * h, t.n, pv);
       if (BITS == 32) {
-        const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), r_bias2), a.eps);
-        p[k] = __fsub_rn(__fmul_rn(p[k], keep), __fmul_rn(__fdiv_rn(m[k], denom), step_size));
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.m) + e + 128 * h);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.v) + e + 128 * h);
+        m[h][0] = make_float2(x.x, x.y), m[h][1] = make_float2(x.z, x.w);
+        v[h][0] = make_float2(y.x, y.y), v[h][1] = make_float2(y.z, y.w);
       } else {
-        // the hardware's root and quotient (2^-21 of the update at most, whose moments are codes to about 1 %): the step on
-        // codes is bound by its instructions
-        const float denom = __fadd_rn(__fmul_rn(sqrt_approx(v[k]), r_bias2), a.eps);
-        p[k] = __fsub_rn(__fmul_rn(p[k], keep), __fmul_rn(__fdividef(m[k], denom), step_size));
+        mc[h] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const int8_t*>(a.m) + e + 128 * h) ^ 0x80808080u;
+        vc[h] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(a.v) + e + 128 * h);
       }
     }
-    store_any(t.param_dtype, t.param, i, t.n, pv, p);
-    if (BITS == 32) {
-      float4* mp = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.m) + e);
-      float4* vp = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.v) + e);
+    if (BITS == 8) {
+      um = __fmul_rn(a.m_scale[e >> 8], 1.0f / 16129.0f);
+      uv = __fmul_rn(a.v_scale[e >> 8], 1.0f / 4228250625.0f);
+    }
+    uint32_t tm = 0u, tv = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      convert(t.grad_dtype, gr[h], g[h]);
+      convert(t.param_dtype, pr[h], p[h]);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        mp[k] = make_float4(m[4 * k], m[4 * k + 1], m[4 * k + 2], m[4 * k + 3]);
-        vp[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        if (BITS == 8) {
+          const float2 c8 = add2(make_float2(byte_high(mc[h], 2 * k), byte_high(mc[h], 2 * k + 1)), both(-8388736.0f));
+          const float2 mag = mul2(mul2(c8, c8), both(um));
+          m[h][k] = make_float2(copysignf(mag.x, c8.x), copysignf(mag.y, c8.y));
+          v[h][k] = mul2(fourth2(add2(make_float2(byte_high(vc[h], 2 * k), byte_high(vc[h], 2 * k + 1)), both(-8388608.0f))),
+                         both(uv));
+        }
+        const float2 gk = g[h][k];
+        const float2 mk = m[h][k] = add2(product2(m[h][k], both(a.b1), a.minus_zero), product2(gk, both(a.d1), a.minus_zero));
+        const float2 vk = v[h][k] = add2(product2(v[h][k], both(a.b2), a.minus_zero), product2(mul2(gk, gk), both(a.d2), a.minus_zero));
+        float2 upd;
+        if (BITS == 32) {
+          const float2 denom = add2(mul2(make_float2(__fsqrt_rn(vk.x), __fsqrt_rn(vk.y)), both(r_bias2)), both(a.eps));
+          upd = make_float2(__fdiv_rn(mk.x, denom.x), __fdiv_rn(mk.y, denom.y));
+        } else {
+          // the hardware's root and reciprocal (2^-21 of the update at most, whose moments are codes to about 1 %): the
+          // step on codes is bound by its instructions
+          const float2 denom = add2(mul2(make_float2(sqrt_approx(vk.x), sqrt_approx(vk.y)), both(r_bias2)), both(a.eps));
+          upd = mul2(mk, make_float2(rcp_approx(denom.x), rcp_approx(denom.y)));
+          tm = max(tm, max(abs_bits(mk.x), abs_bits(mk.y)));
+          tv = max(tv, max(__float_as_uint(vk.x) & 0x7FFFFFFFu, __float_as_uint(vk.y) & 0x7FFFFFFFu));
+        }
+        p[h][k] = add2(mul2(p[h][k], both(keep)), neg2(mul2(upd, both(step_size))));
       }
-    } else {
-      uint32_t tm = 0u, tv = 0u;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        tm = max(tm, abs_bits(m[k]));
-        tv = max(tv, abs_bits(v[k]));
+      store_any(t.param_dtype, t.param, i + 128 * h, t.n, pv, p[h]);
+      if (BITS == 32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.m) + e + 128 * h) =
+            make_float4(m[h][0].x, m[h][0].y, m[h][1].x, m[h][1].y);
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.v) + e + 128 * h) =
+            make_float4(v[h][0].x, v[h][0].y, v[h][1].x, v[h][1].y);
       }
+    }
+    if (BITS == 8) {
       tm = __reduce_max_sync(0xffffffffu, tm);
       tv = __reduce_max_sync(0xffffffffu, tv);
       float top_m = __uint_as_float(tm), top_v = __uint_as_float(tv);
@@ -248,24 +317,25 @@ __global__ void __launch_bounds__(kAdamThreads)
       if (top_v == 0.0f || top_m < 7.8886090522101181e-31f) top_m = 0.0f;  // 2^-100
       const float im = top_m > 0.0f ? __fdiv_rn(16129.0f, top_m) : 0.0f;
       const float iv = top_v > 0.0f ? __fdiv_rn(4228250625.0f, top_v) : 0.0f;
-      uint32_t qm[8], qv[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int64_t word = (e >> 2) + h;
+        const int64_t word = (e >> 2) + 32 * h;
         const u32x4 r = philox4x32_10(u32x4{(uint32_t)word, (uint32_t)(word >> 32), (uint32_t)step, kSaltAdam}, keys);
         const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+        uint32_t qm[4], qv[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = 4 * h + j;
-          const float q = code_m(__fmul_rn(fabsf(m[k]), im), low_half(rw[j]));
-          qm[k] = int_byte(copysignf(q, m[k]));
-          qv[k] = int_byte(code_v(__fmul_rn(v[k], iv), high_half(rw[j])));
+        for (int k = 0; k < 2; ++k) {
+          const float2 mk = m[h][k], s = mul2(mk, both(im));
+          const float2 cm = codes_m(make_float2(fabsf(s.x), fabsf(s.y)), low_halves(rw[2 * k], rw[2 * k + 1]));
+          const float2 cv = codes_v(mul2(v[h][k], both(iv)), high_halves(rw[2 * k], rw[2 * k + 1]));
+          const float2 im8 = add2(make_float2(copysignf(cm.x, mk.x), copysignf(cm.y, mk.y)), both(12582912.0f));
+          const float2 iv8 = add2(cv, both(12582912.0f));
+          qm[2 * k] = __float_as_uint(im8.x), qm[2 * k + 1] = __float_as_uint(im8.y);
+          qv[2 * k] = __float_as_uint(iv8.x), qv[2 * k + 1] = __float_as_uint(iv8.y);
         }
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<int8_t*>(a.m) + e + 128 * h) = pack_bytes(qm[0], qm[1], qm[2], qm[3]);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.v) + e + 128 * h) = pack_bytes(qv[0], qv[1], qv[2], qv[3]);
       }
-      *reinterpret_cast<uint2*>(reinterpret_cast<int8_t*>(a.m) + e) =
-          make_uint2(pack_bytes(qm[0], qm[1], qm[2], qm[3]), pack_bytes(qm[4], qm[5], qm[6], qm[7]));
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.v) + e) =
-          make_uint2(pack_bytes(qv[0], qv[1], qv[2], qv[3]), pack_bytes(qv[4], qv[5], qv[6], qv[7]));
       if ((threadIdx.x & 31) == 0) {
         a.m_scale[e >> 8] = top_m;
         a.v_scale[e >> 8] = top_v;
@@ -282,24 +352,37 @@ __global__ void __launch_bounds__(kAdamThreads)
   }
 }
 
+// Values of codes: four elements per thread and step, four steps of 1024 elements on their way.
 __global__ void __launch_bounds__(256)
     k_adamw_values(const int8_t* __restrict__ m, const uint8_t* __restrict__ v, const float* __restrict__ m_scale,
                    const float* __restrict__ v_scale, int64_t elements, float* __restrict__ mf, float* __restrict__ vf) {
-  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; e < elements; e += (int64_t)gridDim.x * 2048) {
-    const uint2 mc = *reinterpret_cast<const uint2*>(m + e), vc = *reinterpret_cast<const uint2*>(v + e);
-    const float um = __fmul_rn(m_scale[e >> 8], 1.0f / 16129.0f), uv = __fmul_rn(v_scale[e >> 8], 1.0f / 4228250625.0f);
-    const uint32_t mw[2] = {mc.x ^ 0x80808080u, mc.y ^ 0x80808080u}, vw[2] = {vc.x, vc.y};
+  for (int64_t base = (int64_t)blockIdx.x * 4096; base < elements; base += (int64_t)gridDim.x * 4096) {
+    uint32_t mc[4], vc[4];
+    float um[4], uv[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x[4], y[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float c8 = __fsub_rn(byte_f32(mw[h], k), 128.0f);
-        x[k] = __fmul_rn(__fmul_rn(c8, fabsf(c8)), um);
-        y[k] = __fmul_rn(fourth(byte_f32(vw[h], k)), uv);
+    for (int s = 0; s < 4; ++s) {
+      const int64_t e = base + s * 1024 + 4 * threadIdx.x;
+      if (e < elements) {
+        mc[s] = __ldg(reinterpret_cast<const uint32_t*>(m + e)) ^ 0x80808080u;
+        vc[s] = __ldg(reinterpret_cast<const uint32_t*>(v + e));
+        um[s] = __ldg(m_scale + (e >> 8)), uv[s] = __ldg(v_scale + (e >> 8));
       }
-      reinterpret_cast<float4*>(mf + e)[h] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4*>(vf + e)[h] = make_float4(y[0], y[1], y[2], y[3]);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int64_t e = base + s * 1024 + 4 * threadIdx.x;
+      if (e < elements) {
+        const float x1 = __fmul_rn(um[s], 1.0f / 16129.0f), y1 = __fmul_rn(uv[s], 1.0f / 4228250625.0f);
+        float x[4], y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float c8 = __fsub_rn(byte_high(mc[s], k), 8388736.0f);
+          x[k] = __fmul_rn(__fmul_rn(c8, fabsf(c8)), x1);
+          y[k] = __fmul_rn(fourth(__fsub_rn(byte_high(vc[s], k), 8388608.0f)), y1);
+        }
+        *reinterpret_cast<float4*>(mf + e) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(vf + e) = make_float4(y[0], y[1], y[2], y[3]);
+      }
     }
   }
 }
@@ -342,8 +425,8 @@ extern "C" int tthrml_adamw_step(const tthrml_adamw_tensor* tensors_host, int64_
     set_error("tthrml_adamw_step: state_bits must be 8 or 32 (got %d)", (int)state_bits);
     return TTHRML_ERR_ARG;
   }
-  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0) || !(weight_decay >= 0.0)) {
-    set_error("tthrml_adamw_step: betas must lie in [0, 1), eps above 0 and weight_decay not below 0");
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-30) || !(weight_decay >= 0.0)) {
+    set_error("tthrml_adamw_step: betas must lie in [0, 1), eps be at least 1e-30 and weight_decay not below 0");
     return TTHRML_ERR_ARG;
   }
   if (n_tensors < 0 || (uintptr_t)exp_avg % 16 || (uintptr_t)exp_avg_sq % 16) {
@@ -371,6 +454,7 @@ extern "C" int tthrml_adamw_step(const tthrml_adamw_tensor* tensors_host, int64_
   a.b2 = (float)beta2;
   a.d2 = (float)(1.0 - beta2);
   a.eps = (float)eps;
+  a.minus_zero = -0.0f;
   a.beta1 = beta1;
   a.beta2 = beta2;
   a.weight_decay = weight_decay;
@@ -409,8 +493,8 @@ extern "C" int tthrml_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg
               (long long)elements);
     return TTHRML_ERR_ARG;
   }
-  const int64_t blocks = (elements + 2047) / 2048;
-  k_adamw_values<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, (cudaStream_t)stream>>>(
+  const int64_t blocks = (elements + 4095) / 4096;
+  k_adamw_values<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, (cudaStream_t)stream>>>(
       exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, elements, exp_avg_out, exp_avg_sq_out);
   return launch_status("k_adamw_values launch");
 }

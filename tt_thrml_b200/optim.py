@@ -76,8 +76,8 @@ class AdamW:
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"betas must lie in [0, 1), got {betas!r}")
-        if not eps > 0.0 or not weight_decay >= 0.0 or not lr >= 0.0:
-            raise ValueError("eps must be above 0, lr and weight_decay not below 0")
+        if not eps >= 1e-30 or not weight_decay >= 0.0 or not lr >= 0.0:
+            raise ValueError("eps must be at least 1e-30, lr and weight_decay not below 0")
         self.device, self.betas, self.eps, self.weight_decay = dev, tuple(map(float, betas)), float(eps), float(weight_decay)
         self.state_bits, self.seed = int(state_bits), int(seed) & 0xFFFFFFFFFFFFFFFF
         # segment of each parameter in the moments
