@@ -140,6 +140,11 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float rcp_approx(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -179,12 +184,15 @@ __device__ __noinline__ float2 place_v(float y, float k) {  // (k, y - k^4)
   return make_float2(k, __fsub_rn(y, fourth(k)));
 }
 
+// Whether a remainder lies outside [0, span): a negative one is the larger unsigned integer.
+__device__ __forceinline__ bool outside(float over, float span) { return __float_as_uint(over) >= __float_as_uint(span); }
+
 // Codes of y = |m| 127^2 / max|m|: the largest k with k^2 <= y, or k + 1 with probability (y - k^2) / (2 k + 1).  u65536 is
 // 65536 times the uniform; the scaling by powers of two is exact.
 __device__ __forceinline__ float2 codes_m(float2 y, float2 u65536) {
   float2 k = floor2(make_float2(sqrt_approx(y.x), sqrt_approx(y.y)));
   float2 over = __ffma2_rn(neg2(k), k, y), span = __ffma2_rn(k, both(2.0f), both(1.0f));  // k^2 and 2 k + 1 are exact
-  if (over.x < 0.0f || over.x >= span.x || over.y < 0.0f || over.y >= span.y) {
+  if (outside(over.x, span.x) || outside(over.y, span.y)) {
     const float2 a = place_m(y.x, k.x), b = place_m(y.y, k.y);
     k = make_float2(a.x, b.x);
     over = make_float2(a.y, b.y);
@@ -197,18 +205,17 @@ __device__ __forceinline__ float2 codes_m(float2 y, float2 u65536) {
 __device__ __forceinline__ float2 codes_v(float2 y, float2 u65536) {
   float2 k = floor2(make_float2(sqrt_approx(sqrt_approx(y.x)), sqrt_approx(sqrt_approx(y.y))));
   float2 n = add2(k, both(1.0f)), k4 = fourth2(k), n4 = fourth2(n), over = add2(y, neg2(k4));
-  if (over.x < 0.0f || n4.x <= y.x || over.y < 0.0f || n4.y <= y.y) {
+  float2 span = add2(n4, neg2(k4));
+  if (outside(over.x, span.x) || outside(over.y, span.y)) {
     const float2 a = place_v(y.x, k.x), b = place_v(y.y, k.y);
     k = make_float2(a.x, b.x);
     over = make_float2(a.y, b.y);
     n = add2(k, both(1.0f));
-    k4 = fourth2(k);
-    n4 = fourth2(n);
+    span = add2(fourth2(n), neg2(fourth2(k)));
   }
-  const float2 t = mul2(u65536, add2(n4, neg2(k4))), o = mul2(over, both(65536.0f));
-  const float qx = t.x < o.x ? n.x : k.x, qy = t.y < o.y ? n.y : k.y;
-  // k = 0 is below 1 and y > 0: code 1
-  return make_float2(fminf(y.x > 0.0f ? fmaxf(qx, 1.0f) : qx, 255.0f), fminf(y.y > 0.0f ? fmaxf(qy, 1.0f) : qy, 255.0f));
+  // k = 0 takes no chances: 1 wherever y > 0
+  const float2 t = mul2(mul2(u65536, span), make_float2(fminf(k.x, 1.0f), fminf(k.y, 1.0f))), o = mul2(over, both(65536.0f));
+  return make_float2(fminf(t.x < o.x ? n.x : k.x, 255.0f), fminf(t.y < o.y ? n.y : k.y, 255.0f));
 }
 // The low bytes of four words (the integers held by floats in -2^22 .. 2^22 plus 3 2^22).
 __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -222,26 +229,26 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
   const int chunks = tab.first_chunk[a.n_tensors];
   const int c_first = (int)((int64_t)chunks * blockIdx.x / gridDim.x);
   const int c_last = (int)((int64_t)chunks * (blockIdx.x + 1) / gridDim.x);
-  const int64_t step = a.ctl->step + 1;
-  if (threadIdx.x == 0) {
-    const double lr = a.ctl->lr, t = (double)step;
-    coef[0] = (float)(lr / (1.0 - pow(a.beta1, t)));
-    coef[1] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, t)));
-    coef[2] = (float)(1.0 - lr * a.weight_decay);
-  }
-  __syncthreads();
-  const float step_size = coef[0], r_bias2 = coef[1], keep = coef[2];
-  const PhiloxKeys keys = philox_keys((uint32_t)a.seed, (uint32_t)(a.seed >> 32));
   int ti = 0;
   for (int lo = 0, hi = a.n_tensors; hi - lo > 1;) {  // the tensor of the first chunk
     const int mid = (lo + hi) >> 1;
     (tab.first_chunk[mid] <= c_first ? lo : hi) = mid;
     ti = lo;
   }
+  const int place = 256 * (threadIdx.x >> 5) + 4 * (threadIdx.x & 31);
+  const int64_t step = a.ctl->step + 1;
+  // the coefficients in double, a warp each; every warp passes the barrier once, after its first loads are on their way
+  if (threadIdx.x == 0) coef[0] = (float)(a.ctl->lr / (1.0 - pow(a.beta1, (double)step)));
+  if (threadIdx.x == 32) coef[1] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)step)));
+  if (threadIdx.x == 64) coef[2] = (float)(1.0 - a.ctl->lr * a.weight_decay);
+  const auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kAdamThreads) : "memory"); };
+  bool ready = false;
+  float step_size = 0.0f, r_bias2 = 0.0f, keep = 0.0f;
+  const PhiloxKeys keys = philox_keys((uint32_t)a.seed, (uint32_t)(a.seed >> 32));
   for (int c = c_first; c < c_last; ++c) {
     while (tab.first_chunk[ti + 1] <= c) ++ti;
     const tthrml_adamw_tensor& t = tab.t[ti];
-    const int64_t i = (int64_t)(c - tab.first_chunk[ti]) * kChunk + 256 * (threadIdx.x >> 5) + 4 * (threadIdx.x & 31);
+    const int64_t i = (int64_t)(c - tab.first_chunk[ti]) * kChunk + place;
     if (i - 4 * (threadIdx.x & 31) >= t.n) continue;  // whole warps
     const int64_t e = t.state + i;  // this thread's groups: e .. e + 3 and e + 128 .. e + 131
     const bool pv = (uintptr_t)t.param % (t.param_dtype == TTHRML_DT_F32 ? 16 : 8) == 0;
@@ -268,7 +275,12 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
       um = __fmul_rn(a.m_scale[e >> 8], 1.0f / 16129.0f);
       uv = __fmul_rn(a.v_scale[e >> 8], 1.0f / 4228250625.0f);
     }
-    uint32_t tm = 0u, tv = 0u;
+    if (!ready) {
+      barrier();
+      step_size = coef[0], r_bias2 = coef[1], keep = coef[2];
+      ready = true;
+    }
+    float tm = 0.0f, tv = 0.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       convert(t.grad_dtype, gr[h], g[h]);
@@ -294,8 +306,8 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
           // step on codes is bound by its instructions
           const float2 denom = add2(mul2(make_float2(sqrt_approx(vk.x), sqrt_approx(vk.y)), both(r_bias2)), both(a.eps));
           upd = mul2(mk, make_float2(rcp_approx(denom.x), rcp_approx(denom.y)));
-          tm = max(tm, max(abs_bits(mk.x), abs_bits(mk.y)));
-          tv = max(tv, max(__float_as_uint(vk.x) & 0x7FFFFFFFu, __float_as_uint(vk.y) & 0x7FFFFFFFu));
+          tm = max_nan(max_nan(tm, fabsf(mk.x)), fabsf(mk.y));
+          tv = max_nan(max_nan(tv, vk.x), vk.y);
         }
         p[h][k] = add2(mul2(p[h][k], both(keep)), neg2(mul2(upd, both(step_size))));
       }
@@ -308,10 +320,9 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
       }
     }
     if (BITS == 8) {
-      tm = __reduce_max_sync(0xffffffffu, tm);
-      tv = __reduce_max_sync(0xffffffffu, tv);
-      float top_m = __uint_as_float(tm), top_v = __uint_as_float(tv);
-      const bool finite = tm < 0x7F800000u && tv < 0x7F800000u;
+      const uint32_t bm = __reduce_max_sync(0xffffffffu, abs_bits(tm)), bv = __reduce_max_sync(0xffffffffu, abs_bits(tv));
+      float top_m = __uint_as_float(bm), top_v = __uint_as_float(bv);
+      const bool finite = bm < 0x7F800000u && bv < 0x7F800000u;
       if (!finite) top_m = top_v = __uint_as_float(0x7FC00000u);
       if (top_v < 8.0779356694631609e-28f) top_v = 0.0f;                  // 2^-90
       if (top_v == 0.0f || top_m < 7.8886090522101181e-31f) top_m = 0.0f;  // 2^-100
@@ -342,6 +353,7 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
       }
     }
   }
+  if (!ready) barrier();
   __syncthreads();
   if (threadIdx.x == 0 && a.last) {
     __threadfence();
