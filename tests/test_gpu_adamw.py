@@ -155,6 +155,25 @@ def test_coded_moments_bit_for_bit(tt, ptype, gtype, seed):
             assert ((q.cpu().double() - want[0]).abs() <= tol[0]).all()
 
 
+def test_many_coded_moments_bit_for_bit(tt):
+    """Rare ties between a random word and a remainder: three million codes of each kind, twice."""
+    n, f, (b1, b2) = 3_000_000, np.float32, HYPER["betas"]
+    p = torch.zeros(n, device="cuda")
+    opt = tt.AdamW([p], state_bits=8, seed=77, **HYPER)
+    names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+    for t in (1, 2):
+        g = rand((n,), F32, t)
+        st = opt.state_dict()
+        opt.step([g.cuda()])
+        now = opt.state_dict()
+        m, v = plain_values(*(st[k].cpu().numpy() for k in names))
+        flat = np.zeros(opt.elements, f)
+        flat[:n] = g.numpy()
+        want = plain_codes(m * f(b1) + flat * f(1 - b1), v * f(b2) + (flat * flat) * f(1 - b2), t, 77)
+        for name, w in zip(names, want):
+            assert np.array_equal(now[name].cpu().numpy(), w), name
+
+
 def test_coded_moments_keep_their_mean(tt):
     """Averages whose step is far below a code's step still follow: constant gradients of several sizes in one block,
     v and m against their closed forms.  The mean over n equal elements of a value rounded at random, t times,

@@ -167,9 +167,9 @@ __device__ __forceinline__ float fourth(float k) {
   const float k2 = __fmul_rn(k, k);
   return __fmul_rn(k2, k2);
 }
-__device__ __forceinline__ float2 fourth2(float2 k) {
+__device__ __forceinline__ float2 fourth2(float2 k, float minus_zero) {  // k^2 is exact, k^4 rounds
   const float2 k2 = mul2(k, k);
-  return mul2(k2, k2);
+  return product2(k2, k2, minus_zero);
 }
 
 // The approximate roots are off by one only next to a whole number: the place of y among the squares (fourth powers) again.
@@ -202,16 +202,16 @@ __device__ __forceinline__ float2 codes_m(float2 y, float2 u65536) {
   return make_float2(fminf(t.x < o.x ? n.x : k.x, 127.0f), fminf(t.y < o.y ? n.y : k.y, 127.0f));
 }
 // Codes of y = v 255^4 / max v, likewise with fourth powers; a y > 0 gets at least 1.
-__device__ __forceinline__ float2 codes_v(float2 y, float2 u65536) {
+__device__ __forceinline__ float2 codes_v(float2 y, float2 u65536, float minus_zero) {
   float2 k = floor2(make_float2(sqrt_approx(sqrt_approx(y.x)), sqrt_approx(sqrt_approx(y.y))));
-  float2 n = add2(k, both(1.0f)), k4 = fourth2(k), n4 = fourth2(n), over = add2(y, neg2(k4));
+  float2 n = add2(k, both(1.0f)), k4 = fourth2(k, minus_zero), n4 = fourth2(n, minus_zero), over = add2(y, neg2(k4));
   float2 span = add2(n4, neg2(k4));
   if (outside(over.x, span.x) || outside(over.y, span.y)) {
     const float2 a = place_v(y.x, k.x), b = place_v(y.y, k.y);
     k = make_float2(a.x, b.x);
     over = make_float2(a.y, b.y);
     n = add2(k, both(1.0f));
-    span = add2(fourth2(n), neg2(fourth2(k)));
+    span = add2(fourth2(n, minus_zero), neg2(fourth2(k, minus_zero)));
   }
   // k = 0 takes no chances: 1 wherever y > 0
   const float2 t = mul2(mul2(u65536, span), make_float2(fminf(k.x, 1.0f), fminf(k.y, 1.0f))), o = mul2(over, both(65536.0f));
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
           const float2 c8 = add2(make_float2(byte_high(mc[h], 2 * k), byte_high(mc[h], 2 * k + 1)), both(-8388736.0f));
           const float2 mag = mul2(mul2(c8, c8), both(um));
           m[h][k] = make_float2(copysignf(mag.x, c8.x), copysignf(mag.y, c8.y));
-          v[h][k] = mul2(fourth2(add2(make_float2(byte_high(vc[h], 2 * k), byte_high(vc[h], 2 * k + 1)), both(-8388608.0f))),
+          v[h][k] = mul2(fourth2(add2(make_float2(byte_high(vc[h], 2 * k), byte_high(vc[h], 2 * k + 1)), both(-8388608.0f)), a.minus_zero),
                          both(uv));
         }
         const float2 gk = g[h][k];
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
         for (int k = 0; k < 2; ++k) {
           const float2 mk = m[h][k], s = mul2(mk, both(im));
           const float2 cm = codes_m(make_float2(fabsf(s.x), fabsf(s.y)), low_halves(rw[2 * k], rw[2 * k + 1]));
-          const float2 cv = codes_v(mul2(v[h][k], both(iv)), high_halves(rw[2 * k], rw[2 * k + 1]));
+          const float2 cv = codes_v(product2(v[h][k], both(iv), a.minus_zero), high_halves(rw[2 * k], rw[2 * k + 1]), a.minus_zero);
           const float2 im8 = add2(make_float2(copysignf(cm.x, mk.x), copysignf(cm.y, mk.y)), both(12582912.0f));
           const float2 iv8 = add2(cv, both(12582912.0f));
           qm[2 * k] = __float_as_uint(im8.x), qm[2 * k + 1] = __float_as_uint(im8.y);
