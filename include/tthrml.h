@@ -554,7 +554,7 @@ int tthrml_moments_accumulate(const void* state_dev, int32_t state_dtype, int64_
 
 /*
  * Rows to 8-bit integers: scale[r] = max|x_r| * fl(1/127), values[r][c] =
- * rint(x[r][c] * fl(127 / max|x_r|)) clamped to +-127.  A row whose largest
+ * rint(x[r][c] * fl(127 / max|x_r|)), at most 127.  A row whose largest
  * magnitude is below 2^-120 gets zeros and scale 0; a row with an infinity or
  * NaN gets scale NaN.  x: element (r, c) at r * row_stride + c * col_stride
  * (element units; fast for col_stride 1 and for row_stride 1).  values:
@@ -564,6 +564,9 @@ int tthrml_moments_accumulate(const void* state_dev, int32_t state_dtype, int64_
 int tthrml_quantize_rows(const void* x_dev, int32_t dtype, int64_t rows, int64_t cols,
                          int64_t row_stride, int64_t col_stride, int8_t* values_dev, int64_t pitch,
                          float* scale_dev, void* stream);
+
+/* int8 to bfloat16, both 16-byte aligned. */
+int tthrml_widen_i8(const int8_t* values_dev, int64_t n, void* out_dev, void* stream);
 
 /*
  * out[m][n] = (sum_k x[m][k] * weights[n][k]) * (x_scale[m] * w_scale[n]) + bias[n]

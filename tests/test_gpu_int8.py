@@ -65,6 +65,11 @@ def test_quantize_rows_strides(tt, dtype):
     t = DTYPES[dtype]
     base = rand((70, 301), t, 3)
     d = base.cuda()
+    for shape in ((5000, 100), (4096, 70), (17, 40), (2000, 33)):  # transposed: long rows, an odd number of them
+        wide = rand(shape, t, shape[0])
+        r = tt.quantize_rows(wide.cuda().t())
+        q, s = plain_quantize(wide.t())
+        assert np.array_equal(r.values.cpu().numpy(), q) and np.array_equal(r.scale.cpu().numpy(), s)
     cases = [(base.t(), d.t()), (base[:, ::3], d[:, ::3]), (base[1::2, 5:], d[1::2, 5:]), (base[:, 1:130], d[:, 1:130]),
              (base[:1].expand(9, 301), d[:1].expand(9, 301)), (base[:, :1].expand(70, 40), d[:, :1].expand(70, 40)),
              (base.t()[:, 3:4], d.t()[:, 3:4])]

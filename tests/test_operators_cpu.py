@@ -61,6 +61,8 @@ BAD = [
     ("tthrml_quantize_rows", quantize(pitch=32), b"multiple of 16"),
     ("tthrml_quantize_rows", quantize(values=_M), b"16-byte aligned"),
     ("tthrml_quantize_rows", quantize(dtype=3), b"input type"),
+    ("tthrml_widen_i8", (_A, 5, _M, None), b"16-byte aligned"),
+    ("tthrml_widen_i8", (None, 5, _A, None), b"must be given"),
     ("tthrml_int8_product", product(err=None), b"NULL"),
     ("tthrml_int8_product", product(cols=131072, xp=131072, wp=131072), b"out of range"),
     ("tthrml_int8_product", product(rows=-1), b"out of range"),

@@ -212,6 +212,7 @@ _SIGNATURES = {
     "tthrml_encode_rows": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i32, c_i64, c_i64, c_vp, c_vp]),
     "tthrml_sum_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "tthrml_quantize_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "tthrml_widen_i8": (c_i32, [c_vp, c_i64, c_vp, c_vp]),
     "tthrml_int8_product": (
         c_i32,
         [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp, c_vp],

@@ -140,11 +140,6 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float rcp_approx(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -217,11 +212,6 @@ __device__ __forceinline__ float2 codes_v(float2 y, float2 u65536, float minus_z
   const float2 t = mul2(mul2(u65536, span), make_float2(fminf(k.x, 1.0f), fminf(k.y, 1.0f))), o = mul2(over, both(65536.0f));
   return make_float2(fminf(t.x < o.x ? n.x : k.x, 255.0f), fminf(t.y < o.y ? n.y : k.y, 255.0f));
 }
-// The low bytes of four words (the integers held by floats in -2^22 .. 2^22 plus 3 2^22).
-__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0040u), __byte_perm(c, d, 0x0040u), 0x5410u);
-}
-
 template <int BITS, int T>
 __global__ void __launch_bounds__(kAdamThreads, 4)
     k_adamw(const __grid_constant__ AdamTable<T> tab, const __grid_constant__ AdamArgs a) {
@@ -306,8 +296,8 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
           // step on codes is bound by its instructions
           const float2 denom = add2(mul2(make_float2(sqrt_approx(vk.x), sqrt_approx(vk.y)), both(r_bias2)), both(a.eps));
           upd = mul2(mk, make_float2(rcp_approx(denom.x), rcp_approx(denom.y)));
-          tm = max_nan(max_nan(tm, fabsf(mk.x)), fabsf(mk.y));
-          tv = max_nan(max_nan(tv, vk.x), vk.y);
+          tm = max_abs(max_abs(tm, mk.x), mk.y);
+          tv = max_abs(max_abs(tv, vk.x), vk.y);
         }
         p[h][k] = add2(mul2(p[h][k], both(keep)), neg2(mul2(upd, both(step_size))));
       }
@@ -344,8 +334,8 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
           qm[2 * k] = __float_as_uint(im8.x), qm[2 * k + 1] = __float_as_uint(im8.y);
           qv[2 * k] = __float_as_uint(iv8.x), qv[2 * k + 1] = __float_as_uint(iv8.y);
         }
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<int8_t*>(a.m) + e + 128 * h) = pack_bytes(qm[0], qm[1], qm[2], qm[3]);
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.v) + e + 128 * h) = pack_bytes(qv[0], qv[1], qv[2], qv[3]);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<int8_t*>(a.m) + e + 128 * h) = pack4(qm[0], qm[1], qm[2], qm[3]);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.v) + e + 128 * h) = pack4(qv[0], qv[1], qv[2], qv[3]);
       }
       if ((threadIdx.x & 31) == 0) {
         a.m_scale[e >> 8] = top_m;

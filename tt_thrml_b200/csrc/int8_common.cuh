@@ -1,5 +1,5 @@
 // Element types of the operators' inputs and outputs, and the quantisation of a row to 8-bit integers:
-//     scale = max|x| * fl(1/127),   q = rint(x * fl(127 / max|x|)) clamped to +-127.
+//     scale = max|x| * fl(1/127),   q = rint(x * fl(127 / max|x|)).
 // A row whose largest magnitude is below 2^-120 (127 / max|x| would overflow) is held as zeros with scale 0; a
 // row that holds an infinity or a NaN gets the scale NaN, so every value computed from it is NaN.
 #pragma once
@@ -65,13 +65,27 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits) {
   }
   return r;
 }
-// NaN times inv = 0 stays NaN; its conversion gives 0.
-__device__ __forceinline__ int32_t quantize(float x, float inv) {
-  const int32_t q = __float2int_rn(__fmul_rn(x, inv));
-  return max(-127, min(127, q));
+// rint(x inv) in the low byte of a word: |x| <= max|x| makes |x inv| at most 127 (1 + 2^-23), so no clamp is needed, and 3 2^22
+// added rounds to the nearest integer, ties to even.  (A row that is not finite has inv = 0 and may get any byte: its
+// scale is NaN.)
+__device__ __forceinline__ uint32_t quantize_low(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
 }
-__device__ __forceinline__ uint32_t pack4(int32_t a, int32_t b, int32_t c, int32_t d) {
-  return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)d << 24);
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040u), __byte_perm(c, d, 0x0040u), 0x5410u);
+}
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float inv) {
+  uint32_t q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = quantize_low(f[i], inv);
+  return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+}
+// The larger of a maximum and the magnitude of v, NaN if either is.
+__device__ __forceinline__ float max_abs(float top, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
+  return r;
 }
 
 inline int64_t dtype_bytes(int32_t dtype) {

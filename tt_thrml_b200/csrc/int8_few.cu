@@ -57,7 +57,7 @@ __device__ __forceinline__ void quantize_into(const FewArgs& a, int8_t* xs, int 
   const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)(m < a.M ? m : 0) * a.x_ld;
   const bool vectors = (uintptr_t)xr % 16 == 0;
   const int K = m < a.M ? a.K : 0;
-  uint32_t top = 0u;
+  float most = 0.0f;
   for (int c = 8 * t; c < K; c += 256 * kGroup) {
     float f[8];
     if (vectors && c + 8 <= K) {
@@ -67,9 +67,9 @@ __device__ __forceinline__ void quantize_into(const FewArgs& a, int8_t* xs, int 
       for (int i = 0; i < 8; ++i) f[i] = c + i < K ? to_f32(xr[c + i]) : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
+    for (int i = 0; i < 8; ++i) most = max_abs(most, f[i]);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most));
   if (lane == 0) part[warp] = top;
   __syncthreads();
 #pragma unroll
@@ -84,10 +84,7 @@ __device__ __forceinline__ void quantize_into(const FewArgs& a, int8_t* xs, int 
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = c + i < K ? to_f32(xr[c + i]) : 0.0f;
     }
-    int32_t q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = quantize(f[i], s.inv);
-    *reinterpret_cast<uint2*>(xs + m * kp + c) = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+    *reinterpret_cast<uint2*>(xs + m * kp + c) = quantize8(f, s.inv);
   }
 }
 

@@ -168,20 +168,25 @@ struct ClusterFit {
 };
 inline int cluster_fit(const void* fn, unsigned cluster, unsigned threads, int smem, ClusterFit* out) {
   static std::mutex mu;
-  static std::map<std::tuple<int, const void*, unsigned>, ClusterFit> known;
+  static std::map<std::tuple<int, const void*, unsigned, int>, ClusterFit> known;
+  static std::map<std::pair<int, const void*>, int> limits;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "cudaGetDevice");
   std::lock_guard<std::mutex> lock(mu);
-  const auto key = std::make_tuple(dev, fn, cluster);
+  const auto key = std::make_tuple(dev, fn, cluster, smem);
   const auto it = known.find(key);
   if (it != known.end()) {
     *out = it->second;
     return TTHRML_OK;
   }
   ClusterFit f = {0, 0};
+  int& limit = limits[std::make_pair(dev, fn)];  // never lowered: earlier launches may have needed more
   e = cudaDeviceGetAttribute(&f.sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && smem > limit) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) limit = smem;
+  }
   if (e != cudaSuccess) return cuda_status(e, "kernel attributes");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

@@ -1082,6 +1082,21 @@ class Executor:
                     plan.bias.copy_(bias)
         current.wait_stream(self._stream)
 
+    def share_dense_weights(self, other: "Executor") -> None:
+        """Runs this executor's sweeps on another one's operands (weights and biases) from now on: what
+        update_dense_weights writes there holds here too.  Both need the same program shape, precision, device and
+        stream (executors made from one opened device share its stream)."""
+        mine, theirs = self._dense_plans("share_dense_weights"), other._dense_plans("share_dense_weights")
+        if self._stream != other._stream:
+            raise ValueError("executors on different streams cannot share their weights")
+        for p, q in zip(mine, theirs):
+            if p.weights_nk.shape != q.weights_nk.shape or p.weights_nk.dtype != q.weights_nk.dtype or p.family != q.family:
+                raise ValueError("executors of different programs or precisions cannot share their weights")
+        for p, q in zip(mine, theirs):
+            if p.weights_nk is not q.weights_nk or p.bias is not q.bias:
+                p.weights_nk, p.w_scale, p.bias, p.owned = q.weights_nk, q.w_scale, q.bias, q.owned
+                self._graphs.clear()
+
     def _dense_phases(self, scale: float) -> list:
         """The current states as terms of pair moments: (x, x pitch, y, y pitch, scale, x scale, y scale), 16-bit
         tensors.  A value held in several pieces is a sum over them; products of two remainders below the third
@@ -1098,7 +1113,13 @@ class Executor:
                     copies = self.__dict__.setdefault("_moment_copies", {})
                     if bi not in copies:
                         copies[bi] = torch.empty(state.shape, dtype=torch.bfloat16, device=self._tdev)
-                    state = copies[bi].copy_(state)
+                    nat.bind_device(self._tdev.index)
+                    nat.check(
+                        self._lib.tthrml_widen_i8(state.data_ptr(), state.numel(), copies[bi].data_ptr(),
+                                                  nat.stream_handle(self._stream)),
+                        "tthrml_widen_i8",
+                    )
+                    state = copies[bi]
                 n, p = self.compiled.blocks[bi].spec.n_nodes, self._dense_pieces[bi]
                 # spins have zero remainders
                 spin = self.compiled.blocks[bi].spec.family == Family.SPIN

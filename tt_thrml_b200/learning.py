@@ -9,7 +9,7 @@ takes those differences from the states of executors on the device,
 from __future__ import annotations
 
 from . import _native as nat
-from .core import Family, make_cuda_config
+from .core import Family, make_cuda_config, open_device
 from .executor import Executor
 from .moments import launch
 from .optim import AdamW
@@ -90,6 +90,8 @@ class DenseLearner:
             raise ValueError("DenseLearner draws on the device: rng_mode must be 'philox'")
         if int(sweeps) < 1:
             raise ValueError(f"sweeps must be at least 1, got {sweeps}")
+        if device is None:  # both samplers on one stream
+            device = open_device(None, device_id=torch.cuda.current_device())
         self.program, self.sweeps = program, int(sweeps)
         self.data = Executor(None, device, program, config, n_chains=int(n_data))
         self.model = Executor(None, device, program, config, n_chains=int(n_chains))
@@ -141,8 +143,8 @@ class DenseLearner:
         model.run_sweeps(self.sweeps)
         dense_moments([(data, -1.0 / n), (model, 1.0 / model.n_chains)], out=self.gradient)
         self.optimizer.step(self.gradient)
-        for ex in (data, model):
-            ex.update_dense_weights(self.weights, self.visible_bias, self.hidden_bias)
+        data.update_dense_weights(self.weights, self.visible_bias, self.hidden_bias)
+        model.share_dense_weights(data)
         return self.gradient
 
 
