@@ -6,6 +6,8 @@ import numpy as np
 import pytest
 import torch
 
+from tt_thrml_b200 import _native as nat
+
 pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -250,7 +252,7 @@ def test_replayed_graph_counts_on_and_follows_lr(tt, bits):
         opt.step(grads)
         if capture:
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
+            with nat.capturing(graph):
                 opt.step(grads)
         for k in range(6):
             if k == 3:

@@ -1,6 +1,7 @@
 """Dense sweeps on 8-bit operands (dense_precision="int8"), replaced couplings, dense moments and the learner."""
 
 import ctypes
+import gc
 
 import numpy as np
 import pytest
@@ -205,6 +206,28 @@ def test_graphs_checkpoints_and_readback(spin_visible, tmp_path):
     e = Executor(None, None, program, make_cuda_config(n_chains=C), n_sweeps=8)
     with pytest.raises(ValueError):
         e.restore(c.checkpoint())
+
+
+def test_a_capture_outlives_the_garbage_collector():
+    """A CUDA graph in a reference cycle that becomes garbage before another capture is not freed within it."""
+    ex = int8_executor(rbm(), 128)
+    ex.load_state([np.zeros((128, 256), F), np.ones((128, 512), bool)], [])
+    ex.prepare_rng(1)
+    graph = torch.cuda.CUDAGraph()
+    held = torch.zeros(8, device="cuda")
+    with nat.capturing(graph):
+        held.add_(1)
+    cycle = [graph]
+    cycle.append(cycle)
+    del graph, cycle
+    limits = gc.get_threshold()
+    gc.set_threshold(1)  # collect at every chance
+    try:
+        ex.run_sweeps(4)
+    finally:
+        gc.set_threshold(*limits)
+    ex.check_device_errors()
+    assert gc.isenabled()
 
 
 @pytest.mark.parametrize("precision", ["bf16", "fp32", "int8"])

@@ -4,6 +4,8 @@ import numpy as np
 import pytest
 import torch
 
+from tt_thrml_b200 import _native as nat
+
 pytestmark = pytest.mark.gpu
 
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
@@ -192,7 +194,7 @@ def test_captured_products_on_two_streams_and_graphs(tt, rows):
     graphs, outs = [], []
     for x in held:
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with nat.capturing(g):
             outs.append(tt.int8_product(x, r))
         graphs.append(g)
     torch.cuda.synchronize()

@@ -3,6 +3,8 @@
 import pytest
 import torch
 
+from tt_thrml_b200 import _native as nat
+
 pytestmark = pytest.mark.gpu
 
 BF16, F16 = torch.bfloat16, torch.float16
@@ -171,7 +173,7 @@ def test_two_captured_graphs_on_two_streams(tt):
     graphs, outs = [], []
     for x, y in held:
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with nat.capturing(g):
             outs.append(tt.pair_moments(x, y, 0.5, units=True))
         graphs.append(g)
     torch.cuda.synchronize()

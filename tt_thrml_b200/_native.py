@@ -7,6 +7,7 @@ C layouts field for field.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -327,6 +328,24 @@ def ptr(t) -> int | None:
 
 def stream_handle(stream) -> int | None:
     return None if stream is None else stream.cuda_stream
+
+
+@contextlib.contextmanager
+def capturing(graph, stream=None):
+    """torch.cuda.graph with the cyclic garbage collector paused: a CUDA graph that it frees meanwhile (one held by a
+    reference cycle) would end the capture with an error."""
+    import gc
+
+    import torch
+
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            yield
+    finally:
+        if was:
+            gc.enable()
 
 
 _bound = threading.local()

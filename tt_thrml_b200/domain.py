@@ -510,7 +510,7 @@ class LatticeStrips:
         if g is None:
             g = torch.cuda.CUDAGraph()
             self._stream.synchronize()
-            with torch.cuda.graph(g, stream=self._stream):
+            with nat.capturing(g, self._stream):
                 s = torch.cuda.current_stream(self.device)
                 for j in range(n_periods):
                     self._period(j * per, s, self._ctl.data_ptr())

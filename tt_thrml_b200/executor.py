@@ -397,7 +397,7 @@ class Executor:
             nat.bind_device(self._tdev.index)
             g = torch.cuda.CUDAGraph()
             self._stream.synchronize()
-            with torch.cuda.graph(g, stream=self._stream):
+            with nat.capturing(g, self._stream):
                 for k in range(n):
                     for group in self.compiled.sampling_groups:
                         self._run_sampling_group(group, k, capturing=True)
@@ -466,7 +466,7 @@ class Executor:
             nat.bind_device(self._tdev.index)
             g = torch.cuda.CUDAGraph()
             self._stream.synchronize()
-            with torch.cuda.graph(g, stream=self._stream):
+            with nat.capturing(g, self._stream):
                 s = torch.cuda.current_stream(self._tdev)
                 k = 0
                 for _ in range(n_w):
