@@ -88,13 +88,14 @@ __device__ __forceinline__ void quantize_into(const FewArgs& a, int8_t* xs, int 
   }
 }
 
-// Each warp walks over units, a unit of the weights at a time, kVecs 16-byte vectors per lane and step (a row of 4096
-// weights); the next step's vectors are on their way while the current ones are multiplied, so two CTAs of eight warps
-// keep 128 KB of weights on their way to an SM.
-constexpr int kVecs = 8;
+// Each warp walks over units, a unit of the weights at a time, kVecs 16-byte vectors per lane and step; the next step's
+// vectors are on their way while the current ones are multiplied, so four CTAs of eight warps keep 64 KB of weights on
+// their way to an SM.  33.5 M weights and one row took 9.0 us so, 10.4 us with two CTAs and eight vectors, 9.8 and 10.1 us
+// with three and five CTAs of four vectors, 11.5 us with six of two.
+constexpr int kVecs = 4, kFewCtas = 4;
 
 template <typename T, int MP>
-__global__ void __launch_bounds__(kFewThreads, 2) k_int8_few(FewArgs a) {
+__global__ void __launch_bounds__(kFewThreads, kFewCtas) k_int8_few(FewArgs a) {
   extern __shared__ __align__(16) int8_t xs[];
   __shared__ float sxs[8];
   __shared__ uint32_t part[8];
@@ -173,7 +174,8 @@ int launch_few(const FewArgs& a, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return cuda_status(e, "tthrml_int8_product_few: device query");
-  const int64_t want = (a.N + kFewWarps - 1) / kFewWarps, most = (int64_t)sms * (smem <= 100 * 1024 ? 2 : 1);
+  const int64_t want = (a.N + kFewWarps - 1) / kFewWarps, fit = 224 * 1024 / (smem + 2048);
+  const int64_t most = (int64_t)sms * (fit < 1 ? 1 : (fit > kFewCtas ? kFewCtas : fit));
   const int64_t grid = want < most ? want : most;
   if (smem > 48 * 1024) {  // a per-device attribute of the function; setting it again is cheap
     e = cudaFuncSetAttribute(k_int8_few<T, MP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemMax);
