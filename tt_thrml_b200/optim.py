@@ -62,10 +62,11 @@ class AdamW:
             raise ValueError("AdamW needs at least one parameter")
         dev = getattr(self.params[0], "device", None)
         for i, p in enumerate(self.params):
-            require_cuda(f"parameter {i}", p, dev)
+            if not (isinstance(p, torch.Tensor) and p.is_cuda and p.device == dev):
+                require_cuda(f"parameter {i}", p, dev)
             if dtype_code(p.dtype) is None:
                 raise ValueError(f"parameter {i} must be float32, bfloat16 or float16, got {p.dtype}")
-            if _dense_order(p) is None:
+            if not p.is_contiguous() and _dense_order(p) is None:
                 raise ValueError(f"parameter {i} has gaps or overlaps in memory (strides {tuple(p.stride())})")
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i)
                        for i, p in enumerate(self.params) if p.numel())
