@@ -717,6 +717,13 @@ int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32_t n_phases
                         float* x_sum_dev, float* y_sum_dev, int32_t accumulate, int32_t* error_dev,
                         void* stream);
 
+/* tthrml_pack_rows and tthrml_pair_moments on its targets, whose start overlaps the packing. */
+int tthrml_pair_moments_packed(const tthrml_pack_matrix* matrices_host, int32_t n_matrices,
+                               const tthrml_moment_phase* phases_host, int32_t n_phases, int32_t dtype,
+                               int64_t x_units, int64_t y_units, float* out_dev, int64_t out_ld,
+                               float* x_sum_dev, float* y_sum_dev, int32_t accumulate,
+                               int32_t* error_dev, void* stream);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

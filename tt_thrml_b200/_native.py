@@ -240,6 +240,10 @@ _SIGNATURES = {
     ),
     "tthrml_adamw_values": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
     "tthrml_pack_rows": (c_i32, [c_vp, c_i32, c_vp]),
+    "tthrml_pair_moments_packed": (
+        c_i32,
+        [c_vp, c_i32, c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp],
+    ),
     "tthrml_pair_moments": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),

@@ -81,7 +81,7 @@ bool wants_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.r
 
 using LinearFn = decltype(&tthrml_int8_linear);
 using MomentsFn = decltype(&tthrml_pair_moments);
-using PackFn = decltype(&tthrml_pack_rows);
+using PackedMomentsFn = decltype(&tthrml_pair_moments_packed);
 
 // int8_product(x, weights, weight scales, pitch, bias or None, function, error word, stream, device) -> the product in x's
 // type, an error code, or None.
@@ -131,7 +131,7 @@ PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
-// pair_moments(xs, ys, scales, units, function, pack function, error word, stream, device) -> the moments (with `units` a
+// pair_moments(xs, ys, scales, units, function, its form for packed operands, error word, stream, device) -> the moments (with `units` a
 // triple), an error code, or None.
 PyObject* pair_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 9 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !PyList_Check(args[2])) Py_RETURN_NONE;
@@ -192,12 +192,14 @@ PyObject* pair_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         packed[i].dst = base + reinterpret_cast<uintptr_t>(packed[i].dst);
         *packed_into[i] = packed[i].dst;
       }
-      rc = address<PackFn>(args[5])(packed, n_packed, stream);
     }
-    if (!rc)
-      rc = address<MomentsFn>(args[4])(phases, (int32_t)n, code, M, N, out.mutable_data_ptr<float>(), N,
-                                       units ? xs.mutable_data_ptr<float>() : nullptr,
-                                       units ? ys.mutable_data_ptr<float>() : nullptr, 0, address<int32_t*>(args[6]), stream);
+    float *o = out.mutable_data_ptr<float>(), *xo = units ? xs.mutable_data_ptr<float>() : nullptr,
+          *yo = units ? ys.mutable_data_ptr<float>() : nullptr;
+    int32_t* error = address<int32_t*>(args[6]);
+    if (n_packed)
+      rc = address<PackedMomentsFn>(args[5])(packed, n_packed, phases, (int32_t)n, code, M, N, o, N, xo, yo, 0, error, stream);
+    else
+      rc = address<MomentsFn>(args[4])(phases, (int32_t)n, code, M, N, o, N, xo, yo, 0, error, stream);
     if (rc) return PyLong_FromLong(rc);
     if (!units) return THPVariable_Wrap(out);
     PyObject *a = THPVariable_Wrap(out), *b = THPVariable_Wrap(xs), *c = THPVariable_Wrap(ys);

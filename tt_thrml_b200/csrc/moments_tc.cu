@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   if ((int)blockIdx.x >= a.tile_blocks) {  // whole clusters: the tile blocks are a multiple of the cluster size
+    wait_for_previous_kernel();
     const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks;
     for (int s = (int)blockIdx.x - a.tile_blocks; s < strips; s += others)
       unit_sums<kMomentThreads>(a, s, (int)threadIdx.x, 1, reinterpret_cast<float*>(tiles));
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  wait_for_previous_kernel();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -424,6 +426,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
   float* side = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);
   if ((int)blockIdx.x >= a.tile_blocks) {  // whole clusters
+    wait_for_previous_kernel();
     const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks;
     for (int s = (int)blockIdx.x - a.tile_blocks; s < strips; s += others)
       unit_sums<kMomentThreads>(a, s, (int)threadIdx.x, 1, reinterpret_cast<float*>(tiles));
@@ -457,6 +460,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   cluster_sync_all();  // both CTAs' barriers exist before either signals the other
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  wait_for_previous_kernel();
   int last_chunk[2] = {-1, -1};
 
   if (warp == 0) {
@@ -683,7 +687,7 @@ int consider(const MomentArgs& a, int64_t& best, int& bn, int& split) {
 }
 
 template <int BN>
-int launch_tiles(const MomentMaps& maps, MomentArgs& a, int split, int sms, cudaStream_t st) {
+int launch_tiles(const MomentMaps& maps, MomentArgs& a, int split, int sms, bool early, cudaStream_t st) {
   const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN) * split;
   a.tile_blocks = (int32_t)tiles;
   // CTAs of their own for the unit sums where SMs are left over, else the tiles' CTAs take them along
@@ -692,10 +696,10 @@ int launch_tiles(const MomentMaps& maps, MomentArgs& a, int split, int sms, cuda
   const int64_t grid = tiles + (strips > 0 && left > 0 ? (want < left ? want : left) * split : 0);
   void* params[2] = {(void*)&maps, (void*)&a};
   return launch_clusters((const void*)k_pair_moments<BN>, (unsigned)grid, (unsigned)split, kMomentThreads,
-                         MomentShape<BN>::kSmem, params, st, "k_pair_moments launch");
+                         MomentShape<BN>::kSmem, params, st, "k_pair_moments launch", early);
 }
 
-int launch_moments(const MomentMaps& maps, MomentArgs& a, cudaStream_t st) {
+int launch_moments(const MomentMaps& maps, MomentArgs& a, bool early, cudaStream_t st) {
   ClusterFit fit;
   int rc = cluster_fit((const void*)k_pair_moments_2sm, 2, kMomentThreads, kPairSmem, &fit);
   if (rc) return rc;
@@ -719,11 +723,11 @@ int launch_moments(const MomentMaps& maps, MomentArgs& a, cudaStream_t st) {
     const int64_t others = want < left ? want : left;
     void* params[2] = {(void*)&maps, (void*)&a};
     return launch_clusters((const void*)k_pair_moments_2sm, (unsigned)(2 * (clusters + others)), 2, kMomentThreads, kPairSmem,
-                           params, st, "k_pair_moments_2sm launch");
+                           params, st, "k_pair_moments_2sm launch", early);
   }
-  if (bn == 64) return launch_tiles<64>(maps, a, split, fit.sms, st);
-  if (bn == 128) return launch_tiles<128>(maps, a, split, fit.sms, st);
-  return launch_tiles<256>(maps, a, split, fit.sms, st);
+  if (bn == 64) return launch_tiles<64>(maps, a, split, fit.sms, early, st);
+  if (bn == 128) return launch_tiles<128>(maps, a, split, fit.sms, early, st);
+  return launch_tiles<256>(maps, a, split, fit.sms, early, st);
 }
 
 // Rows of 16-bit elements from any strides to rows that start on 16 bytes, several matrices in one launch
@@ -732,32 +736,42 @@ struct PackArgs {
   tthrml_pack_matrix m[TTHRML_MAX_PACKED];
 };
 __global__ void __launch_bounds__(256) k_pack_rows(const __grid_constant__ PackArgs a) {
+  let_next_kernel_start();
   const tthrml_pack_matrix& m = a.m[blockIdx.y];
   const uint32_t per_row = (uint32_t)(m.pitch / 8);
   const uint32_t rows_at_once = per_row >= 256u ? 1u : 256u / per_row;  // rows that a block takes side by side
   const uint32_t t_row = threadIdx.x / per_row, t_vec = threadIdx.x - t_row * per_row;
   if (per_row < 256u && t_row >= rows_at_once) return;
-  for (int64_t row = (int64_t)blockIdx.x * rows_at_once + (per_row < 256u ? t_row : 0u); row < m.rows;
-       row += (int64_t)gridDim.x * rows_at_once) {
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(m.src) + row * m.row_stride;
+  const int64_t step = (int64_t)gridDim.x * rows_at_once;
+  for (int64_t row0 = (int64_t)blockIdx.x * rows_at_once + (per_row < 256u ? t_row : 0u); row0 < m.rows; row0 += 4 * step) {
     for (uint32_t v = per_row < 256u ? t_vec : threadIdx.x; v < per_row; v += 256u) {
       const int64_t c = (int64_t)v * 8;
-      uint4 out;
-      if (m.col_stride == 1 && c + 8 <= m.cols) {
-        // the words that hold the eight elements; a fifth one where the first element is the upper half of a word
-        const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)(src + c) & ~(uintptr_t)3);
-        const bool odd = ((uintptr_t)(src + c) & 2) != 0;
-        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = odd ? w[4] : 0u;
-        out = odd ? make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
-                               __funnelshift_r(w3, w4, 16))
-                  : make_uint4(w0, w1, w2, w3);
-      } else {
-        uint32_t e[8];
+      uint4 out[4];  // four rows on their way at a time
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = c + j < m.cols ? src[(c + j) * m.col_stride] : 0u;
-        out = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+      for (int j = 0; j < 4; ++j) {
+        const int64_t row = row0 + j * step;
+        if (row >= m.rows) break;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(m.src) + row * m.row_stride;
+        if (m.col_stride == 1 && c + 8 <= m.cols) {
+          // the words that hold the eight elements; a fifth one where the first element is the upper half of a word
+          const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)(src + c) & ~(uintptr_t)3);
+          const bool odd = ((uintptr_t)(src + c) & 2) != 0;
+          const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = odd ? w[4] : 0u;
+          out[j] = odd ? make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
+                                    __funnelshift_r(w3, w4, 16))
+                       : make_uint4(w0, w1, w2, w3);
+        } else {
+          uint32_t e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = c + i < m.cols ? src[(c + i) * m.col_stride] : 0u;
+          out[j] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        }
       }
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(m.dst) + row * m.pitch + c) = out;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t row = row0 + j * step;
+        if (row < m.rows) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(m.dst) + row * m.pitch + c) = out[j];
+      }
     }
   }
 }
@@ -765,9 +779,12 @@ __global__ void __launch_bounds__(256) k_pack_rows(const __grid_constant__ PackA
 }  // namespace
 }  // namespace tthrml
 
-extern "C" int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32_t n_phases, int32_t dtype,
-                                   int64_t x_units, int64_t y_units, float* out, int64_t out_ld, float* x_sum,
-                                   float* y_sum, int32_t accumulate, int32_t* error, void* stream) {
+namespace {
+
+// early: the operands were laid out by the kernel just before on the stream
+int pair_moments(const tthrml_moment_phase* phases_host, int32_t n_phases, int32_t dtype, int64_t x_units, int64_t y_units,
+                 float* out, int64_t out_ld, float* x_sum, float* y_sum, int32_t accumulate, int32_t* error, bool early,
+                 void* stream) {
   using namespace tthrml;
   if (x_units == 0 && y_units == 0) return TTHRML_OK;
   if (!phases_host || !out || !error) {
@@ -841,7 +858,28 @@ extern "C" int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32
   a.vector_store = (uintptr_t)out % 16 == 0 && out_ld % 4 == 0;
   a.f16 = dtype == TTHRML_DT_F16;
   a.error = error;
-  return launch_moments(maps, a, (cudaStream_t)stream);
+  return launch_moments(maps, a, early, (cudaStream_t)stream);
+}
+
+}  // namespace
+
+extern "C" int tthrml_pair_moments(const tthrml_moment_phase* phases_host, int32_t n_phases, int32_t dtype,
+                                   int64_t x_units, int64_t y_units, float* out, int64_t out_ld, float* x_sum,
+                                   float* y_sum, int32_t accumulate, int32_t* error, void* stream) {
+  return pair_moments(phases_host, n_phases, dtype, x_units, y_units, out, out_ld, x_sum, y_sum, accumulate, error, false,
+                      stream);
+}
+
+extern "C" int tthrml_pair_moments_packed(const tthrml_pack_matrix* matrices_host, int32_t n_matrices,
+                                          const tthrml_moment_phase* phases_host, int32_t n_phases, int32_t dtype,
+                                          int64_t x_units, int64_t y_units, float* out, int64_t out_ld, float* x_sum,
+                                          float* y_sum, int32_t accumulate, int32_t* error, void* stream) {
+  const int rc = tthrml_pack_rows(matrices_host, n_matrices, stream);
+  if (rc) return rc;
+  bool packed = false;  // whether a kernel was launched
+  for (int i = 0; i < n_matrices; ++i) packed = packed || matrices_host[i].rows > 0;
+  return pair_moments(phases_host, n_phases, dtype, x_units, y_units, out, out_ld, x_sum, y_sum, accumulate, error, packed,
+                      stream);
 }
 
 extern "C" int tthrml_pack_rows(const tthrml_pack_matrix* matrices_host, int32_t n, void* stream) {
@@ -862,7 +900,7 @@ extern "C" int tthrml_pack_rows(const tthrml_pack_matrix* matrices_host, int32_t
       return TTHRML_ERR_ARG;
     }
     a.m[i] = m;
-    const int64_t at_once = m.pitch / 8 >= 256 ? 1 : 256 / (m.pitch / 8), blocks = (m.rows + at_once - 1) / at_once;
+    const int64_t at_once = 4 * (m.pitch / 8 >= 256 ? 1 : 256 / (m.pitch / 8)), blocks = (m.rows + at_once - 1) / at_once;
     most = blocks > most ? blocks : most;
   }
   if (most == 0) return TTHRML_OK;

@@ -78,7 +78,7 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
         if word is not None and current_device() == index:  # the plain case, from the second call on
             nat.bind_device(index)
             made = nat.hostcall().pair_moments(xs, ys, scales, bool(units), nat.address_of("tthrml_pair_moments"),
-                                               nat.address_of("tthrml_pack_rows"), word, raw_stream(index), index)
+                                               nat.address_of("tthrml_pair_moments_packed"), word, raw_stream(index), index)
             if made is not None:
                 if type(made) is int:
                     nat.check(made, "tthrml_pair_moments")
