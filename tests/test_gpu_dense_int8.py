@@ -348,3 +348,73 @@ def test_learner_steps(precision, bits):
     tt.check_operator_errors()
     with pytest.raises(ValueError):
         learner.step(torch.zeros((64, 256)))
+
+
+def test_mesh_of_one_and_shared_weights():
+    """A MeshExecutor's 8-bit sweeps, weights and moments are its executor's; shared operands follow their owner."""
+    import tt_thrml_b200 as tt
+
+    program, C = rbm(), 128
+    cfg = make_cuda_config(n_chains=C, dense_precision="int8")
+    dev = tt.open_device(device_id=0)
+    one, two = (Executor(None, dev, program, cfg, n_sweeps=8) for _ in range(2))
+    mesh = tt.make_mesh_executor(None, dev, program, cfg, n_sweeps=8)
+    W = torch.from_numpy(rbm(seed=9).W).cuda()
+    one.update_dense_weights(W)
+    two.share_dense_weights(one)
+    mesh.update_dense_weights(W)
+    one.update_dense_weights(W * 0.5)
+    mesh.update_dense_weights(W * 0.5)
+    init = [np.linspace(-1, 1, 256, dtype=F) + np.zeros((C, 1), F), np.ones((C, 512), bool)]
+    states = []
+    for ex in (one, two, mesh):
+        ex.load_state(init, [])
+        ex.prepare_rng(4)
+        ex.run_sweeps(3)
+        states.append(ex)
+    assert np.array_equal(one.raw_state(), two.raw_state())
+    assert np.array_equal(one.raw_state(), mesh.shards[0].raw_state())
+    for a, b in zip(one.dense_moments(0.5), mesh.dense_moments(0.5)):
+        assert torch.equal(a, b)
+    with pytest.raises(NotImplementedError):
+        mesh.share_dense_weights(one)
+    apart = Executor(None, None, program, cfg, n_sweeps=8)
+    with pytest.raises(ValueError):
+        apart.share_dense_weights(one)
+    with pytest.raises(ValueError):
+        Executor(None, dev, program, make_cuda_config(n_chains=C, dense_precision="bf16")).share_dense_weights(one)
+
+
+def test_learner_refusals():
+    import tt_thrml_b200 as tt
+
+    with pytest.raises(ValueError):
+        tt.DenseLearner(rbm(), n_data=128, n_chains=128, sweeps=0)
+    with pytest.raises(ValueError):
+        tt.DenseLearner(rbm(), n_data=128, n_chains=128, config=make_cuda_config(rng_mode="parity"))
+    with pytest.raises(NotImplementedError):  # 100 chains do not reach the dense kernels
+        tt.DenseLearner(rbm(), n_data=100, n_chains=128)
+
+
+def test_learner_on_spins_and_two_learners_at_once():
+    """Spin batches (as bools or +-1), and two learners side by side: each its own streams, draws and operands."""
+    import tt_thrml_b200 as tt
+
+    g = torch.Generator().manual_seed(0)
+    batch = torch.randint(0, 2, (128, 256), generator=g).bool()
+
+    def make(seed):
+        return tt.DenseLearner(rbm(True), n_data=128, n_chains=128, config=make_cuda_config(dense_precision="int8"), seed=seed)
+
+    alone = [make(s) for s in (1, 2)]
+    for ln in alone:
+        for _ in range(3):
+            ln.step(batch.cuda())
+    both = [make(s) for s in (1, 2)]
+    for _ in range(3):
+        for ln in both:
+            ln.step(batch.float().cuda() * 2 - 1)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        assert torch.equal(a.weights, b.weights) and torch.equal(a.hidden_bias, b.hidden_bias)
+    assert not torch.equal(both[0].weights, both[1].weights)

@@ -222,9 +222,12 @@ def test_refusals(tt):
         ((ok, r), {"out": torch.empty((3, 4), device="cuda")}, ValueError),
         ((ok, r), {"out": torch.empty((4, 2), device="cuda").t()}, ValueError),
         ((ok, r), {"out": torch.empty((1, 4), device="cuda").expand(2, 4)}, ValueError),
+        ((ok[:, :4].contiguous(), tt.quantize_rows(torch.ones((4, 4), device="cuda"))), {"out": "x"}, ValueError),
         ((ok, tt.QuantizedRows(r.values)), {}, ValueError),
         ((ok.clone().requires_grad_(True), r), {}, RuntimeError),
     ]:
+        if kw.get("out") is not None and isinstance(kw["out"], str):
+            kw = {"out": args[0]}  # in place: read and written at the same time
         with pytest.raises(exc):
             tt.int8_product(*args, **kw)
     with torch.no_grad():

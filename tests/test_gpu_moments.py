@@ -190,6 +190,7 @@ def test_two_captured_graphs_on_two_streams(tt):
 
 def test_refusals(tt):
     x, y = torch.ones((4, 5), dtype=BF16, device="cuda"), torch.ones((4, 6), dtype=BF16, device="cuda")
+    buffer = torch.zeros((8, 64), dtype=torch.uint8, device="cuda")
     for args, kw, exc in [
         ((x.float(), y.float()), {}, ValueError),
         ((x, y.half()), {}, ValueError),
@@ -206,6 +207,7 @@ def test_refusals(tt):
         ((x, y), {"out": torch.empty((5, 6), device="cuda").half()}, ValueError),
         ((x, y), {"out": (torch.empty((5, 6), device="cuda"), torch.empty(4, device="cuda"), torch.empty(6, device="cuda")),
                   "units": True}, ValueError),
+        ((buffer.view(BF16)[:4, :5], y), {"out": buffer.view(torch.float32)[:5, :6]}, ValueError),
         ((x.clone().requires_grad_(True), y), {}, RuntimeError),
     ]:
         with pytest.raises(exc):

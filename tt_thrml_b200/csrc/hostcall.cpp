@@ -5,6 +5,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
 #include <Python.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/tthrml.h"
@@ -28,6 +29,7 @@ bool plain_cuda(const at::Tensor& t, long device) {
 // plain case (the parameter as the row has it, a gradient of its sizes and strides and of its type or float32).  Fills the
 // gradients' addresses and types into the rows (tthrml_adamw_tensor), which stand for the parameters with elements.
 PyObject* adamw_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 5 || !PyList_Check(args[0]) || !PyList_Check(args[1]) ||
       PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1])) {
     PyErr_SetString(PyExc_TypeError, "adamw_rows(params, grads, rows, n_rows, device): two lists of one length");
@@ -56,10 +58,12 @@ PyObject* adamw_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     r.grad_dtype = gd;
   }
   return PyLong_FromSsize_t(row == n_rows ? -1 : n - 1);
+  END_HANDLE_TH_ERRORS
 }
 
 // bump_versions(tensors): tells autograd that the tensors were written.
 PyObject* bump_versions(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
   if (!PyList_Check(list)) {
     PyErr_SetString(PyExc_TypeError, "bump_versions(tensors): a list");
     return nullptr;
@@ -71,6 +75,7 @@ PyObject* bump_versions(PyObject*, PyObject* list) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
   Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
 }
 
 template <typename Fn>
@@ -86,6 +91,7 @@ using PackedMomentsFn = decltype(&tthrml_pair_moments_packed);
 // int8_product(x, weights, weight scales, pitch, bias or None, function, error word, stream, device) -> the product in x's
 // type, an error code, or None.
 PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 9 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) ||
       !(args[4] == Py_None || THPVariable_Check(args[4])))
     Py_RETURN_NONE;
@@ -109,31 +115,28 @@ PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   const int64_t rs = x.dim() == 2 ? x.stride(0) : K, cs = x.dim() == 2 && K > 1 ? x.stride(1) : 1;
   if (cs == 0 || (cs == 1 && M > 1 && rs < K)) Py_RETURN_NONE;
-  try {
-    at::DimVector sizes(x.sizes().begin(), x.sizes().end());
-    sizes.back() = N;
-    at::Tensor out = at::empty(sizes, x.options().requires_grad(false)), space;
-    int64_t bytes = 0;
-    const int64_t padded = (K + 15) / 16 * 16;
-    if (M > 2 || M * padded > TTHRML_INT8_FEW_BYTES || cs != 1) {
-      bytes = M * padded + (M * 4 + 15) / 16 * 16;
-      space = at::empty({bytes}, x.options().dtype(at::kChar).requires_grad(false));
-    }
-    const int rc = address<LinearFn>(args[5])(
-        x.const_data_ptr(), code, M, K, rs, cs, bytes ? space.mutable_data_ptr() : nullptr, bytes,
-        w.const_data_ptr<int8_t>(), pitch, ws.const_data_ptr<float>(), N, bias, out.mutable_data_ptr(), code, N,
-        address<int32_t*>(args[6]), PyLong_AsVoidPtr(args[7]));
-    if (rc) return PyLong_FromLong(rc);
-    return THPVariable_Wrap(out);
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  at::DimVector sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = N;
+  at::Tensor out = at::empty(sizes, x.options().requires_grad(false)), space;
+  int64_t bytes = 0;
+  const int64_t padded = (K + 15) / 16 * 16;
+  if (M > 2 || M * padded > TTHRML_INT8_FEW_BYTES || cs != 1) {
+    bytes = M * padded + (M * 4 + 15) / 16 * 16;
+    space = at::empty({bytes}, x.options().dtype(at::kChar).requires_grad(false));
   }
+  const int rc = address<LinearFn>(args[5])(
+      x.const_data_ptr(), code, M, K, rs, cs, bytes ? space.mutable_data_ptr() : nullptr, bytes,
+      w.const_data_ptr<int8_t>(), pitch, ws.const_data_ptr<float>(), N, bias, out.mutable_data_ptr(), code, N,
+      address<int32_t*>(args[6]), PyLong_AsVoidPtr(args[7]));
+  if (rc) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
 }
 
 // pair_moments(xs, ys, scales, units, function, its form for packed operands, error word, stream, device) -> the moments (with `units` a
 // triple), an error code, or None.
 PyObject* pair_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 9 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !PyList_Check(args[2])) Py_RETURN_NONE;
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
   if (n < 1 || n > TTHRML_MAX_PHASES || PyList_GET_SIZE(args[1]) != n || PyList_GET_SIZE(args[2]) != n) Py_RETURN_NONE;
@@ -176,42 +179,38 @@ PyObject* pair_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     ph.scale = ph.x_scale = ph.y_scale = (float)s;
   }
   void* stream = PyLong_AsVoidPtr(args[7]);
-  try {
-    const at::Tensor& first = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0));
-    const auto options = first.options().dtype(at::kFloat).requires_grad(false);
-    at::Tensor out = at::empty({M, N}, options), xs, ys, space;
-    if (units) {
-      xs = at::empty({M}, options);
-      ys = at::empty({N}, options);
-    }
-    int rc = 0;
-    if (n_packed) {
-      space = at::empty({elements > 0 ? elements : 8}, first.options().requires_grad(false));
-      char* base = static_cast<char*>(space.mutable_data_ptr());
-      for (int i = 0; i < n_packed; ++i) {
-        packed[i].dst = base + reinterpret_cast<uintptr_t>(packed[i].dst);
-        *packed_into[i] = packed[i].dst;
-      }
-    }
-    float *o = out.mutable_data_ptr<float>(), *xo = units ? xs.mutable_data_ptr<float>() : nullptr,
-          *yo = units ? ys.mutable_data_ptr<float>() : nullptr;
-    int32_t* error = address<int32_t*>(args[6]);
-    if (n_packed)
-      rc = address<PackedMomentsFn>(args[5])(packed, n_packed, phases, (int32_t)n, code, M, N, o, N, xo, yo, 0, error, stream);
-    else
-      rc = address<MomentsFn>(args[4])(phases, (int32_t)n, code, M, N, o, N, xo, yo, 0, error, stream);
-    if (rc) return PyLong_FromLong(rc);
-    if (!units) return THPVariable_Wrap(out);
-    PyObject *a = THPVariable_Wrap(out), *b = THPVariable_Wrap(xs), *c = THPVariable_Wrap(ys);
-    PyObject* t = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
-    Py_XDECREF(a);
-    Py_XDECREF(b);
-    Py_XDECREF(c);
-    return t;
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  const at::Tensor& first = THPVariable_Unpack(PyList_GET_ITEM(args[0], 0));
+  const auto options = first.options().dtype(at::kFloat).requires_grad(false);
+  at::Tensor out = at::empty({M, N}, options), xs, ys, space;
+  if (units) {
+    xs = at::empty({M}, options);
+    ys = at::empty({N}, options);
   }
+  int rc = 0;
+  if (n_packed) {
+    space = at::empty({elements > 0 ? elements : 8}, first.options().requires_grad(false));
+    char* base = static_cast<char*>(space.mutable_data_ptr());
+    for (int i = 0; i < n_packed; ++i) {
+      packed[i].dst = base + reinterpret_cast<uintptr_t>(packed[i].dst);
+      *packed_into[i] = packed[i].dst;
+    }
+  }
+  float *o = out.mutable_data_ptr<float>(), *xo = units ? xs.mutable_data_ptr<float>() : nullptr,
+        *yo = units ? ys.mutable_data_ptr<float>() : nullptr;
+  int32_t* error = address<int32_t*>(args[6]);
+  if (n_packed)
+    rc = address<PackedMomentsFn>(args[5])(packed, n_packed, phases, (int32_t)n, code, M, N, o, N, xo, yo, 0, error, stream);
+  else
+    rc = address<MomentsFn>(args[4])(phases, (int32_t)n, code, M, N, o, N, xo, yo, 0, error, stream);
+  if (rc) return PyLong_FromLong(rc);
+  if (!units) return THPVariable_Wrap(out);
+  PyObject *a = THPVariable_Wrap(out), *b = THPVariable_Wrap(xs), *c = THPVariable_Wrap(ys);
+  PyObject* t = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  Py_XDECREF(c);
+  return t;
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {

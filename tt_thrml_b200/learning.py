@@ -27,9 +27,11 @@ def dense_moments(terms, *, out=None, accumulate: bool = False):
 
     Returns float32 (pair [n_0, n_1], block 0 [n_0], block 1 [n_1]); `out` is such
     a triple to write, or, with `accumulate`, to add to.  Ordered after the
-    executors' sweeps and before their next ones; queued on the current stream."""
+    executors' sweeps and before their next ones; queued on the current stream.  All executors (a MeshExecutor counts as
+    its local shards) must be on one device."""
     torch = _torch()
-    terms = [(ex, float(s)) for ex, s in terms]
+    # a mesh of chains is the sum of its shards
+    terms = [(shard, float(s)) for ex, s in terms for shard in getattr(ex, "shards", [ex])]
     if not terms:
         raise ValueError("dense_moments needs at least one executor")
     first = terms[0][0]

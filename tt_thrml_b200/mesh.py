@@ -276,6 +276,15 @@ class MeshExecutor(Executor):
             return carry, None
         return carry, tree_stack(all_obs)
 
+    def update_dense_weights(self, weights, bias_0=None, bias_1=None) -> None:
+        """Executor.update_dense_weights on every shard (the tensors are copied to the other shards' devices)."""
+        for shard in self.shards:
+            dev = shard.compiled.device
+            shard.update_dense_weights(*(t if t is None or t.device == dev else t.to(dev) for t in (weights, bias_0, bias_1)))
+
+    def share_dense_weights(self, other) -> None:
+        raise NotImplementedError("share the weights of the mesh's executors one by one (MeshExecutor.shards)")
+
     def timing_summary(self) -> dict:
         return self.shards[0].timing_summary()
 

@@ -11,7 +11,7 @@ two dense blocks at once, on the tensor cores.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import _error_addresses, current_device, dtype_code, error_word, on_device, raw_stream, require_cuda
+from .quantized import _error_addresses, current_device, dtype_code, error_word, on_device, raw_stream, refuse_overlap, require_cuda
 
 
 def _torch():
@@ -125,6 +125,10 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
             raise ValueError(f"out must be float32 of shape {(M, N)}, got {out.dtype} of {tuple(out.shape)}")
         if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError("out needs dense rows that do not overlap")
+        inputs = [(f"{name}[{p}]", t) for name, ts in (("x", xs), ("y", ys)) for p, t in enumerate(ts)]
+        for name, t in (("out", out), ("x_sum", x_sum), ("y_sum", y_sum)):
+            if t is not None:
+                refuse_overlap(name, t, inputs)
     phases = (nat.MomentPhase * len(xs))()
     with on_device(dev):
         stream = raw_stream(dev.index)

@@ -114,6 +114,22 @@ def _no_grad(name: str, t):
         raise RuntimeError(f"{name} requires a gradient, but 8-bit products have no backward pass (use torch.no_grad())")
 
 
+def memory_span(t) -> tuple[int, int]:
+    """First and last-plus-one address that a tensor's elements lie in."""
+    if not t.numel():
+        return 0, 0
+    reach = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + reach * t.element_size()
+
+
+def refuse_overlap(name: str, out, inputs) -> None:
+    a, b = memory_span(out)
+    for other, t in inputs:
+        c, d = memory_span(t)
+        if a < d and c < b:
+            raise ValueError(f"{name} shares memory with {other}, which the kernel reads meanwhile")
+
+
 class QuantizedRows:
     """A matrix as int8 rows with one float32 scale per row: value[r, c] = values[r, c] * scale[r].
 
@@ -254,6 +270,8 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
         flat = out.view(-1, N) if N else out  # raises if the rows cannot be one matrix
         if flat.numel() and ((N > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < N)):
             raise ValueError("out needs dense rows that do not overlap")
+        inputs = [("x", rows), ("the weights", w), ("the weights' scales", w_scale)]
+        refuse_overlap("out", out, inputs + ([] if bias is None else [("bias", bias)]))
         out_ld = flat.stride(0) if N and flat.shape[0] > 1 else N
     if not out.numel():
         return out
