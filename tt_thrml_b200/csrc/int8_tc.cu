@@ -27,7 +27,7 @@ struct ProductArgs {
   void* out;             // [M][out_ld]
   int64_t out_ld;
   int32_t out_dtype;
-  int32_t vector_store;  // rows of `out` are aligned for stores of four elements
+  int32_t vector_store;  // tiles: rows of `out` are aligned for stores of four elements; pairs: bytes they are aligned to
   int32_t M, N;
   int32_t num_k;         // 128-column blocks of K
   int32_t box_m;         // rows per A load (16, 32, 64 or 128)
@@ -253,8 +253,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // CTA-pair kernel
 // ---------------------------------------------------------------------------
 constexpr int kPairStages = 6, kPairStage = 2 * 128 * 128, kPairThreads = 320, kPairWarps = 8;
-constexpr int kPairRowPitch = 33;  // floats per row of a warp's 32 x 32 transpose (unaligned outputs)
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kPairWarps * 32 * kPairRowPitch * 4;
+constexpr int kTurnPitch = 80;  // bytes per row of a warp's staged 32 x 64 bytes: rows 20 banks apart
+constexpr int kScaleWords = 2 * 512;  // scales and biases of a tile's units, two tiles
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kScaleWords * 4 + kPairWarps * 32 * kTurnPitch;
 enum : int { kStoreFields = 0, kDrawSpins = 1, kDrawGaussians = 2 };
 
 struct PairArgs {
@@ -273,79 +274,103 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       "r"(0u), "r"(0u), "r"(0u));
 }
 
-// Sums of 32 consecutive units of one row, scaled: (float)sum * (s_x * s_w).
-__device__ __forceinline__ void scale_chunk(const ProductArgs& a, float sx, int n_first, float (&v)[32]) {
-  if (n_first + 32 <= a.N && (uintptr_t)a.w_scale % 16 == 0) {
-    const float4* sw = reinterpret_cast<const float4*>(a.w_scale + n_first);
+// Sums of 32 consecutive units of one row, scaled: (float)sum * (s_x * s_w); sw: the units' scales in shared memory.
+__device__ __forceinline__ void scale_chunk(float sx, const float* sw, float (&v)[32]) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float4 w = __ldg(sw + q);
-      v[4 * q] = __fmul_rn((float)__float_as_int(v[4 * q]), __fmul_rn(sx, w.x));
-      v[4 * q + 1] = __fmul_rn((float)__float_as_int(v[4 * q + 1]), __fmul_rn(sx, w.y));
-      v[4 * q + 2] = __fmul_rn((float)__float_as_int(v[4 * q + 2]), __fmul_rn(sx, w.z));
-      v[4 * q + 3] = __fmul_rn((float)__float_as_int(v[4 * q + 3]), __fmul_rn(sx, w.w));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const float w = n_first + j < a.N ? __ldg(a.w_scale + n_first + j) : 0.0f;
-      v[j] = __fmul_rn((float)__float_as_int(v[j]), __fmul_rn(sx, w));
-    }
+  for (int q = 0; q < 8; ++q) {
+    const float4 w = reinterpret_cast<const float4*>(sw)[q];
+    v[4 * q] = __fmul_rn((float)__float_as_int(v[4 * q]), __fmul_rn(sx, w.x));
+    v[4 * q + 1] = __fmul_rn((float)__float_as_int(v[4 * q + 1]), __fmul_rn(sx, w.y));
+    v[4 * q + 2] = __fmul_rn((float)__float_as_int(v[4 * q + 2]), __fmul_rn(sx, w.z));
+    v[4 * q + 3] = __fmul_rn((float)__float_as_int(v[4 * q + 3]), __fmul_rn(sx, w.w));
   }
 }
 
-// Stores one 32-column chunk of 32 rows (lane = row m0 + lane): each lane its own row where rows are aligned, else by way
-// of shared memory, so that a warp stores consecutive elements.
-__device__ __forceinline__ void store_chunk(const ProductArgs& a, int m, int n_first, const float (&v)[32], float* turn) {
-  float y[32];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    y[j] = v[j];
-    if (a.bias) y[j] = __fadd_rn(y[j], n_first + j < a.N ? __ldg(a.bias + n_first + j) : 0.0f);
+// Stores 32 staged rows of `bytes` each (a power of two up to 64) from column byte `at` of the output rows m0 .. m0 + 31, V at
+// a time: a warp's store covers whole pieces of a few rows, where a store of every lane's own row would touch 32 lines.
+template <typename V>
+__device__ __forceinline__ void drain(const unsigned char* turn, int bytes, unsigned char* out, int64_t pitch, int64_t at,
+                                      int m0, int M, int live_bytes) {
+  const int lane = threadIdx.x & 31, per_row = bytes / (int)sizeof(V), rows = 32 / per_row;
+  const int k = (lane % per_row) * (int)sizeof(V);
+  if (rows == 0) {  // more pieces than lanes: several per lane and row
+    for (int r = 0; r < 32 && m0 + r < M; ++r)
+      for (int j = lane * (int)sizeof(V); j < live_bytes; j += 32 * (int)sizeof(V))
+        *reinterpret_cast<V*>(out + (int64_t)(m0 + r) * pitch + at + j) = *reinterpret_cast<const V*>(turn + r * kTurnPitch + j);
+    return;
   }
-  if (a.vector_store && n_first + 32 <= a.N) {
-    if (m >= a.M) return;
-    const int64_t at = (int64_t)m * a.out_ld + n_first;
-    if (a.out_dtype == TTHRML_DT_F32) {
-      float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at);
+  if (k >= live_bytes) return;
+#pragma unroll 4
+  for (int r = lane / per_row; r < 32 && m0 + r < M; r += rows)
+    *reinterpret_cast<V*>(out + (int64_t)(m0 + r) * pitch + at + k) = *reinterpret_cast<const V*>(turn + r * kTurnPitch + k);
+}
+// words: this lane's row, N16 pieces of 16 bytes.  Every lane calls it; the rows are m0 .. m0 + 31, `align` their alignment.
+template <int N16>
+__device__ __forceinline__ void store_rows(const uint4 (&words)[N16], unsigned char* turn, unsigned char* out, int64_t pitch,
+                                           int64_t at, int m0, int M, int live_bytes, int align) {
+  const int lane = threadIdx.x & 31;
+  uint4* mine = reinterpret_cast<uint4*>(turn + lane * kTurnPitch);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) dst[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
-    } else {
-      uint32_t w[16];
+  for (int q = 0; q < N16; ++q) mine[q] = words[q];
+  __syncwarp();
+  if (live_bytes < 16 * N16) align = align < 4 ? align : (live_bytes % 4 == 0 ? 4 : 2);
+  if (align >= 16)
+    drain<uint4>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  else if (align >= 8)
+    drain<uint2>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  else if (align >= 4)
+    drain<uint32_t>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  else
+    drain<uint16_t>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  __syncwarp();
+}
+
+// Adds the biases to one 32-column chunk of 32 rows (lane = row m) and stores it.
+__device__ __forceinline__ void store_chunk(const ProductArgs& a, int m, int n_first, const float* bias, float (&y)[32],
+                                            unsigned char* turn) {
+  if (a.bias) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (a.out_dtype == TTHRML_DT_BF16) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-          const __half2 h = __floats2half2_rn(y[2 * j], y[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      }
-      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at);
+    for (int q = 0; q < 8; ++q) {
+      const float4 b = reinterpret_cast<const float4*>(bias)[q];
+      y[4 * q] = __fadd_rn(y[4 * q], b.x);
+      y[4 * q + 1] = __fadd_rn(y[4 * q + 1], b.y);
+      y[4 * q + 2] = __fadd_rn(y[4 * q + 2], b.z);
+      y[4 * q + 3] = __fadd_rn(y[4 * q + 3], b.w);
+    }
+  }
+  unsigned char* out = reinterpret_cast<unsigned char*>(a.out);
+  const int m0 = m - (int)(threadIdx.x & 31), live = min(32, a.N - n_first);
+  if (a.out_dtype == TTHRML_DT_F32) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    for (int half = 0; half < 2; ++half) {
+      uint4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        w[q] = make_uint4(__float_as_uint(y[16 * half + 4 * q]), __float_as_uint(y[16 * half + 4 * q + 1]),
+                          __float_as_uint(y[16 * half + 4 * q + 2]), __float_as_uint(y[16 * half + 4 * q + 3]));
+      const int left = min(16, live - 16 * half);
+      if (left > 0) store_rows<4>(w, turn, out, a.out_ld * 4, 4 * (int64_t)(n_first + 16 * half), m0, a.M, 4 * left, a.vector_store);
     }
     return;
   }
-  const int lane = threadIdx.x & 31;
+  uint4 w[4];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) turn[lane * kPairRowPitch + j] = y[j];
-  __syncwarp();
-  const int n = n_first + lane;
-  if (n < a.N) {
-    for (int r = 0; r < 32 && m - lane + r < a.M; ++r) {
-      const int64_t at = (int64_t)(m - lane + r) * a.out_ld + n;
-      const float f = turn[r * kPairRowPitch + lane];
-      if (a.out_dtype == TTHRML_DT_F32)
-        reinterpret_cast<float*>(a.out)[at] = f;
-      else if (a.out_dtype == TTHRML_DT_BF16)
-        reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(f);
-      else
-        reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(f);
+  for (int q = 0; q < 4; ++q) {
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = y[8 * q + 2 * j], hi = y[8 * q + 2 * j + 1];
+      if (a.out_dtype == TTHRML_DT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        p[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        p[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
     }
+    w[q] = make_uint4(p[0], p[1], p[2], p[3]);
   }
-  __syncwarp();
+  store_rows<4>(w, turn, out, a.out_ld * 2, 2 * (int64_t)n_first, m0, a.M, 2 * live, a.vector_store);
 }
 
 template <int EPI, bool VARIATES>
@@ -359,7 +384,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* acc_full = empty + kPairStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  float* turns = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);
+  float* unit_scales = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);  // [2][scales 256, biases 256]
+  unsigned char* turns = reinterpret_cast<unsigned char*>(unit_scales + kScaleWords);
 
   const ProductArgs& a = args.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -452,7 +478,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else {
     const int quad = warp & 3, grp = (warp - 2) >> 2;
-    float* turn = turns + (warp - 2) * 32 * kPairRowPitch;
+    unsigned char* turn = turns + (warp - 2) * 32 * kTurnPitch;
     int it = 0;
     for (int t = first; t < n_tiles; t += step, ++it) {
       int mb, nb;
@@ -460,6 +486,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int b = it & 1;
       const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane;
       const float sx = a.x_scale && m < a.M ? __ldg(a.x_scale + m) : 1.0f;
+      // the tile's scales and biases, a unit per thread; two buffers, so that a warp may run one tile ahead
+      float* sw = unit_scales + b * 512;
+      {
+        const int j = (int)threadIdx.x - 64, n = nb * 256 + j;
+        sw[j] = n < a.N ? __ldg(a.w_scale + n) : 0.0f;
+        sw[256 + j] = EPI == kStoreFields && a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
       if (!mbar_wait(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
         if (lane == 0) atomicExch(a.error, kErrAccWait);
         break;
@@ -475,35 +509,36 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int n_first = nb * 256 + c * 32;
         float v[32];
         tmem_load32(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(c * 32), v);
-        scale_chunk(a, sx, n_first, v);
+        scale_chunk(sx, sw + c * 32, v);
         if (EPI == kStoreFields) {
-          store_chunk(a, m, n_first, v, turn);
-        } else if (m < a.M) {  // draws: N is a multiple of 32
-          if (EPI == kDrawSpins) {
-            uint32_t near;
-            const uint32_t down = spin_chunk<VARIATES>(args.d, v, m, n_first, sweep, keys, vs, near);
-            uint32_t w[8];  // four spins a word: bit -> 0x01 / 0xFF
+          store_chunk(a, m, n_first, sw + 256 + c * 32, v, turn);
+        } else if (EPI == kDrawSpins) {  // N is a multiple of 32; lanes behind the last chain draw for it and store nothing
+          uint32_t near;
+          const uint32_t down = spin_chunk<VARIATES>(args.d, v, m < a.M ? m : a.M - 1, n_first, sweep, keys, vs, near);
+          uint32_t w[8];  // four spins a word: bit -> 0x01 / 0xFF
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const uint32_t four = (down >> (4 * q)) & 15u;
-              w[q] = 0x01010101u | (((four * 0x00204081u) & 0x01010101u) * 0xFEu);
-            }
-            uint4* dst = reinterpret_cast<uint4*>(args.spins + (int64_t)m * a.N + n_first);
-            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-          } else {
-            float f[32];
-            gauss_chunk<VARIATES>(args.d, v, m, n_first, sweep, keys, inv, sd_g, vs, f);
-            uint32_t w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-              w[j] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            uint4* dst = reinterpret_cast<uint4*>(args.values + (int64_t)m * a.N + n_first);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) dst[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t four = (down >> (4 * q)) & 15u;
+            w[q] = 0x01010101u | (((four * 0x00204081u) & 0x01010101u) * 0xFEu);
           }
+          const uint4 row[2] = {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
+          store_rows<2>(row, turn, reinterpret_cast<unsigned char*>(args.spins), a.N, n_first, m - lane, a.M, 32, 16);
+        } else {
+          float f[32];
+          gauss_chunk<VARIATES>(args.d, v, m < a.M ? m : a.M - 1, n_first, sweep, keys, inv, sd_g, vs, f);
+          uint4 row[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(f[8 * q + 2 * j], f[8 * q + 2 * j + 1]);
+              p[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            row[q] = make_uint4(p[0], p[1], p[2], p[3]);
+          }
+          store_rows<4>(row, turn, reinterpret_cast<unsigned char*>(args.values), 2 * (int64_t)a.N, 2 * (int64_t)n_first,
+                        m - lane, a.M, 64, 16);
         }
         __syncwarp();  // the next TMEM load is a warp's
       }
@@ -681,7 +716,8 @@ int int8_product(const int8_t* x, int64_t x_pitch, const float* x_scale, const i
     if (rc) return rc;
     PairArgs pa = {};
     pa.p = a;
-    pa.p.vector_store = (uintptr_t)out % 16 == 0 && (out_ld * dtype_bytes(out_dtype)) % 16 == 0;
+    const uint64_t alignment = (uint64_t)(uintptr_t)out | (uint64_t)(out_ld * dtype_bytes(out_dtype));  // of the rows
+    pa.p.vector_store = alignment % 16 == 0 ? 16 : (alignment % 8 == 0 ? 8 : (alignment % 4 == 0 ? 4 : 0));
     return launch_pair(pair_fn, ma, mb, pa, cols, st);
   }
   rc = make_map_i8(&ma, x, rows, cols, x_pitch, (uint32_t)a.box_m);

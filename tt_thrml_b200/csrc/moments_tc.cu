@@ -130,9 +130,10 @@ __device__ __forceinline__ void add8(float (&s)[8], const uint4& w, bool f16) {
 
 // Strip `strip` of the unit sums (32 units of x, then of y) by NT threads (t = 0 .. NT - 1, named barrier `bar`): four
 // threads take the 64 bytes of a chain, NT / 4 chains at a time; the partial sums meet by shuffles and then in the order
-// of the warps.
-template <int NT>
-__device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t, int bar, float* part) {
+// of the warps.  CLUSTER: the CTAs of a cluster take every `split`-th group of chains each, and rank 0 adds their sums in the
+// order of the ranks.
+template <int NT, bool CLUSTER>
+__device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t, int bar, float* part, int rank, int split) {
   const int xs = a.x_sum ? (a.M + kSumUnits - 1) / kSumUnits : 0;
   const bool of_y = strip >= xs;
   const int u0 = (of_y ? strip - xs : strip) * kSumUnits, units = of_y ? a.N : a.M;
@@ -149,18 +150,19 @@ __device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t,
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = 0.0f;
     if (u + 8 <= units) {  // rows start on 16 bytes and the units on multiples of eight
-      const char* at = base + ((int64_t)lane * ld + u) * 2;
-      const int64_t step = (int64_t)(NT / 4) * ld * 2;
-      for (int64_t c = lane; c < a.chains[p]; c += 16 * (NT / 4), at += 16 * step) {  // 16 loads on their way at a time
+      const int64_t lanes = (int64_t)(NT / 4) * split, step = lanes * ld * 2;
+      const int64_t first = (int64_t)(NT / 4) * rank + lane;
+      const char* at = base + (first * ld + u) * 2;
+      for (int64_t c = first; c < a.chains[p]; c += 16 * lanes, at += 16 * step) {  // 16 loads on their way at a time
         uint4 w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          w[i] = c + i * (NT / 4) < a.chains[p] ? __ldg(reinterpret_cast<const uint4*>(at + i * step)) : make_uint4(0u, 0u, 0u, 0u);
+          w[i] = c + i * lanes < a.chains[p] ? __ldg(reinterpret_cast<const uint4*>(at + i * step)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int i = 0; i < 16; ++i) add8(s, w[i], a.f16 != 0);
       }
     } else {
-      for (int64_t c = lane; c < a.chains[p]; c += NT / 4)
+      for (int64_t c = (NT / 4) * rank + lane; c < a.chains[p]; c += (NT / 4) * split)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (u + i < units) s[i] += elem(base, c * ld + u + i, a.f16 != 0);
@@ -177,9 +179,25 @@ __device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t,
     for (int i = 0; i < 8; ++i) part[(t >> 5) * kSumUnits + (t & 3) * 8 + i] = total[i];
   }
   asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(NT) : "memory");
-  if (t < kSumUnits && u0 + t < units) {
-    float v = 0.0f;
+  float v = 0.0f;
+  if (t < kSumUnits)
     for (int i = 0; i < NT / 32; ++i) v += part[i * kSumUnits + t];
+  if (CLUSTER) {
+    float* mine = part + NT / 32 * kSumUnits;
+    if (t < kSumUnits) mine[t] = v;
+    cluster_sync_all();
+    if (rank == 0 && t < kSumUnits) {
+      for (int r = 1; r < split; ++r) {
+        uint32_t remote;
+        float w;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(mine + t)), "r"(r));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(remote) : "memory");
+        v += w;
+      }
+    }
+    cluster_sync_all();  // before any CTA's next strip, or its end
+  }
+  if (rank == 0 && t < kSumUnits && u0 + t < units) {
     float* dst = (of_y ? a.y_sum : a.x_sum) + u0 + t;
     *dst = a.accumulate ? *dst + v : v;
   }
@@ -188,11 +206,21 @@ __device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t,
 __host__ __device__ inline int sum_strips(const MomentArgs& a) {
   return (a.x_sum ? (a.M + kSumUnits - 1) / kSumUnits : 0) + (a.y_sum ? (a.N + kSumUnits - 1) / kSumUnits : 0);
 }
+// The unit sums of CTAs that have no tile: a strip for a cluster where there are clusters enough, else for a CTA.
+__device__ __forceinline__ void own_sums(const MomentArgs& a, float* part) {
+  const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks, i = (int)blockIdx.x - a.tile_blocks;
+  const int width = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
+  if (strips * width <= others) {
+    if (i / width < strips) unit_sums<kMomentThreads, true>(a, i / width, (int)threadIdx.x, 1, part, rank, width);
+  } else {
+    for (int s = i; s < strips; s += others) unit_sums<kMomentThreads, false>(a, s, (int)threadIdx.x, 1, part, 0, 1);
+  }
+}
 // The unit sums that fall to warps 10 and 11 of a tile's CTA.
 __device__ __forceinline__ void side_sums(const MomentArgs& a, float* part) {
   if ((int)gridDim.x > a.tile_blocks) return;  // CTAs of their own sum the units
   const int strips = sum_strips(a);
-  for (int s = blockIdx.x; s < strips; s += gridDim.x) unit_sums<64>(a, s, (int)threadIdx.x - 320, 1, part);
+  for (int s = blockIdx.x; s < strips; s += gridDim.x) unit_sums<64, false>(a, s, (int)threadIdx.x - 320, 1, part, 0, 1);
 }
 
 template <int BN>
@@ -203,9 +231,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   if ((int)blockIdx.x >= a.tile_blocks) {  // whole clusters: the tile blocks are a multiple of the cluster size
     wait_for_previous_kernel();
-    const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks;
-    for (int s = (int)blockIdx.x - a.tile_blocks; s < strips; s += others)
-      unit_sums<kMomentThreads>(a, s, (int)threadIdx.x, 1, reinterpret_cast<float*>(tiles));
+    own_sums(a, reinterpret_cast<float*>(tiles));
     return;
   }
   uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStage);
@@ -427,9 +453,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   float* side = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);
   if ((int)blockIdx.x >= a.tile_blocks) {  // whole clusters
     wait_for_previous_kernel();
-    const int strips = sum_strips(a), others = (int)gridDim.x - a.tile_blocks;
-    for (int s = (int)blockIdx.x - a.tile_blocks; s < strips; s += others)
-      unit_sums<kMomentThreads>(a, s, (int)threadIdx.x, 1, reinterpret_cast<float*>(tiles));
+    own_sums(a, reinterpret_cast<float*>(tiles));
     return;
   }
 
@@ -691,9 +715,9 @@ int launch_tiles(const MomentMaps& maps, MomentArgs& a, int split, int sms, bool
   const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + BN - 1) / BN) * split;
   a.tile_blocks = (int32_t)tiles;
   // CTAs of their own for the unit sums where SMs are left over, else the tiles' CTAs take them along
+  // (a strip is a cluster's; clusters of 8 and of 4 leave some SMs of a GPU unused, so some of these may run late)
   const int64_t strips = sum_strips(a), left = tiles < sms ? (sms - tiles) / split : 0;
-  const int64_t want = (strips + split - 1) / split;
-  const int64_t grid = tiles + (strips > 0 && left > 0 ? (want < left ? want : left) * split : 0);
+  const int64_t grid = tiles + (strips > 0 && left > 0 ? (strips < left ? strips : left) * split : 0);
   void* params[2] = {(void*)&maps, (void*)&a};
   return launch_clusters((const void*)k_pair_moments<BN>, (unsigned)grid, (unsigned)split, kMomentThreads,
                          MomentShape<BN>::kSmem, params, st, "k_pair_moments launch", early);
@@ -719,7 +743,7 @@ int launch_moments(const MomentMaps& maps, MomentArgs& a, bool early, cudaStream
     const int64_t clusters = pairs < fit.clusters ? pairs : fit.clusters;
     a.tile_blocks = (int32_t)(2 * clusters);
     // clusters of their own for the unit sums where SMs are left over, else warps of the tiles' CTAs take them along
-    const int64_t want = (sum_strips(a) + 1) / 2, left = fit.clusters - clusters;
+    const int64_t want = sum_strips(a), left = fit.clusters - clusters;
     const int64_t others = want < left ? want : left;
     void* params[2] = {(void*)&maps, (void*)&a};
     return launch_clusters((const void*)k_pair_moments_2sm, (unsigned)(2 * (clusters + others)), 2, kMomentThreads, kPairSmem,

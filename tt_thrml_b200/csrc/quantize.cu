@@ -3,8 +3,9 @@
 // One pass over the input: each row is read once, kept in registers while its largest magnitude is reduced, and
 // written as packed bytes.  Bound: memory (b read + 1 written byte per element).
 //   k_quantize_rows<T, W>: W warps per row, as few as hold it in registers (1024 elements a warp, at most 8 warps), so that
-//     a thread has four 16- or 32-byte loads on their way: 8192 x 4096 bfloat16 took 41 us with eight warps a row and
-//     half of their vectors empty.  Longer rows read their tail again.
+//     a thread has four (float32: eight) 16-byte loads on their way: 8192 x 4096 bfloat16 took 41 us with eight warps a
+//     row and half of their vectors empty.  Rows that do not start on 16 bytes are read as aligned vectors and shifted.
+//     Longer rows read their tail again.
 //   k_quantize_cols<T>: rows whose consecutive elements are strided but whose neighbours are adjacent (a transposed
 //     matrix): a cluster of eight CTAs takes 32 rows, an eighth of the columns each; the lanes run along the rows.  A share
 //     that fits stays in shared memory between the maximum, which the CTAs exchange, and the rounding.
@@ -14,46 +15,123 @@
 namespace tthrml {
 namespace {
 
-constexpr int kVecs = 4;  // vectors of eight elements that a thread keeps
+// How the 16-byte vectors of a row are read: at aligned addresses, as two aligned vectors shifted together, or by elements.
+enum : int { kElements = 0, kAligned = 1, kShifted = 2 };
 
-template <typename T, int W>
-__global__ void __launch_bounds__(256)
-    k_quantize_rows(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, int vectors,
+// 16 bytes from any address whose aligned surroundings hold bytes of the row on both sides.
+__device__ __forceinline__ uint4 load_shifted(const char* p, uint32_t off) {
+  const uint4* q = reinterpret_cast<const uint4*>(p - off);
+  const uint4 a = __ldg(q), b = __ldg(q + 1);
+  uint32_t w[5];
+  const uint32_t word = off >> 2, bits = (off & 3u) * 8u;  // the same for the whole row
+  if (word == 0)
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x;
+  else if (word == 1)
+    w[0] = a.y, w[1] = a.z, w[2] = a.w, w[3] = b.x, w[4] = b.y;
+  else if (word == 2)
+    w[0] = a.z, w[1] = a.w, w[2] = b.x, w[3] = b.y, w[4] = b.z;
+  else
+    w[0] = a.w, w[1] = b.x, w[2] = b.y, w[3] = b.z, w[4] = b.w;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
+}
+
+template <typename T, bool ALIGNED>
+struct RowReader {
+  const T* x;
+  int64_t cols, cs;
+  int mode;
+  uint32_t off;
+  __device__ __forceinline__ Vec8<T> vector(int64_t c) const {  // elements c .. c + 7, zeros behind the end
+    Vec8<T> v;
+    if ((ALIGNED || mode != kElements) && c + 8 <= cols) {
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+        v.w[i] = ALIGNED || mode == kAligned ? __ldg(reinterpret_cast<const uint4*>(x + c) + i)
+                                             : load_shifted(reinterpret_cast<const char*>(x + c) + 16 * i, off);
+      return v;
+    }
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) v.w[i] = make_uint4(0u, 0u, 0u, 0u);
+    T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) e[i] = x[(c + i) * cs];
+    return v;
+  }
+};
+
+// Running maximum of magnitudes, NaN once one is met: 16-bit elements two at a time.
+struct MaxF32 {
+  float top = 0.0f;
+  __device__ __forceinline__ void add(const uint4& v) {
+    top = max_abs(max_abs(max_abs(max_abs(top, __uint_as_float(v.x)), __uint_as_float(v.y)), __uint_as_float(v.z)),
+                  __uint_as_float(v.w));
+  }
+  __device__ __forceinline__ float value() const { return top; }
+};
+template <typename T2>
+struct MaxPacked {
+  uint32_t top = 0u;
+  __device__ __forceinline__ void add(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = w[i] & 0x7FFF7FFFu;
+      const T2 t = __hmax2_nan(*reinterpret_cast<const T2*>(&top), *reinterpret_cast<const T2*>(&m));
+      top = *reinterpret_cast<const uint32_t*>(&t);
+    }
+  }
+  __device__ __forceinline__ float value() const {
+    const T2 t = *reinterpret_cast<const T2*>(&top);
+    return max_abs(to_f32(t.x), to_f32(t.y));
+  }
+};
+template <typename T>
+struct MaxOf;
+template <>
+struct MaxOf<float> : MaxF32 {};
+template <>
+struct MaxOf<__nv_bfloat16> : MaxPacked<__nv_bfloat162> {};
+template <>
+struct MaxOf<__half> : MaxPacked<__half2> {};
+
+template <typename T>
+__device__ __forceinline__ void add_vector(MaxOf<T>& most, const Vec8<T>& v) {
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) most.add(v.w[i]);
+}
+// The quantised bytes of a vector.
+template <typename T>
+__device__ __forceinline__ void store_vector(int8_t* q, const Vec8<T>& v, float inv) {
+  float f[8];
+  unpack8(v, f);
+  *reinterpret_cast<uint2*>(q) = quantize8(f, inv);
+}
+
+template <typename T, int W, bool ALIGNED>
+__global__ void __launch_bounds__(256, 4)
+    k_quantize_rows(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, int contiguous,
                     int8_t* __restrict__ q, int64_t pitch, float* __restrict__ scale) {
   __shared__ uint32_t part[8];
   let_next_kernel_start();
+  constexpr int kKept = 4, kStep = 32 * W * 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = (int)threadIdx.x & (32 * W - 1);
   const int64_t row = (int64_t)blockIdx.x * (8 / W) + warp / W;
   const bool live = row < rows;
   if (!live) cols = pitch = 0;
   const T* xr = x + (live ? row : 0) * rs;
-  constexpr int kStep = 32 * W * 8;  // elements per step of the group
-  float kept[kVecs][8];
-  float most = 0.0f;
+  const uint32_t off = (uint32_t)((uintptr_t)xr & 15u);
+  const RowReader<T, ALIGNED> in = {xr, cols, cs, contiguous ? (off ? kShifted : kAligned) : kElements, off};
+  Vec8<T> kept[kKept];
+  MaxOf<T> most;
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const int64_t c = (int64_t)v * kStep + 8 * t;
-    if (vectors && c + 8 <= cols) {
-      unpack8(load8(xr + c), kept[v]);
-    } else {
+  for (int v = 0; v < kKept; ++v) kept[v] = in.vector((int64_t)v * kStep + 8 * t);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) kept[v][i] = c + i < cols ? to_f32(xr[(c + i) * cs]) : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max_abs(most, kept[v][i]);
-  }
-  for (int64_t c = (int64_t)kVecs * kStep + 8 * t; c < cols; c += kStep) {
-    if (vectors && c + 8 <= cols) {
-      float f[8];
-      unpack8(load8(xr + c), f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = max_abs(most, f[i]);
-    } else {
-      for (int i = 0; i < 8 && c + i < cols; ++i) most = max_abs(most, to_f32(xr[(c + i) * cs]));
-    }
-  }
-  uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most));
+  for (int v = 0; v < kKept; ++v) add_vector<T>(most, kept[v]);
+  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < cols; c += kStep) add_vector<T>(most, in.vector(c));
+  uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most.value()));
   if (W > 1) {
     if (lane == 0) part[warp] = top;
     __syncthreads();
@@ -64,22 +142,11 @@ __global__ void __launch_bounds__(256)
   if (live && t == 0) scale[row] = s.scale;
   int8_t* qr = q + row * pitch;  // pitch is a multiple of 16; columns from cols to pitch are written as zeros
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
+  for (int v = 0; v < kKept; ++v) {
     const int64_t c = (int64_t)v * kStep + 8 * t;
-    if (c < pitch) {
-      *reinterpret_cast<uint2*>(qr + c) = quantize8(kept[v], s.inv);
-    }
+    if (c < pitch) store_vector<T>(qr + c, kept[v], s.inv);
   }
-  for (int64_t c = (int64_t)kVecs * kStep + 8 * t; c < pitch; c += kStep) {
-    float f[8];
-    if (vectors && c + 8 <= cols) {
-      unpack8(load8(xr + c), f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = c + i < cols ? to_f32(xr[(c + i) * cs]) : 0.0f;
-    }
-    *reinterpret_cast<uint2*>(qr + c) = quantize8(f, s.inv);
-  }
+  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < pitch; c += kStep) store_vector<T>(qr + c, in.vector(c), s.inv);
 }
 
 // Rows adjacent in memory (row stride 1): lane = row, warp w takes columns w, w + 8, ... of the CTA's share.
@@ -175,15 +242,19 @@ int launch_quantize(const T* x, int64_t rows, int64_t cols, int64_t rs, int64_t 
     return launch_clusters((const void*)k_quantize_cols<T>, (unsigned)((rows + 31) / 32 * kColsCluster), kColsCluster, 256,
                            smem, params, st, "k_quantize_cols launch");
   }
-  const int vectors = cs == 1 && (uintptr_t)x % 16 == 0 && (rs * (int64_t)sizeof(T)) % 16 == 0;
-  if (cols <= 1024)
-    k_quantize_rows<T, 1><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(x, rows, cols, rs, cs, vectors, q, pitch, scale);
-  else if (cols <= 2048)
-    k_quantize_rows<T, 2><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(x, rows, cols, rs, cs, vectors, q, pitch, scale);
-  else if (cols <= 4096)
-    k_quantize_rows<T, 4><<<(unsigned)((rows + 1) / 2), 256, 0, st>>>(x, rows, cols, rs, cs, vectors, q, pitch, scale);
+  const int contiguous = cs == 1;
+  const bool aligned = contiguous && (uintptr_t)x % 16 == 0 && (rs * (int64_t)sizeof(T)) % 16 == 0;
+  const int warps = cols <= 1024 ? 1 : (cols <= 2048 ? 2 : (cols <= 4096 ? 4 : 8));
+  const unsigned grid = (unsigned)((rows + 8 / warps - 1) / (8 / warps));
+  const auto run = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(x, rows, cols, rs, cs, contiguous, q, pitch, scale); };
+  if (warps == 1)
+    aligned ? run(k_quantize_rows<T, 1, true>) : run(k_quantize_rows<T, 1, false>);
+  else if (warps == 2)
+    aligned ? run(k_quantize_rows<T, 2, true>) : run(k_quantize_rows<T, 2, false>);
+  else if (warps == 4)
+    aligned ? run(k_quantize_rows<T, 4, true>) : run(k_quantize_rows<T, 4, false>);
   else
-    k_quantize_rows<T, 8><<<(unsigned)rows, 256, 0, st>>>(x, rows, cols, rs, cs, vectors, q, pitch, scale);
+    aligned ? run(k_quantize_rows<T, 8, true>) : run(k_quantize_rows<T, 8, false>);
   return launch_status("k_quantize_rows launch");
 }
 
