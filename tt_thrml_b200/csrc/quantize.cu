@@ -53,10 +53,12 @@ struct RowReader {
     }
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(T) / 2); ++i) v.w[i] = make_uint4(0u, 0u, 0u, 0u);
-    T* e = reinterpret_cast<T*>(&v);
+    if (c < cols) {
+      T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < cols) e[i] = x[(c + i) * cs];
+      for (int i = 0; i < 8; ++i)
+        if (c + i < cols) e[i] = x[(c + i) * cs];
+    }
     return v;
   }
 };
