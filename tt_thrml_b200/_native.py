@@ -90,6 +90,16 @@ class AdamWTensor(ctypes.Structure):
     ]
 
 
+class AdamWCall(ctypes.Structure):
+    """AdamWCall (csrc/hostcall.cpp): what stays the same from step to step."""
+
+    _fields_ = [
+        ("rows", c_vp), ("n_rows", c_i64), ("state_bits", c_i64), ("exp_avg", c_vp), ("exp_avg_sq", c_vp),
+        ("exp_avg_scale", c_vp), ("exp_avg_sq_scale", c_vp), ("ctl", c_vp), ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double), ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("seed", c_u64),
+    ]
+
+
 class PackMatrix(ctypes.Structure):
     """tthrml_pack_matrix (include/tthrml.h)."""
 

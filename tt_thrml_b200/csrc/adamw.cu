@@ -473,11 +473,16 @@ extern "C" int tthrml_adamw_step(const tthrml_adamw_tensor* tensors_host, int64_
   for (int64_t i = 0; i < n_tensors; i += kMost) {
     const int32_t n = (int32_t)(n_tensors - i < kMost ? n_tensors - i : kMost);
     a.last = i + n == n_tensors;
+    // a launch copies its whole table: the smallest that holds the tensors (25 tensors: 8.6 us a step with the largest)
     int rc;
     if (state_bits == 32)
-      rc = n <= 24 ? launch_adamw<32, 24>(tensors_host + i, n, a, sms, st) : launch_adamw<32, kMost>(tensors_host + i, n, a, sms, st);
+      rc = n <= 24    ? launch_adamw<32, 24>(tensors_host + i, n, a, sms, st)
+           : n <= 150 ? launch_adamw<32, 150>(tensors_host + i, n, a, sms, st)
+                      : launch_adamw<32, kMost>(tensors_host + i, n, a, sms, st);
     else
-      rc = n <= 24 ? launch_adamw<8, 24>(tensors_host + i, n, a, sms, st) : launch_adamw<8, kMost>(tensors_host + i, n, a, sms, st);
+      rc = n <= 24    ? launch_adamw<8, 24>(tensors_host + i, n, a, sms, st)
+           : n <= 150 ? launch_adamw<8, 150>(tensors_host + i, n, a, sms, st)
+                      : launch_adamw<8, kMost>(tensors_host + i, n, a, sms, st);
     if (rc) return rc;
   }
   return TTHRML_OK;

@@ -25,19 +25,58 @@ bool plain_cuda(const at::Tensor& t, long device) {
   return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() && !t.is_conj();
 }
 
-// adamw_rows(params, grads, rows address, number of rows, device) -> -1, or the place of the first pair that is not the
-// plain case (the parameter as the row has it, a gradient of its sizes and strides and of its type or float32).  Fills the
-// gradients' addresses and types into the rows (tthrml_adamw_tensor), which stand for the parameters with elements.
-PyObject* adamw_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// Tells autograd that the tensors of a list were written.
+void bump(PyObject* list) {
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    if (!THPVariable_Check(o)) continue;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+}
+PyObject* bump_versions(PyObject*, PyObject* list) {
   HANDLE_TH_ERRORS
-  if (nargs != 5 || !PyList_Check(args[0]) || !PyList_Check(args[1]) ||
-      PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1])) {
-    PyErr_SetString(PyExc_TypeError, "adamw_rows(params, grads, rows, n_rows, device): two lists of one length");
+  if (!PyList_Check(list)) {
+    PyErr_SetString(PyExc_TypeError, "bump_versions(tensors): a list");
     return nullptr;
   }
-  auto* rows = reinterpret_cast<tthrml_adamw_tensor*>(PyLong_AsVoidPtr(args[2]));
-  const Py_ssize_t n_rows = PyLong_AsSsize_t(args[3]);
-  const long device = PyLong_AsLong(args[4]);
+  bump(list);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+template <typename Fn>
+Fn address(PyObject* o) {
+  return reinterpret_cast<Fn>(PyLong_AsVoidPtr(o));
+}
+bool wants_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
+// What stays the same from step to step of an optimizer (AdamWCall in _native.py).
+struct AdamWCall {
+  tthrml_adamw_tensor* rows;  // of the parameters that have elements
+  int64_t n_rows;
+  int64_t state_bits;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  tthrml_adamw_ctl* ctl;
+  double beta1, beta2, eps, weight_decay;
+  uint64_t seed;
+};
+using AdamWFn = decltype(&tthrml_adamw_step);
+
+// adamw_step(params, grads, call, function, stream, device) -> -1 for a step queued, the place of the first pair that is not
+// the plain case (the parameter as its row has it, a gradient of its sizes and strides and of its type or float32), or an
+// error code less 1000.
+PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6 || !PyList_Check(args[0]) || !PyList_Check(args[1]) ||
+      PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "adamw_step(params, grads, call, function, stream, device): two lists of one length");
+    return nullptr;
+  }
+  AdamWCall* call = address<AdamWCall*>(args[2]);
+  void* stream = PyLong_AsVoidPtr(args[4]);
+  const long device = PyLong_AsLong(args[5]);
   if (PyErr_Occurred()) return nullptr;
   Py_ssize_t row = 0;
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
@@ -51,38 +90,21 @@ PyObject* adamw_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         (gd != TTHRML_DT_F32 && gd != dtype_code(p)))
       return PyLong_FromSsize_t(i);
     if (p.numel() == 0) continue;
-    if (row >= n_rows) return PyLong_FromSsize_t(i);
-    tthrml_adamw_tensor& r = rows[row++];
+    if (row >= call->n_rows) return PyLong_FromSsize_t(i);
+    tthrml_adamw_tensor& r = call->rows[row++];
     if (r.param != p.data_ptr() || r.n != p.numel() || r.param_dtype != dtype_code(p)) return PyLong_FromSsize_t(i);
     r.grad = g.data_ptr();
     r.grad_dtype = gd;
   }
-  return PyLong_FromSsize_t(row == n_rows ? -1 : n - 1);
+  if (row != call->n_rows) return PyLong_FromSsize_t(n - 1);
+  const int rc = address<AdamWFn>(args[3])(call->rows, call->n_rows, (int32_t)call->state_bits, call->exp_avg,
+                                           call->exp_avg_sq, call->exp_avg_scale, call->exp_avg_sq_scale, call->ctl,
+                                           call->beta1, call->beta2, call->eps, call->weight_decay, call->seed, stream);
+  if (rc) return PyLong_FromLong(rc - 1000);
+  bump(args[0]);
+  return PyLong_FromLong(-1);
   END_HANDLE_TH_ERRORS
 }
-
-// bump_versions(tensors): tells autograd that the tensors were written.
-PyObject* bump_versions(PyObject*, PyObject* list) {
-  HANDLE_TH_ERRORS
-  if (!PyList_Check(list)) {
-    PyErr_SetString(PyExc_TypeError, "bump_versions(tensors): a list");
-    return nullptr;
-  }
-  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-    PyObject* o = PyList_GET_ITEM(list, i);
-    if (!THPVariable_Check(o)) continue;
-    const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  }
-  Py_RETURN_NONE;
-  END_HANDLE_TH_ERRORS
-}
-
-template <typename Fn>
-Fn address(PyObject* o) {
-  return reinterpret_cast<Fn>(PyLong_AsVoidPtr(o));
-}
-bool wants_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 
 using LinearFn = decltype(&tthrml_int8_linear);
 using MomentsFn = decltype(&tthrml_pair_moments);
@@ -218,8 +240,8 @@ PyMethodDef methods[] = {
      "Product of float rows and 8-bit weights: the plain case, or None."},
     {"pair_moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pair_moments)), METH_FASTCALL,
      "Pair moments of lists of phases: the plain case, or None."},
-    {"adamw_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_rows)), METH_FASTCALL,
-     "Fills gradient addresses into AdamW rows; -1 or the first pair that needs a closer look."},
+    {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_step)), METH_FASTCALL,
+     "A step of all parameters: the plain case, or where it is not."},
     {"bump_versions", bump_versions, METH_O, "Marks tensors as written for autograd."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", "Host side of calls with many tensors.", -1, methods,

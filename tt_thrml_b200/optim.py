@@ -16,10 +16,12 @@ graphs.  Nothing synchronises.
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 
 from . import _native as nat
-from .quantized import dtype_code, on_device, raw_stream, require_cuda
+from .quantized import current_device, dtype_code, on_device, raw_stream, require_cuda
 
 BLOCK = 256  # elements per scale of 8-bit moments; segments of the moments are padded to it
 
@@ -103,10 +105,12 @@ class AdamW:
                              ("param", [p.data_ptr() for p in self.params]),
                              ("param_dtype", [dtype_code(p.dtype) for p in self.params])):
             self._rows[name] = [values[i] for i in self._live]
-        self._rows_at, self._n_rows = self._rows.ctypes.data, len(self._rows)
-        self._host, self._lib = nat.hostcall(), nat.lib()
-        self._state_ptrs = tuple(None if t is None else t.data_ptr() for t in
-                                 (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self._ctl))
+        self._host = nat.hostcall()
+        at = [None if t is None else t.data_ptr() for t in
+              (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self._ctl)]
+        self._call = nat.AdamWCall(self._rows.ctypes.data, len(self._rows), self.state_bits, *at, *self.betas, self.eps,
+                                   self.weight_decay, self.seed)
+        self._call_at, self._entry = ctypes.addressof(self._call), nat.address_of("tthrml_adamw_step")
 
     # ---------------------------------------------------------------- control
 
@@ -160,14 +164,20 @@ class AdamW:
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} parameters, {len(grads)} gradients")
         index = self.device.index
-        if self._host.adamw_rows(self.params, grads, self._rows_at, self._n_rows, index) >= 0:
-            self._check(grads)
-        m, v, ms, vs, ctl = self._state_ptrs
+        if current_device() == index:
+            nat.bind_device(index)
+            done = self._host.adamw_step(self.params, grads, self._call_at, self._entry, raw_stream(index), index)
+            if done == -1:
+                return
+            if done < -1:
+                nat.check(done + 1000, "tthrml_adamw_step")
+        self._check(grads)
+        c = self._call
         with on_device(self.device):
             nat.check(
-                self._lib.tthrml_adamw_step(
-                    self._rows_at, self._n_rows, self.state_bits, m, v, ms, vs, ctl, self.betas[0], self.betas[1],
-                    self.eps, self.weight_decay, self.seed, raw_stream(index),
+                nat.lib().tthrml_adamw_step(
+                    c.rows, c.n_rows, c.state_bits, c.exp_avg, c.exp_avg_sq, c.exp_avg_scale, c.exp_avg_sq_scale, c.ctl,
+                    c.beta1, c.beta2, c.eps, c.weight_decay, c.seed, raw_stream(index),
                 ),
                 "tthrml_adamw_step",
             )
@@ -182,16 +192,17 @@ class AdamW:
         m, v = self.exp_avg, self.exp_avg_sq
         if self.state_bits == 8:
             m, v = (torch.empty(t.shape, dtype=torch.float32, device=self.device) for t in (m, v))
+            c = self._call
             with on_device(self.device):
                 nat.check(
                     nat.lib().tthrml_adamw_values(
-                        *self._state_ptrs[:4], m.numel(), m.data_ptr(), v.data_ptr(),
+                        c.exp_avg, c.exp_avg_sq, c.exp_avg_scale, c.exp_avg_sq_scale, m.numel(), m.data_ptr(), v.data_ptr(),
                         raw_stream(self.device.index),
                     ),
                     "tthrml_adamw_values",
                 )
         if flat:
-            return m[: self.elements], v[: self.elements]
+            return (m, v) if m.numel() == self.elements else (m[: self.elements], v[: self.elements])
         return tuple([torch.as_strided(t, p.shape, p.stride(), o) if p.numel() else t[:0].view(p.shape)
                       for p, o in zip(self.params, self.offsets)] for t in (m, v))
 
