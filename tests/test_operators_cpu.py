@@ -49,6 +49,19 @@ def moments(ph, n=1, dt=1, m=8, k=8, out=_A, ld=8, err=_A):
     return ph, n, dt, m, k, out, ld, None, None, 0, err, None
 
 
+def linear(x=_A, dt=1, rows=20, cols=40, rs=40, cs=1, ws=None, size=0, w=_A, wp=48, scale=_A, units=8, out=_A, od=1, ld=8, err=_A):
+    return x, dt, rows, cols, rs, cs, ws, size, w, wp, scale, units, None, out, od, ld, err, None
+
+
+def pack(**kw):
+    rows = (nat.PackMatrix * 1)()
+    r = rows[0]
+    r.src, r.dst, r.rows, r.cols, r.row_stride, r.col_stride, r.pitch = _A, _A, 3, 5, 5, 1, 8
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return rows
+
+
 def adamw(t, n=1, bits=32, m=_A, v=_A, ms=None, vs=None, ctl=_A, b1=0.9, b2=0.99, eps=1e-8, wd=0.0):
     return t, n, bits, m, v, ms, vs, ctl, b1, b2, eps, wd, 0, None
 
@@ -95,6 +108,21 @@ BAD = [
     ("tthrml_pair_moments", moments(phases(y_ld=60)), b"16-byte aligned"),
     ("tthrml_pair_moments", moments(phases(x_ld=8), m=9), b"16-byte aligned"),
     ("tthrml_pair_moments", moments(phases(chains=-1)), b"16-byte aligned"),
+    ("tthrml_int8_linear", linear(), b"workspace"),
+    ("tthrml_int8_linear", linear(ws=_A, size=979), b"needs a 16-byte aligned workspace of 1040 bytes"),
+    ("tthrml_int8_linear", linear(ws=_M, size=4096), b"workspace"),
+    ("tthrml_int8_linear", linear(rows=1, cs=2), b"workspace"),
+    ("tthrml_int8_linear", linear(rows=2, rs=39), b"workspace"),
+    ("tthrml_int8_linear", linear(cols=0), b"out of range"),
+    ("tthrml_int8_linear", linear(rows=2, w=None), b"NULL"),
+    ("tthrml_int8_linear", linear(rows=1, dt=9), b"unknown element type"),
+    ("tthrml_pack_rows", (None, 1, None), b"matrices"),
+    ("tthrml_pack_rows", (pack(), 13, None), b"0 to 12 matrices"),
+    ("tthrml_pack_rows", (pack(pitch=4), 1, None), b"matrix 0"),
+    ("tthrml_pack_rows", (pack(pitch=12), 1, None), b"matrix 0"),
+    ("tthrml_pack_rows", (pack(dst=_M), 1, None), b"matrix 0"),
+    ("tthrml_pack_rows", (pack(src=_A + 1), 1, None), b"matrix 0"),
+    ("tthrml_pair_moments_packed", (pack(rows=-1), 1, *moments(phases())), b"matrix 0"),
     ("tthrml_adamw_step", adamw(None), b"NULL"),
     ("tthrml_adamw_step", adamw(tensors(), bits=8), b"NULL"),
     ("tthrml_adamw_step", adamw(tensors(), bits=16), b"8 or 32"),
@@ -123,6 +151,10 @@ def test_bad_arguments_are_rejected_before_any_cuda_call(name, args, message):
     ("tthrml_int8_product", product(rows=0, x=None)),
     ("tthrml_int8_product", product(units=0, w=None)),
     ("tthrml_int8_product_few", few(rows=0, x=None)),
+    ("tthrml_int8_linear", linear(rows=0, x=None)),
+    ("tthrml_int8_linear", linear(units=0, w=None)),
+    ("tthrml_pack_rows", (None, 0, None)),
+    ("tthrml_pack_rows", (pack(rows=0, src=None), 1, None)),
     ("tthrml_adamw_step", adamw(None, n=0)),
     ("tthrml_adamw_values", (None, None, None, None, 0, None, None, None)),
 ])
@@ -132,6 +164,33 @@ def test_empty_calls_do_nothing(name, args):
 
 def test_structures_have_the_header_layout():
     assert ctypes.sizeof(nat.AdamWTensor) == 40 and ctypes.sizeof(nat.MomentPhase) == 56
+    assert ctypes.sizeof(nat.PackMatrix) == 56 and ctypes.sizeof(nat.AdamWCall) == 104
+
+
+def test_workspace_of_the_linear_entry():
+    lib = nat.lib()
+    assert lib.tthrml_int8_linear_workspace(1, 163840) == 0 and lib.tthrml_int8_linear_workspace(2, 81920) == 0
+    assert lib.tthrml_int8_linear_workspace(2, 81921) == 2 * 81936 + 16
+    assert lib.tthrml_int8_linear_workspace(20, 40) == 20 * 48 + 80
+
+
+def test_host_module_leaves_other_cases_to_python():
+    host, x = nat.hostcall(), torch.ones((2, 4))
+    assert host.int8_product(x, x, x[0], 16, None, 0, 0, 0, 0) is None
+    assert host.int8_product("x", x, x[0], 16, None, 0, 0, 0, 0) is None
+    assert host.pair_moments([x], [x], [1.0], False, 0, 0, 0, 0, 0) is None
+    assert host.pair_moments([x], [], [1.0], False, 0, 0, 0, 0, 0) is None
+    call = nat.AdamWCall()
+    assert host.adamw_step([x], [x], ctypes.addressof(call), 0, 0, 0) == 0  # the first pair is not on the device
+    assert host.adamw_step([x], [None], ctypes.addressof(call), 0, 0, 0) == 0
+    for bad in ((), ([x], [x, x], 0, 0, 0, 0), ((x,), [x], 0, 0, 0, 0)):
+        with pytest.raises(TypeError):
+            host.adamw_step(*bad)
+    version = x._version
+    host.bump_versions([x, 3])
+    assert x._version == version + 1
+    with pytest.raises(TypeError):
+        host.bump_versions(x)
 
 
 def test_cpu_tensors_are_refused():
