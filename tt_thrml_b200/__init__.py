@@ -5,7 +5,9 @@ on the GPU, same public surface as tt-thrml (tt_thrml/__init__.py:1-96):
 sample_states, sample_with_observation, make_executor/Executor,
 make_mesh_executor/MeshExecutor, GaussianConditional, the device helpers and
 the configuration factory (make_cuda_config; make_ttmlir_config kept for
-drop-in callers).
+drop-in callers).  Around dense programs: 8-bit integer products
+(quantize_rows, int8_product), pair moments (pair_moments, dense_moments),
+AdamW over many tensors and DenseLearner.
 """
 
 from .compiler import compile_program
