@@ -293,12 +293,6 @@ __device__ __forceinline__ void drain(const unsigned char* turn, int bytes, unsi
                                       int m0, int M, int live_bytes) {
   const int lane = threadIdx.x & 31, per_row = bytes / (int)sizeof(V), rows = 32 / per_row;
   const int k = (lane % per_row) * (int)sizeof(V);
-  if (rows == 0) {  // more pieces than lanes: several per lane and row
-    for (int r = 0; r < 32 && m0 + r < M; ++r)
-      for (int j = lane * (int)sizeof(V); j < live_bytes; j += 32 * (int)sizeof(V))
-        *reinterpret_cast<V*>(out + (int64_t)(m0 + r) * pitch + at + j) = *reinterpret_cast<const V*>(turn + r * kTurnPitch + j);
-    return;
-  }
   if (k >= live_bytes) return;
 #pragma unroll 4
   for (int r = lane / per_row; r < 32 && m0 + r < M; r += rows)
@@ -480,6 +474,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int quad = warp & 3, grp = (warp - 2) >> 2;
     unsigned char* turn = turns + (warp - 2) * 32 * kTurnPitch;
     int it = 0;
+    bool failed = false;
     for (int t = first; t < n_tiles; t += step, ++it) {
       int mb, nb;
       tile_coords(t, m_blocks, n_blocks, args.d.group, mb, nb);
@@ -494,10 +489,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         sw[256 + j] = EPI == kStoreFields && a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      if (!mbar_wait(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
+      if (!failed && !mbar_wait(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
         if (lane == 0) atomicExch(a.error, kErrAccWait);
-        break;
+        failed = true;
       }
+      if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
       tc_fence_after();
       const uint32_t sweep = args.d.sweep + (EPI != kStoreFields && args.d.ctl ? args.d.ctl->sweep : 0u);
       const uint64_t sd = EPI != kStoreFields && args.d.ctl ? args.d.ctl->seed : args.d.seed;

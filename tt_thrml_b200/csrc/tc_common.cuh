@@ -108,6 +108,7 @@ __device__ __forceinline__ uint32_t n_clusters_x() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();  // the barrier is a whole warp's
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_leader, int c0,
