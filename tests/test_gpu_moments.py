@@ -93,6 +93,20 @@ def test_accumulate_output_strides_and_untouched_columns(tt):
     assert (big[:, :7] == 3).all() and (big[:, 137:] == 3).all()
 
 
+@pytest.mark.parametrize("m,n,pitch", [(2305, 2080, 2080), (2305, 2077, 2080), (2300, 2049, 2049), (2049, 2336, 2343)])
+def test_sums_added_to_large_outputs(tt, m, n, pitch):
+    """Whole numbers: rows that start on 16 bytes and others, tiles cut off in rows and columns."""
+    x, y = ints((70, m), 5, 1).to(BF16), ints((70, n), 5, 2).to(BF16)
+    w, _, _, _ = exact([x], [y], [1.0])
+    start = ints((m, pitch), 9, 3)
+    out = start.cuda()
+    tt.pair_moments(x.cuda(), y.cuda(), 2.0, out=out[:, :n], accumulate=True)
+    assert torch.equal(out[:, :n].cpu().double(), start[:, :n].double() + 2 * w)
+    assert torch.equal(out[:, n:].cpu(), start[:, n:])
+    tt.pair_moments(x.cuda(), y.cuda(), out=out[:, :n])
+    assert torch.equal(out[:, :n].cpu().double(), w) and torch.equal(out[:, n:].cpu(), start[:, n:])
+
+
 def test_strides_of_the_operands(tt):
     base = ints((400, 333), 6, 3).to(F16)
     y = ints((200, 48), 6, 4).to(F16)

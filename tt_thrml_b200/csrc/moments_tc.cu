@@ -419,8 +419,45 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
 // CTA-pair kernel
 // ---------------------------------------------------------------------------
 constexpr int kPairStages = 6, kPairHalf = 128 * 64 * 2, kPairStage = 2 * kPairHalf;
-constexpr int kTurnPitch = 33;  // floats per row of a warp's 32 x 32 transpose (outputs whose rows are not aligned)
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 /*barriers*/ + 256 /*unit sums*/ + 8 * 32 * kTurnPitch * 4;
+constexpr int kTurnBytes = 32 * 128;  // a warp's 32 x 32 floats, turned on their way out
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 /*barriers*/ + 256 /*unit sums*/ + 8 * kTurnBytes;
+
+__device__ __forceinline__ float added(float a, float b) { return a + b; }
+__device__ __forceinline__ float4 added(const float4& a, const float4& b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+// Stores (or adds) a warp's turned 32 x 32 floats to the rows at o, V at a time: each access of the warp covers whole lines of
+// one row (float) or four (float4), where each lane storing its own row touched 32 lines (4096 x 8192, 256 chains: 76 us, now
+// 50).  What is added to is read a batch ahead of its stores, which would otherwise order every read behind the store before
+// it (adding to 4096 x 8192 floats, 256 chains: 192 us, now 105; to 4096 x 8191, 1024 chains: 409 us, now 148).
+template <typename V>
+__device__ __forceinline__ void put_rows(const unsigned char* turn, float* o, int64_t ld, int rows, int live, bool add) {
+  constexpr int kPerRow = 128 / (int)sizeof(V), kRows = 32 / kPerRow, kBatch = sizeof(V) == 16 ? 4 : 8;
+  const int lane = threadIdx.x & 31, k = lane % kPerRow * (int)sizeof(V);
+  if (k / 4 >= live) return;
+  o += k / 4;
+  auto staged = [&](int r) {
+    return *reinterpret_cast<const V*>(turn + r * 128 + ((k & ~15) ^ ((r & 7) << 4)) + (k & 15));
+  };
+  int r0 = lane / kPerRow;
+  if (!add) {
+#pragma unroll 8
+    for (int r = r0; r < rows; r += kRows) *reinterpret_cast<V*>(o + (int64_t)r * ld) = staged(r);
+    return;
+  }
+#pragma unroll 1
+  for (; r0 < rows; r0 += kBatch * kRows) {
+    V old[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      old[i] = *reinterpret_cast<const V*>(o + (int64_t)min(r0 + i * kRows, rows - 1) * ld);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = r0 + i * kRows;
+      if (r < rows) *reinterpret_cast<V*>(o + (int64_t)r * ld) = added(staged(r), old[i]);
+    }
+  }
+}
 
 __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -563,7 +600,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
     side_sums(a, side);
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
-    float* turn = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 512) + (warp - 2) * 32 * kTurnPitch;
+    unsigned char* turn = tiles + kPairStages * kPairStage + 512 + (warp - 2) * kTurnBytes;
     int chunk = 0;
     bool failed = false;
     for (int t = first; t < n_tiles && !failed; t += step) {
@@ -595,40 +632,21 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
         b += c.length;
       }
       if (failed) break;
-      const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane, n = nb * 256 + half * 128;
-      float* o = a.out + (int64_t)m * a.out_ld + n;
+      const int m0 = mb * 256 + (int)rank * 128 + quad * 32, n = nb * 256 + half * 128;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int nq = n + q * 32;
-        if (a.vector_store && nq + 32 <= a.N) {  // each lane its own row, 128 bytes of it
-          if (m < a.M) {
+      for (int q = 0; q < 4; ++q) {  // 32 columns of the warp's 32 rows at a time
+        const int live = min(32, a.N - n - q * 32), rows = min(32, a.M - m0);
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              float4 s = make_float4(acc[q * 32 + j], acc[q * 32 + j + 1], acc[q * 32 + j + 2], acc[q * 32 + j + 3]);
-              float4* at = reinterpret_cast<float4*>(o + q * 32 + j);
-              if (a.accumulate) {
-                const float4 old = *at;
-                s = make_float4(old.x + s.x, old.y + s.y, old.z + s.z, old.w + s.w);
-              }
-              *at = s;
-            }
-          }
-        } else {  // by way of shared memory, so that a warp stores consecutive columns
-#pragma unroll
-          for (int j = 0; j < 32; ++j) turn[lane * kTurnPitch + j] = acc[q * 32 + j];
-          __syncwarp();
-          if (nq + lane < a.N) {
-            float* row = a.out + (int64_t)(m - lane) * a.out_ld + nq + lane;
-#pragma unroll 8
-            for (int r = 0; r < 32; ++r) {
-              if (m - lane + r < a.M) {
-                const float v = turn[r * kTurnPitch + lane];
-                row[r * a.out_ld] = a.accumulate ? row[r * a.out_ld] + v : v;
-              }
-            }
-          }
-          __syncwarp();
-        }
+        for (int j = 0; j < 8; ++j)  // piece j of row r lies at j ^ (r & 7): rows and columns both cover every bank
+          *reinterpret_cast<float4*>(turn + lane * 128 + 16 * (j ^ (lane & 7))) =
+              make_float4(acc[q * 32 + 4 * j], acc[q * 32 + 4 * j + 1], acc[q * 32 + 4 * j + 2], acc[q * 32 + 4 * j + 3]);
+        __syncwarp();
+        float* o = a.out + (int64_t)m0 * a.out_ld + n + q * 32;
+        if (a.vector_store && live == 32)
+          put_rows<float4>(turn, o, a.out_ld, rows, live, a.accumulate != 0);
+        else
+          put_rows<float>(turn, o, a.out_ld, rows, live, a.accumulate != 0);
+        __syncwarp();
       }
     }
   }
