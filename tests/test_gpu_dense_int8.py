@@ -385,6 +385,28 @@ def test_mesh_of_one_and_shared_weights():
         Executor(None, dev, program, make_cuda_config(n_chains=C, dense_precision="bf16")).share_dense_weights(one)
 
 
+@pytest.mark.parametrize("precision", ["int8", "bf16"])
+def test_weights_shared_before_the_first_update(precision):
+    import tt_thrml_b200 as tt
+
+    program, C = rbm(), 128
+    cfg = make_cuda_config(n_chains=C, dense_precision=precision)
+    dev = tt.open_device(device_id=0)
+    one, two, other = (Executor(None, dev, program, cfg, n_sweeps=8) for _ in range(3))
+    two.share_dense_weights(one)
+    new = rbm(seed=9)
+    one.update_dense_weights(torch.from_numpy(new.W).cuda(), torch.from_numpy(new.b_v).cuda())
+    for p, q, kept in zip(one._plans(), two._plans(), other._plans()):
+        assert p.weights_nk.data_ptr() == q.weights_nk.data_ptr() and p.bias.data_ptr() == q.bias.data_ptr()
+        assert not torch.equal(p.weights_nk, kept.weights_nk)  # an executor that does not share keeps the program's
+    init = [np.linspace(-1, 1, 256, dtype=F) + np.zeros((C, 1), F), np.ones((C, 512), bool)]
+    for ex in (one, two):
+        ex.load_state(init, [])
+        ex.prepare_rng(4)
+        ex.run_sweeps(3)
+    assert np.array_equal(one.raw_state(), two.raw_state())
+
+
 def test_learner_refusals():
     import tt_thrml_b200 as tt
 

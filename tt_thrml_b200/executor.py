@@ -1059,11 +1059,7 @@ class Executor:
         self._stream.wait_stream(current)
         with torch.no_grad(), torch.cuda.stream(self._stream):
             for plan, w, bias in ((plans[0], weights, bias_0), (plans[1], weights.t(), bias_1)):
-                if not plan.owned:
-                    plan.weights_nk, plan.bias = plan.weights_nk.clone(), plan.bias.clone()
-                    plan.w_scale = None if plan.w_scale is None else plan.w_scale.clone()
-                    plan.owned = True
-                    self._graphs.clear()
+                self._own_operands(plan)
                 if plan.w_scale is not None:
                     nat.check(
                         self._lib.tthrml_quantize_rows(
@@ -1082,6 +1078,15 @@ class Executor:
                     plan.bias.copy_(bias)
         current.wait_stream(self._stream)
 
+    def _own_operands(self, plan) -> None:
+        """Operands of this executor's own in place of the plan cache's, once; call it on the executor's stream."""
+        if plan.owned:
+            return
+        plan.weights_nk, plan.bias = plan.weights_nk.clone(), plan.bias.clone()
+        plan.w_scale = None if plan.w_scale is None else plan.w_scale.clone()
+        plan.owned = True
+        self._graphs.clear()
+
     def share_dense_weights(self, other: "Executor") -> None:
         """Runs this executor's sweeps on another one's operands (weights and biases) from now on: what
         update_dense_weights writes there holds here too.  Both need the same program shape, precision, device and
@@ -1092,9 +1097,13 @@ class Executor:
         for p, q in zip(mine, theirs):
             if p.weights_nk.shape != q.weights_nk.shape or p.weights_nk.dtype != q.weights_nk.dtype or p.family != q.family:
                 raise ValueError("executors of different programs or precisions cannot share their weights")
+        nat.bind_device(self._tdev.index)
+        with _torch().cuda.stream(self._stream):
+            for q in theirs:
+                other._own_operands(q)  # else the other's first update would take new ones and leave this executor behind
         for p, q in zip(mine, theirs):
             if p.weights_nk is not q.weights_nk or p.bias is not q.bias:
-                p.weights_nk, p.w_scale, p.bias, p.owned = q.weights_nk, q.w_scale, q.bias, q.owned
+                p.weights_nk, p.w_scale, p.bias, p.owned = q.weights_nk, q.w_scale, q.bias, True
                 self._graphs.clear()
 
     def _dense_phases(self, scale: float) -> list:
