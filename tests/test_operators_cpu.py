@@ -224,3 +224,24 @@ def test_host_quantisation_and_the_int8_plan():
         tt.make_cuda_config(dense_precision="int4")
     a, b = tt.make_cuda_config(dense_precision="int8"), tt.make_cuda_config(dense_precision="bf16")
     assert a.resolved_dense_precision == "int8" and a.plan_key() != b.plan_key()
+
+
+def test_an_error_on_another_device_leaves_no_binding(monkeypatch):
+    """The library's device is looked up again after a call on a device that is not current, also one that raises."""
+    import contextlib
+    import types
+
+    from tt_thrml_b200 import quantized
+
+    bound = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(nat, "lib", lambda: types.SimpleNamespace(tthrml_set_device=lambda i: bound.append(i) or nat.OK))
+    monkeypatch.setattr(nat, "_bound", types.SimpleNamespace())
+    with pytest.raises(RuntimeError, match="inside"):
+        with quantized.on_device(torch.device("cuda", 1)):
+            assert nat._bound.device == 1
+            raise RuntimeError("inside")
+    assert nat._bound.device is None
+    nat.bind_device(0)
+    assert bound == [1, 0]

@@ -84,8 +84,10 @@ def _other_device(index: int):
     with torch.cuda.device(index):
         nat.check(nat.lib().tthrml_set_device(index), "tthrml_set_device")
         nat._bound.device = index
-        yield
-    nat._bound.device = None  # the library's current device follows torch's again at the next call
+        try:
+            yield
+        finally:
+            nat._bound.device = None  # the library's current device follows torch's again at the next call
 
 
 def on_device(device):
