@@ -673,7 +673,7 @@ typedef struct tthrml_moment_phase {
   const void* y;  /* [chains][y_ld], likewise */
   int64_t x_ld, y_ld, chains; /* chains may be 0 */
   float scale;    /* of x^T y */
-  float x_scale, y_scale; /* of the unit sums */
+  float x_scale, y_scale; /* of the unit sums; 0 with a scale that is not: the phase is left out of them */
   float reserved;
 } tthrml_moment_phase;
 

@@ -140,6 +140,20 @@ def test_values_that_are_not_finite_stay_with_their_units(tt):
     assert torch.isnan(sx[3]) and torch.isinf(sy[299]) and torch.isfinite(sx[4:]).all() and torch.isfinite(sy[:299]).all()
 
 
+def test_a_phase_of_scale_zero_is_zero_times_its_sums(tt):
+    x, y = torch.ones((70, 40), dtype=BF16), torch.ones((70, 90), dtype=BF16)
+    z, w = x.clone(), y.clone()
+    z[5, 7] = float("nan")
+    w[69, 80] = float("inf")
+    out, sx, sy = (t.cpu() for t in tt.pair_moments([x.cuda(), z.cuda()], [y.cuda(), w.cuda()], [1.0, 0.0], units=True))
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[7] = True
+    bad[:, 80] = True
+    assert torch.equal(torch.isnan(out), bad) and (out[~bad] == 70).all()
+    assert torch.equal(torch.isnan(sx), bad[:, 0]) and torch.equal(torch.isnan(sy), bad[0])
+    assert (sx[~bad[:, 0]] == 70).all() and (sy[~bad[0]] == 70).all()
+
+
 def test_gradient_of_the_log_likelihood_by_differences(tt):
     """d log p / d W of a small Boltzmann machine of two spin blocks, by enumeration, against the moments of its own
     distribution given as weighted phases: data minus model, and against differences of the log likelihood."""

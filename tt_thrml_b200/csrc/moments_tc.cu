@@ -145,7 +145,7 @@ __device__ __forceinline__ void unit_sums(const MomentArgs& a, int strip, int t,
     const char* base = reinterpret_cast<const char*>(of_y ? a.y[p] : a.x[p]);
     const int64_t ld = of_y ? a.y_ld[p] : a.x_ld[p];
     const float scale = of_y ? a.y_scale[p] : a.x_scale[p];
-    if (scale == 0.0f) continue;
+    if (scale == 0.0f && a.scale[p] != 0.0f) continue;  // a term of the products only; a phase of scale 0 is 0 times its sums
     float s[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = 0.0f;
