@@ -84,16 +84,19 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PyObject *po = PyList_GET_ITEM(args[0], i), *go = PyList_GET_ITEM(args[1], i);
     if (!THPVariable_Check(po) || !THPVariable_Check(go)) return PyLong_FromSsize_t(i);
     const at::Tensor &p = THPVariable_Unpack(po), &g = THPVariable_Unpack(go);
-    if (!plain_cuda(p, device) || !plain_cuda(g, device)) return PyLong_FromSsize_t(i);
-    const int32_t gd = dtype_code(g);
+    // the same keys: what holds for the parameter's device type and layout holds for the gradient's
+    const bool alike = p.key_set() == g.key_set() && p.device() == g.device();
+    if (!plain_cuda(p, device) || !(alike || plain_cuda(g, device))) return PyLong_FromSsize_t(i);
+    const int32_t pd = dtype_code(p), gd = p.dtype() == g.dtype() ? pd : dtype_code(g);
     if (p.sizes() != g.sizes() || p.strides() != g.strides() || !p.is_non_overlapping_and_dense() ||
-        (gd != TTHRML_DT_F32 && gd != dtype_code(p)))
+        (gd != TTHRML_DT_F32 && gd != pd))
       return PyLong_FromSsize_t(i);
-    if (p.numel() == 0) continue;
+    const int64_t numel = p.numel();
+    if (numel == 0) continue;
     if (row >= call->n_rows) return PyLong_FromSsize_t(i);
     tthrml_adamw_tensor& r = call->rows[row++];
-    if (r.param != p.data_ptr() || r.n != p.numel() || r.param_dtype != dtype_code(p)) return PyLong_FromSsize_t(i);
-    r.grad = g.data_ptr();
+    if (r.param != p.data_ptr() || r.n != numel || r.param_dtype != pd) return PyLong_FromSsize_t(i);
+    r.grad = g.const_data_ptr();
     r.grad_dtype = gd;
   }
   if (row != call->n_rows) return PyLong_FromSsize_t(n - 1);
@@ -103,6 +106,35 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (rc) return PyLong_FromLong(rc - 1000);
   bump(args[0]);
   return PyLong_FromLong(-1);
+  END_HANDLE_TH_ERRORS
+}
+
+using AdamWValuesFn = decltype(&tthrml_adamw_values);
+
+// adamw_values(call, codes, elements, function, stream) -> both moments as float32 tensors of `elements` on the codes' device
+// (the padded segments, at least one block), or an error code.
+PyObject* adamw_values(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !THPVariable_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "adamw_values(call, codes, elements, function, stream)");
+    return nullptr;
+  }
+  const AdamWCall* call = address<const AdamWCall*>(args[0]);
+  const int64_t elements = PyLong_AsLongLong(args[2]);
+  void* stream = PyLong_AsVoidPtr(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  const auto options = THPVariable_Unpack(args[1]).options().dtype(at::kFloat);
+  at::Tensor m = at::empty({elements}, options), v = at::empty({elements}, options);
+  const int rc = address<AdamWValuesFn>(args[3])(static_cast<const int8_t*>(call->exp_avg),
+                                                 static_cast<const uint8_t*>(call->exp_avg_sq), call->exp_avg_scale,
+                                                 call->exp_avg_sq_scale, elements, m.mutable_data_ptr<float>(),
+                                                 v.mutable_data_ptr<float>(), stream);
+  if (rc) return PyLong_FromLong(rc);
+  PyObject *a = THPVariable_Wrap(m), *b = THPVariable_Wrap(v);
+  PyObject* t = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return t;
   END_HANDLE_TH_ERRORS
 }
 
@@ -242,6 +274,8 @@ PyMethodDef methods[] = {
      "Pair moments of lists of phases: the plain case, or None."},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_step)), METH_FASTCALL,
      "A step of all parameters: the plain case, or where it is not."},
+    {"adamw_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_values)), METH_FASTCALL,
+     "The 8-bit moments as float32."},
     {"bump_versions", bump_versions, METH_O, "Marks tensors as written for autograd."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", "Host side of calls with many tensors.", -1, methods,

@@ -111,6 +111,7 @@ class AdamW:
         self._call = nat.AdamWCall(self._rows.ctypes.data, len(self._rows), self.state_bits, *at, *self.betas, self.eps,
                                    self.weight_decay, self.seed)
         self._call_at, self._entry = ctypes.addressof(self._call), nat.address_of("tthrml_adamw_step")
+        self._values_entry = nat.address_of("tthrml_adamw_values")
 
     # ---------------------------------------------------------------- control
 
@@ -191,16 +192,12 @@ class AdamW:
         torch = _torch()
         m, v = self.exp_avg, self.exp_avg_sq
         if self.state_bits == 8:
-            m, v = (torch.empty(t.shape, dtype=torch.float32, device=self.device) for t in (m, v))
-            c = self._call
+            index = self.device.index
             with on_device(self.device):
-                nat.check(
-                    nat.lib().tthrml_adamw_values(
-                        c.exp_avg, c.exp_avg_sq, c.exp_avg_scale, c.exp_avg_sq_scale, m.numel(), m.data_ptr(), v.data_ptr(),
-                        raw_stream(self.device.index),
-                    ),
-                    "tthrml_adamw_values",
-                )
+                made = self._host.adamw_values(self._call_at, m, m.numel(), self._values_entry, raw_stream(index))
+            if type(made) is int:
+                nat.check(made, "tthrml_adamw_values")
+            m, v = made
         if flat:
             return (m, v) if m.numel() == self.elements else (m[: self.elements], v[: self.elements])
         return tuple([torch.as_strided(t, p.shape, p.stride(), o) if p.numel() else t[:0].view(p.shape)
