@@ -10,11 +10,11 @@
 // own copy.  The moments of all tensors lie in one buffer, each tensor's segment padded to 256 elements.  The CTAs walk
 // side by side over 2048-element chunks of the concatenated tensors (a chunk never spans two tensors); a warp holds 256
 // of them, a thread two groups of four 128 apart, so that every load and store of a warp is contiguous.  33.6 M float32
-// weights take 154 us so (6.1 TB/s, 93 % of the measured copy rate), 167 us with a range of chunks of its own for each
-// CTA, 178 us with eight adjacent elements per thread; with codes 138 (instruction issue), 147 and 171 us.
+// weights take 142 us so (6.6 TB/s, the measured copy rate); of 154 us, a range of chunks of its own for each CTA made 167,
+// eight adjacent elements per thread 178.  With codes 138 us (instruction issue).
 //
-// The step counter and the learning rate stand in device memory, so a replayed graph counts on; the last CTA of a step's
-// last launch advances the counter.
+// The step counter and the learning rate stand in device memory, so a replayed graph counts on; in a step's last launch the
+// last CTA that has read the counter advances it.
 //
 // 8-bit codes, one warp per block of 256 elements with the block's largest |m| and v as scales:
 //     m = sign q^2 max|m| / 127^2, q = 0..127;      v = q^4 max v / 255^4, q = 0..255.
@@ -215,33 +215,59 @@ __device__ __forceinline__ float2 codes_v(float2 y, float2 u65536, float minus_z
   const float2 t = mul2(mul2(u65536, span), make_float2(fminf(k.x, 1.0f), fminf(k.y, 1.0f))), o = mul2(over, both(65536.0f));
   return make_float2(fminf(t.x < o.x ? n.x : k.x, 255.0f), fminf(t.y < o.y ? n.y : k.y, 255.0f));
 }
+// b^t by squaring, t >= 1: the library's power is a few hundred instructions on the way of a small step's only round.  At most
+// 2 log2 t roundings of 2^-53, and none at t = 1, where 1 - b is smallest.
+__device__ __forceinline__ double power(double b, int64_t t) {
+  double r = 1.0;
+  for (;; b *= b) {
+    if (t & 1) r *= b;
+    t >>= 1;
+    if (t == 0) return r;
+  }
+}
+
+// The tensor that holds chunk c: the last of n whose first chunk is not behind c.  A warp looks at 32 places at a time.
+__device__ __forceinline__ int tensor_of(const int32_t* first_chunk, int n, int c) {
+  const int lane = threadIdx.x & 31, stride = (n + 31) / 32;
+  int at = lane * stride;
+  const int found = 31 - __clz(__ballot_sync(0xffffffffu, at < n && first_chunk[at] <= c));
+  if (stride == 1) return found;
+  at = found * stride + lane;  // stride <= 32
+  return found * stride + 31 - __clz(__ballot_sync(0xffffffffu, at < n && first_chunk[at] <= c));
+}
+
 template <int BITS, int T>
 __global__ void __launch_bounds__(kAdamThreads, 4)
     k_adamw(const __grid_constant__ AdamTable<T> tab, const __grid_constant__ AdamArgs a) {
   __shared__ float coef[4];  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd, step
+  static_assert(T <= 1024, "two rounds of 32 places");
   const int chunks = tab.first_chunk[a.n_tensors];
+  // The table by generic addresses: its lookups are by a warp's lanes, and a constant bank serves one address at a time.
+  const AdamTable<T>* table = &tab;
+  asm("" : "+l"(table));
   int ti = 0;
   const int place = 256 * (threadIdx.x >> 5) + 4 * (threadIdx.x & 31);
   const int64_t step = a.ctl->step + 1;
   // the coefficients in double, a warp each; every warp passes the barrier once, after its first loads are on their way
-  if (threadIdx.x == 0) coef[0] = (float)(a.ctl->lr / (1.0 - pow(a.beta1, (double)step)));
-  if (threadIdx.x == 32) coef[1] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)step)));
+  if (threadIdx.x == 0) coef[0] = (float)(a.ctl->lr / (1.0 - power(a.beta1, step)));
+  if (threadIdx.x == 32) coef[1] = (float)(1.0 / sqrt(1.0 - power(a.beta2, step)));
   if (threadIdx.x == 64) coef[2] = (float)(1.0 - a.ctl->lr * a.weight_decay);
   const auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kAdamThreads) : "memory"); };
   bool ready = false;
+  // The last CTA that has read the step advances the counter.  The count goes out early: nothing waits for it before the end.
+  unsigned long long before = 0ull;
+  const auto count = [&] {
+    if (threadIdx.x == 0 && a.last) {
+      __threadfence();
+      before = atomicAdd(&a.ctl->ticket, 1ull);
+    }
+  };
   float step_size = 0.0f, r_bias2 = 0.0f, keep = 0.0f;
   const PhiloxKeys keys = philox_keys((uint32_t)a.seed, (uint32_t)(a.seed >> 32));
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    if (tab.first_chunk[ti + 1] <= c) {  // a later tensor's chunk
-      int lo = ti + 1, hi = a.n_tensors;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        (tab.first_chunk[mid] <= c ? lo : hi) = mid;
-      }
-      ti = lo;
-    }
-    const tthrml_adamw_tensor& t = tab.t[ti];
-    const int64_t i = (int64_t)(c - tab.first_chunk[ti]) * kChunk + place;
+    if (tab.first_chunk[ti + 1] <= c) ti = tensor_of(table->first_chunk, a.n_tensors, c);
+    const tthrml_adamw_tensor& t = table->t[ti];
+    const int64_t i = (int64_t)(c - table->first_chunk[ti]) * kChunk + place;
     if (i - 4 * (threadIdx.x & 31) >= t.n) continue;  // whole warps
     const int64_t e = t.state + i;  // this thread's groups: e .. e + 3 and e + 128 .. e + 131
     const bool pv = (uintptr_t)t.param % (t.param_dtype == TTHRML_DT_F32 ? 16 : 8) == 0;
@@ -271,6 +297,7 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
     if (!ready) {
       barrier();
       step_size = coef[0], r_bias2 = coef[1], keep = coef[2];
+      count();
       ready = true;
     }
     float tm = 0.0f, tv = 0.0f;
@@ -346,14 +373,13 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
       }
     }
   }
-  if (!ready) barrier();
-  __syncthreads();
-  if (threadIdx.x == 0 && a.last) {
-    __threadfence();
-    if (atomicAdd(&a.ctl->ticket, 1ull) == gridDim.x - 1) {  // every CTA has read the step
-      a.ctl->step = step;
-      a.ctl->ticket = 0ull;
-    }
+  if (!ready) {
+    barrier();
+    count();
+  }
+  if (threadIdx.x == 0 && a.last && before == gridDim.x - 1) {
+    a.ctl->step = step;
+    a.ctl->ticket = 0ull;
   }
 }
 
@@ -407,8 +433,10 @@ int launch_adamw(const tthrml_adamw_tensor* t, int32_t n, AdamArgs a, int sms, c
   }
   tab.first_chunk[n] = (int32_t)chunks;
   a.n_tensors = n;
-  const int64_t want = 8 * (int64_t)sms;
-  const int grid = (int)(chunks < want ? (chunks > 0 ? chunks : 1) : want);
+  // Two chunks a CTA, but no fewer CTAs than run at once: 33.6 M float32 weights took 142 us so, 149 with one chunk a CTA, 144
+  // and 147 with three and six, 155 with 8 CTAs an SM; 600 tensors of 4.6 M bfloat16 weights 22.3, 23.0, 27.8 and 23.5, 21.9.
+  const int64_t least = 4 * (int64_t)sms < chunks ? 4 * (int64_t)sms : chunks, want = (chunks + 1) / 2;
+  const int grid = (int)(want > least ? want : least);
   k_adamw<BITS, T><<<grid, kAdamThreads, 0, st>>>(tab, a);
   return launch_status("k_adamw launch");
 }
@@ -442,7 +470,7 @@ extern "C" int tthrml_adamw_step(const tthrml_adamw_tensor* tensors_host, int64_
     const tthrml_adamw_tensor& t = tensors_host[i];
     const int64_t pb = dtype_bytes(t.param_dtype), gb = dtype_bytes(t.grad_dtype);
     if (t.n < 1 || !t.param || !t.grad || t.state < 0 || t.state % 256 || pb < 2 || gb < 2 ||
-        (uintptr_t)t.param % pb || (uintptr_t)t.grad % gb) {
+        ((uintptr_t)t.param & (pb - 1)) || ((uintptr_t)t.grad & (gb - 1))) {  // 2 or 4 bytes
       set_error("tthrml_adamw_step: tensor %lld: elements %lld, state offset %lld (a multiple of 256), types %d, %d",
                 (long long)i, (long long)t.n, (long long)t.state, (int)t.param_dtype, (int)t.grad_dtype);
       return TTHRML_ERR_ARG;
