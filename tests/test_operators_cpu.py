@@ -186,6 +186,9 @@ def test_host_module_leaves_other_cases_to_python():
     for bad in ((), ([x], [x, x], 0, 0, 0, 0), ((x,), [x], 0, 0, 0, 0)):
         with pytest.raises(TypeError):
             host.adamw_step(*bad)
+    for bad in ((0,), (0, 1, 256, 0, 0), (0, "codes", 256, 0, 0)):
+        with pytest.raises(TypeError):
+            host.adamw_values(*bad)
     version = x._version
     host.bump_versions([x, 3])
     assert x._version == version + 1

@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(kAdamThreads, 4)
   }
 }
 
-// Values of codes: four elements per thread and step, four steps of 1024 elements on their way.
+// Values of codes: four elements per thread and step, four steps of 1024 elements on their way; 4096 elements a CTA, for short
+// CTAs that follow each other keep the memory busier than loops (33.6 M: 58 us, 5.8 TB/s; 67 us with 8 CTAs an SM).
 __global__ void __launch_bounds__(256)
     k_adamw_values(const int8_t* __restrict__ m, const uint8_t* __restrict__ v, const float* __restrict__ m_scale,
                    const float* __restrict__ v_scale, int64_t elements, float* __restrict__ mf, float* __restrict__ vf) {
@@ -532,7 +533,7 @@ extern "C" int tthrml_adamw_values(const int8_t* exp_avg, const uint8_t* exp_avg
     return TTHRML_ERR_ARG;
   }
   const int64_t blocks = (elements + 4095) / 4096;
-  k_adamw_values<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, (cudaStream_t)stream>>>(
+  k_adamw_values<<<(unsigned)(blocks < 148 * 64 ? blocks : 148 * 64), 256, 0, (cudaStream_t)stream>>>(
       exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, elements, exp_avg_out, exp_avg_sq_out);
   return launch_status("k_adamw_values launch");
 }
