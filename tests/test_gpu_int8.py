@@ -129,6 +129,27 @@ def test_product_matches_the_64_bit_sum(tt, rows, units, cols, dtype):
     tt.check_operator_errors()
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,units,cols", [(140, 8190, 700), (777, 3001, 1000), (300, 1501, 5001), (200, 3001, 6000),
+                                             (257, 4500, 3333), (520, 3001, 2500)])
+def test_products_of_some_hundred_rows(tt, rows, units, cols, dtype):
+    """Tiles of 256 rows, whole and cut off, the columns in one share or several: exact sums on every path, so the result of
+    128 rows at a time (tiles of 128) is the same to the bit."""
+    t = DTYPES[dtype]
+    x, w = rand((rows, cols), t, rows + cols), rand((units, cols), torch.float32, units)
+    bias = rand((units,), torch.float32, 9)
+    wq, sw = plain_quantize(w)
+    q, sx = plain_quantize(x)
+    r = tt.quantize_rows(w.cuda())
+    d, b = x.cuda(), bias.cuda()
+    y = tt.int8_product(d, r, bias=b)
+    check_product(y, q, sx, wq, sw, bias.numpy(), t)
+    parts = torch.cat([tt.int8_product(d[m : m + 128], r, bias=b) for m in range(0, rows, 128)])
+    assert torch.equal(y, parts)
+    assert torch.equal(tt.int8_product(tt.quantize_rows(d), r, bias=b, out_dtype=t), y)
+    tt.check_operator_errors()
+
+
 @pytest.mark.parametrize("rows", [1, 6, 33, 200])
 @pytest.mark.parametrize("out", list(DTYPES))
 def test_quantized_rows_as_input(tt, rows, out):

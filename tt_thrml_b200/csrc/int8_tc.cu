@@ -12,6 +12,8 @@
 // sweeps does): each CTA holds 128 rows of either operand per stage, the even CTA issues every MMA, two TMEM accumulators let
 // the epilogue of one tile run under the main loop of the next.  The epilogue stores the scaled sums, or takes them as
 // the fields of a dense block and draws its new state.
+#include <algorithm>
+
 #include "dense_draw.cuh"
 #include "int8_common.cuh"
 
@@ -140,56 +142,64 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t tmem = *tmem_holder;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = (uint32_t)(a.box_m * 128 + S::kBBytes);
-      const int ahead = min(S::kStages, k_last - k_first);
-      for (int s = 0; s < ahead; ++s) {  // the weights of the first stages, while the rows are still being quantised
+    const bool one = elect_one();
+    const uint32_t bytes = (uint32_t)(a.box_m * 128 + S::kBBytes);
+    const int ahead = min(S::kStages, k_last - k_first);
+    for (int s = 0; s < ahead; ++s) {  // the weights of the first stages, while the rows are still being quantised
+      if (one) {
         mbar_expect_tx(&full[s], bytes);
         tma_load_2d(tiles + s * S::kStage + S::kABytes, &map_b, &full[s], (k_first + s) * 128, n0);
       }
-      wait_for_previous_kernel();
-      for (int s = 0; s < ahead; ++s) tma_load_2d(tiles + s * S::kStage, &map_a, &full[s], (k_first + s) * 128, m0);
-      int issued = ahead;
-      for (int kb = k_first + ahead; kb < k_last; ++kb, ++issued) {
-        const int s = issued % S::kStages;
-        if (!mbar_wait(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
-          atomicExch(a.error, kErrEmptyWait);
-          break;
-        }
+    }
+    wait_for_previous_kernel();
+    for (int s = 0; s < ahead; ++s)
+      if (one) tma_load_2d(tiles + s * S::kStage, &map_a, &full[s], (k_first + s) * 128, m0);
+    int issued = ahead;
+    for (int kb = k_first + ahead; kb < k_last; ++kb, ++issued) {
+      const int s = issued % S::kStages;
+      if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
+        if (one) atomicExch(a.error, kErrEmptyWait);
+        break;
+      }
+      if (one) {
         mbar_expect_tx(&full[s], bytes);
         unsigned char* t = tiles + s * S::kStage;
         tma_load_2d(t, &map_a, &full[s], kb * 128, m0);
         tma_load_2d(t + S::kABytes, &map_b, &full[s], kb * 128, n0);
       }
-      // the copies issued must land before the stages are used again or the CTA exits
-      for (int j = issued > S::kStages ? issued - S::kStages : 0; j < issued; ++j)
-        if (!mbar_wait(&full[j % S::kStages], (uint32_t)(j / S::kStages) & 1u)) atomicExch(a.error, kErrFullWait);
+      __syncwarp();
     }
+    // the copies issued must land before the stages are used again or the CTA exits
+    for (int j = issued > S::kStages ? issued - S::kStages : 0; j < issued; ++j)
+      if (!mbar_wait_all(&full[j % S::kStages], (uint32_t)(j / S::kStages) & 1u) && one) atomicExch(a.error, kErrFullWait);
   } else if (warp == 1) {
-    if (lane == 0) {
-      int used = 0;
-      for (int kb = k_first; kb < k_last; ++kb, ++used) {
-        const int s = used % S::kStages;
-        if (!mbar_wait(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
-          atomicExch(a.error, kErrFullWait);
-          break;
-        }
-        tc_fence_after();
-        const unsigned char* t = tiles + s * S::kStage;
-        const uint64_t ad = umma_desc_sw128(t), bd = umma_desc_sw128(t + S::kABytes);
+    const bool one = elect_one();
+    int used = 0;
+    for (int kb = k_first; kb < k_last; ++kb, ++used) {
+      const int s = used % S::kStages;
+      if (!mbar_wait_all(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
+        if (one) atomicExch(a.error, kErrFullWait);
+        break;
+      }
+      tc_fence_after();
+      const unsigned char* t = tiles + s * S::kStage;
+      const uint64_t ad = umma_desc_sw128(t), bd = umma_desc_sw128(t + S::kABytes);
+      if (one) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)  // K = 32 bytes per MMA
           umma_i8(tmem, ad + 2ull * kk, bd + 2ull * kk, idesc_i8(128, BN), (used > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&empty[s]);
       }
-      umma_commit(done);
+      __syncwarp();
     }
+    if (one) umma_commit(done);
+    __syncwarp();
   } else if (warp >= 4) {
     const int row = (int)threadIdx.x - 128;
     wait_for_previous_kernel();
     row_scale_of[row] = a.x_scale && m0 + row < a.M ? a.x_scale[m0 + row] : 1.0f;
   }
-  const bool ok = mbar_wait(done, 0u);
+  const bool ok = mbar_wait_warp(done, 0u);
   if (!ok && lane == 0) atomicExch(a.error, kErrAccWait);
   tc_fence_after();
   __syncthreads();  // the stages are free: every copy has landed and every MMA has read them
@@ -411,62 +421,69 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = *tmem_holder;
   int last_it[2] = {-1, -1};
 
-  if (warp == 0) {
-    if (lane == 0) {  // producer (both CTAs): this CTA's halves of the A and B slices
-      int64_t issued = 0;
-      bool failed = false;
-      for (int t = first; t < n_tiles && !failed; t += step) {
-        int mb, nb;
-        tile_coords(t, m_blocks, n_blocks, args.d.group, mb, nb);
-        for (int kb = 0; kb < a.num_k; ++kb) {
-          const int s = (int)(issued % kPairStages);
-          if (!mbar_wait(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
-            atomicExch(a.error, kErrEmptyWait);
-            failed = true;
-            break;
-          }
+  if (warp == 0) {  // producer (both CTAs): this CTA's halves of the A and B slices
+    const bool one = elect_one();
+    int64_t issued = 0;
+    bool failed = false;
+    for (int t = first; t < n_tiles && !failed; t += step) {
+      int mb, nb;
+      tile_coords(t, m_blocks, n_blocks, args.d.group, mb, nb);
+      for (int kb = 0; kb < a.num_k; ++kb) {
+        const int s = (int)(issued % kPairStages);
+        if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
+          if (one) atomicExch(a.error, kErrEmptyWait);
+          failed = true;
+          break;
+        }
+        if (one) {
           if (leader) mbar_expect_tx(&full[s], 2 * kPairStage);  // the stage's bytes of both CTAs
           unsigned char* st = tiles + s * kPairStage;
           const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
           tma_load_2d_pair(st, &map_a, bar, kb * 128, mb * 256 + (int)rank * 128);
           tma_load_2d_pair(st + kPairStage / 2, &map_b, bar, kb * 128, nb * 256 + (int)rank * 128);
-          ++issued;
         }
+        __syncwarp();
+        ++issued;
       }
-      // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
-      for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
-        if (!mbar_wait(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u)) atomicExch(a.error, kErrEmptyWait);
     }
+    // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
+    for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
+      if (!mbar_wait_all(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u) && one) atomicExch(a.error, kErrEmptyWait);
   } else if (warp == 1) {
-    if (lane == 0 && leader) {  // MMA issue: the leader only
+    if (leader) {  // MMA issue: the leader only
+      const bool one = elect_one();
       int64_t used = 0;
       int it = 0;
       bool failed = false;
       for (int t = first; t < n_tiles && !failed; t += step, ++it) {
         const int b = it & 1;
-        if (!mbar_wait(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
-          atomicExch(a.error, kErrAccWait);
+        if (!mbar_wait_all(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
+          if (one) atomicExch(a.error, kErrAccWait);
           break;
         }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(b * 256);
         for (int kb = 0; kb < a.num_k; ++kb) {
           const int s = (int)(used % kPairStages);
-          if (!mbar_wait(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
-            atomicExch(a.error, kErrFullWait);
+          if (!mbar_wait_all(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
+            if (one) atomicExch(a.error, kErrFullWait);
             failed = true;
             break;
           }
           tc_fence_after();
           const unsigned char* st = tiles + s * kPairStage;
           const uint64_t ad = umma_desc_sw128(st), bd = umma_desc_sw128(st + kPairStage / 2);
+          if (one) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)  // K = 32 bytes per MMA
-            umma_i8_pair(d, ad + 2ull * kk, bd + 2ull * kk, (kb > 0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+            for (int kk = 0; kk < 4; ++kk)  // K = 32 bytes per MMA
+              umma_i8_pair(d, ad + 2ull * kk, bd + 2ull * kk, (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+          }
+          __syncwarp();
           ++used;
         }
-        umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
+        if (one) umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
+        __syncwarp();
         last_it[b] = it;
       }
     }
@@ -489,7 +506,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         sw[256 + j] = EPI == kStoreFields && a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      if (!failed && !mbar_wait(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
+      if (!failed && !mbar_wait_all(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
         if (lane == 0) atomicExch(a.error, kErrAccWait);
         failed = true;
       }
@@ -599,10 +616,17 @@ int resident_tiles(const int** out) {
   return TTHRML_OK;
 }
 
-// Estimated clocks of the tiles on clusters of S CTAs: the main loop by its bytes (loop_clocks), about 6000 clocks beside
-// it, and for S > 1 a barrier and the partial tiles at about 32 bytes a clock.  Measured over (BN, S) at five sizes: the
-// choice is the fastest or within 10 % of it (256 x 8192 x 4096: 15.6 us of 15.6 to 76; 128 x 4096 x 8192: 12.8 of 12.8 to
-// 60; 64 x 5008 x 2048: 8.6 of 8.6 to 24).
+// Clocks of a 128-column block of K that brings `bytes` into each of `ctas` SMs at once: an SM takes in 68 bytes a clock, all
+// of them 7900 from L2; mma: the multiplications' own.
+inline int64_t block_clocks(int64_t bytes, int64_t ctas, int64_t mma) {
+  return std::max({mma, bytes / 68, bytes * ctas / 7900});
+}
+
+// Estimated clocks of the tiles on clusters of S CTAs: per wave the blocks of a CTA's share of K, at least 360 clocks each to
+// issue, the tile's store, and for S > 1 a barrier and the partial tiles.  The constants are those with which the choice among
+// (BN, S) and the pair kernel came out best over 56 sizes of 3 to 8192 rows with every choice measured: 1.5 % behind the
+// fastest on average, 28 % at most.  256 x 8192 x 4096: (256, 4) 15.7 us of 15.7 to 76; 256 x 4096 x 8192: (128, 1) 14.6 of
+// 14.6 to 109; 64 x 5008 x 2048: (64, 4) 8.1 of 8.1 to 24.
 template <int BN>
 int consider(const ProductArgs& a, int64_t& best, int& bn, int& split) {
   const int* resident;
@@ -612,9 +636,9 @@ int consider(const ProductArgs& a, int64_t& best, int& bn, int& split) {
   for (int i = 0; i < 4 && (1 << i) <= a.num_k; ++i) {
     const int s = 1 << i;
     const int64_t waves = (tiles + resident[i] - 1) / resident[i];
-    const int64_t bytes = (int64_t)((a.num_k + s - 1) / s) * (a.box_m + BN) * 128;
-    const int64_t c = waves * (loop_clocks(bytes, (tiles < resident[i] ? tiles : resident[i]) * s) + 6000 +
-                               (s > 1 ? 1500 + (int64_t)(a.M < 128 ? a.M : 128) * BN / 8 : 0));
+    const int64_t block = block_clocks((a.box_m + BN) * 128, (tiles < resident[i] ? tiles : resident[i]) * s, std::max(2 * BN, 360));
+    const int64_t c = 8300 + waves * ((a.num_k + s - 1) / s * block + 20 * BN +
+                                      (s > 1 ? 850 + (int64_t)(a.M < 128 ? a.M : 128) * BN / 10 : 0));
     if (c < best) best = c, bn = BN, split = s;
   }
   return TTHRML_OK;
@@ -706,7 +730,7 @@ int int8_product(const int8_t* x, int64_t x_pitch, const float* x_scale, const i
     return rc;
   // the pair kernel overlaps a tile's epilogue with the next tile's loop
   const int64_t pairs = ((rows + 255) / 256) * ((units + 255) / 256), at_once = pairs < fit.clusters ? pairs : fit.clusters;
-  if ((pairs + fit.clusters - 1) / fit.clusters * loop_clocks((int64_t)a.num_k * kPairStage, 2 * at_once) + 14000 < best) {
+  if ((pairs + fit.clusters - 1) / fit.clusters * a.num_k * block_clocks(kPairStage, 2 * at_once, 684) + 13700 < best) {
     rc = make_map_i8(&ma, x, rows, cols, x_pitch, 128u);
     if (rc == TTHRML_OK) rc = make_map_i8(&mb, weights, units, cols, w_pitch, 128u);
     if (rc) return rc;

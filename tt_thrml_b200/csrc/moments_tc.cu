@@ -271,18 +271,19 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   wait_for_previous_kernel();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      bool failed = false;
-      for (int b = first; b < last && !failed;) {
-        const Chunk c = chunk_at(a, b, last);
-        for (int i = 0; i < c.length; ++i, ++issued) {
-          const int s = issued % S::kStages;
-          if (!mbar_wait(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
-            atomicExch(a.error, kErrEmptyWait);
-            failed = true;
-            break;
-          }
+    const bool one = elect_one();
+    int issued = 0;
+    bool failed = false;
+    for (int b = first; b < last && !failed;) {
+      const Chunk c = chunk_at(a, b, last);
+      for (int i = 0; i < c.length; ++i, ++issued) {
+        const int s = issued % S::kStages;
+        if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
+          if (one) atomicExch(a.error, kErrEmptyWait);
+          failed = true;
+          break;
+        }
+        if (one) {
           mbar_expect_tx(&full[s], S::kStage);
           unsigned char* t = tiles + s * S::kStage;
           const int chain = (c.block + i) * 64;
@@ -292,45 +293,49 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
           for (int k = 0; k < BN / 64; ++k)
             tma_load_2d(t + S::kABytes + k * 8192, &maps.y[c.phase], &full[s], n0 + 64 * k, chain);
         }
-        b += c.length;
+        __syncwarp();
       }
-      // the copies issued must land before the stages are used again or the CTA exits
-      for (int j = issued > S::kStages ? issued - S::kStages : 0; j < issued; ++j)
-        if (!mbar_wait(&full[j % S::kStages], (uint32_t)(j / S::kStages) & 1u)) atomicExch(a.error, kErrFullWait);
+      b += c.length;
     }
+    // the copies issued must land before the stages are used again or the CTA exits
+    for (int j = issued > S::kStages ? issued - S::kStages : 0; j < issued; ++j)
+      if (!mbar_wait_all(&full[j % S::kStages], (uint32_t)(j / S::kStages) & 1u) && one) atomicExch(a.error, kErrFullWait);
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_moments(BN, a.f16 != 0);
-      int used = 0, chunk = 0;
-      bool failed = false;
-      for (int b = first; b < last && !failed; ++chunk) {
-        const Chunk c = chunk_at(a, b, last);
-        const int buf = chunk & 1;
-        if (!mbar_wait(&acc_empty[buf], ((uint32_t)(chunk >> 1) & 1u) ^ 1u)) {
-          atomicExch(a.error, kErrAccWait);
+    const bool one = elect_one();
+    const uint32_t idesc = idesc_moments(BN, a.f16 != 0);
+    int used = 0, chunk = 0;
+    bool failed = false;
+    for (int b = first; b < last && !failed; ++chunk) {
+      const Chunk c = chunk_at(a, b, last);
+      const int buf = chunk & 1;
+      if (!mbar_wait_all(&acc_empty[buf], ((uint32_t)(chunk >> 1) & 1u) ^ 1u)) {
+        if (one) atomicExch(a.error, kErrAccWait);
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + (uint32_t)(buf * BN);
+      for (int i = 0; i < c.length; ++i, ++used) {
+        const int s = used % S::kStages;
+        if (!mbar_wait_all(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
+          if (one) atomicExch(a.error, kErrFullWait);
           failed = true;
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(buf * BN);
-        for (int i = 0; i < c.length; ++i, ++used) {
-          const int s = used % S::kStages;
-          if (!mbar_wait(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
-            atomicExch(a.error, kErrFullWait);
-            failed = true;
-            break;
-          }
-          tc_fence_after();
-          const unsigned char* t = tiles + s * S::kStage;
-          const uint64_t ad = umma_desc_mn128(t), bd = umma_desc_mn128(t + S::kABytes);
+        const unsigned char* t = tiles + s * S::kStage;
+        const uint64_t ad = umma_desc_mn128(t), bd = umma_desc_mn128(t + S::kABytes);
+        if (one) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 16 chains per MMA: two groups of eight, 2048 bytes
             umma_f16(d, ad + 128ull * kk, bd + 128ull * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&empty[s]);
         }
-        umma_commit(&acc_full[buf]);
-        b += c.length;
+        __syncwarp();
       }
+      if (one) umma_commit(&acc_full[buf]);
+      __syncwarp();
+      b += c.length;
     }
   } else if (warp >= 10) {
     side_sums(a, side);
@@ -344,7 +349,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
     for (int b = first; b < last; ++chunk) {
       const Chunk c = chunk_at(a, b, last);
       const int buf = chunk & 1;
-      if (!mbar_wait(&acc_full[buf], (uint32_t)(chunk >> 1) & 1u)) {
+      if (!mbar_wait_warp(&acc_full[buf], (uint32_t)(chunk >> 1) & 1u)) {
         if (lane == 0) atomicExch(a.error, kErrAccWait);
         break;
       }
@@ -524,23 +529,24 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
   wait_for_previous_kernel();
   int last_chunk[2] = {-1, -1};
 
-  if (warp == 0) {
-    if (lane == 0) {  // producer (both CTAs): this CTA's halves of the x and y units
-      int64_t issued = 0;
-      bool failed = false;
-      for (int t = first; t < n_tiles && !failed; t += step) {
-        int mb, nb;
-        pair_tile(a, t, mb, nb);
-        const int m0 = mb * 256 + (int)rank * 128, n0 = nb * 256 + (int)rank * 128;
-        for (int b = 0; b < total && !failed;) {
-          const Chunk c = chunk_at(a, b, total);
-          for (int i = 0; i < c.length; ++i, ++issued) {
-            const int s = (int)(issued % kPairStages);
-            if (!mbar_wait(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
-              atomicExch(a.error, kErrEmptyWait);
-              failed = true;
-              break;
-            }
+  if (warp == 0) {  // producer (both CTAs): this CTA's halves of the x and y units
+    const bool one = elect_one();
+    int64_t issued = 0;
+    bool failed = false;
+    for (int t = first; t < n_tiles && !failed; t += step) {
+      int mb, nb;
+      pair_tile(a, t, mb, nb);
+      const int m0 = mb * 256 + (int)rank * 128, n0 = nb * 256 + (int)rank * 128;
+      for (int b = 0; b < total && !failed;) {
+        const Chunk c = chunk_at(a, b, total);
+        for (int i = 0; i < c.length; ++i, ++issued) {
+          const int s = (int)(issued % kPairStages);
+          if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
+            if (one) atomicExch(a.error, kErrEmptyWait);
+            failed = true;
+            break;
+          }
+          if (one) {
             if (leader) mbar_expect_tx(&full[s], 2 * kPairStage);  // the stage's bytes of both CTAs
             unsigned char* st = tiles + s * kPairStage;
             const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
@@ -551,15 +557,17 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
               tma_load_2d_pair(st + kPairHalf + k * 8192, &maps.y[c.phase], bar, n0 + 64 * k, chain);
             }
           }
-          b += c.length;
+          __syncwarp();
         }
+        b += c.length;
       }
-      // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
-      for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
-        if (!mbar_wait(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u)) atomicExch(a.error, kErrEmptyWait);
     }
+    // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
+    for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
+      if (!mbar_wait_all(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u) && one) atomicExch(a.error, kErrEmptyWait);
   } else if (warp == 1) {
-    if (lane == 0 && leader) {  // MMA issue: the leader only
+    if (leader) {  // MMA issue: the leader only
+      const bool one = elect_one();
       const uint32_t idesc = (idesc_moments(256, a.f16 != 0) & 0x00FFFFFFu) | (16u << 24);  // M = 256
       int64_t used = 0;
       int chunk = 0;
@@ -568,8 +576,8 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
         for (int b = 0; b < total && !failed; ++chunk) {
           const Chunk c = chunk_at(a, b, total);
           const int buf = chunk & 1;
-          if (!mbar_wait(&acc_empty[buf], ((uint32_t)(chunk >> 1) & 1u) ^ 1u)) {
-            atomicExch(a.error, kErrAccWait);
+          if (!mbar_wait_all(&acc_empty[buf], ((uint32_t)(chunk >> 1) & 1u) ^ 1u)) {
+            if (one) atomicExch(a.error, kErrAccWait);
             failed = true;
             break;
           }
@@ -577,20 +585,24 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
           const uint32_t d = tmem + (uint32_t)(buf * 256);
           for (int i = 0; i < c.length; ++i, ++used) {
             const int s = (int)(used % kPairStages);
-            if (!mbar_wait(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
-              atomicExch(a.error, kErrFullWait);
+            if (!mbar_wait_all(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
+              if (one) atomicExch(a.error, kErrFullWait);
               failed = true;
               break;
             }
             tc_fence_after();
             const unsigned char* st = tiles + s * kPairStage;
             const uint64_t ad = umma_desc_mn128(st), bd = umma_desc_mn128(st + kPairHalf);
+            if (one) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // 16 chains per MMA: two groups of eight, 2048 bytes
-              umma_f16_pair(d, ad + 128ull * kk, bd + 128ull * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
-            umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+              for (int kk = 0; kk < 4; ++kk)  // 16 chains per MMA: two groups of eight, 2048 bytes
+                umma_f16_pair(d, ad + 128ull * kk, bd + 128ull * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+              umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+            }
+            __syncwarp();
           }
-          umma_commit_pair(&acc_full[buf]);  // both CTAs' accumulator halves complete
+          if (one) umma_commit_pair(&acc_full[buf]);  // both CTAs' accumulator halves complete
+          __syncwarp();
           last_chunk[buf] = chunk;
           b += c.length;
         }
@@ -612,7 +624,7 @@ __global__ void __launch_bounds__(kMomentThreads, 1)
       for (int b = 0; b < total; ++chunk) {
         const Chunk c = chunk_at(a, b, total);
         const int buf = chunk & 1;
-        if (!mbar_wait(&acc_full[buf], (uint32_t)(chunk >> 1) & 1u)) {
+        if (!mbar_wait_warp(&acc_full[buf], (uint32_t)(chunk >> 1) & 1u)) {
           if (lane == 0) atomicExch(a.error, kErrAccWait);
           failed = true;
           break;
