@@ -131,7 +131,8 @@ def test_product_matches_the_64_bit_sum(tt, rows, units, cols, dtype):
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,units,cols", [(140, 8190, 700), (777, 3001, 1000), (300, 1501, 5001), (200, 3001, 6000),
-                                             (257, 4500, 3333), (520, 3001, 2500)])
+                                             (257, 4500, 3333), (520, 3001, 2500), (1000, 4001, 2100),
+                                             (1000, 4008, 2100)])
 def test_products_of_some_hundred_rows(tt, rows, units, cols, dtype):
     """Tiles of 256 rows, whole and cut off, the columns in one share or several: exact sums on every path, so the result of
     128 rows at a time (tiles of 128) is the same to the bit."""

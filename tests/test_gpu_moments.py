@@ -45,7 +45,7 @@ def bound(a, chains):
 
 SHAPES = [(1, 1, [1]), (1, 9, [3, 0]), (8, 64, [16, 16]), (65, 63, [17, 64]), (127, 129, [65, 1]), (128, 256, [512]),
           (129, 257, [513, 100]), (200, 1000, [1023, 2050]), (640, 72, [64, 128, 192]), (1000, 513, [4000, 70]),
-          (64, 3, [5, 6, 7, 8, 9, 10]), (2, 300, [9000]), (2100, 2333, [70, 1100]), (2600, 2049, [129])]
+          (64, 3, [5, 6, 7, 8, 9, 10]), (2, 300, [9000]), (2100, 2333, [70, 1100]), (2600, 2049, [129]), (1501, 3001, [1100, 1300])]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -68,7 +68,7 @@ def test_moments_match_the_64_bit_sums(tt, m, n, chains, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("m,n,chains", [(300, 520, [3000, 700]), (130, 70, [100, 1]), (1, 1, [5000, 5000]), (2305, 2049, [300, 1100])])
+@pytest.mark.parametrize("m,n,chains", [(300, 520, [3000, 700]), (130, 70, [100, 1]), (1, 1, [5000, 5000]), (2305, 2049, [300, 1100]), (1500, 2990, [1500, 1100])])
 def test_whole_numbers_are_exact(tt, m, n, chains, dtype):
     xs = [ints((c, m), 8, i).to(dtype) for i, c in enumerate(chains)]
     ys = [(ints((c, n), 8, 20 + i) * 2 + 1).sign().to(dtype) for i, c in enumerate(chains)]
@@ -93,7 +93,8 @@ def test_accumulate_output_strides_and_untouched_columns(tt):
     assert (big[:, :7] == 3).all() and (big[:, 137:] == 3).all()
 
 
-@pytest.mark.parametrize("m,n,pitch", [(2305, 2080, 2080), (2305, 2077, 2080), (2300, 2049, 2049), (2049, 2336, 2343)])
+@pytest.mark.parametrize("m,n,pitch", [(2305, 2080, 2080), (2305, 2077, 2080), (2300, 2049, 2049), (2049, 2336, 2343),
+                                       (2900, 4160, 4160), (2900, 4101, 4104), (2817, 4097, 4097)])
 def test_sums_added_to_large_outputs(tt, m, n, pitch):
     """Whole numbers: rows that start on 16 bytes and others, tiles cut off in rows and columns."""
     x, y = ints((70, m), 5, 1).to(BF16), ints((70, n), 5, 2).to(BF16)

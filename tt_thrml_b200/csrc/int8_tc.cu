@@ -12,8 +12,6 @@
 // sweeps does): each CTA holds 128 rows of either operand per stage, the even CTA issues every MMA, two TMEM accumulators let
 // the epilogue of one tile run under the main loop of the next.  The epilogue stores the scaled sums, or takes them as
 // the fields of a dense block and draws its new state.
-#include <algorithm>
-
 #include "dense_draw.cuh"
 #include "int8_common.cuh"
 
@@ -616,14 +614,8 @@ int resident_tiles(const int** out) {
   return TTHRML_OK;
 }
 
-// Clocks of a 128-column block of K that brings `bytes` into each of `ctas` SMs at once: an SM takes in 68 bytes a clock, all
-// of them 7900 from L2; mma: the multiplications' own.
-inline int64_t block_clocks(int64_t bytes, int64_t ctas, int64_t mma) {
-  return std::max({mma, bytes / 68, bytes * ctas / 7900});
-}
-
-// Estimated clocks of the tiles on clusters of S CTAs: per wave the blocks of a CTA's share of K, at least 360 clocks each to
-// issue, the tile's store, and for S > 1 a barrier and the partial tiles.  The constants are those with which the choice among
+// Estimated clocks of the tiles on clusters of S CTAs: per wave the blocks of a CTA's share of K (block_clocks), at least 360
+// clocks each to issue, the tile's store, and for S > 1 a barrier and the partial tiles.  The constants are those with which the choice among
 // (BN, S) and the pair kernel came out best over 56 sizes of 3 to 8192 rows with every choice measured: 1.5 % behind the
 // fastest on average, 28 % at most.  256 x 8192 x 4096: (256, 4) 15.7 us of 15.7 to 76; 256 x 4096 x 8192: (128, 1) 14.6 of
 // 14.6 to 109; 64 x 5008 x 2048: (64, 4) 8.1 of 8.1 to 24.

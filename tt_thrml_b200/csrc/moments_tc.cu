@@ -719,10 +719,11 @@ int resident_tiles(const int** out) {
   return TTHRML_OK;
 }
 
-// Estimated clocks of the tiles on clusters of S CTAs: the main loop by its bytes (loop_clocks), about 6000 clocks beside
-// it, and for S > 1 a barrier and the partial tiles at about 32 bytes a clock.  Measured over (BN, S) at five sizes: the
-// choice is the fastest or within 10 % of it (777 x 1999 x 1523 chains: 15.2 us of 15.2 to 92; 512 x 1024 x 9216: 19.7
-// of 19.7 to 60; 256 x 512 x 192: 5.2 of 5.2 to 10).
+// Estimated clocks of the tiles on clusters of S CTAs: per wave the blocks of a CTA's share of the chains (block_clocks), at
+// least 360 clocks each to issue, the tile's store, and for S > 1 a barrier and the partial tiles.  The constants are those
+// of the 8-bit tiles; over 28 sizes with every (BN, S) and the pair kernel measured the choice is 0.4 % behind the fastest on
+// average, 7 % at most (777 x 2000 x 1523 chains: (128, 1) 12.9 us of 12.9 to 87; 512 x 1024 x 9216: (128, 4) 17.1 of 17.1 to
+// 51; 1500 x 1500 x 5000: (256, 2) 26.8 of 26.8 to 150).
 template <int BN>
 int consider(const MomentArgs& a, int64_t& best, int& bn, int& split) {
   const int* resident;
@@ -732,9 +733,9 @@ int consider(const MomentArgs& a, int64_t& best, int& bn, int& split) {
   for (int i = 0; i < 4 && (i == 0 || (1 << i) <= a.total_blocks); ++i) {
     const int s = 1 << i;
     const int64_t waves = (tiles + resident[i] - 1) / resident[i];
-    const int64_t bytes = (int64_t)((a.total_blocks + s - 1) / s) * MomentShape<BN>::kStage;
-    const int64_t c = waves * (loop_clocks(bytes, (tiles < resident[i] ? tiles : resident[i]) * s) + 6000 +
-                               (s > 1 ? 1500 + 128 * BN / 8 : 0));
+    const int64_t block =
+        block_clocks(MomentShape<BN>::kStage, (tiles < resident[i] ? tiles : resident[i]) * s, std::max(2 * BN, 360));
+    const int64_t c = 8300 + waves * ((int64_t)((a.total_blocks + s - 1) / s) * block + 20 * BN + (s > 1 ? 850 + 128 * BN / 10 : 0));
     if (c < best) best = c, bn = BN, split = s;
   }
   return TTHRML_OK;
@@ -765,7 +766,8 @@ int launch_moments(const MomentMaps& maps, MomentArgs& a, bool early, cudaStream
   const int64_t mblk = (a.M + 255) / 256, nblk = (a.N + 255) / 256, pairs = mblk * nblk;
   // the pair kernel overlaps a tile's store with the next tile's loop
   const int64_t waves = (pairs + fit.clusters - 1) / fit.clusters;
-  const int64_t clocks = waves * loop_clocks((int64_t)a.total_blocks * kPairStage, 2 * (pairs < fit.clusters ? pairs : fit.clusters)) + 20000;
+  const int64_t block = block_clocks(kPairStage, 2 * (pairs < fit.clusters ? pairs : fit.clusters), 684);
+  const int64_t clocks = 13700 + waves * ((int64_t)a.total_blocks * block + 3000);
   if (a.total_blocks > 0 && clocks < best) {
     int64_t g = 1;  // about square rectangles of the tiles in flight
     while ((g + 1) * (g + 1) <= fit.clusters) ++g;

@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -176,11 +177,10 @@ int encode_fn(EncodeTiledFn* out) {
   return TTHRML_OK;
 }
 
-// Clocks of a main loop that brings `bytes` into each of `ctas` SMs: an SM takes in at most 64 bytes a clock, all of them
-// together about 5100 (L2; 9.5 TB/s measured at 1.85 GHz with 128 CTAs loading tiles).
-inline int64_t loop_clocks(int64_t bytes, int64_t ctas) {
-  const int64_t rate = ctas * 64 <= 5100 ? 64 : 5100 / ctas;
-  return bytes / (rate > 0 ? rate : 1);
+// Clocks of a block of the main loop (128 bytes of K) that brings `bytes` into each of `ctas` SMs at once: an SM takes in 68
+// bytes a clock, all of them 7900 from L2; mma: the multiplications' own, or what it takes to issue them.
+inline int64_t block_clocks(int64_t bytes, int64_t ctas, int64_t mma) {
+  return std::max({mma, bytes / 68, bytes * ctas / 7900});
 }
 
 // What a launch of fn in clusters needs to know about the current device, asked once per device and function:
