@@ -93,7 +93,9 @@ class AdamW:
         self.exp_avg, self.exp_avg_sq = (torch.zeros(max(total, BLOCK), dtype=k, device=dev) for k in kinds)
         self.exp_avg_scale = self.exp_avg_sq_scale = None
         if state_bits == 8:
-            self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(max(total, BLOCK) // BLOCK, device=dev) for _ in range(2))
+            self.exp_avg_scale, self.exp_avg_sq_scale = (
+                torch.zeros(max(total, BLOCK) // BLOCK, dtype=torch.float32, device=dev) for _ in range(2)
+            )
         self._ctl = torch.zeros(3, dtype=torch.int64, device=dev)  # tthrml_adamw_ctl: step, lr (float64), ticket
         self._lr = None
         self.lr = lr
