@@ -1,5 +1,9 @@
 """Calls of the operators around dense programs that their documentation allows beside the ordinary ones."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -39,3 +43,29 @@ def test_coded_moments_under_another_default_dtype(tt, default_dtype, kind):
     default_dtype(kind)
     for a, b in zip(run(), want):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+FRESH = """
+import sys
+sys.path[:0] = {paths!r}
+import torch, tt_thrml_b200 as tt
+from test_gpu_int8 import check_product, plain_quantize, rand
+for kind in (torch.float32, torch.bfloat16, torch.float16, torch.int8):
+    for rows, cols in {sizes!r}:
+        w = rand((5, cols), torch.float32, cols)
+        wq, sw = plain_quantize(w)
+        x = rand((rows, cols), torch.float32 if kind == torch.int8 else kind, rows)
+        weights = tt.QuantizedRows(torch.from_numpy(wq).to(torch.int8).cuda(), torch.from_numpy(sw).cuda())
+        y = tt.int8_product(tt.quantize_rows(x.cuda()) if kind == torch.int8 else x.cuda(), weights)
+        check_product(y, *plain_quantize(x), wq, sw, None, y.dtype)
+"""
+
+
+@pytest.mark.parametrize("sizes", [((1, 49152), (2, 24576)), ((1, 49089), (2, 24545)), ((1, 49120), (2, 24560))])
+def test_rows_that_fill_48_kilobytes_of_shared_memory(sizes):
+    """One and two rows around the shared memory that a launch has without asking for more, in a process that has not
+    launched longer rows before (they raise the limit for later calls)."""
+    root = Path(__file__).resolve().parents[1]
+    code = FRESH.format(paths=[str(root), str(root / "tests")], sizes=sizes)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr

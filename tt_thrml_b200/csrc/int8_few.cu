@@ -177,7 +177,9 @@ int launch_few(const FewArgs& a, cudaStream_t st) {
   const int64_t want = (a.N + kFewWarps - 1) / kFewWarps, fit = 224 * 1024 / (smem + 2048);
   const int64_t most = (int64_t)sms * (fit < 1 ? 1 : (fit > kFewCtas ? kFewCtas : fit));
   const int64_t grid = want < most ? want : most;
-  if (smem > 48 * 1024) {  // a per-device attribute of the function; setting it again is cheap
+  // The 48 KiB of a launch without the attribute hold the kernel's static shared memory too (64 bytes).  The attribute is per
+  // device and function; setting it again is cheap.
+  if (smem > 47 * 1024) {
     e = cudaFuncSetAttribute(k_int8_few<T, MP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemMax);
     if (e != cudaSuccess) return cuda_status(e, "k_int8_few shared memory attribute");
   }
