@@ -4,8 +4,11 @@ import subprocess
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
+
+from tt_thrml_b200 import make_cuda_config, workloads
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +72,23 @@ def test_rows_that_fill_48_kilobytes_of_shared_memory(sizes):
     code = FRESH.format(paths=[str(root), str(root / "tests")], sizes=sizes)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def rbm():
+    return workloads.gaussian_bernoulli_rbm(256, 512, seed=2, w_std=0.05)
+
+
+@pytest.mark.parametrize("pinned", [True, False])
+def test_a_host_batch_may_be_filled_anew_at_once(tt, pinned):
+    """The learner's stream is busy while step() is called; the batch is overwritten as soon as it returns."""
+    learner = tt.DenseLearner(rbm(), n_data=128, n_chains=128, config=make_cuda_config(dense_precision="fp32"))
+    g = torch.Generator().manual_seed(1)
+    staging = torch.empty((128, 256), pin_memory=pinned)
+    for _ in range(3):
+        rows = torch.randn((128, 256), generator=g)
+        staging.copy_(rows)
+        with torch.cuda.stream(learner.data.stream):
+            torch.cuda._sleep(100_000_000)  # about 50 ms
+        learner.step(staging)
+        staging.fill_(7.0)
+        assert np.array_equal(learner.data.raw_state()[:256].T, rows.numpy())

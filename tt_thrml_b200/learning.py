@@ -80,8 +80,10 @@ class DenseLearner:
     their hidden units, runs `sweeps` sweeps of the persistent chains, takes the
     moment differences, steps the masters and rounds them into both samplers'
     operands.  It returns the gradient of minus the mean log likelihood as the
-    triple that was stepped with (overwritten by the next step) and does not
-    synchronise.
+    triple that was stepped with (overwritten by the next step).  It does not wait
+    for the device's work; of a batch in host memory (complete when step is called)
+    it waits for the copy, which runs beside that work, so the caller may fill the
+    batch anew at once.
     """
 
     def __init__(self, program, *, n_data, n_chains, config=None, device=None, sweeps=1, lr=1e-3, betas=(0.9, 0.999),
@@ -122,6 +124,7 @@ class DenseLearner:
             ex.load_state([start(ex.n_chains, n_v, self._visible_family), start(ex.n_chains, n_h, Family.SPIN)], [])
             # one stream of draws for the whole run, another one for each executor
             ex._prepare_rng_for_n_sweeps((int(seed) << 1) + k, 2**31 - 1)
+        self._copies = torch.cuda.Stream(device=dev)
         self._hidden_group = next(gr for gr in self.data.compiled.sampling_groups if tuple(gr.block_indices) == (1,))
 
     def step(self, batch):
@@ -131,6 +134,11 @@ class DenseLearner:
         if not isinstance(batch, torch.Tensor) or tuple(batch.shape) != (n, n_v):
             raise ValueError(f"batch must be a tensor of shape {(n, n_v)}, got {getattr(batch, 'shape', type(batch))}")
         current = torch.cuda.current_stream(data._tdev)
+        if batch.device.type == "cpu":
+            # on a stream of its own: behind the sweeps of earlier steps the copy would still read the batch long after
+            # step has returned
+            with torch.cuda.stream(self._copies):
+                batch = batch.to(data._tdev)
         data.stream.wait_stream(current)
         with torch.cuda.stream(data.stream):
             values = batch.to(data._tdev, non_blocking=True)
