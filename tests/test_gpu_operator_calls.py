@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from tt_thrml_b200 import make_cuda_config, workloads
+from tt_thrml_b200 import Executor, make_cuda_config, workloads
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,47 @@ def test_a_host_batch_may_be_filled_anew_at_once(tt, pinned):
         learner.step(staging)
         staging.fill_(7.0)
         assert np.array_equal(learner.data.raw_state()[:256].T, rows.numpy())
+
+
+def loaded(program, config, chains=128, device=None):
+    ex = Executor(None, device, program, config, n_chains=chains)
+    g = torch.Generator().manual_seed(3)
+    ex.load_state([torch.randn((chains, 256), generator=g), torch.randint(0, 2, (chains, 512), generator=g).bool()], [])
+    return ex
+
+
+def outputs_of(tt, operator):
+    """A call that writes the tensors it is given, and their shapes."""
+    if operator == "int8":
+        w, x = tt.quantize_rows(torch.ones((4, 64), device="cuda")), torch.ones((2, 64), device="cuda")
+        return (lambda o: tt.int8_product(x, w, out=o[0])), [(2, 4)]
+    if operator == "moments":
+        x, y = torch.ones((4, 5), dtype=BF16, device="cuda"), torch.ones((4, 6), dtype=BF16, device="cuda")
+        return (lambda o: tt.pair_moments(x, y, out=tuple(o), units=True)), [(5, 6), (5,), (6,)]
+    ex = loaded(rbm(), make_cuda_config(dense_precision="int8"))
+    return (lambda o: ex.dense_moments(out=tuple(o), accumulate=True)), [(256, 512), (256,), (512,)]
+
+
+@pytest.mark.parametrize("operator", ["int8", "moments", "dense"])
+def test_autograd_sees_that_an_output_was_written(tt, operator):
+    call, shapes = outputs_of(tt, operator)
+    for i in range(len(shapes)):
+        outs = [torch.zeros(s, device="cuda") for s in shapes]
+        leaf = torch.ones(shapes[i], device="cuda", requires_grad=True)
+        saved = (leaf * outs[i]).sum()
+        call(outs)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+
+
+@pytest.mark.parametrize("operator", ["int8", "moments", "dense"])
+def test_outputs_that_require_a_gradient_are_refused(tt, operator):
+    call, shapes = outputs_of(tt, operator)
+    for i in range(len(shapes)):
+        outs = [torch.zeros(s, device="cuda") for s in shapes]
+        outs[i].requires_grad_(True)
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call(outs)
+        assert not any(o.detach().any() for o in outs)
+        with torch.no_grad():
+            call(outs)

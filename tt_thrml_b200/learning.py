@@ -13,7 +13,7 @@ from .core import Family, make_cuda_config, open_device
 from .executor import Executor
 from .moments import launch
 from .optim import AdamW
-from .quantized import require_cuda
+from .quantized import mark_written, refuse_written_grad, require_cuda
 
 
 def _torch():
@@ -51,6 +51,8 @@ def dense_moments(terms, *, out=None, accumulate: bool = False):
             require_cuda(name, t, dev)
             if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
+            refuse_written_grad(name, t)
+        mark_written(*out)
     for ex, _ in terms:
         current.wait_stream(ex.stream)
     nat.bind_device(dev.index)

@@ -11,7 +11,18 @@ two dense blocks at once, on the tensor cores.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import _error_addresses, current_device, dtype_code, error_word, on_device, raw_stream, refuse_overlap, require_cuda
+from .quantized import (
+    _error_addresses,
+    current_device,
+    dtype_code,
+    error_word,
+    mark_written,
+    on_device,
+    raw_stream,
+    refuse_overlap,
+    refuse_written_grad,
+    require_cuda,
+)
 
 
 def _torch():
@@ -129,6 +140,8 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
         for name, t in (("out", out), ("x_sum", x_sum), ("y_sum", y_sum)):
             if t is not None:
                 refuse_overlap(name, t, inputs)
+                refuse_written_grad(name, t)
+        mark_written(*(t for t in (out, x_sum, y_sum) if t is not None))
     phases = (nat.MomentPhase * len(xs))()
     with on_device(dev):
         stream = raw_stream(dev.index)

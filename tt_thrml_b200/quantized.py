@@ -116,6 +116,18 @@ def _no_grad(name: str, t):
         raise RuntimeError(f"{name} requires a gradient, but 8-bit products have no backward pass (use torch.no_grad())")
 
 
+def refuse_written_grad(name: str, out) -> None:
+    """Raises for an output that requires a gradient: kernels write it behind autograd's back."""
+    torch = _torch()
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise RuntimeError(f"{name} requires a gradient and cannot be written in place (use torch.no_grad())")
+
+
+def mark_written(*outs) -> None:
+    """Tells autograd that a kernel wrote the tensors: backward passes that saved them raise."""
+    nat.hostcall().bump_versions(list(outs))
+
+
 def memory_span(t) -> tuple[int, int]:
     """First and last-plus-one address that a tensor's elements lie in."""
     if not t.numel():
@@ -262,13 +274,14 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
     out_code = dtype_code(out_dtype)
     if out_code is None:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    if out is None:
+    given = out is not None
+    if not given:
         out, out_ld = torch.empty((*lead, N), dtype=out_dtype, device=dev), N
     else:
         require_cuda("out", out, dev)
         if out.dtype != out_dtype or out.shape != (*lead, N):
             raise ValueError(f"out must be {out_dtype} of shape {(*lead, N)}, got {out.dtype} of {tuple(out.shape)}")
-        _no_grad("out", out)
+        refuse_written_grad("out", out)
         flat = out.view(-1, N) if N else out  # raises if the rows cannot be one matrix
         if flat.numel() and ((N > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < N)):
             raise ValueError("out needs dense rows that do not overlap")
@@ -277,6 +290,8 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
         out_ld = flat.stride(0) if N and flat.shape[0] > 1 else N
     if not out.numel():
         return out
+    if given:
+        mark_written(out)
     if rows.dim() != 2:
         rows = rows.reshape(-1, K)
     M = rows.shape[0]
