@@ -136,3 +136,18 @@ def test_outputs_that_require_a_gradient_are_refused(tt, operator):
         assert not any(o.detach().any() for o in outs)
         with torch.no_grad():
             call(outs)
+
+
+def test_outputs_that_share_memory_are_refused(tt):
+    x = torch.ones((4, 6), dtype=BF16, device="cuda")
+    out, s = torch.zeros((6, 6), device="cuda"), torch.zeros(6, device="cuda")
+    for outs in ((out, s, s), (out, out[1], s), (out, s, out[5])):
+        with pytest.raises(ValueError, match="share memory"):
+            tt.pair_moments(x, x, out=outs, units=True)
+    ex = loaded(rbm(), make_cuda_config())
+    out, s = torch.zeros((256, 512), device="cuda"), torch.zeros(512, device="cuda")
+    for outs in ((out, s[:256], s), (out, out[0, :256], s)):
+        with pytest.raises(ValueError, match="share memory"):
+            ex.dense_moments(out=outs)
+    torch.cuda.synchronize()
+    assert not out.any() and not s.any()

@@ -248,3 +248,15 @@ def test_an_error_on_another_device_leaves_no_binding(monkeypatch):
     assert nat._bound.device is None
     nat.bind_device(0)
     assert bound == [1, 0]
+
+
+def test_outputs_that_share_memory_are_refused():
+    from tt_thrml_b200.quantized import refuse_shared_outputs
+
+    buffer = torch.zeros(100)
+    out, x_sum, y_sum = buffer[:25].view(5, 5), buffer[25:30], buffer[30:35]
+    refuse_shared_outputs([("out", out), ("x_sum", x_sum), ("y_sum", y_sum)])
+    refuse_shared_outputs([("out", out[:0]), ("x_sum", buffer[:0])])
+    for outs in ([out, x_sum, x_sum], [out, out[2], y_sum], [out, buffer[24:29], y_sum], [out, x_sum, buffer[29:34]]):
+        with pytest.raises(ValueError, match="share memory"):
+            refuse_shared_outputs(list(zip(("out", "x_sum", "y_sum"), outs)))

@@ -13,7 +13,7 @@ from .core import Family, make_cuda_config, open_device
 from .executor import Executor
 from .moments import launch
 from .optim import AdamW
-from .quantized import mark_written, refuse_written_grad, require_cuda
+from .quantized import mark_written, refuse_shared_outputs, refuse_written_grad, require_cuda
 
 
 def _torch():
@@ -52,6 +52,7 @@ def dense_moments(terms, *, out=None, accumulate: bool = False):
             if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float32 of shape {shape}, got {t.dtype} of {tuple(t.shape)}")
             refuse_written_grad(name, t)
+        refuse_shared_outputs([(f"out[{i}]", t) for i, t in enumerate(out)])
         mark_written(*out)
     for ex, _ in terms:
         current.wait_stream(ex.stream)

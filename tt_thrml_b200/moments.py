@@ -20,6 +20,7 @@ from .quantized import (
     on_device,
     raw_stream,
     refuse_overlap,
+    refuse_shared_outputs,
     refuse_written_grad,
     require_cuda,
 )
@@ -137,11 +138,12 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
         if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError("out needs dense rows that do not overlap")
         inputs = [(f"{name}[{p}]", t) for name, ts in (("x", xs), ("y", ys)) for p, t in enumerate(ts)]
-        for name, t in (("out", out), ("x_sum", x_sum), ("y_sum", y_sum)):
-            if t is not None:
-                refuse_overlap(name, t, inputs)
-                refuse_written_grad(name, t)
-        mark_written(*(t for t in (out, x_sum, y_sum) if t is not None))
+        outs = [(name, t) for name, t in (("out", out), ("x_sum", x_sum), ("y_sum", y_sum)) if t is not None]
+        refuse_shared_outputs(outs)
+        for name, t in outs:
+            refuse_overlap(name, t, inputs)
+            refuse_written_grad(name, t)
+        mark_written(*(t for _, t in outs))
     phases = (nat.MomentPhase * len(xs))()
     with on_device(dev):
         stream = raw_stream(dev.index)

@@ -144,6 +144,16 @@ def refuse_overlap(name: str, out, inputs) -> None:
             raise ValueError(f"{name} shares memory with {other}, which the kernel reads meanwhile")
 
 
+def refuse_shared_outputs(outs) -> None:
+    """Raises if two of the (name, tensor) outputs of one call share memory: the kernel writes both."""
+    for i, (name, t) in enumerate(outs):
+        a, b = memory_span(t)
+        for other, u in outs[i + 1 :]:
+            c, d = memory_span(u)
+            if a < d and c < b:
+                raise ValueError(f"{name} and {other} share memory, and the kernel writes both")
+
+
 class QuantizedRows:
     """A matrix as int8 rows with one float32 scale per row: value[r, c] = values[r, c] * scale[r].
 
