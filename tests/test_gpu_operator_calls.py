@@ -7,6 +7,7 @@ from pathlib import Path
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from tt_thrml_b200 import Executor, make_cuda_config, workloads
 
@@ -151,3 +152,39 @@ def test_outputs_that_share_memory_are_refused(tt):
             ex.dense_moments(out=outs)
     torch.cuda.synchronize()
     assert not out.any() and not s.any()
+
+
+@pytest.mark.parametrize("derivative", ["gradient", "tangent"])
+def test_derivatives_are_not_dropped(tt, derivative):
+    """Every input that a derivative could be asked of, from the first call and in the plain case after it."""
+    r, m = tt.quantize_rows(torch.ones((4, 64), device="cuda")), torch.ones((4, 5), dtype=BF16, device="cuda")
+    x, bias = torch.ones((2, 64), device="cuda"), torch.ones(4, device="cuda")
+    tt.int8_product(x, r)
+    tt.pair_moments(m, m)
+    out = torch.zeros((2, 4), device="cuda")
+    with fw.dual_level():
+        def d(t):
+            return t.clone().requires_grad_(True) if derivative == "gradient" else fw.make_dual(t.clone(), torch.ones_like(t))
+
+        calls = {
+            "x": lambda: tt.int8_product(d(x), r),
+            "x, strided": lambda: tt.int8_product(d(x.repeat(1, 2))[:, ::2], r),
+            "x, given output": lambda: tt.int8_product(d(x), r, out=out),
+            "bias": lambda: tt.int8_product(x, r, bias=d(bias)),
+            "scale": lambda: tt.int8_product(x, tt.QuantizedRows(r.values, d(r.scale))),
+            "scale, given output": lambda: tt.int8_product(x, tt.QuantizedRows(r.values, d(r.scale)), out=out),
+            "scale of x": lambda: tt.int8_product(tt.QuantizedRows(r.values, d(r.scale)), r),
+            "rows": lambda: tt.quantize_rows(d(x)),
+            "moments of x": lambda: tt.pair_moments(d(m), m),
+            "moments of y": lambda: tt.pair_moments(m, d(m), units=True),
+            "moments, given output": lambda: tt.pair_moments([m, d(m)], [m, m], out=torch.zeros((5, 5), device="cuda")),
+        }
+        for name, call in calls.items():
+            with pytest.raises(RuntimeError, match="requires a gradient" if derivative == "gradient" else "tangent"):
+                call()
+                pytest.fail(name)
+        if derivative == "gradient":
+            with torch.no_grad():
+                for call in calls.values():
+                    call()
+    assert tt.int8_product(x, r).requires_grad is False

@@ -49,7 +49,10 @@ template <typename Fn>
 Fn address(PyObject* o) {
   return reinterpret_cast<Fn>(PyLong_AsVoidPtr(o));
 }
-bool wants_grad(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// Whether a derivative is asked of t: a gradient, or the tangent of a forward-mode dual tensor.
+bool wants_grad(const at::Tensor& t) {
+  return (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined();
+}
 
 // What stays the same from step to step of an optimizer (AdamWCall in _native.py).
 struct AdamWCall {
@@ -154,7 +157,7 @@ PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t pitch = PyLong_AsLongLong(args[3]);
   if (PyErr_Occurred()) return nullptr;
   const int32_t code = dtype_code(x);
-  if (!plain_cuda(x, device) || code < 0 || x.dim() < 1 || wants_grad(x) || (x.dim() != 2 && !x.is_contiguous()))
+  if (!plain_cuda(x, device) || code < 0 || x.dim() < 1 || wants_grad(x) || wants_grad(ws) || (x.dim() != 2 && !x.is_contiguous()))
     Py_RETURN_NONE;
   const int64_t K = x.size(-1), N = w.size(0);
   if (K != w.size(1) || K < 1 || N < 1 || x.numel() == 0) Py_RETURN_NONE;

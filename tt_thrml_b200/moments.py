@@ -19,6 +19,7 @@ from .quantized import (
     mark_written,
     on_device,
     raw_stream,
+    refuse_grad,
     refuse_overlap,
     refuse_shared_outputs,
     refuse_written_grad,
@@ -100,17 +101,13 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
     code = dtype_code(dtype)
     if code not in (nat.DT_BF16, nat.DT_F16):
         raise ValueError(f"x and y must be bfloat16 or float16, got {dtype}")
-    grad = torch.is_grad_enabled()
     shapes = []
     for p, (a, b) in enumerate(zip(xs, ys)):
         for name, t in (("x", a), ("y", b)):
             require_cuda(name, t, dev)
             if t.dtype != dtype or t.dim() != 2:
                 raise ValueError(f"{name}[{p}] must be a {dtype} matrix, got {t.dtype} of shape {tuple(t.shape)}")
-            if grad and t.requires_grad:
-                raise RuntimeError(
-                    f"{name}[{p}] requires a gradient, but pair moments have no backward pass (use torch.no_grad())"
-                )
+            refuse_grad(f"{name}[{p}]", t, "pair moments")
         (chains, m), (other, n) = a.shape, b.shape
         if chains != other:
             raise ValueError(f"phase {p}: x has {chains} chains, y has {other}")

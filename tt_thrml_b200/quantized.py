@@ -10,8 +10,8 @@ on how the kernels split them.  A dense program runs its sweeps on the same
 arithmetic with `dense_precision="int8"` (make_cuda_config).
 
 The kernels launch on the current stream of the rows' device; nothing
-synchronises.  There is no backward pass: rows that require a gradient are
-refused.
+synchronises.  There is no backward pass and no forward-mode derivative: rows,
+biases and scales that require a gradient or carry a tangent are refused.
 """
 
 from __future__ import annotations
@@ -110,10 +110,18 @@ def require_cuda(name: str, t, device=None):
     raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
-def _no_grad(name: str, t):
+def refuse_grad(name: str, t, what: str) -> None:
+    """Raises for an input whose derivative `what`, which have none, would drop: a gradient asked for, or the tangent
+    of a forward-mode dual tensor."""
     torch = _torch()
     if torch.is_grad_enabled() and t.requires_grad:
-        raise RuntimeError(f"{name} requires a gradient, but 8-bit products have no backward pass (use torch.no_grad())")
+        raise RuntimeError(f"{name} requires a gradient, but {what} have no backward pass (use torch.no_grad())")
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} carries a tangent, but {what} have no forward-mode derivative")
+
+
+def _no_grad(name: str, t):
+    refuse_grad(name, t, "8-bit products")
 
 
 def refuse_written_grad(name: str, out) -> None:
@@ -268,6 +276,9 @@ def int8_product(x, weights: QuantizedRows, *, bias=None, out_dtype=None, out=No
     if code is None or rows.dim() < 1:
         raise ValueError(f"x must hold float32, bfloat16 or float16 rows, got {x.dtype} of shape {tuple(x.shape)}")
     _no_grad("x", rows)
+    for name, q in (("x", x), ("weights", weights)):
+        if isinstance(q, QuantizedRows) and q.scale is not None:
+            _no_grad(f"the scale of {name}", q.scale)
     lead, K = rows.shape[:-1], rows.shape[-1]
     if K != w.shape[1]:
         raise ValueError(f"x has rows of {K}, the weights have {w.shape[1]} columns")
