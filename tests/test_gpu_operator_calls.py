@@ -188,3 +188,19 @@ def test_derivatives_are_not_dropped(tt, derivative):
                 for call in calls.values():
                     call()
     assert tt.int8_product(x, r).requires_grad is False
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp32", "int8"])
+@pytest.mark.parametrize("device", ["cuda", "cpu"])
+def test_a_batch_that_requires_a_gradient_leaves_no_graph(tt, precision, device):
+    def run(requires_grad):
+        learner = tt.DenseLearner(rbm(), n_data=128, n_chains=128, config=make_cuda_config(dense_precision=precision))
+        g = torch.Generator().manual_seed(5)
+        for _ in range(2):
+            batch = torch.randn((128, 256), generator=g).to(device).requires_grad_(requires_grad)
+            gradient = learner.step(batch * 1.0)
+            assert not any(t.requires_grad for t in (*gradient, *learner.data._block_states))
+        return learner.data.raw_state(), learner.weights.cpu()
+
+    (s1, w1), (s2, w2) = run(False), run(True)
+    assert np.array_equal(s1, s2) and torch.equal(w1, w2)

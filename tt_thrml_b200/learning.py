@@ -132,10 +132,16 @@ class DenseLearner:
 
     def step(self, batch):
         torch = _torch()
-        data, model = self.data, self.model
-        n, n_v = data.n_chains, self.weights.shape[0]
+        n, n_v = self.data.n_chains, self.weights.shape[0]
         if not isinstance(batch, torch.Tensor) or tuple(batch.shape) != (n, n_v):
             raise ValueError(f"batch must be a tensor of shape {(n, n_v)}, got {getattr(batch, 'shape', type(batch))}")
+        with torch.no_grad():  # the states are drawn: nothing of the batch's graph goes on into them
+            return self._step(batch.detach())
+
+    def _step(self, batch):
+        torch = _torch()
+        data, model = self.data, self.model
+        n = data.n_chains
         current = torch.cuda.current_stream(data._tdev)
         if batch.device.type == "cpu":
             # on a stream of its own: behind the sweeps of earlier steps the copy would still read the batch long after
