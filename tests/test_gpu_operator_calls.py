@@ -9,6 +9,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
+from test_gpu_adamw import formula64
 from tt_thrml_b200 import Executor, make_cuda_config, workloads
 
 pytestmark = pytest.mark.gpu
@@ -204,3 +205,28 @@ def test_a_batch_that_requires_a_gradient_leaves_no_graph(tt, precision, device)
 
     (s1, w1), (s2, w2) = run(False), run(True)
     assert np.array_equal(s1, s2) and torch.equal(w1, w2)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("beta2", [0.999, 0.5, 0.9999999])
+@pytest.mark.parametrize("eps", [1e-30, 1e-20, 1e-18, 1e-12, 4e-10, 5e-10, 1e-8])
+def test_tiny_gradients_with_tiny_eps(tt, bits, eps, beta2):
+    """Second moments below the smallest normal float32, some below the smallest subnormal: the update is the formula's
+    for every eps that is allowed.  The computed v lies within ev of v1 (formula64: its roundings and 1e-44 for
+    subnormal ones), not below 0, and the root, the denominator and the quotient are monotonic in it, so the
+    update lies between those of v1 - ev and v1 + ev, less and more the 13.1 roundings of the coded steps elsewhere.
+    (Where v1 <= ev, float32 need not hold v at all and m / eps is within this bound; elsewhere it is narrow.)"""
+    g = torch.Generator().manual_seed(1)
+    grads = torch.randn(4000, generator=g) * 10.0 ** (torch.rand(4000, generator=g) * 6 - 23)
+    h = dict(lr=1e-3, betas=(0.9, beta2), eps=eps, weight_decay=0.0)
+    p, zero = torch.zeros(4000, device="cuda"), torch.zeros(4000)
+    opt = tt.AdamW([p], state_bits=bits, **h)
+    opt.step([grads.cuda()])
+    (_, m1, v1), (_, em, ev) = formula64(zero, grads, zero, zero, 1, h, F32)
+    step, r = 1e-3 / (1 - 0.9), (1 - beta2) ** -0.5
+    least = step * (m1.abs() - em) / ((v1 + ev).sqrt() * r + eps) * (1 - 14.1 * 2.0**-24)
+    most = step * (m1.abs() + em) / ((v1 - ev).clamp_min(0).sqrt() * r + eps) * (1 + 14.1 * 2.0**-24)
+    got = -p.cpu().double() * grads.sign()
+    assert ((least <= got) & (got <= most)).all()
+    narrow = v1 > 4 * ev  # the bound says something there
+    assert narrow.sum() > 500 and (most[narrow] < 1.4 * least[narrow]).all()

@@ -3,6 +3,8 @@
     m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
     p = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
+in float32 throughout: a v that float32 cannot hold (below 7e-46) is 0, as it is in float32 arithmetic elsewhere.
+
 What a sampler's moments are turned into: the couplings and biases of a
 program (see `pair_moments` and `DenseLearner`) are tensors of very different
 sizes, stepped together.  With `state_bits=8` the moments take 2 bytes and a
