@@ -230,3 +230,23 @@ def test_tiny_gradients_with_tiny_eps(tt, bits, eps, beta2):
     assert ((least <= got) & (got <= most)).all()
     narrow = v1 > 4 * ev  # the bound says something there
     assert narrow.sum() > 500 and (most[narrow] < 1.4 * least[narrow]).all()
+
+
+def test_a_learner_reports_expired_waits(tt):
+    """The words are set from the host, as a kernel that gives up sets them."""
+    from tt_thrml_b200 import quantized
+
+    learner = tt.DenseLearner(rbm(), n_data=128, n_chains=128)
+    learner.step(torch.zeros((128, 256)))
+    learner.check()
+    for word in (quantized.error_word(learner.weights.device), learner.model._error_word, learner.data._error_word):
+        word.fill_(2)
+        with pytest.raises(RuntimeError, match="expired wait"):
+            learner.check()
+        word.zero_()
+        torch.cuda.synchronize()
+        learner.check()
+    quantized.error_word(learner.weights.device).fill_(2)
+    with pytest.raises(RuntimeError, match="expired wait"):
+        tt.check_operator_errors()
+    tt.check_operator_errors()

@@ -260,3 +260,20 @@ def test_outputs_that_share_memory_are_refused():
     for outs in ([out, x_sum, x_sum], [out, out[2], y_sum], [out, buffer[24:29], y_sum], [out, x_sum, buffer[29:34]]):
         with pytest.raises(ValueError, match="share memory"):
             refuse_shared_outputs(list(zip(("out", "x_sum", "y_sum"), outs)))
+
+
+def test_an_expired_wait_is_reported_once(monkeypatch):
+    from tt_thrml_b200 import quantized
+
+    words = {0: torch.tensor([3], dtype=torch.int32), 1: torch.tensor([1], dtype=torch.int32), 2: torch.zeros(1, dtype=torch.int32)}
+    monkeypatch.setattr(quantized, "_error_words", words)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda index=None: None)
+    tt.check_operator_errors("cuda:2")
+    with pytest.raises(RuntimeError, match=r"code 1, device 1"):
+        tt.check_operator_errors(torch.device("cuda", 1))
+    tt.check_operator_errors("cuda:1")
+    words[1].fill_(2)
+    with pytest.raises(RuntimeError, match=r"code 3, device 0.*code 2, device 1"):
+        tt.check_operator_errors()
+    tt.check_operator_errors()
+    assert not any(w.item() for w in words.values())

@@ -13,7 +13,7 @@ from .core import Family, make_cuda_config, open_device
 from .executor import Executor
 from .moments import launch
 from .optim import AdamW
-from .quantized import mark_written, refuse_shared_outputs, refuse_written_grad, require_cuda
+from .quantized import check_operator_errors, mark_written, refuse_shared_outputs, refuse_written_grad, require_cuda
 
 
 def _torch():
@@ -28,7 +28,8 @@ def dense_moments(terms, *, out=None, accumulate: bool = False):
     Returns float32 (pair [n_0, n_1], block 0 [n_0], block 1 [n_1]); `out` is such
     a triple to write, or, with `accumulate`, to add to.  Ordered after the
     executors' sweeps and before their next ones; queued on the current stream.  All executors (a MeshExecutor counts as
-    its local shards) must be on one device."""
+    its local shards) must be on one device.
+    An in-kernel wait that expires is reported by check_operator_errors()."""
     torch = _torch()
     # a mesh of chains is the sum of its shards
     terms = [(shard, float(s)) for ex, s in terms for shard in getattr(ex, "shards", [ex])]
@@ -86,7 +87,8 @@ class DenseLearner:
     triple that was stepped with (overwritten by the next step).  It does not wait
     for the device's work; of a batch in host memory (complete when step is called)
     it waits for the copy, which runs beside that work, so the caller may fill the
-    batch anew at once.
+    batch anew at once.  check() raises if a kernel of the steps so far gave up a
+    wait: the masters are not to be relied on then.
     """
 
     def __init__(self, program, *, n_data, n_chains, config=None, device=None, sweeps=1, lr=1e-3, betas=(0.9, 0.999),
@@ -165,6 +167,12 @@ class DenseLearner:
         data.update_dense_weights(self.weights, self.visible_bias, self.hidden_bias)
         model.share_dense_weights(data)
         return self.gradient
+
+    def check(self) -> None:
+        """Raises if a kernel of the steps so far gave up an in-kernel wait.  Synchronises."""
+        self.data.check_device_errors()
+        self.model.check_device_errors()
+        check_operator_errors(self.data._tdev)
 
 
 __all__ = ["dense_moments", "DenseLearner"]

@@ -77,6 +77,7 @@ def pair_moments(x, y, scale=1.0, *, out=None, accumulate=False, units=False):
     between phases and may be 0); scale: a number or one per phase.  out: float32
     [M, N] with dense rows (with `units` a tuple of out, x_sum [M], y_sum [N]) to
     write, or, with `accumulate`, to add to.  The result is the same every time.
+    An in-kernel wait that expires is reported by check_operator_errors().
     """
     torch = _torch()
     xs, ys = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (x, y))

@@ -10,8 +10,10 @@ on how the kernels split them.  A dense program runs its sweeps on the same
 arithmetic with `dense_precision="int8"` (make_cuda_config).
 
 The kernels launch on the current stream of the rows' device; nothing
-synchronises.  There is no backward pass and no forward-mode derivative: rows,
-biases and scales that require a gradient or carry a tangent are refused.
+synchronises.  A kernel whose wait for its own copies or products expires (two
+seconds) gives up and leaves a code that check_operator_errors reports.
+There is no backward pass and no forward-mode derivative: rows, biases and
+scales that require a gradient or carry a tangent are refused.
 """
 
 from __future__ import annotations
@@ -67,15 +69,21 @@ def error_word(device):
 
 
 def check_operator_errors(device=None) -> None:
-    """Raises if an operator kernel on `device` (default: every device used) reported an expired wait."""
+    """Raises if an operator kernel on `device` (default: every device used) reported an expired wait since the last
+    report; what such a kernel wrote is not its result.  Synchronises."""
     torch = _torch()
+    found = []
     for index, word in list(_error_words.items()):
         if device is not None and torch.device(device).index not in (None, index):
             continue
         torch.cuda.synchronize(index)
         code = int(word.item())
         if code:
-            raise RuntimeError(f"a device kernel reported an expired wait (code {code})")
+            found.append(f"a device kernel reported an expired wait (code {code}, device {index})")
+            word.zero_()  # reported once
+            torch.cuda.synchronize(index)
+    if found:
+        raise RuntimeError("; ".join(found))
 
 
 @contextlib.contextmanager
