@@ -1,6 +1,9 @@
 """Operators' argument checks on the CPU: rejected calls touch neither the device nor the stand-in pointers."""
 
+import contextlib
 import ctypes
+import gc
+import threading
 
 import numpy as np
 import pytest
@@ -277,3 +280,34 @@ def test_an_expired_wait_is_reported_once(monkeypatch):
         tt.check_operator_errors()
     tt.check_operator_errors()
     assert not any(w.item() for w in words.values())
+
+
+@pytest.mark.parametrize("ran", [True, False])
+def test_captures_in_two_threads_pause_the_collector_together(monkeypatch, ran):
+    monkeypatch.setattr(torch.cuda, "graph", lambda graph, stream=None: contextlib.nullcontext())
+    started, finish, seen = threading.Event(), threading.Event(), []
+
+    def other():
+        with nat.capturing(None):
+            started.set()
+            finish.wait(10)
+            seen.append(gc.isenabled())
+
+    was = gc.isenabled()
+    (gc.enable if ran else gc.disable)()
+    try:
+        thread = threading.Thread(target=other)
+        with nat.capturing(None):
+            thread.start()
+            assert started.wait(10) and not gc.isenabled()
+        assert not gc.isenabled()  # the other thread still captures
+        finish.set()
+        thread.join(10)
+        assert seen == [False] and gc.isenabled() is ran
+        with pytest.raises(RuntimeError, match="inside"):
+            with nat.capturing(None):
+                raise RuntimeError("inside")
+        assert gc.isenabled() is ran
+    finally:
+        finish.set()
+        (gc.enable if was else gc.disable)()

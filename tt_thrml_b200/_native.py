@@ -344,22 +344,34 @@ def stream_handle(stream) -> int | None:
     return None if stream is None else stream.cuda_stream
 
 
+_captures_lock = threading.Lock()
+_captures = 0  # under way in this process, and whether the collector ran before the first of them
+_collector_ran = False
+
+
 @contextlib.contextmanager
 def capturing(graph, stream=None):
     """torch.cuda.graph with the cyclic garbage collector paused: a CUDA graph that it frees meanwhile (one held by a
-    reference cycle) would end the capture with an error."""
+    reference cycle) would end the capture with an error.  The collector is the process's: with captures in several
+    threads the last one to end starts it again."""
     import gc
 
     import torch
 
-    was = gc.isenabled()
-    gc.disable()
+    global _captures, _collector_ran
+    with _captures_lock:
+        if _captures == 0:
+            _collector_ran = gc.isenabled()
+        _captures += 1
+        gc.disable()
     try:
         with torch.cuda.graph(graph, stream=stream):
             yield
     finally:
-        if was:
-            gc.enable()
+        with _captures_lock:
+            _captures -= 1
+            if _captures == 0 and _collector_ran:
+                gc.enable()
 
 
 _bound = threading.local()
