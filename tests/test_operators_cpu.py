@@ -311,3 +311,33 @@ def test_captures_in_two_threads_pause_the_collector_together(monkeypatch, ran):
     finally:
         finish.set()
         (gc.enable if was else gc.disable)()
+
+
+def test_the_host_module_is_made_again_for_another_torch(monkeypatch, tmp_path):
+    from tt_thrml_b200 import build
+
+    made = []
+
+    def compiler(cmd, check):
+        assert check
+        made.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("module")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    monkeypatch.setattr(build, "BUILD_DIR", tmp_path / "objects")
+    monkeypatch.setattr(build, "HOSTCALL_PATH", tmp_path / "_hostcall.so")
+    for count in (1, 1):
+        assert build.build_hostcall() == tmp_path / "_hostcall.so" and len(made) == count
+    with monkeypatch.context() as other:
+        other.setattr(torch, "__version__", torch.__version__ + ".other")
+        for count in (2, 2):
+            build.build_hostcall()
+            assert len(made) == count
+    build.build_hostcall()
+    with monkeypatch.context() as other:
+        other.setattr(build.sys, "version", "another Python")
+        build.build_hostcall()
+    assert len(made) == 4
+    build.build_hostcall(force=True)
+    assert len(made) == 5

@@ -47,14 +47,18 @@ def _headers() -> list[Path]:
 
 
 def build_hostcall(verbose: bool = False, force: bool = False) -> Path:
-    """The CPython module that reads tensors' addresses (g++ against torch's headers)."""
-    src = CSRC / "hostcall.cpp"
-    newest = max(src.stat().st_mtime, (REPO_DIR / "include" / "tthrml.h").stat().st_mtime)
-    if not force and HOSTCALL_PATH.exists() and HOSTCALL_PATH.stat().st_mtime >= newest:
-        return HOSTCALL_PATH
+    """The CPython module that reads tensors' addresses (g++ against torch's headers); made again for another torch or
+    Python, whose layouts it has compiled in."""
     import torch
 
+    src = CSRC / "hostcall.cpp"
+    newest = max(src.stat().st_mtime, (REPO_DIR / "include" / "tthrml.h").stat().st_mtime)
     root = Path(torch.__file__).resolve().parent
+    key = f"torch {torch.__version__} {torch.version.git_version} at {root}, {sys.version}\n"
+    stamp = BUILD_DIR / "hostcall.key"
+    if (not force and HOSTCALL_PATH.exists() and HOSTCALL_PATH.stat().st_mtime >= newest and stamp.exists()
+            and stamp.read_text() == key):
+        return HOSTCALL_PATH
     tmp = HOSTCALL_PATH.with_suffix(".so.tmp")
     cmd = [
         os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
@@ -67,6 +71,8 @@ def build_hostcall(verbose: bool = False, force: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, HOSTCALL_PATH)
+    BUILD_DIR.mkdir(parents=True, exist_ok=True)
+    stamp.write_text(key)
     return HOSTCALL_PATH
 
 
