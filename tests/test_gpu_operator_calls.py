@@ -250,3 +250,23 @@ def test_a_learner_reports_expired_waits(tt):
     with pytest.raises(RuntimeError, match="expired wait"):
         tt.check_operator_errors()
     tt.check_operator_errors()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 70])
+def test_outputs_beside_their_inputs_in_one_matrix(tt, rows):
+    """Ranges of columns that do not meet, as a program that concatenates keeps them."""
+    g = torch.Generator().manual_seed(2)
+    w = tt.quantize_rows(torch.randn((40, 64), generator=g).cuda())
+    both = torch.zeros((rows, 112), device="cuda")
+    x = torch.randn((rows, 64), generator=g).cuda()
+    both[:, 40:104] = x
+    assert tt.int8_product(both[:, 40:104], w, out=both[:, :40]).data_ptr() == both.data_ptr()
+    assert torch.equal(both[:, :40], tt.int8_product(x, w)) and torch.equal(both[:, 40:104], x) and not both[:, 104:].any()
+    with pytest.raises(ValueError, match="shares memory"):
+        tt.int8_product(both[:, 39:103], w, out=both[:, :40])
+    a, b = (torch.randint(-4, 5, (rows, n), generator=g).to(BF16).cuda() for n in (6, 10))
+    buffer = torch.zeros((7, 16), device="cuda")
+    outs = (buffer[:6, :10], buffer[6, 10:], buffer[6, :10])
+    tt.pair_moments(a, b, out=outs, units=True)
+    assert torch.equal(outs[0], a.float().t() @ b.float()) and not buffer[:6, 10:].any()
+    assert torch.equal(outs[1], a.float().sum(0)) and torch.equal(outs[2], b.float().sum(0))

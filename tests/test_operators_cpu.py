@@ -341,3 +341,44 @@ def test_the_host_module_is_made_again_for_another_torch(monkeypatch, tmp_path):
     assert len(made) == 4
     build.build_hostcall(force=True)
     assert len(made) == 5
+
+
+def views(base, seed):
+    """A view of a few rows and columns, of any strides, into a buffer of 600 elements."""
+    r = np.random.default_rng(seed)
+    pitch = int(r.choice([7, 12, 20]))
+    m = base[: 600 // pitch * pitch].view(-1, pitch)
+    r0, c0 = int(r.integers(0, 20)), int(r.integers(0, pitch))
+    v = m[r0 : r0 + int(r.integers(1, 9)), c0 : c0 + int(r.integers(1, 9))]
+    kind = r.integers(0, 6)
+    if kind == 0:
+        return v[::2]
+    if kind == 1:
+        return v.t()
+    if kind == 2:
+        return v[0]
+    if kind == 3:
+        return v[:, ::2]
+    if kind == 4:
+        return v[: v.shape[0] // 2 * 2].unflatten(0, (-1, 2)) if v.shape[0] > 1 else v
+    return v
+
+
+def test_views_that_share_memory():
+    """Against the elements themselves: nothing shared passes, and ranges of columns of one matrix do not collide."""
+    from tt_thrml_b200.quantized import share_memory
+
+    kept, base = 0, torch.arange(600)  # an element's value is its place
+    for i in range(6000):
+        a, b = views(base, 2 * i), views(base, 2 * i + 1)
+        shared = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert not shared or (share_memory(a, b) and share_memory(b, a)), (i, a.shape, a.stride(), b.shape, b.stride())
+        kept += not shared and not share_memory(a, b)
+    assert kept > 2000
+    both = torch.zeros(6, 20)
+    x, out = both[:, :8], both[:, 8:]
+    assert not share_memory(out, x) and not share_memory(x, out)
+    assert share_memory(both[:, :9], out) and share_memory(out, both[:, :9]) and share_memory(both[1:3, 19:], out)
+    assert not share_memory(both[2, :8], out) and not share_memory(out, both[5:, :8])
+    assert share_memory(out, both[2, 7:9]) and not share_memory(both[:0], both)
+    assert not share_memory(both.view(2, 3, 20)[:, :, :8], both.view(2, 3, 20)[..., 8:])

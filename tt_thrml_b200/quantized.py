@@ -152,21 +152,47 @@ def memory_span(t) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + reach * t.element_size()
 
 
+def _memory_rows(t) -> tuple[int, int] | None:
+    """(bytes from row to row, bytes of a row) of a tensor whose rows are dense and equally far apart, else None; one row
+    is as far from the next as any other tensor's."""
+    dims = [(n, st) for n, st in zip(t.shape, t.stride()) if n != 1]
+    width = 1
+    if dims and dims[-1][1] == 1:
+        width = dims.pop()[0]
+    if not dims:
+        return 0, width * t.element_size()
+    pitch = dims[-1][1]
+    if any(a[1] != b[0] * b[1] for a, b in zip(dims, dims[1:])):
+        return None
+    return pitch * t.element_size(), width * t.element_size()
+
+
+def share_memory(t, u) -> bool:
+    """Whether two tensors may share memory: their spans meet, and they are not two ranges of columns of one matrix."""
+    (a, b), (c, d) = memory_span(t), memory_span(u)
+    if not (a < d and c < b):
+        return False
+    rows, other = _memory_rows(t), _memory_rows(u)
+    if rows is None or other is None:
+        return True
+    pitch = rows[0] or other[0]
+    if pitch == 0 or (other[0] or pitch) != pitch:
+        return True
+    gap = (c - a) % pitch  # from a row of t to the next start of one of u
+    return not (rows[1] <= gap and gap + other[1] <= pitch)
+
+
 def refuse_overlap(name: str, out, inputs) -> None:
-    a, b = memory_span(out)
     for other, t in inputs:
-        c, d = memory_span(t)
-        if a < d and c < b:
+        if share_memory(out, t):
             raise ValueError(f"{name} shares memory with {other}, which the kernel reads meanwhile")
 
 
 def refuse_shared_outputs(outs) -> None:
     """Raises if two of the (name, tensor) outputs of one call share memory: the kernel writes both."""
     for i, (name, t) in enumerate(outs):
-        a, b = memory_span(t)
         for other, u in outs[i + 1 :]:
-            c, d = memory_span(u)
-            if a < d and c < b:
+            if share_memory(t, u):
                 raise ValueError(f"{name} and {other} share memory, and the kernel writes both")
 
 
