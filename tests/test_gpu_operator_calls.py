@@ -270,3 +270,18 @@ def test_outputs_beside_their_inputs_in_one_matrix(tt, rows):
     tt.pair_moments(a, b, out=outs, units=True)
     assert torch.equal(outs[0], a.float().t() @ b.float()) and not buffer[:6, 10:].any()
     assert torch.equal(outs[1], a.float().sum(0)) and torch.equal(outs[2], b.float().sum(0))
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp32", "int8"])
+def test_weights_of_any_strides(tt, precision):
+    """Expanded, transposed and cut-out couplings become the operands that their contiguous copies become."""
+    line = torch.linspace(-1, 1, 512, device="cuda")
+    whole = torch.randn((600, 700), generator=torch.Generator().manual_seed(1)).cuda()
+    a, b = (Executor(None, None, rbm(), make_cuda_config(n_chains=128, dense_precision=precision)) for _ in range(2))
+    for w in (line.expand(256, 512), line[:256, None].expand(256, 512), line[:1].expand(256, 512), whole[:512, :256].t(),
+              whole[3:259, 5:517], whole[::2, :][:256, 100:612]):
+        a.update_dense_weights(w)
+        b.update_dense_weights(w.clone(memory_format=torch.contiguous_format))
+        for p, q in zip(a._plans(), b._plans()):
+            assert torch.equal(p.weights_nk, q.weights_nk)
+            assert p.w_scale is None or torch.equal(p.w_scale, q.w_scale)

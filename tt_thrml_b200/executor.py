@@ -1058,6 +1058,8 @@ class Executor:
         nat.bind_device(self._tdev.index)
         self._stream.wait_stream(current)
         with torch.no_grad(), torch.cuda.stream(self._stream):
+            if not all(weights.stride()):  # an expanded matrix, which the 8-bit operands are not read from
+                weights = weights.contiguous()
             for plan, w, bias in ((plans[0], weights, bias_0), (plans[1], weights.t(), bias_1)):
                 self._own_operands(plan)
                 if plan.w_scale is not None:
