@@ -10,7 +10,7 @@ import torch
 import torch.autograd.forward_ad as fw
 
 from test_gpu_adamw import formula64
-from tt_thrml_b200 import Executor, make_cuda_config, workloads
+from tt_thrml_b200 import Executor, _native as nat, make_cuda_config, workloads
 
 pytestmark = pytest.mark.gpu
 
@@ -285,3 +285,28 @@ def test_weights_of_any_strides(tt, precision):
         for p, q in zip(a._plans(), b._plans()):
             assert torch.equal(p.weights_nk, q.weights_nk)
             assert p.w_scale is None or torch.equal(p.w_scale, q.w_scale)
+
+
+def test_a_learning_rate_set_in_a_capture(tt):
+    """It acts when the graph is replayed, and what is set outside acts at once, also where it is the same number."""
+    p, g = torch.zeros(4, device="cuda"), [torch.ones(4, device="cuda")]
+    opt = tt.AdamW([p], lr=0.5, betas=(0.0, 0.0), eps=1e-30, weight_decay=0.0)  # a step is -lr exactly
+
+    def stepped(run):
+        p.zero_()
+        run()
+        return -p[0].item()
+
+    assert stepped(lambda: opt.step(g)) == 0.5
+    graph = torch.cuda.CUDAGraph()
+    with nat.capturing(graph):
+        opt.lr = 0.25
+        opt.step(g)
+    assert stepped(lambda: opt.step(g)) == 0.5  # nothing was replayed yet
+    opt.lr = 0.25
+    assert stepped(lambda: opt.step(g)) == 0.25
+    opt.lr = 0.125
+    assert stepped(lambda: opt.step(g)) == 0.125
+    assert stepped(graph.replay) == 0.25 and stepped(lambda: opt.step(g)) == 0.25
+    opt.lr = 0.125
+    assert stepped(lambda: opt.step(g)) == 0.125

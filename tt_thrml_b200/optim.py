@@ -99,7 +99,7 @@ class AdamW:
                 torch.zeros(max(total, BLOCK) // BLOCK, dtype=torch.float32, device=dev) for _ in range(2)
             )
         self._ctl = torch.zeros(3, dtype=torch.int64, device=dev)  # tthrml_adamw_ctl: step, lr (float64), ticket
-        self._lr = None
+        self._lr, self._lr_captured = None, False
         self.lr = lr
         self._kinds = [(p.dtype, p.device, p.shape, p.stride()) for p in self.params]
         # tthrml_adamw_tensor rows of the parameters that have elements
@@ -125,15 +125,18 @@ class AdamW:
 
     @lr.setter
     def lr(self, value) -> None:
-        """Queued on the current stream; steps launched (or replayed) after it use the new rate."""
+        """Queued on the current stream; steps launched (or replayed) after it use the new rate.  In a capture it becomes
+        part of the graph: every replay sets the rate anew."""
         value = float(value)
         if not value >= 0.0:
             raise ValueError(f"lr must not be below 0, got {value}")
-        if value != self._lr:
-            torch = _torch()
-            with torch.cuda.device(self.device):
+        torch = _torch()
+        with torch.cuda.device(self.device):
+            # a captured setting acts when it is replayed, which the host does not see: from then on none is skipped
+            self._lr_captured = self._lr_captured or torch.cuda.is_current_stream_capturing()
+            if value != self._lr or self._lr_captured:
                 self._ctl.view(torch.float64)[1].fill_(value)
-            self._lr = value
+        self._lr = value
 
     @property
     def steps(self) -> int:
