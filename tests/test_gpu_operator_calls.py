@@ -310,3 +310,15 @@ def test_a_learning_rate_set_in_a_capture(tt):
     assert stepped(graph.replay) == 0.25 and stepped(lambda: opt.step(g)) == 0.25
     opt.lr = 0.125
     assert stepped(lambda: opt.step(g)) == 0.125
+
+
+def test_settings_that_are_fixed_cannot_be_set(tt):
+    opt = tt.AdamW([torch.ones(4, device="cuda")], betas=(0.5, 0.75), eps=1e-6, weight_decay=0.25, state_bits=8, seed=3)
+    for name, value in (("betas", (0.5, 0.75)), ("eps", 1e-6), ("weight_decay", 0.25), ("state_bits", 8), ("seed", 3)):
+        assert getattr(opt, name) == value
+        with pytest.raises(AttributeError):
+            setattr(opt, name, value)
+    opt.params.append(torch.ones(4, device="cuda"))
+    with pytest.raises(ValueError, match="made for 1"):
+        opt.step([torch.ones(4, device="cuda")] * 2)
+    assert opt.steps == 0

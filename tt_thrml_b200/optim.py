@@ -56,7 +56,8 @@ class AdamW:
     the parameter's type or float32, the parameter's shape and memory order;
     None reads every parameter's `.grad`.  16-bit parameters are rounded to
     nearest after the step.  state_bits: 32, or 8 for coded moments
-    (`seed` keys their rounding).
+    (`seed` keys their rounding).  Of the settings `lr` alone may be changed later.
+    A gradient may be its parameter's own memory, but no other parameter's.
     """
 
     def __init__(self, params, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
@@ -83,8 +84,8 @@ class AdamW:
             raise ValueError(f"betas must lie in [0, 1), got {betas!r}")
         if not eps >= 1e-30 or not weight_decay >= 0.0 or not lr >= 0.0:
             raise ValueError("eps must be at least 1e-30, lr and weight_decay not below 0")
-        self.device, self.betas, self.eps, self.weight_decay = dev, tuple(map(float, betas)), float(eps), float(weight_decay)
-        self.state_bits, self.seed = int(state_bits), int(seed) & 0xFFFFFFFFFFFFFFFF
+        self.device, self._betas, self._eps, self._weight_decay = dev, tuple(map(float, betas)), float(eps), float(weight_decay)
+        self._state_bits, self._seed = int(state_bits), int(seed) & 0xFFFFFFFFFFFFFFFF
         # segment of each parameter in the moments
         self.offsets, total = [], 0
         for p in self.params:
@@ -118,6 +119,13 @@ class AdamW:
         self._values_entry = nat.address_of("tthrml_adamw_values")
 
     # ---------------------------------------------------------------- control
+
+    # fixed when the optimizer is made: captured steps and the host module's calls hold them
+    betas = property(lambda self: self._betas)
+    eps = property(lambda self: self._eps)
+    weight_decay = property(lambda self: self._weight_decay)
+    state_bits = property(lambda self: self._state_bits)
+    seed = property(lambda self: self._seed)
 
     @property
     def lr(self) -> float:
@@ -169,6 +177,8 @@ class AdamW:
     def step(self, grads=None) -> None:
         """One step of all parameters, queued on the current stream of their device."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(self.params) != len(self._kinds):
+            raise ValueError(f"made for {len(self._kinds)} parameters, params has {len(self.params)} now")
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} parameters, {len(grads)} gradients")
         index = self.device.index
