@@ -322,3 +322,45 @@ def test_settings_that_are_fixed_cannot_be_set(tt):
     with pytest.raises(ValueError, match="made for 1"):
         opt.step([torch.ones(4, device="cuda")] * 2)
     assert opt.steps == 0
+
+
+@pytest.mark.parametrize("precision", ["bf16", "int8"])
+def test_shared_weights_of_an_executor_that_shares_a_third_ones(tt, precision):
+    """Sharing goes along chains, through captured sweeps too, and ends where an executor shares another one's."""
+    cfg, dev = make_cuda_config(dense_precision=precision), tt.open_device(device_id=0)
+    a, b, c, d = (loaded(rbm(), cfg, device=dev) for _ in range(4))
+    weights = [torch.from_numpy(workloads.gaussian_bernoulli_rbm(256, 512, seed=k, w_std=0.05).W).cuda() for k in range(4)]
+
+    def same(x, y):
+        assert all(p.weights_nk is q.weights_nk and p.w_scale is q.w_scale and p.bias is q.bias for p, q in zip(x._plans(), y._plans()))
+        states = []
+        for ex in (x, y):
+            ex.set_raw_state(start)
+            ex.prepare_rng(4)
+            ex.run_sweeps(3)
+            states.append(ex.raw_state())
+        assert np.array_equal(*states)
+
+    start = a.raw_state()
+    a.share_dense_weights(b)
+    b.update_dense_weights(weights[0])
+    same(a, b)  # their sweeps are captured now
+    b.share_dense_weights(c)
+    same(a, c)
+    c.update_dense_weights(weights[1])
+    same(a, c)
+    same(b, c)
+    b.update_dense_weights(weights[2])  # writes what all three run on
+    same(a, c)
+    a.share_dense_weights(d)
+    d.update_dense_weights(weights[3])
+    same(a, d)
+    same(b, c)
+    assert a._plans()[0].weights_nk is not b._plans()[0].weights_nk
+    b.share_dense_weights(d)  # a no longer follows b, c never did
+    same(a, b)
+    assert c._plans()[0].weights_nk is not d._plans()[0].weights_nk
+    d.share_dense_weights(a)  # a circle
+    a.share_dense_weights(a)
+    d.update_dense_weights(weights[0])
+    same(a, d)

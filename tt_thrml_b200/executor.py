@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import time
+import weakref
 from typing import Any, Sequence
 
 import numpy as np
@@ -111,6 +112,7 @@ class Executor:
         self._timing_log: list[tuple[str, float, float]] = []
         self._scratch: dict[int, Any] = {}
         self._graphs: dict[int, Any] = {}
+        self._follows, self._followers = None, weakref.WeakSet()  # share_dense_weights
         self._ctl = None  # device tthrml_run_ctl read by graph-captured kernels
         self._ctl_value = None
 
@@ -1092,7 +1094,8 @@ class Executor:
     def share_dense_weights(self, other: "Executor") -> None:
         """Runs this executor's sweeps on another one's operands (weights and biases) from now on: what
         update_dense_weights writes there holds here too.  Both need the same program shape, precision, device and
-        stream (executors made from one opened device share its stream)."""
+        stream (executors made from one opened device share its stream).  Where the other one comes to share a third
+        one's, this executor goes along."""
         mine, theirs = self._dense_plans("share_dense_weights"), other._dense_plans("share_dense_weights")
         if self._stream != other._stream:
             raise ValueError("executors on different streams cannot share their weights")
@@ -1103,10 +1106,27 @@ class Executor:
         with _torch().cuda.stream(self._stream):
             for q in theirs:
                 other._own_operands(q)  # else the other's first update would take new ones and leave this executor behind
-        for p, q in zip(mine, theirs):
+        if other is self:
+            return
+        before = self._follows() if self._follows is not None else None
+        if before is not other:
+            if before is not None:
+                before._followers.discard(self)
+            self._follows = weakref.ref(other)
+            other._followers.add(self)
+        self._adopt_operands(other)
+
+    def _adopt_operands(self, other: "Executor") -> None:
+        """Takes the operands of an executor that this one shares, and hands them on to those that share this one's."""
+        changed = False
+        for p, q in zip(self._dense_plans("share_dense_weights"), other._dense_plans("share_dense_weights")):
             if p.weights_nk is not q.weights_nk or p.bias is not q.bias:
                 p.weights_nk, p.w_scale, p.bias, p.owned = q.weights_nk, q.w_scale, q.bias, True
-                self._graphs.clear()
+                changed = True
+        if changed:
+            self._graphs.clear()
+            for follower in list(self._followers):
+                follower._adopt_operands(self)
 
     def _dense_phases(self, scale: float) -> list:
         """The current states as terms of pair moments: (x, x pitch, y, y pitch, scale, x scale, y scale), 16-bit
