@@ -11,6 +11,7 @@ import torch.autograd.forward_ad as fw
 
 from test_gpu_adamw import formula64
 from tt_thrml_b200 import Executor, _native as nat, make_cuda_config, workloads
+from tt_thrml_b200.core import Family
 
 pytestmark = pytest.mark.gpu
 
@@ -364,3 +365,27 @@ def test_shared_weights_of_an_executor_that_shares_a_third_ones(tt, precision):
     a.share_dense_weights(a)
     d.update_dense_weights(weights[0])
     same(a, d)
+
+
+def test_host_batches_of_several_types_in_turn(tt):
+    """Bools, floats and halves one after the other without waiting, each the data states of its step."""
+    program = workloads.DenseBipartiteProgram(rbm().W, rbm().b_v, rbm().b_h, visible_family=Family.SPIN)
+    g = torch.Generator().manual_seed(6)
+    spins = [torch.randint(0, 2, (128, 256), generator=g).bool() for _ in range(9)]
+    kinds = [torch.bool, F32, F32, torch.float16, torch.bool, F32, F32, F32, torch.float64]
+
+    def run(to):
+        learner = tt.DenseLearner(program, n_data=128, n_chains=128, config=make_cuda_config(dense_precision="int8"))
+        gradients = []
+        for s, kind in zip(spins, kinds):
+            batch = s.clone() if kind == torch.bool else (s.to(kind) * 2 - 1)
+            batch = to(batch)
+            gradients.append([t.clone() for t in learner.step(batch)])
+            if batch.device.type == "cpu":
+                batch.zero_()
+        return learner, gradients
+
+    host, wanted = run(lambda t: t.pin_memory()), run(lambda t: t.cuda())
+    for a, b in zip(host[1], wanted[1]):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(host[0].weights, wanted[0].weights)

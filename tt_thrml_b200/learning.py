@@ -85,10 +85,11 @@ class DenseLearner:
     moment differences, steps the masters and rounds them into both samplers'
     operands.  It returns the gradient of minus the mean log likelihood as the
     triple that was stepped with (overwritten by the next step).  It does not wait
-    for the device's work; of a batch in host memory (complete when step is called)
-    it waits for the copy, which runs beside that work, so the caller may fill the
-    batch anew at once.  check() raises if a kernel of the steps so far gave up a
-    wait: the masters are not to be relied on then.
+    for its own work.  A batch in host memory (complete when step is called) has been
+    read when step returns, so the caller may fill it anew at once: the copy runs
+    beside the device's work, and the host stays within two steps of it.
+    check() raises if a kernel of the steps so far gave up a wait: the masters are
+    not to be relied on then.
     """
 
     def __init__(self, program, *, n_data, n_chains, config=None, device=None, sweeps=1, lr=1e-3, betas=(0.9, 0.999),
@@ -130,6 +131,7 @@ class DenseLearner:
             # one stream of draws for the whole run, another one for each executor
             ex._prepare_rng_for_n_sweeps((int(seed) << 1) + k, 2**31 - 1)
         self._copies = torch.cuda.Stream(device=dev)
+        self._uploads = [(None, torch.cuda.Event()) for _ in range(2)]
         self._hidden_group = next(gr for gr in self.data.compiled.sampling_groups if tuple(gr.block_indices) == (1,))
 
     def step(self, batch):
@@ -145,18 +147,18 @@ class DenseLearner:
         data, model = self.data, self.model
         n = data.n_chains
         current = torch.cuda.current_stream(data._tdev)
-        if batch.device.type == "cpu":
-            # on a stream of its own: behind the sweeps of earlier steps the copy would still read the batch long after
-            # step has returned
-            with torch.cuda.stream(self._copies):
-                batch = batch.to(data._tdev)
+        upload = self._upload(batch) if batch.device.type == "cpu" else None
+        if upload is not None:
+            batch = upload[0]
         data.stream.wait_stream(current)
         with torch.cuda.stream(data.stream):
             values = batch.to(data._tdev, non_blocking=True)
             if self._visible_family == Family.SPIN:
                 values = torch.where(values > 0, 1.0, -1.0)
             data._dense_write_block(0, values)
-            if batch.device == data._tdev:
+            if upload is not None:
+                upload[1].record(data.stream)
+            elif batch.device == data._tdev:
                 batch.record_stream(data.stream)
         data._check_ready()
         data._run_sampling_group(self._hidden_group, data._sweep_counter)
@@ -167,6 +169,22 @@ class DenseLearner:
         data.update_dense_weights(self.weights, self.visible_bias, self.hidden_bias)
         model.share_dense_weights(data)
         return self.gradient
+
+    def _upload(self, batch):
+        """(device copy, event to record when it has been read) of a host batch, on a stream of its own: behind the sweeps
+        of earlier steps the copy would still read the batch long after step has returned.  Two buffers in turn keep the
+        host within two steps of the device."""
+        torch = _torch()
+        self._uploads.reverse()
+        buffer, read = self._uploads[0]
+        with torch.cuda.stream(self._copies):
+            self._copies.wait_event(read)
+            if buffer is None or buffer.dtype != batch.dtype:
+                buffer = torch.empty(batch.shape, dtype=batch.dtype, device=self.data._tdev)
+                buffer.record_stream(self.data.stream)
+                self._uploads[0] = (buffer, read)
+            buffer.copy_(batch)  # waits for the copy
+        return self._uploads[0]
 
     def check(self) -> None:
         """Raises if a kernel of the steps so far gave up an in-kernel wait.  Synchronises."""
