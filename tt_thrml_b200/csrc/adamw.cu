@@ -452,7 +452,7 @@ int launch_adamw(const tthrml_adamw_tensor* t, int32_t n, AdamArgs a, int sms, c
   tab.first_chunk[n] = (int32_t)chunks;
   a.n_tensors = n;
   // Two chunks a CTA, but no fewer CTAs than run at once: 33.6 M float32 weights took 142 us so, 149 with one chunk a CTA, 144
-  // and 147 with three and six, 155 with 8 CTAs an SM; 600 tensors of 4.6 M bfloat16 weights 22.3, 23.0, 27.8 and 23.5, 21.9.
+  // and 147 with three and six, 155 with 8 CTAs an SM; 600 tensors of 3.34 M bfloat16 weights 22.3, 23.0, 27.8 and 23.5, 21.9.
   const int64_t least = 4 * (int64_t)sms < chunks ? 4 * (int64_t)sms : chunks, want = (chunks + 1) / 2;
   const int grid = (int)(want > least ? want : least);
   k_adamw<BITS, T, ROOTS><<<grid, kAdamThreads, 0, st>>>(tab, a);

@@ -4,8 +4,9 @@
 // Bound: the weights are read once (N K bytes); there is nothing to reuse them for, so the tensor cores are left
 // alone.  Every CTA quantises the rows itself into shared memory (M K elements from L2; a launch of its own would cost
 // more than that), while the first weight vectors are already on their way.  The multiplications are dp4a (exact in int32
-// for K <= 131071), whose rate is what ends this form: one and two rows take 3.6 and 3.8 us of 1000 x 3000 weights against 6.4
-// on the tensor cores, 6.9 and 8.7 of 4096 x 8192 against 9.3, 8.1 and 10.8 of 8192 x 4096 against 9.3.
+// for K <= 131071), whose rate is what ends this form.  One and two rows, and three (on the tensor cores) beside them, replayed
+// from a graph: K = 1000, N = 3000 in 3.3, 3.7 and 6.4 us; 4096, 8192 in 7.0, 8.8 and 9.4 with the weights in L2, 9.4, 10.4
+// and 11.9 with weights that take turns; 8192, 4096 in 8.0, 10.7 and 9.2, or 10.3, 12.2 and 11.8.
 #include "int8_common.cuh"
 
 namespace tthrml {

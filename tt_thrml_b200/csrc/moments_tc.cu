@@ -433,8 +433,8 @@ __device__ __forceinline__ float4 added(const float4& a, const float4& b) {
 }
 // Stores (or adds) a warp's turned 32 x 32 floats to the rows at o, V at a time: each access of the warp covers whole lines of
 // one row (float) or four (float4), where each lane storing its own row touched 32 lines (4096 x 8192, 256 chains: 76 us, now
-// 50).  What is added to is read a batch ahead of its stores, which would otherwise order every read behind the store before
-// it (adding to 4096 x 8192 floats, 256 chains: 192 us, now 105; to 4096 x 8191, 1024 chains: 409 us, now 148).
+// 39).  What is added to is read a batch ahead of its stores, which would otherwise order every read behind the store before
+// it (adding to 4096 x 8192 floats, 256 chains: 192 us, now 91; to 4096 x 8191, 1024 chains: 409 us, now 151).
 template <typename V>
 __device__ __forceinline__ void put_rows(const unsigned char* turn, float* o, int64_t ld, int rows, int live, bool add) {
   constexpr int kPerRow = 128 / (int)sizeof(V), kRows = 32 / kPerRow, kBatch = sizeof(V) == 16 ? 4 : 8;
@@ -721,9 +721,12 @@ int resident_tiles(const int** out) {
 
 // Estimated clocks of the tiles on clusters of S CTAs: per wave the blocks of a CTA's share of the chains (block_clocks), at
 // least 360 clocks each to issue, the tile's store, and for S > 1 a barrier and the partial tiles.  The constants are those
-// of the 8-bit tiles; over 28 sizes with every (BN, S) and the pair kernel measured the choice is 0.4 % behind the fastest on
-// average, 7 % at most (777 x 2000 x 1523 chains: (128, 1) 12.9 us of 12.9 to 87; 512 x 1024 x 9216: (128, 4) 17.1 of 17.1 to
-// 51; 1500 x 1500 x 5000: (256, 2) 26.8 of 26.8 to 150).
+// of the 8-bit tiles; over 28 sizes with every (BN, S) and the pair kernel measured, without unit sums and on rows that start
+// on 16 bytes, the choice is 0.4 % behind the fastest on average, 7 % at most (777 x 2000 x 1523 chains: (128, 1) 12.1 us of
+// 12.1 to 87; 512 x 1024 x 9216: (128, 4) 16.2 of 16.2 to 51; 1500 x 1500 x 5000: (256, 2) 26.0 of 26.0 to 150).  The unit
+// sums are not counted.  Where the tiles leave a few SMs over, these take all strips and end long after the tiles: 2304 x
+// 2048 x 9216 chains 62 us, with sums 760; 1500 x 1500 x 5000 157; 512 x 1024 x 9216 44; 4096 x 8192 x 9216 (no SM is left
+// over) 444 and 468.
 template <int BN>
 int consider(const MomentArgs& a, int64_t& best, int& bn, int& split) {
   const int* resident;
