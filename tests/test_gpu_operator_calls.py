@@ -389,3 +389,30 @@ def test_host_batches_of_several_types_in_turn(tt):
     for a, b in zip(host[1], wanted[1]):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert torch.equal(host[0].weights, wanted[0].weights)
+
+
+@pytest.mark.parametrize("chains", [640, 2176])
+def test_dense_moments_of_many_chains(tt, chains):
+    """One MMA adds 16 products to its accumulator within 17 steps of 2^-23 of the sum of magnitudes; at most 64 of them (1024
+    chains) follow each other before the sum moves to a float32 register, with a rounding for each further 1024 chains
+    and for the parts of a split (8 at most); a value in three bf16 pieces adds its phases (6) and 2^-24 of itself."""
+    ex = loaded(rbm(), make_cuda_config(dense_precision="fp32"), chains)
+    state = ex.raw_state().astype(np.float64)
+    v, h = state[:256], state[256:]
+    got = ex.dense_moments(0.5)
+    steps = 17 * min(64, -(-chains // 16)) + -(-chains // 1024) + 8 + 6 + 1
+    for g, want, mags in zip(got, (v @ h.T, v.sum(1), h.sum(1)), (np.abs(v) @ np.abs(h).T, np.abs(v).sum(1), np.abs(h).sum(1))):
+        # (the unit sums are float32 additions, half a step each: at most a sixteenth of the chains one after the other)
+        assert (np.abs(g.double().cpu().numpy() - 0.5 * want) <= 0.5 * steps * 2.0**-23 * mags).all()
+
+
+def test_second_moments_of_one_block_never_fall_to_zero(tt):
+    """Gradients over 20 orders of magnitude, v over 40, within one block of 256 that shares a scale."""
+    g = torch.logspace(-10, 10, 256, device="cuda")
+    p = torch.zeros(256, device="cuda")
+    opt = tt.AdamW([p], state_bits=8, lr=0.1)
+    for _ in range(20):
+        opt.step([g])
+    m, v = opt.state_values(flat=True)
+    assert (v > 0).all() and torch.isfinite(v).all() and torch.isfinite(m).all()
+    assert torch.isfinite(p).all()
