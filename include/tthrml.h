@@ -724,6 +724,59 @@ int tthrml_pair_moments_packed(const tthrml_pack_matrix* matrices_host, int32_t 
                                float* x_sum_dev, float* y_sum_dev, int32_t accumulate,
                                int32_t* error_dev, void* stream);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Softmax cross entropy of categories read out of a block's units.
+ *     l[t][v] = sum_k x[t][k] w[v][k] + bias[v],  z[t] = log sum_v exp l[t][v],
+ *     loss[t] = z[t] - l[t][y[t]],
+ * the logits computed in pieces and never held as a whole.
+ * ---------------------------------------------------------------------------
+ */
+#define TTHRML_XENT_MAX_ROWS (1 << 24)
+#define TTHRML_XENT_MAX_CATEGORIES (1 << 24)
+#define TTHRML_XENT_MAX_COLS (1 << 20)
+
+/* Both matrices 16-byte aligned, pitches multiples of 8 elements >= cols. */
+typedef struct tthrml_xent {
+  const void* x;        /* [rows][x_ld], TTHRML_DT_BF16 or _F16 */
+  const void* w;        /* [categories][w_ld], the same type */
+  const void* targets;  /* [rows] int64 (wide_targets) or int32 */
+  const float* bias;    /* [categories] or NULL; -inf: a category that cannot occur */
+  int64_t x_ld, w_ld, rows, categories, cols;
+  int64_t ignored;      /* rows with this target do not count: loss 0, no gradient */
+  int32_t dtype, wide_targets;
+} tthrml_xent;
+
+/*
+ * log2_z: [rows], z / ln 2, which the backward pass takes.  row_loss: [rows].
+ * A row in which no category is possible has loss inf and no gradient; a
+ * target outside 0 .. categories-1 that is not `ignored` has loss NaN (and NaN
+ * gradients).  reduction 0: rows only; 1: reduced[0] is the mean over the rows
+ * that count (0 if there are none), 2: their sum; reduced[1] is 1 / their
+ * number or 1, the second factor of the backward pass.  The same every time.
+ * workspace: tthrml_xent_forward_workspace(rows, categories) bytes (of the
+ * current device; negative: an error), 16-byte aligned, free again once the
+ * work on `stream` is done.
+ */
+int tthrml_xent_forward(const tthrml_xent* problem_host, float* log2_z_dev, float* row_loss_dev,
+                        float* reduced_dev, int32_t reduction, void* workspace_dev,
+                        int64_t workspace_bytes, int32_t* error_dev, void* stream);
+int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories);
+
+/*
+ * dx [rows][dx_ld], dw [categories][dw_ld] (grad_dtype: float32, bfloat16 or
+ * float16) and db [categories], each NULL or written, of
+ * sum_t weight[t] loss[t].  weight: grad[0] * (inv_count ? *inv_count : 1), or,
+ * grad_per_row, grad[t].
+ */
+int tthrml_xent_backward(const tthrml_xent* problem_host, const float* log2_z_dev,
+                         const float* grad_dev, int32_t grad_per_row, const float* inv_count_dev,
+                         void* dx_dev, int64_t dx_ld, void* dw_dev, int64_t dw_ld,
+                         int32_t grad_dtype, float* db_dev, void* workspace_dev,
+                         int64_t workspace_bytes, int32_t* error_dev, void* stream);
+int64_t tthrml_xent_backward_workspace(int64_t rows, int64_t categories, int64_t cols, int32_t dx,
+                                       int32_t dw, int32_t db);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

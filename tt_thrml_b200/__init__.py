@@ -35,6 +35,7 @@ from .core import (
 )
 from .executor import Executor, make_executor
 from .learning import DenseLearner, dense_moments
+from .losses import softmax_cross_entropy
 from .mesh import MeshExecutor, make_mesh_executor, mesh_barrier, mesh_device_ids, mesh_size
 from .moments import pair_moments
 from .optim import AdamW
@@ -105,4 +106,5 @@ __all__ = [
     "dense_moments",
     "DenseLearner",
     "AdamW",
+    "softmax_cross_entropy",
 ]

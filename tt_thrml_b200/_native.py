@@ -24,6 +24,8 @@ DT_F32, DT_BF16, DT_F16, DT_I8 = 0, 1, 2, 3
 INT8_MAX_COLS = 131071
 INT8_FEW_BYTES = 163840
 MAX_PHASES = 6
+XENT_MAX_ROWS = XENT_MAX_CATEGORIES = 1 << 24
+XENT_MAX_COLS = 1 << 20
 MAX_CAT_SOURCES = 4
 MAX_CATEGORIES = 64
 
@@ -122,6 +124,14 @@ class MomentPhase(ctypes.Structure):
         ("y_scale", ctypes.c_float),
         ("reserved", ctypes.c_float),
     ]
+
+
+class Xent(ctypes.Structure):
+    """tthrml_xent (include/tthrml.h)."""
+
+    _fields_ = [(name, c_vp) for name in ("x", "w", "targets", "bias")] + [
+        (name, c_i64) for name in ("x_ld", "w_ld", "rows", "categories", "cols", "ignored")
+    ] + [("dtype", c_i32), ("wide_targets", c_i32)]
 
 
 class GroupDesc(ctypes.Structure):
@@ -255,6 +265,13 @@ _SIGNATURES = {
         [c_vp, c_i32, c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp],
     ),
     "tthrml_pair_moments": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "tthrml_xent_forward": (c_i32, [ctypes.POINTER(Xent), c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]),
+    "tthrml_xent_forward_workspace": (c_i64, [c_i64, c_i64]),
+    "tthrml_xent_backward": (
+        c_i32,
+        [ctypes.POINTER(Xent), c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp],
+    ),
+    "tthrml_xent_backward_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i32, c_i32, c_i32]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),
     "tthrml_last_error": (ctypes.c_char_p, []),

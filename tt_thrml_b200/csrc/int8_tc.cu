@@ -261,7 +261,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // CTA-pair kernel
 // ---------------------------------------------------------------------------
 constexpr int kPairStages = 6, kPairStage = 2 * 128 * 128, kPairThreads = 320, kPairWarps = 8;
-constexpr int kTurnPitch = 80;  // bytes per row of a warp's staged 32 x 64 bytes: rows 20 banks apart
 constexpr int kScaleWords = 2 * 512;  // scales and biases of a tile's units, two tiles
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kScaleWords * 4 + kPairWarps * 32 * kTurnPitch;
 enum : int { kStoreFields = 0, kDrawSpins = 1, kDrawGaussians = 2 };
@@ -292,39 +291,6 @@ __device__ __forceinline__ void scale_chunk(float sx, const float* sw, float (&v
     v[4 * q + 2] = __fmul_rn((float)__float_as_int(v[4 * q + 2]), __fmul_rn(sx, w.z));
     v[4 * q + 3] = __fmul_rn((float)__float_as_int(v[4 * q + 3]), __fmul_rn(sx, w.w));
   }
-}
-
-// Stores 32 staged rows of `bytes` each (a power of two up to 64) from column byte `at` of the output rows m0 .. m0 + 31, V at
-// a time: a warp's store covers whole pieces of a few rows, where a store of every lane's own row would touch 32 lines.
-template <typename V>
-__device__ __forceinline__ void drain(const unsigned char* turn, int bytes, unsigned char* out, int64_t pitch, int64_t at,
-                                      int m0, int M, int live_bytes) {
-  const int lane = threadIdx.x & 31, per_row = bytes / (int)sizeof(V), rows = 32 / per_row;
-  const int k = (lane % per_row) * (int)sizeof(V);
-  if (k >= live_bytes) return;
-#pragma unroll 4
-  for (int r = lane / per_row; r < 32 && m0 + r < M; r += rows)
-    *reinterpret_cast<V*>(out + (int64_t)(m0 + r) * pitch + at + k) = *reinterpret_cast<const V*>(turn + r * kTurnPitch + k);
-}
-// words: this lane's row, N16 pieces of 16 bytes.  Every lane calls it; the rows are m0 .. m0 + 31, `align` their alignment.
-template <int N16>
-__device__ __forceinline__ void store_rows(const uint4 (&words)[N16], unsigned char* turn, unsigned char* out, int64_t pitch,
-                                           int64_t at, int m0, int M, int live_bytes, int align) {
-  const int lane = threadIdx.x & 31;
-  uint4* mine = reinterpret_cast<uint4*>(turn + lane * kTurnPitch);
-#pragma unroll
-  for (int q = 0; q < N16; ++q) mine[q] = words[q];
-  __syncwarp();
-  if (live_bytes < 16 * N16) align = align < 4 ? align : (live_bytes % 4 == 0 ? 4 : 2);
-  if (align >= 16)
-    drain<uint4>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
-  else if (align >= 8)
-    drain<uint2>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
-  else if (align >= 4)
-    drain<uint32_t>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
-  else
-    drain<uint16_t>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
-  __syncwarp();
 }
 
 // Adds the biases to one 32-column chunk of 32 rows (lane = row m) and stores it.

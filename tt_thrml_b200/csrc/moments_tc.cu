@@ -64,12 +64,6 @@ struct MomentShape {
   static_assert(128 * kPitch * 4 <= kStages * kStage, "the staged tile reuses the operand stages");
 };
 
-// Shared-memory descriptor of an MN-major tile in the 128-byte swizzle: boxes of 64 units x 64 chains (8 KiB), so
-// groups of 64 units are 8192 bytes apart (leading offset) and groups of 8 chains 1024 bytes (stride offset).
-__device__ __forceinline__ uint64_t umma_desc_mn128(const void* tile) {
-  const uint64_t addr = (uint64_t)(smem_u32(tile) >> 4) & 0x3FFFull;
-  return addr | (512ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
 // D float32, A and B bfloat16 (or float16), both MN-major.
 __device__ __forceinline__ uint32_t idesc_moments(int n, bool f16) {
   const uint32_t t = f16 ? 0u : 1u;
@@ -464,15 +458,6 @@ __device__ __forceinline__ void put_rows(const unsigned char* turn, float* o, in
   }
 }
 
-__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u),
-      "r"(0u), "r"(0u));
-}
 // Tile t -> (m, n) block: `group` row blocks at a time, row-fastest, so that the tiles in flight form a rectangle and
 // share their operands' panels in L2.
 __device__ __forceinline__ void pair_tile(const MomentArgs& a, int t, int& mb, int& nb) {

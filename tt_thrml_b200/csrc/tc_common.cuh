@@ -153,6 +153,56 @@ __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(smem_u32(bar) & kPeerMask) : "memory");
 }
 
+// Shared-memory descriptor of an MN-major tile in the 128-byte swizzle: boxes of 64 units x 64 chains (8 KiB), so
+// groups of 64 units are 8192 bytes apart (leading offset) and groups of 8 chains 1024 bytes (stride offset).
+__device__ __forceinline__ uint64_t umma_desc_mn128(const void* tile) {
+  const uint64_t addr = (uint64_t)(smem_u32(tile) >> 4) & 0x3FFFull;
+  return addr | (512ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u),
+      "r"(0u), "r"(0u));
+}
+
+constexpr int kTurnPitch = 80;  // bytes per row of a warp's staged 32 x 64 bytes: rows 20 banks apart
+// Stores 32 staged rows of `bytes` each (a power of two up to 64) from column byte `at` of the output rows m0 .. m0 + 31, V at
+// a time: a warp's store covers whole pieces of a few rows, where a store of every lane's own row would touch 32 lines.
+template <typename V>
+__device__ __forceinline__ void drain(const unsigned char* turn, int bytes, unsigned char* out, int64_t pitch, int64_t at,
+                                      int m0, int M, int live_bytes) {
+  const int lane = threadIdx.x & 31, per_row = bytes / (int)sizeof(V), rows = 32 / per_row;
+  const int k = (lane % per_row) * (int)sizeof(V);
+  if (k >= live_bytes) return;
+#pragma unroll 4
+  for (int r = lane / per_row; r < 32 && m0 + r < M; r += rows)
+    *reinterpret_cast<V*>(out + (int64_t)(m0 + r) * pitch + at + k) = *reinterpret_cast<const V*>(turn + r * kTurnPitch + k);
+}
+// words: this lane's row, N16 pieces of 16 bytes.  Every lane calls it; the rows are m0 .. m0 + 31, `align` their alignment.
+template <int N16>
+__device__ __forceinline__ void store_rows(const uint4 (&words)[N16], unsigned char* turn, unsigned char* out, int64_t pitch,
+                                           int64_t at, int m0, int M, int live_bytes, int align) {
+  const int lane = threadIdx.x & 31;
+  uint4* mine = reinterpret_cast<uint4*>(turn + lane * kTurnPitch);
+#pragma unroll
+  for (int q = 0; q < N16; ++q) mine[q] = words[q];
+  __syncwarp();
+  if (live_bytes < 16 * N16) align = align < 4 ? align : (live_bytes % 4 == 0 ? 4 : 2);
+  if (align >= 16)
+    drain<uint4>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  else if (align >= 8)
+    drain<uint2>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  else if (align >= 4)
+    drain<uint32_t>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  else
+    drain<uint16_t>(turn, 16 * N16, out, pitch, at, m0, M, live_bytes);
+  __syncwarp();
+}
+
 // --- host side --------------------------------------------------------------
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -1,0 +1,950 @@
+// Softmax cross entropy over a large set of categories on the tensor cores, in pieces, without keeping the logits:
+//     l[t][v] = sum_k x[t][k] w[v][k] + b[v],   z[t] = log sum_v exp l[t][v],   loss[t] = z[t] - l[t][y[t]],
+// and, with r[t] the weight of row t in what is differentiated,
+//     g[t][v] = r[t] (exp(l[t][v] - z[t]) - [v == y[t]]),   dx = g w,   dw = g^T x,   db = sum_t g.
+//
+// The forward pass is one product whose epilogue folds each tile of logits into a running maximum and sum per row (a row
+// per thread; log2 domain), so only a pair of floats per row and unit of work leaves the SM; k_xent_loss joins them.  The
+// backward pass takes the categories in pieces of at most kPieceBytes of g: the logits of a piece are computed again and
+// turned into g (16 bits), which two further products reduce to this piece's rows of dw and to sums of dx in float32.
+//
+// One kernel serves the four products: persistent clusters of two CTAs walk 256 x BN tiles (tcgen05 cta_group::2, two
+// TMEM accumulators, six stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
+// transposed.  Warp 0 loads (TMA), warp 1 of the even CTA multiplies, warps 2-9 run the epilogue of a tile under the main
+// loop of the next one.
+//
+// g is rounded to the operands' 16 bits: by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
+// themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
+// sums, z, losses and the sums of db are float32; dx and dw accumulate in float32.
+#include "int8_common.cuh"
+#include "tc_common.cuh"
+
+namespace tthrml {
+namespace {
+
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr int kThreads = 320, kEpilogueWarps = 8;
+constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
+enum : int { kPartials = 0, kGradient = 1, kProduct = 2 };
+
+struct RowTargets {
+  const void* y;  // [rows] int64 or int32
+  int32_t wide;
+  int64_t ignored;
+};
+__device__ __forceinline__ int64_t target_of(const RowTargets& t, int64_t row) {
+  return t.wide ? __ldg(reinterpret_cast<const long long*>(t.y) + row) : (int64_t)__ldg(reinterpret_cast<const int*>(t.y) + row);
+}
+
+struct XentArgs {
+  int32_t M, N;       // the product's rows and columns
+  int32_t num_k;      // 64-wide blocks of its sum
+  int32_t f16;
+  int32_t units, segments, seg, splits, group;  // units of work: `seg` tiles along N of one row of tiles and one share of K
+  // epilogues of logits: N categories from `first` on
+  const float* bias;  // of the first category, or NULL
+  int64_t first, categories;  // of this piece, and of all
+  RowTargets targets;
+  // kPartials
+  float2* part;       // [M][slots] (maximum, sum) in the log2 domain
+  int32_t slots;
+  float* target_logit;  // [M]
+  uint32_t* counter;    // zeroed for k_xent_loss
+  // kGradient
+  const float* log2_z;    // [M]
+  const float* row_grad;  // [M] weights, or NULL: ones
+  const float* top_grad;  // what they are divided by
+  float unit;             // g is held times this
+  unsigned char* g;       // [M][g_ld] 16-bit
+  int64_t g_ld;
+  float* bias_part;       // [ceil(M / 32)][bias_ld] sums over 32 rows, or NULL
+  int64_t bias_ld;
+  // kProduct, scaled: out = sums * factor[0] * factor[1] / unit; else planes of plain float32 sums, a plane per split, whose
+  // rows have room for whole tiles of 32 columns
+  void* out;
+  int64_t out_ld, plane;  // elements from row to row, and from plane to plane
+  int32_t out_dtype, align, accumulate, scaled;
+  const float* factor[2];
+  int* error;
+};
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float factor_of(const float* const (&f)[2]) {
+  return (f[0] ? __ldg(f[0]) : 1.0f) * (f[1] ? __ldg(f[1]) : 1.0f);
+}
+// (m, s) stands for s 2^m; an empty sum has m = -inf and s = 0.  A NaN in s stays.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+  s = s * exp2_fast(m - base) + s2 * exp2_fast(m2 - base);
+  m = top;
+}
+
+template <int BN>
+struct XentShape {
+  static constexpr int kA = 128 * 64 * 2, kB = BN / 2 * 64 * 2, kStage = kA + kB;
+  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kBarriers = 256;
+  static constexpr int kSmem = 1024 + kStages * kStage + kBarriers + 2 * 256 * 4 /*biases*/ + kEpilogueWarps * 32 * kTurnPitch;
+};
+
+// Unit u -> its split, row of tiles and segment: splits slowest, `group` rows of tiles at a time.
+__device__ __forceinline__ void unit_at(const XentArgs& a, int u, int& split, int& mb, int& sg) {
+  const int m_blocks = (a.M + 255) / 256, all = m_blocks * a.segments;
+  split = u / all;
+  const int t = u - split * all, per = a.group * a.segments, g = t / per, w = t - g * per;
+  const int rows = min(a.group, m_blocks - g * a.group);
+  mb = g * a.group + w % rows;
+  sg = w / rows;
+}
+
+// Sums over the warp's 32 lanes of 32 values each: lane j returns that of value j.
+__device__ __forceinline__ float column_sums(float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int w = 16; w >= 1; w >>= 1) {
+    const bool high = (lane & w) != 0;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float keep = high ? v[i + w] : v[i], give = high ? v[i] : v[i + w];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+    }
+  }
+  return v[0];
+}
+
+// 32 values of each of a warp's rows m0 + lane, from column n on, to 16-bit or float32 rows.
+__device__ __forceinline__ void store_values(const float (&v)[32], int32_t dtype, unsigned char* turn, unsigned char* out,
+                                             int64_t ld, int64_t n, int m0, int M, int live, int align) {
+  if (dtype == TTHRML_DT_F32) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        w[q] = make_uint4(__float_as_uint(v[16 * half + 4 * q]), __float_as_uint(v[16 * half + 4 * q + 1]),
+                          __float_as_uint(v[16 * half + 4 * q + 2]), __float_as_uint(v[16 * half + 4 * q + 3]));
+      const int left = min(16, live - 16 * half);
+      if (left > 0) store_rows<4>(w, turn, out, ld * 4, 4 * (n + 16 * half), m0, M, 4 * left, align);
+    }
+    return;
+  }
+  uint4 w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = v[8 * q + 2 * j], hi = v[8 * q + 2 * j + 1];
+      if (dtype == TTHRML_DT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        p[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        p[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    w[q] = make_uint4(p[0], p[1], p[2], p[3]);
+  }
+  store_rows<4>(w, turn, out, ld * 2, 2 * n, m0, M, 2 * live, align);
+}
+
+template <int EPI, bool A_MN, bool B_MN, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_xent(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+           const __grid_constant__ XentArgs a) {
+  using S = XentShape<BN>;
+  static_assert(!B_MN || BN == 256, "MN-major halves of B are whole boxes of 64");
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStage);
+  uint64_t* empty = full + S::kStages;
+  uint64_t* acc_full = empty + S::kStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;       // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* biases = reinterpret_cast<float*>(tiles + S::kStages * S::kStage + S::kBarriers);  // [2][256]
+  unsigned char* turns = reinterpret_cast<unsigned char*>(biases + 2 * 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int n_blocks = (a.N + BN - 1) / BN;
+  const int first = (int)cluster_id_x(), step = (int)n_clusters_x();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kEpilogueWarps);  // every epilogue warp of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers exist before either signals the other
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  wait_for_previous_kernel();
+  if (EPI == kPartials && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0u;
+  int last_it[2] = {-1, -1};
+
+  if (warp == 0) {  // producer (both CTAs): this CTA's halves of the A and B slices
+    const bool one = elect_one();
+    int64_t issued = 0;
+    bool failed = false;
+    for (int u = first; u < a.units && !failed; u += step) {
+      int split, mb, sg;
+      unit_at(a, u, split, mb, sg);
+      const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
+      const int m0 = mb * 256 + (int)rank * 128;
+      for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb) {
+        const int n0 = nb * BN + (int)rank * (BN / 2);
+        for (int kb = k_first; kb < k_last; ++kb) {
+          const int s = (int)(issued % S::kStages);
+          if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
+            if (one) atomicExch(a.error, kErrEmptyWait);
+            failed = true;
+            break;
+          }
+          if (one) {
+            if (leader) mbar_expect_tx(&full[s], 2 * S::kStage);  // the stage's bytes of both CTAs
+            unsigned char* st = tiles + s * S::kStage;
+            const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
+            if (A_MN) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) tma_load_2d_pair(st + i * 8192, &map_a, bar, m0 + 64 * i, kb * 64);
+            } else {
+              tma_load_2d_pair(st, &map_a, bar, kb * 64, m0);
+            }
+            if (B_MN) {
+#pragma unroll
+              for (int i = 0; i < BN / 128; ++i)
+                tma_load_2d_pair(st + S::kA + i * 8192, &map_b, bar, n0 + 64 * i, kb * 64);
+            } else {
+              tma_load_2d_pair(st + S::kA, &map_b, bar, kb * 64, n0);
+            }
+          }
+          __syncwarp();
+          ++issued;
+        }
+      }
+    }
+    // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
+    for (int64_t j = issued > S::kStages ? issued - S::kStages : 0; j < issued; ++j)
+      if (!mbar_wait_all(&empty[j % S::kStages], (uint32_t)(j / S::kStages) & 1u) && one) atomicExch(a.error, kErrEmptyWait);
+  } else if (warp == 1) {
+    if (leader) {  // MMA issue: the leader only
+      const bool one = elect_one();
+      const uint32_t type = a.f16 ? 0u : 1u;
+      const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                             ((uint32_t)(BN >> 3) << 17) | (16u << 24);  // D float32, M = 256
+      int64_t used = 0;
+      int it = 0;
+      bool failed = false;
+      for (int u = first; u < a.units && !failed; u += step) {
+        int split, mb, sg;
+        unit_at(a, u, split, mb, sg);
+        const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
+        for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb, ++it) {
+          const int b = it & 1;
+          if (!mbar_wait_all(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
+            if (one) atomicExch(a.error, kErrAccWait);
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(b * 256);
+          for (int kb = k_first; kb < k_last; ++kb) {
+            const int s = (int)(used % S::kStages);
+            if (!mbar_wait_all(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
+              if (one) atomicExch(a.error, kErrFullWait);
+              failed = true;
+              break;
+            }
+            tc_fence_after();
+            const unsigned char* st = tiles + s * S::kStage;
+            const uint64_t ad = A_MN ? umma_desc_mn128(st) : umma_desc_sw128(st);
+            const uint64_t bd = B_MN ? umma_desc_mn128(st + S::kA) : umma_desc_sw128(st + S::kA);
+            if (one) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)  // 16 of K per MMA: 32 bytes of each row, or two groups of eight rows
+                umma_f16_pair(d, ad + (A_MN ? 128ull : 2ull) * kk, bd + (B_MN ? 128ull : 2ull) * kk, idesc,
+                              (kb > k_first || kk > 0) ? 1u : 0u);
+              umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+            }
+            __syncwarp();
+            ++used;
+          }
+          if (one) umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
+          __syncwarp();
+          last_it[b] = it;
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* turn = turns + (warp - 2) * 32 * kTurnPitch;
+    int it = 0;
+    bool failed = false;
+    for (int u = first; u < a.units; u += step) {
+      int split, mb, sg;
+      unit_at(a, u, split, mb, sg);
+      const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane;
+      float top = -INFINITY, sum = 0.0f;  // kPartials: sum 2^top
+      int64_t y = -1;                     // column of the row's target
+      float weight = 0.0f, log2_z = 0.0f, factor = 1.0f;
+      if (EPI != kProduct && m < a.M) {
+        const int64_t t = target_of(a.targets, m);
+        y = t - a.first;
+        if (EPI == kGradient) {
+          log2_z = __ldg(a.log2_z + m);
+          weight = a.unit;
+          if (a.row_grad) {
+            const float most = __ldg(a.top_grad);
+            weight = most > 0.0f ? weight * (__ldg(a.row_grad + m) / most) : 0.0f;
+          }
+          if (t < 0 || t >= a.categories) weight = __uint_as_float(0x7FC00000u);
+          if (log2_z == -INFINITY || t == a.targets.ignored) weight = 0.0f;
+        }
+      }
+      if (EPI == kProduct && a.scaled) factor = factor_of(a.factor) / a.unit;
+      for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb, ++it) {
+        const int b = it & 1;
+        float* bias = biases + b * 256;
+        if (EPI != kProduct && a.bias) {  // two buffers, so that a warp may run one tile ahead
+          const int j = (int)threadIdx.x - 64, n = nb * BN + j;
+          if (j < BN) bias[j] = n < a.N ? __ldg(a.bias + n) : 0.0f;
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        if (!failed && !mbar_wait_warp(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
+          if (lane == 0) atomicExch(a.error, kErrAccWait);
+          failed = true;
+        }
+        if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
+        tc_fence_after();
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2) && nb * BN + c < a.N; c += 32) {
+          const int n = nb * BN + c, live = min(32, a.N - n);
+          float v[32];
+          tmem_load32(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
+          if (EPI != kProduct) {
+            if (a.bias) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float4 w = reinterpret_cast<const float4*>(bias + c)[q];
+                v[4 * q] += w.x, v[4 * q + 1] += w.y, v[4 * q + 2] += w.z, v[4 * q + 3] += w.w;
+              }
+            }
+            if (live < 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = j < live ? v[j] : -INFINITY;
+            }
+          }
+          if (EPI == kPartials) {
+            const bool mine = y >= n && y < n + live;
+            if (__any_sync(0xffffffffu, (int)mine)) {
+              float z = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) z = y - n == j ? v[j] : z;
+              if (mine) a.target_logit[m] = z;
+            }
+            float most[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int j = 4; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
+            const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * kLog2E;
+            if (now > top) {
+              sum *= top == -INFINITY ? 0.0f : exp2_fast(top - now);
+              top = now;
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast(fmaf(v[j], kLog2E, -base));
+            sum += (s[0] + s[1]) + (s[2] + s[3]);
+          } else if (EPI == kGradient) {
+            if (weight == 0.0f) {  // a row that does not count, whatever it holds
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = weight * exp2_fast(fmaf(v[j], kLog2E, -log2_z));
+              const bool mine = y >= n && y < n + live;
+              if (mine) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = y - n == j ? v[j] - weight : v[j];
+              }
+            }
+            __syncwarp();
+            store_values(v, a.f16 ? TTHRML_DT_F16 : TTHRML_DT_BF16, turn, a.g, a.g_ld, n, m - lane, a.M, live, 16);
+            if (a.bias_part) {
+              const float s = column_sums(v);
+              if (m - lane < a.M && lane < live) a.bias_part[(int64_t)(m >> 5) * a.bias_ld + n + lane] = s;
+            }
+          } else {
+            if (a.scaled) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= factor;
+              store_values(v, a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m - lane, a.M, live, a.align);
+            } else if (m < a.M) {  // rows of whole 32 floats, a row per lane: a long main loop hides it
+              float4* out = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + split * a.plane + (int64_t)m * a.out_ld + n);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                float4 w = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                if (a.accumulate) {
+                  const float4 old = __ldcg(out + q);
+                  w.x += old.x, w.y += old.y, w.z += old.z, w.w += old.w;
+                }
+                out[q] = w;
+              }
+            }
+          }
+          __syncwarp();  // the next TMEM load is a warp's
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_leader(&acc_empty[b]);
+      }
+      if (EPI == kPartials && m < a.M) a.part[(int64_t)m * a.slots + 2 * sg + half] = make_float2(top, sum);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1 && leader) {
+    // every MMA the pair issued has completed (in both CTAs' TMEM) before TMEM is freed
+    if (lane == 0) {
+      for (int b = 0; b < 2; ++b)
+        if (last_it[b] >= 0) (void)mbar_wait(&acc_full[b], (uint32_t)(last_it[b] >> 1) & 1u);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA frees TMEM or exits while the other may still signal it
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// Joins the partial sums of a row (a warp per row) into log2 z and the row's loss; the last block adds the losses, in an
+// order that does not depend on which block is the last.
+struct LossArgs {
+  const float2* part;
+  const float* target_logit;
+  RowTargets targets;
+  int64_t rows, categories;
+  int32_t slots, reduction;  // 0: none, 1: mean over the rows that count, 2: sum
+  float *log2_z, *loss;      // [rows]
+  float* reduced;            // the loss, and 1 / the rows that count (1 at least)
+  uint32_t* counter;
+};
+__global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
+  __shared__ double sums[8];
+  __shared__ int64_t counts[8];
+  __shared__ bool last;
+  wait_for_previous_kernel();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + warp;
+  if (row < a.rows) {
+    float m = -INFINITY, s = 0.0f;
+    const float2* p = a.part + row * a.slots;
+    for (int i = lane; i < a.slots; i += 32) {
+      const float2 v = __ldcg(p + i);
+      join(m, s, v.x, v.y);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane & o) {  // both lanes of a pair join in the same order
+        float m1 = m2, s1 = s2;
+        join(m1, s1, m, s);
+        m = m1, s = s1;
+      } else {
+        join(m, s, m2, s2);
+      }
+    }
+    if (lane == 0) {
+      const float z = s == 0.0f ? -INFINITY : m + log2f(s);  // no category is possible: z = -inf
+      const int64_t y = target_of(a.targets, row);
+      float loss = 0.0f;
+      if (y != a.targets.ignored) {
+        if (y < 0 || y >= a.categories)
+          loss = __uint_as_float(0x7FC00000u);
+        else
+          loss = z == -INFINITY ? INFINITY : z * kLn2 - __ldcg(a.target_logit + row);
+      }
+      a.log2_z[row] = z;
+      a.loss[row] = loss;
+    }
+  }
+  if (a.reduction == 0) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.counter, 1u) == gridDim.x - 1u;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double sum = 0.0;
+  int64_t count = 0;
+  for (int64_t i = threadIdx.x; i < a.rows; i += 256) {
+    sum += (double)__ldcg(a.loss + i);
+    count += target_of(a.targets, i) != a.targets.ignored;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  if (lane == 0) sums[warp] = sum, counts[warp] = count;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) sum += sums[i], count += counts[i];
+    const double n = a.reduction == 1 ? (double)(count > 0 ? count : 1) : 1.0;
+    a.reduced[0] = (float)(sum / n);
+    a.reduced[1] = (float)(1.0 / n);
+  }
+}
+
+// The largest magnitude of the weights of the rows that count; one block.
+__global__ void __launch_bounds__(1024) k_xent_top(const float* grad, RowTargets targets, int64_t rows, float* top) {
+  __shared__ float part[32];
+  wait_for_previous_kernel();
+  float most = 0.0f;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024)
+    if (target_of(targets, i) != targets.ignored) most = fmaxf(most, fabsf(__ldg(grad + i)));
+  for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    most = part[threadIdx.x];
+    for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (threadIdx.x == 0) *top = most;
+  }
+}
+
+// out[r][c] = factor * sum of planes[i][r][c], in the order of the planes.
+struct JoinArgs {
+  const float* planes;
+  int64_t plane, ld, rows, cols;
+  int32_t n;
+  void* out;
+  int64_t out_ld;
+  int32_t out_dtype;
+  const float* factor[2];
+  float unit;
+};
+__global__ void __launch_bounds__(256) k_xent_join(const JoinArgs a) {
+  wait_for_previous_kernel();
+  const float factor = factor_of(a.factor) / a.unit;
+  const int64_t quads = (a.cols + 3) / 4, all = a.rows * quads;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / quads, c = (i - r * quads) * 4;
+    const float* p = a.planes + r * a.ld + c;
+    float4 s = __ldcg(reinterpret_cast<const float4*>(p));
+    for (int k = 1; k < a.n; ++k) {
+      const float4 t = __ldcg(reinterpret_cast<const float4*>(p + k * a.plane));
+      s.x += t.x, s.y += t.y, s.z += t.z, s.w += t.w;
+    }
+    const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c + j >= a.cols) break;
+      const int64_t at = r * a.out_ld + c + j;
+      if (a.out_dtype == TTHRML_DT_F32)
+        reinterpret_cast<float*>(a.out)[at] = v[j];
+      else if (a.out_dtype == TTHRML_DT_BF16)
+        reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v[j]);
+      else
+        reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(v[j]);
+    }
+  }
+}
+
+// db[n] = factor * sum over the groups of 32 rows, in their order; eight threads share a column.
+__global__ void __launch_bounds__(256) k_xent_bias(const float* part, int64_t groups, int64_t ld, int64_t n, float* db,
+                                                   const float* f0, const float* f1, float unit) {
+  __shared__ float sums[8][33];
+  wait_for_previous_kernel();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (c < n)
+    for (int64_t g = warp; g < groups; g += 8) s += __ldcg(part + g * ld + c);
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < n) {
+    for (int i = 1; i < 8; ++i) s += sums[i][lane];
+    const float* const f[2] = {f0, f1};
+    db[c] = s * (factor_of(f) / unit);
+  }
+}
+
+// Tensor map of a 16-bit matrix [rows][cols] with rows ld elements apart, in boxes of 64 columns x box_rows, 128-byte swizzle.
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows, bool f16) {
+  EncodeTiledFn fn;
+  int rc = encode_fn(&fn);
+  if (rc) return rc;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64u, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d) for a %lld x %lld 16-bit matrix", (int)r, (long long)rows, (long long)cols);
+    return TTHRML_ERR_CUDA;
+  }
+  return TTHRML_OK;
+}
+
+constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+template <int EPI, bool A_MN, bool B_MN, int BN>
+int launch_xent(const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
+  const void* fn = (const void*)k_xent<EPI, A_MN, B_MN, BN>;
+  ClusterFit fit;
+  const int rc = cluster_fit(fn, 2, kThreads, XentShape<BN>::kSmem, &fit);
+  if (rc) return rc;
+  const int64_t clusters = a.units < fit.clusters ? a.units : fit.clusters;
+  void* params[3] = {(void*)&ma, (void*)&mb, (void*)&a};
+  return launch_clusters(fn, (unsigned)(2 * clusters), 2, kThreads, XentShape<BN>::kSmem, params, st, "k_xent launch", true);
+}
+template <int EPI>
+int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
+  if (bn == 64) return launch_xent<EPI, false, false, 64>(ma, mb, a, st);
+  if (bn == 128) return launch_xent<EPI, false, false, 128>(ma, mb, a, st);
+  return launch_xent<EPI, false, false, 256>(ma, mb, a, st);
+}
+
+// How many pairs of CTAs work at once (every form of the kernel fills an SM).
+int resident_pairs(int64_t* out) {
+  ClusterFit fit;
+  const int rc = cluster_fit((const void*)k_xent<kProduct, false, true, 256>, 2, kThreads, XentShape<256>::kSmem, &fit);
+  *out = fit.clusters;
+  return rc;
+}
+// The widest tile that still gives every pair work.
+int tile_width(int64_t rows, int64_t n, int64_t pairs) {
+  const int64_t m_blocks = up(rows, 256) / 256;
+  for (int bn = 256; bn > 64; bn /= 2)
+    if (m_blocks * (up(n, bn) / bn) >= pairs) return bn;
+  return 64;
+}
+// Tiles along N per unit: as few rounds of units as possible, then as few partial sums.
+int tiles_per_unit(int64_t m_blocks, int64_t n_blocks, int64_t pairs) {
+  int64_t best = INT64_MAX, seg = 1;
+  for (int64_t s = 1; s <= n_blocks && s <= 128; ++s) {
+    const int64_t units = m_blocks * ((n_blocks + s - 1) / s), cost = (units + pairs - 1) / pairs * s;
+    if (cost <= best) best = cost, seg = s;
+  }
+  return (int)seg;
+}
+// Shares of a product's sum: as many as give every pair a tile, of at least four blocks of 64.
+int64_t shares(int64_t m, int64_t n, int64_t k, int64_t pairs) {
+  const int64_t tiles = (up(m, 256) / 256) * (up(n, 256) / 256), most = std::max<int64_t>(1, up(k, 64) / 64 / 4);
+  return std::max<int64_t>(1, std::min(pairs / tiles, most));
+}
+
+struct ForwardPlan {
+  int bn, seg, segments;
+  int64_t logits, counter, bytes;  // places in the workspace behind the partial sums
+};
+int plan_forward(int64_t rows, int64_t categories, ForwardPlan* p) {
+  int64_t pairs;
+  const int rc = resident_pairs(&pairs);
+  if (rc) return rc;
+  p->bn = tile_width(rows, categories, pairs);
+  const int64_t n_blocks = up(categories, p->bn) / p->bn;
+  p->seg = tiles_per_unit(up(rows, 256) / 256, n_blocks, pairs);
+  p->segments = (int)((n_blocks + p->seg - 1) / p->seg);
+  p->logits = up(rows * 2 * p->segments * 8, 16);
+  p->counter = p->logits + up(rows * 4, 16);
+  p->bytes = p->counter + 16;
+  return TTHRML_OK;
+}
+
+struct BackwardPlan {
+  int64_t piece, pieces, g_ld, plane_ld, dx_shares, dw_shares;
+  bool dx_planes;
+  int64_t bias, top, dx, dw, bytes;  // places in the workspace behind g
+};
+int plan_backward(int64_t rows, int64_t categories, int64_t cols, bool want_x, bool want_w, bool want_b, BackwardPlan* p) {
+  int64_t pairs;
+  const int rc = resident_pairs(&pairs);
+  if (rc) return rc;
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / rows / 256 * 256);
+  p->pieces = (categories + most - 1) / most;
+  p->piece = up((categories + p->pieces - 1) / p->pieces, 256);
+  p->pieces = (categories + p->piece - 1) / p->piece;
+  const int64_t width = std::min(p->piece, categories);
+  p->g_ld = up(width, 64);
+  p->plane_ld = up(cols, 32);
+  p->dx_shares = want_x ? shares(rows, cols, width, pairs) : 0;
+  p->dw_shares = want_w ? shares(width, cols, rows, pairs) : 0;
+  p->dx_planes = p->dx_shares > 1 || (want_x && p->pieces > 1);
+  p->bias = up(rows * p->g_ld * 2, 16);
+  p->top = p->bias + (want_b ? up(rows, 32) / 32 * p->g_ld * 4 : 0);
+  p->dx = p->top + 16;
+  p->dw = p->dx + (p->dx_planes ? p->dx_shares * rows * p->plane_ld * 4 : 0);
+  p->bytes = p->dw + (p->dw_shares > 1 ? p->dw_shares * width * p->plane_ld * 4 : 0);
+  return TTHRML_OK;
+}
+
+int check_problem(const char* what, const tthrml_xent* p) {
+  if (!p || !p->x || !p->w || !p->targets) {
+    set_error("%s: NULL argument", what);
+    return TTHRML_ERR_ARG;
+  }
+  if (p->dtype != TTHRML_DT_BF16 && p->dtype != TTHRML_DT_F16) {
+    set_error("%s: x and weights must be bfloat16 or float16 (got code %d)", what, (int)p->dtype);
+    return TTHRML_ERR_ARG;
+  }
+  if (p->rows < 1 || p->categories < 1 || p->cols < 1 || p->rows > TTHRML_XENT_MAX_ROWS ||
+      p->categories > TTHRML_XENT_MAX_CATEGORIES || p->cols > TTHRML_XENT_MAX_COLS) {
+    set_error("%s: sizes out of range (%lld rows of %lld columns, %lld categories)", what, (long long)p->rows,
+              (long long)p->cols, (long long)p->categories);
+    return TTHRML_ERR_ARG;
+  }
+  if ((uintptr_t)p->x % 16 || (uintptr_t)p->w % 16 || p->x_ld % 8 || p->w_ld % 8 || p->x_ld < p->cols || p->w_ld < p->cols ||
+      (uintptr_t)p->targets % (p->wide_targets ? 8 : 4) || (p->bias && (uintptr_t)p->bias % 4)) {
+    set_error("%s: x and weights must be 16-byte aligned with pitches that are multiples of 8 elements and not below the "
+              "columns (got pitches %lld, %lld)", what, (long long)p->x_ld, (long long)p->w_ld);
+    return TTHRML_ERR_ARG;
+  }
+  return TTHRML_OK;
+}
+
+// One product of the backward pass, [m][k] x [k][n], into out (scaled) or planes.
+template <bool A_MN>
+int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m, int64_t n, int64_t k, int64_t n_shares,
+            int64_t pairs, cudaStream_t st) {
+  a.M = (int32_t)m;
+  a.N = (int32_t)n;
+  a.num_k = (int32_t)(up(k, 64) / 64);
+  a.seg = 1;
+  a.segments = (int32_t)(up(n, 256) / 256);
+  a.splits = (int32_t)n_shares;
+  const int64_t m_blocks = up(m, 256) / 256;
+  a.units = (int32_t)(m_blocks * a.segments * n_shares);
+  int64_t g = 1;  // about square rectangles of the tiles in flight
+  while ((g + 1) * (g + 1) <= pairs) ++g;
+  a.group = (int32_t)std::min(g, m_blocks);
+  return launch_xent<kProduct, A_MN, true, 256>(ma, mb, a, st);
+}
+int join_planes(const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols, int64_t n, const XentArgs& a, void* out,
+                int64_t out_ld, int32_t out_dtype, cudaStream_t st) {
+  JoinArgs j = {planes, plane, ld, rows, cols, (int32_t)n, out, out_ld, out_dtype, {a.factor[0], a.factor[1]}, a.unit};
+  const int64_t blocks = (rows * ((cols + 3) / 4) + 255) / 256;
+  void* params[1] = {(void*)&j};
+  return launch_clusters((const void*)k_xent_join, (unsigned)std::min<int64_t>(blocks, 148 * 8), 1, 256, 0, params, st,
+                         "k_xent_join launch", true);
+}
+
+}  // namespace
+}  // namespace tthrml
+
+extern "C" int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories) {
+  using namespace tthrml;
+  if (rows < 1 || categories < 1 || rows > TTHRML_XENT_MAX_ROWS || categories > TTHRML_XENT_MAX_CATEGORIES) return 0;
+  ForwardPlan p;
+  const int rc = plan_forward(rows, categories, &p);
+  return rc ? rc : p.bytes;
+}
+
+extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* row_loss, float* reduced, int32_t reduction,
+                                   void* workspace, int64_t workspace_bytes, int32_t* error, void* stream) {
+  using namespace tthrml;
+  int rc = check_problem("tthrml_xent_forward", p);
+  if (rc) return rc;
+  if (!log2_z || !row_loss || !workspace || !error || reduction < 0 || reduction > 2 || (reduction && !reduced)) {
+    set_error("tthrml_xent_forward: NULL argument or unknown reduction %d", (int)reduction);
+    return TTHRML_ERR_ARG;
+  }
+  ForwardPlan f;
+  rc = plan_forward(p->rows, p->categories, &f);
+  if (rc) return rc;
+  if ((uintptr_t)workspace % 16 || workspace_bytes < f.bytes) {
+    set_error("tthrml_xent_forward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)f.bytes,
+              (long long)workspace_bytes);
+    return TTHRML_ERR_ARG;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool f16 = p->dtype == TTHRML_DT_F16;
+  unsigned char* ws = (unsigned char*)workspace;
+  CUtensorMap ma, mb;
+  rc = make_map(&ma, p->x, p->rows, p->cols, p->x_ld, 128u, f16);
+  if (rc == TTHRML_OK) rc = make_map(&mb, p->w, p->categories, p->cols, p->w_ld, (uint32_t)f.bn / 2, f16);
+  if (rc) return rc;
+  XentArgs a = {};
+  a.M = (int32_t)p->rows;
+  a.N = (int32_t)p->categories;
+  a.num_k = (int32_t)(up(p->cols, 64) / 64);
+  a.f16 = f16;
+  a.seg = f.seg;
+  a.segments = f.segments;
+  a.splits = 1;
+  const int64_t m_blocks = up(p->rows, 256) / 256, g = ((int64_t)32 << 20) / (512 * p->cols);
+  a.units = (int32_t)(m_blocks * f.segments);
+  a.group = (int32_t)std::max<int64_t>(1, std::min(g, m_blocks));  // raster groups of about 32 MiB of A panels
+  a.bias = p->bias;
+  a.categories = p->categories;
+  a.targets = {p->targets, p->wide_targets, p->ignored};
+  a.part = (float2*)ws;
+  a.slots = 2 * f.segments;
+  a.target_logit = (float*)(ws + f.logits);
+  a.counter = (uint32_t*)(ws + f.counter);
+  a.error = error;
+  rc = launch_logits<kPartials>(f.bn, ma, mb, a, st);
+  if (rc) return rc;
+  LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, log2_z, row_loss, reduced, a.counter};
+  void* params[1] = {(void*)&l};
+  return launch_clusters((const void*)k_xent_loss, (unsigned)((p->rows + 7) / 8), 1, 256, 0, params, st, "k_xent_loss launch",
+                         true);
+}
+
+extern "C" int64_t tthrml_xent_backward_workspace(int64_t rows, int64_t categories, int64_t cols, int32_t dx, int32_t dw,
+                                                  int32_t db) {
+  using namespace tthrml;
+  if (rows < 1 || categories < 1 || cols < 1 || rows > TTHRML_XENT_MAX_ROWS || categories > TTHRML_XENT_MAX_CATEGORIES ||
+      cols > TTHRML_XENT_MAX_COLS)
+    return 0;
+  BackwardPlan p;
+  const int rc = plan_backward(rows, categories, cols, dx != 0, dw != 0, db != 0, &p);
+  return rc ? rc : p.bytes;
+}
+
+extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, const float* grad, int32_t grad_per_row,
+                                    const float* inv_count, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld,
+                                    int32_t grad_dtype, float* db, void* workspace, int64_t workspace_bytes, int32_t* error,
+                                    void* stream) {
+  using namespace tthrml;
+  int rc = check_problem("tthrml_xent_backward", p);
+  if (rc) return rc;
+  if (!log2_z || !grad || !workspace || !error || (dx && dx_ld < p->cols) || (dw && dw_ld < p->cols)) {
+    set_error("tthrml_xent_backward: NULL argument, or gradients whose rows overlap");
+    return TTHRML_ERR_ARG;
+  }
+  if (grad_dtype == TTHRML_DT_I8 || dtype_bytes(grad_dtype) == 0) {
+    set_error("tthrml_xent_backward: gradients must be float32, bfloat16 or float16 (got code %d)", (int)grad_dtype);
+    return TTHRML_ERR_ARG;
+  }
+  if (!dx && !dw && !db) return TTHRML_OK;
+  BackwardPlan f;
+  rc = plan_backward(p->rows, p->categories, p->cols, dx, dw, db, &f);
+  int64_t pairs;
+  if (rc == TTHRML_OK) rc = resident_pairs(&pairs);
+  if (rc) return rc;
+  if ((uintptr_t)workspace % 16 || workspace_bytes < f.bytes) {
+    set_error("tthrml_xent_backward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)f.bytes,
+              (long long)workspace_bytes);
+    return TTHRML_ERR_ARG;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool f16 = p->dtype == TTHRML_DT_F16;
+  unsigned char* ws = (unsigned char*)workspace;
+  float* top = (float*)(ws + f.top);
+  XentArgs base = {};
+  base.f16 = f16;
+  base.unit = f16 ? 16384.0f : 1.0f;
+  base.categories = p->categories;
+  base.targets = {p->targets, p->wide_targets, p->ignored};
+  base.log2_z = log2_z;
+  base.g = ws;
+  base.g_ld = f.g_ld;
+  base.error = error;
+  base.factor[0] = grad_per_row ? top : grad;
+  base.factor[1] = inv_count;
+  if (grad_per_row) {
+    base.row_grad = grad;
+    base.top_grad = top;
+    void* params[4] = {(void*)&grad, (void*)&base.targets, (void*)&p->rows, (void*)&top};
+    rc = launch_clusters((const void*)k_xent_top, 1, 1, 1024, 0, params, st, "k_xent_top launch", true);
+    if (rc) return rc;
+  }
+  const int64_t bytes = dtype_bytes(grad_dtype);
+  auto alignment = [&](const void* out, int64_t ld) {
+    const uint64_t v = (uint64_t)(uintptr_t)out | (uint64_t)(ld * bytes);
+    return v % 16 == 0 ? 16 : (v % 8 == 0 ? 8 : (v % 4 == 0 ? 4 : 2));
+  };
+  CUtensorMap mx, mx_mn;
+  rc = make_map(&mx, p->x, p->rows, p->cols, p->x_ld, 128u, f16);
+  if (rc == TTHRML_OK) rc = make_map(&mx_mn, p->x, p->rows, p->cols, p->x_ld, 64u, f16);
+  for (int64_t i = 0; i < f.pieces && rc == TTHRML_OK; ++i) {
+    const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
+    const char* w = (const char*)p->w + first * p->w_ld * 2;
+    CUtensorMap mw, mw_mn, mg, mg_mn;
+    const int bn = tile_width(p->rows, width, pairs);
+    rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)bn / 2, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mg, ws, p->rows, width, f.g_ld, 128u, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mg_mn, ws, p->rows, width, f.g_ld, 64u, f16);
+    if (rc) return rc;
+    XentArgs a = base;
+    a.M = (int32_t)p->rows;
+    a.N = (int32_t)width;
+    a.num_k = (int32_t)(up(p->cols, 64) / 64);
+    a.seg = 1;
+    a.segments = (int32_t)(up(width, bn) / bn);
+    a.splits = 1;
+    const int64_t m_blocks = up(p->rows, 256) / 256;
+    a.units = (int32_t)(m_blocks * a.segments);
+    int64_t g = 1;
+    while ((g + 1) * (g + 1) <= pairs) ++g;
+    a.group = (int32_t)std::min(g, m_blocks);
+    a.bias = p->bias ? p->bias + first : nullptr;
+    a.first = first;
+    a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
+    a.bias_ld = f.g_ld;
+    rc = launch_logits<kGradient>(bn, mx, mw, a, st);
+    if (rc) return rc;
+    if (dx) {
+      XentArgs d = base;
+      d.scaled = !f.dx_planes;
+      d.out = f.dx_planes ? (void*)(ws + f.dx) : dx;
+      d.out_ld = f.dx_planes ? f.plane_ld : dx_ld;
+      d.plane = f.dx_planes ? p->rows * f.plane_ld : 0;
+      d.out_dtype = grad_dtype;
+      d.align = alignment(dx, dx_ld);
+      d.accumulate = i > 0;
+      rc = product<false>(mg, mw_mn, d, p->rows, p->cols, width, std::min(f.dx_shares, up(width, 64) / 64), pairs, st);
+      if (rc) return rc;
+    }
+    if (dw) {
+      XentArgs d = base;
+      char* out = (char*)dw + first * dw_ld * bytes;
+      const bool planes = f.dw_shares > 1;
+      d.scaled = !planes;
+      d.out = planes ? (void*)(ws + f.dw) : out;
+      d.out_ld = planes ? f.plane_ld : dw_ld;
+      d.plane = planes ? width * f.plane_ld : 0;
+      d.out_dtype = grad_dtype;
+      d.align = alignment(out, dw_ld);
+      rc = product<true>(mg_mn, mx_mn, d, width, p->cols, p->rows, f.dw_shares, pairs, st);
+      if (rc == TTHRML_OK && planes)
+        rc = join_planes((const float*)(ws + f.dw), d.plane, f.plane_ld, width, p->cols, f.dw_shares, base, out, dw_ld, grad_dtype, st);
+      if (rc) return rc;
+    }
+    if (db) {
+      const float* part = a.bias_part;
+      const int64_t groups = up(p->rows, 32) / 32;
+      float* out = db + first;
+      void* params[8] = {(void*)&part, (void*)&groups, (void*)&f.g_ld, (void*)&width, (void*)&out, (void*)&base.factor[0],
+                         (void*)&base.factor[1], (void*)&base.unit};
+      rc = launch_clusters((const void*)k_xent_bias, (unsigned)((width + 31) / 32), 1, 256, 0, params, st, "k_xent_bias launch",
+                           true);
+      if (rc) return rc;
+    }
+  }
+  if (rc == TTHRML_OK && dx && f.dx_planes)
+    rc = join_planes((const float*)(ws + f.dx), p->rows * f.plane_ld, f.plane_ld, p->rows, p->cols, f.dx_shares, base, dx, dx_ld,
+                     grad_dtype, st);
+  return rc;
+}
