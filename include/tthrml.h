@@ -777,6 +777,53 @@ int tthrml_xent_backward(const tthrml_xent* problem_host, const float* log2_z_de
 int64_t tthrml_xent_backward_workspace(int64_t rows, int64_t categories, int64_t cols, int32_t dx,
                                        int32_t dw, int32_t db);
 
+/*
+ * ---------------------------------------------------------------------------
+ * 4-bit floating point rows: value[r][c] = code * block[r][c / 16] * scale[r].
+ * Codes e2m1, two to a byte (the even column in the low half), rows of `pitch`
+ * bytes.  Block scales e4m3 in the order of the tensor core: for each 128 rows,
+ * for each 256 columns 2048 bytes; in them for each 64 columns 512 bytes; in
+ * those the four scales of row r at byte (r % 32) * 16 + (r % 128 / 32) * 4,
+ * zeros behind the ends.  Both 16-byte aligned, pitch a multiple of 16.
+ * ---------------------------------------------------------------------------
+ */
+#define TTHRML_FP4_MAX_COLS (1 << 20)
+
+/* Bytes of the block scales of a matrix. */
+int64_t tthrml_fp4_scale_bytes(int64_t rows, int64_t cols);
+
+/*
+ * scale = max|x_r| / 2688, block = e4m3(max|x_b| / (6 scale)), code =
+ * e2m1(x / (block scale)), in float32 (fl(2688 / max|x_r|) first).  Rows below
+ * 2^-100 get scale 0, rows that are not finite scale NaN.  Strides in elements.
+ */
+int tthrml_fp4_quantize(const void* x_dev, int32_t dtype, int64_t rows, int64_t cols,
+                        int64_t row_stride, int64_t col_stride, void* codes_dev, int64_t pitch,
+                        void* blocks_dev, float* scale_dev, void* stream);
+
+/* The float32 values, [rows][cols] dense, 16-byte aligned. */
+int tthrml_fp4_values(const void* codes_dev, int64_t pitch, const void* blocks_dev,
+                      const float* scale_dev, int64_t rows, int64_t cols, float* out_dev,
+                      void* stream);
+
+/* out[m][n] = (sum_k x[m][k] w[n][k]) * (x_scale[m] * w_scale[n]) + bias[n], sums in float32. */
+int tthrml_fp4_product(const void* x_codes_dev, int64_t x_pitch, const void* x_blocks_dev,
+                       const float* x_scale_dev, const void* w_codes_dev, int64_t w_pitch,
+                       const void* w_blocks_dev, const float* w_scale_dev, int64_t rows,
+                       int64_t units, int64_t cols, const float* bias_dev, void* out_dev,
+                       int32_t out_dtype, int64_t out_ld, int32_t* error_dev, void* stream);
+
+/*
+ * Rows of floats through 4-bit weights: tthrml_fp4_quantize into the workspace, then tthrml_fp4_product.  workspace: 16-byte
+ * aligned device memory of tthrml_fp4_linear_workspace(rows, cols) bytes, free again once the work on `stream` is done.
+ */
+int tthrml_fp4_linear(const void* x_dev, int32_t x_dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                      int64_t col_stride, void* workspace_dev, int64_t workspace_bytes,
+                      const void* w_codes_dev, int64_t w_pitch, const void* w_blocks_dev,
+                      const float* w_scale_dev, int64_t units, const float* bias_dev, void* out_dev,
+                      int32_t out_dtype, int64_t out_ld, int32_t* error_dev, void* stream);
+int64_t tthrml_fp4_linear_workspace(int64_t rows, int64_t cols);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

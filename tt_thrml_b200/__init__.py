@@ -34,6 +34,7 @@ from .core import (
     open_mesh_device,
 )
 from .executor import Executor, make_executor
+from .fp4 import Fp4Rows, fp4_product, quantize_fp4
 from .learning import DenseLearner, dense_moments
 from .losses import softmax_cross_entropy
 from .mesh import MeshExecutor, make_mesh_executor, mesh_barrier, mesh_device_ids, mesh_size
@@ -107,4 +108,7 @@ __all__ = [
     "DenseLearner",
     "AdamW",
     "softmax_cross_entropy",
+    "Fp4Rows",
+    "quantize_fp4",
+    "fp4_product",
 ]

@@ -23,6 +23,7 @@ STATE_F32, STATE_I8, STATE_BITS = 0, 1, 2
 DT_F32, DT_BF16, DT_F16, DT_I8 = 0, 1, 2, 3
 INT8_MAX_COLS = 131071
 INT8_FEW_BYTES = 163840
+FP4_MAX_COLS = 1 << 20
 MAX_PHASES = 6
 XENT_MAX_ROWS = XENT_MAX_CATEGORIES = 1 << 24
 XENT_MAX_COLS = 1 << 20
@@ -272,6 +273,19 @@ _SIGNATURES = {
         [ctypes.POINTER(Xent), c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp],
     ),
     "tthrml_xent_backward_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i32, c_i32, c_i32]),
+    "tthrml_fp4_scale_bytes": (c_i64, [c_i64, c_i64]),
+    "tthrml_fp4_quantize": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "tthrml_fp4_values": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp]),
+    "tthrml_fp4_product": (
+        c_i32,
+        [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp, c_vp],
+    ),
+    "tthrml_fp4_linear": (
+        c_i32,
+        [c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp,
+         c_vp],
+    ),
+    "tthrml_fp4_linear_workspace": (c_i64, [c_i64, c_i64]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),
     "tthrml_last_error": (ctypes.c_char_p, []),
