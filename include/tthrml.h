@@ -824,6 +824,19 @@ int tthrml_fp4_linear(const void* x_dev, int32_t x_dtype, int64_t rows, int64_t 
                       int32_t out_dtype, int64_t out_ld, int32_t* error_dev, void* stream);
 int64_t tthrml_fp4_linear_workspace(int64_t rows, int64_t cols);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Dropout: y[i] = keep[i] ? x[i] * 65536 / (65536 - cut) : 0, keep[i] =
+ * (half-word i % 8, low halves first, of Philox4x32-10 keyed by seed at counter
+ * (i / 8, i / 8 >> 32, step, "DROP")) >= cut.  step_at: a device int32 (or, with
+ * step_wide, int64) whose low 32 bits are taken for step; step_used: where the
+ * step is left (4 bytes); both may be NULL.
+ * ---------------------------------------------------------------------------
+ */
+int tthrml_dropout(const void* x_dev, int32_t dtype, int64_t n, int32_t cut, uint64_t seed,
+                   uint32_t step, const void* step_at_dev, int32_t step_wide,
+                   uint32_t* step_used_dev, void* y_dev, void* stream);
+
 /* Host-only: greedy graph colouring in node order (smallest free colour).
  * Returns the number of colours in *n_colours.  No device work. */
 int tthrml_greedy_colouring(int64_t n_nodes, const int64_t* row_ptr_host,

@@ -41,6 +41,7 @@ from .mesh import MeshExecutor, make_mesh_executor, mesh_barrier, mesh_device_id
 from .moments import pair_moments
 from .optim import AdamW
 from .quantized import QuantizedRows, check_operator_errors, int8_product, quantize_rows
+from .regularise import dropout
 from .rng import generate_bulk_rng, make_rng_spec, slice_rng_for_sweep
 
 
@@ -108,6 +109,7 @@ __all__ = [
     "DenseLearner",
     "AdamW",
     "softmax_cross_entropy",
+    "dropout",
     "Fp4Rows",
     "quantize_fp4",
     "fp4_product",
