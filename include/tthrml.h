@@ -751,15 +751,15 @@ typedef struct tthrml_xent {
  * log2_z: [rows], z / ln 2, which the backward pass takes.  row_loss: [rows].
  * A row in which no category is possible has loss inf and no gradient; a
  * target outside 0 .. categories-1 that is not `ignored` has loss NaN (and NaN
- * gradients).  reduction 0: rows only; 1: reduced[0] is the mean over the rows
- * that count (0 if there are none), 2: their sum; reduced[1] is 1 / their
- * number or 1, the second factor of the backward pass.  The same every time.
+ * gradients).  reduction 0: rows only; 1: *loss is the mean over the rows that
+ * count (0 if there are none) and *inv_count 1 / their number, 2: their sum and
+ * 1; *inv_count is the second factor of the backward pass.  The same every time.
  * workspace: tthrml_xent_forward_workspace(rows, categories) bytes (of the
  * current device; negative: an error), 16-byte aligned, free again once the
  * work on `stream` is done.
  */
 int tthrml_xent_forward(const tthrml_xent* problem_host, float* log2_z_dev, float* row_loss_dev,
-                        float* reduced_dev, int32_t reduction, void* workspace_dev,
+                        float* loss_dev, float* inv_count_dev, int32_t reduction, void* workspace_dev,
                         int64_t workspace_bytes, int32_t* error_dev, void* stream);
 int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories);
 

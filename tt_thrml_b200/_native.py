@@ -266,7 +266,7 @@ _SIGNATURES = {
         [c_vp, c_i32, c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp],
     ),
     "tthrml_pair_moments": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
-    "tthrml_xent_forward": (c_i32, [ctypes.POINTER(Xent), c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]),
+    "tthrml_xent_forward": (c_i32, [ctypes.POINTER(Xent), c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]),
     "tthrml_xent_forward_workspace": (c_i64, [c_i64, c_i64]),
     "tthrml_xent_backward": (
         c_i32,
@@ -346,6 +346,23 @@ def hostcall():
         except ImportError as e:
             raise RuntimeError("tt_thrml_b200/_hostcall.so is missing or stale: run python -m tt_thrml_b200.build") from e
     return _host
+
+
+# entry points that the host module calls by itself, in the order of its Library (csrc/hostcall.h)
+_HOST_ENTRIES = ("set_device", "last_error", "pack_rows", "xent_forward", "xent_forward_workspace", "xent_backward",
+                 "xent_backward_workspace", "dropout", "fp4_quantize", "fp4_scale_bytes", "fp4_values", "fp4_linear",
+                 "fp4_linear_workspace")
+_host_bound = None
+
+
+def bound_hostcall():
+    """The host module with the library's entry points given to it."""
+    global _host_bound
+    if _host_bound is None:
+        host = hostcall()
+        host.bind_library(*(address_of("tthrml_" + name) for name in _HOST_ENTRIES))
+        _host_bound = host
+    return _host_bound
 
 
 _addresses: dict = {}

@@ -42,6 +42,10 @@ def _nvcc() -> str:
     return cand
 
 
+def _cuda_include() -> Path:
+    return Path(shutil.which(_nvcc()) or _nvcc()).resolve().parent.parent / "include"
+
+
 def _headers() -> list[Path]:
     return sorted(CSRC.glob("*.cuh")) + sorted((REPO_DIR / "include").glob("*.h"))
 
@@ -51,8 +55,8 @@ def build_hostcall(verbose: bool = False, force: bool = False) -> Path:
     Python, whose layouts it has compiled in."""
     import torch
 
-    src = CSRC / "hostcall.cpp"
-    newest = max(src.stat().st_mtime, (REPO_DIR / "include" / "tthrml.h").stat().st_mtime)
+    sources = sorted(CSRC.glob("*.cpp"))
+    newest = max(f.stat().st_mtime for f in [*sources, *CSRC.glob("*.h"), REPO_DIR / "include" / "tthrml.h"])
     root = Path(torch.__file__).resolve().parent
     key = f"torch {torch.__version__} {torch.version.git_version} at {root}, {sys.version}\n"
     stamp = BUILD_DIR / "hostcall.key"
@@ -64,8 +68,8 @@ def build_hostcall(verbose: bool = False, force: bool = False) -> Path:
         os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-        f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp), f"-L{root / 'lib'}",
-        "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+        f"-I{sysconfig.get_paths()['include']}", f"-I{_cuda_include()}", *map(str, sources), "-o", str(tmp),
+        f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10",
     ]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -2,28 +2,13 @@
 // libtthrml_b200.so in one pass.  Python needs about 0.4 us per tensor and attribute, 2.3 us per allocation and 2 us per
 // ctypes call, which is more than the smallest kernels take.  Each function handles the plain case and returns None for
 // any other, which the Python caller then checks, refuses or lays out.
-#include <ATen/ops/empty.h>
-#include <c10/core/GradMode.h>
-#include <Python.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include "../../include/tthrml.h"
+#include "hostcall.h"
 
 namespace {
 
-int32_t dtype_code(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return TTHRML_DT_F32;
-    case at::kBFloat16: return TTHRML_DT_BF16;
-    case at::kHalf: return TTHRML_DT_F16;
-    default: return -1;
-  }
-}
-
-bool plain_cuda(const at::Tensor& t, long device) {
-  return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() && !t.is_conj();
-}
+using hostcall::dtype_code;
+using hostcall::plain_cuda;
+using hostcall::wants_grad;
 
 // Tells autograd that the tensors of a list were written.
 void bump(PyObject* list) {
@@ -48,10 +33,6 @@ PyObject* bump_versions(PyObject*, PyObject* list) {
 template <typename Fn>
 Fn address(PyObject* o) {
   return reinterpret_cast<Fn>(PyLong_AsVoidPtr(o));
-}
-// Whether a derivative is asked of t: a gradient, or the tangent of a forward-mode dual tensor.
-bool wants_grad(const at::Tensor& t) {
-  return (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined();
 }
 
 // What stays the same from step to step of an optimizer (AdamWCall in _native.py).
@@ -279,6 +260,18 @@ PyMethodDef methods[] = {
      "A step of all parameters: the plain case, or where it is not."},
     {"adamw_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_values)), METH_FASTCALL,
      "The 8-bit moments as float32."},
+    {"bind_library", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::bind_library)), METH_FASTCALL,
+     "Takes the addresses of the library's entry points."},
+    {"softmax_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::softmax_cross_entropy)), METH_FASTCALL,
+     "Losses of checked tensors, differentiable."},
+    {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::dropout)), METH_FASTCALL,
+     "Kept elements of a checked tensor, differentiable."},
+    {"quantize_fp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::quantize_fp4)), METH_FASTCALL,
+     "Rows in 4 bits: the plain case, or None."},
+    {"fp4_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::fp4_values)), METH_FASTCALL,
+     "The float32 values of 4-bit rows."},
+    {"fp4_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::fp4_product)), METH_FASTCALL,
+     "Product of float rows and 4-bit weights: the plain case, or None."},
     {"bump_versions", bump_versions, METH_O, "Marks tensors as written for autograd."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", "Host side of calls with many tensors.", -1, methods,

@@ -1,0 +1,342 @@
+// Host side of the operators that autograd differentiates, and of the 4-bit rows: one node of the graph each, written in
+// C++ (a Python one costs 30 us forward and 40 backward, more than the smallest kernels take).  Python checks the arguments
+// of the differentiable operators before the call; the 4-bit calls handle the plain case and return None for any other.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+
+#include "hostcall.h"
+
+namespace hostcall {
+
+Library library = {};
+
+PyObject* bind_library(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  constexpr Py_ssize_t n = sizeof(Library) / sizeof(void*);
+  if (nargs != n) {
+    PyErr_Format(PyExc_TypeError, "bind_library: %zd addresses expected, got %zd", n, nargs);
+    return nullptr;
+  }
+  void* at[n];
+  for (Py_ssize_t i = 0; i < n; ++i) at[i] = PyLong_AsVoidPtr(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  memcpy(&library, at, sizeof(Library));
+  Py_RETURN_NONE;
+}
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == TTHRML_OK, what, " failed (", rc, "): ", library.last_error()); }
+
+// Makes a tensor's device current for torch and for the library on this thread, and the old one again at the end.
+class On {
+ public:
+  explicit On(const Tensor& t) : guard_(t.device()), before_(guard_.original_device().index()), now_(t.device().index()) {
+    check(library.set_device(now_), "tthrml_set_device");
+  }
+  ~On() {
+    if (before_ != now_) library.set_device(before_);
+  }
+  void* stream() const { return c10::cuda::getCurrentCUDAStream(now_).stream(); }
+
+ private:
+  c10::cuda::CUDAGuard guard_;
+  c10::DeviceIndex before_, now_;
+};
+
+Tensor floats(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat).requires_grad(false)); }
+Tensor bytes(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte).requires_grad(false)); }
+
+// The operands as the kernels read them: rows of 16-byte multiples from 16-byte boundaries, or one buffer they are laid out in.
+struct Operand {
+  const void* at;
+  int64_t ld;
+};
+Tensor lay_out(const Tensor& x, const Tensor& w, Operand (&o)[2], void* stream) {
+  const Tensor* t[2] = {&x, &w};
+  tthrml_pack_matrix m[2];
+  int which[2], n = 0;
+  int64_t size = 0;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
+    o[i].at = t[i]->const_data_ptr();
+    o[i].ld = rows > 1 ? t[i]->stride(0) : (cols + 7) / 8 * 8;
+    if ((cols == 1 || t[i]->stride(1) == 1) && o[i].ld % 8 == 0 && o[i].ld >= cols && reinterpret_cast<uintptr_t>(o[i].at) % 16 == 0)
+      continue;
+    o[i].ld = (cols + 7) / 8 * 8;
+    m[n] = {o[i].at, reinterpret_cast<void*>(size * 2), rows, cols, t[i]->stride(0), t[i]->stride(1), o[i].ld};
+    size += rows * o[i].ld;
+    which[n++] = i;
+  }
+  if (!n) return Tensor();
+  Tensor space = at::empty({size}, x.options().requires_grad(false));
+  char* base = static_cast<char*>(space.mutable_data_ptr());
+  for (int i = 0; i < n; ++i) {
+    m[i].dst = base + reinterpret_cast<uintptr_t>(m[i].dst);
+    o[which[i]].at = m[i].dst;
+  }
+  check(library.pack_rows(m, n, stream), "tthrml_pack_rows");
+  return space;
+}
+
+struct XentSaved {
+  Tensor laid, log2_z, inv_count;
+};
+
+tthrml_xent problem(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& targets, int64_t ignored, const Operand (&o)[2]) {
+  tthrml_xent p = {};
+  p.x = o[0].at, p.x_ld = o[0].ld;
+  p.w = o[1].at, p.w_ld = o[1].ld;
+  p.targets = targets.const_data_ptr();
+  p.bias = bias.defined() ? bias.const_data_ptr<float>() : nullptr;
+  p.rows = x.size(0), p.cols = x.size(1), p.categories = w.size(0);
+  p.ignored = ignored;
+  p.dtype = dtype_code(x);
+  p.wide_targets = targets.scalar_type() == at::kLong;
+  return p;
+}
+
+// bias and targets dense.
+Tensor xent_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& targets, int64_t reduction, int64_t ignored,
+                    int64_t error, XentSaved& saved) {
+  const On on(x);
+  Operand o[2];
+  saved.laid = lay_out(x, w, o, on.stream());
+  const tthrml_xent p = problem(x, w, bias, targets, ignored, o);
+  const int64_t size = library.xent_forward_workspace(p.rows, p.categories);
+  if (size < 0) check((int)size, "tthrml_xent_forward_workspace");
+  const Tensor space = bytes(x, size);
+  saved.log2_z = floats(x, {p.rows});
+  Tensor rows = floats(x, {p.rows}), total;
+  if (reduction) {
+    total = floats(x, {});
+    saved.inv_count = floats(x, {});
+  }
+  check(library.xent_forward(&p, saved.log2_z.mutable_data_ptr<float>(), rows.mutable_data_ptr<float>(),
+                             reduction ? total.mutable_data_ptr<float>() : nullptr,
+                             reduction ? saved.inv_count.mutable_data_ptr<float>() : nullptr, (int32_t)reduction,
+                             space.mutable_data_ptr(), size, reinterpret_cast<int32_t*>(error), on.stream()),
+        "tthrml_xent_forward");
+  return reduction ? total : rows;
+}
+
+struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
+  // every argument of a node is a defined tensor: without a bias the targets stand in its place
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& bias_or_targets, const Tensor& targets,
+                        bool with_bias, int64_t reduction, int64_t ignored, int64_t error) {
+    XentSaved s;
+    const Tensor bias = with_bias ? bias_or_targets : Tensor();
+    Tensor loss = xent_forward(x, w, bias, targets, reduction, ignored, error, s);
+    // the tensors themselves, so that a change in place before the backward pass is noticed
+    ctx->save_for_backward({x, w, bias, targets, s.laid, s.log2_z, s.inv_count});
+    ctx->saved_data["ignored"] = ignored;
+    ctx->saved_data["error"] = error;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!c10::GradMode::is_enabled(), "softmax_cross_entropy has no second derivative (create_graph=True)");
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1], &bias = s[2], &targets = s[3], &laid = s[4], &log2_z = s[5], &inv_count = s[6];
+    variable_list out(8);
+    if (!grads[0].defined()) return out;
+    const On on(x);
+    Operand o[2];
+    const Tensor *t[2] = {&x, &w};
+    const char* base = laid.defined() ? static_cast<const char*>(laid.const_data_ptr()) : nullptr;
+    for (int i = 0; i < 2; ++i) {  // as lay_out left them
+      const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
+      o[i].at = t[i]->const_data_ptr();
+      o[i].ld = rows > 1 ? t[i]->stride(0) : (cols + 7) / 8 * 8;
+      if ((cols == 1 || t[i]->stride(1) == 1) && o[i].ld % 8 == 0 && o[i].ld >= cols && reinterpret_cast<uintptr_t>(o[i].at) % 16 == 0)
+        continue;
+      o[i].ld = (cols + 7) / 8 * 8;
+      o[i].at = base;
+      base += rows * o[i].ld * 2;
+    }
+    const tthrml_xent p = problem(x, w, bias, targets, ctx->saved_data["ignored"].toInt(), o);
+    const Tensor grad = grads[0].to(at::kFloat).contiguous();
+    if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().requires_grad(false));
+    if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options().requires_grad(false));
+    if (bias.defined() && ctx->needs_input_grad(2)) out[2] = floats(x, bias.sizes());
+    const int64_t size = library.xent_backward_workspace(p.rows, p.categories, p.cols, out[0].defined(), out[1].defined(), out[2].defined());
+    if (size < 0) check((int)size, "tthrml_xent_backward_workspace");
+    const Tensor space = bytes(x, size);
+    check(library.xent_backward(&p, log2_z.const_data_ptr<float>(), grad.const_data_ptr<float>(), grad.dim() ? 1 : 0,
+                                inv_count.defined() ? inv_count.const_data_ptr<float>() : nullptr,
+                                out[0].defined() ? out[0].mutable_data_ptr() : nullptr, p.cols,
+                                out[1].defined() ? out[1].mutable_data_ptr() : nullptr, p.cols, p.dtype,
+                                out[2].defined() ? out[2].mutable_data_ptr<float>() : nullptr, space.mutable_data_ptr(), size,
+                                reinterpret_cast<int32_t*>(ctx->saved_data["error"].toInt()), on.stream()),
+          "tthrml_xent_backward");
+    return out;
+  }
+};
+
+Tensor drop(const Tensor& x, int64_t cut, int64_t seed, int64_t step, const Tensor& step_at, const Tensor& used) {
+  Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
+  if (!x.numel()) return y;
+  const On on(x);
+  const Tensor in = x.contiguous();
+  check(library.dropout(in.const_data_ptr(), dtype_code(x), in.numel(), (int32_t)cut, (uint64_t)seed, (uint32_t)step,
+                        step_at.defined() ? step_at.const_data_ptr() : nullptr,
+                        step_at.defined() && step_at.scalar_type() == at::kLong,
+                        used.defined() ? static_cast<uint32_t*>(used.mutable_data_ptr()) : nullptr, y.mutable_data_ptr(),
+                        on.stream()),
+        "tthrml_dropout");
+  return y;
+}
+
+struct Dropout : Function<Dropout> {
+  // step_at: a pointer, so that it is no argument of the node; it may be undefined
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor* step_at, int64_t cut, int64_t seed, int64_t step) {
+    // a step on the device may have moved on by the time of the backward pass: the kernel leaves what it used
+    Tensor used;
+    if (step_at->defined() && x.numel()) used = at::empty({1}, x.options().dtype(at::kInt).requires_grad(false));
+    ctx->save_for_backward({used});
+    ctx->saved_data["cut"] = cut;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["step"] = step;
+    return drop(x, cut, seed, step, *step_at, used);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    const variable_list s = ctx->get_saved_variables();
+    if (grads[0].defined())
+      out[0] = apply(grads[0], &s[0], ctx->saved_data["cut"].toInt(), ctx->saved_data["seed"].toInt(),
+                     ctx->saved_data["step"].toInt());
+    return out;
+  }
+};
+
+Tensor tensor_or_none(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
+
+}  // namespace
+
+// softmax_cross_entropy(x, weights, bias or None, targets, reduction, ignored, error word) -> the loss; x, weights and targets
+// as checked by the caller (two, two and one dimensions).
+PyObject* softmax_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7) {
+    PyErr_SetString(PyExc_TypeError, "softmax_cross_entropy(x, weights, bias, targets, reduction, ignored, error)");
+    return nullptr;
+  }
+  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+  Tensor bias = tensor_or_none(args[2]);
+  const int64_t reduction = PyLong_AsLongLong(args[4]), ignored = PyLong_AsLongLong(args[5]), error = PyLong_AsLongLong(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (bias.defined()) bias = bias.contiguous();
+  const Tensor targets = THPVariable_Unpack(args[3]).contiguous();
+  if (wants_grad(x) || wants_grad(w) || (bias.defined() && wants_grad(bias)))
+    return THPVariable_Wrap(SoftmaxCrossEntropy::apply(x, w, bias.defined() ? bias : targets, targets, bias.defined(), reduction,
+                                                       ignored, error));
+  XentSaved s;
+  return THPVariable_Wrap(xent_forward(x, w, bias, targets, reduction, ignored, error, s));
+  END_HANDLE_TH_ERRORS
+}
+
+// dropout(x, cut, seed, step, step tensor or None) -> the kept elements, scaled.
+PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "dropout(x, cut, seed, step, step_at)");
+    return nullptr;
+  }
+  const Tensor& x = THPVariable_Unpack(args[0]);
+  const int64_t cut = PyLong_AsLongLong(args[1]), seed = (int64_t)PyLong_AsUnsignedLongLongMask(args[2]),
+                step = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor step_at = tensor_or_none(args[4]);
+  if (wants_grad(x)) return THPVariable_Wrap(Dropout::apply(x, &step_at, cut, seed, step));
+  return THPVariable_Wrap(drop(x, cut, seed, step, step_at, Tensor()));
+  END_HANDLE_TH_ERRORS
+}
+
+// quantize_fp4(x, stream, device) -> (codes [rows, pitch], block scales, scales), an error code, or None.
+PyObject* quantize_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 3 || !THPVariable_Check(args[0])) Py_RETURN_NONE;
+  const Tensor& x = THPVariable_Unpack(args[0]);
+  const long device = PyLong_AsLong(args[2]);
+  void* stream = PyLong_AsVoidPtr(args[1]);
+  if (PyErr_Occurred()) return nullptr;
+  const int32_t code = dtype_code(x);
+  if (!plain_cuda(x, device) || code < 0 || x.dim() != 2 || wants_grad(x) || x.numel() == 0 || x.size(1) > TTHRML_FP4_MAX_COLS ||
+      (x.size(1) > 1 && x.stride(1) != 1))
+    Py_RETURN_NONE;
+  const int64_t rows = x.size(0), cols = x.size(1), pitch = (cols + 31) / 32 * 16;
+  Tensor codes = at::empty({rows, pitch}, x.options().dtype(at::kByte).requires_grad(false));
+  Tensor blocks = bytes(x, library.fp4_scale_bytes(rows, cols)), scale = floats(x, {rows});
+  const int rc = library.fp4_quantize(x.const_data_ptr(), code, rows, cols, x.stride(0), 1, codes.mutable_data_ptr(), pitch,
+                                      blocks.mutable_data_ptr(), scale.mutable_data_ptr<float>(), stream);
+  if (rc) return PyLong_FromLong(rc);
+  PyObject *a = THPVariable_Wrap(codes), *b = THPVariable_Wrap(blocks), *c = THPVariable_Wrap(scale);
+  PyObject* t = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  Py_XDECREF(c);
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// fp4_values(codes, pitch, block scales, scales, columns, stream) -> the float32 matrix, or an error code.
+PyObject* fp4_values(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6) {
+    PyErr_SetString(PyExc_TypeError, "fp4_values(codes, pitch, blocks, scale, cols, stream)");
+    return nullptr;
+  }
+  const Tensor &codes = THPVariable_Unpack(args[0]), &blocks = THPVariable_Unpack(args[2]), &scale = THPVariable_Unpack(args[3]);
+  const int64_t pitch = PyLong_AsLongLong(args[1]), cols = PyLong_AsLongLong(args[4]), rows = codes.size(0);
+  void* stream = PyLong_AsVoidPtr(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor out = floats(codes, {rows, cols});
+  const int rc = library.fp4_values(codes.const_data_ptr(), pitch, blocks.const_data_ptr(), scale.const_data_ptr<float>(), rows, cols,
+                                    out.mutable_data_ptr<float>(), stream);
+  if (rc) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// fp4_product(x, codes, pitch, block scales, scales, columns, bias or None, error word, stream, device) -> the product in x's
+// type, an error code, or None.
+PyObject* fp4_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10 || !THPVariable_Check(args[0]) || !(args[6] == Py_None || THPVariable_Check(args[6]))) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]), &codes = THPVariable_Unpack(args[1]), &blocks = THPVariable_Unpack(args[3]),
+               &scale = THPVariable_Unpack(args[4]);
+  const int64_t pitch = PyLong_AsLongLong(args[2]), K = PyLong_AsLongLong(args[5]), N = codes.size(0);
+  const long device = PyLong_AsLong(args[9]);
+  if (PyErr_Occurred()) return nullptr;
+  const int32_t code = dtype_code(x);
+  if (!plain_cuda(x, device) || code < 0 || x.dim() < 1 || wants_grad(x) || wants_grad(scale) || (x.dim() != 2 && !x.is_contiguous()) ||
+      x.size(-1) != K || N < 1 || x.numel() == 0)
+    Py_RETURN_NONE;
+  if (x.dim() == 2 && K > 1 && x.stride(1) != 1) Py_RETURN_NONE;
+  const float* bias = nullptr;
+  if (args[6] != Py_None) {
+    const Tensor& b = THPVariable_Unpack(args[6]);
+    if (!plain_cuda(b, device) || b.scalar_type() != at::kFloat || b.dim() != 1 || b.size(0) != N || !b.is_contiguous() || wants_grad(b))
+      Py_RETURN_NONE;
+    bias = b.const_data_ptr<float>();
+  }
+  const int64_t M = x.numel() / K;
+  at::DimVector sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = N;
+  Tensor out = at::empty(sizes, x.options().requires_grad(false));
+  const int64_t size = library.fp4_linear_workspace(M, K);
+  Tensor space = bytes(x, size);
+  const int rc = library.fp4_linear(x.const_data_ptr(), code, M, K, x.dim() == 2 ? x.stride(0) : K, 1, space.mutable_data_ptr(), size,
+                                    codes.const_data_ptr(), pitch, blocks.const_data_ptr(), scale.const_data_ptr<float>(), N, bias,
+                                    out.mutable_data_ptr(), code, N, reinterpret_cast<int32_t*>(PyLong_AsVoidPtr(args[7])),
+                                    PyLong_AsVoidPtr(args[8]));
+  if (rc) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+}  // namespace hostcall

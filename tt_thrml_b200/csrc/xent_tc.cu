@@ -25,6 +25,7 @@ namespace {
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kThreads = 320, kEpilogueWarps = 8;
 constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
+constexpr int kChunk = 4;  // 64-wide blocks of K that a logit's sum stays in tensor memory for
 enum : int { kPartials = 0, kGradient = 1, kProduct = 2 };
 
 struct RowTargets {
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
            const __grid_constant__ XentArgs a) {
   using S = XentShape<BN>;
   static_assert(!B_MN || BN == 256, "MN-major halves of B are whole boxes of 64");
+  constexpr int kLength = EPI == kProduct ? 0x40000000 : kChunk;  // blocks of K per accumulation
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStage);
@@ -249,56 +251,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
                              ((uint32_t)(BN >> 3) << 17) | (16u << 24);  // D float32, M = 256
       int64_t used = 0;
-      int it = 0;
+      int it = 0;  // accumulations so far
       bool failed = false;
       for (int u = first; u < a.units && !failed; u += step) {
         int split, mb, sg;
         unit_at(a, u, split, mb, sg);
         const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
-        for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb, ++it) {
-          const int b = it & 1;
-          if (!mbar_wait_all(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
-            if (one) atomicExch(a.error, kErrAccWait);
-            failed = true;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(b * 256);
-          for (int kb = k_first; kb < k_last; ++kb) {
-            const int s = (int)(used % S::kStages);
-            if (!mbar_wait_all(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
-              if (one) atomicExch(a.error, kErrFullWait);
+        for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb) {
+          for (int k0 = k_first; k0 < k_last && !failed; k0 += kLength, ++it) {
+            const int b = it & 1;
+            if (!mbar_wait_all(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
+              if (one) atomicExch(a.error, kErrAccWait);
               failed = true;
               break;
             }
             tc_fence_after();
-            const unsigned char* st = tiles + s * S::kStage;
-            const uint64_t ad = A_MN ? umma_desc_mn128(st) : umma_desc_sw128(st);
-            const uint64_t bd = B_MN ? umma_desc_mn128(st + S::kA) : umma_desc_sw128(st + S::kA);
-            if (one) {
+            const uint32_t d = tmem + (uint32_t)(b * 256);
+            for (int kb = k0; kb < min(k0 + kLength, k_last); ++kb) {
+              const int s = (int)(used % S::kStages);
+              if (!mbar_wait_all(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
+                if (one) atomicExch(a.error, kErrFullWait);
+                failed = true;
+                break;
+              }
+              tc_fence_after();
+              const unsigned char* st = tiles + s * S::kStage;
+              const uint64_t ad = A_MN ? umma_desc_mn128(st) : umma_desc_sw128(st);
+              const uint64_t bd = B_MN ? umma_desc_mn128(st + S::kA) : umma_desc_sw128(st + S::kA);
+              if (one) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)  // 16 of K per MMA: 32 bytes of each row, or two groups of eight rows
-                umma_f16_pair(d, ad + (A_MN ? 128ull : 2ull) * kk, bd + (B_MN ? 128ull : 2ull) * kk, idesc,
-                              (kb > k_first || kk > 0) ? 1u : 0u);
-              umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+                for (int kk = 0; kk < 4; ++kk)  // 16 of K per MMA: 32 bytes of each row, or two groups of eight rows
+                  umma_f16_pair(d, ad + (A_MN ? 128ull : 2ull) * kk, bd + (B_MN ? 128ull : 2ull) * kk, idesc,
+                                (kb > k0 || kk > 0) ? 1u : 0u);
+                umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+              }
+              __syncwarp();
+              ++used;
             }
+            if (one) umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
             __syncwarp();
-            ++used;
+            last_it[b] = it;
           }
-          if (one) umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
-          __syncwarp();
-          last_it[b] = it;
         }
       }
     }
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
     unsigned char* turn = turns + (warp - 2) * 32 * kTurnPitch;
-    int it = 0;
+    int it = 0, tile = 0;
     bool failed = false;
     for (int u = first; u < a.units; u += step) {
       int split, mb, sg;
       unit_at(a, u, split, mb, sg);
+      const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
       const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane;
       float top = -INFINITY, sum = 0.0f;  // kPartials: sum 2^top
       int64_t y = -1;                     // column of the row's target
@@ -318,30 +323,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (EPI == kProduct && a.scaled) factor = factor_of(a.factor) / a.unit;
-      for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb, ++it) {
-        const int b = it & 1;
-        float* bias = biases + b * 256;
+      for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb) {
+        float* bias = biases + (tile++ & 1) * 256;
         if (EPI != kProduct && a.bias) {  // two buffers, so that a warp may run one tile ahead
           const int j = (int)threadIdx.x - 64, n = nb * BN + j;
           if (j < BN) bias[j] = n < a.N ? __ldg(a.bias + n) : 0.0f;
           asm volatile("bar.sync 1, 256;" ::: "memory");
         }
-        if (!failed && !mbar_wait_warp(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
+        constexpr int kMine = EPI == kProduct ? 32 : BN / 2;  // logits of this thread, summed over the accumulations
+        float acc[kMine];
+        if (EPI != kProduct) {
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) acc[j] = 0.0f;
+          for (int k0 = k_first; k0 < k_last && !failed; k0 += kLength, ++it) {
+            const int b = it & 1;
+            if (!mbar_wait_warp(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
+              if (lane == 0) atomicExch(a.error, kErrAccWait);
+              failed = true;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < kMine / 32; ++q) {
+              float v[32];
+              tmem_load32(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * (BN / 2) + q * 32), v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) acc[q * 32 + j] += v[j];
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader(&acc_empty[b]);
+          }
+        } else if (!failed && !mbar_wait_warp(&acc_full[it & 1], (uint32_t)(it >> 1) & 1u)) {
           if (lane == 0) atomicExch(a.error, kErrAccWait);
           failed = true;
         }
         if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
         tc_fence_after();
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2) && nb * BN + c < a.N; c += 32) {
-          const int n = nb * BN + c, live = min(32, a.N - n);
+#pragma unroll
+        for (int q = 0; q < BN / 64; ++q) {
+          const int c = half * (BN / 2) + q * 32, n = nb * BN + c, live = min(32, a.N - n);
+          if (live <= 0) break;
           float v[32];
-          tmem_load32(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
-          if (EPI != kProduct) {
+          if (EPI == kProduct) {
+            tmem_load32(tmem + (uint32_t)((it & 1) * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = acc[(kMine == 32 ? 0 : q * 32) + j];
             if (a.bias) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const float4 w = reinterpret_cast<const float4*>(bias + c)[q];
-                v[4 * q] += w.x, v[4 * q + 1] += w.y, v[4 * q + 2] += w.z, v[4 * q + 3] += w.w;
+              for (int i = 0; i < 8; ++i) {
+                const float4 w = reinterpret_cast<const float4*>(bias + c)[i];
+                v[4 * i] += w.x, v[4 * i + 1] += w.y, v[4 * i + 2] += w.z, v[4 * i + 3] += w.w;
               }
             }
             if (live < 32) {
@@ -409,9 +442,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();  // the next TMEM load is a warp's
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_leader(&acc_empty[b]);
+        if (EPI == kProduct) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader(&acc_empty[it & 1]);
+          ++it;
+        }
       }
       if (EPI == kPartials && m < a.M) a.part[(int64_t)m * a.slots + 2 * sg + half] = make_float2(top, sum);
     }
@@ -442,7 +478,7 @@ struct LossArgs {
   int64_t rows, categories;
   int32_t slots, reduction;  // 0: none, 1: mean over the rows that count, 2: sum
   float *log2_z, *loss;      // [rows]
-  float* reduced;            // the loss, and 1 / the rows that count (1 at least)
+  float *total, *inv_count;  // the reduced loss, and 1 / the rows that count (1 at least) or 1
   uint32_t* counter;
 };
 __global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
@@ -507,8 +543,8 @@ __global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
   if (threadIdx.x == 0) {
     for (int i = 1; i < 8; ++i) sum += sums[i], count += counts[i];
     const double n = a.reduction == 1 ? (double)(count > 0 ? count : 1) : 1.0;
-    a.reduced[0] = (float)(sum / n);
-    a.reduced[1] = (float)(1.0 / n);
+    *a.total = (float)(sum / n);
+    *a.inv_count = (float)(1.0 / n);
   }
 }
 
@@ -759,12 +795,12 @@ extern "C" int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categorie
   return rc ? rc : p.bytes;
 }
 
-extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* row_loss, float* reduced, int32_t reduction,
-                                   void* workspace, int64_t workspace_bytes, int32_t* error, void* stream) {
+extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* row_loss, float* loss, float* inv_count,
+                                   int32_t reduction, void* workspace, int64_t workspace_bytes, int32_t* error, void* stream) {
   using namespace tthrml;
   int rc = check_problem("tthrml_xent_forward", p);
   if (rc) return rc;
-  if (!log2_z || !row_loss || !workspace || !error || reduction < 0 || reduction > 2 || (reduction && !reduced)) {
+  if (!log2_z || !row_loss || !workspace || !error || reduction < 0 || reduction > 2 || (reduction && (!loss || !inv_count))) {
     set_error("tthrml_xent_forward: NULL argument or unknown reduction %d", (int)reduction);
     return TTHRML_ERR_ARG;
   }
@@ -804,7 +840,8 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.error = error;
   rc = launch_logits<kPartials>(f.bn, ma, mb, a, st);
   if (rc) return rc;
-  LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, log2_z, row_loss, reduced, a.counter};
+  LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, log2_z, row_loss, loss, inv_count,
+                a.counter};
   void* params[1] = {(void*)&l};
   return launch_clusters((const void*)k_xent_loss, (unsigned)((p->rows + 7) / 8), 1, 256, 0, params, st, "k_xent_loss launch",
                          true);

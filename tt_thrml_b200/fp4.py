@@ -20,6 +20,8 @@ from __future__ import annotations
 
 from . import _native as nat
 from .quantized import (
+    _error_addresses,
+    current_device,
     dtype_code,
     error_word,
     mark_written,
@@ -117,17 +119,12 @@ class Fp4Rows:
 
     def dequantize(self):
         """The float32 matrix that the codes and scales stand for."""
-        torch = _torch()
-        rows, cols = self.shape
-        out = torch.empty((rows, cols), dtype=torch.float32, device=self.device)
-        if rows:
-            with on_device(self.device):
-                nat.check(
-                    nat.lib().tthrml_fp4_values(self.codes.data_ptr(), self.pitch, self.blocks.data_ptr(),
-                                                self.scale.data_ptr(), rows, cols, out.data_ptr(), raw_stream(self.index)),
-                    "tthrml_fp4_values",
-                )
-        return out
+        with on_device(self.device):
+            made = nat.bound_hostcall().fp4_values(self.codes, self.pitch, self.blocks, self.scale, self.cols,
+                                                   raw_stream(self.index))
+        if type(made) is int:
+            nat.check(made, "tthrml_fp4_values")
+        return made
 
 
 def _readable(x):
@@ -147,6 +144,15 @@ def quantize_fp4(x) -> Fp4Rows:
     other are copied first).
     """
     torch = _torch()
+    if isinstance(x, torch.Tensor) and x.is_cuda and current_device() == x.get_device():  # the plain case
+        index = x.get_device()
+        nat.bind_device(index)
+        made = nat.bound_hostcall().quantize_fp4(x, raw_stream(index), index)
+        if type(made) is int:
+            nat.check(made, "tthrml_fp4_quantize")
+        if made is not None:
+            (rows, cols), (codes, blocks, scale) = x.shape, made
+            return Fp4Rows.__new__(Fp4Rows)._hold(codes[:, : -(-cols // 2)], codes.shape[1], blocks, scale, cols)
     require_cuda("x", x)
     code = dtype_code(x.dtype)
     if code is None or x.dim() != 2:
@@ -177,6 +183,17 @@ def fp4_product(x, weights: Fp4Rows, *, bias=None, out_dtype=None, out=None):
     to write, its rows dense.  The sums are float32 on the tensor cores; the result
     is the same every time.
     """
+    if out is None and out_dtype is None and type(weights) is Fp4Rows:
+        index = weights.index
+        word = _error_addresses.get(index)
+        if word is not None and current_device() == index:  # the plain case, from the second call on
+            nat.bind_device(index)
+            y = nat.bound_hostcall().fp4_product(x, weights.codes, weights.pitch, weights.blocks, weights.scale, weights.cols,
+                                                 bias, word, raw_stream(index), index)
+            if y is not None:
+                if type(y) is int:
+                    nat.check(y, "tthrml_fp4_linear")
+                return y
     torch = _torch()
     if not isinstance(weights, Fp4Rows):
         raise TypeError(f"weights must be Fp4Rows (see quantize_fp4), got {type(weights).__name__}")

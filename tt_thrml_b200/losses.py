@@ -15,112 +15,15 @@ check_operator_errors reports.
 from __future__ import annotations
 
 from . import _native as nat
-from .moments import _lay_out
-from .quantized import dtype_code, error_word, on_device, raw_stream, require_cuda
+from .quantized import _error_addresses, dtype_code, error_word, require_cuda
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-_function = None
 
 
 def _torch():
     import torch
 
     return torch
-
-
-class _Call:
-    """What the passes over one batch share: the problem as the library takes it, and what it points to."""
-
-    def __init__(self, x, weights, targets, bias, ignored, stream):
-        torch = _torch()
-        dev = x.device
-        laid, held = _lay_out([x, weights], dev, stream)
-        bias = None if bias is None else bias.contiguous()
-        targets = targets.contiguous()
-        self.held = (x, weights, targets, bias, held)
-        p = self.problem = nat.Xent()
-        p.x, p.x_ld = laid[0]
-        p.w, p.w_ld = laid[1]
-        p.targets = targets.data_ptr()
-        p.bias = None if bias is None else bias.data_ptr()
-        p.rows, p.cols = x.shape
-        p.categories = weights.shape[0]
-        p.ignored = ignored
-        p.dtype = dtype_code(x.dtype)
-        p.wide_targets = 1 if targets.dtype == torch.int64 else 0
-
-
-def _workspace(size: int, dev, what: str):
-    torch = _torch()
-    if size < 0:
-        nat.check(size, what)
-    return torch.empty(max(size, 16), dtype=torch.uint8, device=dev), size
-
-
-def _forward(call, reduction):
-    """(losses of the rows, (reduced loss, 1 / rows that count) or None, log2 of the normalisers)."""
-    torch = _torch()
-    p, dev = call.problem, call.held[0].device
-    lib = nat.lib()
-    space, size = _workspace(lib.tthrml_xent_forward_workspace(p.rows, p.categories), dev, "tthrml_xent_forward_workspace")
-    rows = torch.empty((2, p.rows), dtype=torch.float32, device=dev)
-    reduced = torch.empty(2, dtype=torch.float32, device=dev) if reduction else None
-    nat.check(
-        lib.tthrml_xent_forward(p, rows[0].data_ptr(), rows[1].data_ptr(), nat.ptr(reduced), reduction, space.data_ptr(), size,
-                                error_word(dev).data_ptr(), raw_stream(dev.index)),
-        "tthrml_xent_forward",
-    )
-    return rows[1], reduced, rows[0]
-
-
-def backward(call, log2_z, grad, inv_count, dx, dw, db) -> None:
-    """Gradients of sum_t weight_t loss_t into dx, dw (one type, dense rows) and db, each a tensor or None.  The weights are
-    grad * inv_count (one element each, inv_count may be None), or grad's elements, one per row."""
-    p, dev = call.problem, call.held[0].device
-    lib = nat.lib()
-    space, size = _workspace(
-        lib.tthrml_xent_backward_workspace(p.rows, p.categories, p.cols, dx is not None, dw is not None, db is not None), dev,
-        "tthrml_xent_backward_workspace")
-    code = dtype_code(next((t.dtype for t in (dx, dw) if t is not None), call.held[0].dtype))
-    nat.check(
-        lib.tthrml_xent_backward(p, log2_z.data_ptr(), grad.data_ptr(), 1 if grad.dim() else 0, nat.ptr(inv_count), nat.ptr(dx),
-                                 p.cols, nat.ptr(dw), p.cols, code, nat.ptr(db), space.data_ptr(), size,
-                                 error_word(dev).data_ptr(), raw_stream(dev.index)),
-        "tthrml_xent_backward",
-    )
-
-
-def _autograd_function():
-    global _function
-    if _function is not None:
-        return _function
-    torch = _torch()
-
-    class SoftmaxCrossEntropy(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, weights, bias, targets, reduction, ignored):
-            with on_device(x.device):
-                call = _Call(x, weights, targets, bias, ignored, raw_stream(x.device.index))
-                rows, reduced, log2_z = _forward(call, reduction)
-            ctx.call, ctx.reduction = call, reduction
-            # the tensors themselves, so that a change in place before the backward pass is noticed
-            ctx.save_for_backward(x, weights, bias, targets, log2_z, reduced)
-            return rows if reduction == 0 else reduced[0]
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, grad):
-            x, weights, bias, _, log2_z, reduced = ctx.saved_tensors
-            need_x, need_w, need_b = ctx.needs_input_grad[:3]
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-            dw = torch.empty(weights.shape, dtype=weights.dtype, device=x.device) if need_w else None
-            db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if need_b else None
-            with on_device(x.device):
-                backward(ctx.call, log2_z, grad.contiguous(), None if reduced is None else reduced[1], dx, dw, db)
-            return dx, dw, db, None, None, None
-
-    _function = SoftmaxCrossEntropy
-    return _function
 
 
 def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", ignore_index=-100):
@@ -171,10 +74,11 @@ def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", i
     if rows == 0:  # nothing counts
         zero = x.sum(-1).float() + weights[:0].sum().float() + (0.0 if bias is None else bias[:0].sum())
         return zero if reduction == "none" else zero.sum()
-    error_word(dev)  # made before the first capture
-    flat = x.reshape(rows, K)
-    loss = _autograd_function().apply(flat, weights, bias, targets.reshape(rows), _REDUCTIONS[reduction], int(ignore_index))
-    return loss.reshape(lead) if reduction == "none" else loss
+    word = _error_addresses.get(dev.index) or error_word(dev).data_ptr()
+    flat = x if x.dim() == 2 else x.reshape(rows, K)
+    loss = nat.bound_hostcall().softmax_cross_entropy(flat, weights, bias, targets if targets.dim() == 1 else targets.reshape(rows),
+                                                      _REDUCTIONS[reduction], int(ignore_index), word)
+    return loss.reshape(lead) if reduction == "none" and len(lead) != 1 else loss
 
 
 __all__ = ["softmax_cross_entropy"]

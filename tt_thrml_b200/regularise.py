@@ -11,54 +11,13 @@ goes with it, so means are kept exactly.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import dtype_code, on_device, raw_stream, require_cuda
-
-_function = None
+from .quantized import dtype_code, require_cuda
 
 
 def _torch():
     import torch
 
     return torch
-
-
-def _launch(x, cut, seed, step, step_at, used):
-    torch = _torch()
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    if x.numel():
-        with on_device(x.device):
-            nat.check(
-                nat.lib().tthrml_dropout(x.data_ptr(), dtype_code(x.dtype), x.numel(), cut, seed, step, nat.ptr(step_at),
-                                         1 if step_at is not None and step_at.dtype == torch.int64 else 0, nat.ptr(used),
-                                         y.data_ptr(), raw_stream(x.device.index)),
-                "tthrml_dropout",
-            )
-    return y
-
-
-def _autograd_function():
-    global _function
-    if _function is not None:
-        return _function
-    torch = _torch()
-
-    class Dropout(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, cut, seed, step, step_at):
-            # a step on the device may have moved on by the time of the backward pass: the kernel leaves what it used
-            used = None if step_at is None else torch.empty(1, dtype=torch.int32, device=x.device)
-            ctx.draws = (cut, seed, step)
-            ctx.save_for_backward(used if x.numel() else None)
-            return _launch(x, cut, seed, step, step_at, used)
-
-        @staticmethod
-        def backward(ctx, grad):
-            (used,) = ctx.saved_tensors
-            return Dropout.apply(grad, *ctx.draws, used), None, None, None, None
-
-    _function = Dropout
-    return _function
 
 
 def dropout(x, p=0.5, *, seed, step=0):
@@ -92,7 +51,7 @@ def dropout(x, p=0.5, *, seed, step=0):
         step = int(step)
         if not 0 <= step < 2**32:
             raise ValueError(f"step must be between 0 and 2^32 - 1, got {step}")
-    return _autograd_function().apply(x, round(65536 * p), seed, step, step_at)
+    return nat.bound_hostcall().dropout(x, round(65536 * p), seed, step, step_at)
 
 
 __all__ = ["dropout"]
