@@ -124,3 +124,8 @@ def run_product(tt, m, n, k, dtype, bias, seed):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 def test_products(tt, m, n, k, dtype):
     run_product(tt, m, n, k, dtype, (m + n) % 2 == 0, m + n + k)
+
+
+@pytest.mark.parametrize("m,n,k", [(4100, 4203, 600), (2560, 5120, 1280), (8192, 300, 257)])
+def test_products_of_many_tiles(tt, m, n, k):
+    run_product(tt, m, n, k, "bf16", True, 3)

@@ -10,6 +10,12 @@
 // blocks.  Warp 0 loads (TMA, columns and rows behind the ends read as zeros), warp 1 copies scales and multiplies, then all
 // eight warps move the accumulator to shared memory, and CTA r of the cluster adds the S partial tiles of rows r, r + S, ...
 // in the order of the CTAs, scales and stores them as whole rows.
+//
+// k_fp4_pair: persistent clusters of two CTAs walk 256 x 256 tiles (tcgen05 cta_group::2): an SM takes in at most 68 bytes a
+// clock, and a 128 x 256 tile of one CTA needs 108 at the full MMA rate, a CTA of a pair 76 (16 KB of either operand, the
+// scales of its rows and of all 256 units per 512 clocks).  The accumulator (256 columns) and the scales leave no room for a
+// second one: the epilogue's eight warps take a finished tile into registers at once, free the accumulator for the next tile's
+// MMAs and then scale and store.
 #include "fp4_common.cuh"
 #include "tc_common.cuh"
 
@@ -29,6 +35,7 @@ struct Fp4Args {
   int32_t M, N;
   int32_t num_k;         // 256-column blocks of K
   int32_t box_m;         // rows per A load (16, 32, 64 or 128)
+  int32_t group, align;  // pairs: raster, bytes that the rows of `out` are aligned to
   int* error;
 };
 
@@ -284,6 +291,222 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (split > 1) cluster_sync_all();  // no CTA leaves while another still reads its shared memory
 }
 
+// ---------------------------------------------------------------------------
+// CTA-pair kernel
+// ---------------------------------------------------------------------------
+constexpr int kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf + 3 * kScales, kPairStages = 5, kPairThreads = 320, kPairWarps = 8;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + 2 * 512 * 4 /*scales and biases of two tiles' units*/ +
+                          kPairWarps * 32 * kTurnPitch;
+
+__device__ __forceinline__ void umma_fp4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t a_scales,
+                                              uint32_t b_scales, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc_fp4(256, 256)), "r"(a_scales), "r"(b_scales), "r"(accumulate));
+}
+// From each CTA's own shared memory into its own tensor memory.
+__device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc));
+}
+// Tile t -> (m, n) block: `group` row blocks at a time, row-fastest, so that the tiles in flight share panels in L2.
+__device__ __forceinline__ void pair_tile(const Fp4Args& a, int t, int& mb, int& nb) {
+  const int m_blocks = (a.M + 255) / 256, n_blocks = (a.N + 255) / 256;
+  const int per = a.group * n_blocks, g = t / per, w = t - g * per;
+  const int rows = min(a.group, m_blocks - g * a.group);
+  mb = g * a.group + w % rows;
+  nb = w / rows;
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+    k_fp4_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+               const __grid_constant__ Fp4Args a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + kPairStages * kPairStage);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  float* unit_scales = reinterpret_cast<float*>(tiles + kPairStages * kPairStage + 256);  // [2][scales 256, biases 256]
+  unsigned char* turns = reinterpret_cast<unsigned char*>(unit_scales + 2 * 512);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int n_tiles = ((a.M + 255) / 256) * ((a.N + 255) / 256);
+  const int first = (int)cluster_id_x(), step = (int)n_clusters_x();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * kPairWarps);  // every epilogue warp of both CTAs
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers exist before either signals the other
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  wait_for_previous_kernel();
+  int last_it = -1;
+
+  if (warp == 0) {  // producer (both CTAs): this CTA's halves of the A and B slices, its rows' scales and all units'
+    const bool one = elect_one();
+    int64_t issued = 0;
+    bool failed = false;
+    for (int t = first; t < n_tiles && !failed; t += step) {
+      int mb, nb;
+      pair_tile(a, t, mb, nb);
+      for (int kb = 0; kb < a.num_k; ++kb) {
+        const int s = (int)(issued % kPairStages);
+        if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / kPairStages) & 1u) ^ 1u)) {
+          if (one) atomicExch(a.error, kErrEmptyWait);
+          failed = true;
+          break;
+        }
+        if (one) {
+          if (leader) mbar_expect_tx(&full[s], 2 * kPairStage);  // the stage's bytes of both CTAs
+          unsigned char* st = tiles + s * kPairStage;
+          const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
+          tma_load_2d_pair(st, &map_a, bar, kb * 128, mb * 256 + (int)rank * 128);
+          tma_load_2d_pair(st + kPairHalf, &map_b, bar, kb * 128, nb * 256 + (int)rank * 128);
+          st += 2 * kPairHalf;  // row blocks behind the last read as zeros
+          tma_load_2d_pair(st, &map_sa, bar, 0, 2 * ((mb * 2 + (int)rank) * a.num_k + kb));
+          tma_load_2d_pair(st + kScales, &map_sb, bar, 0, 2 * (nb * 2 * a.num_k + kb));
+          tma_load_2d_pair(st + 2 * kScales, &map_sb, bar, 0, 2 * ((nb * 2 + 1) * a.num_k + kb));
+        }
+        __syncwarp();
+        ++issued;
+      }
+    }
+    // every stage this CTA filled has been consumed (released by the leader's MMAs) before exit
+    for (int64_t j = issued > kPairStages ? issued - kPairStages : 0; j < issued; ++j)
+      if (!mbar_wait_all(&empty[j % kPairStages], (uint32_t)(j / kPairStages) & 1u) && one) atomicExch(a.error, kErrEmptyWait);
+  } else if (warp == 1) {
+    if (leader) {  // MMA issue: the leader only
+      const bool one = elect_one();
+      const uint32_t a_scales = tmem + 256, b_scales = a_scales + 16;
+      int64_t used = 0;
+      int it = 0;
+      bool failed = false;
+      for (int t = first; t < n_tiles && !failed; t += step, ++it) {
+        if (!mbar_wait_all(acc_empty, ((uint32_t)it & 1u) ^ 1u)) {
+          if (one) atomicExch(a.error, kErrAccWait);
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < a.num_k; ++kb) {
+          const int s = (int)(used % kPairStages);
+          if (!mbar_wait_all(&full[s], (uint32_t)(used / kPairStages) & 1u)) {
+            if (one) atomicExch(a.error, kErrFullWait);
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          const unsigned char* st = tiles + s * kPairStage;
+          const uint64_t ad = umma_desc_sw128(st), bd = umma_desc_sw128(st + kPairHalf), sd = scales_desc(st + 2 * kPairHalf);
+          if (one) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {  // 512 bytes of scales: 32 in the descriptor's units of 16
+              copy_scales_pair(a_scales + 4 * kk, sd + 32ull * kk);
+              copy_scales_pair(b_scales + 8 * kk, sd + 128ull + 32ull * kk);
+              copy_scales_pair(b_scales + 8 * kk + 4, sd + 256ull + 32ull * kk);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // K = 64 columns, 32 bytes, per MMA
+              umma_fp4_pair(tmem, ad + 2ull * kk, bd + 2ull * kk, a_scales + 4 * kk, b_scales + 8 * kk,
+                            (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+          }
+          __syncwarp();
+          ++used;
+        }
+        if (one) umma_commit_pair(acc_full);  // both CTAs' accumulator halves complete
+        __syncwarp();
+        last_it = it;
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* turn = turns + (warp - 2) * 32 * kTurnPitch;
+    int it = 0;
+    bool failed = false;
+    for (int t = first; t < n_tiles; t += step, ++it) {
+      int mb, nb;
+      pair_tile(a, t, mb, nb);
+      const int m0 = mb * 256 + (int)rank * 128 + quad * 32;
+      const float sx = m0 + lane < a.M ? __ldg(a.x_scale + m0 + lane) : 0.0f;
+      // the tile's scales and biases, a unit per thread; two buffers, so that a warp may run one tile ahead
+      float* sw = unit_scales + (it & 1) * 512;
+      {
+        const int j = (int)threadIdx.x - 64, n = nb * 256 + j;
+        sw[j] = n < a.N ? __ldg(a.w_scale + n) : 0.0f;
+        sw[256 + j] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      if (!failed && !mbar_wait_warp(acc_full, (uint32_t)it & 1u)) {
+        if (lane == 0) atomicExch(a.error, kErrAccWait);
+        failed = true;
+      }
+      if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
+      tc_fence_after();
+      float acc[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128 + q * 32), acc[q]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(acc_empty);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = half * 128 + q * 32, n = nb * 256 + c, live = min(32, a.N - n);
+        if (live <= 0) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 w = reinterpret_cast<const float4*>(sw + c)[i];
+          acc[q][4 * i] = __fmul_rn(acc[q][4 * i], __fmul_rn(sx, w.x));
+          acc[q][4 * i + 1] = __fmul_rn(acc[q][4 * i + 1], __fmul_rn(sx, w.y));
+          acc[q][4 * i + 2] = __fmul_rn(acc[q][4 * i + 2], __fmul_rn(sx, w.z));
+          acc[q][4 * i + 3] = __fmul_rn(acc[q][4 * i + 3], __fmul_rn(sx, w.w));
+        }
+        if (a.bias) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 b = reinterpret_cast<const float4*>(sw + 256 + c)[i];
+            acc[q][4 * i] = __fadd_rn(acc[q][4 * i], b.x);
+            acc[q][4 * i + 1] = __fadd_rn(acc[q][4 * i + 1], b.y);
+            acc[q][4 * i + 2] = __fadd_rn(acc[q][4 * i + 2], b.z);
+            acc[q][4 * i + 3] = __fadd_rn(acc[q][4 * i + 3], b.w);
+          }
+        }
+        store_values(acc[q], a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m0, a.M, live, a.align);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1 && leader) {
+    // every MMA the pair issued has completed (in both CTAs' TMEM) before TMEM is freed
+    if (lane == 0 && last_it >= 0) (void)mbar_wait(acc_full, (uint32_t)last_it & 1u);
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA frees TMEM or exits while the other may still signal it
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
 // Tensor map of a byte matrix [rows][cols] with rows `pitch` bytes apart, in (box_rows x 128) tiles, 128-byte swizzle.
 int make_map_codes(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, uint32_t box_rows) {
   EncodeTiledFn fn;
@@ -423,7 +646,28 @@ int fp4_product(const void* x_codes, int64_t x_pitch, const void* x_blocks, cons
   if ((rc = consider<64>(a, best, bn, split)) || (rc = consider<128>(a, best, bn, split)) ||
       (rc = consider<256>(a, best, bn, split)))
     return rc;
-  CUtensorMap ma, msa, msb;
+  CUtensorMap ma, mb, msa, msb;
+  // the pair kernel overlaps a tile's store with the next tile's loop
+  ClusterFit fit;
+  rc = cluster_fit((const void*)k_fp4_pair, 2, kPairThreads, kPairSmem, &fit);
+  if (rc) return rc;
+  const int64_t m_pairs = (rows + 255) / 256, pairs = m_pairs * ((units + 255) / 256);
+  const int64_t at_once = pairs < fit.clusters ? pairs : fit.clusters;
+  if ((pairs + fit.clusters - 1) / fit.clusters * (a.num_k * block_clocks(kPairStage, 2 * at_once, 512) + 1000) + 13700 < best) {
+    rc = make_map_codes(&ma, x_codes, rows, (cols + 1) / 2, x_pitch, 128u);
+    if (rc == TTHRML_OK) rc = make_map_codes(&mb, w_codes, units, (cols + 1) / 2, w_pitch, 128u);
+    if (rc == TTHRML_OK) rc = make_map_scales(&msa, x_blocks, rows, cols);
+    if (rc == TTHRML_OK) rc = make_map_scales(&msb, w_blocks, units, cols);
+    if (rc) return rc;
+    const uint64_t alignment = (uint64_t)(uintptr_t)out | (uint64_t)(out_ld * dtype_bytes(out_dtype));  // of the rows
+    a.align = alignment % 16 == 0 ? 16 : (alignment % 8 == 0 ? 8 : (alignment % 4 == 0 ? 4 : 2));
+    int64_t g = 1;  // about square rectangles of the tiles in flight
+    while ((g + 1) * (g + 1) <= fit.clusters) ++g;
+    a.group = (int32_t)(g < m_pairs ? g : m_pairs);
+    void* params[5] = {(void*)&ma, (void*)&mb, (void*)&msa, (void*)&msb, (void*)&a};
+    return launch_clusters((const void*)k_fp4_pair, (unsigned)(2 * at_once), 2, kPairThreads, kPairSmem, params, st,
+                           "k_fp4_pair launch", early);
+  }
   rc = make_map_codes(&ma, x_codes, rows, (cols + 1) / 2, x_pitch, (uint32_t)a.box_m);
   if (rc == TTHRML_OK) rc = make_map_scales(&msa, x_blocks, rows, cols);
   if (rc == TTHRML_OK) rc = make_map_scales(&msb, w_blocks, units, cols);

@@ -117,42 +117,6 @@ __device__ __forceinline__ float column_sums(float (&v)[32]) {
   return v[0];
 }
 
-// 32 values of each of a warp's rows m0 + lane, from column n on, to 16-bit or float32 rows.
-__device__ __forceinline__ void store_values(const float (&v)[32], int32_t dtype, unsigned char* turn, unsigned char* out,
-                                             int64_t ld, int64_t n, int m0, int M, int live, int align) {
-  if (dtype == TTHRML_DT_F32) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint4 w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        w[q] = make_uint4(__float_as_uint(v[16 * half + 4 * q]), __float_as_uint(v[16 * half + 4 * q + 1]),
-                          __float_as_uint(v[16 * half + 4 * q + 2]), __float_as_uint(v[16 * half + 4 * q + 3]));
-      const int left = min(16, live - 16 * half);
-      if (left > 0) store_rows<4>(w, turn, out, ld * 4, 4 * (n + 16 * half), m0, M, 4 * left, align);
-    }
-    return;
-  }
-  uint4 w[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t p[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float lo = v[8 * q + 2 * j], hi = v[8 * q + 2 * j + 1];
-      if (dtype == TTHRML_DT_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        p[j] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        p[j] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    w[q] = make_uint4(p[0], p[1], p[2], p[3]);
-  }
-  store_rows<4>(w, turn, out, ld * 2, 2 * n, m0, M, 2 * live, align);
-}
-
 template <int EPI, bool A_MN, bool B_MN, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     k_xent(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
