@@ -108,6 +108,33 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The same without the wait: v holds its values only after tmem_wait.
+__device__ __forceinline__ void tmem_load32_async(uint32_t taddr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr));
+}
+// Waits for the warp's loads; every use of v stays behind it.
+template <int N>
+__device__ __forceinline__ void tmem_wait(float (&v)[N][32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+    asm volatile(""
+                 : "+f"(v[q][0]), "+f"(v[q][1]), "+f"(v[q][2]), "+f"(v[q][3]), "+f"(v[q][4]), "+f"(v[q][5]), "+f"(v[q][6]),
+                   "+f"(v[q][7]), "+f"(v[q][8]), "+f"(v[q][9]), "+f"(v[q][10]), "+f"(v[q][11]), "+f"(v[q][12]),
+                   "+f"(v[q][13]), "+f"(v[q][14]), "+f"(v[q][15]), "+f"(v[q][16]), "+f"(v[q][17]), "+f"(v[q][18]),
+                   "+f"(v[q][19]), "+f"(v[q][20]), "+f"(v[q][21]), "+f"(v[q][22]), "+f"(v[q][23]), "+f"(v[q][24]),
+                   "+f"(v[q][25]), "+f"(v[q][26]), "+f"(v[q][27]), "+f"(v[q][28]), "+f"(v[q][29]), "+f"(v[q][30]),
+                   "+f"(v[q][31]));
+}
+
 constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit of a shared::cluster address
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -240,6 +267,57 @@ __device__ __forceinline__ void store_values(const float (&v)[32], int32_t dtype
   store_rows<4>(w, turn, out, ld * 2, 2 * n, m0, M, 2 * live, align);
 }
 
+// Rows of 128 bytes on their way out through a bulk tensor store: a warp's 32 rows (a row per lane) in a buffer of 4096 bytes
+// (1024-byte aligned), in the 128-byte swizzle, which both the lanes' writes and the store's reads spread over all banks.  The
+// lane that issues the stores waits for their reads before a buffer is written again.
+constexpr int kOutBytes = 32 * 128;
+__device__ __forceinline__ void stage_row(uint32_t buffer, const uint4 (&w)[8]) {
+  const uint32_t lane = threadIdx.x & 31, row = buffer + lane * 128;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + 16 * (j ^ (lane & 7))), "r"(w[j].x), "r"(w[j].y), "r"(w[j].z),
+                 "r"(w[j].w)
+                 : "memory");
+}
+__device__ __forceinline__ void send_rows(const CUtensorMap* map, uint32_t buffer, int column, int row) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(buffer), "r"(column),
+                 "r"(row)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+// All but the last `PENDING` stores of this warp have read their buffers.
+template <int PENDING>
+__device__ __forceinline__ void sent_rows_read() {
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PENDING) : "memory");
+  __syncwarp();
+}
+__device__ __forceinline__ void sent_rows_done() {
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  __syncwarp();
+}
+// Eight 16-byte words of 64 16-bit values, or of 32 float32 ones.
+__device__ __forceinline__ void pack_row(const float* v, int32_t dtype, uint4 (&w)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (dtype == TTHRML_DT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * q + 2 * j], v[8 * q + 2 * j + 1]);
+        p[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(v[8 * q + 2 * j], v[8 * q + 2 * j + 1]);
+        p[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    w[q] = make_uint4(p[0], p[1], p[2], p[3]);
+  }
+}
+
 // --- host side --------------------------------------------------------------
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -262,6 +340,23 @@ int encode_fn(EncodeTiledFn* out) {
   }
   *out = fn;
   return TTHRML_OK;
+}
+
+// Tensor map of an output matrix [rows][cols] with rows `ld` elements apart for stores of 32 rows x 128 bytes; false where
+// its rows do not start on 16 bytes (or are too far apart).
+inline bool make_out_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int32_t dtype) {
+  const int64_t bytes = dtype == TTHRML_DT_F32 ? 4 : 2;
+  EncodeTiledFn fn;
+  if ((uintptr_t)base % 16 || ld * bytes % 16 || ld * bytes >= (int64_t)1 << 40 || encode_fn(&fn)) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * bytes)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), 32u};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == TTHRML_DT_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == TTHRML_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Clocks of a block of the main loop (128 bytes of K) that brings `bytes` into each of `ctas` SMs at once: an SM takes in 68
