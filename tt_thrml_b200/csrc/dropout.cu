@@ -28,9 +28,15 @@ struct DropoutArgs {
   uint32_t* step_used;  // where it is left for the backward pass, or NULL
 };
 
-// Eight elements with those below the cut cleared.
-__device__ __forceinline__ uint2 keep_pair(uint32_t bits, uint32_t cut) {
-  return make_uint2((bits & 0xFFFFu) >= cut ? 0xFFFFFFFFu : 0u, (bits >> 16) >= cut ? 0xFFFFFFFFu : 0u);
+// Philox4x32-10 with 64-bit products and the round keys at hand: four instructions a round.
+__device__ __forceinline__ u32x4 draw8(int64_t g, uint32_t step, const PhiloxKeys& k) {
+  u32x4 c = {(uint32_t)g, (uint32_t)(g >> 32), step, kSaltDropout};
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c.x, p1 = (uint64_t)0xCD9E8D57u * c.z;
+    c = u32x4{(uint32_t)(p1 >> 32) ^ c.y ^ k.a[r], (uint32_t)p1, (uint32_t)(p0 >> 32) ^ c.w ^ k.b[r], (uint32_t)p0};
+  }
+  return c;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t packed_pair(float lo, float hi);
@@ -45,20 +51,21 @@ __device__ __forceinline__ uint32_t packed_pair<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename T>
-__device__ __forceinline__ Vec8<T> dropped(const Vec8<T>& v, const u32x4& draw, uint32_t cut, float scale) {
+__device__ __forceinline__ Vec8<T> dropped(const Vec8<T>& v, const u32x4& draw, uint32_t cut16, bool all, float scale) {
   float f[8];
   unpack8(v, f);
   Vec8<T> o;
   uint32_t* w = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const uint2 keep = keep_pair(word_of(draw, q), cut);
-    const float lo = __fmul_rn(f[2 * q], scale), hi = __fmul_rn(f[2 * q + 1], scale);
+    const uint32_t bits = word_of(draw, q);  // a half against the cut: shifted to the top, whole words
+    const float lo = (bits << 16) >= cut16 && !all ? __fmul_rn(f[2 * q], scale) : 0.0f;
+    const float hi = bits >= cut16 && !all ? __fmul_rn(f[2 * q + 1], scale) : 0.0f;
     if constexpr (sizeof(T) == 4) {
-      w[2 * q] = __float_as_uint(lo) & keep.x;
-      w[2 * q + 1] = __float_as_uint(hi) & keep.y;
+      w[2 * q] = __float_as_uint(lo);
+      w[2 * q + 1] = __float_as_uint(hi);
     } else {
-      w[q] = packed_pair<T>(lo, hi) & ((keep.x & 0xFFFFu) | (keep.y & 0xFFFF0000u));
+      w[q] = packed_pair<T>(lo, hi);
     }
   }
   return o;
@@ -71,7 +78,9 @@ __global__ void __launch_bounds__(256) k_dropout(const DropoutArgs a) {
     step = a.step_wide ? (uint32_t)__ldg(reinterpret_cast<const unsigned long long*>(a.step_at))
                        : (uint32_t)__ldg(reinterpret_cast<const unsigned int*>(a.step_at));
   if (a.step_used && blockIdx.x == 0 && threadIdx.x == 0) *a.step_used = step;
-  const uint32_t k0 = seed_lo(a.seed), k1 = seed_hi(a.seed);
+  const PhiloxKeys keys = philox_keys(seed_lo(a.seed), seed_hi(a.seed));
+  const uint32_t cut16 = a.cut << 16;  // a cut of 65536 leaves nothing
+  const bool all = a.cut == 65536u;
   const T* x = reinterpret_cast<const T*>(a.x);
   T* y = reinterpret_cast<T*>(a.y);
   const int64_t groups = (a.n + 7) / 8;
@@ -93,8 +102,7 @@ __global__ void __launch_bounds__(256) k_dropout(const DropoutArgs a) {
     for (int j = 0; j < kGroups; ++j) {
       const int64_t g = first + 256 * j, at = g * 8;
       if (at >= a.n) break;
-      const u32x4 draw = philox4x32_10(u32x4{(uint32_t)g, (uint32_t)(g >> 32), step, kSaltDropout}, k0, k1);
-      const Vec8<T> o = dropped(v[j], draw, a.cut, a.scale);
+      const Vec8<T> o = dropped(v[j], draw8(g, step, keys), cut16, all, a.scale);
       if (ALIGNED && at + 8 <= a.n) {
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(y + at)[i] = o.w[i];
