@@ -55,17 +55,30 @@ __device__ __forceinline__ float fp4_block_value(uint32_t e4m3) {
 __device__ __forceinline__ uint32_t fp4_block_scale(float most, float inv) {
   return __nv_cvt_float_to_fp8(__fmul_rn(__fmul_rn(most, inv), 1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ float fp4_code_factor(uint32_t block, float inv) {
-  return block ? __fdiv_rn(inv, fp4_block_value(block)) : 0.0f;
+// inv / block for any block scale from the eight quotients of inv by 1, 9/8, ..., 15/8, which the lanes of a warp hold (lane j
+// that by 1 + (j % 8) / 8): e4m3 is such a number times a power of two, by which a quotient scales exactly.
+__device__ __forceinline__ float fp4_quotients(float inv) {
+  return __fdiv_rn(inv, 1.0f + 0.125f * (float)(threadIdx.x & 7));
+}
+__device__ __forceinline__ float fp4_code_factor(uint32_t block, float quotients) {
+  const uint32_t bits = __float_as_uint(fp4_block_value(block));
+  const float q = __shfl_sync(0xffffffffu, quotients, (int)(bits >> 20) & 7);
+  return block ? __fmul_rn(q, __uint_as_float((254u << 23) - (bits & 0x7F800000u))) : 0.0f;
 }
 // Eight codes in a word.
 __device__ __forceinline__ uint32_t fp4_codes8(const float (&f)[8], float factor) {
-  uint32_t w = 0u;
+  float y[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(__fmul_rn(f[2 * i], factor), __fmul_rn(f[2 * i + 1], factor)), __NV_E2M1,
-                                            cudaRoundNearest)
-         << (8 * i);
+  for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(f[i], factor);
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return w;
 }
 

@@ -2,8 +2,8 @@
 //
 // k_fp4_quantize<T, W>: one pass, W warps per row, as few as hold it in registers (1024 elements a warp, at most eight
 // warps; longer rows read their tail again), as the 8-bit quantisation does.  A lane holds eight columns at a time, two
-// lanes a block: its maximum is one shuffle away, and eight lanes gather the four scales that lie together.  Bound:
-// memory (b bytes read and 9/16 written per element).
+// lanes a block: its maximum is one shuffle away.  Bound: memory (b bytes read and 9/16 written per element), close to the
+// instructions.
 #include "fp4_common.cuh"
 
 namespace tthrml {
@@ -27,18 +27,27 @@ __global__ void __launch_bounds__(256, 4)
   const int t = (int)threadIdx.x & (32 * W - 1);
   const int64_t row = (int64_t)blockIdx.x * (8 / W) + warp / W;  // up to the end of the last 128 rows
   const bool live = row < rows;
-  const int64_t k_blocks = fp4_up(cols, 256) / 256, end = k_blocks * 256;
+  const int end = (int)fp4_up(cols, 256), code_cols = live ? (int)(2 * o.pitch) : 0;
   const T* xr = x + (live ? row : 0) * rs;
   const uint32_t off = (uint32_t)((uintptr_t)xr & 15u);
-  const RowReader<T, ALIGNED> in = {xr, live ? cols : 0, cs, contiguous ? (off ? kShifted : kAligned) : kElements, off};
+  const RowReader<T, ALIGNED> in = {xr, live ? (int32_t)cols : 0, cs, contiguous ? (off ? kShifted : kAligned) : kElements, off};
   Vec8<T> kept[kKept];
-  MaxOf<T> most;
+  float most[kKept];  // of each vector
+  float all = 0.0f;
+  const auto largest = [](const Vec8<T>& v) {
+    MaxOf<T> m;
+    add_vector<T>(m, v);
+    return m.value();
+  };
 #pragma unroll
-  for (int v = 0; v < kKept; ++v) kept[v] = in.vector((int64_t)v * kStep + 8 * t);
+  for (int v = 0; v < kKept; ++v) kept[v] = in.vector(v * kStep + 8 * t);
 #pragma unroll
-  for (int v = 0; v < kKept; ++v) add_vector<T>(most, kept[v]);
-  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < in.cols; c += kStep) add_vector<T>(most, in.vector(c));
-  uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most.value()));
+  for (int v = 0; v < kKept; ++v) {
+    most[v] = largest(kept[v]);
+    all = max_abs(all, most[v]);
+  }
+  for (int c = kKept * kStep + 8 * t; c < in.cols; c += kStep) all = max_abs(all, largest(in.vector(c)));
+  uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(all));
   if (W > 1) {
     if (lane == 0) part[warp] = top;
     __syncthreads();
@@ -47,28 +56,27 @@ __global__ void __launch_bounds__(256, 4)
   }
   const Fp4RowScale s = fp4_row_scale(top);
   if (live && t == 0) o.scale[row] = s.scale;
+  const float quotients = fp4_quotients(s.inv);
   unsigned char* codes = o.codes + row * o.pitch;
-  unsigned char* blocks = o.blocks + fp4_scale_at(row, 0, k_blocks);  // 512 bytes further per 64 columns
-  const auto store = [&](const Vec8<T>& v, int64_t c) {  // whole warps: c runs to a multiple of 256
-    MaxOf<T> m;
-    add_vector<T>(m, v);
-    const float mine = m.value();
+  unsigned char* blocks = o.blocks + fp4_scale_at(row, 0, end / 256);  // 512 bytes further per 64 columns
+  const auto store = [&](const Vec8<T>& v, float mine, int c) {  // whole warps: c runs to a multiple of 256
     const uint32_t block = fp4_block_scale(max_abs(mine, __shfl_xor_sync(0xffffffffu, mine, 1)), s.inv);
-    uint32_t four = (lane & 1) ? 0u : block << (8 * ((lane >> 1) & 3));
-    four |= __shfl_xor_sync(0xffffffffu, four, 2);
-    four |= __shfl_xor_sync(0xffffffffu, four, 4);
-    if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(blocks + c / 64 * 512) = four;
-    if (!live || c >= 2 * o.pitch) return;
+    const float factor = fp4_code_factor(block, quotients);
+    if ((lane & 1) == 0) blocks[c / 64 * 512 + (c / 16 & 3)] = (unsigned char)block;
+    if (c >= code_cols) return;
     float f[8];
     unpack8(v, f);
-    *reinterpret_cast<uint32_t*>(codes + c / 2) = fp4_codes8(f, fp4_code_factor(block, s.inv));
+    *reinterpret_cast<uint32_t*>(codes + c / 2) = fp4_codes8(f, factor);
   };
 #pragma unroll
   for (int v = 0; v < kKept; ++v) {
-    const int64_t c = (int64_t)v * kStep + 8 * t;
-    if (c - 8 * lane < end) store(kept[v], c);
+    const int c = v * kStep + 8 * t;
+    if (c - 8 * lane < end) store(kept[v], most[v], c);
   }
-  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c - 8 * lane < end; c += kStep) store(in.vector(c), c);
+  for (int c = kKept * kStep + 8 * t; c - 8 * lane < end; c += kStep) {
+    const Vec8<T> v = in.vector(c);
+    store(v, largest(v), c);
+  }
 }
 
 // The float32 values: (code * block) * scale, code * block exact.  A thread takes four columns at a time, so that a warp's

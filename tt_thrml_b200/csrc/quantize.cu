@@ -37,14 +37,14 @@ __global__ void __launch_bounds__(256, 4)
   if (!live) cols = pitch = 0;
   const T* xr = x + (live ? row : 0) * rs;
   const uint32_t off = (uint32_t)((uintptr_t)xr & 15u);
-  const RowReader<T, ALIGNED> in = {xr, cols, cs, contiguous ? (off ? kShifted : kAligned) : kElements, off};
+  const RowReader<T, ALIGNED> in = {xr, (int32_t)cols, cs, contiguous ? (off ? kShifted : kAligned) : kElements, off};
   Vec8<T> kept[kKept];
   MaxOf<T> most;
 #pragma unroll
-  for (int v = 0; v < kKept; ++v) kept[v] = in.vector((int64_t)v * kStep + 8 * t);
+  for (int v = 0; v < kKept; ++v) kept[v] = in.vector(v * kStep + 8 * t);
 #pragma unroll
   for (int v = 0; v < kKept; ++v) add_vector<T>(most, kept[v]);
-  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < cols; c += kStep) add_vector<T>(most, in.vector(c));
+  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < cols; c += kStep) add_vector<T>(most, in.vector((int32_t)c));
   uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most.value()));
   if (W > 1) {
     if (lane == 0) part[warp] = top;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256, 4)
     const int64_t c = (int64_t)v * kStep + 8 * t;
     if (c < pitch) store_vector<T>(qr + c, kept[v], s.inv);
   }
-  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < pitch; c += kStep) store_vector<T>(qr + c, in.vector(c), s.inv);
+  for (int64_t c = (int64_t)kKept * kStep + 8 * t; c < pitch; c += kStep) store_vector<T>(qr + c, in.vector((int32_t)c), s.inv);
 }
 
 // Rows adjacent in memory (row stride 1): lane = row, warp w takes columns w, w + 8, ... of the CTA's share.

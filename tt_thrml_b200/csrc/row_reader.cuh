@@ -30,10 +30,11 @@ __device__ __forceinline__ uint4 load_shifted(const char* p, uint32_t off) {
 template <typename T, bool ALIGNED>
 struct RowReader {
   const T* x;
-  int64_t cols, cs;
+  int32_t cols;
+  int64_t cs;
   int mode;
   uint32_t off;
-  __device__ __forceinline__ Vec8<T> vector(int64_t c) const {  // elements c .. c + 7, zeros behind the end
+  __device__ __forceinline__ Vec8<T> vector(int32_t c) const {  // elements c .. c + 7, zeros behind the end
     Vec8<T> v;
     if ((ALIGNED || mode != kElements) && c + 8 <= cols) {
 #pragma unroll
@@ -48,7 +49,7 @@ struct RowReader {
       T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (c + i < cols) e[i] = x[(c + i) * cs];
+        if (c + i < cols) e[i] = x[(int64_t)(c + i) * cs];
     }
     return v;
   }
