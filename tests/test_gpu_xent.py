@@ -129,3 +129,17 @@ def test_losses_and_gradients(tt, rows, k, v, dtype):
 def test_reductions(tt, reduction, dtype, with_bias):
     x, w, y, bias = batch(200, 136, 777, DTYPES[dtype], 5, bias=with_bias)
     check(tt, x, w, y, bias, reduction)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,k,v", [(16500, 40, 8700), (9000, 257, 16001)])
+def test_categories_in_several_pieces(tt, rows, k, v, dtype):
+    """More than 256 MiB of differences: the gradients of x are sums over pieces of the categories."""
+    x, w, y, bias = batch(rows, k, v, DTYPES[dtype], 3)
+    check(tt, x, w, y, bias, "mean")
+
+
+@pytest.mark.parametrize("rows,k,v", [(4000, 2048, 6000), (2500, 1000, 9000)])
+def test_many_tiles(tt, rows, k, v):
+    x, w, y, bias = batch(rows, k, v, torch.bfloat16, 4, bias=k == 1000)
+    check(tt, x, w, y, bias, "mean")

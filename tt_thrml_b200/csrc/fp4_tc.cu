@@ -526,7 +526,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int q = 0; q < 4; q += 2) {
             uint4 w[8];
-            pack_row(&acc[q][0], a.out_dtype, w);
+            pack_row<4>(acc[q], a.out_dtype, w);
+            pack_row<4>(acc[q + 1], a.out_dtype, w + 4);
             send(w, n0 + q * 32);
           }
         }

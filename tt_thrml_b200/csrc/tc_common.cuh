@@ -279,13 +279,20 @@ __device__ __forceinline__ void stage_row(uint32_t buffer, const uint4 (&w)[8]) 
                  "r"(w[j].w)
                  : "memory");
 }
-__device__ __forceinline__ void send_rows(const CUtensorMap* map, uint32_t buffer, int column, int row) {
+// To rows `row` .. row + 31 of plane `plane` from column `column` on; add: onto the float32 values there.
+__device__ __forceinline__ void send_rows(const CUtensorMap* map, uint32_t buffer, int column, int row, int plane = 0,
+                                          bool add = false) {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
   if ((threadIdx.x & 31) == 0) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(buffer), "r"(column),
-                 "r"(row)
-                 : "memory");
+    if (add)
+      asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                   "r"(buffer), "r"(column), "r"(row), "r"(plane)
+                   : "memory");
+    else
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(buffer),
+                   "r"(column), "r"(row), "r"(plane)
+                   : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
 }
@@ -299,10 +306,11 @@ __device__ __forceinline__ void sent_rows_done() {
   if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   __syncwarp();
 }
-// Eight 16-byte words of 64 16-bit values, or of 32 float32 ones.
-__device__ __forceinline__ void pack_row(const float* v, int32_t dtype, uint4 (&w)[8]) {
+// N 16-byte words of 8 N values rounded to 16 bits.
+template <int N>
+__device__ __forceinline__ void pack_row(const float* v, int32_t dtype, uint4* w) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
+  for (int q = 0; q < N; ++q) {
     uint32_t p[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -342,20 +350,23 @@ int encode_fn(EncodeTiledFn* out) {
   return TTHRML_OK;
 }
 
-// Tensor map of an output matrix [rows][cols] with rows `ld` elements apart for stores of 32 rows x 128 bytes; false where
-// its rows do not start on 16 bytes (or are too far apart).
-inline bool make_out_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int32_t dtype) {
-  const int64_t bytes = dtype == TTHRML_DT_F32 ? 4 : 2;
+// Tensor map of output matrices [planes][rows][cols], rows `ld` and planes `plane` elements apart, for stores of 32 rows x
+// 128 bytes; false where the rows do not start on 16 bytes (or are too far apart).
+inline bool make_out_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int32_t dtype,
+                         int64_t planes = 1, int64_t plane = 0) {
+  const int64_t bytes = dtype == TTHRML_DT_F32 ? 4 : 2, apart = planes > 1 ? plane : rows * ld;
   EncodeTiledFn fn;
-  if ((uintptr_t)base % 16 || ld * bytes % 16 || ld * bytes >= (int64_t)1 << 40 || encode_fn(&fn)) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(ld * bytes)};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), 32u};
-  const cuuint32_t estr[2] = {1, 1};
+  if ((uintptr_t)base % 16 || ld * bytes % 16 || apart * bytes % 16 || ld * bytes >= (int64_t)1 << 40 ||
+      apart * bytes >= (int64_t)1 << 40 || encode_fn(&fn))
+    return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * bytes), (cuuint64_t)(apart * bytes)};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / bytes), 32u, 1u};
+  const cuuint32_t estr[3] = {1, 1, 1};
   const CUtensorMapDataType type = dtype == TTHRML_DT_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == TTHRML_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

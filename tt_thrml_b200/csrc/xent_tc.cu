@@ -25,7 +25,9 @@ namespace {
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kThreads = 320, kEpilogueWarps = 8;
 constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
-constexpr int kChunk = 4;  // 64-wide blocks of K that a logit's sum stays in tensor memory for
+// 64-wide blocks of K that a logit's sum stays in tensor memory for.  Where only g of 16 bits is made of it, longer: the
+// multiplications may run two sums ahead of an epilogue that still stores a tile.
+constexpr int kChunk = 8, kLongChunk = 16;
 enum : int { kPartials = 0, kGradient = 1, kProduct = 2 };
 
 struct RowTargets {
@@ -41,6 +43,7 @@ struct XentArgs {
   int32_t M, N;       // the product's rows and columns
   int32_t num_k;      // 64-wide blocks of its sum
   int32_t f16;
+  int32_t chunk;      // blocks of K per accumulation
   int32_t units, segments, seg, splits, group;  // units of work: `seg` tiles along N of one row of tiles and one share of K
   // epilogues of logits: N categories from `first` on
   const float* bias;  // of the first category, or NULL
@@ -56,15 +59,14 @@ struct XentArgs {
   const float* row_grad;  // [M] weights, or NULL: ones
   const float* top_grad;  // what they are divided by
   float unit;             // g is held times this
-  unsigned char* g;       // [M][g_ld] 16-bit
-  int64_t g_ld;
   float* bias_part;       // [ceil(M / 32)][bias_ld] sums over 32 rows, or NULL
   int64_t bias_ld;
-  // kProduct, scaled: out = sums * factor[0] * factor[1] / unit; else planes of plain float32 sums, a plane per split, whose
-  // rows have room for whole tiles of 32 columns
+  // kGradient: out = g.  kProduct: scaled, out = sums * factor[0] * factor[1] / unit; else planes of plain float32 sums, one per
+  // split, added to where `accumulate`.  tma_store: the rows of `out` are aligned for bulk stores, as those of g and of
+  // planes always are.
   void* out;
-  int64_t out_ld, plane;  // elements from row to row, and from plane to plane
-  int32_t out_dtype, align, accumulate, scaled;
+  int64_t out_ld;
+  int32_t out_dtype, align, accumulate, scaled, tma_store;
   const float* factor[2];
   int* error;
 };
@@ -89,7 +91,7 @@ struct XentShape {
   static constexpr int kA = 128 * 64 * 2, kB = BN / 2 * 64 * 2, kStage = kA + kB;
   static constexpr int kStages = BN == 256 ? 6 : 8;
   static constexpr int kBarriers = 256;
-  static constexpr int kSmem = 1024 + kStages * kStage + kBarriers + 2 * 256 * 4 /*biases*/ + kEpilogueWarps * 32 * kTurnPitch;
+  static constexpr int kSmem = 1024 + kStages * kStage + kEpilogueWarps * kOutBytes + kBarriers + 256 * 4 /*biases*/;
 };
 
 // Unit u -> its split, row of tiles and segment: splits slowest, `group` rows of tiles at a time.
@@ -120,19 +122,18 @@ __device__ __forceinline__ float column_sums(float (&v)[32]) {
 template <int EPI, bool A_MN, bool B_MN, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     k_xent(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-           const __grid_constant__ XentArgs a) {
+           const __grid_constant__ CUtensorMap map_out, const __grid_constant__ XentArgs a) {
   using S = XentShape<BN>;
   static_assert(!B_MN || BN == 256, "MN-major halves of B are whole boxes of 64");
-  constexpr int kLength = EPI == kProduct ? 0x40000000 : kChunk;  // blocks of K per accumulation
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStage);
+  unsigned char* turns = tiles + S::kStages * S::kStage;  // a buffer per epilogue warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(turns + kEpilogueWarps * kOutBytes);
   uint64_t* empty = full + S::kStages;
   uint64_t* acc_full = empty + S::kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;       // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  float* biases = reinterpret_cast<float*>(tiles + S::kStages * S::kStage + S::kBarriers);  // [2][256]
-  unsigned char* turns = reinterpret_cast<unsigned char*>(biases + 2 * 256);
+  float* bias = reinterpret_cast<float*>(turns + kEpilogueWarps * kOutBytes + S::kBarriers);  // [256]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         unit_at(a, u, split, mb, sg);
         const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
         for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb) {
-          for (int k0 = k_first; k0 < k_last && !failed; k0 += kLength, ++it) {
+          for (int k0 = k_first; k0 < k_last && !failed; k0 += a.chunk, ++it) {
             const int b = it & 1;
             if (!mbar_wait_all(&acc_empty[b], ((uint32_t)(it >> 1) & 1u) ^ 1u)) {
               if (one) atomicExch(a.error, kErrAccWait);
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_after();
             const uint32_t d = tmem + (uint32_t)(b * 256);
-            for (int kb = k0; kb < min(k0 + kLength, k_last); ++kb) {
+            for (int kb = k0; kb < min(k0 + a.chunk, k_last); ++kb) {
               const int s = (int)(used % S::kStages);
               if (!mbar_wait_all(&full[s], (uint32_t)(used / S::kStages) & 1u)) {
                 if (one) atomicExch(a.error, kErrFullWait);
@@ -261,8 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
-    unsigned char* turn = turns + (warp - 2) * 32 * kTurnPitch;
-    int it = 0, tile = 0;
+    unsigned char* turn = turns + (warp - 2) * kOutBytes;
+    const uint32_t buffer = smem_u32(turn);
+    int it = 0;
     bool failed = false;
     for (int u = first; u < a.units; u += step) {
       int split, mb, sg;
@@ -288,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (EPI == kProduct && a.scaled) factor = factor_of(a.factor) / a.unit;
       for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb) {
-        float* bias = biases + (tile++ & 1) * 256;
-        if (EPI != kProduct && a.bias) {  // two buffers, so that a warp may run one tile ahead
+        if (EPI != kProduct && a.bias) {
+          asm volatile("bar.sync 1, 256;" ::: "memory");  // every warp has read the biases of the tile before
           const int j = (int)threadIdx.x - 64, n = nb * BN + j;
           if (j < BN) bias[j] = n < a.N ? __ldg(a.bias + n) : 0.0f;
           asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (EPI != kProduct) {
 #pragma unroll
           for (int j = 0; j < kMine; ++j) acc[j] = 0.0f;
-          for (int k0 = k_first; k0 < k_last && !failed; k0 += kLength, ++it) {
+          for (int k0 = k_first; k0 < k_last && !failed; k0 += a.chunk, ++it) {
             const int b = it & 1;
             if (!mbar_wait_warp(&acc_full[b], (uint32_t)(it >> 1) & 1u)) {
               if (lane == 0) atomicExch(a.error, kErrAccWait);
@@ -324,10 +326,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
         tc_fence_after();
+        // 32 rows x 128 bytes on their way out: 64 columns of 16 bits, or 32 of float32
+        uint4 words[8];
+        const auto send = [&](int column) {
+          if (m - lane >= a.M) return;
+          sent_rows_read<0>();
+          stage_row(buffer, words);
+          send_rows(&map_out, buffer, column, m - lane, split, EPI == kProduct && a.accumulate);
+        };
 #pragma unroll
         for (int q = 0; q < BN / 64; ++q) {
           const int c = half * (BN / 2) + q * 32, n = nb * BN + c, live = min(32, a.N - n);
-          if (live <= 0) break;
+          if (live <= 0) {  // nothing behind the last column; the 32 columns before this may still wait for their store
+            if (EPI != kPartials && (q & 1) && live + 32 > 0 && a.tma_store && a.out_dtype != TTHRML_DT_F32) send(n - 32);
+            break;
+          }
           float v[32];
           if (EPI == kProduct) {
             tmem_load32(tmem + (uint32_t)((it & 1) * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
@@ -381,27 +394,30 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             __syncwarp();
-            store_values(v, a.f16 ? TTHRML_DT_F16 : TTHRML_DT_BF16, turn, a.g, a.g_ld, n, m - lane, a.M, live, 16);
+            if (BN > 64) {
+              pack_row<4>(v, a.out_dtype, words + 4 * (q & 1));
+              if (q & 1) send(n - 32);
+            } else {
+              store_values(v, a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m - lane, a.M, live, 16);
+            }
             if (a.bias_part) {
               const float s = column_sums(v);
               if (m - lane < a.M && lane < live) a.bias_part[(int64_t)(m >> 5) * a.bias_ld + n + lane] = s;
             }
           } else {
-            if (a.scaled) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= factor;
+            for (int j = 0; j < 32; ++j) v[j] *= factor;
+            if (!a.tma_store) {
               store_values(v, a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m - lane, a.M, live, a.align);
-            } else if (m < a.M) {  // rows of whole 32 floats, a row per lane: a long main loop hides it
-              float4* out = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + split * a.plane + (int64_t)m * a.out_ld + n);
+            } else if (a.out_dtype == TTHRML_DT_F32) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                float4 w = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                if (a.accumulate) {
-                  const float4 old = __ldcg(out + q);
-                  w.x += old.x, w.y += old.y, w.z += old.z, w.w += old.w;
-                }
-                out[q] = w;
-              }
+              for (int i = 0; i < 8; ++i)
+                words[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                      __float_as_uint(v[4 * i + 3]));
+              send(n);
+            } else {
+              pack_row<4>(v, a.out_dtype, words + 4 * (q & 1));
+              if (q & 1) send(n - 32);
             }
           }
           __syncwarp();  // the next TMEM load is a warp's
@@ -415,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (EPI == kPartials && m < a.M) a.part[(int64_t)m * a.slots + 2 * sg + half] = make_float2(top, sum);
     }
+    if (EPI != kPartials) sent_rows_done();
   }
 
   tc_fence_before();
@@ -608,20 +625,20 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int
 constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 template <int EPI, bool A_MN, bool B_MN, int BN>
-int launch_xent(const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
+int launch_xent(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const XentArgs& a, cudaStream_t st) {
   const void* fn = (const void*)k_xent<EPI, A_MN, B_MN, BN>;
   ClusterFit fit;
   const int rc = cluster_fit(fn, 2, kThreads, XentShape<BN>::kSmem, &fit);
   if (rc) return rc;
   const int64_t clusters = a.units < fit.clusters ? a.units : fit.clusters;
-  void* params[3] = {(void*)&ma, (void*)&mb, (void*)&a};
+  void* params[4] = {(void*)&ma, (void*)&mb, (void*)&mo, (void*)&a};
   return launch_clusters(fn, (unsigned)(2 * clusters), 2, kThreads, XentShape<BN>::kSmem, params, st, "k_xent launch", true);
 }
 template <int EPI>
-int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
-  if (bn == 64) return launch_xent<EPI, false, false, 64>(ma, mb, a, st);
-  if (bn == 128) return launch_xent<EPI, false, false, 128>(ma, mb, a, st);
-  return launch_xent<EPI, false, false, 256>(ma, mb, a, st);
+int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const XentArgs& a, cudaStream_t st) {
+  if (bn == 64) return launch_xent<EPI, false, false, 64>(ma, mb, mo, a, st);
+  if (bn == 128) return launch_xent<EPI, false, false, 128>(ma, mb, mo, a, st);
+  return launch_xent<EPI, false, false, 256>(ma, mb, mo, a, st);
 }
 
 // How many pairs of CTAs work at once (every form of the kernel fills an SM).
@@ -737,7 +754,14 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
   int64_t g = 1;  // about square rectangles of the tiles in flight
   while ((g + 1) * (g + 1) <= pairs) ++g;
   a.group = (int32_t)std::min(g, m_blocks);
-  return launch_xent<kProduct, A_MN, true, 256>(ma, mb, a, st);
+  a.chunk = a.num_k;
+  CUtensorMap mo = ma;  // never used where the rows are not aligned
+  a.tma_store = make_out_map(&mo, a.out, m, n, a.out_ld, a.out_dtype, n_shares, m * a.out_ld);
+  if (!a.scaled && !a.tma_store) {
+    set_error("planes of %lld x %lld sums take no tensor map", (long long)m, (long long)n);
+    return TTHRML_ERR_CUDA;
+  }
+  return launch_xent<kProduct, A_MN, true, 256>(ma, mb, mo, a, st);
 }
 int join_planes(const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols, int64_t n, const XentArgs& a, void* out,
                 int64_t out_ld, int32_t out_dtype, cudaStream_t st) {
@@ -802,7 +826,8 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.target_logit = (float*)(ws + f.logits);
   a.counter = (uint32_t*)(ws + f.counter);
   a.error = error;
-  rc = launch_logits<kPartials>(f.bn, ma, mb, a, st);
+  a.chunk = kChunk;
+  rc = launch_logits<kPartials>(f.bn, ma, mb, ma, a, st);
   if (rc) return rc;
   LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, log2_z, row_loss, loss, inv_count,
                 a.counter};
@@ -858,8 +883,6 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
   base.categories = p->categories;
   base.targets = {p->targets, p->wide_targets, p->ignored};
   base.log2_z = log2_z;
-  base.g = ws;
-  base.g_ld = f.g_ld;
   base.error = error;
   base.factor[0] = grad_per_row ? top : grad;
   base.factor[1] = inv_count;
@@ -881,7 +904,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
   for (int64_t i = 0; i < f.pieces && rc == TTHRML_OK; ++i) {
     const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
     const char* w = (const char*)p->w + first * p->w_ld * 2;
-    CUtensorMap mw, mw_mn, mg, mg_mn;
+    CUtensorMap mw, mw_mn, mg, mg_mn, mo;
     const int bn = tile_width(p->rows, width, pairs);
     rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)bn / 2, f16);
     if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
@@ -904,15 +927,23 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     a.first = first;
     a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
     a.bias_ld = f.g_ld;
-    rc = launch_logits<kGradient>(bn, mx, mw, a, st);
+    a.chunk = db ? kChunk : kLongChunk;
+    a.out = ws;
+    a.out_ld = f.g_ld;
+    a.out_dtype = p->dtype;
+    a.tma_store = 1;
+    if (!make_out_map(&mo, ws, p->rows, width, f.g_ld, p->dtype)) {
+      set_error("tthrml_xent_backward: the workspace takes no tensor map");
+      return TTHRML_ERR_CUDA;
+    }
+    rc = launch_logits<kGradient>(bn, mx, mw, mo, a, st);
     if (rc) return rc;
     if (dx) {
       XentArgs d = base;
       d.scaled = !f.dx_planes;
       d.out = f.dx_planes ? (void*)(ws + f.dx) : dx;
       d.out_ld = f.dx_planes ? f.plane_ld : dx_ld;
-      d.plane = f.dx_planes ? p->rows * f.plane_ld : 0;
-      d.out_dtype = grad_dtype;
+      d.out_dtype = f.dx_planes ? TTHRML_DT_F32 : grad_dtype;
       d.align = alignment(dx, dx_ld);
       d.accumulate = i > 0;
       rc = product<false>(mg, mw_mn, d, p->rows, p->cols, width, std::min(f.dx_shares, up(width, 64) / 64), pairs, st);
@@ -925,12 +956,11 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
       d.scaled = !planes;
       d.out = planes ? (void*)(ws + f.dw) : out;
       d.out_ld = planes ? f.plane_ld : dw_ld;
-      d.plane = planes ? width * f.plane_ld : 0;
-      d.out_dtype = grad_dtype;
+      d.out_dtype = planes ? TTHRML_DT_F32 : grad_dtype;
       d.align = alignment(out, dw_ld);
       rc = product<true>(mg_mn, mx_mn, d, width, p->cols, p->rows, f.dw_shares, pairs, st);
       if (rc == TTHRML_OK && planes)
-        rc = join_planes((const float*)(ws + f.dw), d.plane, f.plane_ld, width, p->cols, f.dw_shares, base, out, dw_ld, grad_dtype, st);
+        rc = join_planes((const float*)(ws + f.dw), width * f.plane_ld, f.plane_ld, width, p->cols, f.dw_shares, base, out, dw_ld, grad_dtype, st);
       if (rc) return rc;
     }
     if (db) {
