@@ -135,6 +135,39 @@ __device__ __forceinline__ void tmem_wait(float (&v)[N][32]) {
                    "+f"(v[q][31]));
 }
 
+// 16 columns, for epilogues that hold many values already.
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Two float32 operations in one instruction, each rounded by itself.
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b));
+}
+// a b + c
+__device__ __forceinline__ void fma2(float a0, float a1, float b, float c, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+
 constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit of a shared::cluster address
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -231,6 +264,30 @@ __device__ __forceinline__ void store_rows(const uint4 (&words)[N16], unsigned c
   __syncwarp();
 }
 
+// store_rows of 64 whole bytes to rows that start on 16 bytes.
+__device__ __forceinline__ void store_rows64(const uint4 (&words)[4], uint32_t turn, unsigned char* out, int64_t pitch, int m0,
+                                             int M) {
+  const uint32_t lane = threadIdx.x & 31, mine = turn + lane * kTurnPitch;
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + 16 * q), "r"(words[q].x), "r"(words[q].y), "r"(words[q].z),
+                 "r"(words[q].w)
+                 : "memory");
+  __syncwarp();
+  const int r0 = (int)lane >> 2;
+  unsigned char* o = out + (int64_t)(m0 + r0) * pitch + 16 * (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(turn + (r0 + 8 * i) * kTurnPitch + 16 * (lane & 3))
+                 : "memory");
+    if (m0 + r0 + 8 * i < M) *reinterpret_cast<uint4*>(o + (int64_t)(8 * i) * pitch) = v;
+  }
+  __syncwarp();
+}
+
 // 32 values of each of a warp's rows m0 + lane, from column n on, to 16-bit or float32 rows.
 __device__ __forceinline__ void store_values(const float (&v)[32], int32_t dtype, unsigned char* turn, unsigned char* out,
                                              int64_t ld, int64_t n, int m0, int M, int live, int align) {
@@ -271,11 +328,12 @@ __device__ __forceinline__ void store_values(const float (&v)[32], int32_t dtype
 // (1024-byte aligned), in the 128-byte swizzle, which both the lanes' writes and the store's reads spread over all banks.  The
 // lane that issues the stores waits for their reads before a buffer is written again.
 constexpr int kOutBytes = 32 * 128;
-__device__ __forceinline__ void stage_row(uint32_t buffer, const uint4 (&w)[8]) {
+template <int N>
+__device__ __forceinline__ void stage_row(uint32_t buffer, const uint4 (&w)[N], uint32_t first = 0) {  // N of its eight pieces
   const uint32_t lane = threadIdx.x & 31, row = buffer + lane * 128;
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j)
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + 16 * (j ^ (lane & 7))), "r"(w[j].x), "r"(w[j].y), "r"(w[j].z),
+  for (uint32_t j = 0; j < N; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + 16 * ((first + j) ^ (lane & 7))), "r"(w[j].x), "r"(w[j].y), "r"(w[j].z),
                  "r"(w[j].w)
                  : "memory");
 }

@@ -25,10 +25,8 @@ namespace {
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kThreads = 320, kEpilogueWarps = 8;
 constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
-// 64-wide blocks of K that a logit's sum stays in tensor memory for.  Where only g of 16 bits is made of it, longer: the
-// multiplications may run two sums ahead of an epilogue that still stores a tile.
-constexpr int kChunk = 8, kLongChunk = 16;
-enum : int { kPartials = 0, kGradient = 1, kProduct = 2 };
+constexpr int kChunk = 8;  // 64-wide blocks of K that a logit's sum stays in tensor memory for
+enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
 
 struct RowTargets {
   const void* y;  // [rows] int64 or int32
@@ -62,8 +60,7 @@ struct XentArgs {
   float* bias_part;       // [ceil(M / 32)][bias_ld] sums over 32 rows, or NULL
   int64_t bias_ld;
   // kGradient: out = g.  kProduct: scaled, out = sums * factor[0] * factor[1] / unit; else planes of plain float32 sums, one per
-  // split, added to where `accumulate`.  tma_store: the rows of `out` are aligned for bulk stores, as those of g and of
-  // planes always are.
+  // split, added to where `accumulate`.  tma_store: `out` takes bulk stores (planes always do).
   void* out;
   int64_t out_ld;
   int32_t out_dtype, align, accumulate, scaled, tma_store;
@@ -104,19 +101,25 @@ __device__ __forceinline__ void unit_at(const XentArgs& a, int u, int& split, in
   sg = w / rows;
 }
 
-// Sums over the warp's 32 lanes of 32 values each: lane j returns that of value j.
-__device__ __forceinline__ float column_sums(float (&v)[32]) {
-  const int lane = threadIdx.x & 31;
+// Sums over the warp's 32 lanes of 32 values each, turned in a buffer of 4096 bytes: lane j returns that of value j.  (By
+// shuffles it takes 124 instructions, so 75.)
+__device__ __forceinline__ float column_sums(const float (&v)[32], uint32_t buffer) {
+  const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-  for (int w = 16; w >= 1; w >>= 1) {
-    const bool high = (lane & w) != 0;
+  for (uint32_t j = 0; j < 8; ++j)  // piece j of row r lies at j ^ (r & 7): rows and columns both cover every bank
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buffer + lane * 128 + 16 * (j ^ (lane & 7))), "f"(v[4 * j]),
+                 "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
+                 : "memory");
+  __syncwarp();
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < w; ++i) {
-      const float keep = high ? v[i + w] : v[i], give = high ? v[i] : v[i + w];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
-    }
+  for (uint32_t r = 0; r < 32; ++r) {
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buffer + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+    s[r & 3] += x;
   }
-  return v[0];
+  __syncwarp();
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 template <int EPI, bool A_MN, bool B_MN, int BN>
@@ -125,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
            const __grid_constant__ CUtensorMap map_out, const __grid_constant__ XentArgs a) {
   using S = XentShape<BN>;
   static_assert(!B_MN || BN == 256, "MN-major halves of B are whole boxes of 64");
+  constexpr bool kChunked = EPI == kPartials || EPI == kGradientSums;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* turns = tiles + S::kStages * S::kStage;  // a buffer per epilogue warp
@@ -277,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (EPI != kProduct && m < a.M) {
         const int64_t t = target_of(a.targets, m);
         y = t - a.first;
-        if (EPI == kGradient) {
+        if (EPI != kPartials) {
           log2_z = __ldg(a.log2_z + m);
           weight = a.unit;
           if (a.row_grad) {
@@ -289,6 +293,110 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (EPI == kProduct && a.scaled) factor = factor_of(a.factor) / a.unit;
+      // what becomes of 32 sums of this thread's row, from column n on (called by whole warps)
+      const auto finish = [&](float (&v)[32], int n) {
+        const int live = min(32, a.N - n);
+        if (live <= 0) return;
+        if (EPI != kProduct) {
+          if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 w = *reinterpret_cast<const float4*>(bias + (n % BN) + 4 * i);
+              add2(v[4 * i], v[4 * i + 1], w.x, w.y);
+              add2(v[4 * i + 2], v[4 * i + 3], w.z, w.w);
+            }
+          }
+          if (live < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = j < live ? v[j] : -INFINITY;
+          }
+        }
+        if (EPI == kPartials) {
+          const bool mine = y >= n && y < n + live;
+          if (__any_sync(0xffffffffu, (int)mine)) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z = y - n == j ? v[j] : z;
+            if (mine) a.target_logit[m] = z;
+          }
+          float most[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int j = 4; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
+          const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * kLog2E;
+          if (now > top) {
+            sum *= top == -INFINITY ? 0.0f : exp2_fast(top - now);
+            top = now;
+          }
+          const float base = top == -INFINITY ? 0.0f : -top;
+          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float e0, e1;
+            fma2(v[j], v[j + 1], kLog2E, base, e0, e1);
+            add2(s[j & 2], s[(j & 2) + 1], exp2_fast(e0), exp2_fast(e1));
+          }
+          sum += (s[0] + s[1]) + (s[2] + s[3]);
+        } else if (EPI == kGradient || EPI == kGradientSums) {
+          if (weight == 0.0f) {  // a row that does not count, whatever it holds
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              fma2(v[j], v[j + 1], kLog2E, -log2_z, v[j], v[j + 1]);
+              v[j] = exp2_fast(v[j]);
+              v[j + 1] = exp2_fast(v[j + 1]);
+              mul2(v[j], v[j + 1], weight);
+            }
+            if (y >= n && y < n + live) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = y - n == j ? v[j] - weight : v[j];
+            }
+          }
+          __syncwarp();
+          if (EPI == kGradientSums) {
+            const float s = column_sums(v, buffer);
+            if (m - lane < a.M && lane < live) a.bias_part[(int64_t)(m >> 5) * a.bias_ld + n + lane] = s;
+          }
+          uint4 w[4];
+          pack_row<4>(v, a.out_dtype, w);
+          if (live == 32)
+            store_rows64(w, buffer, (unsigned char*)a.out + 2 * n, 2 * a.out_ld, m - lane, a.M);
+          else
+            store_rows<4>(w, turn, (unsigned char*)a.out, 2 * a.out_ld, 2 * n, m - lane, a.M, 2 * live, 16);
+        } else if (a.tma_store) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], factor);
+          if (m - lane >= a.M) return;
+          if (a.out_dtype == TTHRML_DT_F32) {
+            sent_rows_read<0>();
+            uint4 w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                __float_as_uint(v[4 * i + 3]));
+            stage_row(buffer, w);
+            send_rows(&map_out, buffer, n, m - lane, split, a.accumulate != 0);
+          } else {  // 64 columns at a time
+            uint4 w[4];
+            pack_row<4>(v, a.out_dtype, w);
+            const bool second = (n & 32) != 0;
+            if (!second) sent_rows_read<0>();
+            stage_row(buffer, w, second ? 4u : 0u);
+            if (second || n + 32 >= a.N) send_rows(&map_out, buffer, n & ~63, m - lane, split);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], factor);
+          if (a.align == 16 && a.out_dtype != TTHRML_DT_F32 && live == 32) {
+            uint4 w[4];
+            pack_row<4>(v, a.out_dtype, w);
+            store_rows64(w, buffer, (unsigned char*)a.out + 2 * n, 2 * a.out_ld, m - lane, a.M);
+          } else {
+            store_values(v, a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m - lane, a.M, live, a.align);
+          }
+        }
+      };
       for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb) {
         if (EPI != kProduct && a.bias) {
           asm volatile("bar.sync 1, 256;" ::: "memory");  // every warp has read the biases of the tile before
@@ -296,9 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j < BN) bias[j] = n < a.N ? __ldg(a.bias + n) : 0.0f;
           asm volatile("bar.sync 1, 256;" ::: "memory");
         }
-        constexpr int kMine = EPI == kProduct ? 32 : BN / 2;  // logits of this thread, summed over the accumulations
-        float acc[kMine];
-        if (EPI != kProduct) {
+        constexpr int kMine = BN / 2;  // columns of this thread
+        if constexpr (kChunked) {
+          float acc[kMine];
 #pragma unroll
           for (int j = 0; j < kMine; ++j) acc[j] = 0.0f;
           for (int k0 = k_first; k0 < k_last && !failed; k0 += a.chunk, ++it) {
@@ -310,119 +418,38 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_after();
 #pragma unroll
-            for (int q = 0; q < kMine / 32; ++q) {
-              float v[32];
-              tmem_load32(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * (BN / 2) + q * 32), v);
+            for (int q = 0; q < kMine / 16; ++q) {
+              float v[16];
+              tmem_load16(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * kMine + q * 16), v);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) acc[q * 32 + j] += v[j];
+              for (int j = 0; j < 16; j += 2) add2(acc[q * 16 + j], acc[q * 16 + j + 1], v[j], v[j + 1]);
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(&acc_empty[b]);
           }
-        } else if (!failed && !mbar_wait_warp(&acc_full[it & 1], (uint32_t)(it >> 1) & 1u)) {
-          if (lane == 0) atomicExch(a.error, kErrAccWait);
-          failed = true;
-        }
-        if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
-        tc_fence_after();
-        // 32 rows x 128 bytes on their way out: 64 columns of 16 bits, or 32 of float32
-        uint4 words[8];
-        const auto send = [&](int column) {
-          if (m - lane >= a.M) return;
-          sent_rows_read<0>();
-          stage_row(buffer, words);
-          send_rows(&map_out, buffer, column, m - lane, split, EPI == kProduct && a.accumulate);
-        };
+          if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
 #pragma unroll
-        for (int q = 0; q < BN / 64; ++q) {
-          const int c = half * (BN / 2) + q * 32, n = nb * BN + c, live = min(32, a.N - n);
-          if (live <= 0) {  // nothing behind the last column; the 32 columns before this may still wait for their store
-            if (EPI != kPartials && (q & 1) && live + 32 > 0 && a.tma_store && a.out_dtype != TTHRML_DT_F32) send(n - 32);
-            break;
+          for (int q = 0; q < kMine / 32; ++q) {
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = acc[q * 32 + j];
+            finish(v, nb * BN + half * kMine + q * 32);
           }
-          float v[32];
-          if (EPI == kProduct) {
+        } else {
+          if (!failed && !mbar_wait_warp(&acc_full[it & 1], (uint32_t)(it >> 1) & 1u)) {
+            if (lane == 0) atomicExch(a.error, kErrAccWait);
+            failed = true;
+          }
+          if (failed) continue;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = half * kMine; c < (half + 1) * kMine; c += 32) {
+            float v[32];
             tmem_load32(tmem + (uint32_t)((it & 1) * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = acc[(kMine == 32 ? 0 : q * 32) + j];
-            if (a.bias) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 w = reinterpret_cast<const float4*>(bias + c)[i];
-                v[4 * i] += w.x, v[4 * i + 1] += w.y, v[4 * i + 2] += w.z, v[4 * i + 3] += w.w;
-              }
-            }
-            if (live < 32) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = j < live ? v[j] : -INFINITY;
-            }
+            finish(v, nb * BN + c);
+            __syncwarp();  // the next TMEM load is a warp's
           }
-          if (EPI == kPartials) {
-            const bool mine = y >= n && y < n + live;
-            if (__any_sync(0xffffffffu, (int)mine)) {
-              float z = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) z = y - n == j ? v[j] : z;
-              if (mine) a.target_logit[m] = z;
-            }
-            float most[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-            for (int j = 4; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
-            const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * kLog2E;
-            if (now > top) {
-              sum *= top == -INFINITY ? 0.0f : exp2_fast(top - now);
-              top = now;
-            }
-            const float base = top == -INFINITY ? 0.0f : top;
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s[j & 3] += exp2_fast(fmaf(v[j], kLog2E, -base));
-            sum += (s[0] + s[1]) + (s[2] + s[3]);
-          } else if (EPI == kGradient) {
-            if (weight == 0.0f) {  // a row that does not count, whatever it holds
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = weight * exp2_fast(fmaf(v[j], kLog2E, -log2_z));
-              const bool mine = y >= n && y < n + live;
-              if (mine) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = y - n == j ? v[j] - weight : v[j];
-              }
-            }
-            __syncwarp();
-            if (BN > 64) {
-              pack_row<4>(v, a.out_dtype, words + 4 * (q & 1));
-              if (q & 1) send(n - 32);
-            } else {
-              store_values(v, a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m - lane, a.M, live, 16);
-            }
-            if (a.bias_part) {
-              const float s = column_sums(v);
-              if (m - lane < a.M && lane < live) a.bias_part[(int64_t)(m >> 5) * a.bias_ld + n + lane] = s;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= factor;
-            if (!a.tma_store) {
-              store_values(v, a.out_dtype, turn, (unsigned char*)a.out, a.out_ld, n, m - lane, a.M, live, a.align);
-            } else if (a.out_dtype == TTHRML_DT_F32) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                words[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                                      __float_as_uint(v[4 * i + 3]));
-              send(n);
-            } else {
-              pack_row<4>(v, a.out_dtype, words + 4 * (q & 1));
-              if (q & 1) send(n - 32);
-            }
-          }
-          __syncwarp();  // the next TMEM load is a warp's
-        }
-        if (EPI == kProduct) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_leader(&acc_empty[it & 1]);
@@ -756,7 +783,8 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
   a.group = (int32_t)std::min(g, m_blocks);
   a.chunk = a.num_k;
   CUtensorMap mo = ma;  // never used where the rows are not aligned
-  a.tma_store = make_out_map(&mo, a.out, m, n, a.out_ld, a.out_dtype, n_shares, m * a.out_ld);
+  // Bulk stores are the quicker way out of short sums, but queue behind the loads of long ones, as in the 4-bit product.
+  a.tma_store = (!a.scaled || a.num_k <= 8) && make_out_map(&mo, a.out, m, n, a.out_ld, a.out_dtype, n_shares, m * a.out_ld);
   if (!a.scaled && !a.tma_store) {
     set_error("planes of %lld x %lld sums take no tensor map", (long long)m, (long long)n);
     return TTHRML_ERR_CUDA;
@@ -904,7 +932,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
   for (int64_t i = 0; i < f.pieces && rc == TTHRML_OK; ++i) {
     const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
     const char* w = (const char*)p->w + first * p->w_ld * 2;
-    CUtensorMap mw, mw_mn, mg, mg_mn, mo;
+    CUtensorMap mw, mw_mn, mg, mg_mn;
     const int bn = tile_width(p->rows, width, pairs);
     rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)bn / 2, f16);
     if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
@@ -927,16 +955,11 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     a.first = first;
     a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
     a.bias_ld = f.g_ld;
-    a.chunk = db ? kChunk : kLongChunk;
+    a.chunk = db ? kChunk : a.num_k;
     a.out = ws;
     a.out_ld = f.g_ld;
     a.out_dtype = p->dtype;
-    a.tma_store = 1;
-    if (!make_out_map(&mo, ws, p->rows, width, f.g_ld, p->dtype)) {
-      set_error("tthrml_xent_backward: the workspace takes no tensor map");
-      return TTHRML_ERR_CUDA;
-    }
-    rc = launch_logits<kGradient>(bn, mx, mw, mo, a, st);
+    rc = db ? launch_logits<kGradientSums>(bn, mx, mw, mx, a, st) : launch_logits<kGradient>(bn, mx, mw, mx, a, st);
     if (rc) return rc;
     if (dx) {
       XentArgs d = base;
