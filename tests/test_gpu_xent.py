@@ -65,7 +65,8 @@ def expected(x, w, y, bias, weight, ignore=-100):
     dg0 = r.abs() * (p * (dl + (dz + 12 * u * spread)[:, None]) + 4 * u * (p + hit))  # before its rounding
     # float16 holds g as 2^14 g / (the largest weight): its smallest step is 2^-24 of that
     tiny = 2.0**-25 * 2.0**-14 * float(r.abs().max()) if x.dtype == torch.float16 else 0.0
-    dg = dg0 + half * g.abs() + torch.where(r != 0, tiny, 0.0)
+    few = x.shape[0] <= 128  # g in two pieces: the rounding of the second one, 16 bits further down
+    dg = dg0 + (half * half if few else half) * g.abs() + torch.where(r != 0, tiny, 0.0)
 
     def product(a, da, b, n):
         exact = a @ b

@@ -13,7 +13,8 @@
 // transposed.  Warp 0 loads (TMA), warp 1 of the even CTA multiplies, warps 2-9 run the epilogue of a tile under the main
 // loop of the next one.
 //
-// g is rounded to the operands' 16 bits: by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
+// g is rounded to the operands' 16 bits (up to kFewRows rows: held in two such pieces, their sum good to 2^-16; the
+// second piece is more rows of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
 // themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
 // sums, z, losses and the sums of db are float32; dx and dw accumulate in float32.
 #include "int8_common.cuh"
@@ -25,6 +26,7 @@ namespace {
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kThreads = 320, kEpilogueWarps = 8;
 constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
+constexpr int64_t kFewRows = 128;             // whose g is held in two pieces of 16 bits
 constexpr int kChunk = 8;  // 64-wide blocks of K that a logit's sum stays in tensor memory for
 enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
 
@@ -64,6 +66,8 @@ struct XentArgs {
   void* out;
   int64_t out_ld;
   int32_t out_dtype, align, accumulate, scaled, tma_store;
+  int32_t second;  // kGradient: the row of `out` where the remainders of the rounding begin, 0: they are dropped.  kProduct: the
+                   // block of K from which on B's rows begin again
   const float* factor[2];
   int* error;
 };
@@ -90,6 +94,26 @@ struct XentShape {
   static constexpr int kBarriers = 256;
   static constexpr int kSmem = 1024 + kStages * kStage + kEpilogueWarps * kOutBytes + kBarriers + 256 * 4 /*biases*/;
 };
+
+// v less its values rounded to 16 bits (w, packed).
+__device__ __forceinline__ void less_row(float (&v)[32], int32_t dtype, const uint4 (&w)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t p[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      if (dtype == TTHRML_DT_BF16) {
+        lo = __uint_as_float(p[j] << 16), hi = __uint_as_float(p[j] & 0xFFFF0000u);
+      } else {
+        const __half2 h = *reinterpret_cast<const __half2*>(&p[j]);
+        lo = __low2float(h), hi = __high2float(h);
+      }
+      v[8 * q + 2 * j] -= lo;
+      v[8 * q + 2 * j + 1] -= hi;
+    }
+  }
+}
 
 // Unit u -> its split, row of tiles and segment: splits slowest, `group` rows of tiles at a time.
 __device__ __forceinline__ void unit_at(const XentArgs& a, int u, int& split, int& mb, int& sg) {
@@ -200,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (B_MN) {
 #pragma unroll
               for (int i = 0; i < BN / 128; ++i)
-                tma_load_2d_pair(st + S::kA + i * 8192, &map_b, bar, n0 + 64 * i, kb * 64);
+                tma_load_2d_pair(st + S::kA + i * 8192, &map_b, bar, n0 + 64 * i, (a.second && kb >= a.second ? kb - a.second : kb) * 64);
             } else {
               tma_load_2d_pair(st + S::kA, &map_b, bar, kb * 64, n0);
             }
@@ -358,12 +382,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float s = column_sums(v, buffer);
             if (m - lane < a.M && lane < live) a.bias_part[(int64_t)(m >> 5) * a.bias_ld + n + lane] = s;
           }
+          const int rows = a.second ? a.second : a.M;  // those behind the last row are zeros
           uint4 w[4];
           pack_row<4>(v, a.out_dtype, w);
+          unsigned char* out = (unsigned char*)a.out;
           if (live == 32)
-            store_rows64(w, buffer, (unsigned char*)a.out + 2 * n, 2 * a.out_ld, m - lane, a.M);
+            store_rows64(w, buffer, out + 2 * n, 2 * a.out_ld, m - lane, rows);
           else
-            store_rows<4>(w, turn, (unsigned char*)a.out, 2 * a.out_ld, 2 * n, m - lane, a.M, 2 * live, 16);
+            store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, 2 * live, 16);
+          if (a.second) {
+            less_row(v, a.out_dtype, w);
+            pack_row<4>(v, a.out_dtype, w);
+            out += 2 * a.second * a.out_ld;
+            store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, 2 * live, 16);
+          }
         } else if (a.tma_store) {
 #pragma unroll
           for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], factor);
@@ -577,6 +609,7 @@ __global__ void __launch_bounds__(1024) k_xent_top(const float* grad, RowTargets
 struct JoinArgs {
   const float* planes;
   int64_t plane, ld, rows, cols;
+  int64_t second;  // rows further lies another part of each row's sum; 0: none
   int32_t n;
   void* out;
   int64_t out_ld;
@@ -592,8 +625,10 @@ __global__ void __launch_bounds__(256) k_xent_join(const JoinArgs a) {
     const int64_t r = i / quads, c = (i - r * quads) * 4;
     const float* p = a.planes + r * a.ld + c;
     float4 s = __ldcg(reinterpret_cast<const float4*>(p));
-    for (int k = 1; k < a.n; ++k) {
-      const float4 t = __ldcg(reinterpret_cast<const float4*>(p + k * a.plane));
+    const int parts = a.second ? 2 * a.n : a.n;
+    for (int k = 1; k < parts; ++k) {
+      const float* q = k < a.n ? p + k * a.plane : p + (k - a.n) * a.plane + a.second * a.ld;
+      const float4 t = __ldcg(reinterpret_cast<const float4*>(q));
       s.x += t.x, s.y += t.y, s.z += t.z, s.w += t.w;
     }
     const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
@@ -717,6 +752,7 @@ int plan_forward(int64_t rows, int64_t categories, ForwardPlan* p) {
 
 struct BackwardPlan {
   int64_t piece, pieces, g_ld, plane_ld, dx_shares, dw_shares;
+  int64_t second, g_rows;  // the row where the second pieces begin (0: none), and all rows of g
   bool dx_planes;
   int64_t bias, top, dx, dw, bytes;  // places in the workspace behind g
 };
@@ -731,13 +767,15 @@ int plan_backward(int64_t rows, int64_t categories, int64_t cols, bool want_x, b
   const int64_t width = std::min(p->piece, categories);
   p->g_ld = up(width, 64);
   p->plane_ld = up(cols, 32);
-  p->dx_shares = want_x ? shares(rows, cols, width, pairs) : 0;
-  p->dw_shares = want_w ? shares(width, cols, rows, pairs) : 0;
-  p->dx_planes = p->dx_shares > 1 || (want_x && p->pieces > 1);
-  p->bias = up(rows * p->g_ld * 2, 16);
+  p->second = rows <= kFewRows ? up(rows, 64) : 0;
+  p->g_rows = p->second ? 2 * p->second : rows;
+  p->dx_shares = want_x ? shares(p->g_rows, cols, width, pairs) : 0;
+  p->dw_shares = want_w ? shares(width, cols, p->g_rows, pairs) : 0;
+  p->dx_planes = want_x && (p->dx_shares > 1 || p->pieces > 1 || p->second);
+  p->bias = up(p->g_rows * p->g_ld * 2, 16);
   p->top = p->bias + (want_b ? up(rows, 32) / 32 * p->g_ld * 4 : 0);
   p->dx = p->top + 16;
-  p->dw = p->dx + (p->dx_planes ? p->dx_shares * rows * p->plane_ld * 4 : 0);
+  p->dw = p->dx + (p->dx_planes ? p->dx_shares * p->g_rows * p->plane_ld * 4 : 0);
   p->bytes = p->dw + (p->dw_shares > 1 ? p->dw_shares * width * p->plane_ld * 4 : 0);
   return TTHRML_OK;
 }
@@ -791,9 +829,9 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
   }
   return launch_xent<kProduct, A_MN, true, 256>(ma, mb, mo, a, st);
 }
-int join_planes(const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols, int64_t n, const XentArgs& a, void* out,
-                int64_t out_ld, int32_t out_dtype, cudaStream_t st) {
-  JoinArgs j = {planes, plane, ld, rows, cols, (int32_t)n, out, out_ld, out_dtype, {a.factor[0], a.factor[1]}, a.unit};
+int join_planes(const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols, int64_t second, int64_t n,
+                const XentArgs& a, void* out, int64_t out_ld, int32_t out_dtype, cudaStream_t st) {
+  JoinArgs j = {planes, plane, ld, rows, cols, second, (int32_t)n, out, out_ld, out_dtype, {a.factor[0], a.factor[1]}, a.unit};
   const int64_t blocks = (rows * ((cols + 3) / 4) + 255) / 256;
   void* params[1] = {(void*)&j};
   return launch_clusters((const void*)k_xent_join, (unsigned)std::min<int64_t>(blocks, 148 * 8), 1, 256, 0, params, st,
@@ -936,8 +974,8 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     const int bn = tile_width(p->rows, width, pairs);
     rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)bn / 2, f16);
     if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
-    if (rc == TTHRML_OK) rc = make_map(&mg, ws, p->rows, width, f.g_ld, 128u, f16);
-    if (rc == TTHRML_OK) rc = make_map(&mg_mn, ws, p->rows, width, f.g_ld, 64u, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mg, ws, f.g_rows, width, f.g_ld, 128u, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mg_mn, ws, f.g_rows, width, f.g_ld, 64u, f16);
     if (rc) return rc;
     XentArgs a = base;
     a.M = (int32_t)p->rows;
@@ -955,7 +993,9 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     a.first = first;
     a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
     a.bias_ld = f.g_ld;
-    a.chunk = db ? kChunk : a.num_k;
+    // db is a sum over the rows: where many of them meet in a category, its logits have to be as good as the losses'
+    a.chunk = db ? (p->rows <= p->categories ? 4 * kChunk : kChunk) : a.num_k;
+    a.second = (int32_t)f.second;
     a.out = ws;
     a.out_ld = f.g_ld;
     a.out_dtype = p->dtype;
@@ -969,7 +1009,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
       d.out_dtype = f.dx_planes ? TTHRML_DT_F32 : grad_dtype;
       d.align = alignment(dx, dx_ld);
       d.accumulate = i > 0;
-      rc = product<false>(mg, mw_mn, d, p->rows, p->cols, width, std::min(f.dx_shares, up(width, 64) / 64), pairs, st);
+      rc = product<false>(mg, mw_mn, d, f.g_rows, p->cols, width, std::min(f.dx_shares, up(width, 64) / 64), pairs, st);
       if (rc) return rc;
     }
     if (dw) {
@@ -981,9 +1021,11 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
       d.out_ld = planes ? f.plane_ld : dw_ld;
       d.out_dtype = planes ? TTHRML_DT_F32 : grad_dtype;
       d.align = alignment(out, dw_ld);
-      rc = product<true>(mg_mn, mx_mn, d, width, p->cols, p->rows, f.dw_shares, pairs, st);
+      d.second = (int32_t)(f.second / 64);
+      rc = product<true>(mg_mn, mx_mn, d, width, p->cols, f.g_rows, f.dw_shares, pairs, st);
       if (rc == TTHRML_OK && planes)
-        rc = join_planes((const float*)(ws + f.dw), width * f.plane_ld, f.plane_ld, width, p->cols, f.dw_shares, base, out, dw_ld, grad_dtype, st);
+        rc = join_planes((const float*)(ws + f.dw), width * f.plane_ld, f.plane_ld, width, p->cols, 0, f.dw_shares, base, out, dw_ld, grad_dtype,
+                         st);
       if (rc) return rc;
     }
     if (db) {
@@ -998,7 +1040,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     }
   }
   if (rc == TTHRML_OK && dx && f.dx_planes)
-    rc = join_planes((const float*)(ws + f.dx), p->rows * f.plane_ld, f.plane_ld, p->rows, p->cols, f.dx_shares, base, dx, dx_ld,
-                     grad_dtype, st);
+    rc = join_planes((const float*)(ws + f.dx), f.g_rows * f.plane_ld, f.plane_ld, p->rows, p->cols, f.second, f.dx_shares, base, dx,
+                     dx_ld, grad_dtype, st);
   return rc;
 }
