@@ -814,15 +814,27 @@ int tthrml_fp4_product(const void* x_codes_dev, int64_t x_pitch, const void* x_b
                        int32_t out_dtype, int64_t out_ld, int32_t* error_dev, void* stream);
 
 /*
- * Rows of floats through 4-bit weights: tthrml_fp4_quantize into the workspace, then tthrml_fp4_product.  workspace: 16-byte
- * aligned device memory of tthrml_fp4_linear_workspace(rows, cols) bytes, free again once the work on `stream` is done.
+ * The same for one to four rows of floats with dense columns, quantised in the launch exactly as tthrml_fp4_quantize does;
+ * tthrml_fp4_few_rows tells whether the sizes allow it.
+ */
+int tthrml_fp4_few_rows(int64_t rows, int64_t cols, int64_t units);
+int tthrml_fp4_product_few(const void* x_dev, int32_t x_dtype, int64_t x_ld, const void* w_codes_dev,
+                           int64_t w_pitch, const void* w_blocks_dev, const float* w_scale_dev,
+                           int64_t rows, int64_t units, int64_t cols, const float* bias_dev,
+                           void* out_dev, int32_t out_dtype, int64_t out_ld, int32_t* error_dev,
+                           void* stream);
+
+/*
+ * Rows of floats through 4-bit weights: tthrml_fp4_product_few where it takes them (columns dense), else tthrml_fp4_quantize
+ * into the workspace, then tthrml_fp4_product.  workspace: 16-byte aligned device memory of
+ * tthrml_fp4_linear_workspace(rows, cols, units) bytes (0: none is needed), free again once the work on `stream` is done.
  */
 int tthrml_fp4_linear(const void* x_dev, int32_t x_dtype, int64_t rows, int64_t cols, int64_t row_stride,
                       int64_t col_stride, void* workspace_dev, int64_t workspace_bytes,
                       const void* w_codes_dev, int64_t w_pitch, const void* w_blocks_dev,
                       const float* w_scale_dev, int64_t units, const float* bias_dev, void* out_dev,
                       int32_t out_dtype, int64_t out_ld, int32_t* error_dev, void* stream);
-int64_t tthrml_fp4_linear_workspace(int64_t rows, int64_t cols);
+int64_t tthrml_fp4_linear_workspace(int64_t rows, int64_t cols, int64_t units);
 
 /*
  * ---------------------------------------------------------------------------

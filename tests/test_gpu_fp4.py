@@ -129,3 +129,10 @@ def test_products(tt, m, n, k, dtype):
 @pytest.mark.parametrize("m,n,k", [(4100, 4203, 600), (2560, 5120, 1280), (8192, 300, 257)])
 def test_products_of_many_tiles(tt, m, n, k):
     run_product(tt, m, n, k, "bf16", True, 3)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+@pytest.mark.parametrize("n,k", [(1, 1), (130, 16), (257, 1000), (1000, 1024), (2048, 4096), (300, 4097), (129, 9001), (19000, 500)])
+def test_products_of_few_rows(tt, m, n, k):
+    for dtype in DTYPES:
+        run_product(tt, m, n, k, dtype, n % 2 == 0, m + n + k)

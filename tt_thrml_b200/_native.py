@@ -285,7 +285,11 @@ _SIGNATURES = {
         [c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp,
          c_vp],
     ),
-    "tthrml_fp4_linear_workspace": (c_i64, [c_i64, c_i64]),
+    "tthrml_fp4_linear_workspace": (c_i64, [c_i64, c_i64, c_i64]),
+    "tthrml_fp4_few_rows": (c_i32, [c_i64, c_i64, c_i64]),
+    "tthrml_fp4_product_few": (
+        c_i32, [c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp, c_vp],
+    ),
     "tthrml_dropout": (c_i32, [c_vp, c_i32, c_i64, c_i32, c_u64, c_u32, c_vp, c_i32, c_vp, c_vp, c_vp]),
     "tthrml_greedy_colouring": (c_i32, [c_i64, c_vp, c_vp, c_vp, ctypes.POINTER(c_i32)]),
     "tthrml_set_device": (c_i32, [c_i32]),

@@ -16,8 +16,7 @@
 // scales of its rows and of all 256 units per 512 clocks).  The accumulator (256 columns) and the scales leave no room for a
 // second one: the epilogue's eight warps take a finished tile into registers at once, free the accumulator for the next tile's
 // MMAs and then scale and store.
-#include "fp4_common.cuh"
-#include "tc_common.cuh"
+#include "fp4_tc.cuh"
 
 namespace tthrml {
 namespace {
@@ -40,8 +39,6 @@ struct Fp4Args {
   int* error;
 };
 
-constexpr int kScales = 2048;  // bytes of the block scales of 128 rows and 256 columns
-
 template <int BN>
 struct TileShape {
   static constexpr int kABytes = 128 * 128, kBBytes = BN * 128, kChunks = BN == 256 ? 2 : 1;  // row blocks of B's scales
@@ -54,26 +51,6 @@ struct TileShape {
   static_assert(BN + 16 + 16 * kChunks <= kColumns, "accumulator and scales fit");
 };
 
-// Instruction descriptor: D float32, A and B e2m1, K-major, scales e4m3 (one per 16 columns).
-__host__ __device__ constexpr uint32_t idesc_fp4(int m, int n) {
-  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
-                                         uint32_t b_scales, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate));
-}
-// 32 rows of 16 bytes that lie one behind the other: groups of eight rows 128 bytes apart, no swizzle.
-__device__ __forceinline__ uint64_t scales_desc(const void* p) {
-  const uint64_t addr = (uint64_t)(smem_u32(p) >> 4) & 0x3FFFull;
-  return addr | (1ull << 16) | (8ull << 32) | (1ull << 46);
-}
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc));
-}
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
@@ -556,43 +533,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-// Tensor map of a byte matrix [rows][cols] with rows `pitch` bytes apart, in (box_rows x 128) tiles, 128-byte swizzle.
-int make_map_codes(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, uint32_t box_rows) {
-  EncodeTiledFn fn;
-  int rc = encode_fn(&fn);
-  if (rc) return rc;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {128u, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    set_error("cuTensorMapEncodeTiled failed (%d) for %lld x %lld bytes of codes", (int)r, (long long)rows, (long long)cols);
-    return TTHRML_ERR_CUDA;
-  }
-  return TTHRML_OK;
-}
-// The block scales as rows of 1024 bytes, read two at a time: those of 128 rows and 256 columns.
-int make_map_scales(CUtensorMap* map, const void* base, int64_t rows, int64_t cols) {
-  EncodeTiledFn fn;
-  int rc = encode_fn(&fn);
-  if (rc) return rc;
-  const cuuint64_t dims[2] = {256, (cuuint64_t)(fp4_scale_bytes(rows, cols) / 1024)};
-  const cuuint64_t strides[1] = {1024};
-  const cuuint32_t box[2] = {256u, 2u};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    set_error("cuTensorMapEncodeTiled failed (%d) for the scales of %lld x %lld values", (int)r, (long long)rows, (long long)cols);
-    return TTHRML_ERR_CUDA;
-  }
-  return TTHRML_OK;
-}
-
 // Clusters of 1, 2, 4 and 8 CTAs of k_fp4_tile<BN> that are resident at once on the current device.
 template <int BN>
 int resident_tiles(int (&out)[4]) {
@@ -741,9 +681,9 @@ extern "C" int tthrml_fp4_product(const void* x_codes, int64_t x_pitch, const vo
                      out_dtype, out_ld, error, false, stream);
 }
 
-extern "C" int64_t tthrml_fp4_linear_workspace(int64_t rows, int64_t cols) {
+extern "C" int64_t tthrml_fp4_linear_workspace(int64_t rows, int64_t cols, int64_t units) {
   using namespace tthrml;
-  if (rows < 1 || cols < 1 || rows > 0x0fffffffLL || cols > TTHRML_FP4_MAX_COLS) return 0;
+  if (rows < 1 || cols < 1 || rows > 0x0fffffffLL || cols > TTHRML_FP4_MAX_COLS || tthrml_fp4_few_rows(rows, cols, units)) return 0;
   return rows * (fp4_up(cols, 32) / 2) + fp4_scale_bytes(rows, cols) + fp4_up(rows * 4, 16);
 }
 
@@ -753,7 +693,15 @@ extern "C" int tthrml_fp4_linear(const void* x, int32_t x_dtype, int64_t rows, i
                                  void* out, int32_t out_dtype, int64_t out_ld, int32_t* error, void* stream) {
   using namespace tthrml;
   if (rows == 0 || units == 0) return TTHRML_OK;
-  const int64_t need = tthrml_fp4_linear_workspace(rows, cols);
+  const bool few = tthrml_fp4_few_rows(rows, cols, units) != 0;
+  if (col_stride == 1 && few)
+    return tthrml_fp4_product_few(x, x_dtype, row_stride, w_codes, w_pitch, w_blocks, w_scale, rows, units, cols, bias, out,
+                                  out_dtype, out_ld, error, stream);
+  const int64_t need = tthrml_fp4_linear_workspace(rows, cols, units);
+  if (need == 0 && few) {
+    set_error("tthrml_fp4_linear: few rows need dense columns (got a stride of %lld)", (long long)col_stride);
+    return TTHRML_ERR_ARG;
+  }
   if (need == 0) {
     set_error("tthrml_fp4_linear: sizes out of range (rows %lld, columns %lld of at most %d)", (long long)rows, (long long)cols,
               TTHRML_FP4_MAX_COLS);

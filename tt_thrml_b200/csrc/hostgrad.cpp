@@ -328,9 +328,10 @@ PyObject* fp4_product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::DimVector sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = N;
   Tensor out = at::empty(sizes, x.options().requires_grad(false));
-  const int64_t size = library.fp4_linear_workspace(M, K);
-  Tensor space = bytes(x, size);
-  const int rc = library.fp4_linear(x.const_data_ptr(), code, M, K, x.dim() == 2 ? x.stride(0) : K, 1, space.mutable_data_ptr(), size,
+  const int64_t size = library.fp4_linear_workspace(M, K, N);
+  Tensor space;
+  if (size) space = bytes(x, size);
+  const int rc = library.fp4_linear(x.const_data_ptr(), code, M, K, x.dim() == 2 ? x.stride(0) : K, 1, size ? space.mutable_data_ptr() : nullptr, size,
                                     codes.const_data_ptr(), pitch, blocks.const_data_ptr(), scale.const_data_ptr<float>(), N, bias,
                                     out.mutable_data_ptr(), code, N, reinterpret_cast<int32_t*>(PyLong_AsVoidPtr(args[7])),
                                     PyLong_AsVoidPtr(args[8]));

@@ -69,6 +69,8 @@ struct XentArgs {
   int32_t second;  // kGradient: the row of `out` where the remainders of the rounding begin, 0: they are dropped.  kProduct: the
                    // block of K from which on B's rows begin again
   const float* factor[2];
+  const float* carry;  // kProduct, scaled: sums of earlier pieces to add, [M][carry_ld] with room for whole 32 columns
+  int64_t carry_ld;
   int* error;
 };
 
@@ -418,6 +420,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (second || n + 32 >= a.N) send_rows(&map_out, buffer, n & ~63, m - lane, split);
           }
         } else {
+          if (a.carry && m < a.M) {  // a row per lane: a long main loop hides it
+            const float4* old = reinterpret_cast<const float4*>(a.carry + (int64_t)m * a.carry_ld + n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 c = __ldcg(old + i);
+              add2(v[4 * i], v[4 * i + 1], c.x, c.y);
+              add2(v[4 * i + 2], v[4 * i + 3], c.z, c.w);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], factor);
           if (a.align == 16 && a.out_dtype != TTHRML_DT_F32 && live == 32) {
@@ -822,7 +833,7 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
   a.chunk = a.num_k;
   CUtensorMap mo = ma;  // never used where the rows are not aligned
   // Bulk stores are the quicker way out of short sums, but queue behind the loads of long ones, as in the 4-bit product.
-  a.tma_store = (!a.scaled || a.num_k <= 8) && make_out_map(&mo, a.out, m, n, a.out_ld, a.out_dtype, n_shares, m * a.out_ld);
+  a.tma_store = (!a.scaled || (a.num_k <= 8 && !a.carry)) && make_out_map(&mo, a.out, m, n, a.out_ld, a.out_dtype, n_shares, m * a.out_ld);
   if (!a.scaled && !a.tma_store) {
     set_error("planes of %lld x %lld sums take no tensor map", (long long)m, (long long)n);
     return TTHRML_ERR_CUDA;
@@ -1003,12 +1014,16 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     if (rc) return rc;
     if (dx) {
       XentArgs d = base;
-      d.scaled = !f.dx_planes;
-      d.out = f.dx_planes ? (void*)(ws + f.dx) : dx;
-      d.out_ld = f.dx_planes ? f.plane_ld : dx_ld;
-      d.out_dtype = f.dx_planes ? TTHRML_DT_F32 : grad_dtype;
+      const bool ends = f.dx_planes && f.dx_shares == 1 && !f.second && i + 1 == f.pieces;  // takes the plane's sums along
+      const bool planes = f.dx_planes && !ends;
+      d.scaled = !planes;
+      d.out = planes ? (void*)(ws + f.dx) : dx;
+      d.out_ld = planes ? f.plane_ld : dx_ld;
+      d.out_dtype = planes ? TTHRML_DT_F32 : grad_dtype;
       d.align = alignment(dx, dx_ld);
-      d.accumulate = i > 0;
+      d.accumulate = planes && i > 0;
+      d.carry = ends ? (const float*)(ws + f.dx) : nullptr;
+      d.carry_ld = f.plane_ld;
       rc = product<false>(mg, mw_mn, d, f.g_rows, p->cols, width, std::min(f.dx_shares, up(width, 64) / 64), pairs, st);
       if (rc) return rc;
     }
@@ -1039,7 +1054,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
       if (rc) return rc;
     }
   }
-  if (rc == TTHRML_OK && dx && f.dx_planes)
+  if (rc == TTHRML_OK && dx && f.dx_planes && (f.dx_shares > 1 || f.second))
     rc = join_planes((const float*)(ws + f.dx), f.g_rows * f.plane_ld, f.plane_ld, p->rows, p->cols, f.second, f.dx_shares, base, dx,
                      dx_ld, grad_dtype, st);
   return rc;

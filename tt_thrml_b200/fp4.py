@@ -257,10 +257,10 @@ def fp4_product(x, weights: Fp4Rows, *, bias=None, out_dtype=None, out=None):
             )
             return out
         rows = _readable(x.reshape(-1, K))
-        size = lib.tthrml_fp4_linear_workspace(rows.shape[0], K)
-        space = torch.empty(size, dtype=torch.uint8, device=dev)
+        size = lib.tthrml_fp4_linear_workspace(rows.shape[0], K, N)
+        space = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         nat.check(
-            lib.tthrml_fp4_linear(rows.data_ptr(), code, rows.shape[0], K, rows.stride(0), 1, space.data_ptr(), size, *w_at, N,
+            lib.tthrml_fp4_linear(rows.data_ptr(), code, rows.shape[0], K, rows.stride(0), 1, nat.ptr(space), size, *w_at, N,
                                   nat.ptr(bias), out.data_ptr(), out_code, out_ld, error, stream),
             "tthrml_fp4_linear",
         )
