@@ -48,3 +48,107 @@ def test_values_and_gradients(tt, shape, dtype, p):
     assert torch.equal(y.detach().cpu(), plain(x, p, seed, step))
     y.backward(g.cuda())
     assert torch.equal(a.grad.cpu(), plain(g, p, seed, step))
+
+
+def test_dropped_elements_are_zero_whatever_they_held(tt):
+    x = torch.full((1000,), np.inf, device="cuda")
+    x[::3] = np.nan
+    y = tt.dropout(x, 0.4, seed=3)
+    keep = torch.from_numpy(half_words(1000, 3, 0) >= round(65536 * 0.4)).cuda()
+    assert (y[~keep] == 0).all() and torch.equal(torch.isnan(y), keep & torch.isnan(x)) and (y[keep & ~torch.isnan(x)] == np.inf).all()
+    assert (tt.dropout(x, 1.0, seed=3) == 0).all()
+
+
+@pytest.mark.parametrize("layout", ["transposed", "sliced", "shifted", "expanded gradient", "scalar", "empty"])
+def test_strides_and_shapes(tt, layout):
+    x = torch.randn(40, 56, device="cuda")
+    if layout == "transposed":
+        x = x.t()
+    elif layout == "sliced":
+        x = x[::2, 3:50]
+    elif layout == "shifted":
+        x = torch.randn(40 * 56 + 1, device="cuda")[1:].view(40, 56)
+    elif layout == "scalar":
+        x = x[0, 0]
+    elif layout == "empty":
+        x = x[:0]
+    a = x.detach().requires_grad_(True)
+    y = tt.dropout(a, 0.3, seed=5, step=2)
+    assert torch.equal(y.detach().cpu(), plain(x.cpu(), 0.3, 5, 2))
+    (g,) = torch.autograd.grad(y.sum(), a)  # an expanded gradient
+    assert torch.equal(g.cpu(), plain(torch.ones(x.shape), 0.3, 5, 2))
+
+
+def test_gradient_of_the_gradient(tt):
+    x = torch.randn(100, device="cuda", dtype=torch.float32, requires_grad=True)
+    g = torch.randn(100, device="cuda", requires_grad=True)
+    y = tt.dropout(x, 0.5, seed=9)
+    (gx,) = torch.autograd.grad(y, x, g, create_graph=True)
+    (gg,) = torch.autograd.grad(gx.square().sum(), g)
+    mask = plain(torch.ones(100), 0.5, 9, 0).cuda()
+    assert torch.equal(gg, 2 * g * mask * mask)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_step_on_the_device(tt, kind):
+    """A captured forward and backward takes another mask when the step was changed, and the backward pass its own forward
+    pass's mask even when the step has moved on."""
+    x = torch.randn(500, device="cuda", requires_grad=True)
+    g = torch.randn(500, device="cuda")
+    step = torch.zeros(1, dtype=kind, device="cuda")
+    y = tt.dropout(x, 0.5, seed=2, step=step)
+    step += 1
+    (gx,) = torch.autograd.grad(y, x, g)
+    assert torch.equal(gx.cpu(), plain(g.cpu(), 0.5, 2, 0))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        z = x.detach().clone().requires_grad_(True)
+        torch.autograd.grad(tt.dropout(z, 0.5, seed=2, step=step), z, g)
+        with torch.cuda.graph(graph, stream=side):
+            y = tt.dropout(z, 0.5, seed=2, step=step)
+            step += 1
+            (gz,) = torch.autograd.grad(y, z, g)
+    torch.cuda.synchronize()
+    for k in range(3):
+        step.fill_(2**31 - 1 + k if kind == torch.int32 and k == 0 else 10 + k)
+        torch.cuda.synchronize()
+        now = int(step)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.detach().cpu(), plain(z.detach().cpu(), 0.5, 2, now))
+        assert torch.equal(gz.cpu(), plain(g.cpu(), 0.5, 2, now))
+
+
+def test_more_than_2_to_the_32_elements(tt):
+    n = 2**32 + 100
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = tt.dropout(x, 0.5, seed=77, step=1)
+    for first in (0, 2**29 - 4, 2**29):  # groups of eight elements
+        m = min(64, n - 8 * first)
+        keep = half_words(m, 77, 1, first) >= 32768
+        assert np.array_equal((y[8 * first : 8 * first + m] != 0).cpu().numpy(), keep)
+
+
+def test_mean_is_kept(tt):
+    """2^24 draws at p = 0.1: the mean of the kept ones within six standard deviations of 1."""
+    n = 2**24
+    y = tt.dropout(torch.ones(n, device="cuda"), 0.1, seed=4)
+    p = round(6553.6) / 65536
+    assert abs(float(y.double().mean()) - 1) < 6 * (p / (1 - p) / n) ** 0.5
+
+
+def test_refusals(tt):
+    x = torch.ones(8, device="cuda")
+    for kw, match in [({"p": 1.5}, "between 0 and 1"), ({"p": float("nan")}, "between 0 and 1"), ({"seed": -1}, "seed"),
+                      ({"seed": 2**64}, "seed"), ({"step": -1}, "step"), ({"step": 2**32}, "step"),
+                      ({"step": torch.zeros(2, dtype=torch.int64, device="cuda")}, "step"),
+                      ({"step": torch.zeros(1, device="cuda")}, "step"),
+                      ({"step": torch.zeros(1, dtype=torch.int64)}, "CUDA")]:
+        with pytest.raises(ValueError, match=match):
+            tt.dropout(x, **({"p": 0.5, "seed": 1} | kw))
+    with pytest.raises(ValueError, match="float32"):
+        tt.dropout(x.int(), 0.5, seed=1)
+    with pytest.raises(ValueError, match="CUDA"):
+        tt.dropout(x.cpu(), 0.5, seed=1)

@@ -7,7 +7,10 @@ make_mesh_executor/MeshExecutor, GaussianConditional, the device helpers and
 the configuration factory (make_cuda_config; make_ttmlir_config kept for
 drop-in callers).  Around dense programs: 8-bit integer products
 (quantize_rows, int8_product), pair moments (pair_moments, dense_moments),
-AdamW over many tensors and DenseLearner.
+AdamW over many tensors and DenseLearner.  For categories read out of a block's
+units: softmax cross entropy without logits (softmax_cross_entropy), dropout,
+4-bit floating point products (quantize_fp4, fp4_product) and
+CategoricalReadout.
 """
 
 from .compiler import compile_program
@@ -41,6 +44,7 @@ from .mesh import MeshExecutor, make_mesh_executor, mesh_barrier, mesh_device_id
 from .moments import pair_moments
 from .optim import AdamW
 from .quantized import QuantizedRows, check_operator_errors, int8_product, quantize_rows
+from .readout import CategoricalReadout
 from .regularise import dropout
 from .rng import generate_bulk_rng, make_rng_spec, slice_rng_for_sweep
 
@@ -113,4 +117,5 @@ __all__ = [
     "Fp4Rows",
     "quantize_fp4",
     "fp4_product",
+    "CategoricalReadout",
 ]

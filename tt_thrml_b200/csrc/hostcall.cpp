@@ -264,6 +264,9 @@ PyMethodDef methods[] = {
      "Takes the addresses of the library's entry points."},
     {"softmax_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::softmax_cross_entropy)), METH_FASTCALL,
      "Losses of checked tensors, differentiable."},
+    {"softmax_cross_entropy_gradients",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::softmax_cross_entropy_gradients)), METH_FASTCALL,
+     "The mean loss of checked tensors, its gradients written."},
     {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::dropout)), METH_FASTCALL,
      "Kept elements of a checked tensor, differentiable."},
     {"quantize_fp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(hostcall::quantize_fp4)), METH_FASTCALL,

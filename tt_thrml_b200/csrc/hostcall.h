@@ -47,6 +47,7 @@ extern Library library;
 
 PyObject* bind_library(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 PyObject* softmax_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t nargs);
+PyObject* softmax_cross_entropy_gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 PyObject* quantize_fp4(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 PyObject* fp4_values(PyObject*, PyObject* const* args, Py_ssize_t nargs);

@@ -57,17 +57,20 @@ struct Operand {
   const void* at;
   int64_t ld;
 };
+bool as_it_lies(const Tensor& t, Operand& o) {
+  const int64_t rows = t.size(0), cols = t.size(1);
+  o.at = t.const_data_ptr();
+  o.ld = rows > 1 ? t.stride(0) : (cols + 7) / 8 * 8;
+  return (cols == 1 || t.stride(1) == 1) && o.ld % 8 == 0 && o.ld >= cols && reinterpret_cast<uintptr_t>(o.at) % 16 == 0;
+}
 Tensor lay_out(const Tensor& x, const Tensor& w, Operand (&o)[2], void* stream) {
   const Tensor* t[2] = {&x, &w};
   tthrml_pack_matrix m[2];
   int which[2], n = 0;
   int64_t size = 0;
   for (int i = 0; i < 2; ++i) {
+    if (as_it_lies(*t[i], o[i])) continue;
     const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
-    o[i].at = t[i]->const_data_ptr();
-    o[i].ld = rows > 1 ? t[i]->stride(0) : (cols + 7) / 8 * 8;
-    if ((cols == 1 || t[i]->stride(1) == 1) && o[i].ld % 8 == 0 && o[i].ld >= cols && reinterpret_cast<uintptr_t>(o[i].at) % 16 == 0)
-      continue;
     o[i].ld = (cols + 7) / 8 * 8;
     m[n] = {o[i].at, reinterpret_cast<void*>(size * 2), rows, cols, t[i]->stride(0), t[i]->stride(1), o[i].ld};
     size += rows * o[i].ld;
@@ -82,6 +85,18 @@ Tensor lay_out(const Tensor& x, const Tensor& w, Operand (&o)[2], void* stream) 
   }
   check(library.pack_rows(m, n, stream), "tthrml_pack_rows");
   return space;
+}
+
+// The same operands once more, from the buffer that lay_out returned.
+void held_operands(const Tensor& x, const Tensor& w, const Tensor& laid, Operand (&o)[2]) {
+  const Tensor* t[2] = {&x, &w};
+  const char* base = laid.defined() ? static_cast<const char*>(laid.const_data_ptr()) : nullptr;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
+    if (as_it_lies(*t[i], o[i])) continue;
+    o[i] = {base, (cols + 7) / 8 * 8};
+    base += rows * o[i].ld * 2;
+  }
 }
 
 struct XentSaved {
@@ -125,6 +140,21 @@ Tensor xent_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const 
   return reduction ? total : rows;
 }
 
+// Gradients into dx and dw (one type, dense rows) and db, each may be undefined.
+void xent_backward(const Tensor& x, const tthrml_xent& p, const Tensor& log2_z, const Tensor& grad, const Tensor& inv_count,
+                   const Tensor& dx, const Tensor& dw, const Tensor& db, int64_t error, void* stream) {
+  const int64_t size = library.xent_backward_workspace(p.rows, p.categories, p.cols, dx.defined(), dw.defined(), db.defined());
+  if (size < 0) check((int)size, "tthrml_xent_backward_workspace");
+  const Tensor space = bytes(x, size);
+  check(library.xent_backward(&p, log2_z.const_data_ptr<float>(), grad.const_data_ptr<float>(), grad.dim() ? 1 : 0,
+                              inv_count.defined() ? inv_count.const_data_ptr<float>() : nullptr,
+                              dx.defined() ? dx.mutable_data_ptr() : nullptr, p.cols, dw.defined() ? dw.mutable_data_ptr() : nullptr,
+                              p.cols, dx.defined() ? dtype_code(dx) : (dw.defined() ? dtype_code(dw) : p.dtype),
+                              db.defined() ? db.mutable_data_ptr<float>() : nullptr, space.mutable_data_ptr(), size,
+                              reinterpret_cast<int32_t*>(error), stream),
+        "tthrml_xent_backward");
+}
+
 struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
   // every argument of a node is a defined tensor: without a bias the targets stand in its place
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& bias_or_targets, const Tensor& targets,
@@ -146,33 +176,13 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
     if (!grads[0].defined()) return out;
     const On on(x);
     Operand o[2];
-    const Tensor *t[2] = {&x, &w};
-    const char* base = laid.defined() ? static_cast<const char*>(laid.const_data_ptr()) : nullptr;
-    for (int i = 0; i < 2; ++i) {  // as lay_out left them
-      const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
-      o[i].at = t[i]->const_data_ptr();
-      o[i].ld = rows > 1 ? t[i]->stride(0) : (cols + 7) / 8 * 8;
-      if ((cols == 1 || t[i]->stride(1) == 1) && o[i].ld % 8 == 0 && o[i].ld >= cols && reinterpret_cast<uintptr_t>(o[i].at) % 16 == 0)
-        continue;
-      o[i].ld = (cols + 7) / 8 * 8;
-      o[i].at = base;
-      base += rows * o[i].ld * 2;
-    }
+    held_operands(x, w, laid, o);
     const tthrml_xent p = problem(x, w, bias, targets, ctx->saved_data["ignored"].toInt(), o);
     const Tensor grad = grads[0].to(at::kFloat).contiguous();
     if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().requires_grad(false));
     if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options().requires_grad(false));
     if (bias.defined() && ctx->needs_input_grad(2)) out[2] = floats(x, bias.sizes());
-    const int64_t size = library.xent_backward_workspace(p.rows, p.categories, p.cols, out[0].defined(), out[1].defined(), out[2].defined());
-    if (size < 0) check((int)size, "tthrml_xent_backward_workspace");
-    const Tensor space = bytes(x, size);
-    check(library.xent_backward(&p, log2_z.const_data_ptr<float>(), grad.const_data_ptr<float>(), grad.dim() ? 1 : 0,
-                                inv_count.defined() ? inv_count.const_data_ptr<float>() : nullptr,
-                                out[0].defined() ? out[0].mutable_data_ptr() : nullptr, p.cols,
-                                out[1].defined() ? out[1].mutable_data_ptr() : nullptr, p.cols, p.dtype,
-                                out[2].defined() ? out[2].mutable_data_ptr<float>() : nullptr, space.mutable_data_ptr(), size,
-                                reinterpret_cast<int32_t*>(ctx->saved_data["error"].toInt()), on.stream()),
-          "tthrml_xent_backward");
+    xent_backward(x, p, log2_z, grad, inv_count, out[0], out[1], out[2], ctx->saved_data["error"].toInt(), on.stream());
     return out;
   }
 };
@@ -236,6 +246,29 @@ PyObject* softmax_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t nar
                                                        ignored, error));
   XentSaved s;
   return THPVariable_Wrap(xent_forward(x, w, bias, targets, reduction, ignored, error, s));
+  END_HANDLE_TH_ERRORS
+}
+
+// softmax_cross_entropy_gradients(x, weights, bias, targets, ignored, error word, one, dw, db) -> the mean loss, with its
+// gradients in dw (float32 or the weights' type, dense) and db; no node of a graph.  one: the float32 number 1 on the device.
+PyObject* softmax_cross_entropy_gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) {
+    PyErr_SetString(PyExc_TypeError, "softmax_cross_entropy_gradients(x, weights, bias, targets, ignored, error, one, dw, db)");
+    return nullptr;
+  }
+  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &bias = THPVariable_Unpack(args[2]);
+  const Tensor targets = THPVariable_Unpack(args[3]).contiguous();
+  const int64_t ignored = PyLong_AsLongLong(args[4]), error = PyLong_AsLongLong(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor &unit = THPVariable_Unpack(args[6]), &dw = THPVariable_Unpack(args[7]), &db = THPVariable_Unpack(args[8]);
+  const On on(x);
+  XentSaved s;
+  Tensor loss = xent_forward(x, w, bias, targets, 1, ignored, error, s);
+  Operand o[2];
+  held_operands(x, w, s.laid, o);
+  xent_backward(x, problem(x, w, bias, targets, ignored, o), s.log2_z, unit, s.inv_count, Tensor(), dw, db, error, on.stream());
+  return THPVariable_Wrap(loss);
   END_HANDLE_TH_ERRORS
 }
 

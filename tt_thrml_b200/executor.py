@@ -1162,6 +1162,17 @@ class Executor:
             if i + j < 3
         ]
 
+    def dense_units(self, block: int):
+        """The current values of a block of a dense program as a bfloat16 matrix [chains, units] on the device (spins as +-1;
+        gaussians rounded), current on this executor's stream until its next sweep."""
+        torch = _torch()
+        self._dense_plans("dense units")
+        if not self._state_loaded:
+            raise RuntimeError("State must be loaded before reading units")
+        state = self._block_states[block][:, : self.compiled.blocks[block].spec.n_nodes]
+        with torch.cuda.stream(self._stream):
+            return state.to(torch.bfloat16)  # bfloat16 states as they lie
+
     def dense_moments(self, scale: float = 1.0, *, out=None, accumulate: bool = False):
         """Moments of a dense program's current states over the chains, in float32: (pair [n_0, n_1], sums of
         block 0 [n_0], sums of block 1 [n_1]), each times `scale`; spins as +-1.  `out` receives them, or with

@@ -26,23 +26,7 @@ def _torch():
     return torch
 
 
-def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", ignore_index=-100):
-    """Minus the log likelihood of the target categories under softmax(x weights^T + bias), differentiable in x, weights
-    and bias.
-
-    x: bfloat16 or float16 [..., K]; weights: the same type [V, K], any strides
-    (rows that are not 16-byte aligned are laid out again in each call); targets:
-    int64 or int32 [...]; bias: float32 [V], -inf for categories that cannot occur.
-    reduction "mean" (over the rows that count), "sum" (float32 scalars) or "none"
-    (float32 [...]).  Rows whose target is `ignore_index` do not count: loss 0, no
-    gradient (their values must be finite, as 0 times them is added to the weights'
-    gradient); a mean over no rows is 0.  A target outside 0 .. V - 1 gives NaN.  A
-    row in which no category can occur has loss inf and no gradient.
-
-    Sums and normalisers are float32; the gradients are products of 16-bit
-    differences, accumulated in float32.  The result is the same every time.
-    Gradients of gradients and forward-mode derivatives are not available.
-    """
+def _check(x, weights, targets, bias) -> None:
     torch = _torch()
     require_cuda("x", x)
     dev = x.device
@@ -65,12 +49,46 @@ def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", i
         require_cuda("bias", bias, dev)
         if bias.dtype != torch.float32 or bias.shape != (V,):
             raise ValueError(f"bias must be float32 of shape ({V},), got {bias.dtype} of {tuple(bias.shape)}")
+    rows = targets.numel()
+    if rows > nat.XENT_MAX_ROWS:
+        raise ValueError(f"at most {nat.XENT_MAX_ROWS} rows are supported, got {rows}")
+
+
+def mean_and_gradients(x, weights, targets, bias, ignore_index, one, dw, db):
+    """The mean loss of x [rows, K], a float32 scalar on the device, with its gradients written into dw [V, K] (float32 or
+    weights' type, dense) and db; nothing of it is recorded for autograd.  one: the float32 number 1 on x's device."""
+    _check(x, weights, targets, bias)
+    if x.dim() != 2 or not x.shape[0]:
+        raise ValueError(f"x must hold rows of units, got shape {tuple(x.shape)}")
+    word = _error_addresses.get(x.device.index) or error_word(x.device).data_ptr()
+    return nat.bound_hostcall().softmax_cross_entropy_gradients(x, weights, bias, targets, int(ignore_index), word, one, dw, db)
+
+
+def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", ignore_index=-100):
+    """Minus the log likelihood of the target categories under softmax(x weights^T + bias), differentiable in x, weights
+    and bias.
+
+    x: bfloat16 or float16 [..., K]; weights: the same type [V, K], any strides
+    (rows that are not 16-byte aligned are laid out again in each call); targets:
+    int64 or int32 [...]; bias: float32 [V], -inf for categories that cannot occur.
+    reduction "mean" (over the rows that count), "sum" (float32 scalars) or "none"
+    (float32 [...]).  Rows whose target is `ignore_index` do not count: loss 0, no
+    gradient (their values must be finite, as 0 times them is added to the weights'
+    gradient); a mean over no rows is 0.  A target outside 0 .. V - 1 gives NaN.  A
+    row in which no category can occur has loss inf and no gradient.
+
+    Sums and normalisers are float32; the gradients are products of 16-bit
+    differences, accumulated in float32.  The result is the same every time.
+    Gradients of gradients and forward-mode derivatives are not available.
+    """
+    torch = _torch()
+    _check(x, weights, targets, bias)
+    V, K = weights.shape
+    dev = x.device
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
     lead = x.shape[:-1]
     rows = targets.numel()
-    if rows > nat.XENT_MAX_ROWS:
-        raise ValueError(f"at most {nat.XENT_MAX_ROWS} rows are supported, got {rows}")
     if rows == 0:  # nothing counts
         zero = x.sum(-1).float() + weights[:0].sum().float() + (0.0 if bias is None else bias[:0].sum())
         return zero if reduction == "none" else zero.sum()
