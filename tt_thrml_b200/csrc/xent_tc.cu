@@ -10,7 +10,8 @@
 //
 // One kernel serves the four products: persistent clusters of two CTAs walk 256 x BN tiles (tcgen05 cta_group::2, two
 // TMEM accumulators, six stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
-// transposed.  Warp 0 loads (TMA), warp 1 of the even CTA multiplies, warps 2-9 run the epilogue of a tile under the main
+// transposed.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for half the weights, which
+// are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the even CTA multiplies, warps 2-9 run the epilogue of a tile under the main
 // loop of the next one.
 //
 // g is rounded to the operands' 16 bits (up to kFewRows rows: held in two such pieces, their sum good to 2^-16; the
@@ -89,10 +90,10 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-template <int BN>
+template <int BN, int CTAS>
 struct XentShape {
-  static constexpr int kA = 128 * 64 * 2, kB = BN / 2 * 64 * 2, kStage = kA + kB;
-  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kA = 128 * 64 * 2, kB = BN / CTAS * 64 * 2, kStage = kA + kB;
+  static constexpr int kStages = kStage >= 49152 ? 4 : (kStage >= 32768 ? 6 : 8);
   static constexpr int kBarriers = 256;
   static constexpr int kSmem = 1024 + kStages * kStage + kEpilogueWarps * kOutBytes + kBarriers + 256 * 4 /*biases*/;
 };
@@ -117,9 +118,18 @@ __device__ __forceinline__ void less_row(float (&v)[32], int32_t dtype, const ui
   }
 }
 
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (CTAS == 2)
+    umma_commit_pair(bar);
+  else
+    umma_commit(bar);
+}
+
 // Unit u -> its split, row of tiles and segment: splits slowest, `group` rows of tiles at a time.
+template <int ROWS>
 __device__ __forceinline__ void unit_at(const XentArgs& a, int u, int& split, int& mb, int& sg) {
-  const int m_blocks = (a.M + 255) / 256, all = m_blocks * a.segments;
+  const int m_blocks = (a.M + ROWS - 1) / ROWS, all = m_blocks * a.segments;
   split = u / all;
   const int t = u - split * all, per = a.group * a.segments, g = t / per, w = t - g * per;
   const int rows = min(a.group, m_blocks - g * a.group);
@@ -148,12 +158,13 @@ __device__ __forceinline__ float column_sums(const float (&v)[32], uint32_t buff
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <int EPI, bool A_MN, bool B_MN, int BN>
+template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS>
 __global__ void __launch_bounds__(kThreads, 1)
     k_xent(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
            const __grid_constant__ CUtensorMap map_out, const __grid_constant__ XentArgs a) {
-  using S = XentShape<BN>;
-  static_assert(!B_MN || BN == 256, "MN-major halves of B are whole boxes of 64");
+  using S = XentShape<BN, CTAS>;
+  constexpr int kRows = 128 * CTAS;  // of a tile
+  static_assert(!B_MN || (BN == 256 && CTAS == 2), "MN-major halves of B are whole boxes of 64");
   constexpr bool kChunked = EPI == kPartials || EPI == kGradientSums;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -178,14 +189,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * kEpilogueWarps);  // every epilogue warp of both CTAs
+      mbar_init(&acc_empty[b], CTAS * kEpilogueWarps);  // every epilogue warp of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                 "r"(512u));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    if (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(512u));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(512u));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
   }
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers exist before either signals the other
@@ -201,11 +218,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool failed = false;
     for (int u = first; u < a.units && !failed; u += step) {
       int split, mb, sg;
-      unit_at(a, u, split, mb, sg);
+      unit_at<kRows>(a, u, split, mb, sg);
       const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
-      const int m0 = mb * 256 + (int)rank * 128;
+      const int m0 = mb * kRows + (int)rank * 128;
       for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb) {
-        const int n0 = nb * BN + (int)rank * (BN / 2);
+        const int n0 = nb * BN + (int)rank * (BN / CTAS);
         for (int kb = k_first; kb < k_last; ++kb) {
           const int s = (int)(issued % S::kStages);
           if (!mbar_wait_all(&empty[s], ((uint32_t)(issued / S::kStages) & 1u) ^ 1u)) {
@@ -214,16 +231,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           if (one) {
-            if (leader) mbar_expect_tx(&full[s], 2 * S::kStage);  // the stage's bytes of both CTAs
+            if (leader) mbar_expect_tx(&full[s], CTAS * S::kStage);  // the stage's bytes of both CTAs
             unsigned char* st = tiles + s * S::kStage;
             const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
-            if (A_MN) {
+            if (CTAS == 1) {
+              tma_load_2d(st, &map_a, &full[s], kb * 64, m0);
+              tma_load_2d(st + S::kA, &map_b, &full[s], kb * 64, n0);
+            } else if (A_MN) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) tma_load_2d_pair(st + i * 8192, &map_a, bar, m0 + 64 * i, kb * 64);
             } else {
               tma_load_2d_pair(st, &map_a, bar, kb * 64, m0);
             }
-            if (B_MN) {
+            if (CTAS == 1) {
+            } else if (B_MN) {
 #pragma unroll
               for (int i = 0; i < BN / 128; ++i)
                 tma_load_2d_pair(st + S::kA + i * 8192, &map_b, bar, n0 + 64 * i, (a.second && kb >= a.second ? kb - a.second : kb) * 64);
@@ -244,13 +265,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool one = elect_one();
       const uint32_t type = a.f16 ? 0u : 1u;
       const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                             ((uint32_t)(BN >> 3) << 17) | (16u << 24);  // D float32, M = 256
+                             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);  // D float32, M = 128 or 256
       int64_t used = 0;
       int it = 0;  // accumulations so far
       bool failed = false;
       for (int u = first; u < a.units && !failed; u += step) {
         int split, mb, sg;
-        unit_at(a, u, split, mb, sg);
+        unit_at<kRows>(a, u, split, mb, sg);
         const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
         for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks) && !failed; ++nb) {
           for (int k0 = k_first; k0 < k_last && !failed; k0 += a.chunk, ++it) {
@@ -275,15 +296,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint64_t bd = B_MN ? umma_desc_mn128(st + S::kA) : umma_desc_sw128(st + S::kA);
               if (one) {
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)  // 16 of K per MMA: 32 bytes of each row, or two groups of eight rows
-                  umma_f16_pair(d, ad + (A_MN ? 128ull : 2ull) * kk, bd + (B_MN ? 128ull : 2ull) * kk, idesc,
-                                (kb > k0 || kk > 0) ? 1u : 0u);
-                umma_commit_pair(&empty[s]);  // the stage is free again in both CTAs
+                for (int kk = 0; kk < 4; ++kk) {  // 16 of K per MMA: 32 bytes of each row, or two groups of eight rows
+                  const uint64_t a_desc = ad + (A_MN ? 128ull : 2ull) * kk, b_desc = bd + (B_MN ? 128ull : 2ull) * kk;
+                  if (CTAS == 2)
+                    umma_f16_pair(d, a_desc, b_desc, idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+                  else
+                    umma_f16(d, a_desc, b_desc, idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+                }
+                commit<CTAS>(&empty[s]);  // the stage is free again in both CTAs
               }
               __syncwarp();
               ++used;
             }
-            if (one) umma_commit_pair(&acc_full[b]);  // both CTAs' accumulator halves complete
+            if (one) commit<CTAS>(&acc_full[b]);  // both CTAs' accumulator halves complete
             __syncwarp();
             last_it[b] = it;
           }
@@ -298,9 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool failed = false;
     for (int u = first; u < a.units; u += step) {
       int split, mb, sg;
-      unit_at(a, u, split, mb, sg);
+      unit_at<kRows>(a, u, split, mb, sg);
       const int k_first = (int)((int64_t)a.num_k * split / a.splits), k_last = (int)((int64_t)a.num_k * (split + 1) / a.splits);
-      const int m = mb * 256 + (int)rank * 128 + quad * 32 + lane;
+      const int m = mb * kRows + (int)rank * 128 + quad * 32 + lane;
       float top = -INFINITY, sum = 0.0f;  // kPartials: sum 2^top
       int64_t y = -1;                     // column of the row's target
       float weight = 0.0f, log2_z = 0.0f, factor = 1.0f;
@@ -517,7 +542,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   cluster_sync_all();  // neither CTA frees TMEM or exits while the other may still signal it
   tc_fence_after();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  if (warp == 1) {
+    if (CTAS == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
 }
 
 // Joins the partial sums of a row (a warp per row) into log2 z and the row's loss; the last block adds the losses, in an
@@ -697,35 +727,41 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int
 
 constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-template <int EPI, bool A_MN, bool B_MN, int BN>
+template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS>
 int launch_xent(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const XentArgs& a, cudaStream_t st) {
-  const void* fn = (const void*)k_xent<EPI, A_MN, B_MN, BN>;
+  const void* fn = (const void*)k_xent<EPI, A_MN, B_MN, BN, CTAS>;
+  constexpr int kSmem = XentShape<BN, CTAS>::kSmem;
   ClusterFit fit;
-  const int rc = cluster_fit(fn, 2, kThreads, XentShape<BN>::kSmem, &fit);
+  const int rc = cluster_fit(fn, CTAS, kThreads, kSmem, &fit);
   if (rc) return rc;
   const int64_t clusters = a.units < fit.clusters ? a.units : fit.clusters;
   void* params[4] = {(void*)&ma, (void*)&mb, (void*)&mo, (void*)&a};
-  return launch_clusters(fn, (unsigned)(2 * clusters), 2, kThreads, XentShape<BN>::kSmem, params, st, "k_xent launch", true);
+  return launch_clusters(fn, (unsigned)(CTAS * clusters), CTAS, kThreads, kSmem, params, st, "k_xent launch", true);
+}
+template <int EPI, int CTAS>
+int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
+  if (bn == 64) return launch_xent<EPI, false, false, 64, CTAS>(ma, mb, ma, a, st);
+  if (bn == 128) return launch_xent<EPI, false, false, 128, CTAS>(ma, mb, ma, a, st);
+  return launch_xent<EPI, false, false, 256, CTAS>(ma, mb, ma, a, st);
 }
 template <int EPI>
-int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const XentArgs& a, cudaStream_t st) {
-  if (bn == 64) return launch_xent<EPI, false, false, 64>(ma, mb, mo, a, st);
-  if (bn == 128) return launch_xent<EPI, false, false, 128>(ma, mb, mo, a, st);
-  return launch_xent<EPI, false, false, 256>(ma, mb, mo, a, st);
+int launch_logits(int ctas, int bn, const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
+  return ctas == 1 ? launch_logits<EPI, 1>(bn, ma, mb, a, st) : launch_logits<EPI, 2>(bn, ma, mb, a, st);
 }
 
 // How many pairs of CTAs work at once (every form of the kernel fills an SM).
 int resident_pairs(int64_t* out) {
   ClusterFit fit;
-  const int rc = cluster_fit((const void*)k_xent<kProduct, false, true, 256>, 2, kThreads, XentShape<256>::kSmem, &fit);
+  const int rc = cluster_fit((const void*)k_xent<kProduct, false, true, 256, 2>, 2, kThreads, XentShape<256, 2>::kSmem, &fit);
   *out = fit.clusters;
   return rc;
 }
-// The widest tile that still gives every pair work.
+// CTAs per tile of logits, and the widest tile that still gives every cluster work.
+int tile_ctas(int64_t rows) { return rows <= 128 ? 1 : 2; }
 int tile_width(int64_t rows, int64_t n, int64_t pairs) {
-  const int64_t m_blocks = up(rows, 256) / 256;
+  const int64_t ctas = tile_ctas(rows), m_blocks = up(rows, 128 * ctas) / (128 * ctas), at_once = pairs * 2 / ctas;
   for (int bn = 256; bn > 64; bn /= 2)
-    if (m_blocks * (up(n, bn) / bn) >= pairs) return bn;
+    if (m_blocks * (up(n, bn) / bn) >= at_once) return bn;
   return 64;
 }
 // Tiles along N per unit: as few rounds of units as possible, then as few partial sums.
@@ -753,7 +789,8 @@ int plan_forward(int64_t rows, int64_t categories, ForwardPlan* p) {
   if (rc) return rc;
   p->bn = tile_width(rows, categories, pairs);
   const int64_t n_blocks = up(categories, p->bn) / p->bn;
-  p->seg = tiles_per_unit(up(rows, 256) / 256, n_blocks, pairs);
+  const int64_t ctas = tile_ctas(rows);
+  p->seg = tiles_per_unit(up(rows, 128 * ctas) / (128 * ctas), n_blocks, pairs * 2 / ctas);
   p->segments = (int)((n_blocks + p->seg - 1) / p->seg);
   p->logits = up(rows * 2 * p->segments * 8, 16);
   p->counter = p->logits + up(rows * 4, 16);
@@ -838,7 +875,7 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
     set_error("planes of %lld x %lld sums take no tensor map", (long long)m, (long long)n);
     return TTHRML_ERR_CUDA;
   }
-  return launch_xent<kProduct, A_MN, true, 256>(ma, mb, mo, a, st);
+  return launch_xent<kProduct, A_MN, true, 256, 2>(ma, mb, mo, a, st);
 }
 int join_planes(const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols, int64_t second, int64_t n,
                 const XentArgs& a, void* out, int64_t out_ld, int32_t out_dtype, cudaStream_t st) {
@@ -880,9 +917,10 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = p->dtype == TTHRML_DT_F16;
   unsigned char* ws = (unsigned char*)workspace;
+  const int ctas = tile_ctas(p->rows);
   CUtensorMap ma, mb;
   rc = make_map(&ma, p->x, p->rows, p->cols, p->x_ld, 128u, f16);
-  if (rc == TTHRML_OK) rc = make_map(&mb, p->w, p->categories, p->cols, p->w_ld, (uint32_t)f.bn / 2, f16);
+  if (rc == TTHRML_OK) rc = make_map(&mb, p->w, p->categories, p->cols, p->w_ld, (uint32_t)(f.bn / ctas), f16);
   if (rc) return rc;
   XentArgs a = {};
   a.M = (int32_t)p->rows;
@@ -892,7 +930,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.seg = f.seg;
   a.segments = f.segments;
   a.splits = 1;
-  const int64_t m_blocks = up(p->rows, 256) / 256, g = ((int64_t)32 << 20) / (512 * p->cols);
+  const int64_t m_blocks = up(p->rows, 128 * ctas) / (128 * ctas), g = ((int64_t)32 << 20) / (512 * p->cols);
   a.units = (int32_t)(m_blocks * f.segments);
   a.group = (int32_t)std::max<int64_t>(1, std::min(g, m_blocks));  // raster groups of about 32 MiB of A panels
   a.bias = p->bias;
@@ -904,7 +942,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.counter = (uint32_t*)(ws + f.counter);
   a.error = error;
   a.chunk = kChunk;
-  rc = launch_logits<kPartials>(f.bn, ma, mb, ma, a, st);
+  rc = launch_logits<kPartials>(ctas, f.bn, ma, mb, a, st);
   if (rc) return rc;
   LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, log2_z, row_loss, loss, inv_count,
                 a.counter};
@@ -982,8 +1020,8 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
     const char* w = (const char*)p->w + first * p->w_ld * 2;
     CUtensorMap mw, mw_mn, mg, mg_mn;
-    const int bn = tile_width(p->rows, width, pairs);
-    rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)bn / 2, f16);
+    const int bn = tile_width(p->rows, width, pairs), ctas = tile_ctas(p->rows);
+    rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)(bn / ctas), f16);
     if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
     if (rc == TTHRML_OK) rc = make_map(&mg, ws, f.g_rows, width, f.g_ld, 128u, f16);
     if (rc == TTHRML_OK) rc = make_map(&mg_mn, ws, f.g_rows, width, f.g_ld, 64u, f16);
@@ -995,7 +1033,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     a.seg = 1;
     a.segments = (int32_t)(up(width, bn) / bn);
     a.splits = 1;
-    const int64_t m_blocks = up(p->rows, 256) / 256;
+    const int64_t m_blocks = up(p->rows, 128 * ctas) / (128 * ctas);
     a.units = (int32_t)(m_blocks * a.segments);
     int64_t g = 1;
     while ((g + 1) * (g + 1) <= pairs) ++g;
@@ -1010,7 +1048,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     a.out = ws;
     a.out_ld = f.g_ld;
     a.out_dtype = p->dtype;
-    rc = db ? launch_logits<kGradientSums>(bn, mx, mw, mx, a, st) : launch_logits<kGradient>(bn, mx, mw, mx, a, st);
+    rc = db ? launch_logits<kGradientSums>(ctas, bn, mx, mw, a, st) : launch_logits<kGradient>(ctas, bn, mx, mw, a, st);
     if (rc) return rc;
     if (dx) {
       XentArgs d = base;
