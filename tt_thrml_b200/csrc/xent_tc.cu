@@ -44,6 +44,7 @@ struct XentArgs {
   int32_t M, N;       // the product's rows and columns
   int32_t num_k;      // 64-wide blocks of its sum
   int32_t f16;
+  int32_t box_m;      // rows per load of A (16, 32, 64 or 128); those behind are whatever the stage held, and not used
   int32_t chunk;      // blocks of K per accumulation
   int32_t units, segments, seg, splits, group;  // units of work: `seg` tiles along N of one row of tiles and one share of K
   // epilogues of logits: N categories from `first` on
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync_all();  // both CTAs' barriers exist before either signals the other
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  let_next_kernel_start();  // its setup beside this kernel; it waits for this one's end as this one does here
   wait_for_previous_kernel();
   if (EPI == kPartials && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0u;
   int last_it[2] = {-1, -1};
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           if (one) {
-            if (leader) mbar_expect_tx(&full[s], CTAS * S::kStage);  // the stage's bytes of both CTAs
+            if (leader) mbar_expect_tx(&full[s], CTAS == 2 ? 2 * S::kStage : S::kB + a.box_m * 128);  // the stage's bytes of both CTAs
             unsigned char* st = tiles + s * S::kStage;
             const uint32_t bar = smem_u32(&full[s]) & kPeerMask;
             if (CTAS == 1) {
@@ -566,6 +568,7 @@ __global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
   __shared__ double sums[8];
   __shared__ int64_t counts[8];
   __shared__ bool last;
+  let_next_kernel_start();
   wait_for_previous_kernel();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + warp;
@@ -632,6 +635,7 @@ __global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
 // The largest magnitude of the weights of the rows that count; one block.
 __global__ void __launch_bounds__(1024) k_xent_top(const float* grad, RowTargets targets, int64_t rows, float* top) {
   __shared__ float part[32];
+  let_next_kernel_start();
   wait_for_previous_kernel();
   float most = 0.0f;
   for (int64_t i = threadIdx.x; i < rows; i += 1024)
@@ -659,6 +663,7 @@ struct JoinArgs {
   float unit;
 };
 __global__ void __launch_bounds__(256) k_xent_join(const JoinArgs a) {
+  let_next_kernel_start();
   wait_for_previous_kernel();
   const float factor = factor_of(a.factor) / a.unit;
   const int64_t quads = (a.cols + 3) / 4, all = a.rows * quads;
@@ -691,6 +696,7 @@ __global__ void __launch_bounds__(256) k_xent_join(const JoinArgs a) {
 __global__ void __launch_bounds__(256) k_xent_bias(const float* part, int64_t groups, int64_t ld, int64_t n, float* db,
                                                    const float* f0, const float* f1, float unit) {
   __shared__ float sums[8][33];
+  let_next_kernel_start();
   wait_for_previous_kernel();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
@@ -758,6 +764,7 @@ int resident_pairs(int64_t* out) {
 }
 // CTAs per tile of logits, and the widest tile that still gives every cluster work.
 int tile_ctas(int64_t rows) { return rows <= 128 ? 1 : 2; }
+int box_rows(int64_t rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128)); }
 int tile_width(int64_t rows, int64_t n, int64_t pairs) {
   const int64_t ctas = tile_ctas(rows), m_blocks = up(rows, 128 * ctas) / (128 * ctas), at_once = pairs * 2 / ctas;
   for (int bn = 256; bn > 64; bn /= 2)
@@ -919,7 +926,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   unsigned char* ws = (unsigned char*)workspace;
   const int ctas = tile_ctas(p->rows);
   CUtensorMap ma, mb;
-  rc = make_map(&ma, p->x, p->rows, p->cols, p->x_ld, 128u, f16);
+  rc = make_map(&ma, p->x, p->rows, p->cols, p->x_ld, (uint32_t)box_rows(p->rows), f16);
   if (rc == TTHRML_OK) rc = make_map(&mb, p->w, p->categories, p->cols, p->w_ld, (uint32_t)(f.bn / ctas), f16);
   if (rc) return rc;
   XentArgs a = {};
@@ -927,6 +934,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.N = (int32_t)p->categories;
   a.num_k = (int32_t)(up(p->cols, 64) / 64);
   a.f16 = f16;
+  a.box_m = box_rows(p->rows);
   a.seg = f.seg;
   a.segments = f.segments;
   a.splits = 1;
@@ -994,6 +1002,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
   float* top = (float*)(ws + f.top);
   XentArgs base = {};
   base.f16 = f16;
+  base.box_m = box_rows(p->rows);
   base.unit = f16 ? 16384.0f : 1.0f;
   base.categories = p->categories;
   base.targets = {p->targets, p->wide_targets, p->ignored};
@@ -1014,7 +1023,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     return v % 16 == 0 ? 16 : (v % 8 == 0 ? 8 : (v % 4 == 0 ? 4 : 2));
   };
   CUtensorMap mx, mx_mn;
-  rc = make_map(&mx, p->x, p->rows, p->cols, p->x_ld, 128u, f16);
+  rc = make_map(&mx, p->x, p->rows, p->cols, p->x_ld, (uint32_t)box_rows(p->rows), f16);
   if (rc == TTHRML_OK) rc = make_map(&mx_mn, p->x, p->rows, p->cols, p->x_ld, 64u, f16);
   for (int64_t i = 0; i < f.pieces && rc == TTHRML_OK; ++i) {
     const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
