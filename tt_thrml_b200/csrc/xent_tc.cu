@@ -662,12 +662,10 @@ struct JoinArgs {
   const float* factor[2];
   float unit;
 };
-__global__ void __launch_bounds__(256) k_xent_join(const JoinArgs a) {
-  let_next_kernel_start();
-  wait_for_previous_kernel();
+__device__ __forceinline__ void join_rows(const JoinArgs& a, int64_t block, int64_t blocks) {
   const float factor = factor_of(a.factor) / a.unit;
   const int64_t quads = (a.cols + 3) / 4, all = a.rows * quads;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = block * 256 + threadIdx.x; i < all; i += blocks * 256) {
     const int64_t r = i / quads, c = (i - r * quads) * 4;
     const float* p = a.planes + r * a.ld + c;
     float4 s = __ldcg(reinterpret_cast<const float4*>(p));
@@ -693,22 +691,44 @@ __global__ void __launch_bounds__(256) k_xent_join(const JoinArgs a) {
 }
 
 // db[n] = factor * sum over the groups of 32 rows, in their order; eight threads share a column.
-__global__ void __launch_bounds__(256) k_xent_bias(const float* part, int64_t groups, int64_t ld, int64_t n, float* db,
-                                                   const float* f0, const float* f1, float unit) {
+struct BiasArgs {
+  const float* part;
+  int64_t groups, ld, n;
+  float* db;
+  const float* factor[2];
+  float unit;
+};
+__device__ __forceinline__ void bias_sums(const BiasArgs& a, int64_t block) {
   __shared__ float sums[8][33];
-  let_next_kernel_start();
-  wait_for_previous_kernel();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = block * 32 + lane;
   float s = 0.0f;
-  if (c < n)
-    for (int64_t g = warp; g < groups; g += 8) s += __ldcg(part + g * ld + c);
+  if (c < a.n)
+    for (int64_t g = warp; g < a.groups; g += 8) s += __ldcg(a.part + g * a.ld + c);
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && c < n) {
+  if (warp == 0 && c < a.n) {
     for (int i = 1; i < 8; ++i) s += sums[i][lane];
-    const float* const f[2] = {f0, f1};
-    db[c] = s * (factor_of(f) / unit);
+    a.db[c] = s * (factor_of(a.factor) / a.unit);
+  }
+}
+
+// What the products of a piece leave to add up: planes of dx, planes of dw, the sums for db; a range of blocks each.
+struct FinishArgs {
+  JoinArgs x, w;
+  BiasArgs b;
+  int32_t x_blocks, w_blocks, b_blocks;
+};
+__global__ void __launch_bounds__(256) k_xent_finish(const __grid_constant__ FinishArgs a) {
+  let_next_kernel_start();
+  wait_for_previous_kernel();
+  int64_t block = blockIdx.x;
+  if (block < a.x_blocks) {
+    join_rows(a.x, block, a.x_blocks);
+  } else if ((block -= a.x_blocks) < a.w_blocks) {
+    join_rows(a.w, block, a.w_blocks);
+  } else {
+    bias_sums(a.b, block - a.w_blocks);
   }
 }
 
@@ -884,13 +904,10 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
   }
   return launch_xent<kProduct, A_MN, true, 256, 2>(ma, mb, mo, a, st);
 }
-int join_planes(const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols, int64_t second, int64_t n,
-                const XentArgs& a, void* out, int64_t out_ld, int32_t out_dtype, cudaStream_t st) {
-  JoinArgs j = {planes, plane, ld, rows, cols, second, (int32_t)n, out, out_ld, out_dtype, {a.factor[0], a.factor[1]}, a.unit};
-  const int64_t blocks = (rows * ((cols + 3) / 4) + 255) / 256;
-  void* params[1] = {(void*)&j};
-  return launch_clusters((const void*)k_xent_join, (unsigned)std::min<int64_t>(blocks, 148 * 8), 1, 256, 0, params, st,
-                         "k_xent_join launch", true);
+void join_later(JoinArgs& j, int32_t& blocks, const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols,
+                int64_t second, int64_t n, const XentArgs& a, void* out, int64_t out_ld, int32_t out_dtype) {
+  j = {planes, plane, ld, rows, cols, second, (int32_t)n, out, out_ld, out_dtype, {a.factor[0], a.factor[1]}, a.unit};
+  blocks = (int32_t)std::min<int64_t>((rows * ((cols + 3) / 4) + 255) / 256, 148 * 8);
 }
 
 }  // namespace
@@ -1029,6 +1046,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
     const char* w = (const char*)p->w + first * p->w_ld * 2;
     CUtensorMap mw, mw_mn, mg, mg_mn;
+    FinishArgs finish = {};
     const int bn = tile_width(p->rows, width, pairs), ctas = tile_ctas(p->rows);
     rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)(bn / ctas), f16);
     if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
@@ -1085,24 +1103,23 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
       d.align = alignment(out, dw_ld);
       d.second = (int32_t)(f.second / 64);
       rc = product<true>(mg_mn, mx_mn, d, width, p->cols, f.g_rows, f.dw_shares, pairs, st);
-      if (rc == TTHRML_OK && planes)
-        rc = join_planes((const float*)(ws + f.dw), width * f.plane_ld, f.plane_ld, width, p->cols, 0, f.dw_shares, base, out, dw_ld, grad_dtype,
-                         st);
       if (rc) return rc;
+      if (planes)
+        join_later(finish.w, finish.w_blocks, (const float*)(ws + f.dw), width * f.plane_ld, f.plane_ld, width, p->cols, 0,
+                   f.dw_shares, base, out, dw_ld, grad_dtype);
     }
     if (db) {
-      const float* part = a.bias_part;
-      const int64_t groups = up(p->rows, 32) / 32;
-      float* out = db + first;
-      void* params[8] = {(void*)&part, (void*)&groups, (void*)&f.g_ld, (void*)&width, (void*)&out, (void*)&base.factor[0],
-                         (void*)&base.factor[1], (void*)&base.unit};
-      rc = launch_clusters((const void*)k_xent_bias, (unsigned)((width + 31) / 32), 1, 256, 0, params, st, "k_xent_bias launch",
-                           true);
-      if (rc) return rc;
+      finish.b = {a.bias_part, up(p->rows, 32) / 32, f.g_ld, width, db + first, {base.factor[0], base.factor[1]}, base.unit};
+      finish.b_blocks = (int32_t)((width + 31) / 32);
+    }
+    if (dx && i + 1 == f.pieces && f.dx_planes && (f.dx_shares > 1 || f.second))
+      join_later(finish.x, finish.x_blocks, (const float*)(ws + f.dx), f.g_rows * f.plane_ld, f.plane_ld, p->rows, p->cols, f.second,
+                 f.dx_shares, base, dx, dx_ld, grad_dtype);
+    const int64_t blocks = (int64_t)finish.x_blocks + finish.w_blocks + finish.b_blocks;
+    if (blocks) {
+      void* params[1] = {(void*)&finish};
+      rc = launch_clusters((const void*)k_xent_finish, (unsigned)blocks, 1, 256, 0, params, st, "k_xent_finish launch", true);
     }
   }
-  if (rc == TTHRML_OK && dx && f.dx_planes && (f.dx_shares > 1 || f.second))
-    rc = join_planes((const float*)(ws + f.dx), f.g_rows * f.plane_ld, f.plane_ld, p->rows, p->cols, f.second, f.dx_shares, base, dx,
-                     dx_ld, grad_dtype, st);
   return rc;
 }
