@@ -178,7 +178,7 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
     Operand o[2];
     held_operands(x, w, laid, o);
     const tthrml_xent p = problem(x, w, bias, targets, ctx->saved_data["ignored"].toInt(), o);
-    const Tensor grad = grads[0].to(at::kFloat).contiguous();
+    const Tensor grad = grads[0].scalar_type() == at::kFloat ? grads[0].contiguous() : grads[0].to(at::kFloat).contiguous();
     if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().requires_grad(false));
     if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options().requires_grad(false));
     if (bias.defined() && ctx->needs_input_grad(2)) out[2] = floats(x, bias.sizes());
@@ -215,10 +215,11 @@ struct Dropout : Function<Dropout> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(5);
+    if (!grads[0].defined()) return out;
     const variable_list s = ctx->get_saved_variables();
-    if (grads[0].defined())
-      out[0] = apply(grads[0], &s[0], ctx->saved_data["cut"].toInt(), ctx->saved_data["seed"].toInt(),
-                     ctx->saved_data["step"].toInt());
+    const int64_t cut = ctx->saved_data["cut"].toInt(), seed = ctx->saved_data["seed"].toInt(), step = ctx->saved_data["step"].toInt();
+    // a node of its own only where this pass is differentiated in turn
+    out[0] = c10::GradMode::is_enabled() ? apply(grads[0], &s[0], cut, seed, step) : drop(grads[0], cut, seed, step, s[0], Tensor());
     return out;
   }
 };
