@@ -15,7 +15,8 @@
 // clock, and a 128 x 256 tile of one CTA needs 108 at the full MMA rate, a CTA of a pair 76 (16 KB of either operand, the
 // scales of its rows and of all 256 units per 512 clocks).  The accumulator (256 columns) and the scales leave no room for a
 // second one: the epilogue's eight warps take a finished tile into registers at once, free the accumulator for the next tile's
-// MMAs and then scale and store.
+// MMAs and then scale and store.  8192 x 4096 x 8192 to bfloat16: 106 us (5.2 PFLOP/s, the tensor pipe 72 % active; the loads
+// alone would leave it 71 to 76 %), in tiles of one CTA 205.
 #include "fp4_tc.cuh"
 
 namespace tthrml {

@@ -18,6 +18,10 @@
 // second piece is more rows of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
 // themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
 // sums, z, losses and the sums of db are float32; dx and dw accumulate in float32.
+//
+// What bounds it: the tensor pipe (97 % active in each of the four products; 4096 rows, 4096 columns, 16384 categories: logits
+// 332 us, g 340, dx 379, dw 339, 1.45 to 1.65 PFLOP/s at the clocks of a short run) and, over longer runs, the power cap
+// (8192 x 4096 x 32768, the whole step: 6.5 to 6.7 ms, 1.31 to 1.36 PFLOP/s); the weights' bytes for few rows.
 #include "int8_common.cuh"
 #include "tc_common.cuh"
 
