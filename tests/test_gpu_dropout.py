@@ -152,3 +152,13 @@ def test_refusals(tt):
         tt.dropout(x.int(), 0.5, seed=1)
     with pytest.raises(ValueError, match="CUDA"):
         tt.dropout(x.cpu(), 0.5, seed=1)
+
+
+def test_gradient_against_differences(tt):
+    """Dropout is linear: with p = 1/2 and whole numbers the difference along a direction is the gradient's product exactly."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randint(-9, 10, (300,), generator=g, device="cuda").float().requires_grad_(True)
+    d, w = (torch.randint(-9, 10, (300,), generator=g, device="cuda").float() for _ in range(2))
+    (grad,) = torch.autograd.grad(tt.dropout(x, 0.5, seed=8), x, w)
+    up, down = (tt.dropout(x.detach() + s * d, 0.5, seed=8) for s in (1, -1))
+    assert ((up - down) * w).sum() / 2 == (grad * d).sum()

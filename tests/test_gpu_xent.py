@@ -407,3 +407,48 @@ def test_weights_of_more_than_2_to_the_31_elements(tt):
         exact = p @ x.double()
         assert ((dw[at].double() - exact).abs() <= 2.0**-7 * exact.abs() + 1e-4 * exact.abs().max()).all()
     tt.check_operator_errors()
+
+
+def test_weights_of_rows_that_are_nan(tt):
+    """NaN among the weights of 'none': the row's own gradient and the weights' are NaN, the other rows' are not; also where
+    it stands alone."""
+    x, w, y, _ = batch(10, 16, 40, torch.bfloat16, 19, bias=False, ignored=0)
+    for others in (1.0, 0.0):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        weight = torch.full((10,), others, device="cuda")
+        weight[3] = math.nan
+        tt.softmax_cross_entropy(a, b, y, reduction="none").backward(weight)
+        rest = torch.arange(10, device="cuda") != 3
+        assert torch.isnan(a.grad[3]).all() and torch.isfinite(a.grad[rest]).all() and torch.isnan(b.grad).all()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_gradients_against_differences(tt, which):
+    """Central differences of the loss along a direction.  x and w are multiples of 2^-6 below 2, so that x +- d and w +- d are
+    exact in bfloat16.  The difference's own error: a third of a derivative, at most R^3 / 6 with R the range of the logits'
+    change; the losses' (1e-6 each); the gradient's: 2^-8 of each element, twice (g and the result)."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+
+    def grid(*shape):
+        return (torch.randint(-64, 65, shape, generator=g, device="cuda") / 64.0)
+
+    x, w, bias = grid(150, 48), grid(200, 48) / 4, torch.randn(200, generator=g, device="cuda")
+    w = torch.round(w * 64) / 64
+    y = torch.randint(0, 200, (150,), generator=g, device="cuda")
+    values = [x, w, bias]
+    d = torch.where(torch.rand(values[which].shape, generator=g, device="cuda") < 0.5, -1.0, 1.0) / 64
+
+    def loss(sign):
+        v = [t + sign * d if i == which else t for i, t in enumerate(values)]
+        assert torch.equal(v[0].bfloat16().float(), v[0]) and torch.equal(v[1].bfloat16().float(), v[1])
+        return tt.softmax_cross_entropy(v[0].bfloat16(), v[1].bfloat16(), y, bias=v[2]).double()
+
+    leaves = [x.bfloat16(), w.bfloat16(), bias.clone()]
+    leaf = leaves[which].requires_grad_(True)
+    (grad,) = torch.autograd.grad(tt.softmax_cross_entropy(leaves[0], leaves[1], y, bias=leaves[2]), leaf)
+    slope = (grad.double() * d.double()).sum()
+    change = d.double() @ w.double().t() if which == 0 else (x.double() @ d.double().t() if which == 1 else d.double()[None])
+    reach = float((change.amax(1) - change.amin(1)).max())
+    size = float((grad.double().abs() * d.double().abs()).sum())
+    assert abs(float(loss(1) - loss(-1)) / 2 - float(slope)) <= reach**3 / 6 + 1e-6 * 6 + 2 * 2.0**-8 * size
+    assert abs(float(slope)) > 1e-4

@@ -12,6 +12,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -85,7 +86,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     newest_header = max((h.stat().st_mtime for h in _headers()), default=0.0)
-    objects = []
+    objects, commands = [], []
     for src in sources:
         obj = BUILD_DIR / (src.stem + ".o")
         objects.append(obj)
@@ -94,7 +95,9 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        commands.append(cmd)
+    with ThreadPoolExecutor(max(1, min(8, os.cpu_count() or 1))) as pool:  # the compiler uses one core per source
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), commands))
     newest_obj = max(o.stat().st_mtime for o in objects)
     build_hostcall(verbose=verbose, force=force)
     if force or not LIB_PATH.exists() or LIB_PATH.stat().st_mtime < newest_obj:

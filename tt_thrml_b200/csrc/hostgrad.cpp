@@ -33,7 +33,8 @@ using torch::autograd::variable_list;
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == TTHRML_OK, what, " failed (", rc, "): ", library.last_error()); }
 
-// Makes a tensor's device current for torch and for the library on this thread, and the old one again at the end.
+// Makes a tensor's device current for torch and for the library on this thread (a backward pass has a thread of its own), and
+// the old one again at the end.
 class On {
  public:
   explicit On(const Tensor& t) : guard_(t.device()), before_(guard_.original_device().index()), now_(t.device().index()) {

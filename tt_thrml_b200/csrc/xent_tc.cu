@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           weight = a.unit;
           if (a.row_grad) {
             const float most = __ldg(a.top_grad);
-            weight = most > 0.0f ? weight * (__ldg(a.row_grad + m) / most) : 0.0f;
+            const float own = __ldg(a.row_grad + m);
+            weight *= most > 0.0f ? own / most : own * 0.0f;  // nothing but zeros and NaN: a NaN stays
           }
           if (t < 0 || t >= a.categories) weight = __uint_as_float(0x7FC00000u);
           if (log2_z == -INFINITY || t == a.targets.ignored) weight = 0.0f;
@@ -839,15 +840,15 @@ int plan_backward(int64_t rows, int64_t categories, int64_t cols, bool want_x, b
   int64_t pairs;
   const int rc = resident_pairs(&pairs);
   if (rc) return rc;
-  const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / rows / 256 * 256);
+  p->second = rows <= kFewRows ? up(rows, 64) : 0;
+  p->g_rows = p->second ? 2 * p->second : rows;
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / p->g_rows / 256 * 256);
   p->pieces = (categories + most - 1) / most;
   p->piece = up((categories + p->pieces - 1) / p->pieces, 256);
   p->pieces = (categories + p->piece - 1) / p->piece;
   const int64_t width = std::min(p->piece, categories);
   p->g_ld = up(width, 64);
   p->plane_ld = up(cols, 32);
-  p->second = rows <= kFewRows ? up(rows, 64) : 0;
-  p->g_rows = p->second ? 2 * p->second : rows;
   p->dx_shares = want_x ? shares(p->g_rows, cols, width, pairs) : 0;
   p->dw_shares = want_w ? shares(width, cols, p->g_rows, pairs) : 0;
   p->dx_planes = want_x && (p->dx_shares > 1 || p->pieces > 1 || p->second);

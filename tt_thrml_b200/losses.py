@@ -15,7 +15,7 @@ check_operator_errors reports.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import _error_addresses, dtype_code, error_word, require_cuda
+from .quantized import _error_addresses, dtype_code, error_word, on_device, require_cuda
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -61,7 +61,8 @@ def mean_and_gradients(x, weights, targets, bias, ignore_index, one, dw, db):
     if x.dim() != 2 or not x.shape[0]:
         raise ValueError(f"x must hold rows of units, got shape {tuple(x.shape)}")
     word = _error_addresses.get(x.device.index) or error_word(x.device).data_ptr()
-    return nat.bound_hostcall().softmax_cross_entropy_gradients(x, weights, bias, targets, int(ignore_index), word, one, dw, db)
+    with on_device(x.device):
+        return nat.bound_hostcall().softmax_cross_entropy_gradients(x, weights, bias, targets, int(ignore_index), word, one, dw, db)
 
 
 def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", ignore_index=-100):
@@ -94,8 +95,10 @@ def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", i
         return zero if reduction == "none" else zero.sum()
     word = _error_addresses.get(dev.index) or error_word(dev).data_ptr()
     flat = x if x.dim() == 2 else x.reshape(rows, K)
-    loss = nat.bound_hostcall().softmax_cross_entropy(flat, weights, bias, targets if targets.dim() == 1 else targets.reshape(rows),
-                                                      _REDUCTIONS[reduction], int(ignore_index), word)
+    targets = targets if targets.dim() == 1 else targets.reshape(rows)
+    with on_device(dev):
+        loss = nat.bound_hostcall().softmax_cross_entropy(flat, weights, bias, targets, _REDUCTIONS[reduction], int(ignore_index),
+                                                          word)
     return loss.reshape(lead) if reduction == "none" and len(lead) != 1 else loss
 
 

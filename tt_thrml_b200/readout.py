@@ -38,8 +38,8 @@ class CategoricalReadout:
     the next step.  x: [rows, n_units], or an Executor of a dense program whose hidden block
     (block 1) has n_units, a row per chain.  targets: int64 or int32 [rows],
     `ignore_index` for rows that do not count.  Nothing waits for the device; a step
-    may be captured into a CUDA graph after a first one outside, and takes other
-    units each time the graph is replayed.
+    on a tensor may be captured into a CUDA graph after a first one outside, and
+    leaves out other units each time the graph is replayed.
     loss(x, targets): the mean loss without dropout.
     quantize() rounds the weights to 4 bits (`served`); fields(x) are then x W^T + b
     with them, in x's type.

@@ -11,7 +11,7 @@ goes with it, so means are kept exactly.
 from __future__ import annotations
 
 from . import _native as nat
-from .quantized import dtype_code, require_cuda
+from .quantized import dtype_code, on_device, require_cuda
 
 
 def _torch():
@@ -51,7 +51,8 @@ def dropout(x, p=0.5, *, seed, step=0):
         step = int(step)
         if not 0 <= step < 2**32:
             raise ValueError(f"step must be between 0 and 2^32 - 1, got {step}")
-    return nat.bound_hostcall().dropout(x, round(65536 * p), seed, step, step_at)
+    with on_device(x.device):
+        return nat.bound_hostcall().dropout(x, round(65536 * p), seed, step, step_at)
 
 
 __all__ = ["dropout"]
