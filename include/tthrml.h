@@ -754,14 +754,14 @@ typedef struct tthrml_xent {
  * gradients).  reduction 0: rows only; 1: *loss is the mean over the rows that
  * count (0 if there are none) and *inv_count 1 / their number, 2: their sum and
  * 1; *inv_count is the second factor of the backward pass.  The same every time.
- * workspace: tthrml_xent_forward_workspace(rows, categories) bytes (of the
+ * workspace: tthrml_xent_forward_workspace(rows, categories, cols) bytes (of the
  * current device; negative: an error), 16-byte aligned, free again once the
  * work on `stream` is done.
  */
 int tthrml_xent_forward(const tthrml_xent* problem_host, float* log2_z_dev, float* row_loss_dev,
                         float* loss_dev, float* inv_count_dev, int32_t reduction, void* workspace_dev,
                         int64_t workspace_bytes, int32_t* error_dev, void* stream);
-int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories);
+int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories, int64_t cols);
 
 /*
  * dx [rows][dx_ld], dw [categories][dw_ld] (grad_dtype: float32, bfloat16 or

@@ -267,7 +267,7 @@ _SIGNATURES = {
     ),
     "tthrml_pair_moments": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
     "tthrml_xent_forward": (c_i32, [ctypes.POINTER(Xent), c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]),
-    "tthrml_xent_forward_workspace": (c_i64, [c_i64, c_i64]),
+    "tthrml_xent_forward_workspace": (c_i64, [c_i64, c_i64, c_i64]),
     "tthrml_xent_backward": (
         c_i32,
         [ctypes.POINTER(Xent), c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp],

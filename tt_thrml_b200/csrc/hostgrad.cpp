@@ -124,7 +124,7 @@ Tensor xent_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const 
   Operand o[2];
   saved.laid = lay_out(x, w, o, on.stream());
   const tthrml_xent p = problem(x, w, bias, targets, ignored, o);
-  const int64_t size = library.xent_forward_workspace(p.rows, p.categories);
+  const int64_t size = library.xent_forward_workspace(p.rows, p.categories, p.cols);
   if (size < 0) check((int)size, "tthrml_xent_forward_workspace");
   const Tensor space = bytes(x, size);
   saved.log2_z = floats(x, {p.rows});

@@ -10,9 +10,9 @@
 //
 // One kernel serves the four products: persistent clusters of two CTAs walk 256 x BN tiles (tcgen05 cta_group::2, two
 // TMEM accumulators, six stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
-// transposed.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for half the weights, which
-// are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the even CTA multiplies, warps 2-9 run the epilogue of a tile under the main
-// loop of the next one.
+// transposed.  Warps 2 on run the epilogue of a tile beside the main loop of the next one: eight, or sixteen on the wider tiles of
+// logits.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for half the weights, which
+// are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the even CTA multiplies.
 //
 // g is rounded to the operands' 16 bits (up to kFewRows rows: held in two such pieces, their sum good to 2^-16; the
 // second piece is more rows of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
@@ -29,10 +29,9 @@ namespace tthrml {
 namespace {
 
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr int kThreads = 320, kEpilogueWarps = 8;
 constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
 constexpr int64_t kFewRows = 128;             // whose g is held in two pieces of 16 bits
-constexpr int kChunk = 8;  // 64-wide blocks of K that a logit's sum stays in tensor memory for
+constexpr int kChunk = 8;  // 64-wide blocks of K that a logit's sum stays in tensor memory for; at least kShort
 enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
 
 struct RowTargets {
@@ -95,12 +94,23 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-template <int BN, int CTAS>
+// Parts of a tile's columns that the epilogue's warps share: four warps, a row per lane, take one.
+// Sixteen warps where the sums are short (kShort blocks) and the epilogue is what a tile waits for; beside long sums eight do, and
+// leave room for more stages (8192 x 32768, 128 and 4096 columns, losses: 128 us and 1.38 ms with sixteen, 162 and 1.35 with eight).
+constexpr int kShort = 8;
+static_assert(kShort <= kChunk, "short sums are one accumulation");
+constexpr int parts_of(bool brief, int bn) { return brief && bn >= 128 ? 4 : 2; }
+template <int EPI, int BN, int CTAS, bool BRIEF>
 struct XentShape {
+  static constexpr int kParts = parts_of(BRIEF, BN), kWarps = 4 * kParts, kThreads = 64 + 32 * kWarps;
   static constexpr int kA = 128 * 64 * 2, kB = BN / CTAS * 64 * 2, kStage = kA + kB;
-  static constexpr int kStages = kStage >= 49152 ? 4 : (kStage >= 32768 ? 6 : 8);
+  static constexpr int kOut = EPI == kPartials ? 0 : kWarps * kOutBytes;  // rows on their way out
   static constexpr int kBarriers = 256;
-  static constexpr int kSmem = 1024 + kStages * kStage + kEpilogueWarps * kOutBytes + kBarriers + 256 * 4 /*biases*/;
+  // the biases of two tiles where that costs no stage, so that a warp may run one tile ahead; else of one
+  static constexpr int kBiases = EPI == kPartials ? 2 : 1;
+  static constexpr int kRest = 1024 + kOut + kBarriers + kBiases * 256 * 4;
+  static constexpr int kFit = (232448 - kRest) / kStage, kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kSmem = kRest + kStages * kStage;
 };
 
 // v less its values rounded to 16 bits (w, packed).
@@ -163,23 +173,23 @@ __device__ __forceinline__ float column_sums(const float (&v)[32], uint32_t buff
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS, bool BRIEF>
+__global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
     k_xent(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
            const __grid_constant__ CUtensorMap map_out, const __grid_constant__ XentArgs a) {
-  using S = XentShape<BN, CTAS>;
+  using S = XentShape<EPI, BN, CTAS, BRIEF>;
   constexpr int kRows = 128 * CTAS;  // of a tile
   static_assert(!B_MN || (BN == 256 && CTAS == 2), "MN-major halves of B are whole boxes of 64");
-  constexpr bool kChunked = EPI == kPartials || EPI == kGradientSums;
+  constexpr bool kChunked = !BRIEF && (EPI == kPartials || EPI == kGradientSums);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* turns = tiles + S::kStages * S::kStage;  // a buffer per epilogue warp
-  uint64_t* full = reinterpret_cast<uint64_t*>(turns + kEpilogueWarps * kOutBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(turns + S::kOut);
   uint64_t* empty = full + S::kStages;
   uint64_t* acc_full = empty + S::kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;       // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  float* bias = reinterpret_cast<float*>(turns + kEpilogueWarps * kOutBytes + S::kBarriers);  // [256]
+  float* biases = reinterpret_cast<float*>(turns + S::kOut + S::kBarriers);  // [kBiases][256]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -194,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], CTAS * kEpilogueWarps);  // every epilogue warp of both CTAs
+      mbar_init(&acc_empty[b], CTAS * S::kWarps);  // every epilogue warp of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -322,10 +332,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int quad = warp & 3, part = (warp - 2) >> 2;
     unsigned char* turn = turns + (warp - 2) * kOutBytes;
     const uint32_t buffer = smem_u32(turn);
-    int it = 0;
+    int it = 0, tile = 0, next_nb = -1;
+    float next_bias = 0.0f, *bias = biases;
     bool failed = false;
     for (int u = first; u < a.units; u += step) {
       int split, mb, sg;
@@ -474,12 +485,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb) {
         if (EPI != kProduct && a.bias) {
-          asm volatile("bar.sync 1, 256;" ::: "memory");  // every warp has read the biases of the tile before
+          if (S::kBiases == 2)
+            bias = biases + (tile++ & 1) * 256;
+          else
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");  // every warp has read the biases of the tile before
           const int j = (int)threadIdx.x - 64, n = nb * BN + j;
-          if (j < BN) bias[j] = n < a.N ? __ldg(a.bias + n) : 0.0f;
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (j < BN) bias[j] = nb == next_nb ? next_bias : (n < a.N ? __ldg(a.bias + n) : 0.0f);
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");
+          // the next tile's are on their way meanwhile: of this unit, or of the next one
+          next_nb = nb + 1;
+          if (next_nb >= min((sg + 1) * a.seg, n_blocks) && u + step < a.units) {
+            int next_split, next_mb, next_sg;
+            unit_at<kRows>(a, u + step, next_split, next_mb, next_sg);
+            next_nb = next_sg * a.seg;
+          }
+          if (j < BN) next_bias = next_nb * BN + j < a.N ? __ldg(a.bias + next_nb * BN + j) : 0.0f;
         }
-        constexpr int kMine = BN / 2;  // columns of this thread
+        constexpr int kMine = BN / S::kParts;  // columns of this thread
         if constexpr (kChunked) {
           float acc[kMine];
 #pragma unroll
@@ -495,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int q = 0; q < kMine / 16; ++q) {
               float v[16];
-              tmem_load16(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * kMine + q * 16), v);
+              tmem_load16(tmem + (uint32_t)(b * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * kMine + q * 16), v);
 #pragma unroll
               for (int j = 0; j < 16; j += 2) add2(acc[q * 16 + j], acc[q * 16 + j + 1], v[j], v[j + 1]);
             }
@@ -509,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = acc[q * 32 + j];
-            finish(v, nb * BN + half * kMine + q * 32);
+            finish(v, nb * BN + part * kMine + q * 32);
           }
         } else {
           if (!failed && !mbar_wait_warp(&acc_full[it & 1], (uint32_t)(it >> 1) & 1u)) {
@@ -519,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (failed) continue;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = half * kMine; c < (half + 1) * kMine; c += 32) {
+          for (int c = part * kMine; c < (part + 1) * kMine; c += 32) {
             float v[32];
             tmem_load32(tmem + (uint32_t)((it & 1) * 256) + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
             finish(v, nb * BN + c);
@@ -531,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++it;
         }
       }
-      if (EPI == kPartials && m < a.M) a.part[(int64_t)m * a.slots + 2 * sg + half] = make_float2(top, sum);
+      if (EPI == kPartials && m < a.M) a.part[(int64_t)m * a.slots + S::kParts * sg + part] = make_float2(top, sum);
     }
     if (EPI != kPartials) sent_rows_done();
   }
@@ -758,10 +780,10 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int
 
 constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS>
+template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS, bool BRIEF>
 int launch_xent(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const XentArgs& a, cudaStream_t st) {
-  const void* fn = (const void*)k_xent<EPI, A_MN, B_MN, BN, CTAS>;
-  constexpr int kSmem = XentShape<BN, CTAS>::kSmem;
+  const void* fn = (const void*)k_xent<EPI, A_MN, B_MN, BN, CTAS, BRIEF>;
+  constexpr int kThreads = XentShape<EPI, BN, CTAS, BRIEF>::kThreads, kSmem = XentShape<EPI, BN, CTAS, BRIEF>::kSmem;
   ClusterFit fit;
   const int rc = cluster_fit(fn, CTAS, kThreads, kSmem, &fit);
   if (rc) return rc;
@@ -769,21 +791,26 @@ int launch_xent(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap&
   void* params[4] = {(void*)&ma, (void*)&mb, (void*)&mo, (void*)&a};
   return launch_clusters(fn, (unsigned)(CTAS * clusters), CTAS, kThreads, kSmem, params, st, "k_xent launch", true);
 }
-template <int EPI, int CTAS>
+template <int EPI, int CTAS, bool BRIEF>
 int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
-  if (bn == 64) return launch_xent<EPI, false, false, 64, CTAS>(ma, mb, ma, a, st);
-  if (bn == 128) return launch_xent<EPI, false, false, 128, CTAS>(ma, mb, ma, a, st);
-  return launch_xent<EPI, false, false, 256, CTAS>(ma, mb, ma, a, st);
+  if (bn == 64) return launch_xent<EPI, false, false, 64, CTAS, BRIEF>(ma, mb, ma, a, st);
+  if (bn == 128) return launch_xent<EPI, false, false, 128, CTAS, BRIEF>(ma, mb, ma, a, st);
+  return launch_xent<EPI, false, false, 256, CTAS, BRIEF>(ma, mb, ma, a, st);
 }
 template <int EPI>
-int launch_logits(int ctas, int bn, const CUtensorMap& ma, const CUtensorMap& mb, const XentArgs& a, cudaStream_t st) {
-  return ctas == 1 ? launch_logits<EPI, 1>(bn, ma, mb, a, st) : launch_logits<EPI, 2>(bn, ma, mb, a, st);
+int launch_logits(int ctas, int bn, const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, cudaStream_t st) {
+  if (a.num_k <= kShort) {
+    a.chunk = a.num_k;
+    return ctas == 1 ? launch_logits<EPI, 1, true>(bn, ma, mb, a, st) : launch_logits<EPI, 2, true>(bn, ma, mb, a, st);
+  }
+  return ctas == 1 ? launch_logits<EPI, 1, false>(bn, ma, mb, a, st) : launch_logits<EPI, 2, false>(bn, ma, mb, a, st);
 }
 
 // How many pairs of CTAs work at once (every form of the kernel fills an SM).
 int resident_pairs(int64_t* out) {
   ClusterFit fit;
-  const int rc = cluster_fit((const void*)k_xent<kProduct, false, true, 256, 2>, 2, kThreads, XentShape<256, 2>::kSmem, &fit);
+  const int rc = cluster_fit((const void*)k_xent<kProduct, false, true, 256, 2, false>, 2,
+                             XentShape<kProduct, 256, 2, false>::kThreads, XentShape<kProduct, 256, 2, false>::kSmem, &fit);
   *out = fit.clusters;
   return rc;
 }
@@ -812,10 +839,10 @@ int64_t shares(int64_t m, int64_t n, int64_t k, int64_t pairs) {
 }
 
 struct ForwardPlan {
-  int bn, seg, segments;
+  int bn, seg, segments, slots;
   int64_t logits, counter, bytes;  // places in the workspace behind the partial sums
 };
-int plan_forward(int64_t rows, int64_t categories, ForwardPlan* p) {
+int plan_forward(int64_t rows, int64_t categories, int64_t cols, ForwardPlan* p) {
   int64_t pairs;
   const int rc = resident_pairs(&pairs);
   if (rc) return rc;
@@ -824,7 +851,8 @@ int plan_forward(int64_t rows, int64_t categories, ForwardPlan* p) {
   const int64_t ctas = tile_ctas(rows);
   p->seg = tiles_per_unit(up(rows, 128 * ctas) / (128 * ctas), n_blocks, pairs * 2 / ctas);
   p->segments = (int)((n_blocks + p->seg - 1) / p->seg);
-  p->logits = up(rows * 2 * p->segments * 8, 16);
+  p->slots = parts_of(up(cols, 64) / 64 <= kShort, p->bn) * p->segments;
+  p->logits = up(rows * p->slots * 8, 16);
   p->counter = p->logits + up(rows * 4, 16);
   p->bytes = p->counter + 16;
   return TTHRML_OK;
@@ -907,7 +935,7 @@ int product(const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, int64_t m,
     set_error("planes of %lld x %lld sums take no tensor map", (long long)m, (long long)n);
     return TTHRML_ERR_CUDA;
   }
-  return launch_xent<kProduct, A_MN, true, 256, 2>(ma, mb, mo, a, st);
+  return launch_xent<kProduct, A_MN, true, 256, 2, false>(ma, mb, mo, a, st);
 }
 void join_later(JoinArgs& j, int32_t& blocks, const float* planes, int64_t plane, int64_t ld, int64_t rows, int64_t cols,
                 int64_t second, int64_t n, const XentArgs& a, void* out, int64_t out_ld, int32_t out_dtype) {
@@ -918,11 +946,13 @@ void join_later(JoinArgs& j, int32_t& blocks, const float* planes, int64_t plane
 }  // namespace
 }  // namespace tthrml
 
-extern "C" int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories) {
+extern "C" int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories, int64_t cols) {
   using namespace tthrml;
-  if (rows < 1 || categories < 1 || rows > TTHRML_XENT_MAX_ROWS || categories > TTHRML_XENT_MAX_CATEGORIES) return 0;
+  if (rows < 1 || categories < 1 || cols < 1 || rows > TTHRML_XENT_MAX_ROWS || categories > TTHRML_XENT_MAX_CATEGORIES ||
+      cols > TTHRML_XENT_MAX_COLS)
+    return 0;
   ForwardPlan p;
-  const int rc = plan_forward(rows, categories, &p);
+  const int rc = plan_forward(rows, categories, cols, &p);
   return rc ? rc : p.bytes;
 }
 
@@ -936,7 +966,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
     return TTHRML_ERR_ARG;
   }
   ForwardPlan f;
-  rc = plan_forward(p->rows, p->categories, &f);
+  rc = plan_forward(p->rows, p->categories, p->cols, &f);
   if (rc) return rc;
   if ((uintptr_t)workspace % 16 || workspace_bytes < f.bytes) {
     set_error("tthrml_xent_forward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)f.bytes,
@@ -967,7 +997,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.categories = p->categories;
   a.targets = {p->targets, p->wide_targets, p->ignored};
   a.part = (float2*)ws;
-  a.slots = 2 * f.segments;
+  a.slots = f.slots;
   a.target_logit = (float*)(ws + f.logits);
   a.counter = (uint32_t*)(ws + f.counter);
   a.error = error;
