@@ -96,7 +96,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 // Parts of a tile's columns that the epilogue's warps share: four warps, a row per lane, take one.
 // Sixteen warps where the sums are short (kShort blocks) and the epilogue is what a tile waits for; beside long sums eight do, and
-// leave room for more stages (8192 x 32768, 128 and 4096 columns, losses: 128 us and 1.38 ms with sixteen, 162 and 1.35 with eight).
+// leave room for more stages (losses of 8192 x 32768: 128 columns 105 us with sixteen, 162 with eight; 4096 columns 1.38 ms, 1.35).
 constexpr int kShort = 8;
 static_assert(kShort <= kChunk, "short sums are one accumulation");
 constexpr int parts_of(bool brief, int bn) { return brief && bn >= 128 ? 4 : 2; }
@@ -106,9 +106,8 @@ struct XentShape {
   static constexpr int kA = 128 * 64 * 2, kB = BN / CTAS * 64 * 2, kStage = kA + kB;
   static constexpr int kOut = EPI == kPartials ? 0 : kWarps * kOutBytes;  // rows on their way out
   static constexpr int kBarriers = 256;
-  // the biases of two tiles where that costs no stage, so that a warp may run one tile ahead; else of one
-  static constexpr int kBiases = EPI == kPartials ? 2 : 1;
-  static constexpr int kRest = 1024 + kOut + kBarriers + kBiases * 256 * 4;
+  static constexpr int kMine = BN / kParts;  // columns of a warp
+  static constexpr int kRest = 1024 + kOut + kBarriers + (EPI == kProduct ? 0 : kWarps * kMine * 4 /*their biases*/);
   static constexpr int kFit = (232448 - kRest) / kStage, kStages = kFit < 8 ? kFit : 8;
   static constexpr int kSmem = kRest + kStages * kStage;
 };
@@ -189,7 +188,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
   uint64_t* acc_full = empty + S::kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;       // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  float* biases = reinterpret_cast<float*>(turns + S::kOut + S::kBarriers);  // [kBiases][256]
+  float* biases = reinterpret_cast<float*>(turns + S::kOut + S::kBarriers);  // [kWarps][kMine]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -335,8 +334,10 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
     const int quad = warp & 3, part = (warp - 2) >> 2;
     unsigned char* turn = turns + (warp - 2) * kOutBytes;
     const uint32_t buffer = smem_u32(turn);
-    int it = 0, tile = 0, next_nb = -1;
-    float next_bias = 0.0f, *bias = biases;
+    constexpr int kMine = S::kMine;  // columns of this warp
+    float* bias = biases + (warp - 2) * kMine;
+    int it = 0, next_nb = -1;
+    float next_bias[(kMine + 31) / 32] = {};
     bool failed = false;
     for (int u = first; u < a.units; u += step) {
       int split, mb, sg;
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
           if (a.bias) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float4 w = *reinterpret_cast<const float4*>(bias + (n % BN) + 4 * i);
+              const float4 w = *reinterpret_cast<const float4*>(bias + n % kMine + 4 * i);
               add2(v[4 * i], v[4 * i + 1], w.x, w.y);
               add2(v[4 * i + 2], v[4 * i + 3], w.z, w.w);
             }
@@ -484,24 +485,27 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
         }
       };
       for (int nb = sg * a.seg; nb < min((sg + 1) * a.seg, n_blocks); ++nb) {
-        if (EPI != kProduct && a.bias) {
-          if (S::kBiases == 2)
-            bias = biases + (tile++ & 1) * 256;
-          else
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");  // every warp has read the biases of the tile before
-          const int j = (int)threadIdx.x - 64, n = nb * BN + j;
-          if (j < BN) bias[j] = nb == next_nb ? next_bias : (n < a.N ? __ldg(a.bias + n) : 0.0f);
-          asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");
-          // the next tile's are on their way meanwhile: of this unit, or of the next one
-          next_nb = nb + 1;
+        if (EPI != kProduct && a.bias) {  // each warp keeps its own columns' biases: no barrier of all of them
+          const auto fetch = [&](int block) {
+#pragma unroll
+            for (int i = 0; i < kMine / 32; ++i) {
+              const int n = block * BN + part * kMine + 32 * i + lane;
+              next_bias[i] = n < a.N ? __ldg(a.bias + n) : 0.0f;
+            }
+          };
+          if (next_nb != nb) fetch(nb);
+          __syncwarp();  // the lanes have read those of the tile before
+#pragma unroll
+          for (int i = 0; i < kMine / 32; ++i) bias[32 * i + lane] = next_bias[i];
+          __syncwarp();
+          next_nb = nb + 1;  // the next tile's are on their way meanwhile: of this unit, or of the next one
           if (next_nb >= min((sg + 1) * a.seg, n_blocks) && u + step < a.units) {
             int next_split, next_mb, next_sg;
             unit_at<kRows>(a, u + step, next_split, next_mb, next_sg);
             next_nb = next_sg * a.seg;
           }
-          if (j < BN) next_bias = next_nb * BN + j < a.N ? __ldg(a.bias + next_nb * BN + j) : 0.0f;
+          fetch(next_nb);
         }
-        constexpr int kMine = BN / S::kParts;  // columns of this thread
         if constexpr (kChunked) {
           float acc[kMine];
 #pragma unroll
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(&acc_empty[b]);
           }
-          if (failed) continue;  // on to the next tile's barrier, which the other warps wait at
+          if (failed) break;
 #pragma unroll
           for (int q = 0; q < kMine / 32; ++q) {
             float v[32];
@@ -538,7 +542,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
             if (lane == 0) atomicExch(a.error, kErrAccWait);
             failed = true;
           }
-          if (failed) continue;
+          if (failed) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = part * kMine; c < (part + 1) * kMine; c += 32) {
