@@ -748,7 +748,8 @@ typedef struct tthrml_xent {
 } tthrml_xent;
 
 /*
- * log2_z: [rows], z / ln 2, which the backward pass takes.  row_loss: [rows].
+ * sums: [rows][2], 8-byte aligned, (m, s) with s 2^m the sum of exp(logits),
+ * which the backward pass takes.  row_loss: [rows].
  * A row in which no category is possible has loss inf and no gradient; a
  * target outside 0 .. categories-1 that is not `ignored` has loss NaN (and NaN
  * gradients).  reduction 0: rows only; 1: *loss is the mean over the rows that
@@ -758,7 +759,7 @@ typedef struct tthrml_xent {
  * current device; negative: an error), 16-byte aligned, free again once the
  * work on `stream` is done.
  */
-int tthrml_xent_forward(const tthrml_xent* problem_host, float* log2_z_dev, float* row_loss_dev,
+int tthrml_xent_forward(const tthrml_xent* problem_host, float* sums_dev, float* row_loss_dev,
                         float* loss_dev, float* inv_count_dev, int32_t reduction, void* workspace_dev,
                         int64_t workspace_bytes, int32_t* error_dev, void* stream);
 int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories, int64_t cols);
@@ -769,7 +770,7 @@ int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories, int64_t 
  * sum_t weight[t] loss[t].  weight: grad[0] * (inv_count ? *inv_count : 1), or,
  * grad_per_row, grad[t].
  */
-int tthrml_xent_backward(const tthrml_xent* problem_host, const float* log2_z_dev,
+int tthrml_xent_backward(const tthrml_xent* problem_host, const float* sums_dev,
                          const float* grad_dev, int32_t grad_per_row, const float* inv_count_dev,
                          void* dx_dev, int64_t dx_ld, void* dw_dev, int64_t dw_ld,
                          int32_t grad_dtype, float* db_dev, void* workspace_dev,

@@ -65,7 +65,7 @@ def expected(x, w, y, bias, weight, ignore=-100):
     dg0 = r.abs() * (p * (dl + (dz + 12 * u * spread)[:, None]) + 4 * u * (p + hit))  # before its rounding
     # float16 holds g as 2^14 g / (the largest weight): its smallest step is 2^-24 of that
     tiny = 2.0**-25 * 2.0**-14 * float(r.abs().max()) if x.dtype == torch.float16 else 0.0
-    few = x.shape[0] <= 128  # g in two pieces: the rounding of the second one, 16 bits further down
+    few = T <= 128 or V <= 64  # g in two pieces: the rounding of the second one, 16 bits further down
     dg = dg0 + (half * half if few else half) * g.abs() + torch.where(r != 0, tiny, 0.0)
 
     def product(a, da, b, n):
@@ -122,6 +122,31 @@ SIZES = [(1, 8, 2), (1, 1, 1), (3, 5, 7), (1, 512, 1000), (31, 64, 33), (33, 72,
 def test_losses_and_gradients(tt, rows, k, v, dtype):
     x, w, y, bias = batch(rows, k, v, DTYPES[dtype], rows + k + v)
     check(tt, x, w, y, bias, "mean")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,k,v", [(129, 8, 3), (515, 9, 2), (2000, 64, 64), (2000, 72, 65), (987, 20, 4), (21000, 40, 1),
+                                      (40000, 33, 31), (3000, 2001, 33)])
+def test_few_categories(tt, rows, k, v, dtype):
+    """The differences of few categories cancel in the gradients of x: up to 64 are held in two pieces."""
+    x, w, y, bias = batch(rows, k, v, DTYPES[dtype], rows + v)
+    check(tt, x, w, y, bias, "mean" if rows % 2 else "none")
+
+
+@pytest.mark.parametrize("which", ["x", "w", "bias"])
+def test_one_gradient_of_few_categories(tt, which):
+    """Each gradient by itself is that of all three; rows without a target keep theirs at zero."""
+    x, w, y, bias = batch(700, 50, 11, torch.bfloat16, 12)
+    leaves = {"x": x, "w": w, "bias": bias}
+
+    def grads(names):
+        t = {n: v.clone().requires_grad_(n in names) for n, v in leaves.items()}
+        loss = tt.softmax_cross_entropy(t["x"], t["w"], y, bias=t["bias"])
+        return dict(zip(names, torch.autograd.grad(loss, [t[n] for n in names])))
+
+    all_three = grads(["x", "w", "bias"])
+    assert torch.equal(grads([which])[which], all_three[which])
+    assert torch.equal(all_three["x"][y == -100], torch.zeros_like(x[y == -100])) and bool((y == -100).any())
 
 
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])

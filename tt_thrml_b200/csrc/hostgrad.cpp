@@ -101,7 +101,7 @@ void held_operands(const Tensor& x, const Tensor& w, const Tensor& laid, Operand
 }
 
 struct XentSaved {
-  Tensor laid, log2_z, inv_count;
+  Tensor laid, sums, inv_count;
 };
 
 tthrml_xent problem(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& targets, int64_t ignored, const Operand (&o)[2]) {
@@ -127,13 +127,13 @@ Tensor xent_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const 
   const int64_t size = library.xent_forward_workspace(p.rows, p.categories, p.cols);
   if (size < 0) check((int)size, "tthrml_xent_forward_workspace");
   const Tensor space = bytes(x, size);
-  saved.log2_z = floats(x, {p.rows});
+  saved.sums = floats(x, {p.rows, 2});
   Tensor rows = floats(x, {p.rows}), total;
   if (reduction) {
     total = floats(x, {});
     saved.inv_count = floats(x, {});
   }
-  check(library.xent_forward(&p, saved.log2_z.mutable_data_ptr<float>(), rows.mutable_data_ptr<float>(),
+  check(library.xent_forward(&p, saved.sums.mutable_data_ptr<float>(), rows.mutable_data_ptr<float>(),
                              reduction ? total.mutable_data_ptr<float>() : nullptr,
                              reduction ? saved.inv_count.mutable_data_ptr<float>() : nullptr, (int32_t)reduction,
                              space.mutable_data_ptr(), size, reinterpret_cast<int32_t*>(error), on.stream()),
@@ -142,12 +142,12 @@ Tensor xent_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const 
 }
 
 // Gradients into dx and dw (one type, dense rows) and db, each may be undefined.
-void xent_backward(const Tensor& x, const tthrml_xent& p, const Tensor& log2_z, const Tensor& grad, const Tensor& inv_count,
+void xent_backward(const Tensor& x, const tthrml_xent& p, const Tensor& sums, const Tensor& grad, const Tensor& inv_count,
                    const Tensor& dx, const Tensor& dw, const Tensor& db, int64_t error, void* stream) {
   const int64_t size = library.xent_backward_workspace(p.rows, p.categories, p.cols, dx.defined(), dw.defined(), db.defined());
   if (size < 0) check((int)size, "tthrml_xent_backward_workspace");
   const Tensor space = bytes(x, size);
-  check(library.xent_backward(&p, log2_z.const_data_ptr<float>(), grad.const_data_ptr<float>(), grad.dim() ? 1 : 0,
+  check(library.xent_backward(&p, sums.const_data_ptr<float>(), grad.const_data_ptr<float>(), grad.dim() ? 1 : 0,
                               inv_count.defined() ? inv_count.const_data_ptr<float>() : nullptr,
                               dx.defined() ? dx.mutable_data_ptr() : nullptr, p.cols, dw.defined() ? dw.mutable_data_ptr() : nullptr,
                               p.cols, dx.defined() ? dtype_code(dx) : (dw.defined() ? dtype_code(dw) : p.dtype),
@@ -164,7 +164,7 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
     const Tensor bias = with_bias ? bias_or_targets : Tensor();
     Tensor loss = xent_forward(x, w, bias, targets, reduction, ignored, error, s);
     // the tensors themselves, so that a change in place before the backward pass is noticed
-    ctx->save_for_backward({x, w, bias, targets, s.laid, s.log2_z, s.inv_count});
+    ctx->save_for_backward({x, w, bias, targets, s.laid, s.sums, s.inv_count});
     ctx->saved_data["ignored"] = ignored;
     ctx->saved_data["error"] = error;
     return loss;
@@ -172,7 +172,7 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), "softmax_cross_entropy has no second derivative (create_graph=True)");
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &bias = s[2], &targets = s[3], &laid = s[4], &log2_z = s[5], &inv_count = s[6];
+    const Tensor &x = s[0], &w = s[1], &bias = s[2], &targets = s[3], &laid = s[4], &sums = s[5], &inv_count = s[6];
     variable_list out(8);
     if (!grads[0].defined()) return out;
     const On on(x);
@@ -183,7 +183,7 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
     if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().requires_grad(false));
     if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options().requires_grad(false));
     if (bias.defined() && ctx->needs_input_grad(2)) out[2] = floats(x, bias.sizes());
-    xent_backward(x, p, log2_z, grad, inv_count, out[0], out[1], out[2], ctx->saved_data["error"].toInt(), on.stream());
+    xent_backward(x, p, sums, grad, inv_count, out[0], out[1], out[2], ctx->saved_data["error"].toInt(), on.stream());
     return out;
   }
 };
@@ -269,7 +269,7 @@ PyObject* softmax_cross_entropy_gradients(PyObject*, PyObject* const* args, Py_s
   Tensor loss = xent_forward(x, w, bias, targets, 1, ignored, error, s);
   Operand o[2];
   held_operands(x, w, s.laid, o);
-  xent_backward(x, problem(x, w, bias, targets, ignored, o), s.log2_z, unit, s.inv_count, Tensor(), dw, db, error, on.stream());
+  xent_backward(x, problem(x, w, bias, targets, ignored, o), s.sums, unit, s.inv_count, Tensor(), dw, db, error, on.stream());
   return THPVariable_Wrap(loss);
   END_HANDLE_TH_ERRORS
 }

@@ -28,10 +28,17 @@
 namespace tthrml {
 namespace {
 
-constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2E = 1.44269504088896340736f;
 constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
-constexpr int64_t kFewRows = 128;             // whose g is held in two pieces of 16 bits
-constexpr int kChunk = 8;  // 64-wide blocks of K that a logit's sum stays in tensor memory for; at least kShort
+// The products take g in 16 bits.  Where few of its values meet in a sum, their roundings' errors do not average out, and g is held
+// in two pieces, the rounding's remainder the second: below the first rows, or beside the first columns.  (64 columns are one block of
+// the sum for dx, 128 half a tile's rows for dw: the products take as long.)
+constexpr int64_t kFewRows = 128, kFewCategories = 64;
+// 64-wide blocks of K that a logit's sum stays in tensor memory for.  The tensor core cuts its sums off instead of rounding them;
+// float32 registers add them up every few blocks.  Four leave errors of losses and db below 3e-7, eight below 5e-7, 32 some of 3e-6
+// (relative, 2 to 8192 columns).  Up to 128 rows wait for the weights anyway (64 x 4096 x 32768, losses: 56 us with four, 56 with
+// eight, 62 with two); more rows wait for the MMAs (8192 rows: 1.53 ms, 1.36, 1.67).
+constexpr int chunk_of(int64_t rows) { return rows <= 128 ? 4 : 8; }
 enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
 
 struct RowTargets {
@@ -60,7 +67,7 @@ struct XentArgs {
   float* target_logit;  // [M]
   uint32_t* counter;    // zeroed for k_xent_loss
   // kGradient
-  const float* log2_z;    // [M]
+  const float2* sums;     // [M] (maximum, sum) over all categories
   const float* row_grad;  // [M] weights, or NULL: ones
   const float* top_grad;  // what they are divided by
   float unit;             // g is held times this
@@ -71,8 +78,9 @@ struct XentArgs {
   void* out;
   int64_t out_ld;
   int32_t out_dtype, align, accumulate, scaled, tma_store;
-  int32_t second;  // kGradient: the row of `out` where the remainders of the rounding begin, 0: they are dropped.  kProduct: the
-                   // block of K from which on B's rows begin again
+  int32_t second;  // kGradient: the row of `out` where the remainders of the rounding begin, or 0.  kProduct: the block of K from
+                   // which on B's rows begin again
+  int32_t beside;  // kGradient: the column where they begin, all columns before and behind it written, or 0.  Neither: dropped
   const float* factor[2];
   const float* carry;  // kProduct, scaled: sums of earlier pieces to add, [M][carry_ld] with room for whole 32 columns
   int64_t carry_ld;
@@ -98,7 +106,6 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // Sixteen warps where the sums are short (kShort blocks) and the epilogue is what a tile waits for; beside long sums eight do, and
 // leave room for more stages (losses of 8192 x 32768: 128 columns 105 us with sixteen, 162 with eight; 4096 columns 1.38 ms, 1.35).
 constexpr int kShort = 8;
-static_assert(kShort <= kChunk, "short sums are one accumulation");
 constexpr int parts_of(bool brief, int bn) { return brief && bn >= 128 ? 4 : 2; }
 template <int EPI, int BN, int CTAS, bool BRIEF>
 struct XentShape {
@@ -346,12 +353,13 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
       const int m = mb * kRows + (int)rank * 128 + quad * 32 + lane;
       float top = -INFINITY, sum = 0.0f;  // kPartials: sum 2^top
       int64_t y = -1;                     // column of the row's target
-      float weight = 0.0f, log2_z = 0.0f, factor = 1.0f;
+      float weight = 0.0f, share = 0.0f, factor = 1.0f;  // of a gradient: softmax times weight is 2^(l - top) share
       if (EPI != kProduct && m < a.M) {
         const int64_t t = target_of(a.targets, m);
         y = t - a.first;
         if (EPI != kPartials) {
-          log2_z = __ldg(a.log2_z + m);
+          const float2 z = __ldg(a.sums + m);
+          top = z.x;
           weight = a.unit;
           if (a.row_grad) {
             const float most = __ldg(a.top_grad);
@@ -359,14 +367,15 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
             weight *= most > 0.0f ? own / most : own * 0.0f;  // nothing but zeros and NaN: a NaN stays
           }
           if (t < 0 || t >= a.categories) weight = __uint_as_float(0x7FC00000u);
-          if (log2_z == -INFINITY || t == a.targets.ignored) weight = 0.0f;
+          if (z.y == 0.0f || t == a.targets.ignored) weight = 0.0f;
+          share = weight / z.y;  // the sum beside its maximum: their logarithm would be rounded at the size of the logits
         }
       }
       if (EPI == kProduct && a.scaled) factor = factor_of(a.factor) / a.unit;
       // what becomes of 32 sums of this thread's row, from column n on (called by whole warps)
       const auto finish = [&](float (&v)[32], int n) {
         const int live = min(32, a.N - n);
-        if (live <= 0) return;
+        if (a.beside ? n >= a.beside : live <= 0) return;
         if (EPI != kProduct) {
           if (a.bias) {
 #pragma unroll
@@ -413,10 +422,10 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              fma2(v[j], v[j + 1], kLog2E, -log2_z, v[j], v[j + 1]);
+              fma2(v[j], v[j + 1], kLog2E, -top, v[j], v[j + 1]);
               v[j] = exp2_fast(v[j]);
               v[j + 1] = exp2_fast(v[j + 1]);
-              mul2(v[j], v[j + 1], weight);
+              mul2(v[j], v[j + 1], share);
             }
             if (y >= n && y < n + live) {
 #pragma unroll
@@ -432,15 +441,15 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
           uint4 w[4];
           pack_row<4>(v, a.out_dtype, w);
           unsigned char* out = (unsigned char*)a.out;
-          if (live == 32)
+          if (live == 32 || a.beside)
             store_rows64(w, buffer, out + 2 * n, 2 * a.out_ld, m - lane, rows);
           else
             store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, 2 * live, 16);
-          if (a.second) {
+          if (a.second || a.beside) {
             less_row(v, a.out_dtype, w);
             pack_row<4>(v, a.out_dtype, w);
-            out += 2 * a.second * a.out_ld;
-            store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, 2 * live, 16);
+            out += 2 * (a.second * a.out_ld + a.beside);
+            store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, a.beside ? 64 : 2 * live, 16);
           }
         } else if (a.tma_store) {
 #pragma unroll
@@ -583,7 +592,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
   }
 }
 
-// Joins the partial sums of a row (a warp per row) into log2 z and the row's loss; the last block adds the losses, in an
+// Joins the partial sums of a row (a warp per row) into one and the row's loss, in 64 bits from there on; the last block adds the losses, in an
 // order that does not depend on which block is the last.
 struct LossArgs {
   const float2* part;
@@ -591,7 +600,8 @@ struct LossArgs {
   RowTargets targets;
   int64_t rows, categories;
   int32_t slots, reduction;  // 0: none, 1: mean over the rows that count, 2: sum
-  float *log2_z, *loss;      // [rows]
+  float2* sums;              // [rows]
+  float* loss;               // [rows]
   float *total, *inv_count;  // the reduced loss, and 1 / the rows that count (1 at least) or 1
   uint32_t* counter;
 };
@@ -622,16 +632,16 @@ __global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
       }
     }
     if (lane == 0) {
-      const float z = s == 0.0f ? -INFINITY : m + log2f(s);  // no category is possible: z = -inf
       const int64_t y = target_of(a.targets, row);
       float loss = 0.0f;
       if (y != a.targets.ignored) {
         if (y < 0 || y >= a.categories)
           loss = __uint_as_float(0x7FC00000u);
         else
-          loss = z == -INFINITY ? INFINITY : z * kLn2 - __ldcg(a.target_logit + row);
+          loss = s == 0.0f ? INFINITY  // no category is possible
+                           : (float)(((double)m + log2((double)s)) * (1.0 / (double)kLog2E) - (double)__ldcg(a.target_logit + row));
       }
-      a.log2_z[row] = z;
+      a.sums[row] = make_float2(m, s);
       a.loss[row] = loss;
     }
   }
@@ -824,7 +834,7 @@ int box_rows(int64_t rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <
 int tile_width(int64_t rows, int64_t n, int64_t pairs) {
   const int64_t ctas = tile_ctas(rows), m_blocks = up(rows, 128 * ctas) / (128 * ctas), at_once = pairs * 2 / ctas;
   for (int bn = 256; bn > 64; bn /= 2)
-    if (m_blocks * (up(n, bn) / bn) >= at_once) return bn;
+    if (n > bn / 2 && m_blocks * (up(n, bn) / bn) >= at_once) return bn;
   return 64;
 }
 // Tiles along N per unit: as few rounds of units as possible, then as few partial sums.
@@ -864,31 +874,35 @@ int plan_forward(int64_t rows, int64_t categories, int64_t cols, ForwardPlan* p)
 
 struct BackwardPlan {
   int64_t piece, pieces, g_ld, plane_ld, dx_shares, dw_shares;
-  int64_t second, g_rows;  // the row where the second pieces begin (0: none), and all rows of g
-  bool dx_planes;
+  int64_t second, beside;  // the row or the column where the second pieces begin (0: none)
+  int64_t g_rows, g_cols;  // of g with them, of a piece
+  bool dx_planes, dw_planes;
   int64_t bias, top, dx, dw, bytes;  // places in the workspace behind g
 };
 int plan_backward(int64_t rows, int64_t categories, int64_t cols, bool want_x, bool want_w, bool want_b, BackwardPlan* p) {
   int64_t pairs;
   const int rc = resident_pairs(&pairs);
   if (rc) return rc;
-  p->second = rows <= kFewRows ? up(rows, 64) : 0;
+  p->beside = categories <= kFewCategories ? kFewCategories : 0;
+  p->second = rows <= kFewRows && !p->beside ? up(rows, 64) : 0;
   p->g_rows = p->second ? 2 * p->second : rows;
   const int64_t most = std::max<int64_t>(256, kPieceBytes / 2 / p->g_rows / 256 * 256);
   p->pieces = (categories + most - 1) / most;
   p->piece = up((categories + p->pieces - 1) / p->pieces, 256);
   p->pieces = (categories + p->piece - 1) / p->piece;
   const int64_t width = std::min(p->piece, categories);
-  p->g_ld = up(width, 64);
+  p->g_cols = p->beside ? 2 * p->beside : width;
+  p->g_ld = up(p->g_cols, 64);
   p->plane_ld = up(cols, 32);
-  p->dx_shares = want_x ? shares(p->g_rows, cols, width, pairs) : 0;
-  p->dw_shares = want_w ? shares(width, cols, p->g_rows, pairs) : 0;
+  p->dx_shares = want_x ? shares(p->g_rows, cols, p->g_cols, pairs) : 0;
+  p->dw_shares = want_w ? shares(p->g_cols, cols, p->g_rows, pairs) : 0;
   p->dx_planes = want_x && (p->dx_shares > 1 || p->pieces > 1 || p->second);
+  p->dw_planes = want_w && (p->dw_shares > 1 || p->beside);
   p->bias = up(p->g_rows * p->g_ld * 2, 16);
   p->top = p->bias + (want_b ? up(rows, 32) / 32 * p->g_ld * 4 : 0);
   p->dx = p->top + 16;
   p->dw = p->dx + (p->dx_planes ? p->dx_shares * p->g_rows * p->plane_ld * 4 : 0);
-  p->bytes = p->dw + (p->dw_shares > 1 ? p->dw_shares * width * p->plane_ld * 4 : 0);
+  p->bytes = p->dw + (p->dw_planes ? p->dw_shares * p->g_cols * p->plane_ld * 4 : 0);
   return TTHRML_OK;
 }
 
@@ -960,13 +974,13 @@ extern "C" int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categorie
   return rc ? rc : p.bytes;
 }
 
-extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* row_loss, float* loss, float* inv_count,
+extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* sums, float* row_loss, float* loss, float* inv_count,
                                    int32_t reduction, void* workspace, int64_t workspace_bytes, int32_t* error, void* stream) {
   using namespace tthrml;
   int rc = check_problem("tthrml_xent_forward", p);
   if (rc) return rc;
-  if (!log2_z || !row_loss || !workspace || !error || reduction < 0 || reduction > 2 || (reduction && (!loss || !inv_count))) {
-    set_error("tthrml_xent_forward: NULL argument or unknown reduction %d", (int)reduction);
+  if (!sums || (uintptr_t)sums % 8 || !row_loss || !workspace || !error || reduction < 0 || reduction > 2 || (reduction && (!loss || !inv_count))) {
+    set_error("tthrml_xent_forward: NULL argument, sums not 8-byte aligned or unknown reduction %d", (int)reduction);
     return TTHRML_ERR_ARG;
   }
   ForwardPlan f;
@@ -1005,10 +1019,10 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* log2_z, float* r
   a.target_logit = (float*)(ws + f.logits);
   a.counter = (uint32_t*)(ws + f.counter);
   a.error = error;
-  a.chunk = kChunk;
+  a.chunk = chunk_of(p->rows);
   rc = launch_logits<kPartials>(ctas, f.bn, ma, mb, a, st);
   if (rc) return rc;
-  LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, log2_z, row_loss, loss, inv_count,
+  LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, (float2*)sums, row_loss, loss, inv_count,
                 a.counter};
   void* params[1] = {(void*)&l};
   return launch_clusters((const void*)k_xent_loss, (unsigned)((p->rows + 7) / 8), 1, 256, 0, params, st, "k_xent_loss launch",
@@ -1026,15 +1040,15 @@ extern "C" int64_t tthrml_xent_backward_workspace(int64_t rows, int64_t categori
   return rc ? rc : p.bytes;
 }
 
-extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, const float* grad, int32_t grad_per_row,
+extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* sums, const float* grad, int32_t grad_per_row,
                                     const float* inv_count, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld,
                                     int32_t grad_dtype, float* db, void* workspace, int64_t workspace_bytes, int32_t* error,
                                     void* stream) {
   using namespace tthrml;
   int rc = check_problem("tthrml_xent_backward", p);
   if (rc) return rc;
-  if (!log2_z || !grad || !workspace || !error || (dx && dx_ld < p->cols) || (dw && dw_ld < p->cols)) {
-    set_error("tthrml_xent_backward: NULL argument, or gradients whose rows overlap");
+  if (!sums || (uintptr_t)sums % 8 || !grad || !workspace || !error || (dx && dx_ld < p->cols) || (dw && dw_ld < p->cols)) {
+    set_error("tthrml_xent_backward: NULL argument, sums not 8-byte aligned, or gradients whose rows overlap");
     return TTHRML_ERR_ARG;
   }
   if (grad_dtype == TTHRML_DT_I8 || dtype_bytes(grad_dtype) == 0) {
@@ -1062,7 +1076,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
   base.unit = f16 ? 16384.0f : 1.0f;
   base.categories = p->categories;
   base.targets = {p->targets, p->wide_targets, p->ignored};
-  base.log2_z = log2_z;
+  base.sums = (const float2*)sums;
   base.error = error;
   base.factor[0] = grad_per_row ? top : grad;
   base.factor[1] = inv_count;
@@ -1083,14 +1097,15 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
   if (rc == TTHRML_OK) rc = make_map(&mx_mn, p->x, p->rows, p->cols, p->x_ld, 64u, f16);
   for (int64_t i = 0; i < f.pieces && rc == TTHRML_OK; ++i) {
     const int64_t first = i * f.piece, width = std::min(f.piece, p->categories - first);
+    const int64_t g_cols = f.beside ? f.g_cols : width;
     const char* w = (const char*)p->w + first * p->w_ld * 2;
     CUtensorMap mw, mw_mn, mg, mg_mn;
     FinishArgs finish = {};
     const int bn = tile_width(p->rows, width, pairs), ctas = tile_ctas(p->rows);
     rc = make_map(&mw, w, width, p->cols, p->w_ld, (uint32_t)(bn / ctas), f16);
     if (rc == TTHRML_OK) rc = make_map(&mw_mn, w, width, p->cols, p->w_ld, 64u, f16);
-    if (rc == TTHRML_OK) rc = make_map(&mg, ws, f.g_rows, width, f.g_ld, 128u, f16);
-    if (rc == TTHRML_OK) rc = make_map(&mg_mn, ws, f.g_rows, width, f.g_ld, 64u, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mg, ws, f.g_rows, g_cols, f.g_ld, 128u, f16);
+    if (rc == TTHRML_OK) rc = make_map(&mg_mn, ws, f.g_rows, g_cols, f.g_ld, 64u, f16);
     if (rc) return rc;
     XentArgs a = base;
     a.M = (int32_t)p->rows;
@@ -1108,9 +1123,9 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
     a.first = first;
     a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
     a.bias_ld = f.g_ld;
-    // db is a sum over the rows: where many of them meet in a category, its logits have to be as good as the losses'
-    a.chunk = db ? (p->rows <= p->categories ? 4 * kChunk : kChunk) : a.num_k;
+    a.chunk = db ? chunk_of(p->rows) : a.num_k;  // db is not rounded to 16 bits: its logits have to be as good as the losses'
     a.second = (int32_t)f.second;
+    a.beside = (int32_t)f.beside;
     a.out = ws;
     a.out_ld = f.g_ld;
     a.out_dtype = p->dtype;
@@ -1128,23 +1143,24 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* log2_z, c
       d.accumulate = planes && i > 0;
       d.carry = ends ? (const float*)(ws + f.dx) : nullptr;
       d.carry_ld = f.plane_ld;
-      rc = product<false>(mg, mw_mn, d, f.g_rows, p->cols, width, std::min(f.dx_shares, up(width, 64) / 64), pairs, st);
+      d.second = (int32_t)(f.beside / 64);
+      rc = product<false>(mg, mw_mn, d, f.g_rows, p->cols, g_cols, std::min(f.dx_shares, up(g_cols, 64) / 64), pairs, st);
       if (rc) return rc;
     }
     if (dw) {
       XentArgs d = base;
       char* out = (char*)dw + first * dw_ld * bytes;
-      const bool planes = f.dw_shares > 1;
+      const bool planes = f.dw_planes;
       d.scaled = !planes;
       d.out = planes ? (void*)(ws + f.dw) : out;
       d.out_ld = planes ? f.plane_ld : dw_ld;
       d.out_dtype = planes ? TTHRML_DT_F32 : grad_dtype;
       d.align = alignment(out, dw_ld);
       d.second = (int32_t)(f.second / 64);
-      rc = product<true>(mg_mn, mx_mn, d, width, p->cols, f.g_rows, f.dw_shares, pairs, st);
+      rc = product<true>(mg_mn, mx_mn, d, g_cols, p->cols, f.g_rows, f.dw_shares, pairs, st);
       if (rc) return rc;
       if (planes)
-        join_later(finish.w, finish.w_blocks, (const float*)(ws + f.dw), width * f.plane_ld, f.plane_ld, width, p->cols, 0,
+        join_later(finish.w, finish.w_blocks, (const float*)(ws + f.dw), g_cols * f.plane_ld, f.plane_ld, width, p->cols, f.beside,
                    f.dw_shares, base, out, dw_ld, grad_dtype);
     }
     if (db) {
