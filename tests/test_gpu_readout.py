@@ -101,6 +101,29 @@ def test_the_hidden_block_of_a_dense_program(tt, precision):
     assert torch.equal(r.fields(ex), other.fields(ex.dense_units(1).clone()))
 
 
+def test_units_that_are_still_made_are_waited_for(tt, monkeypatch):
+    """Units that are rounded on the executor's stream are used after that, however late it comes."""
+    prog = workloads.gaussian_bernoulli_rbm(32, 64, seed=2, w_std=0.05)
+    ex = tt.Executor(None, tt.open_device(None), prog, tt.make_cuda_config(dense_precision="fp32"), n_chains=16)
+    g = torch.Generator().manual_seed(3)
+    spins = torch.randint(0, 2, (16, 64), generator=g).bool()
+    ex.load_state([torch.randn((16, 32), generator=g), spins], [])
+    units = torch.where(spins, 1.0, -1.0).bfloat16().cuda()
+    _, y = data(16, 1, 10, 3)
+    r = tt.CategoricalReadout(64, 10, seed=5)
+    want = r.loss(units, y)
+    torch.cuda.synchronize()
+
+    def late(block):
+        with torch.cuda.stream(ex.stream):
+            held = torch.zeros_like(units)
+            torch.cuda._sleep(200_000_000)
+            return held.copy_(units)
+
+    monkeypatch.setattr(ex, "dense_units", late)
+    assert torch.equal(r.loss(ex, y), want)
+
+
 def test_fields_are_those_of_the_rounded_weights(tt):
     r = tt.CategoricalReadout(256, 500, seed=2)
     with pytest.raises(RuntimeError, match="quantize"):

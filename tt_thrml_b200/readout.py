@@ -76,8 +76,8 @@ class CategoricalReadout:
         """(the features in the operands' type, the executor that is to wait for their use or None)."""
         torch = _torch()
         if isinstance(x, Executor):
+            units = x.dense_units(1)  # float32 states are rounded on the executor's stream, so that stream is waited for after
             torch.cuda.current_stream(self.device).wait_stream(x.stream)
-            units = x.dense_units(1)
             return units.to(self._operands.dtype), x
         require_cuda("x", x, self.device)
         if not x.is_floating_point():
