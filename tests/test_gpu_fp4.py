@@ -230,6 +230,24 @@ def test_given_codes_with_odd_rows(tt):
         check_product(tt.fp4_product(x.cuda(), q), with_blocks(ca, ba), sa, c, scale.numpy(), None, torch.float32)
 
 
+@pytest.mark.parametrize("m", [1, 3, 70, 300])
+@pytest.mark.parametrize("cols", [1, 33, 255])
+def test_the_half_byte_behind_odd_columns_does_not_count(tt, m, cols):
+    """Codes whose last half byte holds anything, on both sides of a product: the sums are those of the columns."""
+    g = torch.Generator().manual_seed(cols + m)
+    bytes_, blocks = (cols + 1) // 2, (cols + 15) // 16
+
+    def rows(n):
+        codes = torch.randint(0, 256, (n, (bytes_ + 15) // 16 * 16), generator=g, dtype=torch.uint8).cuda()[:, :bytes_]
+        codes[:, -1] |= 0x70
+        return tt.Fp4Rows(codes, torch.full((n, blocks), 2.0).to(torch.float8_e4m3fn).cuda(), torch.ones(n).cuda(), cols=cols)
+
+    x, w = rows(m), rows(90)
+    exact = x.dequantize().double() @ w.dequantize().double().t()
+    assert torch.equal(tt.fp4_product(x, w).double(), exact)  # sums of multiples of 1 below 255 * 144: exact in float32
+    assert x.codes.shape == (m, bytes_) and int((x.codes[:, -1] >> 4).max()) == 0
+
+
 def test_nothing_to_do(tt):
     w = tt.quantize_fp4(torch.ones(4, 32, device="cuda"))
     assert tt.fp4_product(torch.ones(0, 32, device="cuda"), w).shape == (0, 4)

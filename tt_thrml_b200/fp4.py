@@ -61,8 +61,9 @@ class Fp4Rows:
     codes: uint8 [rows, ceil(cols / 2)], two codes to a byte, the even column in
     the low half.  block_scale: float8_e4m3fn [rows, ceil(cols / 16)], not
     negative.  scale: float32 [rows].  cols: the columns (default: two per byte).
-    Codes whose rows are not 16-byte aligned and a multiple of 16 bytes apart, and
-    the block scales, are laid out again once, here.
+    Codes whose rows are not 16-byte aligned and a multiple of 16 bytes apart, or of
+    odd columns (the half byte behind the last one is not read), and the block
+    scales, are laid out again once, here.
     """
 
     def __init__(self, codes, block_scale, scale, *, cols=None):
@@ -84,9 +85,11 @@ class Fp4Rows:
         if scale.dtype != torch.float32 or tuple(scale.shape) != (rows,):
             raise ValueError(f"scale must be float32 of shape ({rows},), got {scale.dtype} of {tuple(scale.shape)}")
         pitch = codes.stride(0) if rows > 1 else -(-bytes_ // 16) * 16
-        if (bytes_ > 1 and codes.stride(1) != 1) or pitch % 16 or pitch < bytes_ or codes.data_ptr() % 16:
+        if cols % 2 or (bytes_ > 1 and codes.stride(1) != 1) or pitch % 16 or pitch < bytes_ or codes.data_ptr() % 16:
             laid = torch.zeros((rows, -(-bytes_ // 16) * 16), dtype=torch.uint8, device=codes.device)
             laid[:, :bytes_].copy_(codes)
+            if cols % 2:
+                laid[:, bytes_ - 1] &= 15  # the half behind the last column counts in no product
             codes, pitch = laid[:, :bytes_], laid.shape[1]
         # [row block, 4 x 32 rows, column block, 4 x 4 scales] -> [row block, column block, 4, 32 rows, 4 row groups, 4]
         m, k = -(-rows // 128), -(-cols // 256)
