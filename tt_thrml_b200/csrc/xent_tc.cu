@@ -731,7 +731,8 @@ __device__ __forceinline__ void join_rows(const JoinArgs& a, int64_t block, int6
   }
 }
 
-// db[n] = factor * sum over the groups of 32 rows, in their order; eight threads share a column.
+// db[n] = factor * sum over the groups of 32 rows, in their order and in 64 bits (there may be half a million); eight threads share
+// a column.
 struct BiasArgs {
   const float* part;
   int64_t groups, ld, n;
@@ -740,17 +741,19 @@ struct BiasArgs {
   float unit;
 };
 __device__ __forceinline__ void bias_sums(const BiasArgs& a, int64_t block) {
-  __shared__ float sums[8][33];
+  __shared__ double sums[8][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = block * 32 + lane;
-  float s = 0.0f;
-  if (c < a.n)
-    for (int64_t g = warp; g < a.groups; g += 8) s += __ldcg(a.part + g * a.ld + c);
+  double s = 0.0;
+  if (c < a.n) {
+#pragma unroll 4
+    for (int64_t g = warp; g < a.groups; g += 8) s += (double)__ldcg(a.part + g * a.ld + c);
+  }
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < a.n) {
     for (int i = 1; i < 8; ++i) s += sums[i][lane];
-    a.db[c] = s * (factor_of(a.factor) / a.unit);
+    a.db[c] = (float)(s * (double)(factor_of(a.factor) / a.unit));
   }
 }
 
