@@ -9,19 +9,19 @@
 // turned into g (16 bits), which two further products reduce to this piece's rows of dw and to sums of dx in float32.
 //
 // One kernel serves the four products: persistent clusters of two CTAs walk 256 x BN tiles (tcgen05 cta_group::2, two
-// TMEM accumulators, six stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
-// transposed.  Warps 2 on run the epilogue of a tile beside the main loop of the next one: eight, or sixteen on the wider tiles of
-// logits.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for half the weights, which
+// TMEM accumulators, five to eight stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
+// transposed.  Warps 2 on run the epilogue of a tile beside the main loop of the next one: eight, or sixteen where the logits are
+// short sums.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for half the weights, which
 // are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the even CTA multiplies.
 //
-// g is rounded to the operands' 16 bits (up to kFewRows rows: held in two such pieces, their sum good to 2^-16; the
-// second piece is more rows of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
+// g is rounded to the operands' 16 bits (up to kFewRows rows or kFewCategories categories: held in two such pieces, their sum
+// good to 2^-16; the second piece is more rows or columns of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
 // themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
 // sums, z, losses and the sums of db are float32; dx and dw accumulate in float32.
 //
 // What bounds it: the tensor pipe (97 % active in each of the four products; 4096 rows, 4096 columns, 16384 categories: logits
 // 332 us, g 340, dx 379, dw 339, 1.45 to 1.65 PFLOP/s at the clocks of a short run) and, over longer runs, the power cap
-// (8192 x 4096 x 32768, the whole step: 6.5 to 6.7 ms, 1.31 to 1.36 PFLOP/s); the weights' bytes for few rows.
+// (8192 x 4096 x 32768, the whole step: 6.1 to 6.7 ms, 1.31 to 1.43 PFLOP/s); the weights' bytes for few rows.
 #include "int8_common.cuh"
 #include "tc_common.cuh"
 
@@ -36,7 +36,7 @@ constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
 constexpr int64_t kFewRows = 128, kFewCategories = 64;
 // 64-wide blocks of K that a logit's sum stays in tensor memory for.  The tensor core cuts its sums off instead of rounding them;
 // float32 registers add them up every few blocks.  Four leave errors of losses and db below 3e-7, eight below 5e-7, 32 some of 3e-6
-// (relative, 2 to 8192 columns).  Up to 128 rows wait for the weights anyway (64 x 4096 x 32768, losses: 56 us with four, 56 with
+// (relative, over 150 random sizes of 8 to 8192 columns).  Up to 128 rows wait for the weights anyway (64 x 4096 x 32768, losses: 56 us with four, 56 with
 // eight, 62 with two); more rows wait for the MMAs (8192 rows: 1.53 ms, 1.36, 1.67).
 constexpr int chunk_of(int64_t rows) { return rows <= 128 ? 4 : 8; }
 enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
