@@ -35,10 +35,11 @@ constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
 // the sum for dx, 128 half a tile's rows for dw: the products take as long.)
 constexpr int64_t kFewRows = 128, kFewCategories = 64;
 // 64-wide blocks of K that a logit's sum stays in tensor memory for.  The tensor core cuts its sums off instead of rounding them;
-// float32 registers add them up every few blocks.  Four leave errors of losses and db below 3e-7, eight below 5e-7, 32 some of 3e-6
-// (relative, over 150 random sizes of 8 to 8192 columns).  Up to 128 rows wait for the weights anyway (64 x 4096 x 32768, losses: 56 us with four, 56 with
-// eight, 62 with two); more rows wait for the MMAs (8192 rows: 1.53 ms, 1.36, 1.67).
-constexpr int chunk_of(int64_t rows) { return rows <= 128 ? 4 : 8; }
+// float32 registers add them up every few blocks, in both passes the same, so that probabilities and normalisers agree.  Errors of
+// losses and db over 150 random sizes of 8 to 8192 columns, relative: four below 3e-7, eight below 5e-7, 32 some of 3e-6 (eight after
+// four 1e-6).  Two, four and eight take 1.67, 1.53 and 1.36 ms for the losses of 8192 x 4096 x 32768, four and eight 62 and 59 us for
+// those of 64 rows; four are taken where few rows meet few categories: nothing averages the errors out, and the time is not the tiles'.
+constexpr int chunk_of(int64_t rows, int64_t categories) { return rows <= 128 && categories <= 4096 ? 4 : 8; }
 enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
 
 struct RowTargets {
@@ -1022,7 +1023,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* sums, float* row
   a.target_logit = (float*)(ws + f.logits);
   a.counter = (uint32_t*)(ws + f.counter);
   a.error = error;
-  a.chunk = chunk_of(p->rows);
+  a.chunk = chunk_of(p->rows, p->categories);
   rc = launch_logits<kPartials>(ctas, f.bn, ma, mb, a, st);
   if (rc) return rc;
   LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, (float2*)sums, row_loss, loss, inv_count,
@@ -1126,7 +1127,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* sums, con
     a.first = first;
     a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
     a.bias_ld = f.g_ld;
-    a.chunk = db ? chunk_of(p->rows) : a.num_k;  // db is not rounded to 16 bits: its logits have to be as good as the losses'
+    a.chunk = db ? chunk_of(p->rows, p->categories) : a.num_k;  // db is not rounded to 16 bits: its logits have to be as good as the losses'
     a.second = (int32_t)f.second;
     a.beside = (int32_t)f.beside;
     a.out = ws;
