@@ -768,7 +768,8 @@ int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories, int64_t 
  * dx [rows][dx_ld], dw [categories][dw_ld] (grad_dtype: float32, bfloat16 or
  * float16) and db [categories], each NULL or written, of
  * sum_t weight[t] loss[t].  weight: grad[0] * (inv_count ? *inv_count : 1), or,
- * grad_per_row, grad[t].
+ * grad_per_row, grad[t].  workspace: tthrml_xent_backward_workspace(...) bytes,
+ * 32-byte aligned.
  */
 int tthrml_xent_backward(const tthrml_xent* problem_host, const float* sums_dev,
                          const float* grad_dev, int32_t grad_per_row, const float* inv_count_dev,

@@ -11,12 +11,13 @@
 // One kernel serves the four products: persistent clusters of two CTAs walk 256 x BN tiles (tcgen05 cta_group::2, two
 // TMEM accumulators, five to eight stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
 // transposed.  Warps 2 on run the epilogue of a tile beside the main loop of the next one: eight, or sixteen where the logits are
-// short sums.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for half the weights, which
-// are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the even CTA multiplies.
+// short sums or db is summed up beside.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for
+// half the weights, which are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the
+// even CTA multiplies.
 //
 // g is rounded to the operands' 16 bits (up to kFewRows rows or kFewCategories categories: held in two such pieces, their sum
-// good to 2^-16; the second piece is more rows or columns of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of each element, as dx and dw
-// themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
+// good to 2^-16; the second piece is more rows or columns of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of
+// each element, as dx and dw themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
 // sums, z, losses and the sums of db are float32; dx and dw accumulate in float32.
 //
 // What bounds it: the tensor pipe (97 % active in each of the four products; 4096 rows, 4096 columns, 16384 categories: logits
@@ -38,8 +39,13 @@ constexpr int64_t kFewRows = 128, kFewCategories = 64;
 // float32 registers add them up every few blocks, in both passes the same, so that probabilities and normalisers agree.  Errors of
 // losses and db over 150 random sizes of 8 to 8192 columns, relative: four below 3e-7, eight below 5e-7, 32 some of 3e-6 (eight after
 // four 1e-6).  Two, four and eight take 1.67, 1.53 and 1.36 ms for the losses of 8192 x 4096 x 32768, four and eight 62 and 59 us for
-// those of 64 rows; four are taken where few rows meet few categories: nothing averages the errors out, and the time is not the tiles'.
-constexpr int chunk_of(int64_t rows, int64_t categories) { return rows <= 128 && categories <= 4096 ? 4 : 8; }
+// those of 64 rows; fewer are taken where few rows meet few categories: nothing averages the errors out, and the time is not the
+// tiles' (db of 13 x 409 x 2: 1.1e-7, 1.4e-7 and 1.8e-7 in the middle of 200 inputs with one, two and four, and 1.0e-7 in plain
+// float32; a step of 100 x 8192 x 10 in 149, 118 and 103 us).
+constexpr int chunk_of(int64_t rows, int64_t categories) {
+  return rows > 128 || categories > 4096 ? 8 : (categories > 64 ? 4 : 2);
+}
+constexpr bool one_chunk(int64_t rows, int64_t categories, int64_t cols) { return (cols + 63) / 64 <= chunk_of(rows, categories); }
 enum : int { kPartials = 0, kGradient = 1, kGradientSums = 2, kProduct = 3 };
 
 struct RowTargets {
@@ -104,15 +110,15 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // Parts of a tile's columns that the epilogue's warps share: four warps, a row per lane, take one.
-// Sixteen warps where the sums are short (kShort blocks) and the epilogue is what a tile waits for; beside long sums eight do, and
-// leave room for more stages (losses of 8192 x 32768: 128 columns 105 us with sixteen, 162 with eight; 4096 columns 1.38 ms, 1.35).
-constexpr int kShort = 8;
-constexpr int parts_of(bool brief, int bn) { return brief && bn >= 128 ? 4 : 2; }
+// Sixteen warps where the epilogue is what a tile waits for: beside short sums (one accumulation; losses of 8192 x 128 x 32768 in 105 us,
+// 162 with eight) and with db's sums of columns (a step of 777 x 1008 x 5008: 77 us, 80 with eight).  Else eight do (losses of 8192 x
+// 4096 x 32768 in 1.35 ms, 1.38 with sixteen).
+constexpr int parts_of(bool brief, int bn, int epi = kPartials) { return (brief || epi == kGradientSums) && bn >= 128 ? 4 : 2; }
 template <int EPI, int BN, int CTAS, bool BRIEF>
 struct XentShape {
-  static constexpr int kParts = parts_of(BRIEF, BN), kWarps = 4 * kParts, kThreads = 64 + 32 * kWarps;
+  static constexpr int kParts = parts_of(BRIEF, BN, EPI), kWarps = 4 * kParts, kThreads = 64 + 32 * kWarps;
   static constexpr int kA = 128 * 64 * 2, kB = BN / CTAS * 64 * 2, kStage = kA + kB;
-  static constexpr int kOut = EPI == kPartials ? 0 : kWarps * kOutBytes;  // rows on their way out
+  static constexpr int kOut = EPI == kProduct ? kWarps * kOutBytes : 0;  // rows on their way out
   static constexpr int kBarriers = 256;
   static constexpr int kMine = BN / kParts;  // columns of a warp
   static constexpr int kRest = 1024 + kOut + kBarriers + (EPI == kProduct ? 0 : kWarps * kMine * 4 /*their biases*/);
@@ -140,6 +146,13 @@ __device__ __forceinline__ void less_row(float (&v)[32], int32_t dtype, const ui
   }
 }
 
+// 32 bytes, a whole sector: a row per lane needs no turning in shared memory (8192 x 128 x 32768, a step: 544 us turned, 522 so).
+__device__ __forceinline__ void store_sector(unsigned char* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x),
+               "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 template <int CTAS>
 __device__ __forceinline__ void commit(uint64_t* bar) {
   if (CTAS == 2)
@@ -159,25 +172,26 @@ __device__ __forceinline__ void unit_at(const XentArgs& a, int u, int& split, in
   sg = w / rows;
 }
 
-// Sums over the warp's 32 lanes of 32 values each, turned in a buffer of 4096 bytes: lane j returns that of value j.  (By
-// shuffles it takes 124 instructions, so 75.)
-__device__ __forceinline__ float column_sums(const float (&v)[32], uint32_t buffer) {
+// Sums over the warp's 32 lanes of 32 values each: lane j returns that of value j.  (Turned in shared memory it takes 75
+// instructions instead of 124, but the MMAs keep shared memory busy: db's pass of 4096 x 512 x 8192 in 47 us, so in 43.)
+__device__ __forceinline__ float column_sums(const float (&v)[32]) {
   const uint32_t lane = threadIdx.x & 31;
+  float s[16];
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j)  // piece j of row r lies at j ^ (r & 7): rows and columns both cover every bank
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buffer + lane * 128 + 16 * (j ^ (lane & 7))), "f"(v[4 * j]),
-                 "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
-                 : "memory");
-  __syncwarp();
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (uint32_t r = 0; r < 32; ++r) {
-    float x;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buffer + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
-    s[r & 3] += x;
+  for (int j = 0; j < 16; ++j) {
+    const bool up = lane & 16;
+    const float mine = up ? v[j + 16] : v[j], other = up ? v[j] : v[j + 16];
+    s[j] = mine + __shfl_xor_sync(0xffffffffu, other, 16);
   }
-  __syncwarp();
-  return (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+    for (int j = 0; j < w; ++j) {
+      const bool up = lane & w;
+      const float mine = up ? s[j + w] : s[j], other = up ? s[j] : s[j + w];
+      s[j] = mine + __shfl_xor_sync(0xffffffffu, other, w);
+    }
+  return s[0];
 }
 
 template <int EPI, bool A_MN, bool B_MN, int BN, int CTAS, bool BRIEF>
@@ -417,40 +431,41 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
           }
           sum += (s[0] + s[1]) + (s[2] + s[3]);
         } else if (EPI == kGradient || EPI == kGradientSums) {
-          if (weight == 0.0f) {  // a row that does not count, whatever it holds
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-          } else {
+          for (int j = 0; j < 32; j += 2) {
+            fma2(v[j], v[j + 1], kLog2E, -top, v[j], v[j + 1]);
+            v[j] = exp2_fast(v[j]);
+            v[j + 1] = exp2_fast(v[j + 1]);
+            mul2(v[j], v[j + 1], share);
+          }
+          // asked of the whole warp: the selections are 64 instructions that most pieces of a row need not make
+          const int hit = y >= n && y < n + live ? (int)(y - n) : -1;
+          if (__any_sync(0xffffffffu, (int)(hit >= 0))) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              fma2(v[j], v[j + 1], kLog2E, -top, v[j], v[j + 1]);
-              v[j] = exp2_fast(v[j]);
-              v[j + 1] = exp2_fast(v[j + 1]);
-              mul2(v[j], v[j + 1], share);
-            }
-            if (y >= n && y < n + live) {
+            for (int j = 0; j < 32; ++j) v[j] = hit == j ? v[j] - weight : v[j];
+          }
+          if (__any_sync(0xffffffffu, (int)(weight == 0.0f))) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = y - n == j ? v[j] - weight : v[j];
-            }
+            for (int j = 0; j < 32; ++j) v[j] = weight == 0.0f ? 0.0f : v[j];  // a row that does not count, whatever it holds
           }
           __syncwarp();
           if (EPI == kGradientSums) {
-            const float s = column_sums(v, buffer);
+            const float s = column_sums(v);
             if (m - lane < a.M && lane < live) a.bias_part[(int64_t)(m >> 5) * a.bias_ld + n + lane] = s;
           }
-          const int rows = a.second ? a.second : a.M;  // those behind the last row are zeros
-          uint4 w[4];
-          pack_row<4>(v, a.out_dtype, w);
-          unsigned char* out = (unsigned char*)a.out;
-          if (live == 32 || a.beside)
-            store_rows64(w, buffer, out + 2 * n, 2 * a.out_ld, m - lane, rows);
-          else
-            store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, 2 * live, 16);
-          if (a.second || a.beside) {
-            less_row(v, a.out_dtype, w);
+          if (m < (a.second ? a.second : a.M)) {  // those behind the last row are zeros
+            unsigned char* out = (unsigned char*)a.out + 2 * ((int64_t)m * a.out_ld + n);  // whole 32 columns: g_ld has room
+            uint4 w[4];
             pack_row<4>(v, a.out_dtype, w);
-            out += 2 * (a.second * a.out_ld + a.beside);
-            store_rows<4>(w, turn, out, 2 * a.out_ld, 2 * n, m - lane, rows, a.beside ? 64 : 2 * live, 16);
+            store_sector(out, w[0], w[1]);
+            store_sector(out + 32, w[2], w[3]);
+            if (a.second || a.beside) {
+              less_row(v, a.out_dtype, w);
+              pack_row<4>(v, a.out_dtype, w);
+              out += 2 * (a.second * a.out_ld + a.beside);
+              store_sector(out, w[0], w[1]);
+              store_sector(out + 32, w[2], w[3]);
+            }
           }
         } else if (a.tma_store) {
 #pragma unroll
@@ -569,7 +584,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
       }
       if (EPI == kPartials && m < a.M) a.part[(int64_t)m * a.slots + S::kParts * sg + part] = make_float2(top, sum);
     }
-    if (EPI != kPartials) sent_rows_done();
+    if (EPI == kProduct) sent_rows_done();
   }
 
   tc_fence_before();
@@ -816,8 +831,8 @@ int launch_logits(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Xe
   return launch_xent<EPI, false, false, 256, CTAS, BRIEF>(ma, mb, ma, a, st);
 }
 template <int EPI>
-int launch_logits(int ctas, int bn, const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, cudaStream_t st) {
-  if (a.num_k <= kShort) {
+int launch_logits(int ctas, int bn, bool brief, const CUtensorMap& ma, const CUtensorMap& mb, XentArgs a, cudaStream_t st) {
+  if (brief) {
     a.chunk = a.num_k;
     return ctas == 1 ? launch_logits<EPI, 1, true>(bn, ma, mb, a, st) : launch_logits<EPI, 2, true>(bn, ma, mb, a, st);
   }
@@ -869,7 +884,7 @@ int plan_forward(int64_t rows, int64_t categories, int64_t cols, ForwardPlan* p)
   const int64_t ctas = tile_ctas(rows);
   p->seg = tiles_per_unit(up(rows, 128 * ctas) / (128 * ctas), n_blocks, pairs * 2 / ctas);
   p->segments = (int)((n_blocks + p->seg - 1) / p->seg);
-  p->slots = parts_of(up(cols, 64) / 64 <= kShort, p->bn) * p->segments;
+  p->slots = parts_of(one_chunk(rows, categories, cols), p->bn) * p->segments;
   p->logits = up(rows * p->slots * 8, 16);
   p->counter = p->logits + up(rows * 4, 16);
   p->bytes = p->counter + 16;
@@ -1024,7 +1039,7 @@ extern "C" int tthrml_xent_forward(const tthrml_xent* p, float* sums, float* row
   a.counter = (uint32_t*)(ws + f.counter);
   a.error = error;
   a.chunk = chunk_of(p->rows, p->categories);
-  rc = launch_logits<kPartials>(ctas, f.bn, ma, mb, a, st);
+  rc = launch_logits<kPartials>(ctas, f.bn, one_chunk(p->rows, p->categories, p->cols), ma, mb, a, st);
   if (rc) return rc;
   LossArgs l = {a.part, a.target_logit, a.targets, p->rows, p->categories, a.slots, reduction, (float2*)sums, row_loss, loss, inv_count,
                 a.counter};
@@ -1065,8 +1080,8 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* sums, con
   int64_t pairs;
   if (rc == TTHRML_OK) rc = resident_pairs(&pairs);
   if (rc) return rc;
-  if ((uintptr_t)workspace % 16 || workspace_bytes < f.bytes) {
-    set_error("tthrml_xent_backward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)f.bytes,
+  if ((uintptr_t)workspace % 32 || workspace_bytes < f.bytes) {
+    set_error("tthrml_xent_backward: needs a 32-byte aligned workspace of %lld bytes (got %lld)", (long long)f.bytes,
               (long long)workspace_bytes);
     return TTHRML_ERR_ARG;
   }
@@ -1133,7 +1148,8 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* sums, con
     a.out = ws;
     a.out_ld = f.g_ld;
     a.out_dtype = p->dtype;
-    rc = db ? launch_logits<kGradientSums>(ctas, bn, mx, mw, a, st) : launch_logits<kGradient>(ctas, bn, mx, mw, a, st);
+    const bool brief = one_chunk(p->rows, p->categories, p->cols);
+    rc = db ? launch_logits<kGradientSums>(ctas, bn, brief, mx, mw, a, st) : launch_logits<kGradient>(ctas, bn, brief, mx, mw, a, st);
     if (rc) return rc;
     if (dx) {
       XentArgs d = base;
