@@ -53,7 +53,7 @@ class On {
 Tensor floats(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat).requires_grad(false)); }
 Tensor bytes(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte).requires_grad(false)); }
 
-// The operands as the kernels read them: rows of 16-byte multiples from 16-byte boundaries, or one buffer they are laid out in.
+// The operands as the kernels read them: rows of 16-byte multiples from 16-byte boundaries, as they lie or in a copy of their own.
 struct Operand {
   const void* at;
   int64_t ld;
@@ -64,44 +64,22 @@ bool as_it_lies(const Tensor& t, Operand& o) {
   o.ld = rows > 1 ? t.stride(0) : (cols + 7) / 8 * 8;
   return (cols == 1 || t.stride(1) == 1) && o.ld % 8 == 0 && o.ld >= cols && reinterpret_cast<uintptr_t>(o.at) % 16 == 0;
 }
-Tensor lay_out(const Tensor& x, const Tensor& w, Operand (&o)[2], void* stream) {
-  const Tensor* t[2] = {&x, &w};
+// laid[i]: the copy that was made of t[i], [rows, pitch], or undefined.
+void lay_out(const Tensor* const (&t)[2], Operand (&o)[2], Tensor (&laid)[2], void* stream) {
   tthrml_pack_matrix m[2];
-  int which[2], n = 0;
-  int64_t size = 0;
+  int n = 0;
   for (int i = 0; i < 2; ++i) {
     if (as_it_lies(*t[i], o[i])) continue;
-    const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
-    o[i].ld = (cols + 7) / 8 * 8;
-    m[n] = {o[i].at, reinterpret_cast<void*>(size * 2), rows, cols, t[i]->stride(0), t[i]->stride(1), o[i].ld};
-    size += rows * o[i].ld;
-    which[n++] = i;
+    const int64_t rows = t[i]->size(0), cols = t[i]->size(1), ld = (cols + 7) / 8 * 8;
+    laid[i] = at::empty({rows, ld}, t[i]->options().requires_grad(false));
+    m[n++] = {o[i].at, laid[i].mutable_data_ptr(), rows, cols, t[i]->stride(0), t[i]->stride(1), ld};
+    o[i] = {laid[i].const_data_ptr(), ld};
   }
-  if (!n) return Tensor();
-  Tensor space = at::empty({size}, x.options().requires_grad(false));
-  char* base = static_cast<char*>(space.mutable_data_ptr());
-  for (int i = 0; i < n; ++i) {
-    m[i].dst = base + reinterpret_cast<uintptr_t>(m[i].dst);
-    o[which[i]].at = m[i].dst;
-  }
-  check(library.pack_rows(m, n, stream), "tthrml_pack_rows");
-  return space;
-}
-
-// The same operands once more, from the buffer that lay_out returned.
-void held_operands(const Tensor& x, const Tensor& w, const Tensor& laid, Operand (&o)[2]) {
-  const Tensor* t[2] = {&x, &w};
-  const char* base = laid.defined() ? static_cast<const char*>(laid.const_data_ptr()) : nullptr;
-  for (int i = 0; i < 2; ++i) {
-    const int64_t rows = t[i]->size(0), cols = t[i]->size(1);
-    if (as_it_lies(*t[i], o[i])) continue;
-    o[i] = {base, (cols + 7) / 8 * 8};
-    base += rows * o[i].ld * 2;
-  }
+  if (n) check(library.pack_rows(m, n, stream), "tthrml_pack_rows");
 }
 
 struct XentSaved {
-  Tensor laid, sums, inv_count;
+  Tensor laid[2], sums, inv_count;
 };
 
 tthrml_xent problem(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& targets, int64_t ignored, const Operand (&o)[2]) {
@@ -117,12 +95,20 @@ tthrml_xent problem(const Tensor& x, const Tensor& w, const Tensor& bias, const 
   return p;
 }
 
+constexpr const char* kRestored = "a saved tensor came back on another device, in another type or of another size";
+void restored(const Tensor& t, const Tensor& x, at::ScalarType type, int64_t numel) {
+  TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.device() == x.device() && t.scalar_type() == type && t.numel() == numel &&
+                  !t.is_neg(),
+              kRestored);
+}
+
 // bias and targets dense.
 Tensor xent_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& targets, int64_t reduction, int64_t ignored,
                     int64_t error, XentSaved& saved) {
   const On on(x);
+  const Tensor* const operands[2] = {&x, &w};
   Operand o[2];
-  saved.laid = lay_out(x, w, o, on.stream());
+  lay_out(operands, o, saved.laid, on.stream());
   const tthrml_xent p = problem(x, w, bias, targets, ignored, o);
   const int64_t size = library.xent_forward_workspace(p.rows, p.categories, p.cols);
   if (size < 0) check((int)size, "tthrml_xent_forward_workspace");
@@ -163,23 +149,45 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
     XentSaved s;
     const Tensor bias = with_bias ? bias_or_targets : Tensor();
     Tensor loss = xent_forward(x, w, bias, targets, reduction, ignored, error, s);
-    // the tensors themselves, so that a change in place before the backward pass is noticed
-    ctx->save_for_backward({x, w, bias, targets, s.laid, s.sums, s.inv_count});
+    // the tensors themselves, so that a change in place before the backward pass is noticed, beside their copies
+    ctx->save_for_backward({x, w, bias, targets, s.laid[0], s.laid[1], s.sums, s.inv_count});
     ctx->saved_data["ignored"] = ignored;
     ctx->saved_data["error"] = error;
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), "softmax_cross_entropy has no second derivative (create_graph=True)");
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &bias = s[2], &targets = s[3], &laid = s[4], &sums = s[5], &inv_count = s[6];
-    variable_list out(8);
+    variable_list s = ctx->get_saved_variables(), out(8);
     if (!grads[0].defined()) return out;
+    // a hook on saved tensors may have given them back elsewhere and with other strides
+    const Tensor &x = s[0], &w = s[1], &bias = s[2], &targets = s[3], &sums = s[6], &inv_count = s[7];
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 && x.numel() && w.numel(), kRestored);
+    const int64_t rows = x.size(0), K = x.size(1), V = w.size(0);
+    const bool wide = targets.scalar_type() == at::kLong;
+    restored(x, x, dtype_code(x) == TTHRML_DT_F16 ? at::kHalf : at::kBFloat16, rows * K);
+    restored(w, x, x.scalar_type(), V * K);
+    restored(s[3], x, wide ? at::kLong : at::kInt, rows);
+    restored(s[6], x, at::kFloat, 2 * rows);
+    if (bias.defined()) restored(s[2], x, at::kFloat, V);
+    if (inv_count.defined()) restored(s[7], x, at::kFloat, 1);
+    for (int i : {2, 3, 6, 7})
+      if (s[i].defined()) s[i] = s[i].contiguous();
     const On on(x);
     Operand o[2];
-    held_operands(x, w, laid, o);
+    const Tensor* operands[2] = {&x, &w};
+    Tensor again[2];
+    for (int i = 0; i < 2; ++i) {  // the forward pass's copies where it made them; what does not lie as it has to now is copied here
+      const Tensor& laid = s[4 + i];
+      if (!laid.defined()) continue;
+      TORCH_CHECK(laid.dim() == 2 && laid.size(0) == s[i].size(0) && laid.size(1) >= K, kRestored);
+      restored(laid, x, x.scalar_type(), laid.numel());
+      operands[i] = &laid;
+    }
+    lay_out({operands[0], operands[1]}, o, again, on.stream());
     const tthrml_xent p = problem(x, w, bias, targets, ctx->saved_data["ignored"].toInt(), o);
-    const Tensor grad = grads[0].scalar_type() == at::kFloat ? grads[0].contiguous() : grads[0].to(at::kFloat).contiguous();
+    const Tensor grad = grads[0].to(at::kFloat).contiguous();
+    TORCH_CHECK(grad.device() == x.device() && grad.dim() <= 1 && grad.numel() == (inv_count.defined() ? 1 : rows),
+                "softmax_cross_entropy: the loss' gradient has another device or shape than the loss");
     if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().requires_grad(false));
     if (ctx->needs_input_grad(1)) out[1] = at::empty(w.sizes(), w.options().requires_grad(false));
     if (bias.defined() && ctx->needs_input_grad(2)) out[2] = floats(x, bias.sizes());
@@ -218,6 +226,7 @@ struct Dropout : Function<Dropout> {
     variable_list out(5);
     if (!grads[0].defined()) return out;
     const variable_list s = ctx->get_saved_variables();
+    if (s[0].defined()) restored(s[0], grads[0], at::kInt, 1);
     const int64_t cut = ctx->saved_data["cut"].toInt(), seed = ctx->saved_data["seed"].toInt(), step = ctx->saved_data["step"].toInt();
     // a node of its own only where this pass is differentiated in turn
     out[0] = c10::GradMode::is_enabled() ? apply(grads[0], &s[0], cut, seed, step) : drop(grads[0], cut, seed, step, s[0], Tensor());
@@ -267,8 +276,9 @@ PyObject* softmax_cross_entropy_gradients(PyObject*, PyObject* const* args, Py_s
   const On on(x);
   XentSaved s;
   Tensor loss = xent_forward(x, w, bias, targets, 1, ignored, error, s);
+  const Tensor* const operands[2] = {s.laid[0].defined() ? &s.laid[0] : &x, s.laid[1].defined() ? &s.laid[1] : &w};
   Operand o[2];
-  held_operands(x, w, s.laid, o);
+  for (int i = 0; i < 2; ++i) as_it_lies(*operands[i], o[i]);
   xent_backward(x, problem(x, w, bias, targets, ignored, o), s.sums, unit, s.inv_count, Tensor(), dw, db, error, on.stream());
   return THPVariable_Wrap(loss);
   END_HANDLE_TH_ERRORS
