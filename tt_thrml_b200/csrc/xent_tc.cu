@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
   using S = XentShape<EPI, BN, CTAS, BRIEF>;
   constexpr int kRows = 128 * CTAS;  // of a tile
   static_assert(!B_MN || (BN == 256 && CTAS == 2), "MN-major halves of B are whole boxes of 64");
-  constexpr bool kChunked = !BRIEF && (EPI == kPartials || EPI == kGradientSums);
+  constexpr bool kChunked = !BRIEF && EPI != kProduct;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* turns = tiles + S::kStages * S::kStage;  // a buffer per epilogue warp
@@ -1142,7 +1142,7 @@ extern "C" int tthrml_xent_backward(const tthrml_xent* p, const float* sums, con
     a.first = first;
     a.bias_part = db ? (float*)(ws + f.bias) : nullptr;
     a.bias_ld = f.g_ld;
-    a.chunk = db ? chunk_of(p->rows, p->categories) : a.num_k;  // db is not rounded to 16 bits: its logits have to be as good as the losses'
+    a.chunk = chunk_of(p->rows, p->categories);  // as the forward pass: the sums belong to these logits
     a.second = (int32_t)f.second;
     a.beside = (int32_t)f.beside;
     a.out = ws;
