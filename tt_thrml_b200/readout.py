@@ -94,8 +94,9 @@ class CategoricalReadout:
             units, source = self._units(x)
             if self.dropout:
                 units = drop(units, self.dropout, seed=self.seed, step=self._steps)
-                self._steps += 1
             loss = mean_and_gradients(units, self._operands, targets, self.bias, self.ignore_index, self._one, *self.gradient)
+            if self.dropout:
+                self._steps += 1  # a step that was refused takes no mask
             self._used(source)
             self.optimizer.step(self.gradient)
             self._operands.copy_(self.weights)
