@@ -26,3 +26,18 @@ def test_a_refused_step_changes_nothing(tt):
             a.step(x[:, :-1], y)
         assert torch.equal(a.step(x, y), b.step(x, y)), step
         assert torch.equal(a.weights, b.weights) and torch.equal(a.bias, b.bias)
+
+
+def test_fields_are_those_of_the_last_quantize(tt):
+    """Weights and bias of one time: steps after quantize() do not show before the next one."""
+    x, y = data(64, 48, 30, 2)
+    r = tt.CategoricalReadout(48, 30, seed=7, lr=1e-1)
+    r.step(x, y)
+    r.quantize()
+    fields, bias = r.fields(x), r.bias.clone()
+    r.step(x, y)
+    assert not torch.equal(r.bias, bias)
+    assert torch.equal(r.fields(x), fields)
+    assert torch.equal(fields, tt.fp4_product(x, r.served, bias=bias))
+    r.quantize()
+    assert torch.equal(r.fields(x), tt.fp4_product(x, tt.quantize_fp4(r.weights), bias=r.bias))

@@ -41,8 +41,8 @@ class CategoricalReadout:
     on a tensor may be captured into a CUDA graph after a first one outside, and
     leaves out other units each time the graph is replayed.
     loss(x, targets): the mean loss without dropout.
-    quantize() rounds the weights to 4 bits (`served`); fields(x) are then x W^T + b
-    with them, in x's type.
+    quantize() rounds the weights to 4 bits (`served`) and keeps the bias that goes with
+    them; fields(x) are then x W^T + b of both, in x's type, whatever steps come after.
     check() raises if a kernel gave up an in-kernel wait.
     """
 
@@ -66,7 +66,7 @@ class CategoricalReadout:
         self._operands = self.weights.to(dtype)
         self._steps = torch.zeros(1, dtype=torch.int64, device=dev)  # which mask of the seed's
         self._one = torch.ones((), dtype=torch.float32, device=dev)
-        self.served = None
+        self.served = self._served_bias = None
 
     @property
     def device(self):
@@ -110,16 +110,16 @@ class CategoricalReadout:
         return loss
 
     def quantize(self) -> None:
-        self.served = quantize_fp4(self.weights)
+        self.served, self._served_bias = quantize_fp4(self.weights), self.bias.clone()
 
     def fields(self, x):
         if self.served is None:
             raise RuntimeError("quantize() makes the weights that fields are served from")
         if not isinstance(x, Executor):
-            return fp4_product(x, self.served, bias=self.bias)
+            return fp4_product(x, self.served, bias=self._served_bias)
         with _torch().no_grad():
             units, source = self._units(x)
-            fields = fp4_product(units, self.served, bias=self.bias)
+            fields = fp4_product(units, self.served, bias=self._served_bias)
             self._used(source)
         return fields
 
