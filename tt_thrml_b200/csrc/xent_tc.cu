@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(XentShape<EPI, BN, CTAS, BRIEF>::kThreads, 1)
           if (a.row_grad) {
             const float most = __ldg(a.top_grad);
             const float own = __ldg(a.row_grad + m);
-            weight *= most > 0.0f ? own / most : own * 0.0f;  // nothing but zeros and NaN: a NaN stays
+            weight *= most > 0.0f ? own / most : own * 0.0f;  // zeros but for what is not finite, which stays NaN
           }
           if (t < 0 || t >= a.categories) weight = __uint_as_float(0x7FC00000u);
           if (z.y == 0.0f || t == a.targets.ignored) weight = 0.0f;
@@ -689,14 +689,17 @@ __global__ void __launch_bounds__(256) k_xent_loss(const LossArgs a) {
   }
 }
 
-// The largest magnitude of the weights of the rows that count; one block.
+// The largest finite magnitude of the weights of the rows that count (one that is not stays with its own row); one block.
 __global__ void __launch_bounds__(1024) k_xent_top(const float* grad, RowTargets targets, int64_t rows, float* top) {
   __shared__ float part[32];
   let_next_kernel_start();
   wait_for_previous_kernel();
   float most = 0.0f;
   for (int64_t i = threadIdx.x; i < rows; i += 1024)
-    if (target_of(targets, i) != targets.ignored) most = fmaxf(most, fabsf(__ldg(grad + i)));
+    if (target_of(targets, i) != targets.ignored) {
+      const float size = fabsf(__ldg(grad + i));
+      if (size < INFINITY) most = fmaxf(most, size);
+    }
   for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
   __syncthreads();
