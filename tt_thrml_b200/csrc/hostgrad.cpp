@@ -185,7 +185,7 @@ struct SoftmaxCrossEntropy : Function<SoftmaxCrossEntropy> {
     }
     lay_out({operands[0], operands[1]}, o, again, on.stream());
     const tthrml_xent p = problem(x, w, bias, targets, ctx->saved_data["ignored"].toInt(), o);
-    const Tensor grad = grads[0].to(at::kFloat).contiguous();
+    const Tensor grad = grads[0].to(at::kFloat).resolve_neg().contiguous();
     TORCH_CHECK(grad.device() == x.device() && grad.dim() <= 1 && grad.numel() == (inv_count.defined() ? 1 : rows),
                 "softmax_cross_entropy: the loss' gradient has another device or shape than the loss");
     if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options().requires_grad(false));
@@ -200,7 +200,7 @@ Tensor drop(const Tensor& x, int64_t cut, int64_t seed, int64_t step, const Tens
   Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
   if (!x.numel()) return y;
   const On on(x);
-  const Tensor in = x.contiguous();
+  const Tensor in = x.resolve_neg().contiguous();
   check(library.dropout(in.const_data_ptr(), dtype_code(x), in.numel(), (int32_t)cut, (uint64_t)seed, (uint32_t)step,
                         step_at.defined() ? step_at.const_data_ptr() : nullptr,
                         step_at.defined() && step_at.scalar_type() == at::kLong,
@@ -234,7 +234,8 @@ struct Dropout : Function<Dropout> {
   }
 };
 
-Tensor tensor_or_none(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
+// The tensor, its values in memory (not those of a negated view); undefined for None.
+Tensor tensor_or_none(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o).resolve_neg(); }
 
 }  // namespace
 
@@ -246,12 +247,12 @@ PyObject* softmax_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t nar
     PyErr_SetString(PyExc_TypeError, "softmax_cross_entropy(x, weights, bias, targets, reduction, ignored, error)");
     return nullptr;
   }
-  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+  const Tensor x = tensor_or_none(args[0]), w = tensor_or_none(args[1]);
   Tensor bias = tensor_or_none(args[2]);
   const int64_t reduction = PyLong_AsLongLong(args[4]), ignored = PyLong_AsLongLong(args[5]), error = PyLong_AsLongLong(args[6]);
   if (PyErr_Occurred()) return nullptr;
   if (bias.defined()) bias = bias.contiguous();
-  const Tensor targets = THPVariable_Unpack(args[3]).contiguous();
+  const Tensor targets = tensor_or_none(args[3]).contiguous();
   if (wants_grad(x) || wants_grad(w) || (bias.defined() && wants_grad(bias)))
     return THPVariable_Wrap(SoftmaxCrossEntropy::apply(x, w, bias.defined() ? bias : targets, targets, bias.defined(), reduction,
                                                        ignored, error));
@@ -268,8 +269,9 @@ PyObject* softmax_cross_entropy_gradients(PyObject*, PyObject* const* args, Py_s
     PyErr_SetString(PyExc_TypeError, "softmax_cross_entropy_gradients(x, weights, bias, targets, ignored, error, one, dw, db)");
     return nullptr;
   }
-  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &bias = THPVariable_Unpack(args[2]);
-  const Tensor targets = THPVariable_Unpack(args[3]).contiguous();
+  const Tensor x = tensor_or_none(args[0]);
+  const Tensor &w = THPVariable_Unpack(args[1]), &bias = THPVariable_Unpack(args[2]);
+  const Tensor targets = tensor_or_none(args[3]).contiguous();
   const int64_t ignored = PyLong_AsLongLong(args[4]), error = PyLong_AsLongLong(args[5]);
   if (PyErr_Occurred()) return nullptr;
   const Tensor &unit = THPVariable_Unpack(args[6]), &dw = THPVariable_Unpack(args[7]), &db = THPVariable_Unpack(args[8]);

@@ -96,7 +96,7 @@ class Fp4Rows:
         padded = torch.zeros((m * 128, k * 16), dtype=torch.uint8, device=codes.device)
         padded[:rows, :blocks].copy_(block_scale.view(torch.uint8))
         laid = padded.view(m, 4, 32, k, 4, 4).permute(0, 3, 4, 2, 1, 5).contiguous()
-        self._hold(codes, int(pitch), laid.view(-1), scale.contiguous(), cols)
+        self._hold(codes, int(pitch), laid.view(-1), scale.resolve_neg().contiguous(), cols)
 
     def _hold(self, codes, pitch, blocks, scale, cols):
         self.codes, self.pitch, self.blocks, self.scale, self.cols = codes, pitch, blocks, scale, cols
@@ -131,7 +131,8 @@ class Fp4Rows:
 
 
 def _readable(x):
-    """A float matrix with strides that the quantisation reads: columns one behind the other, or copied to be so."""
+    """A float matrix as the quantisation reads it: columns one behind the other and no negated view, or copied to be so."""
+    x = x.resolve_neg()
     if x.shape[1] > 1 and x.stride(1) != 1:
         return x.contiguous()
     return x
@@ -220,7 +221,7 @@ def fp4_product(x, weights: Fp4Rows, *, bias=None, out_dtype=None, out=None):
         if bias.dtype != torch.float32 or bias.shape != (N,):
             raise ValueError(f"bias must be float32 of shape ({N},), got {bias.dtype} of {tuple(bias.shape)}")
         _no_grad("bias", bias)
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else (torch.float32 if quantized else x.dtype)
     out_code = dtype_code(out_dtype)
@@ -233,6 +234,8 @@ def fp4_product(x, weights: Fp4Rows, *, bias=None, out_dtype=None, out=None):
         if out.dtype != out_dtype or out.shape != (*lead, N):
             raise ValueError(f"out must be {out_dtype} of shape {(*lead, N)}, got {out.dtype} of {tuple(out.shape)}")
         refuse_written_grad("out", out)
+        if out.is_neg():
+            raise ValueError("out is a negated view, which the kernel cannot write")
         flat = out.view(-1, N) if N else out  # raises if the rows cannot be one matrix
         if flat.numel() and ((N > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < N)):
             raise ValueError("out needs dense rows that do not overlap")
