@@ -41,3 +41,24 @@ def test_fields_are_those_of_the_last_quantize(tt):
     assert torch.equal(fields, tt.fp4_product(x, r.served, bias=bias))
     r.quantize()
     assert torch.equal(r.fields(x), tt.fp4_product(x, tt.quantize_fp4(r.weights), bias=r.bias))
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16, torch.float64])
+def test_another_default_dtype(tt, kind):
+    """The masters are float32 and the same numbers, whatever type new tensors have by default."""
+    x, y = data(64, 48, 30, 3)
+    want = tt.CategoricalReadout(48, 30, dropout=0.2, seed=8)
+    loss = want.step(x, y)
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(kind)
+    try:
+        r = tt.CategoricalReadout(48, 30, dropout=0.2, seed=8)
+        assert torch.equal(r.step(x, y), loss)
+        r.quantize()
+        fields = r.fields(x)
+    finally:
+        torch.set_default_dtype(was)
+    assert r.weights.dtype == r.bias.dtype == r.gradient[0].dtype == torch.float32
+    assert torch.equal(r.weights, want.weights)
+    want.quantize()
+    assert torch.equal(fields, want.fields(x))

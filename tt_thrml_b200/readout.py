@@ -57,7 +57,7 @@ class CategoricalReadout:
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         g = torch.Generator().manual_seed(int(seed) & 0x7FFFFFFF)
         shape = (int(n_categories), int(n_units))
-        self.weights = (torch.randn(shape, generator=g) * shape[1] ** -0.5).to(dev)
+        self.weights = (torch.randn(shape, generator=g, dtype=torch.float32) * shape[1] ** -0.5).to(dev)
         self.bias = torch.zeros(shape[0], dtype=torch.float32, device=dev)
         self.dropout, self.seed, self.ignore_index = float(dropout), int(seed) & (2**64 - 1), int(ignore_index)
         self.optimizer = AdamW((self.weights, self.bias), lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
