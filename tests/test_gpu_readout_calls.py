@@ -62,3 +62,13 @@ def test_another_default_dtype(tt, kind):
     assert torch.equal(r.weights, want.weights)
     want.quantize()
     assert torch.equal(fields, want.fields(x))
+
+
+def test_values_of_4_bit_rows_have_no_gradient(tt):
+    """As products with such rows do, their values refuse a scale that requires one instead of dropping it."""
+    q = tt.quantize_fp4(torch.ones(4, 32, device="cuda"))
+    given = tt.Fp4Rows(q.codes, q.block_scale, q.scale.clone().requires_grad_(True), cols=32)
+    with pytest.raises(RuntimeError, match="scale requires a gradient"):
+        given.dequantize()
+    with torch.no_grad():
+        assert torch.equal(given.dequantize(), q.dequantize())

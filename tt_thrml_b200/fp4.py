@@ -121,7 +121,8 @@ class Fp4Rows:
         return laid[:rows, : -(-cols // BLOCK)].contiguous().view(torch.float8_e4m3fn)
 
     def dequantize(self):
-        """The float32 matrix that the codes and scales stand for."""
+        """The float32 matrix that the codes and scales stand for.  It has no derivative: a scale that requires one is refused."""
+        refuse_grad("the scale", self.scale, "the values of 4-bit rows")
         with on_device(self.device):
             made = nat.bound_hostcall().fp4_values(self.codes, self.pitch, self.blocks, self.scale, self.cols,
                                                    raw_stream(self.index))
