@@ -767,7 +767,7 @@ int64_t tthrml_xent_forward_workspace(int64_t rows, int64_t categories, int64_t 
 /*
  * dx [rows][dx_ld], dw [categories][dw_ld] (grad_dtype: float32, bfloat16 or
  * float16) and db [categories], each NULL or written, of
- * sum_t weight[t] loss[t].  weight: grad[0] * (inv_count ? *inv_count : 1), or,
+ * sum_t weight[t] loss[t], the same whichever others are asked for.  weight: grad[0] * (inv_count ? *inv_count : 1), or,
  * grad_per_row, grad[t].  workspace: tthrml_xent_backward_workspace(...) bytes,
  * 32-byte aligned.
  */
@@ -797,7 +797,8 @@ int64_t tthrml_fp4_scale_bytes(int64_t rows, int64_t cols);
 /*
  * scale = max|x_r| / 2688, block = e4m3(max|x_b| / (6 scale)), code =
  * e2m1(x / (block scale)), in float32 (fl(2688 / max|x_r|) first).  Rows below
- * 2^-100 get scale 0, rows that are not finite scale NaN.  Strides in elements.
+ * 2^-100 get scale 0, rows that are not finite scale NaN.  Strides in elements.  Zeros are
+ * written behind the columns, up to the next multiple of 128 bytes or `pitch`, whichever is less.
  */
 int tthrml_fp4_quantize(const void* x_dev, int32_t dtype, int64_t rows, int64_t cols,
                         int64_t row_stride, int64_t col_stride, void* codes_dev, int64_t pitch,
@@ -808,7 +809,11 @@ int tthrml_fp4_values(const void* codes_dev, int64_t pitch, const void* blocks_d
                       const float* scale_dev, int64_t rows, int64_t cols, float* out_dev,
                       void* stream);
 
-/* out[m][n] = (sum_k x[m][k] w[n][k]) * (x_scale[m] * w_scale[n]) + bias[n], sums in float32. */
+/*
+ * out[m][n] = (sum_k x[m][k] w[n][k]) * (x_scale[m] * w_scale[n]) + bias[n], sums in float32.
+ * Where cols is odd, the half byte behind the last column is multiplied too: it has to be 0 in one
+ * of the operands (tthrml_fp4_quantize writes zeros there).
+ */
 int tthrml_fp4_product(const void* x_codes_dev, int64_t x_pitch, const void* x_blocks_dev,
                        const float* x_scale_dev, const void* w_codes_dev, int64_t w_pitch,
                        const void* w_blocks_dev, const float* w_scale_dev, int64_t rows,
@@ -827,8 +832,9 @@ int tthrml_fp4_product_few(const void* x_dev, int32_t x_dtype, int64_t x_ld, con
                            void* stream);
 
 /*
- * Rows of floats through 4-bit weights: tthrml_fp4_product_few where it takes them (columns dense), else tthrml_fp4_quantize
- * into the workspace, then tthrml_fp4_product.  workspace: 16-byte aligned device memory of
+ * Rows of floats through 4-bit weights: tthrml_fp4_product_few where it takes them, else tthrml_fp4_quantize into the
+ * workspace, then tthrml_fp4_product.  Sizes that tthrml_fp4_few_rows allows need dense columns (col_stride 1; others are
+ * refused: lay them out, or quantise them and call tthrml_fp4_product).  workspace: 16-byte aligned device memory of
  * tthrml_fp4_linear_workspace(rows, cols, units) bytes (0: none is needed), free again once the work on `stream` is done.
  */
 int tthrml_fp4_linear(const void* x_dev, int32_t x_dtype, int64_t rows, int64_t cols, int64_t row_stride,

@@ -5,11 +5,11 @@
 //
 // The forward pass is one product whose epilogue folds each tile of logits into a running maximum and sum per row (a row
 // per thread; log2 domain), so only a pair of floats per row and unit of work leaves the SM; k_xent_loss joins them.  The
-// backward pass takes the categories in pieces of at most kPieceBytes of g: the logits of a piece are computed again and
+// backward pass takes the categories in pieces of kPieceBytes of g, of 256 categories at least: the logits of a piece are computed again and
 // turned into g (16 bits), which two further products reduce to this piece's rows of dw and to sums of dx in float32.
 //
 // One kernel serves the four products: persistent clusters of two CTAs walk 256 x BN tiles (tcgen05 cta_group::2, two
-// TMEM accumulators, five to eight stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
+// TMEM accumulators, four to eight stages of 64 columns of K), operands K-major or MN-major as they lie in memory, so nothing is
 // transposed.  Warps 2 on run the epilogue of a tile beside the main loop of the next one: eight, or sixteen where the logits are
 // short sums or db is summed up beside.  Logits of up to 128 rows are tiles of one CTA each: a pair's MMA would take as long for
 // half the weights, which are what bounds them (64 rows, 4096 x 32768 weights: 58 us in pairs).  Warp 0 loads (TMA), warp 1 of the
@@ -17,12 +17,13 @@
 //
 // g is rounded to the operands' 16 bits (up to kFewRows rows or kFewCategories categories: held in two such pieces, their sum
 // good to 2^-16; the second piece is more rows or columns of the same tiles): by at most 2^-8 (bfloat16) or 2^-11 (float16) of
-// each element, as dx and dw themselves are.  float16 holds g times 2^14, so that probabilities down to 2^-28 stay normal numbers.  Maxima,
-// sums, z, losses and the sums of db are float32; dx and dw accumulate in float32.
+// each element, as dx and dw themselves are.  float16 holds g times 2^14 over the largest weight of a row, so that what is at least 2^-28 of
+// that weight stays a normal number and rows of far smaller weights lose bits.  Maxima and sums are float32, as dx and dw accumulate; losses and
+// the sums of db are joined in 64 bits and leave as float32.
 //
-// What bounds it: the tensor pipe (97 % active in each of the four products; 4096 rows, 4096 columns, 16384 categories: logits
-// 332 us, g 340, dx 379, dw 339, 1.45 to 1.65 PFLOP/s at the clocks of a short run) and, over longer runs, the power cap
-// (8192 x 4096 x 32768, the whole step: 6.1 to 6.7 ms, 1.31 to 1.43 PFLOP/s); the weights' bytes for few rows.
+// What bounds it: the tensor pipe (97 % active, in g 87 %; 4096 rows, 4096 columns, 16384 categories: logits 332 us, g 373 (its epilogue is
+// longer than the two accumulations that run ahead of it), dx 383, dw 344, 1.43 to 1.65 PFLOP/s at the clocks of a short run) and, over
+// longer runs, the power cap (8192 x 4096 x 32768, the whole step: 6.7 to 7.0 ms, 1.25 to 1.32 PFLOP/s); the weights' bytes for few rows.
 #include "int8_common.cuh"
 #include "tc_common.cuh"
 
@@ -30,18 +31,22 @@ namespace tthrml {
 namespace {
 
 constexpr float kLog2E = 1.44269504088896340736f;
-constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time
+constexpr int64_t kPieceBytes = 256ll << 20;  // of g at a time, or 256 categories (128 columns of two pieces) where those are more
 // The products take g in 16 bits.  Where few of its values meet in a sum, their roundings' errors do not average out, and g is held
 // in two pieces, the rounding's remainder the second: below the first rows, or beside the first columns.  (64 columns are one block of
 // the sum for dx, 128 half a tile's rows for dw: the products take as long.)
 constexpr int64_t kFewRows = 128, kFewCategories = 64;
 // 64-wide blocks of K that a logit's sum stays in tensor memory for.  The tensor core cuts its sums off instead of rounding them;
-// float32 registers add them up every few blocks, in both passes the same, so that probabilities and normalisers agree.  Errors of
+// float32 registers add them up every few blocks, in both passes the same, so that probabilities and normalisers agree (a backward pass of
+// one accumulation, which is quicker by 33 us of the 373 above, makes the difference of a row of probability 1 - 1e-4 wrong by a
+// multiple of itself).  Errors of
 // losses and db over 150 random sizes of 8 to 8192 columns, relative: four below 3e-7, eight below 5e-7, 32 some of 3e-6 (eight after
 // four 1e-6).  Two, four and eight take 1.67, 1.53 and 1.36 ms for the losses of 8192 x 4096 x 32768, four and eight 62 and 59 us for
 // those of 64 rows; fewer are taken where few rows meet few categories: nothing averages the errors out, and the time is not the
 // tiles' (db of 13 x 409 x 2: 1.1e-7, 1.4e-7 and 1.8e-7 in the middle of 200 inputs with one, two and four, and 1.0e-7 in plain
-// float32; a step of 100 x 8192 x 10 in 149, 118 and 103 us).
+// float32; a step of 100 x 8192 x 10 in 149, 118 and 103 us).  More categories average them out: 64 x 4096, losses of 128, 4096 and 32768
+// categories off by up to 1.1e-7, 8e-8 and 7e-8 with four, 2.0e-7, 1.4e-7 and 1.2e-7 with eight, in 26.3, 27.1 and 56.5 us with four,
+// 24.5, 25.2 and 56.8 with eight; 16384 categories in 47.0 and 43.3.
 constexpr int chunk_of(int64_t rows, int64_t categories) {
   return rows > 128 || categories > 4096 ? 8 : (categories > 64 ? 4 : 2);
 }

@@ -3,8 +3,9 @@
     l[t, v] = sum_k x[t, k] w[v, k] + bias[v],   loss[t] = log sum_v exp l[t, v] - l[t, y[t]]
 
 The logits are never held as a whole: the forward pass keeps a running maximum
-and sum per row, the backward pass takes the categories in pieces (at most
-256 MiB of 16-bit differences exp(l - z) - [v = y] at a time).  x is a dense
+and sum per row, the backward pass takes the categories in pieces: 256 MiB of
+16-bit differences exp(l - z) - [v = y] at a time, or 512 bytes a row where that is
+more.  x is a dense
 block's units over the chains (or any features), w one row per category.
 
 The kernels launch on the current stream of x's device; nothing synchronises.
@@ -71,7 +72,8 @@ def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", i
 
     x: bfloat16 or float16 [..., K]; weights: the same type [V, K], any strides
     (rows that are not 16-byte aligned are laid out again in each call); targets:
-    int64 or int32 [...]; bias: float32 [V], -inf for categories that cannot occur.
+    int64 or int32 [...]; bias: float32 [V], -inf for categories that cannot occur, whose
+    weights must be finite all the same (logits below -2^127 may count as -inf).
     reduction "mean" (over the rows that count), "sum" (float32 scalars) or "none"
     (float32 [...]).  Rows whose target is `ignore_index` do not count: loss 0, no
     gradient (their values must be finite, as 0 times them is added to the weights'
@@ -79,7 +81,9 @@ def softmax_cross_entropy(x, weights, targets, *, bias=None, reduction="mean", i
     row in which no category can occur has loss inf and no gradient.
 
     Sums and normalisers are float32; the gradients are products of 16-bit
-    differences, accumulated in float32.  The result is the same every time.
+    differences, accumulated in float32 (in float16 the differences are held relative
+    to the largest weight of a row under 'none': below 2^-28 of it they lose bits).
+    The result is the same every time, whichever gradients are asked for.
     Gradients of gradients and forward-mode derivatives are not available.
     """
     torch = _torch()
